@@ -71,6 +71,17 @@ pub const TRS_UN_DIV_SCALAR: i32 = 17;
 pub const TRS_UN_POW_SCALAR: i32 = 18;
 pub const TRS_UN_RPOW_SCALAR: i32 = 19;
 
+// trs_rotary_layout
+pub const TRS_ROTARY_HALF: i32 = 0;
+pub const TRS_ROTARY_INTERLEAVED: i32 = 1;
+
+// trs_rotary_scaling
+pub const TRS_SCALING_NONE: i32 = 0;
+pub const TRS_SCALING_LINEAR: i32 = 1;
+pub const TRS_SCALING_BASE: i32 = 2;
+pub const TRS_SCALING_BANDS: i32 = 3;
+pub const TRS_SCALING_RAMP: i32 = 4;
+
 /// A strided view of a device buffer: the reference's `Tensor` metadata
 /// (linalg/tensor/base.rs:159-164) plus the length of its storage.
 #[repr(C)]
@@ -147,6 +158,11 @@ extern "C" {
     pub fn trs_matmul_tf32x3(a: *const trs_view, b: *const trs_view, out_: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_unfold_2d(x: *const trs_view, kh: i64, kw: i64, sh: i64, sw: i64, ph: i64, pw: i64, out_: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_fold_2d(cols: *const trs_view, kh: i64, kw: i64, sh: i64, sw: i64, ph: i64, pw: i64, out_: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_rotary_frequencies(base: f64, scaling: i32, factor: f64, low_turns: f64, high_turns: f64, trained_context: f64, freqs: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_rotary(q: *const trs_view, k: *const trs_view, positions: *const trs_view, freqs: *const trs_view, layout: i32, magnitude: f64, q_out: *mut trs_view, k_out: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_rotary_backward(grad_q_out: *const trs_view, grad_k_out: *const trs_view, positions: *const trs_view, freqs: *const trs_view, layout: i32, magnitude: f64, grad_q: *mut trs_view, grad_k: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_head_norm_rotary(q: *const trs_view, k: *const trs_view, q_gamma: *const trs_view, k_gamma: *const trs_view, eps: f64, positions: *const trs_view, freqs: *const trs_view, layout: i32, magnitude: f64, q_out: *mut trs_view, k_out: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_head_norm_rotary_backward(grad_q_out: *const trs_view, grad_k_out: *const trs_view, q: *const trs_view, k: *const trs_view, q_gamma: *const trs_view, k_gamma: *const trs_view, eps: f64, positions: *const trs_view, freqs: *const trs_view, layout: i32, magnitude: f64, grad_q: *mut trs_view, grad_k: *mut trs_view, grad_q_gamma: *mut trs_view, grad_k_gamma: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_fill_uniform(out_: *mut trs_view, seed: u64, first: u64, lo: f64, hi: f64, stream: trs_stream) -> trs_status;
     pub fn trs_fill_normal(out_: *mut trs_view, seed: u64, first: u64, stream: trs_stream) -> trs_status;
     pub fn trs_set_device(device: i32) -> trs_status;

@@ -141,6 +141,22 @@ typedef struct trs_ew_program {
   trs_scalar p1;      /* epilogue parameter 1 */
 } trs_ew_program;
 
+/* How rotary positions pair the elements of a head. */
+typedef enum trs_rotary_layout {
+  TRS_ROTARY_HALF = 0,        /* (i, i + rotary / 2) */
+  TRS_ROTARY_INTERLEAVED = 1  /* (2i, 2i + 1)        */
+} trs_rotary_layout;
+
+/* How rotary frequencies are scaled for contexts longer than the trained one
+ * (trs_rotary_frequencies). */
+typedef enum trs_rotary_scaling {
+  TRS_SCALING_NONE = 0,
+  TRS_SCALING_LINEAR = 1,  /* every frequency divided by the factor          */
+  TRS_SCALING_BASE = 2,    /* the base grown by factor^(r / (r - 2))         */
+  TRS_SCALING_BANDS = 3,   /* by turns: kept, mixed, divided                 */
+  TRS_SCALING_RAMP = 4     /* as bands, mixed along the pair's index         */
+} trs_rotary_scaling;
+
 /* ------------------------------------------------------------------ */
 /* Library                                                             */
 /* ------------------------------------------------------------------ */
@@ -452,6 +468,78 @@ trs_status trs_unfold_2d(const trs_view* x, int64_t kh, int64_t kw, int64_t sh,
 trs_status trs_fold_2d(const trs_view* cols, int64_t kh, int64_t kw, int64_t sh,
                        int64_t sw, int64_t ph, int64_t pw, trs_view* out,
                        trs_stream stream);
+
+/* ------------------------------------------------------------------ */
+/* The attention layer between its projections (nn/attention.rs:220-230 */
+/* composes it from matmul and SoftMax): rotary positions, the per-head */
+/* norm, and the fused attention.  Tensors are views of the shape       */
+/* [batch, tokens, heads, head size] with any strides (q, k and v may   */
+/* be slices of one projection's output).  The reference has no         */
+/* counterpart of the rotation and of the norm.                         */
+/* ------------------------------------------------------------------ */
+
+/* The rotation's frequencies f_i = base^(-2i / r), i < r / 2 (r the rotated
+ * elements of a head), into freqs, an f64 view of r / 2 elements that a program
+ * computes once and keeps.  scaling (trs_rotary_scaling) stretches them by
+ * `factor` for contexts longer than trained_context tokens: LINEAR divides
+ * all; BASE raises the base so that the slowest pair is divided by factor and
+ * the fastest kept; BANDS and RAMP keep a pair that makes at least high_turns
+ * turns over the trained context, divide one that makes at most low_turns, and
+ * mix the two linearly in between, BANDS by the pair's turns, RAMP by its
+ * index between the (rounded) indices of the two bounds (the interpolation
+ * "by parts" of YaRN, whose program also passes magnitude =
+ * 0.1 ln(factor) + 1 to the calls below).  low_turns, high_turns and
+ * trained_context are read by BANDS and RAMP alone, factor by all but NONE.
+ * TRS_ERR_ARG: base not above 1, factor not above 0, bounds not
+ * 0 < low < high.  At most 256 frequencies. */
+trs_status trs_rotary_frequencies(double base, int32_t scaling, double factor,
+                                  double low_turns, double high_turns,
+                                  double trained_context, trs_view* freqs,
+                                  trs_stream stream);
+
+/* Rotary positions: pair i of the first 2 * numel(freqs) elements of every
+ * head, (a, b), becomes magnitude * (a cos t - b sin t, b cos t + a sin t)
+ * with t = position * freqs[i]; the other elements are copied.  q is [B, T,
+ * Hq, D], k [B, T, Hk, D] or NULL (with k_out), f32 or f64; positions i32 or
+ * i64, [T], [1, T] or [B, T], any values; layout a trs_rotary_layout.  The
+ * angle is taken in f64.  An output may be its own input (the identical
+ * view), no other overlap (TRS_ERR_ALIAS).  D at most 512 (TRS_ERR_SHAPE). */
+trs_status trs_rotary(const trs_view* q, const trs_view* k,
+                      const trs_view* positions, const trs_view* freqs,
+                      int32_t layout, double magnitude, trs_view* q_out,
+                      trs_view* k_out, trs_stream stream);
+
+/* The gradient of trs_rotary: the rotation by the opposite angles, with the
+ * same magnitude. */
+trs_status trs_rotary_backward(const trs_view* grad_q_out,
+                               const trs_view* grad_k_out,
+                               const trs_view* positions, const trs_view* freqs,
+                               int32_t layout, double magnitude,
+                               trs_view* grad_q, trs_view* grad_k,
+                               trs_stream stream);
+
+/* The norm of every query's and key's head and its rotation in one pass:
+ * n = x / sqrt(sum(x^2) / D + eps), y = rotary(n * gamma).  q_gamma and
+ * k_gamma hold D elements of the tensors' type, or are NULL for ones; the rest
+ * as trs_rotary. */
+trs_status trs_head_norm_rotary(const trs_view* q, const trs_view* k,
+                                const trs_view* q_gamma, const trs_view* k_gamma,
+                                double eps, const trs_view* positions,
+                                const trs_view* freqs, int32_t layout,
+                                double magnitude, trs_view* q_out,
+                                trs_view* k_out, trs_stream stream);
+
+/* The gradients of trs_head_norm_rotary: q and k are its inputs, grad_q and
+ * grad_k the gradients of these, grad_q_gamma and grad_k_gamma (D elements
+ * each, or NULL) those of the gammas, summed over batch, tokens and heads in
+ * f64 in a fixed order and rounded once.  grad_q may be grad_q_out or q
+ * through the identical view, likewise grad_k. */
+trs_status trs_head_norm_rotary_backward(
+    const trs_view* grad_q_out, const trs_view* grad_k_out, const trs_view* q,
+    const trs_view* k, const trs_view* q_gamma, const trs_view* k_gamma,
+    double eps, const trs_view* positions, const trs_view* freqs,
+    int32_t layout, double magnitude, trs_view* grad_q, trs_view* grad_k,
+    trs_view* grad_q_gamma, trs_view* grad_k_gamma, trs_stream stream);
 
 /* ------------------------------------------------------------------ */
 /* Seeded synthetic inputs                                              */

@@ -34,6 +34,12 @@ UNOPS = {
     "pow_scalar": 18, "rpow_scalar": 19,
 }
 
+# trs_rotary_layout
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+
+# trs_rotary_scaling
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
+
 
 class View(ctypes.Structure):
     """trs_view: a strided view of a device buffer (element units)."""
@@ -112,6 +118,12 @@ _SIGNATURES = {
     "trs_matmul_tf32x3": (c_int32, [_V, _V, _V, c_void_p]),
     "trs_unfold_2d": (c_int32, [_V, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _V, c_void_p]),
     "trs_fold_2d": (c_int32, [_V, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _V, c_void_p]),
+    "trs_rotary_frequencies": (c_int32, [c_double, c_int32, c_double, c_double, c_double, c_double, _V, c_void_p]),
+    "trs_rotary": (c_int32, [_V, _V, _V, _V, c_int32, c_double, _V, _V, c_void_p]),
+    "trs_rotary_backward": (c_int32, [_V, _V, _V, _V, c_int32, c_double, _V, _V, c_void_p]),
+    "trs_head_norm_rotary": (c_int32, [_V, _V, _V, _V, c_double, _V, _V, c_int32, c_double, _V, _V, c_void_p]),
+    "trs_head_norm_rotary_backward": (c_int32, [_V, _V, _V, _V, _V, _V, c_double, _V, _V, c_int32, c_double, _V, _V,
+                                                _V, _V, c_void_p]),
     "trs_fill_uniform": (c_int32, [_V, c_uint64, c_uint64, c_double, c_double, c_void_p]),
     "trs_fill_normal": (c_int32, [_V, c_uint64, c_uint64, c_void_p]),
     "trs_set_device": (c_int32, [c_int32]),

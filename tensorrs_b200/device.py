@@ -235,6 +235,57 @@ def fold_2d(cols: abi.View, kernel, stride, padding, out: torch.Tensor) -> torch
     return out
 
 
+def _ref(v: abi.View | None):
+    return ctypes.byref(v) if v is not None else None
+
+
+def _out(t: torch.Tensor | None):
+    return ctypes.byref(view_of(t)) if t is not None else None
+
+
+def rotary_frequencies(out: torch.Tensor, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       low_turns: float = 1.0, high_turns: float = 32.0, trained_context: float = 0.0) -> torch.Tensor:
+    """The frequencies of rotary positions into out (f64, one per rotated pair);
+    scaling as trs_rotary_scaling: none, linear, base, bands or ramp."""
+    _call("trs_rotary_frequencies", float(base), abi.ROTARY_SCALINGS[scaling], float(factor), float(low_turns),
+          float(high_turns), float(trained_context), _out(out), stream_handle())
+    return out
+
+
+def rotary(q: abi.View, k: abi.View | None, positions: abi.View, freqs: abi.View, q_out: torch.Tensor,
+           k_out: torch.Tensor | None, layout: str = "half", magnitude: float = 1.0) -> None:
+    """Rotary positions of q [B, T, Hq, D] and k [B, T, Hk, D]."""
+    _call("trs_rotary", _ref(q), _ref(k), _ref(positions), _ref(freqs), abi.ROTARY_LAYOUTS[layout], float(magnitude),
+          _out(q_out), _out(k_out), stream_handle())
+
+
+def rotary_backward(grad_q_out: abi.View, grad_k_out: abi.View | None, positions: abi.View, freqs: abi.View,
+                    grad_q: torch.Tensor, grad_k: torch.Tensor | None, layout: str = "half",
+                    magnitude: float = 1.0) -> None:
+    """The gradient that rotary passes back to q and k."""
+    _call("trs_rotary_backward", _ref(grad_q_out), _ref(grad_k_out), _ref(positions), _ref(freqs),
+          abi.ROTARY_LAYOUTS[layout], float(magnitude), _out(grad_q), _out(grad_k), stream_handle())
+
+
+def head_norm_rotary(q: abi.View, k: abi.View | None, q_gamma: abi.View | None, k_gamma: abi.View | None, eps: float,
+                     positions: abi.View, freqs: abi.View, q_out: torch.Tensor, k_out: torch.Tensor | None,
+                     layout: str = "half", magnitude: float = 1.0) -> None:
+    """The norm of every head of q and k and its rotation, in one pass."""
+    _call("trs_head_norm_rotary", _ref(q), _ref(k), _ref(q_gamma), _ref(k_gamma), float(eps), _ref(positions),
+          _ref(freqs), abi.ROTARY_LAYOUTS[layout], float(magnitude), _out(q_out), _out(k_out), stream_handle())
+
+
+def head_norm_rotary_backward(grad_q_out: abi.View, grad_k_out: abi.View | None, q: abi.View, k: abi.View | None,
+                              q_gamma: abi.View | None, k_gamma: abi.View | None, eps: float, positions: abi.View,
+                              freqs: abi.View, grad_q: torch.Tensor, grad_k: torch.Tensor | None,
+                              grad_q_gamma: torch.Tensor | None, grad_k_gamma: torch.Tensor | None,
+                              layout: str = "half", magnitude: float = 1.0) -> None:
+    """The gradients of head_norm_rotary for q, k and the gammas."""
+    _call("trs_head_norm_rotary_backward", _ref(grad_q_out), _ref(grad_k_out), _ref(q), _ref(k), _ref(q_gamma),
+          _ref(k_gamma), float(eps), _ref(positions), _ref(freqs), abi.ROTARY_LAYOUTS[layout], float(magnitude),
+          _out(grad_q), _out(grad_k), _out(grad_q_gamma), _out(grad_k_gamma), stream_handle())
+
+
 def fill_uniform(out: torch.Tensor, seed: int, lo: float = -1.0, hi: float = 1.0, first: int = 0) -> torch.Tensor:
     _call("trs_fill_uniform", ctypes.byref(view_of(out)), seed, first, lo, hi, stream_handle())
     return out
