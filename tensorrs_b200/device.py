@@ -24,19 +24,16 @@ def stream_handle() -> int:
 
 def view_of(t: torch.Tensor, shape=None, strides=None, offset=None) -> abi.View:
     """A trs_view into t's storage.  Without overrides it describes t itself."""
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError("view_of needs a CUDA tensor")
     st = t.untyped_storage()
-    es = t.element_size()
-    base = st.data_ptr()
-    storage_len = st.nbytes() // es
-    if shape is None:
-        shape = list(t.shape)
-    if strides is None:
-        strides = list(t.stride()) if shape is not None and list(shape) == list(t.shape) else None
+    if shape is None or list(shape) == list(t.shape):
+        shape = t.shape
+        if strides is None:
+            strides = t.stride()
     if offset is None:
         offset = t.storage_offset()
-    return abi.make_view(base, TORCH_TO_TRS[t.dtype], shape, strides, offset, storage_len)
+    return abi.make_view(st.data_ptr(), TORCH_TO_TRS[t.dtype], shape, strides, offset, st.nbytes() // t.element_size())
 
 
 def _call(name: str, *args) -> int:
