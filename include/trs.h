@@ -541,6 +541,43 @@ trs_status trs_head_norm_rotary_backward(
     int32_t layout, double magnitude, trs_view* grad_q, trs_view* grad_k,
     trs_view* grad_q_gamma, trs_view* grad_k_gamma, trs_stream stream);
 
+/* Attention of queries to the keys and values of another length (an encoder's
+ * states): per head, S = scale q k^T, out = softmax(S) v, lse = ln sum exp S.
+ * q and out are [B, Tq, Hq, D], k and v [B, Tk, Hk, D] with Hq a multiple of
+ * Hk (query head h reads key head h / (Hq / Hk)), f32, D at most 256; any of
+ * Tq, Tk may be 1, or 0.  key_lengths (i32 or i64, [B], or NULL for Tk) says
+ * how many keys of each batch there are (values are clamped to [0, Tk]); what
+ * lies behind them is not read.  A query without keys gives 0 and an lse of
+ * -inf.  lse is [B, Hq, Tq] or NULL; the backward needs it.  The scale is
+ * finite, of either sign.
+ *
+ * Up to D = 128 more than 16 query rows per key head run on the tensor cores
+ * (tcgen05): every operand as two fp16 parts under a power of two per tile of
+ * 8192 elements, three products each, accumulated in f32, results within a few
+ * f32 roundings of the sums' terms (elements below 2^-17 of their tile's
+ * largest are off by 2^-40 of that).  Fewer rows, and larger heads, run on the
+ * CUDA cores in f32, as does a whole call whose inputs hold an infinity or a
+ * NaN (found on the device; these propagate as in the formulas).  Workspaces
+ * come from the stream-ordered pool.  Outputs may overlap nothing
+ * (TRS_ERR_ALIAS); repeated calls give the same bits. */
+trs_status trs_cross_attention(const trs_view* q, const trs_view* k,
+                               const trs_view* v, const trs_view* key_lengths,
+                               double scale, trs_view* out, trs_view* lse,
+                               trs_stream stream);
+
+/* The gradients of trs_cross_attention from grad_out, its inputs, its out and
+ * its lse: with P = exp(S - lse), delta = sum_d grad_out out and dS = P
+ * (grad_out v^T - delta), grad_q = scale dS k, grad_k = scale dS^T q and
+ * grad_v = P^T grad_out, the last two summed over the query heads of a key
+ * head.  Rows of grad_k and grad_v at and behind a key length are set to 0.
+ * Up to D = 128 on the tensor cores as above; no atomics, so repeated calls
+ * give the same bits. */
+trs_status trs_cross_attention_backward(
+    const trs_view* grad_out, const trs_view* q, const trs_view* k,
+    const trs_view* v, const trs_view* key_lengths, const trs_view* out,
+    const trs_view* lse, double scale, trs_view* grad_q, trs_view* grad_k,
+    trs_view* grad_v, trs_stream stream);
+
 /* ------------------------------------------------------------------ */
 /* Seeded synthetic inputs                                              */
 /* ------------------------------------------------------------------ */

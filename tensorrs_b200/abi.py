@@ -129,6 +129,8 @@ _SIGNATURES = {
     "trs_head_norm_rotary": (c_int32, [_V, _V, _V, _V, c_double, _V, _V, c_int32, c_double, _V, _V, c_void_p]),
     "trs_head_norm_rotary_backward": (c_int32, [_V, _V, _V, _V, _V, _V, c_double, _V, _V, c_int32, c_double, _V, _V,
                                                 _V, _V, c_void_p]),
+    "trs_cross_attention": (c_int32, [_V, _V, _V, _V, c_double, _V, _V, c_void_p]),
+    "trs_cross_attention_backward": (c_int32, [_V, _V, _V, _V, _V, _V, _V, c_double, _V, _V, _V, c_void_p]),
     "trs_fill_uniform": (c_int32, [_V, c_uint64, c_uint64, c_double, c_double, c_void_p]),
     "trs_fill_normal": (c_int32, [_V, c_uint64, c_uint64, c_void_p]),
     "trs_set_device": (c_int32, [c_int32]),

@@ -1,0 +1,591 @@
+// cross_attention.cu -- trs_cross_attention and its gradient: the checks, the
+// choice of kernel, and the kernels that run on the CUDA cores.
+//
+//   S = scale q k^T,  P = exp(S - lse),  lse = ln sum exp S,  out = P v
+//   backward: delta = sum_d dout out,  dP = dout v^T,  dS = P (dP - delta),
+//             dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout
+//
+// with keys at and beyond key_lengths[b] absent (never read); a query without
+// keys gives 0, lse = -inf and no gradient.
+//
+// cross_rows_kernel serves few query rows per key head (single tokens), where
+// reading k and v once is all there is to do, and, looping over blocks of
+// rows, head sizes above 128 and inputs that hold infinities or NaNs.  A CTA
+// owns (problem, block of NR rows, part of the keys): groups of L lanes own
+// one key at a time, each lane 4 (8) elements of the head; 4 keys are in
+// flight per group, the dot products fold over the group with shuffles, and
+// the running maximum, sum and output stay in registers until the CTA's groups
+// are joined in shared memory.  Parts of the keys are joined by
+// cross_join_kernel in a fixed order.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "../../include/trs.h"
+#include "cross.h"
+
+namespace trs {
+namespace {
+
+constexpr int kRowsThreads = 256;
+constexpr int kRowsMaxHead = 256;
+
+struct RowsDev {
+  CrossDev c;
+  int blocks;        // blocks of NR rows per problem
+  int splits;        // parts of the keys
+  int items;         // problems * blocks * splits
+  float* part;       // [split][problem][M][D] and then m, l [split][problem][M], when splits > 1
+  float* part_m;
+  float* part_l;
+};
+
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float* p, int d, int D, int64_t sd) {
+  if (VEC) return d < D ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 r;
+  r.x = d < D ? p[d * sd] : 0.f;
+  r.y = d + 1 < D ? p[(d + 1) * sd] : 0.f;
+  r.z = d + 2 < D ? p[(d + 2) * sd] : 0.f;
+  r.w = d + 3 < D ? p[(d + 3) * sd] : 0.f;
+  return r;
+}
+
+__device__ __forceinline__ float dot4(const float4& a, const float4& b, float s) {
+  s = __fmaf_rn(a.x, b.x, s);
+  s = __fmaf_rn(a.y, b.y, s);
+  s = __fmaf_rn(a.z, b.z, s);
+  return __fmaf_rn(a.w, b.w, s);
+}
+
+template <int NR, int L, int NV, bool VEC>
+__global__ void __launch_bounds__(kRowsThreads) cross_rows_kernel(const RowsDev d) {
+  const CrossDev& c = d.c;
+  if (c.nonfinite && *(volatile const int*)c.nonfinite == 0) return;
+  constexpr int U = 4;                                  // keys in flight per group
+  constexpr int NG = kRowsThreads / L;                  // groups
+  constexpr int DP = L * 4 * NV;                        // padded head size
+  __shared__ float s_m[NG][NR], s_l[NG][NR];
+  extern __shared__ float s_acc[];                      // [NG][NR][DP]
+  const int gid = threadIdx.x / L, lane = threadIdx.x % L;
+  const unsigned mask = L == 32 ? 0xffffffffu : (0xffffu << (threadIdx.x & 16));
+  for (int item = blockIdx.x; item < d.items; item += gridDim.x) {
+    const int sp = item % d.splits, rb = item / d.splits % d.blocks, pr = item / d.splits / d.blocks;
+    const int b = pr / c.Hk, hk = pr % c.Hk;
+    const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
+    const int per = (n + d.splits - 1) / d.splits;
+    const int k0 = min(n, sp * per), k1 = min(n, k0 + per);
+    float4 q[NR][NV], acc[NR][NV];
+    float m[NR], l[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int row = rb * NR + r;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+      const int g = row < c.M ? (int)fdiv((uint32_t)row, c.f_Tq) : 0, t = row < c.M ? row - g * c.Tq : 0;
+      const float* qp = static_cast<const float*>(c.q.p) + b * c.q.sb + t * c.q.st + (hk * c.G + g) * c.q.sh;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        acc[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        q[r][i] = row < c.M ? load4<VEC>(qp, (lane + i * L) * 4, c.D, c.q.sd) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    const float f = c.scale * kLog2e;
+    const float* kp = static_cast<const float*>(c.k.p) + b * c.k.sb + hk * c.k.sh;
+    const float* vp = static_cast<const float*>(c.v.p) + b * c.v.sb + hk * c.v.sh;
+    for (int key = k0 + gid * U; key < k1; key += NG * U) {
+      float4 kk[U][NV], vv[U][NV];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = key + u;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const bool on = at < k1;
+          kk[u][i] = on ? load4<VEC>(kp + at * c.k.st, (lane + i * L) * 4, c.D, c.k.sd) : make_float4(0.f, 0.f, 0.f, 0.f);
+          vv[u][i] = on ? load4<VEC>(vp + at * c.v.st, (lane + i * L) * 4, c.D, c.v.sd) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          s[u] = 0.f;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) s[u] = dot4(q[r][i], kk[u][i], s[u]);
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(mask, s[u], o, L);
+        float mx = m[r];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          s[u] = key + u < k1 ? s[u] * f : -INFINITY;
+          mx = fmaxf(mx, s[u]);
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;  // all scores -inf so far: every weight stays 0
+        const float alpha = ex2(m[r] - base);
+        m[r] = mx;
+        l[r] *= alpha;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          s[u] = ex2(s[u] - base);
+          l[r] += s[u];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          float4& a = acc[r][i];
+          a.x *= alpha;
+          a.y *= alpha;
+          a.z *= alpha;
+          a.w *= alpha;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            a.x = __fmaf_rn(s[u], vv[u][i].x, a.x);
+            a.y = __fmaf_rn(s[u], vv[u][i].y, a.y);
+            a.z = __fmaf_rn(s[u], vv[u][i].z, a.z);
+            a.w = __fmaf_rn(s[u], vv[u][i].w, a.w);
+          }
+        }
+      }
+    }
+    // join the CTA's groups
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if (lane == 0) {
+        s_m[gid][r] = m[r];
+        s_l[gid][r] = l[r];
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        *reinterpret_cast<float4*>(&s_acc[(gid * NR + r) * DP + (lane + i * L) * 4]) = acc[r][i];
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < NR * DP; idx += kRowsThreads) {
+      const int r = idx / DP, dd = idx % DP, row = rb * NR + r;
+      if (row >= c.M || dd >= c.D) continue;
+      float mx = -INFINITY;
+      for (int g = 0; g < NG; ++g) mx = fmaxf(mx, s_m[g][r]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f, o = 0.f;
+      for (int g = 0; g < NG; ++g) {
+        const float w = ex2(s_m[g][r] - base);
+        sum = __fmaf_rn(w, s_l[g][r], sum);
+        o = __fmaf_rn(w, s_acc[(g * NR + r) * DP + dd], o);
+      }
+      if (d.splits > 1) {
+        const int64_t at = ((int64_t)sp * (c.B * c.Hk) + pr) * c.M + row;
+        d.part[at * c.D + dd] = o;
+        if (dd == 0) {
+          d.part_m[at] = mx;
+          d.part_l[at] = sum;
+        }
+      } else {
+        const int gq = (int)fdiv((uint32_t)row, c.f_Tq), t = row - gq * c.Tq, h = hk * c.G + gq;
+        float* op = static_cast<float*>(c.out.p) + b * c.out.sb + t * c.out.st + h * c.out.sh;
+        op[dd * c.out.sd] = sum == 0.f ? 0.f : o / sum;
+        if (dd == 0 && c.lse) c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The parts of the keys joined in order: one warp per (problem, row).
+struct JoinDev {
+  CrossDev c;
+  int splits, rows;          // rows per problem in the partials
+  int ld;                    // elements per partial row
+  const float *part, *part_m, *part_l;
+};
+__global__ void __launch_bounds__(256) cross_join_kernel(const JoinDev d) {
+  const CrossDev& c = d.c;
+  const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const int np = c.B * c.Hk;
+  if (w >= (int64_t)np * c.M) return;
+  const int pr = (int)(w / c.M), row = (int)(w % c.M);
+  float mx = -INFINITY;
+  for (int s = lane; s < d.splits; s += 32) mx = fmaxf(mx, d.part_m[((int64_t)s * np + pr) * d.rows + row]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f, acc[kRowsMaxHead / 32];
+#pragma unroll
+  for (int i = 0; i < kRowsMaxHead / 32; ++i) acc[i] = 0.f;
+  for (int s = 0; s < d.splits; ++s) {
+    const int64_t at = ((int64_t)s * np + pr) * d.rows + row;
+    const float wt = ex2(d.part_m[at] - base);
+    sum = __fmaf_rn(wt, d.part_l[at], sum);
+#pragma unroll
+    for (int i = 0; i < kRowsMaxHead / 32; ++i)
+      if (lane + 32 * i < c.D) acc[i] = __fmaf_rn(wt, d.part[at * d.ld + lane + 32 * i], acc[i]);
+  }
+  const int b = pr / c.Hk, hk = pr % c.Hk;
+  const int g = (int)fdiv((uint32_t)row, c.f_Tq), t = row - g * c.Tq, h = hk * c.G + g;
+  float* op = static_cast<float*>(c.out.p) + b * c.out.sb + t * c.out.st + h * c.out.sh;
+#pragma unroll
+  for (int i = 0; i < kRowsMaxHead / 32; ++i)
+    if (lane + 32 * i < c.D) op[(lane + 32 * i) * c.out.sd] = sum == 0.f ? 0.f : acc[i] / sum;
+  if (lane == 0 && c.lse) c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+}
+
+}  // namespace
+
+Error cross_join(const CrossDev& c, int splits, int rows, int ld, const float* part, const float* part_m,
+                 const float* part_l, cudaStream_t stream) {
+  JoinDev j;
+  j.c = c;
+  j.splits = splits;
+  j.rows = rows;
+  j.ld = ld;
+  j.part = part;
+  j.part_m = part_m;
+  j.part_l = part_l;
+  const int64_t warps = (int64_t)c.B * c.Hk * c.M;
+  cross_join_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(j);
+  return check_launch("cross attention join kernel");
+}
+
+namespace {
+
+// The gradient on the CUDA cores, one warp per query row (dq) or key row (dk,
+// dv): head sizes above 128 and inputs that hold infinities or NaNs.  Each
+// lane holds elements lane, lane + 32, ... of a head.
+constexpr int kGradE = kRowsMaxHead / 32;
+
+struct HeadRow {
+  float x[kGradE];
+};
+__device__ __forceinline__ HeadRow load_row(const float* p, int64_t sd, int D) {
+  HeadRow r;
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int i = 0; i < kGradE; ++i) r.x[i] = lane + 32 * i < D ? p[(lane + 32 * i) * sd] : 0.f;
+  return r;
+}
+__device__ __forceinline__ void store_row(float* p, int64_t sd, int D, const HeadRow& r) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int i = 0; i < kGradE; ++i)
+    if (lane + 32 * i < D) p[(lane + 32 * i) * sd] = r.x[i];
+}
+__device__ __forceinline__ float dot_row(const HeadRow& a, const HeadRow& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGradE; ++i) s = __fmaf_rn(a.x[i], b.x[i], s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+__device__ __forceinline__ const float* row_of(const HeadsDev& h, int b, int t, int head) {
+  return static_cast<const float*>(h.p) + b * h.sb + t * h.st + head * h.sh;
+}
+
+__global__ void __launch_bounds__(256) cross_grad_rows_kernel(const CrossDev c) {
+  if (c.nonfinite && *(volatile const int*)c.nonfinite == 0) return;
+  const int64_t warps = (int64_t)gridDim.x * 8, w0 = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t nq = (int64_t)c.B * c.Hq * c.Tq, nk = (int64_t)c.B * c.Hk * c.Tk;
+  for (int64_t w = w0; w < nq + nk; w += warps) {
+    HeadRow z;
+#pragma unroll
+    for (int i = 0; i < kGradE; ++i) z.x[i] = 0.f;
+    if (w < nq) {  // one query: dq
+      const int t = (int)(w % c.Tq), h = (int)(w / c.Tq % c.Hq), b = (int)(w / c.Tq / c.Hq), hk = h / c.G;
+      const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
+      const HeadRow q = load_row(row_of(c.q, b, t, h), c.q.sd, c.D);
+      const HeadRow go = load_row(row_of(c.dout, b, t, h), c.dout.sd, c.D);
+      const float delta = dot_row(go, load_row(row_of(c.out, b, t, h), c.out.sd, c.D));
+      const float lse = c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t];
+      HeadRow acc = z;
+      for (int j = 0; j < n; ++j) {
+        const HeadRow k = load_row(row_of(c.k, b, j, hk), c.k.sd, c.D);
+        const float s = dot_row(q, k) * c.scale;
+        const float p = lse == -INFINITY ? 0.f : ex2((s - lse) * kLog2e);
+        const float dp = dot_row(go, load_row(row_of(c.v, b, j, hk), c.v.sd, c.D));
+        const float ds = p * (dp - delta) * c.scale;
+#pragma unroll
+        for (int i = 0; i < kGradE; ++i) acc.x[i] = __fmaf_rn(ds, k.x[i], acc.x[i]);
+      }
+      store_row(const_cast<float*>(row_of(c.dq, b, t, h)), c.dq.sd, c.D, acc);
+    } else {  // one key: dk, dv
+      const int64_t r = w - nq;
+      const int j = (int)(r % c.Tk), hk = (int)(r / c.Tk % c.Hk), b = (int)(r / c.Tk / c.Hk);
+      HeadRow ak = z, av = z;
+      if (j < key_count(c.len, c.len64, c.len_s, c.Tk, b)) {
+        const HeadRow k = load_row(row_of(c.k, b, j, hk), c.k.sd, c.D);
+        const HeadRow v = load_row(row_of(c.v, b, j, hk), c.v.sd, c.D);
+        for (int h = hk * c.G; h < (hk + 1) * c.G; ++h) {
+          for (int t = 0; t < c.Tq; ++t) {
+            const HeadRow q = load_row(row_of(c.q, b, t, h), c.q.sd, c.D);
+            const HeadRow go = load_row(row_of(c.dout, b, t, h), c.dout.sd, c.D);
+            const float delta = dot_row(go, load_row(row_of(c.out, b, t, h), c.out.sd, c.D));
+            const float lse = c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t];
+            const float s = dot_row(q, k) * c.scale;
+            const float p = lse == -INFINITY ? 0.f : ex2((s - lse) * kLog2e);
+            const float ds = p * (dot_row(go, v) - delta) * c.scale;
+#pragma unroll
+            for (int i = 0; i < kGradE; ++i) {
+              ak.x[i] = __fmaf_rn(ds, q.x[i], ak.x[i]);
+              av.x[i] = __fmaf_rn(p, go.x[i], av.x[i]);
+            }
+          }
+        }
+      }
+      store_row(const_cast<float*>(row_of(c.dk, b, j, hk)), c.dk.sd, c.D, ak);
+      store_row(const_cast<float*>(row_of(c.dv, b, j, hk)), c.dv.sd, c.D, av);
+    }
+  }
+}
+
+// Gradients of no queries or no keys at all.
+__global__ void __launch_bounds__(256) cross_zero_kernel(HeadsDev x, int64_t B, int T, int H, int D) {
+  const int64_t n = B * T * H * D;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t dd = i % D, h = i / D % H, t = i / D / H % T, b = i / D / H / T;
+    static_cast<float*>(x.p)[b * x.sb + t * x.st + h * x.sh + dd * x.sd] = 0.f;
+  }
+}
+__global__ void __launch_bounds__(256) cross_lse_kernel(const CrossDev c) {
+  const int64_t n = (int64_t)c.B * c.Hq * c.Tq;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    c.lse[i / c.Tq / c.Hq * c.ls_b + i / c.Tq % c.Hq * c.ls_h + i % c.Tq * c.ls_t] = -INFINITY;
+}
+
+Error zero_heads(const HeadsDev& x, int64_t B, int T, int H, int D, cudaStream_t s) {
+  const int64_t n = B * T * H * D;
+  if (n == 0) return Error{};
+  const int64_t g = (n + 255) / 256;
+  cross_zero_kernel<<<(unsigned)(g < 4096 ? g : 4096), 256, 0, s>>>(x, B, T, H, D);
+  return check_launch("cross attention zero kernel");
+}
+
+// ---- host side -------------------------------------------------------------------
+
+template <int NR, int L, int NV>
+Error launch_rows(RowsDev& d, int grid, cudaStream_t s) {
+  constexpr int smem = kRowsThreads / L * NR * L * 4 * NV * 4;
+  auto k = d.c.vec ? cross_rows_kernel<NR, L, NV, true> : cross_rows_kernel<NR, L, NV, false>;
+  allow_smem((const void*)k, smem);
+  k<<<(unsigned)grid, kRowsThreads, smem, s>>>(d);
+  return check_launch("cross attention rows kernel");
+}
+
+Error run_rows(const CrossDev& c, bool fallback, cudaStream_t s) {
+  RowsDev d;
+  std::memset(static_cast<void*>(&d), 0, sizeof(d));
+  d.c = c;
+  const int np = c.B * c.Hk;
+  const int most = c.D <= 128 ? 8 : 4;  // rows a CTA keeps in registers
+  int NR = 1;
+  while (NR < most && NR < c.M) NR *= 2;
+  d.blocks = (c.M + NR - 1) / NR;
+  // parts of the keys until the GPU has about four CTAs per SM, of 256 keys at
+  // least (a part's fixed cost is that of about 100 keys)
+  const int sms = current_device_info().sm_count;
+  const int64_t base = (int64_t)np * d.blocks;
+  int64_t splits = fallback ? 1 : 4 * sms / base;
+  if (splits > c.Tk / 256) splits = c.Tk / 256;
+  if (splits < 1) splits = 1;
+  d.splits = (int)splits;
+  const int64_t items = base * splits;
+  if (items >= (1ll << 31)) return make_error(TRS_ERR_SHAPE, "cross_attention: too many query rows");
+  d.items = (int)items;
+  const int grid = fallback ? (int)std::min<int64_t>(items, 2 * sms) : (int)std::min<int64_t>(items, 1 << 24);
+  Scratch part;
+  if (splits > 1) {
+    const size_t rows = (size_t)splits * np * c.M;
+    Error e = part.alloc(sizeof(float) * rows * (c.D + 2), s);
+    if (!e.ok()) return e;
+    d.part = part.as<float>();
+    d.part_m = d.part + rows * c.D;
+    d.part_l = d.part_m + rows;
+  }
+  Error e;
+  if (c.D <= 64) {
+    e = NR == 1 ? launch_rows<1, 16, 1>(d, grid, s) : NR == 2 ? launch_rows<2, 16, 1>(d, grid, s)
+        : NR == 4 ? launch_rows<4, 16, 1>(d, grid, s) : launch_rows<8, 16, 1>(d, grid, s);
+  } else if (c.D <= 128) {
+    e = NR == 1 ? launch_rows<1, 32, 1>(d, grid, s) : NR == 2 ? launch_rows<2, 32, 1>(d, grid, s)
+        : NR == 4 ? launch_rows<4, 32, 1>(d, grid, s) : launch_rows<8, 32, 1>(d, grid, s);
+  } else {
+    e = NR == 1 ? launch_rows<1, 32, 2>(d, grid, s) : NR == 2 ? launch_rows<2, 32, 2>(d, grid, s)
+                                                              : launch_rows<4, 32, 2>(d, grid, s);
+  }
+  if (!e.ok() || splits == 1) return e;
+  return cross_join(c, d.splits, c.M, c.D, d.part, d.part_m, d.part_l, s);
+}
+
+struct CrossCall {
+  const char* fn;
+  const trs_view *q, *k, *v, *len;
+  double scale;
+  trs_view *out, *lse;                // forward outputs; inputs of the backward
+  const trs_view* dout;               // backward
+  trs_view *dq, *dk, *dv;
+};
+
+Error run_cross(const CrossCall& c, bool backward, cudaStream_t stream) {
+  const std::string fn = c.fn;
+  if (!c.q || !c.k || !c.v || !c.out || (backward && (!c.lse || !c.dout || !c.dq || !c.dk || !c.dv)))
+    return make_error(TRS_ERR_ARG, fn + ": null view");
+  const trs_view* heads[] = {c.q, c.k, c.v, c.out, c.dout, c.dq, c.dk, c.dv};
+  const char* names[] = {"q", "k", "v", "the output", "the output gradient", "the q gradient", "the k gradient",
+                         "the v gradient"};
+  Error e;
+  for (int i = 0; i < (backward ? 8 : 4); ++i) {
+    e = check_heads(c.fn, heads[i], TRS_F32, names[i]);
+    if (!e.ok()) return e;
+  }
+  if (!same_shape(c.out, c.q) || (backward && (!same_shape(c.dout, c.q) || !same_shape(c.dq, c.q))))
+    return make_error(TRS_ERR_SHAPE, fn + ": the output and its gradient must have the shape of q");
+  if (!same_shape(c.k, c.v) || (backward && (!same_shape(c.dk, c.k) || !same_shape(c.dv, c.k))))
+    return make_error(TRS_ERR_SHAPE, fn + ": k, v and their gradients must have one shape");
+  const int64_t B = c.q->shape[0], Tq = c.q->shape[1], Hq = c.q->shape[2], D = c.q->shape[3];
+  const int64_t Tk = c.k->shape[1], Hk = c.k->shape[2];
+  if (c.k->shape[0] != B || c.k->shape[3] != D)
+    return make_error(TRS_ERR_SHAPE, fn + ": q and k must agree in batch and head size");
+  if (Hk == 0 ? Hq != 0 : Hq % Hk != 0)
+    return make_error(TRS_ERR_SHAPE, fn + ": the query heads must be a multiple of the key heads");
+  if (D > kRowsMaxHead) return make_error(TRS_ERR_SHAPE, fn + ": a head size above 256");
+  if (D < 1) return make_error(TRS_ERR_SHAPE, fn + ": an empty head");
+  if (!std::isfinite(c.scale) || !std::isfinite((float)c.scale))
+    return make_error(TRS_ERR_ARG, fn + ": the scale must be finite in f32");
+  if (c.lse) {
+    e = validate_view(c.lse, "lse");
+    if (!e.ok()) return e;
+    if (c.lse->dtype != TRS_F32) return make_error(TRS_ERR_DTYPE, fn + ": lse must be f32");
+    if (c.lse->ndim != 3 || c.lse->shape[0] != B || c.lse->shape[1] != Hq || c.lse->shape[2] != Tq)
+      return make_error(TRS_ERR_SHAPE, fn + ": lse must be [batch, query heads, query tokens]");
+  }
+  if (c.len) {
+    e = validate_view(c.len, "key lengths");
+    if (!e.ok()) return e;
+    if (c.len->dtype != TRS_I32 && c.len->dtype != TRS_I64)
+      return make_error(TRS_ERR_DTYPE, fn + ": key lengths must be i32 or i64");
+    if (c.len->ndim != 1 || c.len->shape[0] != B) return make_error(TRS_ERR_SHAPE, fn + ": key lengths must be [batch]");
+  }
+  // no output may share memory with an input or another output
+  const trs_view* reads[] = {c.q, c.k, c.v, c.len, backward ? c.out : nullptr, backward ? c.lse : nullptr, c.dout};
+  const trs_view* fw[] = {c.out, c.lse};
+  const trs_view* bw[] = {c.dq, c.dk, c.dv};
+  const trs_view** writes = backward ? bw : fw;
+  const int nw = backward ? 3 : 2;
+  for (int i = 0; i < nw; ++i) {
+    if (!writes[i]) continue;
+    if (writes_collide(writes[i])) return make_error(TRS_ERR_ALIAS, fn + ": two elements of an output share a place");
+    for (const trs_view* r : reads)
+      if (r && heads_overlap(writes[i], r)) return make_error(TRS_ERR_ALIAS, fn + ": an output overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (writes[j] && heads_overlap(writes[i], writes[j]))
+        return make_error(TRS_ERR_ALIAS, fn + ": two outputs overlap");
+  }
+  const int64_t lim = (1ll << 31) - 65536;
+  if (B * Hq >= lim || Tq >= lim || Tk >= lim || (Hk && Hq / Hk * Tq >= lim))
+    return make_error(TRS_ERR_SHAPE, fn + ": 2^31 or more heads, tokens or rows");
+  CrossDev d;
+  std::memset(static_cast<void*>(&d), 0, sizeof(d));
+  d.B = (int)B;
+  d.Hq = (int)Hq;
+  d.Hk = (int)Hk;
+  d.Tq = (int)Tq;
+  d.Tk = (int)Tk;
+  d.D = (int)D;
+  d.scale = (float)c.scale;
+  d.q = heads_dev(c.q);
+  d.k = heads_dev(c.k);
+  d.v = heads_dev(c.v);
+  d.out = heads_dev(c.out);
+  if (c.lse) {
+    d.lse = static_cast<float*>(c.lse->data) + c.lse->offset;
+    d.ls_b = c.lse->strides[0];
+    d.ls_h = c.lse->strides[1];
+    d.ls_t = c.lse->strides[2];
+  }
+  if (c.len) {
+    d.len64 = c.len->dtype == TRS_I64;
+    d.len = static_cast<char*>(c.len->data) + c.len->offset * dtype_size(c.len->dtype);
+    d.len_s = c.len->strides[0];
+  }
+  if (backward) {
+    d.dout = heads_dev(c.dout);
+    d.dq = heads_dev(c.dq);
+    d.dk = heads_dev(c.dk);
+    d.dv = heads_dev(c.dv);
+  }
+  if (B * Hq * Tq == 0 || Tk == 0) {  // no queries, or no keys at all
+    if (!backward) {
+      e = zero_heads(d.out, B, d.Tq, d.Hq, d.D, stream);
+      if (!e.ok() || !c.lse || B * Hq * Tq == 0) return e;
+      cross_lse_kernel<<<256, 256, 0, stream>>>(d);
+      return check_launch("cross attention lse kernel");
+    }
+    e = zero_heads(d.dq, B, d.Tq, d.Hq, d.D, stream);
+    if (e.ok()) e = zero_heads(d.dk, B, d.Tk, d.Hk, d.D, stream);
+    if (e.ok()) e = zero_heads(d.dv, B, d.Tk, d.Hk, d.D, stream);
+    return e;
+  }
+  d.G = (int)(Hq / Hk);
+  d.M = d.G * d.Tq;
+  d.f_Tq = make_fastdiv((uint32_t)d.Tq);
+  auto aligned = [](const trs_view* v) {
+    if (((uintptr_t)v->data + (uintptr_t)(v->offset * 4)) % 16 || v->shape[3] % 4) return false;
+    if (v->strides[3] != 1) return false;
+    for (int i = 0; i < 3; ++i)
+      if (v->shape[i] > 1 && v->strides[i] % 4) return false;
+    return true;
+  };
+  d.vec = 1;
+  for (int i = 0; i < (backward ? 8 : 4); ++i) d.vec = d.vec && aligned(heads[i]);
+  const int sms = current_device_info().sm_count;
+  const bool tc = D <= 128 && (backward || d.M > 16);
+  if (!tc) {
+    if (!backward) return run_rows(d, false, stream);
+    cross_grad_rows_kernel<<<8 * sms, 256, 0, stream>>>(d);
+    return check_launch("cross attention gradient rows kernel");
+  }
+  // a word that the split kernel sets when some input is not finite; the
+  // CUDA-core kernel then runs over all of the result
+  Scratch flag;
+  e = flag.alloc(sizeof(int), stream);
+  if (!e.ok()) return e;
+  cudaError_t ce = cudaMemsetAsync(flag.get(), 0, sizeof(int), stream);
+  if (ce != cudaSuccess) return cuda_error(ce, "cudaMemsetAsync");
+  e = backward ? cross_tc_backward(d, flag.as<int>(), stream) : cross_tc_forward(d, flag.as<int>(), stream);
+  if (!e.ok()) return e;
+  d.nonfinite = flag.as<int>();
+  if (!backward) return run_rows(d, true, stream);
+  cross_grad_rows_kernel<<<2 * sms, 256, 0, stream>>>(d);
+  return check_launch("cross attention gradient rows kernel");
+}
+
+trs_status finish(const Error& e) {
+  if (!e.ok()) set_last_error(e.msg);
+  return e.status;
+}
+
+}  // namespace
+}  // namespace trs
+
+using namespace trs;
+
+extern "C" {
+
+trs_status trs_cross_attention(const trs_view* q, const trs_view* k, const trs_view* v, const trs_view* key_lengths,
+                               double scale, trs_view* out, trs_view* lse, trs_stream stream) {
+  CrossCall c = {"cross_attention", q, k, v, key_lengths, scale, out, lse, nullptr, nullptr, nullptr, nullptr};
+  return finish(run_cross(c, false, static_cast<cudaStream_t>(stream)));
+}
+
+trs_status trs_cross_attention_backward(const trs_view* grad_out, const trs_view* q, const trs_view* k,
+                                        const trs_view* v, const trs_view* key_lengths, const trs_view* out,
+                                        const trs_view* lse, double scale, trs_view* grad_q, trs_view* grad_k,
+                                        trs_view* grad_v, trs_stream stream) {
+  CrossCall c = {"cross_attention_backward", q, k, v, key_lengths, scale, const_cast<trs_view*>(out),
+                 const_cast<trs_view*>(lse), grad_out, grad_q, grad_k, grad_v};
+  return finish(run_cross(c, true, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,1238 @@
+// cross_tc.cu -- cross attention and its gradient on the 5th-generation tensor
+// cores, for f32 tensors with head sizes up to 128.
+//
+// Products.  A tile x of an operand is written x = 2^e (hi + lo) with hi and lo
+// in fp16: e places the tile's largest magnitude in [2^14, 2^15), hi is x 2^-e
+// rounded to 11 bits and lo the rest rounded to 11 more.  A product is taken
+// as hi hi + (hi lo + lo hi), three tcgen05.mma with f32 accumulation; lo lo
+// (below 2^-22 of it) is dropped.  Elements down to 2^-17 of the tile's
+// largest keep all 22 bits, and below that the error is 2^-40 of the largest:
+// an f32 result, at a third of the fp16 rate instead of the CUDA cores' rate.
+// P and dS are split the same way in registers, P by the fixed 2^15 of its
+// range, dS by a bound on its row (|dout_i| |v_j| + |delta_i|).  The small
+// products of a tile are accumulated before the large ones, and every tile's
+// result leaves the accumulator for f32 registers, so that a long sum is not
+// carried through the tensor core's own (truncating) additions.
+//
+//   cross_pack_kernel     splits q, k, v (and dout) into planes [hi, lo] of
+//                         [problem][rows][DP], DP = 64 or 128, zeros behind the
+//                         last row, key length and head size: strides, ragged
+//                         lengths and odd head sizes end here.  Also delta, and
+//                         the norms that bound dS.
+//   cross_forward_kernel  a CTA owns MT = 1 or 2 tiles of 128 query rows and
+//                         walks key tiles of KN (128 for DP 64, 64 for DP 128).
+//                         Warp 9 streams K and V tiles by TMA through a ring of
+//                         32 KiB slots; warp 8 issues the MMAs; a warpgroup per
+//                         row tile, one thread per row, keeps the running
+//                         maximum and sum of the softmax, turns S (TMEM) into
+//                         the two planes of P in place, and adds O.  With two
+//                         row tiles one is in the softmax while the other is in
+//                         the tensor core.
+//   cross_backward_kernel dq (rows: queries, walking keys) or dk and dv (rows:
+//                         keys, walking queries); both need S and dP = dout v^T
+//                         of the tile, and write each result once: no atomics,
+//                         at the price of computing S and dP twice.  Two
+//                         warpgroups share the 128 rows and halve the columns.
+//   cross_sum_kernel      joins parts of a split walk in a fixed order.
+//
+// Every wait is bounded; a CTA whose wait runs out sets the async-error word,
+// waits (bounded) for its own copies and MMAs, frees its tensor memory and
+// returns.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "cross.h"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace trs {
+
+Error cross_join(const CrossDev& c, int splits, int rows, int ld, const float* part, const float* part_m,
+                 const float* part_l, cudaStream_t stream);
+
+namespace {
+
+constexpr int kSlot = 32 * 1024;             // a streamed tile: KN x DP, two fp16 planes
+constexpr int kTileElems = 8192;             // elements of a packed tile (KN rows of DP)
+
+// ---- pack --------------------------------------------------------------------
+
+struct PackSrc {
+  HeadsDev x;
+  int G, T;              // rows of a problem: G * T
+  int keys;              // rows end at the key length
+  int rows_p;            // rows of a problem in the planes
+  __half *hi, *lo;
+  float* inv;            // [problem][tile] 2^e
+  float* norm;           // [problem][tile] largest row 2-norm, in units of 2^e; or null
+  float sign;
+  int vec;
+  // the output gradient's tiles also carry, per row: lse in units of log2 (+inf
+  // behind the last row), delta, the row's norm in units of 2^e; per tile the
+  // largest |delta|
+  int grad;
+  HeadsDev out;
+  float *lse2, *delta, *rnorm, *dmax;
+  FastDiv f_T;
+};
+struct PackDev {
+  PackSrc s[4];
+  uint32_t first[5];     // first CTA of each source
+  int n;
+  int Hk, D;
+  const void* len;
+  int len64;
+  int64_t len_s;
+  int Tk;
+  const float* lse;
+  int64_t ls_b, ls_h, ls_t;
+  int* nonfinite;
+};
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+__device__ __forceinline__ float block_max(float x, float* sm) {  // 256 threads, x >= 0
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = x;
+  __syncthreads();
+  x = sm[threadIdx.x % 8];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  __syncthreads();
+  return x;
+}
+
+__device__ __forceinline__ float4 head4(const float* p, int d, int D, int64_t sd, bool vec) {
+  if (vec) return *reinterpret_cast<const float4*>(p + d);  // D is a multiple of 4 and d < D
+  float4 r;
+  r.x = p[d * sd];
+  r.y = d + 1 < D ? p[(d + 1) * sd] : 0.f;
+  r.z = d + 2 < D ? p[(d + 2) * sd] : 0.f;
+  r.w = d + 3 < D ? p[(d + 3) * sd] : 0.f;
+  return r;
+}
+
+// One CTA per tile of KN = 8192 / DP rows; DP / 4 lanes per row.
+template <int DP>
+__global__ void __launch_bounds__(256) cross_pack_kernel(const __grid_constant__ PackDev d) {
+  constexpr int L = DP / 4, PT = kTileElems / DP, RP = 256 / L, NP = PT / RP;
+  __shared__ float sm[8];
+  int w = 0;
+  while (w + 1 < d.n && blockIdx.x >= d.first[w + 1]) ++w;
+  const PackSrc& s = d.s[w];
+  const int tiles = s.rows_p / PT;
+  const int at = (int)(blockIdx.x - d.first[w]), pr = at / tiles, tile = at % tiles;
+  const int b = pr / d.Hk, hk = pr % d.Hk;
+  const int n = s.keys ? key_count(d.len, d.len64, d.len_s, d.Tk, b) : s.G * s.T;
+  const int lane = threadIdx.x % L, r0 = tile * PT + threadIdx.x / L, dd = lane * 4;
+  float4 x[NP];
+  float dl[NP];
+  float mx = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int row = r0 + i * RP;
+    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    dl[i] = 0.f;
+    if (row < n && dd < d.D) {
+      const int g = (int)fdiv((uint32_t)row, s.f_T), t = row - g * s.T, h = hk * s.G + g;
+      x[i] = head4(static_cast<const float*>(s.x.p) + b * s.x.sb + t * s.x.st + h * s.x.sh, dd, d.D, s.x.sd, s.vec);
+      if (s.grad) {
+        const float4 o = head4(static_cast<const float*>(s.out.p) + b * s.out.sb + t * s.out.st + h * s.out.sh, dd, d.D,
+                               s.out.sd, s.vec);
+        dl[i] = __fmaf_rn(x[i].x, o.x, __fmaf_rn(x[i].y, o.y, __fmaf_rn(x[i].z, o.z, x[i].w * o.w)));
+      }
+    }
+    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+    bad |= !(fabsf(x[i].x) <= 3e38f && fabsf(x[i].y) <= 3e38f && fabsf(x[i].z) <= 3e38f && fabsf(x[i].w) <= 3e38f);
+  }
+  if (__any_sync(0xffffffffu, bad) && threadIdx.x % 32 == 0) atomicOr(d.nonfinite, 1);
+  mx = block_max(mx, sm);
+  // up = 2^(14 - exponent of mx), within what an f32 holds; a tile of zeros
+  // (and of the smallest magnitudes) takes 2^126
+  int e = (int)(__float_as_uint(mx) >> 23) - 127;
+  int k = 14 - e;
+  k = k > 126 ? 126 : k;
+  const float up = __uint_as_float((uint32_t)(k + 127) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+  if (threadIdx.x == 0) s.inv[pr * tiles + tile] = down;
+  const float us = up * s.sign;
+  float nm = 0.f, dm = 0.f;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int row = r0 + i * RP;
+    const float v[4] = {x[i].x * us, x[i].y * us, x[i].z * us, x[i].w * us};
+    __half h[4], l[4];
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[j] = __float2half_rn(v[j]);
+      l[j] = __float2half_rn(v[j] - __half2float(h[j]));
+      ss = __fmaf_rn(v[j], v[j], ss);
+    }
+    const int64_t o = ((int64_t)pr * s.rows_p + row) * DP + dd;
+    *reinterpret_cast<uint2*>(s.hi + o) = *reinterpret_cast<uint2*>(h);
+    *reinterpret_cast<uint2*>(s.lo + o) = *reinterpret_cast<uint2*>(l);
+    if (s.norm) {
+      const float rn = sqrtf(lanes_sum<L>(ss));
+      nm = fmaxf(nm, rn);
+      if (s.grad) {
+        const float dlt = lanes_sum<L>(dl[i]);
+        dm = fmaxf(dm, fabsf(dlt));
+        if (lane == 0) {
+          const int64_t at_r = (int64_t)pr * s.rows_p + row;
+          float ls = INFINITY;
+          if (row < n) {
+            const int g = (int)fdiv((uint32_t)row, s.f_T), t = row - g * s.T;
+            ls = d.lse[b * d.ls_b + (hk * s.G + g) * d.ls_h + t * d.ls_t] * kLog2e;
+          }
+          s.lse2[at_r] = ls;
+          s.delta[at_r] = dlt;
+          s.rnorm[at_r] = rn;
+        }
+      }
+    }
+  }
+  if (s.norm) {
+    nm = block_max(nm, sm);
+    dm = block_max(dm, sm);
+    if (threadIdx.x == 0) {
+      s.norm[pr * tiles + tile] = nm;
+      if (s.grad) s.dmax[pr * tiles + tile] = dm;
+    }
+  }
+}
+
+// ---- shared pieces of the tensor-core kernels ------------------------------------
+
+// A packed operand as the kernels see it.
+struct Planes {
+  int rows_p;            // rows of a problem
+  int rows_all;          // rows of all problems: where the lo plane starts
+  const float* inv;
+  const float* norm;
+};
+
+__device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, int* failed) {
+  for (uint32_t i = 0; i < kWaitIters; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 63 && *(volatile int*)failed) return false;
+  }
+  atomicExch(failed, 1);
+  return false;
+}
+
+// Rows [row, row + ROWS) of a problem, both planes, as [plane][64-column
+// block][ROWS][64] with 128-byte swizzle.
+template <int DP, int ROWS>
+__device__ __forceinline__ void load_planes(unsigned char* dst, const CUtensorMap* map, const Planes& p, int row,
+                                            uint64_t* bar) {
+#pragma unroll
+  for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+    for (int h = 0; h < DP / 64; ++h)
+      tma_load_2d(dst + (pl * (DP / 64) + h) * ROWS * 128, map, h * 64, pl * p.rows_all + row, bar);
+}
+
+// fp16 x fp16 -> f32, M 128, N columns; B K-major, or MN-major (bit 16)
+constexpr uint32_t idesc_f16(int n, bool mn) {
+  return (1u << 4) | (mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// D = A B^T over DP: A 128 rows, B KN rows, both in shared memory (planes as
+// load_planes leaves them); the two small products first.
+template <int DP, int KN>
+__device__ __forceinline__ void mma_abt(uint32_t dst, const unsigned char* a, const unsigned char* b) {
+  constexpr uint32_t id = idesc_f16(KN, false);
+  constexpr int HA = 128 * 128, HB = KN * 128, NH = DP / 64;
+  uint32_t acc = 0;
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    const uint64_t ah = sw128_desc(a + h * HA), al = sw128_desc(a + (NH + h) * HA);
+    const uint64_t bh = sw128_desc(b + h * HB), bl = sw128_desc(b + (NH + h) * HB);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      umma_f16_ss(dst, al + 2 * k, bh + 2 * k, id, acc);
+      acc = 1;
+      umma_f16_ss(dst, ah + 2 * k, bl + 2 * k, id, 1);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    const uint64_t ah = sw128_desc(a + h * HA), bh = sw128_desc(b + h * HB);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) umma_f16_ss(dst, ah + 2 * k, bh + 2 * k, id, 1);
+  }
+}
+
+// D = A B over KN: A 128 x KN in tensor memory (chunks of 32 columns: 16
+// columns of hi, 16 of lo), B KN rows of DP columns in shared memory.
+template <int DP, int KN>
+__device__ __forceinline__ void mma_ab(uint32_t dst, uint32_t a, const unsigned char* b) {
+  constexpr uint32_t id = idesc_f16(DP, true);
+  constexpr int HB = KN * 128, NH = DP / 64;
+  const uint64_t bh = sw128_mn_desc(b, HB), bl = sw128_mn_desc(b + NH * HB, HB);
+  uint32_t acc = 0;
+#pragma unroll
+  for (int k = 0; k < KN / 16; ++k) {
+    const uint32_t ak = a + 32 * (k / 2) + 8 * (k % 2);
+    umma_f16_ts(dst, ak + 16, bh + 128 * k, id, acc);
+    acc = 1;
+    umma_f16_ts(dst, ak, bl + 128 * k, id, 1);
+  }
+#pragma unroll
+  for (int k = 0; k < KN / 16; ++k) umma_f16_ts(dst, a + 32 * (k / 2) + 8 * (k % 2), bh + 128 * k, id, 1);
+}
+
+// The two planes of two values below 2^16: hi = the value cut to 11 bits, lo =
+// the rest (exact) rounded to 11.
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
+  const float bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+  const __half2 h = __floats2half2_rn(ah, bh), l = __floats2half2_rn(a - ah, b - bh);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// What a CTA still has in flight when it gave up: its copies (the slots'
+// latest phases) and its MMAs.
+__device__ __forceinline__ void drain(uint64_t* full, int slots, int issued) {
+  for (int s = 0; s < slots && s < issued; ++s) {
+    const int last = (issued - 1 - s) / slots;  // uses of this slot so far, less one
+    mbar_wait(&full[s], (uint32_t)last & 1u);
+  }
+}
+
+// ---- forward ---------------------------------------------------------------------
+
+struct FwdDev {
+  CrossDev c;
+  Planes q, k, v;
+  int mtiles, splits;    // CTAs: mtiles * problems * splits
+  float *part, *part_m, *part_l;  // [split][problem][q.rows_p](DP) when splits > 1
+  float f;               // |scale| log2 e
+  const int* nonfinite;
+  int* err;
+};
+
+template <int DP, int MT>
+struct FwdShape {
+  static constexpr int KN = kTileElems / DP;
+  static constexpr int q_bytes = MT * 128 * DP * 4;
+  static constexpr int slots = MT == 2 ? (DP == 64 ? 5 : 3) : 4;
+  static constexpr int smem = q_bytes + slots * kSlot + 1024 + 512;
+  static constexpr int OB = DP == 64 ? 2 : 1;       // output accumulators per row tile
+  static constexpr int cols = KN + OB * DP;         // tensor-memory columns per row tile
+  static constexpr int threads = MT * 128 + 64;
+};
+
+template <int DP, int MT>
+__global__ void __launch_bounds__(MT * 128 + 64, 1)
+cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                     const __grid_constant__ CUtensorMap mv, const __grid_constant__ FwdDev d) {
+  using S = FwdShape<DP, MT>;
+  constexpr int KN = S::KN, OB = S::OB, NS = S::slots;
+  static_assert(MT * S::cols <= 512, "tensor memory");
+  const CrossDev& c = d.c;
+  if (*(volatile const int*)d.nonfinite != 0) return;  // the CUDA-core kernel serves this call
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* sq = smem;
+  unsigned char* ring = smem + S::q_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * kSlot);
+  uint64_t* empty = full + NS;
+  uint64_t* qfull = empty + NS;
+  uint64_t* s_full = qfull + 1;        // [MT]
+  uint64_t* p_ready = s_full + MT;     // [MT]
+  uint64_t* o_full = p_ready + MT;     // [MT][OB]
+  uint64_t* o_free = o_full + MT * OB; // [MT][OB]
+  uint64_t* done = o_free + MT * OB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(qfull, 1);
+    for (int t = 0; t < MT; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_ready[t], 128);
+      for (int o = 0; o < OB; ++o) {
+        mbar_init(&o_full[t * OB + o], 1);
+        mbar_init(&o_free[t * OB + o], 128);
+      }
+    }
+    mbar_init(done, 1);
+    *failed = 0;
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int np = c.B * c.Hk;
+  const int mtile = blockIdx.x % d.mtiles, pr = blockIdx.x / d.mtiles % np, sp = blockIdx.x / d.mtiles / np;
+  const int b = pr / c.Hk, hk = pr % c.Hk;
+  const int len = key_count(c.len, c.len64, c.len_s, c.Tk, b);
+  const int all = (len + KN - 1) / KN, per = (all + d.splits - 1) / d.splits;
+  const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;  // this CTA's key tiles
+
+  if (warp == MT * 4 + 1) {
+    if (lane == 0 && n > 0) {  // TMA
+      mbar_arrive_expect_tx(qfull, S::q_bytes);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        load_planes<DP, 128>(sq + t * 128 * DP * 4, &mq, d.q, pr * d.q.rows_p + (mtile * MT + t) * 128, qfull);
+      int i = 0;
+      for (; i < 2 * n; ++i) {
+        const int s = i % NS;
+        if (i >= NS && !wait_or_fail(&empty[s], (uint32_t)(i / NS - 1) & 1u, failed)) break;
+        mbar_arrive_expect_tx(&full[s], kSlot);
+        const int row = pr * d.k.rows_p + (j0 + i / 2) * KN;
+        if (i & 1) load_planes<DP, KN>(ring + s * kSlot, &mv, d.v, row, &full[s]);
+        else load_planes<DP, KN>(ring + s * kSlot, &mk, d.k, row, &full[s]);
+      }
+      if (i < 2 * n) {
+        mbar_wait(qfull, 0);
+        drain(full, NS, i);
+      }
+    }
+  } else if (warp == MT * 4) {
+    if (lane == 0 && n > 0) {  // MMA
+      bool ok = wait_or_fail(qfull, 0, failed) && wait_or_fail(&full[0], 0, failed);
+      if (ok) {
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          mma_abt<DP, KN>(tmem + t * S::cols, sq + t * 128 * DP * 4, ring);
+          umma_commit(&s_full[t]);
+        }
+        umma_commit(&empty[0]);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int iv = 2 * j + 1, ik = 2 * j + 2, ob = j % OB;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          ok = ok && wait_or_fail(&p_ready[t], (uint32_t)j & 1u, failed) &&
+               (t > 0 || wait_or_fail(&full[iv % NS], (uint32_t)(iv / NS) & 1u, failed)) &&
+               (j < OB || wait_or_fail(&o_free[t * OB + ob], (uint32_t)(j / OB - 1) & 1u, failed));
+          if (!ok) break;
+          tc_fence_after();
+          mma_ab<DP, KN>(tmem + t * S::cols + KN + ob * DP, tmem + t * S::cols, ring + (iv % NS) * kSlot);
+          umma_commit(&o_full[t * OB + ob]);
+          if (t == MT - 1) umma_commit(&empty[iv % NS]);
+          if (j + 1 < n) {
+            ok = t > 0 || wait_or_fail(&full[ik % NS], (uint32_t)(ik / NS) & 1u, failed);
+            if (!ok) break;
+            tc_fence_after();
+            mma_abt<DP, KN>(tmem + t * S::cols, sq + t * 128 * DP * 4, ring + (ik % NS) * kSlot);
+            umma_commit(&s_full[t]);
+            if (t == MT - 1) umma_commit(&empty[ik % NS]);
+          }
+        }
+      }
+      if (!ok) {
+        umma_commit(done);
+        mbar_wait(done, 0);
+      }
+    }
+  } else {  // softmax: one thread per row
+    const int t = warp / 4;
+    const int rl = (warp % 4) * 32 + lane, row = (mtile * MT + t) * 128 + rl;
+    const uint32_t sbase = tmem + ((uint32_t)((warp % 4) * 32) << 16) + t * S::cols, obase = sbase + KN;
+    const int qtiles = d.q.rows_p / KN;
+    const float fq = d.f * d.q.inv[pr * qtiles + row / KN];
+    const float* kinv = d.k.inv + pr * (d.k.rows_p / KN) + j0;
+    const float* vinv = d.v.inv + pr * (d.v.rows_p / KN) + j0;
+    float m = -INFINITY, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
+    float acc[DP];
+#pragma unroll
+    for (int i = 0; i < DP; ++i) acc[i] = 0.f;
+    bool ok = true;
+    // adds tile j's P V to the output
+    auto add_output = [&](int j) {
+      const int ob = j % OB;
+      const bool here = wait_or_fail(&o_full[t * OB + ob], (uint32_t)(j / OB) & 1u, failed);
+      if (!__all_sync(0xffffffffu, here)) return false;
+      tc_fence_after();
+      const float fv = vinv[j];
+#pragma unroll
+      for (int cc = 0; cc < DP / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld32_issue(obase + ob * DP + cc * 32, o);
+        tmem_ld_done(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[cc * 32 + i] = __fmaf_rn(__uint_as_float(o[i]), fv, acc[cc * 32 + i] * keep);
+      }
+      tc_fence_before();
+      mbar_arrive(&o_free[t * OB + ob]);
+      return true;
+    };
+    for (int j = 0; j < n; ++j) {
+      const float f = fq * kinv[j];
+      const int limit = len - (j0 + j) * KN;  // keys of this tile
+      ok = wait_or_fail(&s_full[t], (uint32_t)j & 1u, failed);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+      float mx = -INFINITY;
+#pragma unroll
+      for (int cc = 0; cc < KN / 64; ++cc) {
+        uint32_t a[32], e[32];
+        tmem_ld32_issue(sbase + cc * 64, a);
+        tmem_ld32_issue(sbase + cc * 64 + 32, e);
+        tmem_ld_done(a);
+        tmem_ld_tie(e);
+        if (limit >= (cc + 1) * 64) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(a[i]), __uint_as_float(e[i])));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (cc * 64 + i < limit) mx = fmaxf(mx, __uint_as_float(a[i]));
+            if (cc * 64 + 32 + i < limit) mx = fmaxf(mx, __uint_as_float(e[i]));
+          }
+        }
+      }
+      const float mn = fmaxf(m, mx * f);
+      const float alpha = ex2(m - mn);
+      const float bias = 15.f - mn;
+      m = mn;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < KN / 32; ++cc) {
+        uint32_t a[32], w[32];
+        tmem_ld32_issue(sbase + cc * 32, a);
+        tmem_ld_done(a);
+        const bool part = limit < (cc + 1) * 32;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float p0 = ex2(__fmaf_rn(__uint_as_float(a[2 * i]), f, bias));
+          float p1 = ex2(__fmaf_rn(__uint_as_float(a[2 * i + 1]), f, bias));
+          if (part) {
+            if (cc * 32 + 2 * i >= limit) p0 = 0.f;
+            if (cc * 32 + 2 * i + 1 >= limit) p1 = 0.f;
+          }
+          sum0 += p0;
+          sum1 += p1;
+          split2(p0, p1, &w[i], &w[16 + i]);
+        }
+        tmem_st32(sbase + cc * 32, w);
+      }
+      l = __fmaf_rn(l, alpha, sum0 + sum1);
+      tmem_st_done();
+      tc_fence_before();
+      mbar_arrive(&p_ready[t]);
+      if (j > 0) {
+        ok = add_output(j - 1);
+        if (!ok) break;
+      }
+      keep = alpha;
+    }
+    if (ok && n > 0) ok = add_output(n - 1);
+    if (ok && row < c.M) {
+      if (d.splits > 1) {
+        const int64_t at = ((int64_t)sp * np + pr) * d.q.rows_p + row;
+        float4* o = reinterpret_cast<float4*>(d.part + at * DP);
+#pragma unroll
+        for (int i = 0; i < DP / 4; ++i) o[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+        d.part_m[at] = m - 15.f;  // acc and l carry 2^15
+        d.part_l[at] = l;
+      } else {
+        const int g = (int)fdiv((uint32_t)row, c.f_Tq), tt = row - g * c.Tq, h = hk * c.G + g;
+        float* op = static_cast<float*>(c.out.p) + b * c.out.sb + tt * c.out.st + h * c.out.sh;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (c.vec) {
+#pragma unroll
+          for (int i = 0; i < DP / 4; ++i)
+            if (4 * i < c.D)
+              reinterpret_cast<float4*>(op)[i] =
+                  make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv, acc[4 * i + 3] * inv);
+        } else {
+#pragma unroll
+          for (int i = 0; i < DP; ++i)
+            if (i < c.D) op[i * c.out.sd] = acc[i] * inv;
+        }
+        if (c.lse) c.lse[b * c.ls_b + h * c.ls_h + tt * c.ls_t] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * kLn2;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *failed && d.err) atomicOr(d.err, kAsyncWaitTimeout);
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// ---- backward --------------------------------------------------------------------
+
+struct BwdDev {
+  CrossDev c;
+  Planes a1, a2, b1, b2;       // dq: q, dout, k, v;  dk/dv: k, v, q, dout
+  int mtiles, splits;
+  const float *lse2, *delta, *rnorm, *dmax;  // per query row; per query tile
+  float *part1, *part2;        // [split][problem][a1.rows_p][DP] when splits > 1: dq, or dk and dv
+  float f;                     // |scale| log2 e
+  float out_scale;             // of dq (scale) or dk (|scale|)
+  const int* nonfinite;
+  int* err;
+};
+
+template <int DP>
+struct BwdShape {
+  static constexpr int KN = kTileElems / DP;
+  static constexpr int a_bytes = 128 * DP * 4;
+  static constexpr int n1 = DP == 64 ? 3 : 2, n2 = DP == 64 ? 2 : 1;
+  static constexpr int smem = 2 * a_bytes + (n1 + n2) * kSlot + 1024 + 512;
+  static constexpr int threads = 320;
+};
+
+template <int DP, bool KV>
+__global__ void __launch_bounds__(320, 1)
+cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_constant__ CUtensorMap ma2,
+                      const __grid_constant__ CUtensorMap mb1, const __grid_constant__ CUtensorMap mb2,
+                      const __grid_constant__ BwdDev d) {
+  using S = BwdShape<DP>;
+  constexpr int KN = S::KN, N1 = S::n1, N2 = S::n2, HC = KN / 2;  // HC: columns of a warpgroup
+  constexpr int AC = KV ? DP : DP / 2;                            // result columns of a warpgroup
+  static_assert(3 * KN + (KV ? 2 : 1) * DP <= 512, "tensor memory");
+  const CrossDev& c = d.c;
+  if (*(volatile const int*)d.nonfinite != 0) return;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* sa1 = smem;
+  unsigned char* sa2 = smem + S::a_bytes;
+  unsigned char* ring1 = sa2 + S::a_bytes;
+  unsigned char* ring2 = ring1 + N1 * kSlot;
+  uint64_t* full1 = reinterpret_cast<uint64_t*>(ring2 + N2 * kSlot);
+  uint64_t* empty1 = full1 + N1;
+  uint64_t* full2 = empty1 + N1;
+  uint64_t* empty2 = full2 + N2;
+  uint64_t* afull = empty2 + N2;
+  uint64_t* s_full = afull + 1;    // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* p_ready = dp_full + 1;
+  uint64_t* ds_ready = p_ready + 1;
+  uint64_t* r_full = ds_ready + 1;
+  uint64_t* r_free = r_full + 1;
+  uint64_t* done = r_free + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < N1; ++s) {
+      mbar_init(&full1[s], 1);
+      mbar_init(&empty1[s], 1);
+    }
+    for (int s = 0; s < N2; ++s) {
+      mbar_init(&full2[s], 1);
+      mbar_init(&empty2[s], 1);
+    }
+    mbar_init(afull, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_ready, 256);
+    mbar_init(ds_ready, 256);
+    mbar_init(r_full, 1);
+    mbar_init(r_free, 256);
+    mbar_init(done, 1);
+    *failed = 0;
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // columns: S (two buffers), dP, then the results (dq; dk, dv)
+  const uint32_t t_dp = tmem + 2 * KN, t_r1 = tmem + 3 * KN, t_r2 = t_r1 + DP;
+
+  const int np = c.B * c.Hk;
+  const int mtile = blockIdx.x % d.mtiles, pr = blockIdx.x / d.mtiles % np, sp = blockIdx.x / d.mtiles / np;
+  const int b = pr / c.Hk, hk = pr % c.Hk;
+  const int len = key_count(c.len, c.len64, c.len_s, c.Tk, b);
+  const int cols = KV ? c.M : len;                  // columns of the walk
+  const int rows = KV ? len : c.M;                  // rows with work
+  int all = (cols + KN - 1) / KN;
+  if (mtile * 128 >= rows || len == 0) all = 0;
+  const int per = (all + d.splits - 1) / d.splits;
+  const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;
+
+  if (warp == 9) {
+    if (lane == 0 && n > 0) {  // TMA
+      mbar_arrive_expect_tx(afull, 2 * S::a_bytes);
+      load_planes<DP, 128>(sa1, &ma1, d.a1, pr * d.a1.rows_p + mtile * 128, afull);
+      load_planes<DP, 128>(sa2, &ma2, d.a2, pr * d.a2.rows_p + mtile * 128, afull);
+      int i1 = 0, i2 = 0;
+      for (int j = 0; j < n; ++j) {
+        const int row = pr * d.b1.rows_p + (j0 + j) * KN;
+        const int s1 = j % N1, s2 = j % N2;
+        if (j >= N1 && !wait_or_fail(&empty1[s1], (uint32_t)(j / N1 - 1) & 1u, failed)) break;
+        mbar_arrive_expect_tx(&full1[s1], kSlot);
+        load_planes<DP, KN>(ring1 + s1 * kSlot, &mb1, d.b1, row, &full1[s1]);
+        ++i1;
+        if (j >= N2 && !wait_or_fail(&empty2[s2], (uint32_t)(j / N2 - 1) & 1u, failed)) break;
+        mbar_arrive_expect_tx(&full2[s2], kSlot);
+        load_planes<DP, KN>(ring2 + s2 * kSlot, &mb2, d.b2, row, &full2[s2]);
+        ++i2;
+      }
+      if (i2 < n) {
+        mbar_wait(afull, 0);
+        drain(full1, N1, i1);
+        drain(full2, N2, i2);
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0 && n > 0) {  // MMA
+      auto s_mma = [&](int j) {
+        if (!wait_or_fail(&full1[j % N1], (uint32_t)(j / N1) & 1u, failed)) return false;
+        tc_fence_after();
+        mma_abt<DP, KN>(tmem + (j & 1) * KN, sa1, ring1 + (j % N1) * kSlot);
+        umma_commit(&s_full[j & 1]);
+        return true;
+      };
+      auto dp_mma = [&](int j) {
+        if (!wait_or_fail(&full2[j % N2], (uint32_t)(j / N2) & 1u, failed)) return false;
+        tc_fence_after();
+        mma_abt<DP, KN>(t_dp, sa2, ring2 + (j % N2) * kSlot);
+        umma_commit(dp_full);
+        if (!KV) umma_commit(&empty2[j % N2]);
+        return true;
+      };
+      bool ok = wait_or_fail(afull, 0, failed) && s_mma(0) && dp_mma(0);
+      for (int j = 0; j < n && ok; ++j) {
+        const uint32_t ph = (uint32_t)j & 1u;
+        if (KV) {
+          ok = wait_or_fail(p_ready, ph, failed) && (j == 0 || wait_or_fail(r_free, ph ^ 1u, failed));
+          if (!ok) break;
+          tc_fence_after();
+          mma_ab<DP, KN>(t_r2, tmem + (j & 1) * KN, ring2 + (j % N2) * kSlot);  // P^T dout
+          umma_commit(&empty2[j % N2]);
+        }
+        if (j + 1 < n && !(ok = s_mma(j + 1))) break;
+        ok = wait_or_fail(ds_ready, ph, failed) && (KV || j == 0 || wait_or_fail(r_free, ph ^ 1u, failed));
+        if (!ok) break;
+        tc_fence_after();
+        mma_ab<DP, KN>(t_r1, t_dp, ring1 + (j % N1) * kSlot);  // dS k, or dS^T q
+        umma_commit(&empty1[j % N1]);
+        umma_commit(r_full);
+        if (j + 1 < n) ok = dp_mma(j + 1);
+      }
+      if (!ok) {
+        umma_commit(done);
+        mbar_wait(done, 0);
+      }
+    }
+  } else {
+    const int wg = warp / 4;
+    const int row = mtile * 128 + (warp % 4) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    const int at1 = d.a1.rows_p / KN, bt = d.b1.rows_p / KN;
+    const float ia1 = d.a1.inv[pr * at1 + row / KN], ia2 = d.a2.inv[pr * at1 + row / KN];
+    const float* ib1 = d.b1.inv + pr * bt + j0;
+    const float* ib2 = d.b2.inv + pr * bt + j0;
+    const float* nb2 = d.b2.norm + pr * bt + j0;
+    // per query row: of this row (dq) or of the columns (dk, dv)
+    const int64_t qrow = (int64_t)pr * (KV ? d.b1.rows_p : d.a1.rows_p) + (KV ? j0 * KN + wg * HC : row);
+    const float r_lse = KV ? 0.f : d.lse2[qrow], r_delta = KV ? 0.f : d.delta[qrow];
+    const float r_norm = KV ? d.a2.norm[pr * at1 + row / KN] : d.rnorm[qrow];
+    const float* dmax = KV ? d.dmax + pr * bt + j0 : nullptr;
+    float acc[AC];
+#pragma unroll
+    for (int i = 0; i < AC; ++i) acc[i] = 0.f;
+    float ds_down = 0.f;  // what the dS of the last tile was divided by, undone
+    bool ok = true;
+    auto add_result = [&](int j) {  // tile j's result into registers: wg 0 of (dk, dv) takes dv
+      const bool here = wait_or_fail(r_full, (uint32_t)j & 1u, failed);
+      if (!__all_sync(0xffffffffu, here)) return false;
+      tc_fence_after();
+      const float w = KV ? (wg == 0 ? ib2[j] * 0x1p-15f : ib1[j] * d.out_scale * ds_down) : ib1[j] * d.out_scale * ds_down;
+      const uint32_t src = KV ? (wg == 0 ? t_r2 : t_r1) : t_r1 + wg * AC;
+#pragma unroll
+      for (int cc = 0; cc < AC / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld32_issue(src + lanes + cc * 32, o);
+        tmem_ld_done(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[cc * 32 + i] = __fmaf_rn(__uint_as_float(o[i]), w, acc[cc * 32 + i]);
+      }
+      tc_fence_before();
+      mbar_arrive(r_free);
+      return true;
+    };
+    for (int j = 0; j < n; ++j) {
+      const int limit = cols - (j0 + j) * KN - wg * HC;  // columns of this warpgroup's half
+      const float f = d.f * ia1 * ib1[j];
+      const uint32_t sb = tmem + lanes + (j & 1) * KN + wg * HC, db = t_dp + lanes + wg * HC;
+      ok = wait_or_fail(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, failed);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+      float p[HC];  // dk, dv: P 2^15
+#pragma unroll
+      for (int cc = 0; cc < HC / 32; ++cc) {
+        uint32_t a[32];
+        tmem_ld32_issue(sb + cc * 32, a);
+        tmem_ld_done(a);
+        if (KV) {
+          const float4* ls = reinterpret_cast<const float4*>(d.lse2 + qrow + j * KN + cc * 32);
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 q = __ldg(ls + i);
+            p[cc * 32 + 4 * i] = ex2(__fmaf_rn(__uint_as_float(a[4 * i]), f, 15.f - q.x));
+            p[cc * 32 + 4 * i + 1] = ex2(__fmaf_rn(__uint_as_float(a[4 * i + 1]), f, 15.f - q.y));
+            p[cc * 32 + 4 * i + 2] = ex2(__fmaf_rn(__uint_as_float(a[4 * i + 2]), f, 15.f - q.z));
+            p[cc * 32 + 4 * i + 3] = ex2(__fmaf_rn(__uint_as_float(a[4 * i + 3]), f, 15.f - q.w));
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) split2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1], &w[i], &w[16 + i]);
+          tmem_st32(sb + cc * 32, w);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[cc * 32 + i] = ex2(__fmaf_rn(__uint_as_float(a[i]), f, -r_lse));
+        }
+      }
+      if (KV) {
+        tmem_st_done();
+        tc_fence_before();
+        mbar_arrive(p_ready);
+      }
+      if (j > 0) {
+        ok = add_result(j - 1);
+        if (!ok) break;
+      }
+      // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below 2^15
+      const float g = ia2 * ib2[j];
+      const float bound = __fmaf_rn(r_norm * nb2[j], g, KV ? dmax[j] : fabsf(r_delta));
+      uint32_t eb = __float_as_uint(bound) >> 23;
+      eb = eb < 15u ? 15u : eb;
+      const float up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);
+      ds_down = __uint_as_float((eb - 14u) << 23);
+      const float gu = g * up;
+      ok = wait_or_fail(dp_full, (uint32_t)j & 1u, failed);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int cc = 0; cc < HC / 32; ++cc) {
+        uint32_t a[32], w[32];
+        tmem_ld32_issue(db + cc * 32, a);
+        tmem_ld_done(a);
+        if (KV) {
+          const float4* dl = reinterpret_cast<const float4*>(d.delta + qrow + j * KN + cc * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 q = __ldg(dl + i);
+            const float x0 = p[cc * 32 + 4 * i] * __fmaf_rn(__uint_as_float(a[4 * i]), gu, -q.x * up);
+            const float x1 = p[cc * 32 + 4 * i + 1] * __fmaf_rn(__uint_as_float(a[4 * i + 1]), gu, -q.y * up);
+            const float x2 = p[cc * 32 + 4 * i + 2] * __fmaf_rn(__uint_as_float(a[4 * i + 2]), gu, -q.z * up);
+            const float x3 = p[cc * 32 + 4 * i + 3] * __fmaf_rn(__uint_as_float(a[4 * i + 3]), gu, -q.w * up);
+            split2(x0, x1, &w[2 * i], &w[16 + 2 * i]);
+            split2(x2, x3, &w[2 * i + 1], &w[16 + 2 * i + 1]);
+          }
+        } else {
+          const float du = -r_delta * up;
+          const bool part = limit < (cc + 1) * 32;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float x0 = p[cc * 32 + 2 * i] * __fmaf_rn(__uint_as_float(a[2 * i]), gu, du);
+            float x1 = p[cc * 32 + 2 * i + 1] * __fmaf_rn(__uint_as_float(a[2 * i + 1]), gu, du);
+            if (part) {
+              if (cc * 32 + 2 * i >= limit) x0 = 0.f;
+              if (cc * 32 + 2 * i + 1 >= limit) x1 = 0.f;
+            }
+            split2(x0, x1, &w[i], &w[16 + i]);
+          }
+        }
+        tmem_st32(db + cc * 32, w);
+      }
+      tmem_st_done();
+      tc_fence_before();
+      mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) ok = add_result(n - 1);
+    const int stored = KV ? c.Tk : c.M;  // rows of the result; those without work hold zeros
+    if (ok && row < stored) {
+      const bool live = row < rows;
+      if (d.splits > 1) {
+        float* pp = (KV && wg == 0 ? d.part2 : d.part1) + (((int64_t)sp * np + pr) * d.a1.rows_p + row) * DP + (KV ? 0 : wg * AC);
+#pragma unroll
+        for (int i = 0; i < AC / 4; ++i)
+          reinterpret_cast<float4*>(pp)[i] = live ? make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3])
+                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        const HeadsDev& o = KV ? (wg == 0 ? c.dv : c.dk) : c.dq;
+        const int g = KV ? 0 : (int)fdiv((uint32_t)row, c.f_Tq), t = KV ? row : row - g * c.Tq;
+        const int h = KV ? hk : hk * c.G + g, c0 = KV ? 0 : wg * AC;
+        float* op = static_cast<float*>(o.p) + b * o.sb + t * o.st + h * o.sh;
+#pragma unroll
+        for (int i = 0; i < AC; i += 4) {
+          const float4 x = live ? make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (c.vec) {
+            if (c0 + i < c.D) *reinterpret_cast<float4*>(op + c0 + i) = x;
+          } else {
+            if (c0 + i < c.D) op[(c0 + i) * o.sd] = x.x;
+            if (c0 + i + 1 < c.D) op[(c0 + i + 1) * o.sd] = x.y;
+            if (c0 + i + 2 < c.D) op[(c0 + i + 2) * o.sd] = x.z;
+            if (c0 + i + 3 < c.D) op[(c0 + i + 3) * o.sd] = x.w;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *failed && d.err) atomicOr(d.err, kAsyncWaitTimeout);
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// result[row] = the parts added in order
+struct SumDev {
+  const float* part;
+  HeadsDev out;
+  int splits, np, rows_p, ld, Hk, G, T, D;
+  FastDiv f_T;
+  int64_t n;             // problems * G * T * (ld / 4)
+  const int* nonfinite;
+};
+__global__ void __launch_bounds__(256) cross_sum_kernel(const SumDev d) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= d.n || *(volatile const int*)d.nonfinite != 0) return;
+  const int q = d.ld / 4, c = (int)(i % q) * 4;
+  const int64_t r = i / q;
+  const int row = (int)(r % (d.G * d.T)), pr = (int)(r / (d.G * d.T));
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < d.splits; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(d.part + (((int64_t)k * d.np + pr) * d.rows_p + row) * d.ld + c);
+    s.x += x.x;
+    s.y += x.y;
+    s.z += x.z;
+    s.w += x.w;
+  }
+  const int g = (int)fdiv((uint32_t)row, d.f_T), t = row - g * d.T;
+  float* o = static_cast<float*>(d.out.p) + (pr / d.Hk) * d.out.sb + t * d.out.st + (pr % d.Hk * d.G + g) * d.out.sh;
+  if (c < d.D) o[c * d.out.sd] = s.x;
+  if (c + 1 < d.D) o[(c + 1) * d.out.sd] = s.y;
+  if (c + 2 < d.D) o[(c + 2) * d.out.sd] = s.z;
+  if (c + 3 < d.D) o[(c + 3) * d.out.sd] = s.w;
+}
+
+// ---- host side -------------------------------------------------------------------
+
+// The planes, scales and norms of one operand inside the workspace.
+struct Packed {
+  __half *hi = nullptr, *lo = nullptr;
+  float *inv = nullptr, *norm = nullptr;
+  int rows_p = 0, rows_all = 0;
+  CUtensorMap map128, mapKN;
+  Planes planes() const { return Planes{rows_p, rows_all, inv, norm}; }
+};
+
+struct Arena {  // sizes first (base null), then places
+  char* base = nullptr;
+  size_t used = 0;
+  template <class T> T* take(size_t n) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += (n * sizeof(T) + 1023) / 1024 * 1024;
+    return p;
+  }
+};
+
+Error plane_map(EncodeTiled enc, CUtensorMap* map, const __half* hi, int64_t rows2, int DP, int box) {
+  const cuuint64_t dims[2] = {(cuuint64_t)DP, (cuuint64_t)rows2};
+  const cuuint64_t strides[1] = {(cuuint64_t)DP * 2};
+  const cuuint32_t bx[2] = {64, (cuuint32_t)box};
+  const cuuint32_t es[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(hi), dims, strides, bx, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return make_error(TRS_ERR_CUDA, "cross_attention: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return Error{};
+}
+
+int up_to(int x, int m) { return (x + m - 1) / m * m; }
+
+void place(Arena& a, Packed& p, int np, int rows, int DP, bool norm) {
+  p.rows_p = up_to(rows, 256);
+  p.rows_all = np * p.rows_p;
+  p.hi = a.take<__half>((size_t)p.rows_all * DP * 2);
+  p.lo = p.hi + (size_t)p.rows_all * DP;
+  const int tiles = p.rows_all / (kTileElems / DP);
+  p.inv = a.take<float>(tiles);
+  p.norm = norm ? a.take<float>(tiles) : nullptr;
+}
+
+Error maps(EncodeTiled enc, Packed& p, int DP) {
+  Error e = plane_map(enc, &p.map128, p.hi, 2ll * p.rows_all, DP, 128);
+  if (e.ok()) e = plane_map(enc, &p.mapKN, p.hi, 2ll * p.rows_all, DP, kTileElems / DP);
+  return e;
+}
+
+void add_source(PackDev& d, const CrossDev& c, const HeadsDev& x, const Packed& p, int G, int T, bool keys, int DP) {
+  PackSrc& s = d.s[d.n];
+  s.x = x;
+  s.G = G;
+  s.T = T;
+  s.f_T = make_fastdiv((uint32_t)T);
+  s.keys = keys;
+  s.rows_p = p.rows_p;
+  s.hi = p.hi;
+  s.lo = p.lo;
+  s.inv = p.inv;
+  s.norm = p.norm;
+  s.sign = 1.f;
+  s.vec = c.vec;
+  if (d.n == 0) d.first[0] = 0;
+  d.first[d.n + 1] = d.first[d.n] + (uint32_t)(p.rows_all / (kTileElems / DP));
+  ++d.n;
+}
+
+Error run_pack(PackDev& d, const CrossDev& c, int DP, int* nonfinite, cudaStream_t stream) {
+  d.Hk = c.Hk;
+  d.D = c.D;
+  d.len = c.len;
+  d.len64 = c.len64;
+  d.len_s = c.len_s;
+  d.Tk = c.Tk;
+  d.lse = c.lse;
+  d.ls_b = c.ls_b;
+  d.ls_h = c.ls_h;
+  d.ls_t = c.ls_t;
+  d.nonfinite = nonfinite;
+  if (DP == 64) cross_pack_kernel<64><<<d.first[d.n], 256, 0, stream>>>(d);
+  else cross_pack_kernel<128><<<d.first[d.n], 256, 0, stream>>>(d);
+  return check_launch("cross attention pack kernel");
+}
+
+Error too_large(const CrossDev& c) {
+  // planes of rows and their lo half within a tensor map's 31-bit coordinate
+  const int64_t np = (int64_t)c.B * c.Hk;
+  if (np * (c.M + 256ll) >= (1ll << 29) || np * (c.Tk + 256ll) >= (1ll << 29))
+    return make_error(TRS_ERR_SHAPE, "cross_attention: 2^29 or more rows of all heads");
+  return Error{};
+}
+
+template <int DP, int MT>
+Error launch_forward(const Packed& q, const Packed& k, const Packed& v, FwdDev& f, cudaStream_t stream) {
+  using S = FwdShape<DP, MT>;
+  auto kern = cross_forward_kernel<DP, MT>;
+  allow_smem((const void*)kern, S::smem);
+  kern<<<(unsigned)(f.mtiles * f.c.B * f.c.Hk * f.splits), S::threads, S::smem, stream>>>(q.map128, k.mapKN, v.mapKN, f);
+  return check_launch("cross attention forward kernel");
+}
+
+template <int DP, bool KV>
+Error launch_backward(const Packed& a1, const Packed& a2, const Packed& b1, const Packed& b2, BwdDev& f,
+                      cudaStream_t stream) {
+  using S = BwdShape<DP>;
+  auto kern = cross_backward_kernel<DP, KV>;
+  allow_smem((const void*)kern, S::smem);
+  kern<<<(unsigned)(f.mtiles * f.c.B * f.c.Hk * f.splits), S::threads, S::smem, stream>>>(a1.map128, a2.map128, b1.mapKN,
+                                                                                       b2.mapKN, f);
+  return check_launch(KV ? "cross attention key gradient kernel" : "cross attention query gradient kernel");
+}
+
+Error run_sum(const CrossDev& c, const float* part, const HeadsDev& out, int splits, int rows_p, int DP, int G, int T,
+              const int* nonfinite, cudaStream_t stream) {
+  SumDev s;
+  s.part = part;
+  s.out = out;
+  s.splits = splits;
+  s.np = c.B * c.Hk;
+  s.rows_p = rows_p;
+  s.ld = DP;
+  s.Hk = c.Hk;
+  s.G = G;
+  s.T = T;
+  s.f_T = make_fastdiv((uint32_t)T);
+  s.D = c.D;
+  s.n = (int64_t)s.np * G * T * (DP / 4);
+  s.nonfinite = nonfinite;
+  cross_sum_kernel<<<(unsigned)((s.n + 255) / 256), 256, 0, stream>>>(s);
+  return check_launch("cross attention sum kernel");
+}
+
+// Parts of a walk of `tiles` column tiles so that `ctas` CTAs fill the SMs;
+// every part walks two tiles at least.
+int pick_splits(int64_t ctas, int tiles) {
+  const int sms = current_device_info().sm_count;
+  int64_t s = ctas >= sms ? 1 : sms / ctas;
+  if (s > tiles / 2) s = tiles / 2;
+  return s < 1 ? 1 : (int)s;
+}
+
+}  // namespace
+
+Error cross_tc_forward(const CrossDev& c, int* nonfinite, cudaStream_t stream) {
+  Error e = too_large(c);
+  if (!e.ok()) return e;
+  EncodeTiled enc = encode_fn(&e);
+  if (!enc) return e;
+  const int DP = c.D <= 64 ? 64 : 128, KN = kTileElems / DP, np = c.B * c.Hk;
+  const int MT = c.M > 128 ? 2 : 1;
+  FwdDev f;
+  std::memset(static_cast<void*>(&f), 0, sizeof(f));
+  f.c = c;
+  f.mtiles = (c.M + MT * 128 - 1) / (MT * 128);
+  f.splits = pick_splits((int64_t)f.mtiles * np, (c.Tk + KN - 1) / KN);
+  Packed q, k, v;
+  Scratch buf;
+  for (int pass = 0; pass < 2; ++pass) {
+    Arena a;
+    if (pass) a.base = buf.as<char>();
+    place(a, q, np, c.M, DP, false);
+    place(a, k, np, c.Tk, DP, false);
+    place(a, v, np, c.Tk, DP, false);
+    if (f.splits > 1) {
+      const size_t rows = (size_t)f.splits * np * q.rows_p;
+      f.part = a.take<float>(rows * DP);
+      f.part_m = a.take<float>(rows);
+      f.part_l = a.take<float>(rows);
+    }
+    if (!pass) {
+      e = buf.alloc(a.used, stream);
+      if (!e.ok()) return e;
+    }
+  }
+  e = maps(enc, q, DP);
+  if (e.ok()) e = maps(enc, k, DP);
+  if (e.ok()) e = maps(enc, v, DP);
+  if (!e.ok()) return e;
+  PackDev p;
+  std::memset(static_cast<void*>(&p), 0, sizeof(p));
+  add_source(p, c, c.q, q, c.G, c.Tq, false, DP);
+  if (c.scale < 0.f) p.s[0].sign = -1.f;
+  add_source(p, c, c.k, k, 1, c.Tk, true, DP);
+  add_source(p, c, c.v, v, 1, c.Tk, true, DP);
+  e = run_pack(p, c, DP, nonfinite, stream);
+  if (!e.ok()) return e;
+  f.q = q.planes();
+  f.k = k.planes();
+  f.v = v.planes();
+  f.f = fabsf(c.scale) * kLog2e;
+  f.nonfinite = nonfinite;
+  f.err = async_error_word();
+  if (DP == 64) e = MT == 2 ? launch_forward<64, 2>(q, k, v, f, stream) : launch_forward<64, 1>(q, k, v, f, stream);
+  else e = MT == 2 ? launch_forward<128, 2>(q, k, v, f, stream) : launch_forward<128, 1>(q, k, v, f, stream);
+  if (!e.ok() || f.splits == 1) return e;
+  return cross_join(c, f.splits, q.rows_p, DP, f.part, f.part_m, f.part_l, stream);
+}
+
+Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) {
+  Error e = too_large(c);
+  if (!e.ok()) return e;
+  EncodeTiled enc = encode_fn(&e);
+  if (!enc) return e;
+  const int DP = c.D <= 64 ? 64 : 128, KN = kTileElems / DP, np = c.B * c.Hk;
+  BwdDev q_d, k_d;
+  std::memset(static_cast<void*>(&q_d), 0, sizeof(q_d));
+  q_d.c = c;
+  q_d.f = fabsf(c.scale) * kLog2e;
+  q_d.nonfinite = nonfinite;
+  q_d.err = async_error_word();
+  k_d = q_d;
+  q_d.mtiles = (c.M + 127) / 128;
+  q_d.splits = pick_splits((int64_t)q_d.mtiles * np, (c.Tk + KN - 1) / KN);
+  q_d.out_scale = c.scale;
+  k_d.mtiles = (c.Tk + 127) / 128;
+  k_d.splits = pick_splits((int64_t)k_d.mtiles * np, (c.M + KN - 1) / KN);
+  k_d.out_scale = fabsf(c.scale);
+  Packed q, k, v, g;
+  float *lse2 = nullptr, *delta = nullptr, *rnorm = nullptr, *dmax = nullptr;
+  Scratch buf;
+  for (int pass = 0; pass < 2; ++pass) {
+    Arena a;
+    if (pass) a.base = buf.as<char>();
+    place(a, q, np, c.M, DP, false);
+    place(a, g, np, c.M, DP, true);
+    place(a, k, np, c.Tk, DP, false);
+    place(a, v, np, c.Tk, DP, true);
+    lse2 = a.take<float>(q.rows_all);
+    delta = a.take<float>(q.rows_all);
+    rnorm = a.take<float>(q.rows_all);
+    dmax = a.take<float>(q.rows_all / KN);
+    if (q_d.splits > 1) q_d.part1 = a.take<float>((size_t)q_d.splits * q.rows_all * DP);
+    if (k_d.splits > 1) {
+      k_d.part1 = a.take<float>((size_t)k_d.splits * k.rows_all * DP);
+      k_d.part2 = a.take<float>((size_t)k_d.splits * k.rows_all * DP);
+    }
+    if (!pass) {
+      e = buf.alloc(a.used, stream);
+      if (!e.ok()) return e;
+    }
+  }
+  e = maps(enc, q, DP);
+  if (e.ok()) e = maps(enc, g, DP);
+  if (e.ok()) e = maps(enc, k, DP);
+  if (e.ok()) e = maps(enc, v, DP);
+  if (!e.ok()) return e;
+  PackDev p;
+  std::memset(static_cast<void*>(&p), 0, sizeof(p));
+  add_source(p, c, c.q, q, c.G, c.Tq, false, DP);
+  if (c.scale < 0.f) p.s[0].sign = -1.f;
+  add_source(p, c, c.k, k, 1, c.Tk, true, DP);
+  add_source(p, c, c.v, v, 1, c.Tk, true, DP);
+  add_source(p, c, c.dout, g, c.G, c.Tq, false, DP);
+  PackSrc& gs = p.s[3];
+  gs.grad = 1;
+  gs.out = c.out;
+  gs.lse2 = lse2;
+  gs.delta = delta;
+  gs.rnorm = rnorm;
+  gs.dmax = dmax;
+  e = run_pack(p, c, DP, nonfinite, stream);
+  if (!e.ok()) return e;
+  for (BwdDev* x : {&q_d, &k_d}) {
+    x->lse2 = lse2;
+    x->delta = delta;
+    x->rnorm = rnorm;
+    x->dmax = dmax;
+  }
+  q_d.a1 = q.planes();
+  q_d.a2 = g.planes();
+  q_d.b1 = k.planes();
+  q_d.b2 = v.planes();
+  k_d.a1 = k.planes();
+  k_d.a2 = v.planes();
+  k_d.b1 = q.planes();
+  k_d.b2 = g.planes();
+  e = DP == 64 ? launch_backward<64, false>(q, g, k, v, q_d, stream) : launch_backward<128, false>(q, g, k, v, q_d, stream);
+  if (!e.ok()) return e;
+  e = DP == 64 ? launch_backward<64, true>(k, v, q, g, k_d, stream) : launch_backward<128, true>(k, v, q, g, k_d, stream);
+  if (!e.ok()) return e;
+  if (q_d.splits > 1) {
+    e = run_sum(c, q_d.part1, c.dq, q_d.splits, q.rows_p, DP, c.G, c.Tq, nonfinite, stream);
+    if (!e.ok()) return e;
+  }
+  if (k_d.splits > 1) {
+    e = run_sum(c, k_d.part1, c.dk, k_d.splits, k.rows_p, DP, 1, c.Tk, nonfinite, stream);
+    if (e.ok()) e = run_sum(c, k_d.part2, c.dv, k_d.splits, k.rows_p, DP, 1, c.Tk, nonfinite, stream);
+  }
+  return e;
+}
+
+}  // namespace trs

@@ -47,6 +47,7 @@
 #include <string>
 
 #include "kernels.cuh"
+#include "tcgen05.cuh"
 #include "tma.cuh"
 
 namespace trs {
@@ -194,20 +195,7 @@ __global__ void __launch_bounds__(256) zero_view_kernel(const trs_view v, int64_
   }
 }
 
-// ---- tcgen05 / TMA primitives ---------------------------------------------------
-
-__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// ---- tcgen05 / TMA primitives (the rest in tcgen05.cuh) -------------------------
 
 // D[tmem] (+)= A[smem, K-major] * B[smem, K-major]^T, M 128, N 128, K 8 (tf32).
 __device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
@@ -243,12 +231,6 @@ __device__ __forceinline__ void umma_tf32_lastuse(uint32_t tmem_d, uint64_t da, 
       : "memory");
 }
 
-// Arrives on `bar` once every tcgen05.mma this thread issued before has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-
 // 32 consecutive accumulator columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -261,16 +243,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-
-// Shared-memory matrix descriptor of a K-major tile with 128-byte swizzle:
-// rows of 128 bytes, 8-row groups 1024 bytes apart (SBO), leading offset
-// unused (1), descriptor version 1, layout SWIZZLE_128B (2); the tile starts
-// on a 1024-byte boundary, so the base offset is 0.
-__device__ __forceinline__ uint64_t sw128_desc(const void* tile) {
-  const uint64_t a = (uint64_t)(smem_u32(tile) >> 4) & 0x3FFFull;
-  return a | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
 
 struct TcDev {
   int64_t M, N, Kp, Mp, Np;

@@ -283,6 +283,23 @@ def head_norm_rotary_backward(grad_q_out: abi.View, grad_k_out: abi.View | None,
           _out(grad_q), _out(grad_k), _out(grad_q_gamma), _out(grad_k_gamma), stream_handle())
 
 
+def cross_attention(q: abi.View, k: abi.View, v: abi.View, scale: float, out: torch.Tensor,
+                    lse: torch.Tensor | None = None, key_lengths: abi.View | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v per head: q [B, Tq, Hq, D], k and v [B, Tk, Hk, D], keys of batch b up to
+    key_lengths[b]; lse [B, Hq, Tq] is what the backward needs."""
+    _call("trs_cross_attention", _ref(q), _ref(k), _ref(v), _ref(key_lengths), float(scale), _out(out), _out(lse),
+          stream_handle())
+    return out
+
+
+def cross_attention_backward(grad_out: abi.View, q: abi.View, k: abi.View, v: abi.View, out: abi.View, lse: abi.View,
+                             scale: float, grad_q: torch.Tensor, grad_k: torch.Tensor, grad_v: torch.Tensor,
+                             key_lengths: abi.View | None = None) -> None:
+    """The gradients of cross_attention for q, k and v."""
+    _call("trs_cross_attention_backward", _ref(grad_out), _ref(q), _ref(k), _ref(v), _ref(key_lengths), _ref(out),
+          _ref(lse), float(scale), _out(grad_q), _out(grad_k), _out(grad_v), stream_handle())
+
+
 def fill_uniform(out: torch.Tensor, seed: int, lo: float = -1.0, hi: float = 1.0, first: int = 0) -> torch.Tensor:
     _call("trs_fill_uniform", ctypes.byref(view_of(out)), seed, first, lo, hi, stream_handle())
     return out
