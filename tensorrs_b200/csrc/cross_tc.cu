@@ -251,28 +251,26 @@ constexpr uint32_t idesc_f16(int n, bool mn) {
 }
 
 // D = A B^T over DP: A 128 rows, B KN rows, both in shared memory (planes as
-// load_planes leaves them); the two small products first.
+// load_planes leaves them); the two small products first.  The loops stay
+// loops: the issuing warp runs with few registers.
 template <int DP, int KN>
 __device__ __forceinline__ void mma_abt(uint32_t dst, const unsigned char* a, const unsigned char* b) {
   constexpr uint32_t id = idesc_f16(KN, false);
-  constexpr int HA = 128 * 128, HB = KN * 128, NH = DP / 64;
-  uint32_t acc = 0;
-#pragma unroll
+  constexpr int HA = 128 * 128 / 16, HB = KN * 128 / 16, NH = DP / 64;
+  const uint32_t a0 = sw128_low(a), b0 = sw128_low(b);
+#pragma unroll 1
   for (int h = 0; h < NH; ++h) {
-    const uint64_t ah = sw128_desc(a + h * HA), al = sw128_desc(a + (NH + h) * HA);
-    const uint64_t bh = sw128_desc(b + h * HB), bl = sw128_desc(b + (NH + h) * HB);
+    const uint32_t ah = a0 + h * HA, bh = b0 + h * HB;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      umma_f16_ss(dst, al + 2 * k, bh + 2 * k, id, acc);
-      acc = 1;
-      umma_f16_ss(dst, ah + 2 * k, bl + 2 * k, id, 1);
+      umma_f16_ss(dst, ah + NH * HA + 2 * k, bh + 2 * k, id, h + k);
+      umma_f16_ss(dst, ah + 2 * k, bh + NH * HB + 2 * k, id, 1);
     }
   }
-#pragma unroll
+#pragma unroll 1
   for (int h = 0; h < NH; ++h) {
-    const uint64_t ah = sw128_desc(a + h * HA), bh = sw128_desc(b + h * HB);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) umma_f16_ss(dst, ah + 2 * k, bh + 2 * k, id, 1);
+    for (int k = 0; k < 4; ++k) umma_f16_ss(dst, a0 + h * HA + 2 * k, b0 + h * HB + 2 * k, id, 1);
   }
 }
 
@@ -282,17 +280,20 @@ template <int DP, int KN>
 __device__ __forceinline__ void mma_ab(uint32_t dst, uint32_t a, const unsigned char* b) {
   constexpr uint32_t id = idesc_f16(DP, true);
   constexpr int HB = KN * 128, NH = DP / 64;
-  const uint64_t bh = sw128_mn_desc(b, HB), bl = sw128_mn_desc(b + NH * HB, HB);
-  uint32_t acc = 0;
+  const uint32_t b0 = sw128_low(b, HB);
+#pragma unroll 1
+  for (int c = 0; c < KN / 32; ++c) {
 #pragma unroll
-  for (int k = 0; k < KN / 16; ++k) {
-    const uint32_t ak = a + 32 * (k / 2) + 8 * (k % 2);
-    umma_f16_ts(dst, ak + 16, bh + 128 * k, id, acc);
-    acc = 1;
-    umma_f16_ts(dst, ak, bl + 128 * k, id, 1);
+    for (int k = 0; k < 2; ++k) {
+      umma_f16_ts(dst, a + 32 * c + 8 * k + 16, b0 + 256 * c + 128 * k, id, c + k);
+      umma_f16_ts(dst, a + 32 * c + 8 * k, b0 + NH * HB / 16 + 256 * c + 128 * k, id, 1);
+    }
   }
+#pragma unroll 1
+  for (int c = 0; c < KN / 32; ++c) {
 #pragma unroll
-  for (int k = 0; k < KN / 16; ++k) umma_f16_ts(dst, a + 32 * (k / 2) + 8 * (k % 2), bh + 128 * k, id, 1);
+    for (int k = 0; k < 2; ++k) umma_f16_ts(dst, a + 32 * c + 8 * k, b0 + 256 * c + 128 * k, id, 1);
+  }
 }
 
 // The two planes of two values below 2^16: hi = the value cut to 11 bits, lo =
@@ -305,6 +306,31 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
   *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // What a CTA still has in flight when it gave up: its copies (the slots'
 // latest phases) and its MMAs.
 __device__ __forceinline__ void drain(uint64_t* full, int slots, int issued) {
@@ -313,6 +339,12 @@ __device__ __forceinline__ void drain(uint64_t* full, int slots, int issued) {
     mbar_wait(&full[s], (uint32_t)last & 1u);
   }
 }
+
+// A launch of 384 threads holds 168 registers each; the warpgroup of the MMA
+// and TMA warps gives up all but 56 and the two others take 224
+// (128 * 56 + 256 * 224 = 384 * 168).
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
 
 // ---- forward ---------------------------------------------------------------------
 
@@ -334,11 +366,11 @@ struct FwdShape {
   static constexpr int smem = q_bytes + slots * kSlot + 1024 + 512;
   static constexpr int OB = DP == 64 ? 2 : 1;       // output accumulators per row tile
   static constexpr int cols = KN + OB * DP;         // tensor-memory columns per row tile
-  static constexpr int threads = MT * 128 + 64;
+  static constexpr int threads = MT * 128 + 128;    // row tiles' warpgroups, then MMA and TMA warps (two idle)
 };
 
 template <int DP, int MT>
-__global__ void __launch_bounds__(MT * 128 + 64, 1)
+__global__ void __launch_bounds__(MT * 128 + 128, 1)
 cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ FwdDev d) {
   using S = FwdShape<DP, MT>;
@@ -397,10 +429,11 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   const int all = (len + KN - 1) / KN, per = (all + d.splits - 1) / d.splits;
   const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;  // this CTA's key tiles
 
-  if (warp == MT * 4 + 1) {
-    if (lane == 0 && n > 0) {  // TMA
+  if (warp >= MT * 4) {
+    if (MT == 2) give_registers();
+    if (warp == MT * 4 + 1 && lane == 0 && n > 0) {  // TMA
       mbar_arrive_expect_tx(qfull, S::q_bytes);
-#pragma unroll
+#pragma unroll 1
       for (int t = 0; t < MT; ++t)
         load_planes<DP, 128>(sq + t * 128 * DP * 4, &mq, d.q, pr * d.q.rows_p + (mtile * MT + t) * 128, qfull);
       int i = 0;
@@ -417,12 +450,11 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         drain(full, NS, i);
       }
     }
-  } else if (warp == MT * 4) {
-    if (lane == 0 && n > 0) {  // MMA
+    if (warp == MT * 4 && lane == 0 && n > 0) {  // MMA
       bool ok = wait_or_fail(qfull, 0, failed) && wait_or_fail(&full[0], 0, failed);
       if (ok) {
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < MT; ++t) {
           mma_abt<DP, KN>(tmem + t * S::cols, sq + t * 128 * DP * 4, ring);
           umma_commit(&s_full[t]);
@@ -431,7 +463,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       }
       for (int j = 0; j < n && ok; ++j) {
         const int iv = 2 * j + 1, ik = 2 * j + 2, ob = j % OB;
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < MT; ++t) {
           ok = ok && wait_or_fail(&p_ready[t], (uint32_t)j & 1u, failed) &&
                (t > 0 || wait_or_fail(&full[iv % NS], (uint32_t)(iv / NS) & 1u, failed)) &&
@@ -457,6 +489,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       }
     }
   } else {  // softmax: one thread per row
+    if (MT == 2) take_registers();
     const int t = warp / 4;
     const int rl = (warp % 4) * 32 + lane, row = (mtile * MT + t) * 128 + rl;
     const uint32_t sbase = tmem + ((uint32_t)((warp % 4) * 32) << 16) + t * S::cols, obase = sbase + KN;
@@ -475,69 +508,71 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       const bool here = wait_or_fail(&o_full[t * OB + ob], (uint32_t)(j / OB) & 1u, failed);
       if (!__all_sync(0xffffffffu, here)) return false;
       tc_fence_after();
-      const float fv = vinv[j];
+      const uint64_t fv2 = pack2(vinv[j], vinv[j]), keep2 = pack2(keep, keep);
 #pragma unroll
       for (int cc = 0; cc < DP / 32; ++cc) {
         uint32_t o[32];
         tmem_ld32_issue(obase + ob * DP + cc * 32, o);
         tmem_ld_done(o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[cc * 32 + i] = __fmaf_rn(__uint_as_float(o[i]), fv, acc[cc * 32 + i] * keep);
+        for (int i = 0; i < 32; i += 2) {
+          uint64_t a2 = mul2(pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1]), keep2);
+          a2 = fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), fv2, a2);
+          unpack2(a2, &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
+        }
       }
       tc_fence_before();
       mbar_arrive(&o_free[t * OB + ob]);
       return true;
     };
     for (int j = 0; j < n; ++j) {
-      const float f = fq * kinv[j];
+      const float f = fmaxf(fq * kinv[j], 0x1p-126f);  // not 0: -inf stands for an absent key below
       const int limit = len - (j0 + j) * KN;  // keys of this tile
       ok = wait_or_fail(&s_full[t], (uint32_t)j & 1u, failed);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
-      float mx = -INFINITY;
+      uint32_t x[KN / 32][32];  // the row of S, then of P
 #pragma unroll
-      for (int cc = 0; cc < KN / 64; ++cc) {
-        uint32_t a[32], e[32];
-        tmem_ld32_issue(sbase + cc * 64, a);
-        tmem_ld32_issue(sbase + cc * 64 + 32, e);
-        tmem_ld_done(a);
-        tmem_ld_tie(e);
-        if (limit >= (cc + 1) * 64) {
+      for (int cc = 0; cc < KN / 32; ++cc) tmem_ld32_issue(sbase + cc * 32, x[cc]);
+      tmem_ld_done(x[0]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(a[i]), __uint_as_float(e[i])));
-        } else {
+      for (int cc = 1; cc < KN / 32; ++cc) tmem_ld_tie(x[cc]);
+      if (limit < KN) {  // behind the last key: no weight
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (cc * 64 + i < limit) mx = fmaxf(mx, __uint_as_float(a[i]));
-            if (cc * 64 + 32 + i < limit) mx = fmaxf(mx, __uint_as_float(e[i]));
-          }
-        }
+        for (int cc = 0; cc < KN / 32; ++cc)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (cc * 32 + i >= limit) x[cc][i] = 0xff800000u;
       }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int cc = 0; cc < KN / 32; ++cc)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+          mx4[i / 2 % 4] = fmaxf(fmaxf(mx4[i / 2 % 4], __uint_as_float(x[cc][i])), __uint_as_float(x[cc][i + 1]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       const float mn = fmaxf(m, mx * f);
       const float alpha = ex2(m - mn);
       const float bias = 15.f - mn;
       m = mn;
-      float sum0 = 0.f, sum1 = 0.f;
+      const uint64_t f2 = pack2(f, f), b2 = pack2(bias, bias);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int cc = 0; cc < KN / 32; ++cc) {
-        uint32_t a[32], w[32];
-        tmem_ld32_issue(sbase + cc * 32, a);
-        tmem_ld_done(a);
-        const bool part = limit < (cc + 1) * 32;
+        uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float p0 = ex2(__fmaf_rn(__uint_as_float(a[2 * i]), f, bias));
-          float p1 = ex2(__fmaf_rn(__uint_as_float(a[2 * i + 1]), f, bias));
-          if (part) {
-            if (cc * 32 + 2 * i >= limit) p0 = 0.f;
-            if (cc * 32 + 2 * i + 1 >= limit) p1 = 0.f;
-          }
-          sum0 += p0;
-          sum1 += p1;
+          float p0, p1;
+          unpack2(fma2(pack2(__uint_as_float(x[cc][2 * i]), __uint_as_float(x[cc][2 * i + 1])), f2, b2), &p0, &p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
           split2(p0, p1, &w[i], &w[16 + i]);
         }
         tmem_st32(sbase + cc * 32, w);
       }
+      float sum0, sum1;
+      unpack2(add2(sum[0], sum[1]), &sum0, &sum1);
       l = __fmaf_rn(l, alpha, sum0 + sum1);
       tmem_st_done();
       tc_fence_before();
@@ -602,11 +637,11 @@ struct BwdShape {
   static constexpr int a_bytes = 128 * DP * 4;
   static constexpr int n1 = DP == 64 ? 3 : 2, n2 = DP == 64 ? 2 : 1;
   static constexpr int smem = 2 * a_bytes + (n1 + n2) * kSlot + 1024 + 512;
-  static constexpr int threads = 320;
+  static constexpr int threads = 384;
 };
 
 template <int DP, bool KV>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(384, 1)
 cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_constant__ CUtensorMap ma2,
                       const __grid_constant__ CUtensorMap mb1, const __grid_constant__ CUtensorMap mb2,
                       const __grid_constant__ BwdDev d) {
@@ -682,8 +717,9 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   const int per = (all + d.splits - 1) / d.splits;
   const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;
 
-  if (warp == 9) {
-    if (lane == 0 && n > 0) {  // TMA
+  if (warp >= 8) {
+    give_registers();
+    if (warp == 9 && lane == 0 && n > 0) {  // TMA
       mbar_arrive_expect_tx(afull, 2 * S::a_bytes);
       load_planes<DP, 128>(sa1, &ma1, d.a1, pr * d.a1.rows_p + mtile * 128, afull);
       load_planes<DP, 128>(sa2, &ma2, d.a2, pr * d.a2.rows_p + mtile * 128, afull);
@@ -706,8 +742,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         drain(full2, N2, i2);
       }
     }
-  } else if (warp == 8) {
-    if (lane == 0 && n > 0) {  // MMA
+    if (warp == 8 && lane == 0 && n > 0) {  // MMA
       auto s_mma = [&](int j) {
         if (!wait_or_fail(&full1[j % N1], (uint32_t)(j / N1) & 1u, failed)) return false;
         tc_fence_after();
@@ -748,6 +783,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       }
     }
   } else {
+    take_registers();
     const int wg = warp / 4;
     const int row = mtile * 128 + (warp % 4) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;

@@ -38,31 +38,36 @@ __device__ __forceinline__ uint64_t sw128_desc(const void* tile) {
   return a | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// The same for a tile whose rows are the contraction and whose columns are
-// contiguous (MN-major, 128-byte swizzle): rows of 64 16-bit elements, 8-row
-// groups 1024 bytes apart (SBO); `block` bytes between blocks of 64 columns
-// (LBO).
-__device__ __forceinline__ uint64_t sw128_mn_desc(const void* tile, uint32_t block) {
-  const uint64_t a = (uint64_t)(smem_u32(tile) >> 4) & 0x3FFFull;
-  return a | ((uint64_t)(block >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// The same descriptor as its low word (start address, leading offset) and a
+// constant high word, which keeps it to one register: SW128 tiles of 128-byte
+// rows, 8-row groups 1024 bytes apart.  `block` is the leading offset in bytes:
+// unused (16) for a K-major tile; for a tile whose rows are the contraction
+// and whose columns are contiguous (MN-major), the distance between blocks of
+// 64 16-bit columns.
+constexpr uint32_t kSw128High = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t sw128_low(const void* tile, uint32_t block = 16) {
+  return ((smem_u32(tile) >> 4) & 0x3FFFu) | ((block >> 4) << 16);
 }
 
 // D[tmem] (+)= A * B, M 128, K 16, fp16 inputs, f32 accumulator: A from shared
 // memory or from tensor memory (two elements per 32-bit column).
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kSw128High), "r"(0u)
       : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kSw128High), "r"(0u)
       : "memory");
 }
 
