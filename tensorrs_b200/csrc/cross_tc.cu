@@ -251,50 +251,41 @@ constexpr uint32_t idesc_f16(int n, bool mn) {
 }
 
 // D = A B^T over DP: A 128 rows, B KN rows, both in shared memory (planes as
-// load_planes leaves them); the two small products first.  The loops stay
-// loops: the issuing warp runs with few registers.
+// load_planes leaves them); the two small products first.
 template <int DP, int KN>
-__device__ __forceinline__ void mma_abt(uint32_t dst, const unsigned char* a, const unsigned char* b) {
+__device__ __forceinline__ void mma_abt(uint32_t lead, uint32_t dst, uint32_t a, uint32_t b) {
   constexpr uint32_t id = idesc_f16(KN, false);
   constexpr int HA = 128 * 128 / 16, HB = KN * 128 / 16, NH = DP / 64;
-  const uint32_t a0 = sw128_low(a), b0 = sw128_low(b);
-#pragma unroll 1
-  for (int h = 0; h < NH; ++h) {
-    const uint32_t ah = a0 + h * HA, bh = b0 + h * HB;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      umma_f16_ss(dst, ah + NH * HA + 2 * k, bh + 2 * k, id, h + k);
-      umma_f16_ss(dst, ah + 2 * k, bh + NH * HB + 2 * k, id, 1);
-    }
+  for (int k = 0; k < 4 * NH; ++k) {
+    const int ka = k / 4 * HA + k % 4 * 2, kb = k / 4 * HB + k % 4 * 2;
+    umma_f16_ss<id>(lead, dst, a + NH * HA + ka, b + kb, k > 0);
+    umma_f16_ss<id>(lead, dst, a + ka, b + NH * HB + kb, 1);
   }
-#pragma unroll 1
-  for (int h = 0; h < NH; ++h) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) umma_f16_ss(dst, a0 + h * HA + 2 * k, b0 + h * HB + 2 * k, id, 1);
-  }
+  for (int k = 0; k < 4 * NH; ++k)
+    umma_f16_ss<id>(lead, dst, a + k / 4 * HA + k % 4 * 2, b + k / 4 * HB + k % 4 * 2, 1);
 }
 
 // D = A B over KN: A 128 x KN in tensor memory (chunks of 32 columns: 16
 // columns of hi, 16 of lo), B KN rows of DP columns in shared memory.
 template <int DP, int KN>
-__device__ __forceinline__ void mma_ab(uint32_t dst, uint32_t a, const unsigned char* b) {
+__device__ __forceinline__ void mma_ab(uint32_t lead, uint32_t dst, uint32_t a, uint32_t b) {
   constexpr uint32_t id = idesc_f16(DP, true);
-  constexpr int HB = KN * 128, NH = DP / 64;
-  const uint32_t b0 = sw128_low(b, HB);
-#pragma unroll 1
-  for (int c = 0; c < KN / 32; ++c) {
+  constexpr int LO = DP / 64 * KN * 128 / 16;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      umma_f16_ts(dst, a + 32 * c + 8 * k + 16, b0 + 256 * c + 128 * k, id, c + k);
-      umma_f16_ts(dst, a + 32 * c + 8 * k, b0 + NH * HB / 16 + 256 * c + 128 * k, id, 1);
-    }
+  for (int k = 0; k < KN / 16; ++k) {
+    const uint32_t ak = a + 32 * (k / 2) + 8 * (k % 2);
+    umma_f16_ts<id>(lead, dst, ak + 16, b + 128 * k, k > 0);
+    umma_f16_ts<id>(lead, dst, ak, b + LO + 128 * k, 1);
   }
-#pragma unroll 1
-  for (int c = 0; c < KN / 32; ++c) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) umma_f16_ts(dst, a + 32 * c + 8 * k, b0 + 256 * c + 128 * k, id, 1);
-  }
+  for (int k = 0; k < KN / 16; ++k) umma_f16_ts<id>(lead, dst, a + 32 * (k / 2) + 8 * (k % 2), b + 128 * k, 1);
 }
+// The descriptors' low words of the operands above.
+__device__ __forceinline__ uint32_t rows_desc(const unsigned char* tile) { return sw128_low(tile); }
+template <int KN>
+__device__ __forceinline__ uint32_t cols_desc(const unsigned char* tile) { return sw128_low(tile, KN * 128); }
 
 // The two planes of two values below 2^16: hi = the value cut to 11 bits, lo =
 // the rest (exact) rounded to 11.
@@ -340,11 +331,17 @@ __device__ __forceinline__ void drain(uint64_t* full, int slots, int issued) {
   }
 }
 
-// A launch of 384 threads holds 168 registers each; the warpgroup of the MMA
-// and TMA warps gives up all but 56 and the two others take 224
-// (128 * 56 + 256 * 224 = 384 * 168).
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+// A launch of 384 threads holds 168 registers each.  The warpgroup of the MMA
+// and TMA warps gives up all but LEAN and the two others take FULL, with
+// 128 LEAN + 256 FULL = 384 * 168: (56, 224) where a thread holds a row of
+// results and of scores, (88, 208) where half a row is enough.
+template <int LEAN>
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LEAN)); }
+template <int LEAN>
+__device__ __forceinline__ void take_registers() {
+  static_assert((384 * 168 - 128 * LEAN) % 256 == 0, "all of the registers");
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"((384 * 168 - 128 * LEAN) / 256));
+}
 
 // ---- forward ---------------------------------------------------------------------
 
@@ -430,7 +427,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;  // this CTA's key tiles
 
   if (warp >= MT * 4) {
-    if (MT == 2) give_registers();
+    if (MT == 2) give_registers<56>();
     if (warp == MT * 4 + 1 && lane == 0 && n > 0) {  // TMA
       mbar_arrive_expect_tx(qfull, S::q_bytes);
 #pragma unroll 1
@@ -450,46 +447,53 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         drain(full, NS, i);
       }
     }
-    if (warp == MT * 4 && lane == 0 && n > 0) {  // MMA
+    if (warp == MT * 4 && n > 0) {  // MMA: the warp stays whole, one lane issues
+      const uint32_t lead = elect_lane(), tm = uniform(tmem);
+      const uint32_t dq = uniform(rows_desc(sq)), dk = uniform(rows_desc(ring)), dv = uniform(cols_desc<KN>(ring));
+      constexpr uint32_t QT = 128 * DP * 4 / 16, SLOT = kSlot / 16;  // a row tile, a slot, in descriptor units
       bool ok = wait_or_fail(qfull, 0, failed) && wait_or_fail(&full[0], 0, failed);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
 #pragma unroll 1
         for (int t = 0; t < MT; ++t) {
-          mma_abt<DP, KN>(tmem + t * S::cols, sq + t * 128 * DP * 4, ring);
-          umma_commit(&s_full[t]);
+          mma_abt<DP, KN>(lead, tm + t * S::cols, dq + t * QT, dk);
+          umma_commit(lead, &s_full[t]);
         }
-        umma_commit(&empty[0]);
+        umma_commit(lead, &empty[0]);
       }
       for (int j = 0; j < n && ok; ++j) {
         const int iv = 2 * j + 1, ik = 2 * j + 2, ob = j % OB;
 #pragma unroll 1
         for (int t = 0; t < MT; ++t) {
-          ok = ok && wait_or_fail(&p_ready[t], (uint32_t)j & 1u, failed) &&
+          ok = wait_or_fail(&p_ready[t], (uint32_t)j & 1u, failed) &&
                (t > 0 || wait_or_fail(&full[iv % NS], (uint32_t)(iv / NS) & 1u, failed)) &&
                (j < OB || wait_or_fail(&o_free[t * OB + ob], (uint32_t)(j / OB - 1) & 1u, failed));
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          mma_ab<DP, KN>(tmem + t * S::cols + KN + ob * DP, tmem + t * S::cols, ring + (iv % NS) * kSlot);
-          umma_commit(&o_full[t * OB + ob]);
-          if (t == MT - 1) umma_commit(&empty[iv % NS]);
+          mma_ab<DP, KN>(lead, tm + t * S::cols + KN + ob * DP, tm + t * S::cols, dv + iv % NS * SLOT);
+          umma_commit(lead, &o_full[t * OB + ob]);
+          if (t == MT - 1) umma_commit(lead, &empty[iv % NS]);
           if (j + 1 < n) {
-            ok = t > 0 || wait_or_fail(&full[ik % NS], (uint32_t)(ik / NS) & 1u, failed);
-            if (!ok) break;
-            tc_fence_after();
-            mma_abt<DP, KN>(tmem + t * S::cols, sq + t * 128 * DP * 4, ring + (ik % NS) * kSlot);
-            umma_commit(&s_full[t]);
-            if (t == MT - 1) umma_commit(&empty[ik % NS]);
+            if (t == 0) {
+              ok = __all_sync(0xffffffffu, wait_or_fail(&full[ik % NS], (uint32_t)(ik / NS) & 1u, failed));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            mma_abt<DP, KN>(lead, tm + t * S::cols, dq + t * QT, dk + ik % NS * SLOT);
+            umma_commit(lead, &s_full[t]);
+            if (t == MT - 1) umma_commit(lead, &empty[ik % NS]);
           }
         }
       }
       if (!ok) {
-        umma_commit(done);
+        umma_commit(lead, done);
         mbar_wait(done, 0);
       }
     }
   } else {  // softmax: one thread per row
-    if (MT == 2) take_registers();
+    if (MT == 2) take_registers<56>();
     const int t = warp / 4;
     const int rl = (warp % 4) * 32 + lane, row = (mtile * MT + t) * 128 + rl;
     const uint32_t sbase = tmem + ((uint32_t)((warp % 4) * 32) << 16) + t * S::cols, obase = sbase + KN;
@@ -718,7 +722,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;
 
   if (warp >= 8) {
-    give_registers();
+    give_registers<KV ? 56 : 88>();
     if (warp == 9 && lane == 0 && n > 0) {  // TMA
       mbar_arrive_expect_tx(afull, 2 * S::a_bytes);
       load_planes<DP, 128>(sa1, &ma1, d.a1, pr * d.a1.rows_p + mtile * 128, afull);
@@ -742,48 +746,55 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         drain(full2, N2, i2);
       }
     }
-    if (warp == 8 && lane == 0 && n > 0) {  // MMA
+    if (warp == 8 && n > 0) {  // MMA: the warp stays whole, one lane issues
+      const uint32_t lead = elect_lane(), tm = uniform(tmem);
+      const uint32_t d1 = uniform(rows_desc(sa1)), d2 = uniform(rows_desc(sa2));
+      const uint32_t r1 = uniform(rows_desc(ring1)), r2 = uniform(rows_desc(ring2));
+      const uint32_t c1 = uniform(cols_desc<KN>(ring1)), c2 = uniform(cols_desc<KN>(ring2));
+      constexpr uint32_t SLOT = kSlot / 16;
+      const uint32_t dpc = tm + 2 * KN, rc1 = tm + 3 * KN, rc2 = rc1 + DP;
+      auto all_ok = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
       auto s_mma = [&](int j) {
-        if (!wait_or_fail(&full1[j % N1], (uint32_t)(j / N1) & 1u, failed)) return false;
+        if (!all_ok(wait_or_fail(&full1[j % N1], (uint32_t)(j / N1) & 1u, failed))) return false;
         tc_fence_after();
-        mma_abt<DP, KN>(tmem + (j & 1) * KN, sa1, ring1 + (j % N1) * kSlot);
-        umma_commit(&s_full[j & 1]);
+        mma_abt<DP, KN>(lead, tm + (j & 1) * KN, d1, r1 + j % N1 * SLOT);
+        umma_commit(lead, &s_full[j & 1]);
         return true;
       };
       auto dp_mma = [&](int j) {
-        if (!wait_or_fail(&full2[j % N2], (uint32_t)(j / N2) & 1u, failed)) return false;
+        if (!all_ok(wait_or_fail(&full2[j % N2], (uint32_t)(j / N2) & 1u, failed))) return false;
         tc_fence_after();
-        mma_abt<DP, KN>(t_dp, sa2, ring2 + (j % N2) * kSlot);
-        umma_commit(dp_full);
-        if (!KV) umma_commit(&empty2[j % N2]);
+        mma_abt<DP, KN>(lead, dpc, d2, r2 + j % N2 * SLOT);
+        umma_commit(lead, dp_full);
+        if (!KV) umma_commit(lead, &empty2[j % N2]);
         return true;
       };
-      bool ok = wait_or_fail(afull, 0, failed) && s_mma(0) && dp_mma(0);
+      bool ok = all_ok(wait_or_fail(afull, 0, failed)) && s_mma(0) && dp_mma(0);
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t ph = (uint32_t)j & 1u;
         if (KV) {
-          ok = wait_or_fail(p_ready, ph, failed) && (j == 0 || wait_or_fail(r_free, ph ^ 1u, failed));
+          ok = all_ok(wait_or_fail(p_ready, ph, failed) && (j == 0 || wait_or_fail(r_free, ph ^ 1u, failed)));
           if (!ok) break;
           tc_fence_after();
-          mma_ab<DP, KN>(t_r2, tmem + (j & 1) * KN, ring2 + (j % N2) * kSlot);  // P^T dout
-          umma_commit(&empty2[j % N2]);
+          mma_ab<DP, KN>(lead, rc2, tm + (j & 1) * KN, c2 + j % N2 * SLOT);  // P^T dout
+          umma_commit(lead, &empty2[j % N2]);
         }
         if (j + 1 < n && !(ok = s_mma(j + 1))) break;
-        ok = wait_or_fail(ds_ready, ph, failed) && (KV || j == 0 || wait_or_fail(r_free, ph ^ 1u, failed));
+        ok = all_ok(wait_or_fail(ds_ready, ph, failed) && (KV || j == 0 || wait_or_fail(r_free, ph ^ 1u, failed)));
         if (!ok) break;
         tc_fence_after();
-        mma_ab<DP, KN>(t_r1, t_dp, ring1 + (j % N1) * kSlot);  // dS k, or dS^T q
-        umma_commit(&empty1[j % N1]);
-        umma_commit(r_full);
+        mma_ab<DP, KN>(lead, rc1, dpc, c1 + j % N1 * SLOT);  // dS k, or dS^T q
+        umma_commit(lead, &empty1[j % N1]);
+        umma_commit(lead, r_full);
         if (j + 1 < n) ok = dp_mma(j + 1);
       }
       if (!ok) {
-        umma_commit(done);
+        umma_commit(lead, done);
         mbar_wait(done, 0);
       }
     }
   } else {
-    take_registers();
+    take_registers<KV ? 56 : 88>();
     const int wg = warp / 4;
     const int row = mtile * 128 + (warp % 4) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;

@@ -49,25 +49,54 @@ __device__ __forceinline__ uint32_t sw128_low(const void* tile, uint32_t block =
   return ((smem_u32(tile) >> 4) & 0x3FFFu) | ((block >> 4) << 16);
 }
 
-// D[tmem] (+)= A * B, M 128, K 16, fp16 inputs, f32 accumulator: A from shared
-// memory or from tensor memory (two elements per 32-bit column).
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+// One lane of the converged warp.  The whole warp walks the loops of an MMA
+// warp, so that addresses stay in uniform registers, and the elected lane
+// alone issues (the MMAs of a divergent single thread issue at a third of the
+// rate: each operand has to be moved to a uniform register first).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+// A value that is the same in every lane, as the compiler can see.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// D[tmem] (+)= A * B, M 128, K 16, fp16 inputs, f32 accumulator, issued by the
+// lane with lead != 0: A from shared memory or from tensor memory (two
+// elements per 32-bit column).
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_f16_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
       "mov.b64 da, {%1, %5};\n\t"
       "mov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kSw128High), "r"(0u)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "n"(IDESC), "r"(acc), "n"(kSw128High), "r"(0u), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_f16_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
       "mov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kSw128High), "r"(0u)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "n"(IDESC), "r"(acc), "n"(kSw128High), "r"(0u), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
       : "memory");
 }
 
