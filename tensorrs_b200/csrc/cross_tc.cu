@@ -73,12 +73,12 @@ struct PackSrc {
   float* norm;           // [problem][tile] largest row 2-norm, in units of 2^e; or null
   float sign;
   int vec;
-  // the output gradient's tiles also carry, per row: lse in units of log2 (+inf
-  // behind the last row), delta, the row's norm in units of 2^e; per tile the
-  // largest |delta|
+  // the output gradient's tiles also carry, per row: 15 - lse in units of log2
+  // (-inf behind the last row: no weight), delta, the row's norm in units of
+  // 2^e; per tile the largest |delta|
   int grad;
   HeadsDev out;
-  float *lse2, *delta, *rnorm, *dmax;
+  float *bias, *delta, *rnorm, *dmax;
   FastDiv f_T;
 };
 struct PackDev {
@@ -192,12 +192,12 @@ __global__ void __launch_bounds__(256) cross_pack_kernel(const __grid_constant__
         dm = fmaxf(dm, fabsf(dlt));
         if (lane == 0) {
           const int64_t at_r = (int64_t)pr * s.rows_p + row;
-          float ls = INFINITY;
+          float ls = -INFINITY;
           if (row < n) {
             const int g = (int)fdiv((uint32_t)row, s.f_T), t = row - g * s.T;
-            ls = d.lse[b * d.ls_b + (hk * s.G + g) * d.ls_h + t * d.ls_t] * kLog2e;
+            ls = __fmaf_rn(d.lse[b * d.ls_b + (hk * s.G + g) * d.ls_h + t * d.ls_t], -kLog2e, 15.f);
           }
-          s.lse2[at_r] = ls;
+          s.bias[at_r] = ls;
           s.delta[at_r] = dlt;
           s.rnorm[at_r] = rn;
         }
@@ -224,6 +224,7 @@ struct Planes {
   const float* norm;
 };
 
+// Waits for a phase, bounded, or until some role of the CTA has given up.
 __device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, int* failed) {
   for (uint32_t i = 0; i < kWaitIters; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -287,16 +288,6 @@ __device__ __forceinline__ uint32_t rows_desc(const unsigned char* tile) { retur
 template <int KN>
 __device__ __forceinline__ uint32_t cols_desc(const unsigned char* tile) { return sw128_low(tile, KN * 128); }
 
-// The two planes of two values below 2^16: hi = the value cut to 11 bits, lo =
-// the rest (exact) rounded to 11.
-__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-  const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
-  const float bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-  const __half2 h = __floats2half2_rn(ah, bh), l = __floats2half2_rn(a - ah, b - bh);
-  *hi = *reinterpret_cast<const uint32_t*>(&h);
-  *lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-
 // Two f32 operations in one instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -320,6 +311,19 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// The two planes of two values below 2^16: hi = the value cut to 11 bits, lo =
+// the rest (exact) rounded to 11.
+__device__ __forceinline__ void split2(uint64_t x, uint32_t* hi, uint32_t* lo) {
+  float a, b, c, d;
+  unpack2(x, &a, &b);
+  const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
+  const float bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+  unpack2(fma2(pack2(ah, bh), pack2(-1.f, -1.f), x), &c, &d);
+  const __half2 h = __floats2half2_rn(ah, bh), l = __floats2half2_rn(c, d);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // What a CTA still has in flight when it gave up: its copies (the slots'
@@ -382,11 +386,9 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * kSlot);
   uint64_t* empty = full + NS;
   uint64_t* qfull = empty + NS;
-  uint64_t* s_full = qfull + 1;        // [MT]
-  uint64_t* p_ready = s_full + MT;     // [MT]
-  uint64_t* o_full = p_ready + MT;     // [MT][OB]
-  uint64_t* o_free = o_full + MT * OB; // [MT][OB]
-  uint64_t* done = o_free + MT * OB;
+  uint64_t* s_full = qfull + 1;     // [MT] S of the next key tile, and P V of the last, are there
+  uint64_t* p_ready = s_full + MT;  // [MT] P is there, and the output buffer it goes to has been read
+  uint64_t* done = p_ready + MT;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -400,10 +402,6 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
     for (int t = 0; t < MT; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_ready[t], 128);
-      for (int o = 0; o < OB; ++o) {
-        mbar_init(&o_full[t * OB + o], 1);
-        mbar_init(&o_free[t * OB + o], 128);
-      }
     }
     mbar_init(done, 1);
     *failed = 0;
@@ -451,8 +449,10 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       const uint32_t lead = elect_lane(), tm = uniform(tmem);
       const uint32_t dq = uniform(rows_desc(sq)), dk = uniform(rows_desc(ring)), dv = uniform(cols_desc<KN>(ring));
       constexpr uint32_t QT = 128 * DP * 4 / 16, SLOT = kSlot / 16;  // a row tile, a slot, in descriptor units
-      bool ok = wait_or_fail(qfull, 0, failed) && wait_or_fail(&full[0], 0, failed);
-      ok = __all_sync(0xffffffffu, ok);
+      auto wait_all = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, wait_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
+      };
+      bool ok = wait_all(qfull, 0) && wait_all(&full[0], 0);
       if (ok) {
         tc_fence_after();
 #pragma unroll 1
@@ -462,30 +462,30 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         }
         umma_commit(lead, &empty[0]);
       }
+      int sv = 1, pv = 0, sk = 2 % NS, pk = 2 / NS;  // slots and phases of V of this tile, K of the next
       for (int j = 0; j < n && ok; ++j) {
-        const int iv = 2 * j + 1, ik = 2 * j + 2, ob = j % OB;
+        const bool more = j + 1 < n;
+        const uint32_t ob = OB == 2 ? (j & 1) * DP : 0;
+        ok = wait_all(&full[sv], pv) && (NS < 5 || !more || wait_all(&full[sk], pk));
 #pragma unroll 1
-        for (int t = 0; t < MT; ++t) {
-          ok = wait_or_fail(&p_ready[t], (uint32_t)j & 1u, failed) &&
-               (t > 0 || wait_or_fail(&full[iv % NS], (uint32_t)(iv / NS) & 1u, failed)) &&
-               (j < OB || wait_or_fail(&o_free[t * OB + ob], (uint32_t)(j / OB - 1) & 1u, failed));
-          ok = __all_sync(0xffffffffu, ok);
+        for (int t = 0; t < MT && ok; ++t) {
+          ok = wait_all(&p_ready[t], j);
           if (!ok) break;
           tc_fence_after();
-          mma_ab<DP, KN>(lead, tm + t * S::cols + KN + ob * DP, tm + t * S::cols, dv + iv % NS * SLOT);
-          umma_commit(lead, &o_full[t * OB + ob]);
-          if (t == MT - 1) umma_commit(lead, &empty[iv % NS]);
-          if (j + 1 < n) {
-            if (t == 0) {
-              ok = __all_sync(0xffffffffu, wait_or_fail(&full[ik % NS], (uint32_t)(ik / NS) & 1u, failed));
-              if (!ok) break;
-              tc_fence_after();
-            }
-            mma_abt<DP, KN>(lead, tm + t * S::cols, dq + t * QT, dk + ik % NS * SLOT);
-            umma_commit(lead, &s_full[t]);
-            if (t == MT - 1) umma_commit(lead, &empty[ik % NS]);
+          mma_ab<DP, KN>(lead, tm + t * S::cols + KN + ob, tm + t * S::cols, dv + sv * SLOT);
+          if (t == MT - 1) umma_commit(lead, &empty[sv]);
+          if (more) {
+            // three slots: this K may still be on its way, after the V before last
+            if (NS < 5 && t == 0 && !(ok = wait_all(&full[sk], pk))) break;
+            mma_abt<DP, KN>(lead, tm + t * S::cols, dq + t * QT, dk + sk * SLOT);
           }
+          umma_commit(lead, &s_full[t]);
+          if (more && t == MT - 1) umma_commit(lead, &empty[sk]);
         }
+        sv += 2;
+        if (sv >= NS) { sv -= NS; ++pv; }
+        sk += 2;
+        if (sk >= NS) { sk -= NS; ++pk; }
       }
       if (!ok) {
         umma_commit(lead, done);
@@ -506,17 +506,14 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
 #pragma unroll
     for (int i = 0; i < DP; ++i) acc[i] = 0.f;
     bool ok = true;
-    // adds tile j's P V to the output
+    // adds tile j's P V, complete, to the output
     auto add_output = [&](int j) {
-      const int ob = j % OB;
-      const bool here = wait_or_fail(&o_full[t * OB + ob], (uint32_t)(j / OB) & 1u, failed);
-      if (!__all_sync(0xffffffffu, here)) return false;
-      tc_fence_after();
+      const uint32_t src = obase + (OB == 2 ? (j & 1) * DP : 0);
       const uint64_t fv2 = pack2(vinv[j], vinv[j]), keep2 = pack2(keep, keep);
 #pragma unroll
       for (int cc = 0; cc < DP / 32; ++cc) {
         uint32_t o[32];
-        tmem_ld32_issue(obase + ob * DP + cc * 32, o);
+        tmem_ld32_issue(src + cc * 32, o);
         tmem_ld_done(o);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -525,9 +522,6 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           unpack2(a2, &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
         }
       }
-      tc_fence_before();
-      mbar_arrive(&o_free[t * OB + ob]);
-      return true;
     };
     for (int j = 0; j < n; ++j) {
       const float f = fmaxf(fq * kinv[j], 0x1p-126f);  // not 0: -inf stands for an absent key below
@@ -535,6 +529,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       ok = wait_or_fail(&s_full[t], (uint32_t)j & 1u, failed);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
+      if (OB == 1 && j > 0) add_output(j - 1);
       uint32_t x[KN / 32][32];  // the row of S, then of P
 #pragma unroll
       for (int cc = 0; cc < KN / 32; ++cc) tmem_ld32_issue(sbase + cc * 32, x[cc]);
@@ -570,8 +565,9 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           unpack2(fma2(pack2(__uint_as_float(x[cc][2 * i]), __uint_as_float(x[cc][2 * i + 1])), f2, b2), &p0, &p1);
           p0 = ex2(p0);
           p1 = ex2(p1);
-          sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
-          split2(p0, p1, &w[i], &w[16 + i]);
+          const uint64_t p = pack2(p0, p1);
+          sum[i & 1] = add2(sum[i & 1], p);
+          split2(p, &w[i], &w[16 + i]);
         }
         tmem_st32(sbase + cc * 32, w);
       }
@@ -581,13 +577,16 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       tmem_st_done();
       tc_fence_before();
       mbar_arrive(&p_ready[t]);
-      if (j > 0) {
-        ok = add_output(j - 1);
-        if (!ok) break;
-      }
+      if (OB == 2 && j > 0) add_output(j - 1);
       keep = alpha;
     }
-    if (ok && n > 0) ok = add_output(n - 1);
+    if (ok && n > 0) {
+      ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)n & 1u, failed)) != 0;
+      if (ok) {
+        tc_fence_after();
+        add_output(n - 1);
+      }
+    }
     if (ok && row < c.M) {
       if (d.splits > 1) {
         const int64_t at = ((int64_t)sp * np + pr) * d.q.rows_p + row;
@@ -627,7 +626,7 @@ struct BwdDev {
   CrossDev c;
   Planes a1, a2, b1, b2;       // dq: q, dout, k, v;  dk/dv: k, v, q, dout
   int mtiles, splits;
-  const float *lse2, *delta, *rnorm, *dmax;  // per query row; per query tile
+  const float *bias, *delta, *rnorm, *dmax;  // per query row; per query tile
   float *part1, *part2;        // [split][problem][a1.rows_p][DP] when splits > 1: dq, or dk and dv
   float f;                     // |scale| log2 e
   float out_scale;             // of dq (scale) or dk (|scale|)
@@ -640,6 +639,7 @@ struct BwdShape {
   static constexpr int KN = kTileElems / DP;
   static constexpr int a_bytes = 128 * DP * 4;
   static constexpr int n1 = DP == 64 ? 3 : 2, n2 = DP == 64 ? 2 : 1;
+  static constexpr bool ahead = n1 == 3;  // room for S two tiles ahead
   static constexpr int smem = 2 * a_bytes + (n1 + n2) * kSlot + 1024 + 512;
   static constexpr int threads = 384;
 };
@@ -652,6 +652,9 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   using S = BwdShape<DP>;
   constexpr int KN = S::KN, N1 = S::n1, N2 = S::n2, HC = KN / 2;  // HC: columns of a warpgroup
   constexpr int AC = KV ? DP : DP / 2;                            // result columns of a warpgroup
+  // dq needs no plane of P, so dS takes the place of S, and the next dP can be
+  // issued before the product that reads dS
+  constexpr bool DS_IN_S = !KV && S::ahead;
   static_assert(3 * KN + (KV ? 2 : 1) * DP <= 512, "tensor memory");
   const CrossDev& c = d.c;
   if (*(volatile const int*)d.nonfinite != 0) return;
@@ -668,8 +671,8 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   uint64_t* afull = empty2 + N2;
   uint64_t* s_full = afull + 1;    // [2]
   uint64_t* dp_full = s_full + 2;
-  uint64_t* p_ready = dp_full + 1;
-  uint64_t* ds_ready = p_ready + 1;
+  uint64_t* p_ready = dp_full + 1;  // [2]: may run a phase ahead of the MMA warp
+  uint64_t* ds_ready = p_ready + 2;
   uint64_t* r_full = ds_ready + 1;
   uint64_t* r_free = r_full + 1;
   uint64_t* done = r_free + 1;
@@ -690,10 +693,11 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
     mbar_init(dp_full, 1);
-    mbar_init(p_ready, 256);
+    mbar_init(&p_ready[0], 256);
+    mbar_init(&p_ready[1], 256);
     mbar_init(ds_ready, 256);
     mbar_init(r_full, 1);
-    mbar_init(r_free, 256);
+    mbar_init(r_free, 128);
     mbar_init(done, 1);
     *failed = 0;
     fence_mbar_init();
@@ -769,24 +773,26 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         if (!KV) umma_commit(lead, &empty2[j % N2]);
         return true;
       };
-      bool ok = all_ok(wait_or_fail(afull, 0, failed)) && s_mma(0) && dp_mma(0);
+      auto wait_all = [&](uint64_t* bar, int phase) { return all_ok(wait_or_fail(bar, (uint32_t)phase & 1u, failed)); };
+      bool ok = wait_all(afull, 0) && s_mma(0) && dp_mma(0);
+      if (S::ahead && ok && n > 1) ok = s_mma(1);
       for (int j = 0; j < n && ok; ++j) {
-        const uint32_t ph = (uint32_t)j & 1u;
         if (KV) {
-          ok = all_ok(wait_or_fail(p_ready, ph, failed) && (j == 0 || wait_or_fail(r_free, ph ^ 1u, failed)));
+          ok = wait_all(&p_ready[j & 1], j >> 1) && (j == 0 || wait_all(r_free, j - 1));
           if (!ok) break;
           tc_fence_after();
           mma_ab<DP, KN>(lead, rc2, tm + (j & 1) * KN, c2 + j % N2 * SLOT);  // P^T dout
           umma_commit(lead, &empty2[j % N2]);
         }
-        if (j + 1 < n && !(ok = s_mma(j + 1))) break;
-        ok = all_ok(wait_or_fail(ds_ready, ph, failed) && (KV || j == 0 || wait_or_fail(r_free, ph ^ 1u, failed)));
-        if (!ok) break;
+        if (!S::ahead && j + 1 < n && !(ok = s_mma(j + 1))) break;
+        if (!(ok = wait_all(ds_ready, j))) break;
         tc_fence_after();
-        mma_ab<DP, KN>(lead, rc1, dpc, c1 + j % N1 * SLOT);  // dS k, or dS^T q
+        if (DS_IN_S && j + 1 < n && !(ok = dp_mma(j + 1))) break;
+        mma_ab<DP, KN>(lead, rc1, DS_IN_S ? tm + (j & 1) * KN : dpc, c1 + j % N1 * SLOT);  // dS k, or dS^T q
         umma_commit(lead, &empty1[j % N1]);
         umma_commit(lead, r_full);
-        if (j + 1 < n) ok = dp_mma(j + 1);
+        if (!DS_IN_S && j + 1 < n && !(ok = dp_mma(j + 1))) break;
+        if (S::ahead && j + 2 < n) ok = s_mma(j + 2);
       }
       if (!ok) {
         umma_commit(lead, done);
@@ -805,7 +811,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
     const float* nb2 = d.b2.norm + pr * bt + j0;
     // per query row: of this row (dq) or of the columns (dk, dv)
     const int64_t qrow = (int64_t)pr * (KV ? d.b1.rows_p : d.a1.rows_p) + (KV ? j0 * KN + wg * HC : row);
-    const float r_lse = KV ? 0.f : d.lse2[qrow], r_delta = KV ? 0.f : d.delta[qrow];
+    const float r_bias = KV ? 0.f : d.bias[qrow] - 15.f, r_delta = KV ? 0.f : d.delta[qrow];
     const float r_norm = KV ? d.a2.norm[pr * at1 + row / KN] : d.rnorm[qrow];
     const float* dmax = KV ? d.dmax + pr * bt + j0 : nullptr;
     float acc[AC];
@@ -819,58 +825,67 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       tc_fence_after();
       const float w = KV ? (wg == 0 ? ib2[j] * 0x1p-15f : ib1[j] * d.out_scale * ds_down) : ib1[j] * d.out_scale * ds_down;
       const uint32_t src = KV ? (wg == 0 ? t_r2 : t_r1) : t_r1 + wg * AC;
+      const uint64_t w2 = pack2(w, w);
 #pragma unroll
       for (int cc = 0; cc < AC / 32; ++cc) {
         uint32_t o[32];
         tmem_ld32_issue(src + lanes + cc * 32, o);
         tmem_ld_done(o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[cc * 32 + i] = __fmaf_rn(__uint_as_float(o[i]), w, acc[cc * 32 + i]);
+        for (int i = 0; i < 32; i += 2)
+          unpack2(fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), w2,
+                       pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1])),
+                  &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
       }
       tc_fence_before();
-      mbar_arrive(r_free);
+      if (KV && wg == 0) mbar_arrive(r_free);
       return true;
     };
     for (int j = 0; j < n; ++j) {
       const int limit = cols - (j0 + j) * KN - wg * HC;  // columns of this warpgroup's half
       const float f = d.f * ia1 * ib1[j];
       const uint32_t sb = tmem + lanes + (j & 1) * KN + wg * HC, db = t_dp + lanes + wg * HC;
+      float p[HC];  // the exponent's bias, then P (dk, dv: P 2^15)
+      if (KV) {
+        const float4* bi = reinterpret_cast<const float4*>(d.bias + qrow + j * KN);
+#pragma unroll
+        for (int i = 0; i < HC / 4; ++i) {
+          const float4 x = __ldg(bi + i);
+          p[4 * i] = x.x;
+          p[4 * i + 1] = x.y;
+          p[4 * i + 2] = x.z;
+          p[4 * i + 3] = x.w;
+        }
+      }
       ok = wait_or_fail(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, failed);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
-      float p[HC];  // dk, dv: P 2^15
+      const uint64_t f2 = pack2(f, f);
 #pragma unroll
       for (int cc = 0; cc < HC / 32; ++cc) {
         uint32_t a[32];
         tmem_ld32_issue(sb + cc * 32, a);
         tmem_ld_done(a);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float& p0 = p[cc * 32 + i];
+          float& p1 = p[cc * 32 + i + 1];
+          const uint64_t bias = KV ? pack2(p0, p1) : pack2(r_bias, r_bias);
+          unpack2(fma2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), f2, bias), &p0, &p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+        }
         if (KV) {
-          const float4* ls = reinterpret_cast<const float4*>(d.lse2 + qrow + j * KN + cc * 32);
           uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 q = __ldg(ls + i);
-            p[cc * 32 + 4 * i] = ex2(__fmaf_rn(__uint_as_float(a[4 * i]), f, 15.f - q.x));
-            p[cc * 32 + 4 * i + 1] = ex2(__fmaf_rn(__uint_as_float(a[4 * i + 1]), f, 15.f - q.y));
-            p[cc * 32 + 4 * i + 2] = ex2(__fmaf_rn(__uint_as_float(a[4 * i + 2]), f, 15.f - q.z));
-            p[cc * 32 + 4 * i + 3] = ex2(__fmaf_rn(__uint_as_float(a[4 * i + 3]), f, 15.f - q.w));
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) split2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1], &w[i], &w[16 + i]);
+          for (int i = 0; i < 16; ++i) split2(pack2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1]), &w[i], &w[16 + i]);
           tmem_st32(sb + cc * 32, w);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) p[cc * 32 + i] = ex2(__fmaf_rn(__uint_as_float(a[i]), f, -r_lse));
         }
       }
       if (KV) {
         tmem_st_done();
         tc_fence_before();
-        mbar_arrive(p_ready);
-      }
-      if (j > 0) {
-        ok = add_result(j - 1);
-        if (!ok) break;
+        mbar_arrive(&p_ready[j & 1]);
       }
       // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below 2^15
       const float g = ia2 * ib2[j];
@@ -878,45 +893,48 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       uint32_t eb = __float_as_uint(bound) >> 23;
       eb = eb < 15u ? 15u : eb;
       const float up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);
-      ds_down = __uint_as_float((eb - 14u) << 23);
-      const float gu = g * up;
+      const uint64_t gu = pack2(g * up, g * up), nup = pack2(-up, -up), ndu = pack2(-r_delta * up, -r_delta * up);
       ok = wait_or_fail(dp_full, (uint32_t)j & 1u, failed);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
+      if (KV && j > 0) {
+        ok = add_result(j - 1);
+        if (!ok) break;
+      }
+      if (KV) ds_down = __uint_as_float((eb - 14u) << 23);
 #pragma unroll
       for (int cc = 0; cc < HC / 32; ++cc) {
+        float4 dl[8];
+        if (KV) {
+          const float4* de = reinterpret_cast<const float4*>(d.delta + qrow + j * KN + cc * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dl[i] = __ldg(de + i);
+        }
         uint32_t a[32], w[32];
         tmem_ld32_issue(db + cc * 32, a);
         tmem_ld_done(a);
-        if (KV) {
-          const float4* dl = reinterpret_cast<const float4*>(d.delta + qrow + j * KN + cc * 32);
+        const bool part = !KV && limit < (cc + 1) * 32;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 q = __ldg(dl + i);
-            const float x0 = p[cc * 32 + 4 * i] * __fmaf_rn(__uint_as_float(a[4 * i]), gu, -q.x * up);
-            const float x1 = p[cc * 32 + 4 * i + 1] * __fmaf_rn(__uint_as_float(a[4 * i + 1]), gu, -q.y * up);
-            const float x2 = p[cc * 32 + 4 * i + 2] * __fmaf_rn(__uint_as_float(a[4 * i + 2]), gu, -q.z * up);
-            const float x3 = p[cc * 32 + 4 * i + 3] * __fmaf_rn(__uint_as_float(a[4 * i + 3]), gu, -q.w * up);
-            split2(x0, x1, &w[2 * i], &w[16 + 2 * i]);
-            split2(x2, x3, &w[2 * i + 1], &w[16 + 2 * i + 1]);
+        for (int i = 0; i < 16; ++i) {
+          const float4& q = dl[i / 2];
+          const uint64_t nd = KV ? mul2(i % 2 ? pack2(q.z, q.w) : pack2(q.x, q.y), nup) : ndu;
+          uint64_t x = mul2(pack2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1]),
+                            fma2(pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), gu, nd));
+          if (part) {
+            float x0, x1;
+            unpack2(x, &x0, &x1);
+            x = pack2(cc * 32 + 2 * i < limit ? x0 : 0.f, cc * 32 + 2 * i + 1 < limit ? x1 : 0.f);
           }
-        } else {
-          const float du = -r_delta * up;
-          const bool part = limit < (cc + 1) * 32;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float x0 = p[cc * 32 + 2 * i] * __fmaf_rn(__uint_as_float(a[2 * i]), gu, du);
-            float x1 = p[cc * 32 + 2 * i + 1] * __fmaf_rn(__uint_as_float(a[2 * i + 1]), gu, du);
-            if (part) {
-              if (cc * 32 + 2 * i >= limit) x0 = 0.f;
-              if (cc * 32 + 2 * i + 1 >= limit) x1 = 0.f;
-            }
-            split2(x0, x1, &w[i], &w[16 + i]);
-          }
+          split2(x, &w[i], &w[16 + i]);
         }
-        tmem_st32(db + cc * 32, w);
+        tmem_st32((DS_IN_S ? sb : db) + cc * 32, w);
       }
       tmem_st_done();
+      if (!KV && j > 0) {
+        ok = add_result(j - 1);
+        if (!ok) break;
+      }
+      if (!KV) ds_down = __uint_as_float((eb - 14u) << 23);
       tc_fence_before();
       mbar_arrive(ds_ready);
     }
@@ -1209,7 +1227,7 @@ Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) 
   k_d.splits = pick_splits((int64_t)k_d.mtiles * np, (c.M + KN - 1) / KN);
   k_d.out_scale = fabsf(c.scale);
   Packed q, k, v, g;
-  float *lse2 = nullptr, *delta = nullptr, *rnorm = nullptr, *dmax = nullptr;
+  float *bias = nullptr, *delta = nullptr, *rnorm = nullptr, *dmax = nullptr;
   Scratch buf;
   for (int pass = 0; pass < 2; ++pass) {
     Arena a;
@@ -1218,7 +1236,7 @@ Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) 
     place(a, g, np, c.M, DP, true);
     place(a, k, np, c.Tk, DP, false);
     place(a, v, np, c.Tk, DP, true);
-    lse2 = a.take<float>(q.rows_all);
+    bias = a.take<float>(q.rows_all);
     delta = a.take<float>(q.rows_all);
     rnorm = a.take<float>(q.rows_all);
     dmax = a.take<float>(q.rows_all / KN);
@@ -1247,14 +1265,14 @@ Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) 
   PackSrc& gs = p.s[3];
   gs.grad = 1;
   gs.out = c.out;
-  gs.lse2 = lse2;
+  gs.bias = bias;
   gs.delta = delta;
   gs.rnorm = rnorm;
   gs.dmax = dmax;
   e = run_pack(p, c, DP, nonfinite, stream);
   if (!e.ok()) return e;
   for (BwdDev* x : {&q_d, &k_d}) {
-    x->lse2 = lse2;
+    x->bias = bias;
     x->delta = delta;
     x->rnorm = rnorm;
     x->dmax = dmax;
