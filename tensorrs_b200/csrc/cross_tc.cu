@@ -224,11 +224,36 @@ struct Planes {
   const float* norm;
 };
 
+// A warp's arrival: one lane, after the others' work.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) mbar_arrive(bar);
+}
+
 // Waits for a phase, bounded, or until some role of the CTA has given up.
 __device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, int* failed) {
   for (uint32_t i = 0; i < kWaitIters; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 63) == 63 && *(volatile int*)failed) return false;
+  }
+  atomicExch(failed, 1);
+  return false;
+}
+
+// The same for the MMA warps, without the suspension of try_wait: a hand-over
+// to the tensor core is on the path between two tiles.
+__device__ __forceinline__ bool spin_or_fail(uint64_t* bar, uint32_t parity, int* failed) {
+  for (uint32_t i = 0; i < (1u << 27); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 255) == 255 && *(volatile int*)failed) return false;
   }
   atomicExch(failed, 1);
   return false;
@@ -352,7 +377,8 @@ __device__ __forceinline__ void take_registers() {
 struct FwdDev {
   CrossDev c;
   Planes q, k, v;
-  int mtiles, splits;    // CTAs: mtiles * problems * splits
+  int mtiles, splits;    // items: mtiles * problems * splits
+  int items;
   float *part, *part_m, *part_l;  // [split][problem][q.rows_p](DP) when splits > 1
   float f;               // |scale| log2 e
   const int* nonfinite;
@@ -367,8 +393,31 @@ struct FwdShape {
   static constexpr int smem = q_bytes + slots * kSlot + 1024 + 512;
   static constexpr int OB = DP == 64 ? 2 : 1;       // output accumulators per row tile
   static constexpr int cols = KN + OB * DP;         // tensor-memory columns per row tile
-  static constexpr int threads = MT * 128 + 128;    // row tiles' warpgroups, then MMA and TMA warps (two idle)
+  static constexpr int threads = MT * 128 + 128;    // the row tiles' warpgroups; MT MMA warps, a TMA warp, idle ones
 };
+
+// One item of a persistent CTA: a block of MT row tiles, a problem, a part of
+// its keys.
+struct FwdItem {
+  int mtile, pr, sp, b, hk, len, j0, n;  // n key tiles from j0
+};
+template <int KN>
+__device__ __forceinline__ FwdItem fwd_item(const FwdDev& d, int item) {
+  const CrossDev& c = d.c;
+  FwdItem w;
+  w.mtile = item % d.mtiles;
+  item /= d.mtiles;
+  const int np = c.B * c.Hk;
+  w.pr = item % np;
+  w.sp = item / np;
+  w.b = w.pr / c.Hk;
+  w.hk = w.pr % c.Hk;
+  w.len = key_count(c.len, c.len64, c.len_s, c.Tk, w.b);
+  const int all = (w.len + KN - 1) / KN, per = (all + d.splits - 1) / d.splits;
+  w.j0 = min(all, w.sp * per);
+  w.n = min(all, w.j0 + per) - w.j0;
+  return w;
+}
 
 template <int DP, int MT>
 __global__ void __launch_bounds__(MT * 128 + 128, 1)
@@ -385,25 +434,31 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   unsigned char* ring = smem + S::q_bytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * kSlot);
   uint64_t* empty = full + NS;
-  uint64_t* qfull = empty + NS;
-  uint64_t* s_full = qfull + 1;     // [MT] S of the next key tile, and P V of the last, are there
+  uint64_t* q_full = empty + NS;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;   // [MT] S of the next key tile, and P V of the last, are there
   uint64_t* p_ready = s_full + MT;  // [MT] P is there, and the output buffer it goes to has been read
-  uint64_t* done = p_ready + MT;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* o_read = p_ready + MT;  // [MT] an item's last output has been read
+  uint64_t* first_p = o_read + MT;  // row tile 0 has its first P of an item
+  uint64_t* done = first_p + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + MT);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], MT);
     }
-    mbar_init(qfull, 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, MT);
+    mbar_init(first_p, 4);
     for (int t = 0; t < MT; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_ready[t], 128);
+      mbar_init(&p_ready[t], 4);
+      mbar_init(&o_read[t], 4);
+      mbar_init(&done[t], 1);
     }
-    mbar_init(done, 1);
     *failed = 0;
     fence_mbar_init();
   }
@@ -416,201 +471,222 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-
   const int np = c.B * c.Hk;
-  const int mtile = blockIdx.x % d.mtiles, pr = blockIdx.x / d.mtiles % np, sp = blockIdx.x / d.mtiles / np;
-  const int b = pr / c.Hk, hk = pr % c.Hk;
-  const int len = key_count(c.len, c.len64, c.len_s, c.Tk, b);
-  const int all = (len + KN - 1) / KN, per = (all + d.splits - 1) / d.splits;
-  const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;  // this CTA's key tiles
 
   if (warp >= MT * 4) {
     if (MT == 2) give_registers<56>();
-    if (warp == MT * 4 + 1 && lane == 0 && n > 0) {  // TMA
-      mbar_arrive_expect_tx(qfull, S::q_bytes);
+    if (warp == MT * 5 && lane == 0) {  // TMA
+      int li = 0, qi = 0;               // tiles and query blocks loaded so far
+      bool ok = true;
+      for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+        const FwdItem w = fwd_item<KN>(d, item);
+        if (w.n == 0) continue;
+        if (qi > 0 && !(ok = wait_or_fail(q_empty, (uint32_t)(qi - 1) & 1u, failed))) break;
+        mbar_arrive_expect_tx(q_full, S::q_bytes);
 #pragma unroll 1
-      for (int t = 0; t < MT; ++t)
-        load_planes<DP, 128>(sq + t * 128 * DP * 4, &mq, d.q, pr * d.q.rows_p + (mtile * MT + t) * 128, qfull);
-      int i = 0;
-      for (; i < 2 * n; ++i) {
-        const int s = i % NS;
-        if (i >= NS && !wait_or_fail(&empty[s], (uint32_t)(i / NS - 1) & 1u, failed)) break;
-        mbar_arrive_expect_tx(&full[s], kSlot);
-        const int row = pr * d.k.rows_p + (j0 + i / 2) * KN;
-        if (i & 1) load_planes<DP, KN>(ring + s * kSlot, &mv, d.v, row, &full[s]);
-        else load_planes<DP, KN>(ring + s * kSlot, &mk, d.k, row, &full[s]);
-      }
-      if (i < 2 * n) {
-        mbar_wait(qfull, 0);
-        drain(full, NS, i);
-      }
-    }
-    if (warp == MT * 4 && n > 0) {  // MMA: the warp stays whole, one lane issues
-      const uint32_t lead = elect_lane(), tm = uniform(tmem);
-      const uint32_t dq = uniform(rows_desc(sq)), dk = uniform(rows_desc(ring)), dv = uniform(cols_desc<KN>(ring));
-      constexpr uint32_t QT = 128 * DP * 4 / 16, SLOT = kSlot / 16;  // a row tile, a slot, in descriptor units
-      auto wait_all = [&](uint64_t* bar, int phase) {
-        return __all_sync(0xffffffffu, wait_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
-      };
-      bool ok = wait_all(qfull, 0) && wait_all(&full[0], 0);
-      if (ok) {
-        tc_fence_after();
-#pragma unroll 1
-        for (int t = 0; t < MT; ++t) {
-          mma_abt<DP, KN>(lead, tm + t * S::cols, dq + t * QT, dk);
-          umma_commit(lead, &s_full[t]);
+        for (int t = 0; t < MT; ++t)
+          load_planes<DP, 128>(sq + t * 128 * DP * 4, &mq, d.q, w.pr * d.q.rows_p + (w.mtile * MT + t) * 128, q_full);
+        ++qi;
+        for (int i = 0; i < 2 * w.n; ++i, ++li) {
+          const int s = li % NS;
+          if (li >= NS && !(ok = wait_or_fail(&empty[s], (uint32_t)(li / NS - 1) & 1u, failed))) break;
+          mbar_arrive_expect_tx(&full[s], kSlot);
+          const int row = w.pr * d.k.rows_p + (w.j0 + i / 2) * KN;
+          if (i & 1) load_planes<DP, KN>(ring + s * kSlot, &mv, d.v, row, &full[s]);
+          else load_planes<DP, KN>(ring + s * kSlot, &mk, d.k, row, &full[s]);
         }
-        umma_commit(lead, &empty[0]);
-      }
-      int sv = 1, pv = 0, sk = 2 % NS, pk = 2 / NS;  // slots and phases of V of this tile, K of the next
-      for (int j = 0; j < n && ok; ++j) {
-        const bool more = j + 1 < n;
-        const uint32_t ob = OB == 2 ? (j & 1) * DP : 0;
-        ok = wait_all(&full[sv], pv) && (NS < 5 || !more || wait_all(&full[sk], pk));
-#pragma unroll 1
-        for (int t = 0; t < MT && ok; ++t) {
-          ok = wait_all(&p_ready[t], j);
-          if (!ok) break;
-          tc_fence_after();
-          mma_ab<DP, KN>(lead, tm + t * S::cols + KN + ob, tm + t * S::cols, dv + sv * SLOT);
-          if (t == MT - 1) umma_commit(lead, &empty[sv]);
-          if (more) {
-            // three slots: this K may still be on its way, after the V before last
-            if (NS < 5 && t == 0 && !(ok = wait_all(&full[sk], pk))) break;
-            mma_abt<DP, KN>(lead, tm + t * S::cols, dq + t * QT, dk + sk * SLOT);
-          }
-          umma_commit(lead, &s_full[t]);
-          if (more && t == MT - 1) umma_commit(lead, &empty[sk]);
-        }
-        sv += 2;
-        if (sv >= NS) { sv -= NS; ++pv; }
-        sk += 2;
-        if (sk >= NS) { sk -= NS; ++pk; }
       }
       if (!ok) {
-        umma_commit(lead, done);
-        mbar_wait(done, 0);
+        if (qi > 0) mbar_wait(q_full, (uint32_t)(qi - 1) & 1u);
+        drain(full, NS, li);
+      }
+    } else if (warp < MT * 5) {  // MMA of row tile t: the warp stays whole, one lane issues
+      const int t = warp - MT * 4;
+      const uint32_t lead = elect_lane(), ts = uniform(tmem + t * S::cols);
+      const uint32_t dq = uniform(rows_desc(sq + t * 128 * DP * 4)), dk = uniform(rows_desc(ring));
+      const uint32_t dv = uniform(cols_desc<KN>(ring));
+      constexpr uint32_t SLOT = kSlot / 16;  // in descriptor units
+      auto wait_all = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, spin_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
+      };
+      int slot = 0, ph = 0, qi = 0, pc = 0;  // next tile's slot and its phase; query blocks and P's so far
+      bool ok = true;
+      for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+        const int n = fwd_item<KN>(d, item).n;
+        if (n == 0) continue;
+        ok = wait_all(q_full, qi) && wait_all(&full[slot], ph) && (qi == 0 || wait_all(&o_read[t], qi - 1));
+        // the second row tile starts when the first has left the softmax, so that
+        // from then on one is in the softmax while the other has the tensor core
+        if (ok && t == 1) ok = wait_all(first_p, qi);
+        if (!ok) break;
+        ++qi;
+        tc_fence_after();
+        mma_abt<DP, KN>(lead, ts, dq, dk + slot * SLOT);
+        umma_commit(lead, &s_full[t]);
+        umma_commit(lead, &empty[slot]);
+        if (n == 1) umma_commit(lead, q_empty);
+        if (++slot == NS) { slot = 0; ++ph; }
+        for (int j = 0; j < n; ++j) {
+          const bool more = j + 1 < n;
+          const int sv = slot, sk = slot + 1 == NS ? 0 : slot + 1, pk = sk ? ph : ph + 1;
+          // with three slots the next K may still be on its way when P is there
+          ok = wait_all(&full[sv], ph) && (NS < 5 || !more || wait_all(&full[sk], pk)) && wait_all(&p_ready[t], pc);
+          if (!ok) break;
+          ++pc;
+          tc_fence_after();
+          mma_ab<DP, KN>(lead, ts + KN + (OB == 2 ? (j & 1) * DP : 0), ts, dv + sv * SLOT);
+          if (NS < 5) umma_commit(lead, &empty[sv]);
+          if (more) {
+            if (NS < 5 && !(ok = wait_all(&full[sk], pk))) break;
+            mma_abt<DP, KN>(lead, ts, dq, dk + sk * SLOT);
+          }
+          umma_commit(lead, &s_full[t]);
+          if (NS >= 5) umma_commit(lead, &empty[sv]);
+          slot = sk;
+          ph = pk;
+          if (more) {
+            umma_commit(lead, &empty[sk]);
+            if (j + 2 == n) umma_commit(lead, q_empty);
+            if (++slot == NS) { slot = 0; ++ph; }
+          }
+        }
+      }
+      if (!ok) {
+        umma_commit(lead, &done[t]);
+        mbar_wait(&done[t], 0);
       }
     }
   } else {  // softmax: one thread per row
     if (MT == 2) take_registers<56>();
-    const int t = warp / 4;
-    const int rl = (warp % 4) * 32 + lane, row = (mtile * MT + t) * 128 + rl;
+    const int t = warp / 4, rl = (warp % 4) * 32 + lane;
     const uint32_t sbase = tmem + ((uint32_t)((warp % 4) * 32) << 16) + t * S::cols, obase = sbase + KN;
-    const int qtiles = d.q.rows_p / KN;
-    const float fq = d.f * d.q.inv[pr * qtiles + row / KN];
-    const float* kinv = d.k.inv + pr * (d.k.rows_p / KN) + j0;
-    const float* vinv = d.v.inv + pr * (d.v.rows_p / KN) + j0;
-    float m = -INFINITY, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
-    float acc[DP];
-#pragma unroll
-    for (int i = 0; i < DP; ++i) acc[i] = 0.f;
+    const int qtiles = d.q.rows_p / KN, ktiles = d.k.rows_p / KN;
+    int sc = 0;  // S's taken so far
     bool ok = true;
-    // adds tile j's P V, complete, to the output
-    auto add_output = [&](int j) {
-      const uint32_t src = obase + (OB == 2 ? (j & 1) * DP : 0);
-      const uint64_t fv2 = pack2(vinv[j], vinv[j]), keep2 = pack2(keep, keep);
-#pragma unroll
-      for (int cc = 0; cc < DP / 32; ++cc) {
-        uint32_t o[32];
-        tmem_ld32_issue(src + cc * 32, o);
-        tmem_ld_done(o);
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          uint64_t a2 = mul2(pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1]), keep2);
-          a2 = fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), fv2, a2);
-          unpack2(a2, &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
-        }
+    for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+      int n, kt, limit;  // key tiles, the first one's index among all, keys from it on
+      float fq;
+      {
+        const FwdItem w = fwd_item<KN>(d, item);
+        n = w.n;
+        kt = w.pr * ktiles + w.j0;
+        limit = w.len - w.j0 * KN;
+        fq = d.f * d.q.inv[w.pr * qtiles + ((w.mtile * MT + t) * 128 + rl) / KN];
       }
-    };
-    for (int j = 0; j < n; ++j) {
-      const float f = fmaxf(fq * kinv[j], 0x1p-126f);  // not 0: -inf stands for an absent key below
-      const int limit = len - (j0 + j) * KN;  // keys of this tile
-      ok = wait_or_fail(&s_full[t], (uint32_t)j & 1u, failed);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      if (OB == 1 && j > 0) add_output(j - 1);
-      uint32_t x[KN / 32][32];  // the row of S, then of P
+      float m = -INFINITY, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
+      float acc[DP];
 #pragma unroll
-      for (int cc = 0; cc < KN / 32; ++cc) tmem_ld32_issue(sbase + cc * 32, x[cc]);
-      tmem_ld_done(x[0]);
+      for (int i = 0; i < DP; ++i) acc[i] = 0.f;
+      // adds tile j's P V, complete, to the output
+      auto add_output = [&](int j) {
+        const uint32_t src = obase + (OB == 2 ? (j & 1) * DP : 0);
+        const float fv = d.v.inv[kt + j];
+        const uint64_t fv2 = pack2(fv, fv), keep2 = pack2(keep, keep);
 #pragma unroll
-      for (int cc = 1; cc < KN / 32; ++cc) tmem_ld_tie(x[cc]);
-      if (limit < KN) {  // behind the last key: no weight
+        for (int cc = 0; cc < DP / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32_issue(src + cc * 32, o);
+          tmem_ld_done(o);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            uint64_t a2 = mul2(pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1]), keep2);
+            a2 = fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), fv2, a2);
+            unpack2(a2, &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
+          }
+        }
+      };
+      for (int j = 0; j < n; ++j, limit -= KN) {
+        const float f = fmaxf(fq * d.k.inv[kt + j], 0x1p-126f);  // not 0: -inf stands for an absent key below
+        ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)sc & 1u, failed)) != 0;
+        if (!ok) break;
+        ++sc;
+        tc_fence_after();
+        if (OB == 1 && j > 0) add_output(j - 1);
+        uint32_t x[KN / 32][32];  // the row of S, then of P
+#pragma unroll
+        for (int cc = 0; cc < KN / 32; ++cc) tmem_ld32_issue(sbase + cc * 32, x[cc]);
+        tmem_ld_done(x[0]);
+#pragma unroll
+        for (int cc = 1; cc < KN / 32; ++cc) tmem_ld_tie(x[cc]);
+        if (limit < KN) {  // behind the last key: no weight
+#pragma unroll
+          for (int cc = 0; cc < KN / 32; ++cc)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (cc * 32 + i >= limit) x[cc][i] = 0xff800000u;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int cc = 0; cc < KN / 32; ++cc)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (cc * 32 + i >= limit) x[cc][i] = 0xff800000u;
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int i = 0; i < 32; i += 2)
+            mx4[i / 2 % 4] = fmaxf(fmaxf(mx4[i / 2 % 4], __uint_as_float(x[cc][i])), __uint_as_float(x[cc][i + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        const float mn = fmaxf(m, mx * f);
+        const float alpha = ex2(m - mn);
+        const float bias = 15.f - mn;
+        m = mn;
+        const uint64_t f2 = pack2(f, f), b2 = pack2(bias, bias);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int cc = 0; cc < KN / 32; ++cc)
+        for (int cc = 0; cc < KN / 32; ++cc) {
+          uint32_t y[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          mx4[i / 2 % 4] = fmaxf(fmaxf(mx4[i / 2 % 4], __uint_as_float(x[cc][i])), __uint_as_float(x[cc][i + 1]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-      const float mn = fmaxf(m, mx * f);
-      const float alpha = ex2(m - mn);
-      const float bias = 15.f - mn;
-      m = mn;
-      const uint64_t f2 = pack2(f, f), b2 = pack2(bias, bias);
-      uint64_t sum[2] = {0, 0};
-#pragma unroll
-      for (int cc = 0; cc < KN / 32; ++cc) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float p0, p1;
-          unpack2(fma2(pack2(__uint_as_float(x[cc][2 * i]), __uint_as_float(x[cc][2 * i + 1])), f2, b2), &p0, &p1);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
-          const uint64_t p = pack2(p0, p1);
-          sum[i & 1] = add2(sum[i & 1], p);
-          split2(p, &w[i], &w[16 + i]);
+          for (int i = 0; i < 16; ++i) {
+            float p0, p1;
+            unpack2(fma2(pack2(__uint_as_float(x[cc][2 * i]), __uint_as_float(x[cc][2 * i + 1])), f2, b2), &p0, &p1);
+            const uint64_t p = pack2(ex2(p0), ex2(p1));
+            sum[i & 1] = add2(sum[i & 1], p);
+            split2(p, &y[i], &y[16 + i]);
+          }
+          tmem_st32(sbase + cc * 32, y);
         }
-        tmem_st32(sbase + cc * 32, w);
+        float sum0, sum1;
+        unpack2(add2(sum[0], sum[1]), &sum0, &sum1);
+        l = __fmaf_rn(l, alpha, sum0 + sum1);
+        tmem_st_done();
+        tc_fence_before();
+        warp_arrive(&p_ready[t]);
+        if (MT == 2 && t == 0 && j == 0) warp_arrive(first_p);
+        if (OB == 2 && j > 0) add_output(j - 1);
+        keep = alpha;
       }
-      float sum0, sum1;
-      unpack2(add2(sum[0], sum[1]), &sum0, &sum1);
-      l = __fmaf_rn(l, alpha, sum0 + sum1);
-      tmem_st_done();
-      tc_fence_before();
-      mbar_arrive(&p_ready[t]);
-      if (OB == 2 && j > 0) add_output(j - 1);
-      keep = alpha;
-    }
-    if (ok && n > 0) {
-      ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)n & 1u, failed)) != 0;
-      if (ok) {
+      if (ok && n > 0) {
+        ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)sc & 1u, failed)) != 0;
+        if (!ok) break;
+        ++sc;
         tc_fence_after();
         add_output(n - 1);
+        tc_fence_before();
+        warp_arrive(&o_read[t]);
       }
-    }
-    if (ok && row < c.M) {
-      if (d.splits > 1) {
-        const int64_t at = ((int64_t)sp * np + pr) * d.q.rows_p + row;
-        float4* o = reinterpret_cast<float4*>(d.part + at * DP);
+      const FwdItem w = fwd_item<KN>(d, item);
+      const int row = (w.mtile * MT + t) * 128 + rl;
+      if (ok && row < c.M) {
+        if (d.splits > 1) {
+          const int64_t at = ((int64_t)w.sp * np + w.pr) * d.q.rows_p + row;
+          float4* o = reinterpret_cast<float4*>(d.part + at * DP);
 #pragma unroll
-        for (int i = 0; i < DP / 4; ++i) o[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
-        d.part_m[at] = m - 15.f;  // acc and l carry 2^15
-        d.part_l[at] = l;
-      } else {
-        const int g = (int)fdiv((uint32_t)row, c.f_Tq), tt = row - g * c.Tq, h = hk * c.G + g;
-        float* op = static_cast<float*>(c.out.p) + b * c.out.sb + tt * c.out.st + h * c.out.sh;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (c.vec) {
-#pragma unroll
-          for (int i = 0; i < DP / 4; ++i)
-            if (4 * i < c.D)
-              reinterpret_cast<float4*>(op)[i] =
-                  make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv, acc[4 * i + 3] * inv);
+          for (int i = 0; i < DP / 4; ++i) o[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+          d.part_m[at] = m - 15.f;  // acc and l carry 2^15
+          d.part_l[at] = l;
         } else {
+          const int g = (int)fdiv((uint32_t)row, c.f_Tq), tt = row - g * c.Tq, h = w.hk * c.G + g;
+          float* op = static_cast<float*>(c.out.p) + w.b * c.out.sb + tt * c.out.st + h * c.out.sh;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (c.vec) {
 #pragma unroll
-          for (int i = 0; i < DP; ++i)
-            if (i < c.D) op[i * c.out.sd] = acc[i] * inv;
+            for (int i = 0; i < DP / 4; ++i)
+              if (4 * i < c.D)
+                reinterpret_cast<float4*>(op)[i] =
+                    make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv, acc[4 * i + 3] * inv);
+          } else {
+#pragma unroll
+            for (int i = 0; i < DP; ++i)
+              if (i < c.D) op[i * c.out.sd] = acc[i] * inv;
+          }
+          if (c.lse) c.lse[w.b * c.ls_b + h * c.ls_h + tt * c.ls_t] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * kLn2;
         }
-        if (c.lse) c.lse[b * c.ls_b + h * c.ls_h + tt * c.ls_t] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * kLn2;
       }
     }
   }
@@ -625,7 +701,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
 struct BwdDev {
   CrossDev c;
   Planes a1, a2, b1, b2;       // dq: q, dout, k, v;  dk/dv: k, v, q, dout
-  int mtiles, splits;
+  int mtiles, splits, items;
   const float *bias, *delta, *rnorm, *dmax;  // per query row; per query tile
   float *part1, *part2;        // [split][problem][a1.rows_p][DP] when splits > 1: dq, or dk and dv
   float f;                     // |scale| log2 e
@@ -643,6 +719,31 @@ struct BwdShape {
   static constexpr int smem = 2 * a_bytes + (n1 + n2) * kSlot + 1024 + 512;
   static constexpr int threads = 384;
 };
+
+// One item of a persistent CTA: a row tile, a problem, a part of the walk.
+struct BwdItem {
+  int mtile, pr, sp, b, hk, rows, cols, j0, n;  // rows with work, columns, n column tiles from j0
+};
+template <int KN, bool KV>
+__device__ __forceinline__ BwdItem bwd_item(const BwdDev& d, int item) {
+  const CrossDev& c = d.c;
+  BwdItem w;
+  w.mtile = item % d.mtiles;
+  item /= d.mtiles;
+  const int np = c.B * c.Hk;
+  w.pr = item % np;
+  w.sp = item / np;
+  w.b = w.pr / c.Hk;
+  w.hk = w.pr % c.Hk;
+  const int len = key_count(c.len, c.len64, c.len_s, c.Tk, w.b);
+  w.cols = KV ? c.M : len;
+  w.rows = KV ? len : c.M;
+  const int all = w.mtile * 128 >= w.rows || len == 0 ? 0 : (w.cols + KN - 1) / KN;
+  const int per = (all + d.splits - 1) / d.splits;
+  w.j0 = min(all, w.sp * per);
+  w.n = min(all, w.j0 + per) - w.j0;
+  return w;
+}
 
 template <int DP, bool KV>
 __global__ void __launch_bounds__(384, 1)
@@ -668,13 +769,14 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   uint64_t* empty1 = full1 + N1;
   uint64_t* full2 = empty1 + N1;
   uint64_t* empty2 = full2 + N2;
-  uint64_t* afull = empty2 + N2;
-  uint64_t* s_full = afull + 1;    // [2]
+  uint64_t* a_full = empty2 + N2;
+  uint64_t* a_empty = a_full + 1;
+  uint64_t* s_full = a_empty + 1;   // [2]
   uint64_t* dp_full = s_full + 2;
   uint64_t* p_ready = dp_full + 1;  // [2]: may run a phase ahead of the MMA warp
   uint64_t* ds_ready = p_ready + 2;
-  uint64_t* r_full = ds_ready + 1;
-  uint64_t* r_free = r_full + 1;
+  uint64_t* r_full = ds_ready + 1;  // a tile's results are there
+  uint64_t* r_free = r_full + 1;    // dv's accumulator has been read
   uint64_t* done = r_free + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
@@ -689,15 +791,16 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       mbar_init(&full2[s], 1);
       mbar_init(&empty2[s], 1);
     }
-    mbar_init(afull, 1);
+    mbar_init(a_full, 1);
+    mbar_init(a_empty, 1);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
     mbar_init(dp_full, 1);
-    mbar_init(&p_ready[0], 256);
-    mbar_init(&p_ready[1], 256);
-    mbar_init(ds_ready, 256);
+    mbar_init(&p_ready[0], 8);
+    mbar_init(&p_ready[1], 8);
+    mbar_init(ds_ready, 8);
     mbar_init(r_full, 1);
-    mbar_init(r_free, 128);
+    mbar_init(r_free, 4);
     mbar_init(done, 1);
     *failed = 0;
     fence_mbar_init();
@@ -711,88 +814,112 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // columns: S (two buffers), dP, then the results (dq; dk, dv)
-  const uint32_t t_dp = tmem + 2 * KN, t_r1 = tmem + 3 * KN, t_r2 = t_r1 + DP;
-
   const int np = c.B * c.Hk;
-  const int mtile = blockIdx.x % d.mtiles, pr = blockIdx.x / d.mtiles % np, sp = blockIdx.x / d.mtiles / np;
-  const int b = pr / c.Hk, hk = pr % c.Hk;
-  const int len = key_count(c.len, c.len64, c.len_s, c.Tk, b);
-  const int cols = KV ? c.M : len;                  // columns of the walk
-  const int rows = KV ? len : c.M;                  // rows with work
-  int all = (cols + KN - 1) / KN;
-  if (mtile * 128 >= rows || len == 0) all = 0;
-  const int per = (all + d.splits - 1) / d.splits;
-  const int j0 = min(all, sp * per), n = min(all, j0 + per) - j0;
+  // tensor-memory columns: S (two buffers), dP, then the results (dq; dk, dv)
 
   if (warp >= 8) {
     give_registers<KV ? 56 : 88>();
-    if (warp == 9 && lane == 0 && n > 0) {  // TMA
-      mbar_arrive_expect_tx(afull, 2 * S::a_bytes);
-      load_planes<DP, 128>(sa1, &ma1, d.a1, pr * d.a1.rows_p + mtile * 128, afull);
-      load_planes<DP, 128>(sa2, &ma2, d.a2, pr * d.a2.rows_p + mtile * 128, afull);
-      int i1 = 0, i2 = 0;
-      for (int j = 0; j < n; ++j) {
-        const int row = pr * d.b1.rows_p + (j0 + j) * KN;
-        const int s1 = j % N1, s2 = j % N2;
-        if (j >= N1 && !wait_or_fail(&empty1[s1], (uint32_t)(j / N1 - 1) & 1u, failed)) break;
-        mbar_arrive_expect_tx(&full1[s1], kSlot);
-        load_planes<DP, KN>(ring1 + s1 * kSlot, &mb1, d.b1, row, &full1[s1]);
-        ++i1;
-        if (j >= N2 && !wait_or_fail(&empty2[s2], (uint32_t)(j / N2 - 1) & 1u, failed)) break;
-        mbar_arrive_expect_tx(&full2[s2], kSlot);
-        load_planes<DP, KN>(ring2 + s2 * kSlot, &mb2, d.b2, row, &full2[s2]);
-        ++i2;
+    if (warp == 9 && lane == 0) {  // TMA
+      int t = 0, i2 = 0, ai = 0;   // column tiles of either operand and row tiles loaded so far
+      bool ok = true;
+      for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+        const BwdItem w = bwd_item<KN, KV>(d, item);
+        if (w.n == 0) continue;
+        if (ai > 0 && !(ok = wait_or_fail(a_empty, (uint32_t)(ai - 1) & 1u, failed))) break;
+        mbar_arrive_expect_tx(a_full, 2 * S::a_bytes);
+        load_planes<DP, 128>(sa1, &ma1, d.a1, w.pr * d.a1.rows_p + w.mtile * 128, a_full);
+        load_planes<DP, 128>(sa2, &ma2, d.a2, w.pr * d.a2.rows_p + w.mtile * 128, a_full);
+        ++ai;
+        for (int j = 0; j < w.n; ++j) {
+          const int row = w.pr * d.b1.rows_p + (w.j0 + j) * KN;
+          const int s1 = t % N1, s2 = t % N2;
+          if (t >= N1 && !(ok = wait_or_fail(&empty1[s1], (uint32_t)(t / N1 - 1) & 1u, failed))) break;
+          mbar_arrive_expect_tx(&full1[s1], kSlot);
+          load_planes<DP, KN>(ring1 + s1 * kSlot, &mb1, d.b1, row, &full1[s1]);
+          ++t;
+          if (i2 >= N2 && !(ok = wait_or_fail(&empty2[s2], (uint32_t)(i2 / N2 - 1) & 1u, failed))) break;
+          mbar_arrive_expect_tx(&full2[s2], kSlot);
+          load_planes<DP, KN>(ring2 + s2 * kSlot, &mb2, d.b2, row, &full2[s2]);
+          ++i2;
+        }
       }
-      if (i2 < n) {
-        mbar_wait(afull, 0);
-        drain(full1, N1, i1);
+      if (!ok) {
+        if (ai > 0) mbar_wait(a_full, (uint32_t)(ai - 1) & 1u);
+        drain(full1, N1, t);
         drain(full2, N2, i2);
       }
-    }
-    if (warp == 8 && n > 0) {  // MMA: the warp stays whole, one lane issues
+    } else if (warp == 8) {  // MMA: the warp stays whole, one lane issues
       const uint32_t lead = elect_lane(), tm = uniform(tmem);
       const uint32_t d1 = uniform(rows_desc(sa1)), d2 = uniform(rows_desc(sa2));
       const uint32_t r1 = uniform(rows_desc(ring1)), r2 = uniform(rows_desc(ring2));
       const uint32_t c1 = uniform(cols_desc<KN>(ring1)), c2 = uniform(cols_desc<KN>(ring2));
       constexpr uint32_t SLOT = kSlot / 16;
       const uint32_t dpc = tm + 2 * KN, rc1 = tm + 3 * KN, rc2 = rc1 + DP;
-      auto all_ok = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-      auto s_mma = [&](int j) {
-        if (!all_ok(wait_or_fail(&full1[j % N1], (uint32_t)(j / N1) & 1u, failed))) return false;
-        tc_fence_after();
-        mma_abt<DP, KN>(lead, tm + (j & 1) * KN, d1, r1 + j % N1 * SLOT);
-        umma_commit(lead, &s_full[j & 1]);
-        return true;
+      auto wait_all = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, spin_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
       };
-      auto dp_mma = [&](int j) {
-        if (!all_ok(wait_or_fail(&full2[j % N2], (uint32_t)(j / N2) & 1u, failed))) return false;
-        tc_fence_after();
-        mma_abt<DP, KN>(lead, dpc, d2, r2 + j % N2 * SLOT);
+      // t: column tiles of all items so far, which the slots and phases go by
+      auto s_ready = [&](int t) { return wait_all(&full1[t % N1], t / N1); };
+      auto dp_ready = [&](int t) { return wait_all(&full2[t % N2], t / N2); };
+      auto s_mma = [&](int t) {
+        mma_abt<DP, KN>(lead, tm + (t & 1) * KN, d1, r1 + t % N1 * SLOT);
+        umma_commit(lead, &s_full[t & 1]);
+      };
+      auto dp_mma = [&](int t) {
+        mma_abt<DP, KN>(lead, dpc, d2, r2 + t % N2 * SLOT);
         umma_commit(lead, dp_full);
-        if (!KV) umma_commit(lead, &empty2[j % N2]);
-        return true;
       };
-      auto wait_all = [&](uint64_t* bar, int phase) { return all_ok(wait_or_fail(bar, (uint32_t)phase & 1u, failed)); };
-      bool ok = wait_all(afull, 0) && s_mma(0) && dp_mma(0);
-      if (S::ahead && ok && n > 1) ok = s_mma(1);
-      for (int j = 0; j < n && ok; ++j) {
-        if (KV) {
-          ok = wait_all(&p_ready[j & 1], j >> 1) && (j == 0 || wait_all(r_free, j - 1));
-          if (!ok) break;
-          tc_fence_after();
-          mma_ab<DP, KN>(lead, rc2, tm + (j & 1) * KN, c2 + j % N2 * SLOT);  // P^T dout
-          umma_commit(lead, &empty2[j % N2]);
-        }
-        if (!S::ahead && j + 1 < n && !(ok = s_mma(j + 1))) break;
-        if (!(ok = wait_all(ds_ready, j))) break;
+      int t0 = 0, ai = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+        const int n = bwd_item<KN, KV>(d, item).n;
+        if (n == 0) continue;
+        ok = wait_all(a_full, ai) && s_ready(t0) && dp_ready(t0);
+        if (!ok) break;
+        ++ai;
         tc_fence_after();
-        if (DS_IN_S && j + 1 < n && !(ok = dp_mma(j + 1))) break;
-        mma_ab<DP, KN>(lead, rc1, DS_IN_S ? tm + (j & 1) * KN : dpc, c1 + j % N1 * SLOT);  // dS k, or dS^T q
-        umma_commit(lead, &empty1[j % N1]);
-        umma_commit(lead, r_full);
-        if (!DS_IN_S && j + 1 < n && !(ok = dp_mma(j + 1))) break;
-        if (S::ahead && j + 2 < n) ok = s_mma(j + 2);
+        s_mma(t0);
+        dp_mma(t0);
+        if (!KV) umma_commit(lead, &empty2[t0 % N2]);
+        if (S::ahead && n > 1) {
+          if (!(ok = s_ready(t0 + 1))) break;
+          s_mma(t0 + 1);
+        }
+        if (n == 1) umma_commit(lead, a_empty);
+        for (int j = 0; j < n; ++j) {
+          const int t = t0 + j;
+          const bool more = j + 1 < n, more2 = S::ahead && j + 2 < n;
+          if (S::ahead && more && !(ok = dp_ready(t + 1))) break;  // on its way long since
+          if (KV) {
+            ok = wait_all(&p_ready[t & 1], t >> 1) && (t == 0 || wait_all(r_free, t - 1));
+            if (!ok) break;
+            tc_fence_after();
+            mma_ab<DP, KN>(lead, rc2, tm + (t & 1) * KN, c2 + t % N2 * SLOT);  // P^T dout
+            umma_commit(lead, &empty2[t % N2]);
+          }
+          if (!S::ahead && more) {
+            if (!(ok = s_ready(t + 1))) break;
+            s_mma(t + 1);
+          }
+          if (!(ok = wait_all(ds_ready, t))) break;
+          tc_fence_after();
+          if (DS_IN_S && more) dp_mma(t + 1);
+          mma_ab<DP, KN>(lead, rc1, DS_IN_S ? tm + (t & 1) * KN : dpc, c1 + t % N1 * SLOT);  // dS k, or dS^T q
+          if (!KV && S::ahead && more) umma_commit(lead, &empty2[(t + 1) % N2]);
+          umma_commit(lead, r_full);
+          umma_commit(lead, &empty1[t % N1]);
+          if (!DS_IN_S && more) {
+            if (!S::ahead && !(ok = dp_ready(t + 1))) break;
+            dp_mma(t + 1);
+            if (!KV) umma_commit(lead, &empty2[(t + 1) % N2]);
+          }
+          if (more2) {
+            if (!(ok = s_ready(t + 2))) break;
+            s_mma(t + 2);
+          }
+          if (j + 2 == n) umma_commit(lead, a_empty);
+        }
+        t0 += n;
       }
       if (!ok) {
         umma_commit(lead, done);
@@ -801,168 +928,208 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
     }
   } else {
     take_registers<KV ? 56 : 88>();
-    const int wg = warp / 4;
-    const int row = mtile * 128 + (warp % 4) * 32 + lane;
+    const int wg = warp / 4, rl = (warp % 4) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t t_dp = tmem + lanes + 2 * KN + wg * HC;
+    // wg 0 of (dk, dv) takes dv, wg 1 dk; of dq each takes half of the columns
+    const uint32_t t_res = tmem + lanes + 3 * KN + (KV ? (wg == 0 ? DP : 0) : wg * AC);
     const int at1 = d.a1.rows_p / KN, bt = d.b1.rows_p / KN;
-    const float ia1 = d.a1.inv[pr * at1 + row / KN], ia2 = d.a2.inv[pr * at1 + row / KN];
-    const float* ib1 = d.b1.inv + pr * bt + j0;
-    const float* ib2 = d.b2.inv + pr * bt + j0;
-    const float* nb2 = d.b2.norm + pr * bt + j0;
-    // per query row: of this row (dq) or of the columns (dk, dv)
-    const int64_t qrow = (int64_t)pr * (KV ? d.b1.rows_p : d.a1.rows_p) + (KV ? j0 * KN + wg * HC : row);
-    const float r_bias = KV ? 0.f : d.bias[qrow] - 15.f, r_delta = KV ? 0.f : d.delta[qrow];
-    const float r_norm = KV ? d.a2.norm[pr * at1 + row / KN] : d.rnorm[qrow];
-    const float* dmax = KV ? d.dmax + pr * bt + j0 : nullptr;
-    float acc[AC];
-#pragma unroll
-    for (int i = 0; i < AC; ++i) acc[i] = 0.f;
-    float ds_down = 0.f;  // what the dS of the last tile was divided by, undone
+    int t = 0;  // column tiles so far
     bool ok = true;
-    auto add_result = [&](int j) {  // tile j's result into registers: wg 0 of (dk, dv) takes dv
-      const bool here = wait_or_fail(r_full, (uint32_t)j & 1u, failed);
-      if (!__all_sync(0xffffffffu, here)) return false;
-      tc_fence_after();
-      const float w = KV ? (wg == 0 ? ib2[j] * 0x1p-15f : ib1[j] * d.out_scale * ds_down) : ib1[j] * d.out_scale * ds_down;
-      const uint32_t src = KV ? (wg == 0 ? t_r2 : t_r1) : t_r1 + wg * AC;
-      const uint64_t w2 = pack2(w, w);
+    for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+      int n, kt, limit;  // column tiles, the first one's index among all, columns of this half from it on
+      int64_t qrow;      // per query row: of this row (dq) or of the columns (dk, dv)
+      float ia1, ia2, r_norm;
+      {
+        const BwdItem w = bwd_item<KN, KV>(d, item);
+        n = w.n;
+        kt = w.pr * bt + w.j0;
+        limit = w.cols - w.j0 * KN - wg * HC;
+        const int row = w.mtile * 128 + rl;
+        ia1 = d.f * d.a1.inv[w.pr * at1 + row / KN];
+        ia2 = d.a2.inv[w.pr * at1 + row / KN];
+        qrow = (int64_t)w.pr * (KV ? d.b1.rows_p : d.a1.rows_p) + (KV ? w.j0 * KN + wg * HC : row);
+        r_norm = KV ? d.a2.norm[w.pr * at1 + row / KN] : d.rnorm[qrow];
+      }
+      const float r_bias = KV ? 0.f : d.bias[qrow] - 15.f, r_delta = KV ? 0.f : d.delta[qrow];
+      float acc[AC];
 #pragma unroll
-      for (int cc = 0; cc < AC / 32; ++cc) {
-        uint32_t o[32];
-        tmem_ld32_issue(src + lanes + cc * 32, o);
-        tmem_ld_done(o);
+      for (int i = 0; i < AC; ++i) acc[i] = 0.f;
+      float ds_down = 0.f;  // what the dS of the last tile was divided by, undone
+      // what tile j's result is multiplied by
+      auto weight = [&](int j) {
+        if (KV && wg == 0) return d.b2.inv[kt + j] * 0x1p-15f;
+        return d.b1.inv[kt + j] * d.out_scale * ds_down;
+      };
+      auto add_chunk = [&](int cc, const uint32_t (&o)[32], uint64_t w2) {
 #pragma unroll
         for (int i = 0; i < 32; i += 2)
           unpack2(fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), w2,
                        pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1])),
                   &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
-      }
-      tc_fence_before();
-      if (KV && wg == 0) mbar_arrive(r_free);
-      return true;
-    };
-    for (int j = 0; j < n; ++j) {
-      const int limit = cols - (j0 + j) * KN - wg * HC;  // columns of this warpgroup's half
-      const float f = d.f * ia1 * ib1[j];
-      const uint32_t sb = tmem + lanes + (j & 1) * KN + wg * HC, db = t_dp + lanes + wg * HC;
-      float p[HC];  // the exponent's bias, then P (dk, dv: P 2^15)
-      if (KV) {
-        const float4* bi = reinterpret_cast<const float4*>(d.bias + qrow + j * KN);
+      };
+      auto wait_warp = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, wait_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
+      };
+      for (int j = 0; j < n; ++j, ++t, limit -= KN) {
+        const float f = ia1 * d.b1.inv[kt + j];
+        const uint32_t sb = tmem + lanes + (t & 1) * KN + wg * HC;
+        float p[HC];  // the exponent's bias, then P (dk, dv: P 2^15)
+        if (KV) {
+          const float4* bi = reinterpret_cast<const float4*>(d.bias + qrow + j * KN);
 #pragma unroll
-        for (int i = 0; i < HC / 4; ++i) {
-          const float4 x = __ldg(bi + i);
-          p[4 * i] = x.x;
-          p[4 * i + 1] = x.y;
-          p[4 * i + 2] = x.z;
-          p[4 * i + 3] = x.w;
+          for (int i = 0; i < HC / 4; ++i) {
+            const float4 x = __ldg(bi + i);
+            p[4 * i] = x.x;
+            p[4 * i + 1] = x.y;
+            p[4 * i + 2] = x.z;
+            p[4 * i + 3] = x.w;
+          }
         }
-      }
-      ok = wait_or_fail(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, failed);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      const uint64_t f2 = pack2(f, f);
+        if (!(ok = wait_warp(&s_full[t & 1], t >> 1))) break;
+        tc_fence_after();
+        const uint64_t f2 = pack2(f, f);
+        {
+          uint32_t a[HC / 32][32];
 #pragma unroll
-      for (int cc = 0; cc < HC / 32; ++cc) {
-        uint32_t a[32];
-        tmem_ld32_issue(sb + cc * 32, a);
-        tmem_ld_done(a);
+          for (int cc = 0; cc < HC / 32; ++cc) tmem_ld32_issue(sb + cc * 32, a[cc]);
+          tmem_ld_done(a[0]);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float& p0 = p[cc * 32 + i];
-          float& p1 = p[cc * 32 + i + 1];
-          const uint64_t bias = KV ? pack2(p0, p1) : pack2(r_bias, r_bias);
-          unpack2(fma2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), f2, bias), &p0, &p1);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
+          for (int cc = 1; cc < HC / 32; ++cc) tmem_ld_tie(a[cc]);
+#pragma unroll
+          for (int cc = 0; cc < HC / 32; ++cc) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float& p0 = p[cc * 32 + i];
+              float& p1 = p[cc * 32 + i + 1];
+              const uint64_t bias = KV ? pack2(p0, p1) : pack2(r_bias, r_bias);
+              unpack2(fma2(pack2(__uint_as_float(a[cc][i]), __uint_as_float(a[cc][i + 1])), f2, bias), &p0, &p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
+            if (KV) {
+              uint32_t w[32];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) split2(pack2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1]), &w[i], &w[16 + i]);
+              tmem_st32(sb + cc * 32, w);
+            }
+          }
         }
         if (KV) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) split2(pack2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1]), &w[i], &w[16 + i]);
-          tmem_st32(sb + cc * 32, w);
+          tmem_st_done();
+          tc_fence_before();
+          warp_arrive(&p_ready[t & 1]);
         }
-      }
-      if (KV) {
+        // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below 2^15
+        const float g = ia2 * d.b2.inv[kt + j];
+        const float bound = __fmaf_rn(r_norm * d.b2.norm[kt + j], g, KV ? d.dmax[kt + j] : fabsf(r_delta));
+        uint32_t eb = __float_as_uint(bound) >> 23;
+        eb = eb < 15u ? 15u : eb;
+        const float up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);
+        const uint64_t gu = pack2(g * up, g * up), nup = pack2(-up, -up), ndu = pack2(-r_delta * up, -r_delta * up);
+        if (!(ok = wait_warp(dp_full, t))) break;
+        // the last tile's results: for (dk, dv) complete before this dP was
+        // issued; for dq behind it, and read at the end
+        if (KV && j > 0 && !(ok = wait_warp(r_full, t - 1))) break;
+        tc_fence_after();
+        const float wt = j > 0 ? weight(j - 1) : 0.f;
+        const uint64_t w2 = pack2(wt, wt);
+        if (KV && j > 0) {
+#pragma unroll
+          for (int cc = 0; cc < AC / 32; ++cc) {
+            uint32_t o[32];
+            tmem_ld32_issue(t_res + cc * 32, o);
+            tmem_ld_done(o);
+            add_chunk(cc, o, w2);
+          }
+          tc_fence_before();
+          if (wg == 0) warp_arrive(r_free);
+        }
+#pragma unroll
+        for (int cc = 0; cc < HC / 32; ++cc) {
+          uint32_t a[32], o[32], w[32];
+          float4 dl[8];
+          if (KV) {
+            const float4* de = reinterpret_cast<const float4*>(d.delta + qrow + j * KN + cc * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dl[i] = __ldg(de + i);
+          }
+          tmem_ld32_issue(t_dp + cc * 32, a);
+          tmem_ld_done(a);
+          const bool part = !KV && limit < (cc + 1) * 32;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float4& q = dl[i / 2];
+            const uint64_t nd = KV ? mul2(i % 2 ? pack2(q.z, q.w) : pack2(q.x, q.y), nup) : ndu;
+            uint64_t x = mul2(pack2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1]),
+                              fma2(pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), gu, nd));
+            if (part) {
+              float x0, x1;
+              unpack2(x, &x0, &x1);
+              x = pack2(cc * 32 + 2 * i < limit ? x0 : 0.f, cc * 32 + 2 * i + 1 < limit ? x1 : 0.f);
+            }
+            split2(x, &w[i], &w[16 + i]);
+          }
+          tmem_st32((DS_IN_S ? sb : t_dp) + cc * 32, w);
+        }
+        if (!KV && j > 0) {
+          if (!(ok = wait_warp(r_full, t - 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int cc = 0; cc < AC / 32; ++cc) {
+            uint32_t o[32];
+            tmem_ld32_issue(t_res + cc * 32, o);
+            tmem_ld_done(o);
+            add_chunk(cc, o, w2);
+          }
+        }
+        ds_down = __uint_as_float((eb - 14u) << 23);
         tmem_st_done();
         tc_fence_before();
-        mbar_arrive(&p_ready[j & 1]);
+        warp_arrive(ds_ready);
       }
-      // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below 2^15
-      const float g = ia2 * ib2[j];
-      const float bound = __fmaf_rn(r_norm * nb2[j], g, KV ? dmax[j] : fabsf(r_delta));
-      uint32_t eb = __float_as_uint(bound) >> 23;
-      eb = eb < 15u ? 15u : eb;
-      const float up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);
-      const uint64_t gu = pack2(g * up, g * up), nup = pack2(-up, -up), ndu = pack2(-r_delta * up, -r_delta * up);
-      ok = wait_or_fail(dp_full, (uint32_t)j & 1u, failed);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      if (KV && j > 0) {
-        ok = add_result(j - 1);
-        if (!ok) break;
-      }
-      if (KV) ds_down = __uint_as_float((eb - 14u) << 23);
+      if (!ok) break;
+      if (n > 0) {
+        if (!(ok = wait_warp(r_full, t - 1))) break;
+        tc_fence_after();
+        const float wt = weight(n - 1);
 #pragma unroll
-      for (int cc = 0; cc < HC / 32; ++cc) {
-        float4 dl[8];
-        if (KV) {
-          const float4* de = reinterpret_cast<const float4*>(d.delta + qrow + j * KN + cc * 32);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dl[i] = __ldg(de + i);
+        for (int cc = 0; cc < AC / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32_issue(t_res + cc * 32, o);
+          tmem_ld_done(o);
+          add_chunk(cc, o, pack2(wt, wt));
         }
-        uint32_t a[32], w[32];
-        tmem_ld32_issue(db + cc * 32, a);
-        tmem_ld_done(a);
-        const bool part = !KV && limit < (cc + 1) * 32;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float4& q = dl[i / 2];
-          const uint64_t nd = KV ? mul2(i % 2 ? pack2(q.z, q.w) : pack2(q.x, q.y), nup) : ndu;
-          uint64_t x = mul2(pack2(p[cc * 32 + 2 * i], p[cc * 32 + 2 * i + 1]),
-                            fma2(pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), gu, nd));
-          if (part) {
-            float x0, x1;
-            unpack2(x, &x0, &x1);
-            x = pack2(cc * 32 + 2 * i < limit ? x0 : 0.f, cc * 32 + 2 * i + 1 < limit ? x1 : 0.f);
-          }
-          split2(x, &w[i], &w[16 + i]);
-        }
-        tmem_st32((DS_IN_S ? sb : db) + cc * 32, w);
+        tc_fence_before();
+        if (KV && wg == 0) warp_arrive(r_free);
       }
-      tmem_st_done();
-      if (!KV && j > 0) {
-        ok = add_result(j - 1);
-        if (!ok) break;
-      }
-      if (!KV) ds_down = __uint_as_float((eb - 14u) << 23);
-      tc_fence_before();
-      mbar_arrive(ds_ready);
-    }
-    if (ok && n > 0) ok = add_result(n - 1);
-    const int stored = KV ? c.Tk : c.M;  // rows of the result; those without work hold zeros
-    if (ok && row < stored) {
-      const bool live = row < rows;
-      if (d.splits > 1) {
-        float* pp = (KV && wg == 0 ? d.part2 : d.part1) + (((int64_t)sp * np + pr) * d.a1.rows_p + row) * DP + (KV ? 0 : wg * AC);
+      const BwdItem w = bwd_item<KN, KV>(d, item);
+      const int row = w.mtile * 128 + rl;
+      const int stored = KV ? c.Tk : c.M;  // rows of the result; those without work hold zeros
+      if (row < stored) {
+        const bool live = row < w.rows;
+        if (d.splits > 1) {
+          float* pp = (KV && wg == 0 ? d.part2 : d.part1) + (((int64_t)w.sp * np + w.pr) * d.a1.rows_p + row) * DP + (KV ? 0 : wg * AC);
 #pragma unroll
-        for (int i = 0; i < AC / 4; ++i)
-          reinterpret_cast<float4*>(pp)[i] = live ? make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3])
-                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-      } else {
-        const HeadsDev& o = KV ? (wg == 0 ? c.dv : c.dk) : c.dq;
-        const int g = KV ? 0 : (int)fdiv((uint32_t)row, c.f_Tq), t = KV ? row : row - g * c.Tq;
-        const int h = KV ? hk : hk * c.G + g, c0 = KV ? 0 : wg * AC;
-        float* op = static_cast<float*>(o.p) + b * o.sb + t * o.st + h * o.sh;
+          for (int i = 0; i < AC / 4; ++i)
+            reinterpret_cast<float4*>(pp)[i] = live ? make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3])
+                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          const HeadsDev& o = KV ? (wg == 0 ? c.dv : c.dk) : c.dq;
+          const int g = KV ? 0 : (int)fdiv((uint32_t)row, c.f_Tq), tt = KV ? row : row - g * c.Tq;
+          const int h = KV ? w.hk : w.hk * c.G + g, c0 = KV ? 0 : wg * AC;
+          float* op = static_cast<float*>(o.p) + w.b * o.sb + tt * o.st + h * o.sh;
 #pragma unroll
-        for (int i = 0; i < AC; i += 4) {
-          const float4 x = live ? make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-          if (c.vec) {
-            if (c0 + i < c.D) *reinterpret_cast<float4*>(op + c0 + i) = x;
-          } else {
-            if (c0 + i < c.D) op[(c0 + i) * o.sd] = x.x;
-            if (c0 + i + 1 < c.D) op[(c0 + i + 1) * o.sd] = x.y;
-            if (c0 + i + 2 < c.D) op[(c0 + i + 2) * o.sd] = x.z;
-            if (c0 + i + 3 < c.D) op[(c0 + i + 3) * o.sd] = x.w;
+          for (int i = 0; i < AC; i += 4) {
+            const float4 x = live ? make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c.vec) {
+              if (c0 + i < c.D) *reinterpret_cast<float4*>(op + c0 + i) = x;
+            } else {
+              if (c0 + i < c.D) op[(c0 + i) * o.sd] = x.x;
+              if (c0 + i + 1 < c.D) op[(c0 + i + 1) * o.sd] = x.y;
+              if (c0 + i + 2 < c.D) op[(c0 + i + 2) * o.sd] = x.z;
+              if (c0 + i + 3 < c.D) op[(c0 + i + 3) * o.sd] = x.w;
+            }
           }
         }
       }
@@ -1106,7 +1273,9 @@ Error launch_forward(const Packed& q, const Packed& k, const Packed& v, FwdDev& 
   using S = FwdShape<DP, MT>;
   auto kern = cross_forward_kernel<DP, MT>;
   allow_smem((const void*)kern, S::smem);
-  kern<<<(unsigned)(f.mtiles * f.c.B * f.c.Hk * f.splits), S::threads, S::smem, stream>>>(q.map128, k.mapKN, v.mapKN, f);
+  f.items = f.mtiles * f.c.B * f.c.Hk * f.splits;
+  kern<<<(unsigned)std::min(f.items, current_device_info().sm_count), S::threads, S::smem, stream>>>(q.map128, k.mapKN,
+                                                                                                 v.mapKN, f);
   return check_launch("cross attention forward kernel");
 }
 
@@ -1116,8 +1285,9 @@ Error launch_backward(const Packed& a1, const Packed& a2, const Packed& b1, cons
   using S = BwdShape<DP>;
   auto kern = cross_backward_kernel<DP, KV>;
   allow_smem((const void*)kern, S::smem);
-  kern<<<(unsigned)(f.mtiles * f.c.B * f.c.Hk * f.splits), S::threads, S::smem, stream>>>(a1.map128, a2.map128, b1.mapKN,
-                                                                                       b2.mapKN, f);
+  f.items = f.mtiles * f.c.B * f.c.Hk * f.splits;
+  kern<<<(unsigned)std::min(f.items, current_device_info().sm_count), S::threads, S::smem, stream>>>(
+      a1.map128, a2.map128, b1.mapKN, b2.mapKN, f);
   return check_launch(KV ? "cross attention key gradient kernel" : "cross attention query gradient kernel");
 }
 
