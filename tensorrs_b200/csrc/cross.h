@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "heads.h"
 #include "kernels.cuh"
@@ -33,7 +34,7 @@ struct CrossDev {
   int M;                         // G * Tq
   FastDiv f_Tq;
   float scale;
-  const int* nonfinite;          // when set: run only if *nonfinite != 0
+  const int* nonfinite;          // tensor-core paths: set when an input holds an infinity or a NaN
   int vec;                       // q, k, v (and the outputs) take 16-byte accesses
 };
 
@@ -52,9 +53,32 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The tensor-core paths (head sizes up to 128).  They leave *nonfinite set
-// when an input holds an infinity, a NaN or a value the split cannot carry.
-Error cross_tc_forward(const CrossDev& d, int* nonfinite, cudaStream_t stream);
-Error cross_tc_backward(const CrossDev& d, int* nonfinite, cudaStream_t stream);
+// A launch that may be scheduled while the stream's previous kernel still runs
+// (programmatic dependent launch): the kernel waits for that one with
+// pdl_wait() before it touches anything the other writes.
+template <class... A>
+inline Error launch_after(void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t stream, const char* what,
+                          const std::common_type_t<A>&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_error(e, what);
+  }
+  return check_launch(what);
+}
+
+// The tensor-core paths (head sizes up to 128).
+Error cross_tc_forward(const CrossDev& d, cudaStream_t stream);
+Error cross_tc_backward(const CrossDev& d, cudaStream_t stream);
 
 }  // namespace trs

@@ -9,8 +9,8 @@
 // keys gives 0, lse = -inf and no gradient.
 //
 // cross_rows_kernel serves few query rows per key head (single tokens), where
-// reading k and v once is all there is to do, and, looping over blocks of
-// rows, head sizes above 128 and inputs that hold infinities or NaNs.  A CTA
+// reading k and v once is all there is to do, and, in blocks of rows, head
+// sizes above 128.  A CTA
 // owns (problem, block of NR rows, part of the keys): groups of L lanes own
 // one key at a time, each lane 4 (8) elements of the head; 4 keys are in
 // flight per group, the dot products fold over the group with shuffles, and
@@ -23,6 +23,7 @@
 
 #include "../../include/trs.h"
 #include "cross.h"
+#include "cross_exact.cuh"
 
 namespace trs {
 namespace {
@@ -35,7 +36,8 @@ struct RowsDev {
   int blocks;        // blocks of NR rows per problem
   int splits;        // parts of the keys
   int items;         // problems * blocks * splits
-  float* part;       // [split][problem][M][D] and then m, l [split][problem][M], when splits > 1
+  int ld;            // elements per partial row: the head size, rounded up to 4
+  float* part;       // [split][problem][M][ld] and then m, l [split][problem][M], when splits > 1
   float* part_m;
   float* part_l;
 };
@@ -61,7 +63,7 @@ __device__ __forceinline__ float dot4(const float4& a, const float4& b, float s)
 template <int NR, int L, int NV, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) cross_rows_kernel(const RowsDev d) {
   const CrossDev& c = d.c;
-  if (c.nonfinite && *(volatile const int*)c.nonfinite == 0) return;
+  pdl_launch_dependents();
   constexpr int U = 4;                                  // keys in flight per group
   constexpr int NG = kRowsThreads / L;                  // groups
   constexpr int DP = L * 4 * NV;                        // padded head size
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(kRowsThreads) cross_rows_kernel(const RowsDev 
       }
       if (d.splits > 1) {
         const int64_t at = ((int64_t)sp * (c.B * c.Hk) + pr) * c.M + row;
-        d.part[at * c.D + dd] = o;
+        d.part[at * d.ld + dd] = o;
         if (dd == 0) {
           d.part_m[at] = mx;
           d.part_l[at] = sum;
@@ -193,42 +195,62 @@ __global__ void __launch_bounds__(kRowsThreads) cross_rows_kernel(const RowsDev 
   }
 }
 
-// The parts of the keys joined in order: one warp per (problem, row).
+// The parts of the keys joined in order: one warp per (problem, row), 4
+// elements per lane and step, 8 parts' loads in flight.
 struct JoinDev {
   CrossDev c;
   int splits, rows;          // rows per problem in the partials
-  int ld;                    // elements per partial row
+  int ld;                    // elements per partial row, a multiple of 4
   const float *part, *part_m, *part_l;
 };
-__global__ void __launch_bounds__(256) cross_join_kernel(const JoinDev d) {
+__global__ void __launch_bounds__(128) cross_join_kernel(const JoinDev d) {
+  pdl_wait();
   const CrossDev& c = d.c;
-  const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (c.nonfinite && *(volatile const int*)c.nonfinite != 0) return;  // the result is there already
+  const int64_t w = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   const int np = c.B * c.Hk;
   if (w >= (int64_t)np * c.M) return;
   const int pr = (int)(w / c.M), row = (int)(w % c.M);
+  const int64_t step = (int64_t)np * d.rows, first = (int64_t)pr * d.rows + row;
   float mx = -INFINITY;
-  for (int s = lane; s < d.splits; s += 32) mx = fmaxf(mx, d.part_m[((int64_t)s * np + pr) * d.rows + row]);
+  for (int s = lane; s < d.splits; s += 32) mx = fmaxf(mx, d.part_m[s * step + first]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float base = mx == -INFINITY ? 0.f : mx;
-  float sum = 0.f, acc[kRowsMaxHead / 32];
+  float sum = 0.f;
+  for (int s = lane; s < d.splits; s += 32) sum = __fmaf_rn(ex2(d.part_m[s * step + first] - base), d.part_l[s * step + first], sum);
 #pragma unroll
-  for (int i = 0; i < kRowsMaxHead / 32; ++i) acc[i] = 0.f;
-  for (int s = 0; s < d.splits; ++s) {
-    const int64_t at = ((int64_t)s * np + pr) * d.rows + row;
-    const float wt = ex2(d.part_m[at] - base);
-    sum = __fmaf_rn(wt, d.part_l[at], sum);
-#pragma unroll
-    for (int i = 0; i < kRowsMaxHead / 32; ++i)
-      if (lane + 32 * i < c.D) acc[i] = __fmaf_rn(wt, d.part[at * d.ld + lane + 32 * i], acc[i]);
-  }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const int b = pr / c.Hk, hk = pr % c.Hk;
   const int g = (int)fdiv((uint32_t)row, c.f_Tq), t = row - g * c.Tq, h = hk * c.G + g;
   float* op = static_cast<float*>(c.out.p) + b * c.out.sb + t * c.out.st + h * c.out.sh;
+  for (int e = lane * 4; e < c.D; e += 128) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < d.splits; s0 += 8) {
+      float4 x[8];
+      float wt[8];
 #pragma unroll
-  for (int i = 0; i < kRowsMaxHead / 32; ++i)
-    if (lane + 32 * i < c.D) op[(lane + 32 * i) * c.out.sd] = sum == 0.f ? 0.f : acc[i] / sum;
+      for (int k = 0; k < 8; ++k) {
+        const bool on = s0 + k < d.splits;
+        const int64_t at = (s0 + k) * step + first;
+        x[k] = on ? *reinterpret_cast<const float4*>(d.part + at * d.ld + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        wt[k] = on ? ex2(d.part_m[at] - base) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        acc.x = __fmaf_rn(wt[k], x[k].x, acc.x);
+        acc.y = __fmaf_rn(wt[k], x[k].y, acc.y);
+        acc.z = __fmaf_rn(wt[k], x[k].z, acc.z);
+        acc.w = __fmaf_rn(wt[k], x[k].w, acc.w);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    op[e * c.out.sd] = acc.x * inv;
+    if (e + 1 < c.D) op[(e + 1) * c.out.sd] = acc.y * inv;
+    if (e + 2 < c.D) op[(e + 2) * c.out.sd] = acc.z * inv;
+    if (e + 3 < c.D) op[(e + 3) * c.out.sd] = acc.w * inv;
+  }
   if (lane == 0 && c.lse) c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
@@ -245,99 +267,16 @@ Error cross_join(const CrossDev& c, int splits, int rows, int ld, const float* p
   j.part_m = part_m;
   j.part_l = part_l;
   const int64_t warps = (int64_t)c.B * c.Hk * c.M;
-  cross_join_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(j);
-  return check_launch("cross attention join kernel");
+  return launch_after(cross_join_kernel, dim3((unsigned)((warps + 3) / 4)), 128, 0, stream, "cross attention join kernel", j);
 }
 
 namespace {
 
-// The gradient on the CUDA cores, one warp per query row (dq) or key row (dk,
-// dv): head sizes above 128 and inputs that hold infinities or NaNs.  Each
-// lane holds elements lane, lane + 32, ... of a head.
-constexpr int kGradE = kRowsMaxHead / 32;
-
-struct HeadRow {
-  float x[kGradE];
-};
-__device__ __forceinline__ HeadRow load_row(const float* p, int64_t sd, int D) {
-  HeadRow r;
-  const int lane = threadIdx.x % 32;
-#pragma unroll
-  for (int i = 0; i < kGradE; ++i) r.x[i] = lane + 32 * i < D ? p[(lane + 32 * i) * sd] : 0.f;
-  return r;
-}
-__device__ __forceinline__ void store_row(float* p, int64_t sd, int D, const HeadRow& r) {
-  const int lane = threadIdx.x % 32;
-#pragma unroll
-  for (int i = 0; i < kGradE; ++i)
-    if (lane + 32 * i < D) p[(lane + 32 * i) * sd] = r.x[i];
-}
-__device__ __forceinline__ float dot_row(const HeadRow& a, const HeadRow& b) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < kGradE; ++i) s = __fmaf_rn(a.x[i], b.x[i], s);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
-}
-__device__ __forceinline__ const float* row_of(const HeadsDev& h, int b, int t, int head) {
-  return static_cast<const float*>(h.p) + b * h.sb + t * h.st + head * h.sh;
-}
-
+// The gradient of head sizes above 128 on the CUDA cores, a warp per row.
 __global__ void __launch_bounds__(256) cross_grad_rows_kernel(const CrossDev c) {
-  if (c.nonfinite && *(volatile const int*)c.nonfinite == 0) return;
-  const int64_t warps = (int64_t)gridDim.x * 8, w0 = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  const int64_t nq = (int64_t)c.B * c.Hq * c.Tq, nk = (int64_t)c.B * c.Hk * c.Tk;
-  for (int64_t w = w0; w < nq + nk; w += warps) {
-    HeadRow z;
-#pragma unroll
-    for (int i = 0; i < kGradE; ++i) z.x[i] = 0.f;
-    if (w < nq) {  // one query: dq
-      const int t = (int)(w % c.Tq), h = (int)(w / c.Tq % c.Hq), b = (int)(w / c.Tq / c.Hq), hk = h / c.G;
-      const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
-      const HeadRow q = load_row(row_of(c.q, b, t, h), c.q.sd, c.D);
-      const HeadRow go = load_row(row_of(c.dout, b, t, h), c.dout.sd, c.D);
-      const float delta = dot_row(go, load_row(row_of(c.out, b, t, h), c.out.sd, c.D));
-      const float lse = c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t];
-      HeadRow acc = z;
-      for (int j = 0; j < n; ++j) {
-        const HeadRow k = load_row(row_of(c.k, b, j, hk), c.k.sd, c.D);
-        const float s = dot_row(q, k) * c.scale;
-        const float p = lse == -INFINITY ? 0.f : ex2((s - lse) * kLog2e);
-        const float dp = dot_row(go, load_row(row_of(c.v, b, j, hk), c.v.sd, c.D));
-        const float ds = p * (dp - delta) * c.scale;
-#pragma unroll
-        for (int i = 0; i < kGradE; ++i) acc.x[i] = __fmaf_rn(ds, k.x[i], acc.x[i]);
-      }
-      store_row(const_cast<float*>(row_of(c.dq, b, t, h)), c.dq.sd, c.D, acc);
-    } else {  // one key: dk, dv
-      const int64_t r = w - nq;
-      const int j = (int)(r % c.Tk), hk = (int)(r / c.Tk % c.Hk), b = (int)(r / c.Tk / c.Hk);
-      HeadRow ak = z, av = z;
-      if (j < key_count(c.len, c.len64, c.len_s, c.Tk, b)) {
-        const HeadRow k = load_row(row_of(c.k, b, j, hk), c.k.sd, c.D);
-        const HeadRow v = load_row(row_of(c.v, b, j, hk), c.v.sd, c.D);
-        for (int h = hk * c.G; h < (hk + 1) * c.G; ++h) {
-          for (int t = 0; t < c.Tq; ++t) {
-            const HeadRow q = load_row(row_of(c.q, b, t, h), c.q.sd, c.D);
-            const HeadRow go = load_row(row_of(c.dout, b, t, h), c.dout.sd, c.D);
-            const float delta = dot_row(go, load_row(row_of(c.out, b, t, h), c.out.sd, c.D));
-            const float lse = c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t];
-            const float s = dot_row(q, k) * c.scale;
-            const float p = lse == -INFINITY ? 0.f : ex2((s - lse) * kLog2e);
-            const float ds = p * (dot_row(go, v) - delta) * c.scale;
-#pragma unroll
-            for (int i = 0; i < kGradE; ++i) {
-              ak.x[i] = __fmaf_rn(ds, q.x[i], ak.x[i]);
-              av.x[i] = __fmaf_rn(p, go.x[i], av.x[i]);
-            }
-          }
-        }
-      }
-      store_row(const_cast<float*>(row_of(c.dk, b, j, hk)), c.dk.sd, c.D, ak);
-      store_row(const_cast<float*>(row_of(c.dv, b, j, hk)), c.dv.sd, c.D, av);
-    }
-  }
+  const int64_t warps = (int64_t)gridDim.x * 8, w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  exact_dq_rows(c, w, warps);
+  exact_dkv_rows(c, w, warps);
 }
 
 // Gradients of no queries or no keys at all.
@@ -373,7 +312,7 @@ Error launch_rows(RowsDev& d, int grid, cudaStream_t s) {
   return check_launch("cross attention rows kernel");
 }
 
-Error run_rows(const CrossDev& c, bool fallback, cudaStream_t s) {
+Error run_rows(const CrossDev& c, cudaStream_t s) {
   RowsDev d;
   std::memset(static_cast<void*>(&d), 0, sizeof(d));
   d.c = c;
@@ -386,21 +325,22 @@ Error run_rows(const CrossDev& c, bool fallback, cudaStream_t s) {
   // least (a part's fixed cost is that of about 100 keys)
   const int sms = current_device_info().sm_count;
   const int64_t base = (int64_t)np * d.blocks;
-  int64_t splits = fallback ? 1 : 4 * sms / base;
+  int64_t splits = 4 * sms / base;
   if (splits > c.Tk / 256) splits = c.Tk / 256;
   if (splits < 1) splits = 1;
   d.splits = (int)splits;
   const int64_t items = base * splits;
   if (items >= (1ll << 31)) return make_error(TRS_ERR_SHAPE, "cross_attention: too many query rows");
   d.items = (int)items;
-  const int grid = fallback ? (int)std::min<int64_t>(items, 2 * sms) : (int)std::min<int64_t>(items, 1 << 24);
+  const int grid = (int)std::min<int64_t>(items, 1 << 24);
   Scratch part;
   if (splits > 1) {
     const size_t rows = (size_t)splits * np * c.M;
-    Error e = part.alloc(sizeof(float) * rows * (c.D + 2), s);
+    d.ld = (c.D + 3) / 4 * 4;
+    Error e = part.alloc(sizeof(float) * rows * (d.ld + 2), s);
     if (!e.ok()) return e;
     d.part = part.as<float>();
-    d.part_m = d.part + rows * c.D;
+    d.part_m = d.part + rows * d.ld;
     d.part_l = d.part_m + rows;
   }
   Error e;
@@ -415,7 +355,7 @@ Error run_rows(const CrossDev& c, bool fallback, cudaStream_t s) {
                                                               : launch_rows<4, 32, 2>(d, grid, s);
   }
   if (!e.ok() || splits == 1) return e;
-  return cross_join(c, d.splits, c.M, c.D, d.part, d.part_m, d.part_l, s);
+  return cross_join(c, d.splits, c.M, d.ld, d.part, d.part_m, d.part_l, s);
 }
 
 struct CrossCall {
@@ -542,23 +482,11 @@ Error run_cross(const CrossCall& c, bool backward, cudaStream_t stream) {
   const int sms = current_device_info().sm_count;
   const bool tc = D <= 128 && (backward || d.M > 16);
   if (!tc) {
-    if (!backward) return run_rows(d, false, stream);
+    if (!backward) return run_rows(d, stream);
     cross_grad_rows_kernel<<<8 * sms, 256, 0, stream>>>(d);
     return check_launch("cross attention gradient rows kernel");
   }
-  // a word that the split kernel sets when some input is not finite; the
-  // CUDA-core kernel then runs over all of the result
-  Scratch flag;
-  e = flag.alloc(sizeof(int), stream);
-  if (!e.ok()) return e;
-  cudaError_t ce = cudaMemsetAsync(flag.get(), 0, sizeof(int), stream);
-  if (ce != cudaSuccess) return cuda_error(ce, "cudaMemsetAsync");
-  e = backward ? cross_tc_backward(d, flag.as<int>(), stream) : cross_tc_forward(d, flag.as<int>(), stream);
-  if (!e.ok()) return e;
-  d.nonfinite = flag.as<int>();
-  if (!backward) return run_rows(d, true, stream);
-  cross_grad_rows_kernel<<<2 * sms, 256, 0, stream>>>(d);
-  return check_launch("cross attention gradient rows kernel");
+  return backward ? cross_tc_backward(d, stream) : cross_tc_forward(d, stream);
 }
 
 trs_status finish(const Error& e) {

@@ -48,6 +48,7 @@
 #include <string>
 
 #include "cross.h"
+#include "cross_exact.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
@@ -72,7 +73,6 @@ struct PackSrc {
   float* inv;            // [problem][tile] 2^e
   float* norm;           // [problem][tile] largest row 2-norm, in units of 2^e; or null
   float sign;
-  int vec;
   // the output gradient's tiles also carry, per row: 15 - lse in units of log2
   // (-inf behind the last row: no weight), delta, the row's norm in units of
   // 2^e; per tile the largest |delta|
@@ -114,8 +114,9 @@ __device__ __forceinline__ float block_max(float x, float* sm) {  // 256 threads
   return x;
 }
 
-__device__ __forceinline__ float4 head4(const float* p, int d, int D, int64_t sd, bool vec) {
-  if (vec) return *reinterpret_cast<const float4*>(p + d);  // D is a multiple of 4 and d < D
+template <bool VEC>
+__device__ __forceinline__ float4 head4(const float* p, int d, int D, int64_t sd) {
+  if (VEC) return *reinterpret_cast<const float4*>(p + d);  // D is a multiple of 4 and d < D
   float4 r;
   r.x = p[d * sd];
   r.y = d + 1 < D ? p[(d + 1) * sd] : 0.f;
@@ -125,7 +126,7 @@ __device__ __forceinline__ float4 head4(const float* p, int d, int D, int64_t sd
 }
 
 // One CTA per tile of KN = 8192 / DP rows; DP / 4 lanes per row.
-template <int DP>
+template <int DP, bool VEC>
 __global__ void __launch_bounds__(256) cross_pack_kernel(const __grid_constant__ PackDev d) {
   constexpr int L = DP / 4, PT = kTileElems / DP, RP = 256 / L, NP = PT / RP;
   __shared__ float sm[8];
@@ -137,24 +138,37 @@ __global__ void __launch_bounds__(256) cross_pack_kernel(const __grid_constant__
   const int b = pr / d.Hk, hk = pr % d.Hk;
   const int n = s.keys ? key_count(d.len, d.len64, d.len_s, d.Tk, b) : s.G * s.T;
   const int lane = threadIdx.x % L, r0 = tile * PT + threadIdx.x / L, dd = lane * 4;
+  pdl_launch_dependents();
   float4 x[NP];
   float dl[NP];
-  float mx = 0.f;
-  bool bad = false;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int row = r0 + i * RP;
     x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    dl[i] = 0.f;
     if (row < n && dd < d.D) {
       const int g = (int)fdiv((uint32_t)row, s.f_T), t = row - g * s.T, h = hk * s.G + g;
-      x[i] = head4(static_cast<const float*>(s.x.p) + b * s.x.sb + t * s.x.st + h * s.x.sh, dd, d.D, s.x.sd, s.vec);
-      if (s.grad) {
-        const float4 o = head4(static_cast<const float*>(s.out.p) + b * s.out.sb + t * s.out.st + h * s.out.sh, dd, d.D,
-                               s.out.sd, s.vec);
-        dl[i] = __fmaf_rn(x[i].x, o.x, __fmaf_rn(x[i].y, o.y, __fmaf_rn(x[i].z, o.z, x[i].w * o.w)));
+      x[i] = head4<VEC>(static_cast<const float*>(s.x.p) + b * s.x.sb + t * s.x.st + h * s.x.sh, dd, d.D, s.x.sd);
+    }
+  }
+  if (s.grad) {
+    float4 o[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = r0 + i * RP;
+      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < n && dd < d.D) {
+        const int g = (int)fdiv((uint32_t)row, s.f_T), t = row - g * s.T, h = hk * s.G + g;
+        o[i] = head4<VEC>(static_cast<const float*>(s.out.p) + b * s.out.sb + t * s.out.st + h * s.out.sh, dd, d.D, s.out.sd);
       }
     }
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      dl[i] = __fmaf_rn(x[i].x, o[i].x, __fmaf_rn(x[i].y, o[i].y, __fmaf_rn(x[i].z, o[i].z, x[i].w * o[i].w)));
+  }
+  float mx = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
     mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
     bad |= !(fabsf(x[i].x) <= 3e38f && fabsf(x[i].y) <= 3e38f && fabsf(x[i].z) <= 3e38f && fabsf(x[i].w) <= 3e38f);
   }
@@ -381,7 +395,6 @@ struct FwdDev {
   int items;
   float *part, *part_m, *part_l;  // [split][problem][q.rows_p](DP) when splits > 1
   float f;               // |scale| log2 e
-  const int* nonfinite;
   int* err;
 };
 
@@ -427,7 +440,6 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   constexpr int KN = S::KN, OB = S::OB, NS = S::slots;
   static_assert(MT * S::cols <= 512, "tensor memory");
   const CrossDev& c = d.c;
-  if (*(volatile const int*)d.nonfinite != 0) return;  // the CUDA-core kernel serves this call
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sq = smem;
@@ -472,6 +484,14 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int np = c.B * c.Hk;
+  pdl_launch_dependents();
+  pdl_wait();  // everything from here on reads what the pack kernel wrote
+  if (*(volatile const int*)c.nonfinite != 0) {
+    exact_rows(c, (int64_t)blockIdx.x * (blockDim.x / 32) + warp, (int64_t)gridDim.x * (blockDim.x / 32));
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+    return;
+  }
 
   if (warp >= MT * 4) {
     if (MT == 2) give_registers<56>();
@@ -706,7 +726,6 @@ struct BwdDev {
   float *part1, *part2;        // [split][problem][a1.rows_p][DP] when splits > 1: dq, or dk and dv
   float f;                     // |scale| log2 e
   float out_scale;             // of dq (scale) or dk (|scale|)
-  const int* nonfinite;
   int* err;
 };
 
@@ -758,7 +777,6 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   constexpr bool DS_IN_S = !KV && S::ahead;
   static_assert(3 * KN + (KV ? 2 : 1) * DP <= 512, "tensor memory");
   const CrossDev& c = d.c;
-  if (*(volatile const int*)d.nonfinite != 0) return;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sa1 = smem;
@@ -815,6 +833,16 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int np = c.B * c.Hk;
+  pdl_launch_dependents();
+  pdl_wait();  // everything from here on reads what the pack kernel wrote
+  if (*(volatile const int*)c.nonfinite != 0) {
+    const int64_t w0 = (int64_t)blockIdx.x * (blockDim.x / 32) + warp, nw = (int64_t)gridDim.x * (blockDim.x / 32);
+    if (KV) exact_dkv_rows(c, w0, nw);
+    else exact_dq_rows(c, w0, nw);
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+    return;
+  }
   // tensor-memory columns: S (two buffers), dP, then the results (dq; dk, dv)
 
   if (warp >= 8) {
@@ -1141,35 +1169,49 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// result[row] = the parts added in order
-struct SumDev {
+// result[row] = the parts added in order, of up to three results (blockIdx.y)
+struct SumOne {
   const float* part;
   HeadsDev out;
-  int splits, np, rows_p, ld, Hk, G, T, D;
+  int splits, rows_p, G, T;
   FastDiv f_T;
   int64_t n;             // problems * G * T * (ld / 4)
+};
+struct SumDev {
+  SumOne r[3];
+  int np, ld, Hk, D;
   const int* nonfinite;
 };
-__global__ void __launch_bounds__(256) cross_sum_kernel(const SumDev d) {
+__global__ void __launch_bounds__(256) cross_sum_kernel(const __grid_constant__ SumDev d) {
+  pdl_wait();
+  const SumOne& r = d.r[blockIdx.y];
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= d.n || *(volatile const int*)d.nonfinite != 0) return;
+  if (i >= r.n || *(volatile const int*)d.nonfinite != 0) return;
   const int q = d.ld / 4, c = (int)(i % q) * 4;
-  const int64_t r = i / q;
-  const int row = (int)(r % (d.G * d.T)), pr = (int)(r / (d.G * d.T));
+  const int64_t w = i / q;
+  const int row = (int)(w % (r.G * r.T)), pr = (int)(w / (r.G * r.T));
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < d.splits; ++k) {
-    const float4 x = *reinterpret_cast<const float4*>(d.part + (((int64_t)k * d.np + pr) * d.rows_p + row) * d.ld + c);
-    s.x += x.x;
-    s.y += x.y;
-    s.z += x.z;
-    s.w += x.w;
+  const float* p = r.part + ((int64_t)pr * r.rows_p + row) * d.ld + c;
+  const int64_t step = (int64_t)d.np * r.rows_p * d.ld;
+  for (int k = 0; k < r.splits; k += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      x[u] = k + u < r.splits ? *reinterpret_cast<const float4*>(p + (k + u) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      s.x += x[u].x;
+      s.y += x[u].y;
+      s.z += x[u].z;
+      s.w += x[u].w;
+    }
   }
-  const int g = (int)fdiv((uint32_t)row, d.f_T), t = row - g * d.T;
-  float* o = static_cast<float*>(d.out.p) + (pr / d.Hk) * d.out.sb + t * d.out.st + (pr % d.Hk * d.G + g) * d.out.sh;
-  if (c < d.D) o[c * d.out.sd] = s.x;
-  if (c + 1 < d.D) o[(c + 1) * d.out.sd] = s.y;
-  if (c + 2 < d.D) o[(c + 2) * d.out.sd] = s.z;
-  if (c + 3 < d.D) o[(c + 3) * d.out.sd] = s.w;
+  const int g = (int)fdiv((uint32_t)row, r.f_T), t = row - g * r.T;
+  float* o = static_cast<float*>(r.out.p) + (pr / d.Hk) * r.out.sb + t * r.out.st + (pr % d.Hk * r.G + g) * r.out.sh;
+  if (c < d.D) o[c * r.out.sd] = s.x;
+  if (c + 1 < d.D) o[(c + 1) * r.out.sd] = s.y;
+  if (c + 2 < d.D) o[(c + 2) * r.out.sd] = s.z;
+  if (c + 3 < d.D) o[(c + 3) * r.out.sd] = s.w;
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -1237,7 +1279,6 @@ void add_source(PackDev& d, const CrossDev& c, const HeadsDev& x, const Packed& 
   s.inv = p.inv;
   s.norm = p.norm;
   s.sign = 1.f;
-  s.vec = c.vec;
   if (d.n == 0) d.first[0] = 0;
   d.first[d.n + 1] = d.first[d.n] + (uint32_t)(p.rows_all / (kTileElems / DP));
   ++d.n;
@@ -1255,8 +1296,9 @@ Error run_pack(PackDev& d, const CrossDev& c, int DP, int* nonfinite, cudaStream
   d.ls_h = c.ls_h;
   d.ls_t = c.ls_t;
   d.nonfinite = nonfinite;
-  if (DP == 64) cross_pack_kernel<64><<<d.first[d.n], 256, 0, stream>>>(d);
-  else cross_pack_kernel<128><<<d.first[d.n], 256, 0, stream>>>(d);
+  auto k = DP == 64 ? (c.vec ? cross_pack_kernel<64, true> : cross_pack_kernel<64, false>)
+                    : (c.vec ? cross_pack_kernel<128, true> : cross_pack_kernel<128, false>);
+  k<<<d.first[d.n], 256, 0, stream>>>(d);
   return check_launch("cross attention pack kernel");
 }
 
@@ -1274,9 +1316,8 @@ Error launch_forward(const Packed& q, const Packed& k, const Packed& v, FwdDev& 
   auto kern = cross_forward_kernel<DP, MT>;
   allow_smem((const void*)kern, S::smem);
   f.items = f.mtiles * f.c.B * f.c.Hk * f.splits;
-  kern<<<(unsigned)std::min(f.items, current_device_info().sm_count), S::threads, S::smem, stream>>>(q.map128, k.mapKN,
-                                                                                                 v.mapKN, f);
-  return check_launch("cross attention forward kernel");
+  return launch_after(kern, dim3((unsigned)std::min(f.items, current_device_info().sm_count)), S::threads, S::smem, stream,
+                      "cross attention forward kernel", q.map128, k.mapKN, v.mapKN, f);
 }
 
 template <int DP, bool KV>
@@ -1286,29 +1327,31 @@ Error launch_backward(const Packed& a1, const Packed& a2, const Packed& b1, cons
   auto kern = cross_backward_kernel<DP, KV>;
   allow_smem((const void*)kern, S::smem);
   f.items = f.mtiles * f.c.B * f.c.Hk * f.splits;
-  kern<<<(unsigned)std::min(f.items, current_device_info().sm_count), S::threads, S::smem, stream>>>(
-      a1.map128, a2.map128, b1.mapKN, b2.mapKN, f);
-  return check_launch(KV ? "cross attention key gradient kernel" : "cross attention query gradient kernel");
+  return launch_after(kern, dim3((unsigned)std::min(f.items, current_device_info().sm_count)), S::threads, S::smem, stream,
+                      KV ? "cross attention key gradient kernel" : "cross attention query gradient kernel", a1.map128,
+                      a2.map128, b1.mapKN, b2.mapKN, f);
 }
 
-Error run_sum(const CrossDev& c, const float* part, const HeadsDev& out, int splits, int rows_p, int DP, int G, int T,
-              const int* nonfinite, cudaStream_t stream) {
-  SumDev s;
+void add_sum(SumOne& s, const float* part, const HeadsDev& out, int splits, int rows_p, int G, int T, int np, int DP) {
   s.part = part;
   s.out = out;
   s.splits = splits;
-  s.np = c.B * c.Hk;
   s.rows_p = rows_p;
-  s.ld = DP;
-  s.Hk = c.Hk;
   s.G = G;
   s.T = T;
   s.f_T = make_fastdiv((uint32_t)T);
-  s.D = c.D;
-  s.n = (int64_t)s.np * G * T * (DP / 4);
-  s.nonfinite = nonfinite;
-  cross_sum_kernel<<<(unsigned)((s.n + 255) / 256), 256, 0, stream>>>(s);
-  return check_launch("cross attention sum kernel");
+  s.n = (int64_t)np * G * T * (DP / 4);
+}
+
+// A zeroed word that the pack kernel sets when an input is not finite.
+Error flag_word(Scratch& flag, CrossDev& c, cudaStream_t stream, int** word) {
+  Error e = flag.alloc(sizeof(int), stream);
+  if (!e.ok()) return e;
+  const cudaError_t ce = cudaMemsetAsync(flag.get(), 0, sizeof(int), stream);
+  if (ce != cudaSuccess) return cuda_error(ce, "cudaMemsetAsync");
+  *word = flag.as<int>();
+  c.nonfinite = *word;
+  return Error{};
 }
 
 // Parts of a walk of `tiles` column tiles so that `ctas` CTAs fill the SMs;
@@ -1322,8 +1365,13 @@ int pick_splits(int64_t ctas, int tiles) {
 
 }  // namespace
 
-Error cross_tc_forward(const CrossDev& c, int* nonfinite, cudaStream_t stream) {
+Error cross_tc_forward(const CrossDev& call, cudaStream_t stream) {
+  CrossDev c = call;
   Error e = too_large(c);
+  if (!e.ok()) return e;
+  Scratch flag;
+  int* nonfinite = nullptr;
+  e = flag_word(flag, c, stream, &nonfinite);
   if (!e.ok()) return e;
   EncodeTiled enc = encode_fn(&e);
   if (!enc) return e;
@@ -1369,7 +1417,6 @@ Error cross_tc_forward(const CrossDev& c, int* nonfinite, cudaStream_t stream) {
   f.k = k.planes();
   f.v = v.planes();
   f.f = fabsf(c.scale) * kLog2e;
-  f.nonfinite = nonfinite;
   f.err = async_error_word();
   if (DP == 64) e = MT == 2 ? launch_forward<64, 2>(q, k, v, f, stream) : launch_forward<64, 1>(q, k, v, f, stream);
   else e = MT == 2 ? launch_forward<128, 2>(q, k, v, f, stream) : launch_forward<128, 1>(q, k, v, f, stream);
@@ -1377,8 +1424,13 @@ Error cross_tc_forward(const CrossDev& c, int* nonfinite, cudaStream_t stream) {
   return cross_join(c, f.splits, q.rows_p, DP, f.part, f.part_m, f.part_l, stream);
 }
 
-Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) {
+Error cross_tc_backward(const CrossDev& call, cudaStream_t stream) {
+  CrossDev c = call;
   Error e = too_large(c);
+  if (!e.ok()) return e;
+  Scratch flag;
+  int* nonfinite = nullptr;
+  e = flag_word(flag, c, stream, &nonfinite);
   if (!e.ok()) return e;
   EncodeTiled enc = encode_fn(&e);
   if (!enc) return e;
@@ -1387,7 +1439,6 @@ Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) 
   std::memset(static_cast<void*>(&q_d), 0, sizeof(q_d));
   q_d.c = c;
   q_d.f = fabsf(c.scale) * kLog2e;
-  q_d.nonfinite = nonfinite;
   q_d.err = async_error_word();
   k_d = q_d;
   q_d.mtiles = (c.M + 127) / 128;
@@ -1459,13 +1510,24 @@ Error cross_tc_backward(const CrossDev& c, int* nonfinite, cudaStream_t stream) 
   if (!e.ok()) return e;
   e = DP == 64 ? launch_backward<64, true>(k, v, q, g, k_d, stream) : launch_backward<128, true>(k, v, q, g, k_d, stream);
   if (!e.ok()) return e;
-  if (q_d.splits > 1) {
-    e = run_sum(c, q_d.part1, c.dq, q_d.splits, q.rows_p, DP, c.G, c.Tq, nonfinite, stream);
-    if (!e.ok()) return e;
-  }
-  if (k_d.splits > 1) {
-    e = run_sum(c, k_d.part1, c.dk, k_d.splits, k.rows_p, DP, 1, c.Tk, nonfinite, stream);
-    if (e.ok()) e = run_sum(c, k_d.part2, c.dv, k_d.splits, k.rows_p, DP, 1, c.Tk, nonfinite, stream);
+  if (q_d.splits > 1 || k_d.splits > 1) {
+    SumDev sd;
+    std::memset(static_cast<void*>(&sd), 0, sizeof(sd));
+    sd.np = np;
+    sd.ld = DP;
+    sd.Hk = c.Hk;
+    sd.D = c.D;
+    sd.nonfinite = nonfinite;
+    int m = 0;
+    int64_t most = 0;
+    if (q_d.splits > 1) add_sum(sd.r[m++], q_d.part1, c.dq, q_d.splits, q.rows_p, c.G, c.Tq, np, DP);
+    if (k_d.splits > 1) {
+      add_sum(sd.r[m++], k_d.part1, c.dk, k_d.splits, k.rows_p, 1, c.Tk, np, DP);
+      add_sum(sd.r[m++], k_d.part2, c.dv, k_d.splits, k.rows_p, 1, c.Tk, np, DP);
+    }
+    for (int i = 0; i < m; ++i) most = std::max(most, sd.r[i].n);
+    e = launch_after(cross_sum_kernel, dim3((unsigned)((most + 255) / 256), (unsigned)m), 256, 0, stream,
+                     "cross attention sum kernel", sd);
   }
   return e;
 }

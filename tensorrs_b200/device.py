@@ -18,7 +18,14 @@ from . import abi
 TORCH_TO_TRS = {torch.float32: abi.F32, torch.float64: abi.F64, torch.int32: abi.I32, torch.int64: abi.I64}
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle() -> int:
+    """PyTorch's current stream of the current device (read straight from the binding where it offers that: the
+    Stream object costs 3 us, as much as a launch)."""
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
