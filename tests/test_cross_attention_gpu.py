@@ -80,7 +80,8 @@ def test_against_64_bits(size):
 @pytest.mark.parametrize("size,lengths", [
     ((4, 130, 200, 2, 2, 64), [0, 1, 200, 65]), ((4, 40, 300, 4, 2, 128), [128, 0, 63, 300]),
     ((4, 2, 300, 4, 2, 64), [0, 1, 300, 257]), ((3, 5, 70, 2, 1, 200), [70, 0, 33]), ((3, 64, 128, 1, 1, 64), [-5, 1000, 64]),
-    ((2, 300, 100, 1, 1, 80), [0, 0]),
+    ((2, 300, 100, 1, 1, 80), [0, 0]), ((5, 300, 700, 6, 2, 64), [700, 0, 3, 128, 513]),
+    ((6, 200, 900, 4, 4, 128), [0, 900, 0, 1, 449, 0]), ((40, 20, 70, 1, 1, 64), [(7 * i) % 71 for i in range(40)]),
 ], ids=str)
 def test_key_lengths_and_what_lies_behind_them(size, lengths, dtype):
     q, k, v, g = draw(*size, seed=3)
