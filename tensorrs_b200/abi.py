@@ -58,6 +58,7 @@ class View(ctypes.Structure):
 
 _PACK_VIEW = struct.Struct(f"@Pqii{MAX_DIMS}q{MAX_DIMS}qq").pack
 _ZEROS = (0,) * MAX_DIMS
+_from_bytes = View.from_buffer_copy
 
 
 class Scalar(ctypes.Structure):
@@ -199,16 +200,22 @@ def make_view(ptr: int, dtype: int, shape, strides=None, offset: int = 0,
             strides[i] = step
             step *= int(shape[i])
     strides = tuple(strides)[:n]
+    strides += _ZEROS[:n - len(strides)]
     if storage_len is None:
         hi = offset
         for s, st in zip(shape, strides):
             if s > 0 and st > 0:
                 hi += (s - 1) * st
         storage_len = hi + 1
-    # one pack of the whole struct: a third of the time of setting its fields
-    # one by one, which small calls with several views notice
-    return View.from_buffer_copy(_PACK_VIEW(ptr or 0, storage_len, dtype, n, *shape, *_ZEROS[n:], *strides,
-                                            *_ZEROS[len(strides):], offset))
+    return pack_view(ptr or 0, storage_len, dtype, shape, strides, offset)
+
+
+def pack_view(ptr: int, storage_len: int, dtype: int, shape, strides, offset: int) -> View:
+    """A trs_view from all of its fields; one pack of the whole struct takes a third of the time of setting its fields
+    one by one, which small calls with several views notice."""
+    n = len(shape)
+    pad = _ZEROS[n:]
+    return _from_bytes(_PACK_VIEW(ptr, storage_len, dtype, n, *shape, *pad, *strides, *pad, offset))
 
 
 def program(n_in: int, op1: int = ADD, op2: int = ADD, epilogue: str | int = "none",

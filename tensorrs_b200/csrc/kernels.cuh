@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <map>
 #include <mutex>
+#include <type_traits>
 #include <unordered_map>
 #include <utility>
 
@@ -61,6 +62,30 @@ inline int resident_blocks_smem(const void* kernel, int threads, int smem) {
   }
   cache[key] = b;
   return b;
+}
+
+// A launch that may be scheduled while the stream's previous kernel still runs
+// (programmatic dependent launch): the kernel waits for that one with
+// pdl_wait() before it touches anything the other writes.
+template <class... A>
+inline Error launch_after(void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t stream, const char* what,
+                          const std::common_type_t<A>&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_error(e, what);
+  }
+  return check_launch(what);
 }
 
 // Element-wise launch descriptor (passed by value as a kernel parameter).

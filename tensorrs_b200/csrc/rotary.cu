@@ -27,8 +27,9 @@
 // by less than 2^-24 of a turn), for f64 tensors all of it is f64.
 // The row sums stay in the element type (f32 over at most 512 squares, 32
 // lanes' partial sums folded as a tree); dgamma, a sum over all rows, is
-// accumulated in f64 per lane, folded over the CTA and then over the CTAs in a
-// fixed order, and rounded once.
+// accumulated over the heads of a token (8 at most) in the element type and
+// over the tokens in f64, folded over the CTA and then over the CTAs in a fixed
+// order, and rounded once.
 #include <cmath>
 #include <cstring>
 
@@ -201,12 +202,12 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotDev d) {
       gb[k][i] = MODE != kRotate && gam && un[k].v1 ? gam[(un[k].o1 + i) * d.gs[which]] : T(1);
     }
   }
-  double aa[MODE == kNormBackward ? K : 1][V], ab[MODE == kNormBackward ? K : 1][V];
+  // dgamma: f32 (element type) sums over the heads of an item, at most 8, then
+  // f64 sums over the items in shared memory, one column per thread
+  __shared__ double fold[MODE == kNormBackward ? K * 2 * V : 1][MODE == kNormBackward ? kRotThreads : 1];
   if constexpr (MODE == kNormBackward) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) aa[k][i] = ab[k][i] = 0.0;
+    for (int i = 0; i < K * 2 * V; ++i) fold[i][threadIdx.x] = 0.0;
   }
 
   for (int64_t it = blk * kGroups + grp; it < d.items[which]; it += nblk * kGroups) {
@@ -233,6 +234,13 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotDev d) {
     const T* xt = xp + b * X.sb + t * X.st;
     T* yt = yp + b * Y.sb + t * Y.st;
     const T* dt = dp + b * DY.sb + t * DY.st;
+    T aa[MODE == kNormBackward ? K : 1][V], ab[MODE == kNormBackward ? K : 1][V];
+    if constexpr (MODE == kNormBackward) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) aa[k][i] = ab[k][i] = T(0);
+    }
     for (int h = h0; h < h1; h += UH) {
       T a[UH][K][V], c[UH][K][V];
       T ea[MODE == kNormBackward ? UH : 1][K][V], ec[MODE == kNormBackward ? UH : 1][K][V];
@@ -280,8 +288,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotDev d) {
               for (int i = 0; i < V; ++i) {
                 a[u][k][i] *= r;  // n
                 c[u][k][i] *= r;
-                aa[k][i] += (double)ea[u][k][i] * (double)a[u][k][i];
-                ab[k][i] += (double)ec[u][k][i] * (double)c[u][k][i];
+                aa[k][i] = rfma(ea[u][k][i], a[u][k][i], aa[k][i]);
+                ab[k][i] = rfma(ec[u][k][i], c[u][k][i], ab[k][i]);
                 ea[u][k][i] *= ga[k][i];  // dn
                 ec[u][k][i] *= gb[k][i];
                 dot = rfma(ea[u][k][i], a[u][k][i], dot);
@@ -307,38 +315,34 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotDev d) {
         }
       }
     }
+    if constexpr (MODE == kNormBackward) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          fold[k * 2 * V + i][threadIdx.x] += (double)aa[k][i];
+          fold[k * 2 * V + V + i][threadIdx.x] += (double)ab[k][i];
+        }
+    }
   }
 
   if constexpr (MODE == kNormBackward) {
+    pdl_launch_dependents();
     if (d.part[which] == nullptr) return;
-    __shared__ double fold[kRotThreads][2 * V];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        fold[threadIdx.x][i] = aa[k][i];
-        fold[threadIdx.x][V + i] = ab[k][i];
-      }
-      __syncthreads();
-      if (threadIdx.x < G) {
-        double* out = d.part[which] + blk * d.D;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          double sa = 0.0, sb = 0.0;
-          for (int g = 0; g < kGroups; ++g) {
-            sa += fold[g * G + threadIdx.x][i];
-            sb += fold[g * G + threadIdx.x][V + i];
-          }
-          if (un[k].v0) out[un[k].o0 + i] = sa;
-          if (un[k].v1) out[un[k].o1 + i] = sb;
-        }
-      }
+    __syncthreads();
+    // column i of unit u is spread over the threads of lane u of every group
+    for (int x = threadIdx.x; x < K * 2 * V * G; x += kRotThreads) {
+      const int i = x / G, u = x % G, k = i / (2 * V), e = i % (2 * V);
+      const Unit n = unit_of<V, IL>(d, u + k * G);
+      double s = 0.0;
+      for (int g = 0; g < kGroups; ++g) s += fold[i][g * G + u];
+      const int at = e < V ? n.o0 + e : n.o1 + e - V;
+      if (e < V ? n.v0 : n.v1) d.part[which][blk * d.D + at] = s;
     }
   }
 }
 
-// dgamma[d] = the CTAs' partial sums added in a fixed order: 32 columns by 8
+// dgamma[d] = the CTAs' partial sums added in a fixed order: 32 columns by 32
 // row groups per CTA; blockIdx.y is the tensor.
 struct GammaDev {
   const double* part[2];
@@ -348,19 +352,29 @@ struct GammaDev {
   int D;
 };
 template <class T>
-__global__ void __launch_bounds__(256) gamma_fold_kernel(const GammaDev d) {
-  __shared__ double sm[8][32];
-  const int w = blockIdx.y, col = blockIdx.x * 32 + threadIdx.x % 32, g = threadIdx.x / 32;
+__global__ void __launch_bounds__(1024) gamma_fold_kernel(const GammaDev d) {
+  __shared__ double sm[32][33];
+  pdl_wait();
+  const int w = blockIdx.y, lane = threadIdx.x % 32, col = blockIdx.x * 32 + lane, g = threadIdx.x / 32;
   if (d.out[w] == nullptr) return;
   double s = 0.0;
-  if (col < d.D)
-    for (int64_t r = g; r < d.rows[w]; r += 8) s += d.part[w][r * d.D + col];
-  sm[g][threadIdx.x % 32] = s;
-  __syncthreads();
-  if (g == 0 && col < d.D) {
-    for (int i = 1; i < 8; ++i) s += sm[i][threadIdx.x];
-    static_cast<T*>(d.out[w])[col * d.st[w]] = (T)s;
+  if (col < d.D) {
+    for (int64_t r = g; r < d.rows[w]; r += 128) {
+      double x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = r + 32 * i < d.rows[w] ? d.part[w][(r + 32 * i) * d.D + col] : 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += x[i];
+    }
   }
+  sm[g][lane] = s;
+  __syncthreads();
+  // warp g folds column g as a tree
+  s = sm[lane][g];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int c = blockIdx.x * 32 + g;
+  if (lane == 0 && c < d.D) static_cast<T*>(d.out[w])[c * d.st[w]] = (T)s;
 }
 
 template <class T>
@@ -441,8 +455,8 @@ Error launch_rot(RotDev& d, const RotCall& c, cudaStream_t stream) {
     g.out[w] = static_cast<T*>(outs[w]->data) + outs[w]->offset;
     g.st[w] = outs[w]->strides[0];
   }
-  gamma_fold_kernel<T><<<dim3((unsigned)((d.D + 31) / 32), 2), 256, 0, stream>>>(g);
-  return check_launch("gamma gradient fold kernel");
+  return launch_after(gamma_fold_kernel<T>, dim3((unsigned)((d.D + 31) / 32), 2), 1024, 0, stream,
+                      "gamma gradient fold kernel", g);
 }
 
 // lanes per token and units per lane from the number of units
@@ -454,7 +468,7 @@ Error pick_group(RotDev& d, const RotCall& c, cudaStream_t s) {
     if (d.NU <= 8) return launch_rot<T, V, IL, MODE, 8, 1, UH>(d, c, s);
     if (d.NU <= 16) return launch_rot<T, V, IL, MODE, 16, 1, UH>(d, c, s);
     if (d.NU <= 32) return launch_rot<T, V, IL, MODE, 32, 1, UH>(d, c, s);
-    return launch_rot<T, V, IL, MODE, 32, 4, 1>(d, c, s);  // at most 128 units of a 512-element head
+    return launch_rot<T, V, IL, MODE, 32, 8 / V, 1>(d, c, s);  // a 512-element head: 64 units of 8, 128 of 4
   } else {
     if (d.NU <= 32) return launch_rot<T, V, IL, MODE, 32, 1, UH>(d, c, s);
     if (d.NU <= 128) return launch_rot<T, V, IL, MODE, 32, 4, 1>(d, c, s);

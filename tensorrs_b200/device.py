@@ -29,18 +29,24 @@ def stream_handle() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_DTYPES = {t: (code, abi.DTYPE_SIZE[code]) for t, code in TORCH_TO_TRS.items()}
+
+
 def view_of(t: torch.Tensor, shape=None, strides=None, offset=None) -> abi.View:
     """A trs_view into t's storage.  Without overrides it describes t itself."""
     if not t.is_cuda:
         raise ValueError("view_of needs a CUDA tensor")
     st = t.untyped_storage()
+    code, size = _DTYPES[t.dtype]
+    if shape is None and strides is None and offset is None:
+        return abi.pack_view(st.data_ptr(), st.nbytes() // size, code, t.shape, t.stride(), t.storage_offset())
     if shape is None or list(shape) == list(t.shape):
         shape = t.shape
         if strides is None:
             strides = t.stride()
     if offset is None:
         offset = t.storage_offset()
-    return abi.make_view(st.data_ptr(), TORCH_TO_TRS[t.dtype], shape, strides, offset, st.nbytes() // t.element_size())
+    return abi.make_view(st.data_ptr(), code, shape, strides, offset, st.nbytes() // size)
 
 
 def _call(name: str, *args) -> int:
