@@ -42,34 +42,41 @@ struct RowsDev {
   float* part_l;
 };
 
+// Four elements of a head as two pairs for the packed f32 operations.
+struct Quad {
+  uint64_t a, b;
+};
 template <bool VEC>
-__device__ __forceinline__ float4 load4(const float* p, int d, int D, int64_t sd) {
-  if (VEC) return d < D ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-  float4 r;
-  r.x = d < D ? p[d * sd] : 0.f;
-  r.y = d + 1 < D ? p[(d + 1) * sd] : 0.f;
-  r.z = d + 2 < D ? p[(d + 2) * sd] : 0.f;
-  r.w = d + 3 < D ? p[(d + 3) * sd] : 0.f;
-  return r;
+__device__ __forceinline__ Quad load4(const float* p, int d, int D, int64_t sd) {
+  Quad q;
+  if (VEC) {
+    const ulonglong2 x = d < D ? *reinterpret_cast<const ulonglong2*>(p + d) : make_ulonglong2(0, 0);
+    q.a = x.x;
+    q.b = x.y;
+  } else {
+    q.a = pack2(d < D ? p[d * sd] : 0.f, d + 1 < D ? p[(d + 1) * sd] : 0.f);
+    q.b = pack2(d + 2 < D ? p[(d + 2) * sd] : 0.f, d + 3 < D ? p[(d + 3) * sd] : 0.f);
+  }
+  return q;
 }
 
-__device__ __forceinline__ float dot4(const float4& a, const float4& b, float s) {
-  s = __fmaf_rn(a.x, b.x, s);
-  s = __fmaf_rn(a.y, b.y, s);
-  s = __fmaf_rn(a.z, b.z, s);
-  return __fmaf_rn(a.w, b.w, s);
-}
-
+// Two to four CTAs per SM where the rows leave the registers for it: the bytes
+// in flight per SM carry this kernel.
 template <int NR, int L, int NV, bool VEC>
-__global__ void __launch_bounds__(kRowsThreads) cross_rows_kernel(const RowsDev d) {
+__global__ void __launch_bounds__(kRowsThreads, NR * NV <= 2 ? 4 : NR * NV <= 4 ? 2 : 1) cross_rows_kernel(const RowsDev d) {
   const CrossDev& c = d.c;
   pdl_launch_dependents();
   constexpr int U = 4;                                  // keys in flight per group
   constexpr int NG = kRowsThreads / L;                  // groups
   constexpr int DP = L * 4 * NV;                        // padded head size
+  constexpr int N = NR * U;                             // dot products of a step
+  constexpr int OWN = N > L ? N / L : 1;                // of which a lane keeps OWN, from `mine` on
+  constexpr int DUP = N < L ? L / N : 1;                // lanes that keep the same one
+  constexpr int LPR = L / NR;                           // lanes that keep a row's
   __shared__ float s_m[NG][NR], s_l[NG][NR];
   extern __shared__ float s_acc[];                      // [NG][NR][DP]
   const int gid = threadIdx.x / L, lane = threadIdx.x % L;
+  const int mine = lane * OWN / DUP % U;                // this lane's first key of the four
   const unsigned mask = L == 32 ? 0xffffffffu : (0xffffu << (threadIdx.x & 16));
   for (int item = blockIdx.x; item < d.items; item += gridDim.x) {
     const int sp = item % d.splits, rb = item / d.splits % d.blocks, pr = item / d.splits / d.blocks;
@@ -77,92 +84,111 @@ __global__ void __launch_bounds__(kRowsThreads) cross_rows_kernel(const RowsDev 
     const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
     const int per = (n + d.splits - 1) / d.splits;
     const int k0 = min(n, sp * per), k1 = min(n, k0 + per);
-    float4 q[NR][NV], acc[NR][NV];
-    float m[NR], l[NR];
+    Quad q[NR][NV], acc[NR][NV];
+    float m = -INFINITY, l = 0.f;                       // of this lane's row; l of this lane's keys
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const int row = rb * NR + r;
-      m[r] = -INFINITY;
-      l[r] = 0.f;
       const int g = row < c.M ? (int)fdiv((uint32_t)row, c.f_Tq) : 0, t = row < c.M ? row - g * c.Tq : 0;
       const float* qp = static_cast<const float*>(c.q.p) + b * c.q.sb + t * c.q.st + (hk * c.G + g) * c.q.sh;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        acc[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        q[r][i] = row < c.M ? load4<VEC>(qp, (lane + i * L) * 4, c.D, c.q.sd) : make_float4(0.f, 0.f, 0.f, 0.f);
+        acc[r][i] = Quad{0, 0};
+        q[r][i] = row < c.M ? load4<VEC>(qp, (lane + i * L) * 4, c.D, c.q.sd) : Quad{0, 0};
       }
     }
     const float f = c.scale * kLog2e;
     const float* kp = static_cast<const float*>(c.k.p) + b * c.k.sb + hk * c.k.sh;
     const float* vp = static_cast<const float*>(c.v.p) + b * c.v.sb + hk * c.v.sh;
     for (int key = k0 + gid * U; key < k1; key += NG * U) {
-      float4 kk[U][NV], vv[U][NV];
+      Quad kk[U][NV], vv[U][NV];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t at = key + u;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const bool on = at < k1;
-          kk[u][i] = on ? load4<VEC>(kp + at * c.k.st, (lane + i * L) * 4, c.D, c.k.sd) : make_float4(0.f, 0.f, 0.f, 0.f);
-          vv[u][i] = on ? load4<VEC>(vp + at * c.v.st, (lane + i * L) * 4, c.D, c.v.sd) : make_float4(0.f, 0.f, 0.f, 0.f);
+          kk[u][i] = on ? load4<VEC>(kp + at * c.k.st, (lane + i * L) * 4, c.D, c.k.sd) : Quad{0, 0};
+          vv[u][i] = on ? load4<VEC>(vp + at * c.v.st, (lane + i * L) * 4, c.D, c.v.sd) : Quad{0, 0};
         }
+      }
+      float s[N];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          uint64_t x = 0;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) x = fma2(q[r][i].b, kk[u][i].b, fma2(q[r][i].a, kk[u][i].a, x));
+          float lo, hi;
+          unpack2(x, &lo, &hi);
+          s[r * U + u] = lo + hi;
+        }
+      // fold over the lanes: each step a lane hands over the half that the
+      // other keeps, so that N dot products take about N + log2 L shuffles
+      // instead of N log2 L, and each exponential is taken once
+#pragma unroll
+      for (int o = L / 2, w = N / 2; o > 0; o >>= 1, w >>= 1) {
+        if (w > 0) {
+          const bool up = lane & o;
+#pragma unroll
+          for (int i = 0; i < (w > 0 ? w : 1); ++i) {
+            const float give = up ? s[i] : s[i + w], keep = up ? s[i + w] : s[i];
+            s[i] = keep + __shfl_xor_sync(mask, give, o);
+          }
+        } else {
+          s[0] += __shfl_xor_sync(mask, s[0], o);
+        }
+      }
+      float mx = m;
+#pragma unroll
+      for (int e = 0; e < OWN; ++e) {
+        s[e] = key + mine + e < k1 ? s[e] * f : -INFINITY;
+        mx = fmaxf(mx, s[e]);
+      }
+#pragma unroll
+      for (int o = LPR / 2; o >= DUP; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(mask, mx, o));
+      const float base = mx == -INFINITY ? 0.f : mx;  // all scores -inf so far: every weight stays 0
+      const float alpha = ex2(m - base);
+      m = mx;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < OWN; ++e) {
+        s[e] = ex2(s[e] - base);
+        l += s[e];
       }
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        float s[U];
+        const float al = NR == 1 ? alpha : __shfl_sync(mask, alpha, r * LPR, L);
+        const uint64_t al2 = pack2(al, al);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[r][i] = Quad{mul2(acc[r][i].a, al2), mul2(acc[r][i].b, al2)};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          s[u] = 0.f;
+          constexpr int X = U;  // (r, u) is kept by lane (r U + u) DUP / OWN
+          const float p = __shfl_sync(mask, s[(r * X + u) % OWN], (r * X + u) * DUP / OWN, L);
+          const uint64_t p2 = pack2(p, p);
 #pragma unroll
-          for (int i = 0; i < NV; ++i) s[u] = dot4(q[r][i], kk[u][i], s[u]);
-        }
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1)
-#pragma unroll
-          for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(mask, s[u], o, L);
-        float mx = m[r];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          s[u] = key + u < k1 ? s[u] * f : -INFINITY;
-          mx = fmaxf(mx, s[u]);
-        }
-        const float base = mx == -INFINITY ? 0.f : mx;  // all scores -inf so far: every weight stays 0
-        const float alpha = ex2(m[r] - base);
-        m[r] = mx;
-        l[r] *= alpha;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          s[u] = ex2(s[u] - base);
-          l[r] += s[u];
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float4& a = acc[r][i];
-          a.x *= alpha;
-          a.y *= alpha;
-          a.z *= alpha;
-          a.w *= alpha;
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            a.x = __fmaf_rn(s[u], vv[u][i].x, a.x);
-            a.y = __fmaf_rn(s[u], vv[u][i].y, a.y);
-            a.z = __fmaf_rn(s[u], vv[u][i].z, a.z);
-            a.w = __fmaf_rn(s[u], vv[u][i].w, a.w);
-          }
+          for (int i = 0; i < NV; ++i)
+            acc[r][i] = Quad{fma2(p2, vv[u][i].a, acc[r][i].a), fma2(p2, vv[u][i].b, acc[r][i].b)};
         }
       }
     }
+    // a row's sum over the lanes that keep its keys
+#pragma unroll
+    for (int o = LPR / 2; o >= DUP; o >>= 1) l += __shfl_xor_sync(mask, l, o);
     // join the CTA's groups
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      if (lane == 0) {
-        s_m[gid][r] = m[r];
-        s_l[gid][r] = l[r];
+      if (lane == r * LPR) {
+        s_m[gid][r] = m;
+        s_l[gid][r] = l;
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        *reinterpret_cast<float4*>(&s_acc[(gid * NR + r) * DP + (lane + i * L) * 4]) = acc[r][i];
+        *reinterpret_cast<ulonglong2*>(&s_acc[(gid * NR + r) * DP + (lane + i * L) * 4]) =
+            make_ulonglong2(acc[r][i].a, acc[r][i].b);
     }
     __syncthreads();
     for (int idx = threadIdx.x; idx < NR * DP; idx += kRowsThreads) {
@@ -304,35 +330,32 @@ Error zero_heads(const HeadsDev& x, int64_t B, int T, int H, int D, cudaStream_t
 // ---- host side -------------------------------------------------------------------
 
 template <int NR, int L, int NV>
-Error launch_rows(RowsDev& d, int grid, cudaStream_t s) {
+Error launch_rows(RowsDev& d, cudaStream_t s) {
+  const CrossDev& c = d.c;
   constexpr int smem = kRowsThreads / L * NR * L * 4 * NV * 4;
-  auto k = d.c.vec ? cross_rows_kernel<NR, L, NV, true> : cross_rows_kernel<NR, L, NV, false>;
+  auto k = c.vec ? cross_rows_kernel<NR, L, NV, true> : cross_rows_kernel<NR, L, NV, false>;
   allow_smem((const void*)k, smem);
-  k<<<(unsigned)grid, kRowsThreads, smem, s>>>(d);
-  return check_launch("cross attention rows kernel");
-}
-
-Error run_rows(const CrossDev& c, cudaStream_t s) {
-  RowsDev d;
-  std::memset(static_cast<void*>(&d), 0, sizeof(d));
-  d.c = c;
   const int np = c.B * c.Hk;
-  const int most = c.D <= 128 ? 8 : 4;  // rows a CTA keeps in registers
-  int NR = 1;
-  while (NR < most && NR < c.M) NR *= 2;
   d.blocks = (c.M + NR - 1) / NR;
-  // parts of the keys until the GPU has about four CTAs per SM, of 256 keys at
-  // least (a part's fixed cost is that of about 100 keys)
-  const int sms = current_device_info().sm_count;
+  // the parts of the keys (256 keys each at least: a part's fixed cost is that
+  // of about 100) that leave the fewest CTA places idle in the last wave, up to
+  // four waves
+  const int64_t resident = (int64_t)current_device_info().sm_count * resident_blocks_smem((const void*)k, kRowsThreads, smem);
   const int64_t base = (int64_t)np * d.blocks;
-  int64_t splits = 4 * sms / base;
-  if (splits > c.Tk / 256) splits = c.Tk / 256;
-  if (splits < 1) splits = 1;
-  d.splits = (int)splits;
+  int64_t splits = 1;
+  double best = 0.0;
+  for (int64_t n = 1; n <= std::max<int64_t>(1, c.Tk / 256) && (n == 1 || n * base <= 4 * resident); ++n) {
+    const int64_t waves = (n * base + resident - 1) / resident;
+    const double use = (double)(n * base) / (double)(waves * resident);
+    if (use > best + 0.02) {
+      best = use;
+      splits = n;
+    }
+  }
   const int64_t items = base * splits;
   if (items >= (1ll << 31)) return make_error(TRS_ERR_SHAPE, "cross_attention: too many query rows");
+  d.splits = (int)splits;
   d.items = (int)items;
-  const int grid = (int)std::min<int64_t>(items, 1 << 24);
   Scratch part;
   if (splits > 1) {
     const size_t rows = (size_t)splits * np * c.M;
@@ -343,19 +366,25 @@ Error run_rows(const CrossDev& c, cudaStream_t s) {
     d.part_m = d.part + rows * d.ld;
     d.part_l = d.part_m + rows;
   }
-  Error e;
-  if (c.D <= 64) {
-    e = NR == 1 ? launch_rows<1, 16, 1>(d, grid, s) : NR == 2 ? launch_rows<2, 16, 1>(d, grid, s)
-        : NR == 4 ? launch_rows<4, 16, 1>(d, grid, s) : launch_rows<8, 16, 1>(d, grid, s);
-  } else if (c.D <= 128) {
-    e = NR == 1 ? launch_rows<1, 32, 1>(d, grid, s) : NR == 2 ? launch_rows<2, 32, 1>(d, grid, s)
-        : NR == 4 ? launch_rows<4, 32, 1>(d, grid, s) : launch_rows<8, 32, 1>(d, grid, s);
-  } else {
-    e = NR == 1 ? launch_rows<1, 32, 2>(d, grid, s) : NR == 2 ? launch_rows<2, 32, 2>(d, grid, s)
-                                                              : launch_rows<4, 32, 2>(d, grid, s);
-  }
+  k<<<(unsigned)std::min<int64_t>(items, 1 << 24), kRowsThreads, smem, s>>>(d);
+  Error e = check_launch("cross attention rows kernel");
   if (!e.ok() || splits == 1) return e;
   return cross_join(c, d.splits, c.M, d.ld, d.part, d.part_m, d.part_l, s);
+}
+
+Error run_rows(const CrossDev& c, cudaStream_t s) {
+  RowsDev d;
+  std::memset(static_cast<void*>(&d), 0, sizeof(d));
+  d.c = c;
+  if (c.D <= 64) {
+    return c.M == 1 ? launch_rows<1, 16, 1>(d, s) : c.M == 2 ? launch_rows<2, 16, 1>(d, s)
+           : c.M <= 4 ? launch_rows<4, 16, 1>(d, s) : launch_rows<8, 16, 1>(d, s);
+  }
+  if (c.D <= 128) {
+    return c.M == 1 ? launch_rows<1, 32, 1>(d, s) : c.M == 2 ? launch_rows<2, 32, 1>(d, s)
+           : c.M <= 4 ? launch_rows<4, 32, 1>(d, s) : launch_rows<8, 32, 1>(d, s);
+  }
+  return c.M == 1 ? launch_rows<1, 32, 2>(d, s) : c.M == 2 ? launch_rows<2, 32, 2>(d, s) : launch_rows<4, 32, 2>(d, s);
 }
 
 struct CrossCall {
@@ -480,7 +509,10 @@ Error run_cross(const CrossCall& c, bool backward, cudaStream_t stream) {
   d.vec = 1;
   for (int i = 0; i < (backward ? 8 : 4); ++i) d.vec = d.vec && aligned(heads[i]);
   const int sms = current_device_info().sm_count;
-  const bool tc = D <= 128 && (backward || d.M > 16);
+  // up to 16 rows (8 of heads above 64) the CUDA cores read k and v faster than
+  // the tensor-core path splits them: 16 rows on 4 x 16 heads of 64 and 2048
+  // keys 54 us here, 58 there; 16 rows of 128 129 and 95, 8 rows 66 and 94
+  const bool tc = D <= 128 && (backward || d.M > (D <= 64 ? 16 : 8));
   if (!tc) {
     if (!backward) return run_rows(d, stream);
     cross_grad_rows_kernel<<<8 * sms, 256, 0, stream>>>(d);
