@@ -510,8 +510,9 @@ Error run_cross(const CrossCall& c, bool backward, cudaStream_t stream) {
   for (int i = 0; i < (backward ? 8 : 4); ++i) d.vec = d.vec && aligned(heads[i]);
   const int sms = current_device_info().sm_count;
   // up to 16 rows (8 of heads above 64) the CUDA cores read k and v faster than
-  // the tensor-core path splits them: 16 rows on 4 x 16 heads of 64 and 2048
-  // keys 54 us here, 58 there; 16 rows of 128 129 and 95, 8 rows 66 and 94
+  // the tensor-core path splits them.  4 x 16 heads, 2048 keys, CUDA cores and
+  // tensor cores: heads of 64, 16 rows 40 and 58 us, 24 rows 66 and 58; heads
+  // of 128, 8 rows 58 and 94, 16 rows 97 and 94
   const bool tc = D <= 128 && (backward || d.M > (D <= 64 ? 16 : 8));
   if (!tc) {
     if (!backward) return run_rows(d, stream);
