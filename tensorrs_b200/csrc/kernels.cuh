@@ -8,7 +8,6 @@
 #include <map>
 #include <mutex>
 #include <type_traits>
-#include <unordered_map>
 #include <utility>
 
 #include "bulk.cuh"
@@ -33,17 +32,20 @@ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
   return (uint32_t)(((uint64_t)__umulhi(n, f.m) + n) >> f.s);
 }
 
-// Per-kernel launch set-up done once per process: the dynamic shared memory
-// a kernel may use (raised only upward), and the CTAs of it an SM keeps
-// resident with a given dynamic shared memory (each kernel here has one block
-// size), queried once per pair.
+// Per-kernel launch set-up done once per process and device: the dynamic
+// shared memory a kernel may use (raised only upward), and the CTAs of it an SM
+// keeps resident with a given dynamic shared memory (each kernel here has one
+// block size), queried once per pair.
 inline void allow_smem(const void* kernel, int bytes) {
   static std::mutex mu;
-  static std::unordered_map<const void*, int> done;
+  static std::map<std::pair<int, const void*>, int> done;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) cudaGetLastError();
   std::lock_guard<std::mutex> lock(mu);
-  if (done[kernel] >= bytes) return;
+  int& have = done[{device, kernel}];
+  if (have >= bytes) return;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess)
-    done[kernel] = bytes;
+    have = bytes;
   else
     cudaGetLastError();
 }

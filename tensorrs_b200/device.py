@@ -250,7 +250,11 @@ def _ref(v: abi.View | None):
 
 
 def _out(t: torch.Tensor | None):
-    return ctypes.byref(view_of(t)) if t is not None else None
+    if t is None:
+        return None
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError("the output lies on another device than the current one")
+    return ctypes.byref(view_of(t))
 
 
 def rotary_frequencies(out: torch.Tensor, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
