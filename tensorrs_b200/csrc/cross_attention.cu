@@ -10,13 +10,14 @@
 //
 // cross_rows_kernel serves few query rows per key head (single tokens), where
 // reading k and v once is all there is to do, and, in blocks of rows, head
-// sizes above 128.  A CTA
-// owns (problem, block of NR rows, part of the keys): groups of L lanes own
-// one key at a time, each lane 4 (8) elements of the head; 4 keys are in
-// flight per group, the dot products fold over the group with shuffles, and
-// the running maximum, sum and output stay in registers until the CTA's groups
-// are joined in shared memory.  Parts of the keys are joined by
-// cross_join_kernel in a fixed order.
+// sizes above 128.  A CTA owns (problem, block of NR rows, part of the keys):
+// groups of L lanes own one key at a time, each lane 4 (8) elements of the
+// head; 4 keys are in flight per group, the dot products fold over the group
+// with shuffles, and the running maximum, sum and output stay in registers
+// until the CTA's groups are joined in shared memory.  Parts of the keys are
+// joined by cross_join_kernel in a fixed order.  One row is bound by the loads
+// in flight (8 x 16 heads of 64, 1024 to 2048 keys, 88 MB: 20 us, 4.4 TB/s),
+// eight by arithmetic (4 x 16 heads, 2048 keys, 67 MB: 29 us).
 #include <algorithm>
 #include <cmath>
 #include <cstring>

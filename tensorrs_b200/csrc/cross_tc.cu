@@ -18,22 +18,36 @@
 //                         [problem][rows][DP], DP = 64 or 128, zeros behind the
 //                         last row, key length and head size: strides, ragged
 //                         lengths and odd head sizes end here.  Also delta, and
-//                         the norms that bound dS.
-//   cross_forward_kernel  a CTA owns MT = 1 or 2 tiles of 128 query rows and
-//                         walks key tiles of KN (128 for DP 64, 64 for DP 128).
-//                         Warp 9 streams K and V tiles by TMA through a ring of
-//                         32 KiB slots; warp 8 issues the MMAs; a warpgroup per
-//                         row tile, one thread per row, keeps the running
-//                         maximum and sum of the softmax, turns S (TMEM) into
-//                         the two planes of P in place, and adds O.  With two
-//                         row tiles one is in the softmax while the other is in
-//                         the tensor core.
+//                         the norms that bound dS.  Bound by HBM: three tensors
+//                         of 33.5 MB in 33 us (6.1 TB/s read and written), the
+//                         gradient's five in 65 us (4.6).
+//   cross_forward_kernel  persistent CTAs; an item is MT = 1 or 2 tiles of 128
+//                         query rows, walked over key tiles of KN (128 for DP 64,
+//                         64 for DP 128).  A warp streams K and V tiles by TMA
+//                         through a ring of 32 KiB slots; a warp per row tile
+//                         issues its MMAs; a warpgroup per row tile, one thread
+//                         per row, keeps the running maximum and sum of the
+//                         softmax, turns S (TMEM) into the two planes of P in
+//                         place, and adds O.  The row tiles run half a period
+//                         apart: one is in the softmax while the other has the
+//                         tensor core.  4 x 16 heads of 64, 2048 x 2048 tokens:
+//                         215 us, 320 TFLOP/s of f32 products (960 of fp16, two
+//                         thirds of the sustained cuBLAS rate).
 //   cross_backward_kernel dq (rows: queries, walking keys) or dk and dv (rows:
 //                         keys, walking queries); both need S and dP = dout v^T
 //                         of the tile, and write each result once: no atomics,
 //                         at the price of computing S and dP twice.  Two
 //                         warpgroups share the 128 rows and halve the columns.
-//   cross_sum_kernel      joins parts of a split walk in a fixed order.
+//                         The same case: 280 us and 400 us (740 and 1030
+//                         TFLOP/s of fp16 products).
+//   cross_join_kernel (cross_attention.cu), cross_sum_kernel
+//                         join the parts of a walk that was split over CTAs, in
+//                         a fixed order.
+//
+// What bounds the two tensor-core kernels: the hand-overs between softmax and
+// tensor core.  Per 128 x 128 tile the MMAs of the forward take 1560 cycles
+// (every product at the full rate), the softmax of a warp 1700, and each of the
+// three hand-overs (S, P, O) about 500.
 //
 // Every wait is bounded; a CTA whose wait runs out sets the async-error word,
 // waits (bounded) for its own copies and MMAs, frees its tensor memory and

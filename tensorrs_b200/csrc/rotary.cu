@@ -20,6 +20,9 @@
 // vectors of a head (V pairs); kHeads heads are loaded before the first is
 // used, which keeps 2 kHeads (4 kHeads) 16-byte loads of a lane in flight.
 // The sums of a row (x^2, dn n) are folded over the group with shuffles.
+// Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 62 us rotated
+// (5.4 TB/s, 0.84 of the copy rate), 68 us normed and rotated (4.9 TB/s); the
+// norm's gradient of 4096 tokens of 20 heads of 64 (63 MB) 22 us.
 //
 // Angles: the product p f_i is taken in f64 (positions of a long context times
 // a frequency of 1 lose the fraction of a turn in f32); for f32 tensors the
