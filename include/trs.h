@@ -185,9 +185,9 @@ uint64_t trs_scratch_alloc_count(void);
 /* Reads and clears the current device's async-error word.  A kernel that
  * waits gives up after a bounded number of polls, sets a bit of this word and
  * returns instead of hanging: bit 0 (1) when it waited on its own bulk
- * copies, bit 1 (2) when a sharded sum waited on a peer rank's partial;
- * *code receives the word (0 = none).  Synchronises the device.  Returns
- * TRS_ERR_TIMEOUT when the word was set. */
+ * copies or tensor-core products, bit 1 (2) when a sharded sum waited on a peer
+ * rank's partial; *code receives the word (0 = none).  Synchronises the device.
+ * Returns TRS_ERR_TIMEOUT when the word was set. */
 trs_status trs_async_error(int32_t* code);
 
 /* ------------------------------------------------------------------ */
@@ -551,11 +551,12 @@ trs_status trs_head_norm_rotary_backward(
  * -inf.  lse is [B, Hq, Tq] or NULL; the backward needs it.  The scale is
  * finite, of either sign.
  *
- * Up to D = 128 more than 16 query rows per key head run on the tensor cores
- * (tcgen05): every operand as two fp16 parts under a power of two per tile of
- * 8192 elements, three products each, accumulated in f32, results within a few
- * f32 roundings of the sums' terms (elements below 2^-17 of their tile's
- * largest are off by 2^-40 of that).  Fewer rows, and larger heads, run on the
+ * Up to D = 128 more than 16 query rows per key head (8 for D above 64), and
+ * gradients, run on the tensor cores (tcgen05; fewer than 2^29 rows of all
+ * heads, TRS_ERR_SHAPE otherwise): every operand as two fp16 parts under a
+ * power of two per tile of 8192 elements, three products each, accumulated in
+ * f32, results within a few f32 roundings of the sums' terms (elements below
+ * 2^-17 of their tile's largest are off by 2^-40 of that).  Fewer rows, and larger heads, run on the
  * CUDA cores in f32, as does a whole call whose inputs hold an infinity or a
  * NaN (found on the device; these propagate as in the formulas).  Workspaces
  * come from the stream-ordered pool.  Outputs may overlap nothing

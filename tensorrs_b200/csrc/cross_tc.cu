@@ -1239,8 +1239,8 @@ Error plane_map(EncodeTiled enc, CUtensorMap* map, const __half* hi, int64_t row
 
 int up_to(int x, int m) { return (x + m - 1) / m * m; }
 
-void place(Arena& a, Packed& p, int np, int rows, int DP, bool norm) {
-  p.rows_p = up_to(rows, 256);
+void place(Arena& a, Packed& p, int np, int rows, int DP, bool norm, int pad = 128) {
+  p.rows_p = up_to(rows, pad);
   p.rows_all = np * p.rows_p;
   p.hi = a.take<__half>((size_t)p.rows_all * DP * 2);
   p.lo = p.hi + (size_t)p.rows_all * DP;
@@ -1376,7 +1376,7 @@ Error cross_tc_forward(const CrossDev& call, cudaStream_t stream) {
   for (int pass = 0; pass < 2; ++pass) {
     Arena a;
     if (pass) a.base = buf.as<char>();
-    place(a, q, np, c.M, DP, false);
+    place(a, q, np, c.M, DP, false, MT * 128);
     place(a, k, np, c.Tk, DP, false);
     place(a, v, np, c.Tk, DP, false);
     if (f.splits > 1) {
