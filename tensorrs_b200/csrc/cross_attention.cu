@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kRowsThreads, NR * NV <= 2 ? 4 : NR * NV <= 4 
   extern __shared__ float s_acc[];                      // [NG][NR][DP]
   const int gid = threadIdx.x / L, lane = threadIdx.x % L;
   const int mine = lane * OWN / DUP % U;                // this lane's first key of the four
-  const unsigned mask = L == 32 ? 0xffffffffu : (0xffffu << (threadIdx.x & 16));
+  const unsigned mask = (L == 32 ? 0xffffffffu : (1u << (L & 31)) - 1u) << (threadIdx.x % 32 / L * L);
   for (int item = blockIdx.x; item < d.items; item += gridDim.x) {
     const int sp = item % d.splits, rb = item / d.splits % d.blocks, pr = item / d.splits / d.blocks;
     const int b = pr / c.Hk, hk = pr % c.Hk;
@@ -377,6 +377,10 @@ Error run_rows(const CrossDev& c, cudaStream_t s) {
   RowsDev d;
   std::memset(static_cast<void*>(&d), 0, sizeof(d));
   d.c = c;
+  if (c.D <= 32) {
+    return c.M == 1 ? launch_rows<1, 8, 1>(d, s) : c.M == 2 ? launch_rows<2, 8, 1>(d, s)
+           : c.M <= 4 ? launch_rows<4, 8, 1>(d, s) : launch_rows<8, 8, 1>(d, s);
+  }
   if (c.D <= 64) {
     return c.M == 1 ? launch_rows<1, 16, 1>(d, s) : c.M == 2 ? launch_rows<2, 16, 1>(d, s)
            : c.M <= 4 ? launch_rows<4, 16, 1>(d, s) : launch_rows<8, 16, 1>(d, s);

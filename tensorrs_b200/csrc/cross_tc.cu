@@ -304,28 +304,31 @@ constexpr uint32_t idesc_f16(int n, bool mn) {
   return (1u << 4) | (mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// D = A B^T over DP: A 128 rows, B KN rows, both in shared memory (planes as
+// Head sizes up to DE (64, 96, 128) take the products over DE elements; DP (64,
+// 128) is what a row of the planes holds, zeros from the head size on.
+
+// D = A B^T over DE: A 128 rows, B KN rows, both in shared memory (planes as
 // load_planes leaves them); the two small products first.
-template <int DP, int KN>
+template <int DP, int DE, int KN>
 __device__ __forceinline__ void mma_abt(uint32_t lead, uint32_t dst, uint32_t a, uint32_t b) {
   constexpr uint32_t id = idesc_f16(KN, false);
   constexpr int HA = 128 * 128 / 16, HB = KN * 128 / 16, NH = DP / 64;
 #pragma unroll
-  for (int k = 0; k < 4 * NH; ++k) {
+  for (int k = 0; k < DE / 16; ++k) {
     const int ka = k / 4 * HA + k % 4 * 2, kb = k / 4 * HB + k % 4 * 2;
     umma_f16_ss<id>(lead, dst, a + NH * HA + ka, b + kb, k > 0);
     umma_f16_ss<id>(lead, dst, a + ka, b + NH * HB + kb, 1);
   }
 #pragma unroll
-  for (int k = 0; k < 4 * NH; ++k)
+  for (int k = 0; k < DE / 16; ++k)
     umma_f16_ss<id>(lead, dst, a + k / 4 * HA + k % 4 * 2, b + k / 4 * HB + k % 4 * 2, 1);
 }
 
 // D = A B over KN: A 128 x KN in tensor memory (chunks of 32 columns: 16
-// columns of hi, 16 of lo), B KN rows of DP columns in shared memory.
-template <int DP, int KN>
+// columns of hi, 16 of lo), B KN rows of DE columns in shared memory.
+template <int DP, int DE, int KN>
 __device__ __forceinline__ void mma_ab(uint32_t lead, uint32_t dst, uint32_t a, uint32_t b) {
-  constexpr uint32_t id = idesc_f16(DP, true);
+  constexpr uint32_t id = idesc_f16(DE, true);
   constexpr int LO = DP / 64 * KN * 128 / 16;
 #pragma unroll
   for (int k = 0; k < KN / 16; ++k) {
@@ -421,7 +424,7 @@ __device__ __forceinline__ FwdItem fwd_item(const FwdDev& d, int item) {
   return w;
 }
 
-template <int DP, int MT>
+template <int DP, int DE, int MT>
 __global__ void __launch_bounds__(MT * 128 + 128, 1)
 cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ FwdDev d) {
@@ -530,7 +533,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         if (!ok) break;
         ++qi;
         tc_fence_after();
-        mma_abt<DP, KN>(lead, ts, dq, dk + slot * SLOT);
+        mma_abt<DP, DE, KN>(lead, ts, dq, dk + slot * SLOT);
         umma_commit(lead, &s_full[t]);
         umma_commit(lead, &empty[slot]);
         if (n == 1) umma_commit(lead, q_empty);
@@ -543,11 +546,11 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           if (!ok) break;
           ++pc;
           tc_fence_after();
-          mma_ab<DP, KN>(lead, ts + KN + (OB == 2 ? (j & 1) * DP : 0), ts, dv + sv * SLOT);
+          mma_ab<DP, DE, KN>(lead, ts + KN + (OB == 2 ? (j & 1) * DP : 0), ts, dv + sv * SLOT);
           if (NS < 5) umma_commit(lead, &empty[sv]);
           if (more) {
             if (NS < 5 && !(ok = wait_all(&full[sk], pk))) break;
-            mma_abt<DP, KN>(lead, ts, dq, dk + sk * SLOT);
+            mma_abt<DP, DE, KN>(lead, ts, dq, dk + sk * SLOT);
           }
           umma_commit(lead, &s_full[t]);
           if (NS >= 5) umma_commit(lead, &empty[sv]);
@@ -583,16 +586,16 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         fq = d.f * d.q.inv[w.pr * qtiles + ((w.mtile * MT + t) * 128 + rl) / KN];
       }
       float m = -INFINITY, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
-      float acc[DP];
+      float acc[DE];
 #pragma unroll
-      for (int i = 0; i < DP; ++i) acc[i] = 0.f;
+      for (int i = 0; i < DE; ++i) acc[i] = 0.f;
       // adds tile j's P V, complete, to the output
       auto add_output = [&](int j) {
         const uint32_t src = obase + (OB == 2 ? (j & 1) * DP : 0);
         const float fv = d.v.inv[kt + j];
         const uint64_t fv2 = pack2(fv, fv), keep2 = pack2(keep, keep);
 #pragma unroll
-        for (int cc = 0; cc < DP / 32; ++cc) {
+        for (int cc = 0; cc < DE / 32; ++cc) {
           uint32_t o[32];
           tmem_ld32_issue(src + cc * 32, o);
           tmem_ld_done(o);
@@ -676,7 +679,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           const int64_t at = ((int64_t)w.sp * np + w.pr) * d.q.rows_p + row;
           float4* o = reinterpret_cast<float4*>(d.part + at * DP);
 #pragma unroll
-          for (int i = 0; i < DP / 4; ++i) o[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+          for (int i = 0; i < DE / 4; ++i) o[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
           d.part_m[at] = m - 15.f;  // acc and l carry 2^15
           d.part_l[at] = l;
         } else {
@@ -685,13 +688,13 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           const float inv = l == 0.f ? 0.f : 1.f / l;
           if (c.vec) {
 #pragma unroll
-            for (int i = 0; i < DP / 4; ++i)
+            for (int i = 0; i < DE / 4; ++i)
               if (4 * i < c.D)
                 reinterpret_cast<float4*>(op)[i] =
                     make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv, acc[4 * i + 3] * inv);
           } else {
 #pragma unroll
-            for (int i = 0; i < DP; ++i)
+            for (int i = 0; i < DE; ++i)
               if (i < c.D) op[i * c.out.sd] = acc[i] * inv;
           }
           if (c.lse) c.lse[w.b * c.ls_b + h * c.ls_h + tt * c.ls_t] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * kLn2;
@@ -753,14 +756,14 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdDev& d, int item) {
   return w;
 }
 
-template <int DP, bool KV>
+template <int DP, int DE, bool KV>
 __global__ void __launch_bounds__(384, 1)
 cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_constant__ CUtensorMap ma2,
                       const __grid_constant__ CUtensorMap mb1, const __grid_constant__ CUtensorMap mb2,
                       const __grid_constant__ BwdDev d) {
   using S = BwdShape<DP>;
   constexpr int KN = S::KN, N1 = S::n1, N2 = S::n2, HC = KN / 2;  // HC: columns of a warpgroup
-  constexpr int AC = KV ? DP : DP / 2;                            // result columns of a warpgroup
+  constexpr int AC = KV ? DE : (DE + 63) / 64 * 32;               // result columns of a warpgroup (of 96: 64 and 32)
   // dq needs no plane of P, so dS takes the place of S, and the next dP can be
   // issued before the product that reads dS
   constexpr bool DS_IN_S = !KV && S::ahead;
@@ -879,11 +882,11 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       auto s_ready = [&](int t) { return wait_all(&full1[t % N1], t / N1); };
       auto dp_ready = [&](int t) { return wait_all(&full2[t % N2], t / N2); };
       auto s_mma = [&](int t) {
-        mma_abt<DP, KN>(lead, tm + (t & 1) * KN, d1, r1 + t % N1 * SLOT);
+        mma_abt<DP, DE, KN>(lead, tm + (t & 1) * KN, d1, r1 + t % N1 * SLOT);
         umma_commit(lead, &s_full[t & 1]);
       };
       auto dp_mma = [&](int t) {
-        mma_abt<DP, KN>(lead, dpc, d2, r2 + t % N2 * SLOT);
+        mma_abt<DP, DE, KN>(lead, dpc, d2, r2 + t % N2 * SLOT);
         umma_commit(lead, dp_full);
       };
       int t0 = 0, ai = 0;
@@ -911,7 +914,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
             ok = wait_all(&p_ready[t & 1], t >> 1) && (t == 0 || wait_all(r_free, t - 1));
             if (!ok) break;
             tc_fence_after();
-            mma_ab<DP, KN>(lead, rc2, tm + (t & 1) * KN, c2 + t % N2 * SLOT);  // P^T dout
+            mma_ab<DP, DE, KN>(lead, rc2, tm + (t & 1) * KN, c2 + t % N2 * SLOT);  // P^T dout
             umma_commit(lead, &empty2[t % N2]);
           }
           if (!S::ahead && more) {
@@ -921,7 +924,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
           if (!(ok = wait_all(ds_ready, t))) break;
           tc_fence_after();
           if (DS_IN_S && more) dp_mma(t + 1);
-          mma_ab<DP, KN>(lead, rc1, DS_IN_S ? tm + (t & 1) * KN : dpc, c1 + t % N1 * SLOT);  // dS k, or dS^T q
+          mma_ab<DP, DE, KN>(lead, rc1, DS_IN_S ? tm + (t & 1) * KN : dpc, c1 + t % N1 * SLOT);  // dS k, or dS^T q
           if (!KV && S::ahead && more) umma_commit(lead, &empty2[(t + 1) % N2]);
           umma_commit(lead, r_full);
           umma_commit(lead, &empty1[t % N1]);
@@ -1054,6 +1057,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         if (KV && j > 0) {
 #pragma unroll
           for (int cc = 0; cc < AC / 32; ++cc) {
+            if (!KV && wg * AC + cc * 32 >= DE) continue;
             uint32_t o[32];
             tmem_ld32_issue(t_res + cc * 32, o);
             tmem_ld_done(o);
@@ -1094,6 +1098,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
           tc_fence_after();
 #pragma unroll
           for (int cc = 0; cc < AC / 32; ++cc) {
+            if (!KV && wg * AC + cc * 32 >= DE) continue;
             uint32_t o[32];
             tmem_ld32_issue(t_res + cc * 32, o);
             tmem_ld_done(o);
@@ -1112,6 +1117,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         const float wt = weight(n - 1);
 #pragma unroll
         for (int cc = 0; cc < AC / 32; ++cc) {
+          if (!KV && wg * AC + cc * 32 >= DE) continue;
           uint32_t o[32];
           tmem_ld32_issue(t_res + cc * 32, o);
           tmem_ld_done(o);
@@ -1299,21 +1305,21 @@ Error too_large(const CrossDev& c) {
   return Error{};
 }
 
-template <int DP, int MT>
+template <int DP, int DE, int MT>
 Error launch_forward(const Packed& q, const Packed& k, const Packed& v, FwdDev& f, cudaStream_t stream) {
   using S = FwdShape<DP, MT>;
-  auto kern = cross_forward_kernel<DP, MT>;
+  auto kern = cross_forward_kernel<DP, DE, MT>;
   allow_smem((const void*)kern, S::smem);
   f.items = f.mtiles * f.c.B * f.c.Hk * f.splits;
   return launch_after(kern, dim3((unsigned)std::min(f.items, current_device_info().sm_count)), S::threads, S::smem, stream,
                       "cross attention forward kernel", q.map128, k.mapKN, v.mapKN, f);
 }
 
-template <int DP, bool KV>
+template <int DP, int DE, bool KV>
 Error launch_backward(const Packed& a1, const Packed& a2, const Packed& b1, const Packed& b2, BwdDev& f,
                       cudaStream_t stream) {
   using S = BwdShape<DP>;
-  auto kern = cross_backward_kernel<DP, KV>;
+  auto kern = cross_backward_kernel<DP, DE, KV>;
   allow_smem((const void*)kern, S::smem);
   f.items = f.mtiles * f.c.B * f.c.Hk * f.splits;
   return launch_after(kern, dim3((unsigned)std::min(f.items, current_device_info().sm_count)), S::threads, S::smem, stream,
@@ -1407,8 +1413,9 @@ Error cross_tc_forward(const CrossDev& call, cudaStream_t stream) {
   f.v = v.planes();
   f.f = fabsf(c.scale) * kLog2e;
   f.err = async_error_word();
-  if (DP == 64) e = MT == 2 ? launch_forward<64, 2>(q, k, v, f, stream) : launch_forward<64, 1>(q, k, v, f, stream);
-  else e = MT == 2 ? launch_forward<128, 2>(q, k, v, f, stream) : launch_forward<128, 1>(q, k, v, f, stream);
+  if (DP == 64) e = MT == 2 ? launch_forward<64, 64, 2>(q, k, v, f, stream) : launch_forward<64, 64, 1>(q, k, v, f, stream);
+  else if (c.D <= 96) e = MT == 2 ? launch_forward<128, 96, 2>(q, k, v, f, stream) : launch_forward<128, 96, 1>(q, k, v, f, stream);
+  else e = MT == 2 ? launch_forward<128, 128, 2>(q, k, v, f, stream) : launch_forward<128, 128, 1>(q, k, v, f, stream);
   if (!e.ok() || f.splits == 1) return e;
   return cross_join(c, f.splits, q.rows_p, DP, f.part, f.part_m, f.part_l, stream);
 }
@@ -1495,9 +1502,13 @@ Error cross_tc_backward(const CrossDev& call, cudaStream_t stream) {
   k_d.a2 = v.planes();
   k_d.b1 = q.planes();
   k_d.b2 = g.planes();
-  e = DP == 64 ? launch_backward<64, false>(q, g, k, v, q_d, stream) : launch_backward<128, false>(q, g, k, v, q_d, stream);
+  e = DP == 64      ? launch_backward<64, 64, false>(q, g, k, v, q_d, stream)
+      : c.D <= 96 ? launch_backward<128, 96, false>(q, g, k, v, q_d, stream)
+                    : launch_backward<128, 128, false>(q, g, k, v, q_d, stream);
   if (!e.ok()) return e;
-  e = DP == 64 ? launch_backward<64, true>(k, v, q, g, k_d, stream) : launch_backward<128, true>(k, v, q, g, k_d, stream);
+  e = DP == 64      ? launch_backward<64, 64, true>(k, v, q, g, k_d, stream)
+      : c.D <= 96 ? launch_backward<128, 96, true>(k, v, q, g, k_d, stream)
+                    : launch_backward<128, 128, true>(k, v, q, g, k_d, stream);
   if (!e.ok()) return e;
   if (q_d.splits > 1 || k_d.splits > 1) {
     SumDev sd;

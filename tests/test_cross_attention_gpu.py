@@ -67,6 +67,8 @@ SIZES = [
     (1, 64, 64, 1, 1, 128), (1, 128, 63, 2, 2, 128), (2, 130, 129, 2, 1, 128), (1, 300, 200, 1, 1, 80), (1, 40, 333, 7, 1, 96),
     (1, 19, 257, 1, 1, 7), (1, 5, 70, 2, 2, 160), (1, 20, 33, 2, 1, 256), (1, 1, 1, 1, 1, 1), (1, 16, 2, 1, 1, 130),
     (1, 1, 1500, 8, 1, 64), (1, 2, 1000, 8, 1, 128), (2, 512, 512, 2, 2, 64), (1, 513, 260, 2, 1, 100),
+    (1, 300, 300, 1, 1, 96), (1, 300, 300, 1, 1, 97), (1, 40, 2000, 1, 1, 72), (1, 1500, 40, 1, 1, 96), (2, 200, 150, 3, 1, 65),
+    (2, 1, 500, 7, 1, 32), (1, 2, 300, 8, 2, 24), (2, 1, 700, 2, 2, 32), (1, 1, 64, 4, 1, 17),
 ]
 
 
