@@ -551,8 +551,8 @@ trs_status trs_head_norm_rotary_backward(
  * -inf.  lse is [B, Hq, Tq] or NULL; the backward needs it.  The scale is
  * finite, of either sign.
  *
- * Up to D = 128 more than 16 query rows per key head (8 for D above 64), and
- * gradients, run on the tensor cores (tcgen05; fewer than 2^29 rows of all
+ * Up to D = 128 more than 16 query rows per key head (8 for D above 64 and for
+ * gradients) run on the tensor cores (tcgen05; fewer than 2^29 rows of all
  * heads, TRS_ERR_SHAPE otherwise): every operand as two fp16 parts under a
  * power of two per tile of 8192 elements, three products each, accumulated in
  * f32, results within a few f32 roundings of the sums' terms (elements below

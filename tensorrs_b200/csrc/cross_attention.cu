@@ -61,6 +61,33 @@ __device__ __forceinline__ Quad load4(const float* p, int d, int D, int64_t sd) 
   return q;
 }
 
+// N sums over the L lanes of a group: each step a lane hands over the half that
+// its partner keeps, so that N dot products take about N + log2 L shuffles
+// instead of N log2 L.  Sum i ends in s[i % OWN] of lanes i DUP / OWN .. (OWN =
+// N / L where N > L, DUP = L / N where N < L, else 1).
+template <int L, int N>
+__device__ __forceinline__ void fold_lanes(float (&s)[N], int lane, unsigned mask) {
+#pragma unroll
+  for (int o = L / 2, w = N / 2; o > 0; o >>= 1, w >>= 1) {
+    if (w > 0) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < (w > 0 ? w : 1); ++i) {
+        const float give = up ? s[i] : s[i + w], keep = up ? s[i + w] : s[i];
+        s[i] = keep + __shfl_xor_sync(mask, give, o);
+      }
+    } else {
+      s[0] += __shfl_xor_sync(mask, s[0], o);
+    }
+  }
+}
+
+__device__ __forceinline__ float dot4(const Quad& x, const Quad& y) {
+  float lo, hi;
+  unpack2(fma2(x.b, y.b, mul2(x.a, y.a)), &lo, &hi);
+  return lo + hi;
+}
+
 // Two to four CTAs per SM where the rows leave the registers for it: the bytes
 // in flight per SM carry this kernel.
 template <int NR, int L, int NV, bool VEC>
@@ -125,22 +152,7 @@ __global__ void __launch_bounds__(kRowsThreads, NR * NV <= 2 ? 4 : NR * NV <= 4 
           unpack2(x, &lo, &hi);
           s[r * U + u] = lo + hi;
         }
-      // fold over the lanes: each step a lane hands over the half that the
-      // other keeps, so that N dot products take about N + log2 L shuffles
-      // instead of N log2 L, and each exponential is taken once
-#pragma unroll
-      for (int o = L / 2, w = N / 2; o > 0; o >>= 1, w >>= 1) {
-        if (w > 0) {
-          const bool up = lane & o;
-#pragma unroll
-          for (int i = 0; i < (w > 0 ? w : 1); ++i) {
-            const float give = up ? s[i] : s[i + w], keep = up ? s[i + w] : s[i];
-            s[i] = keep + __shfl_xor_sync(mask, give, o);
-          }
-        } else {
-          s[0] += __shfl_xor_sync(mask, s[0], o);
-        }
-      }
+      fold_lanes<L, N>(s, lane, mask);
       float mx = m;
 #pragma unroll
       for (int e = 0; e < OWN; ++e) {
@@ -299,6 +311,154 @@ Error cross_join(const CrossDev& c, int splits, int rows, int ld, const float* p
 
 namespace {
 
+// The gradient of up to 8 query rows per key head (head sizes up to 128): k and
+// v are read once and dk and dv written once, which bounds it.  Groups of lanes
+// own keys as in cross_rows_kernel; a step takes the scores and dP of NR rows
+// and U keys, folds both, and adds each pair's dS and P to dq (in registers to
+// the end of the CTA's keys) and to the key's dk and dv.
+struct RowsGradDev {
+  CrossDev c;
+  int splits;
+  int ld;            // elements per partial row of dq
+  float* part;       // [split][problem][M][ld] when splits > 1
+};
+template <int NR, int L, bool VEC>
+__global__ void __launch_bounds__(kRowsThreads, NR <= 4 ? 2 : 1) cross_rows_grad_kernel(const RowsGradDev d) {
+  const CrossDev& c = d.c;
+  pdl_launch_dependents();
+  constexpr int U = NR == 8 ? 2 : 4, NG = kRowsThreads / L, DP = L * 4, N = NR * U;
+  constexpr int OWN = N > L ? N / L : 1, DUP = N < L ? L / N : 1, LPR = L / NR;
+  extern __shared__ float s_acc[];  // [NG][NR][DP]
+  const int gid = threadIdx.x / L, lane = threadIdx.x % L, dd = lane * 4;
+  const int mine = lane * OWN / DUP % U, my_row = lane / LPR;
+  const unsigned mask = (L == 32 ? 0xffffffffu : (1u << (L & 31)) - 1u) << (threadIdx.x % 32 / L * L);
+  const int sp = blockIdx.x % d.splits, pr = blockIdx.x / d.splits, b = pr / c.Hk, hk = pr % c.Hk;
+  const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
+  const int per = (n + d.splits - 1) / d.splits, k0 = min(n, sp * per), k1 = min(n, k0 + per);
+  Quad q[NR], go[NR], acc[NR];
+  float lse2 = INFINITY, delta = 0.f;  // of this lane's row
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    acc[r] = q[r] = go[r] = Quad{0, 0};
+    if (r >= c.M) continue;
+    const int g = (int)fdiv((uint32_t)r, c.f_Tq), t = r - g * c.Tq, h = hk * c.G + g;
+    auto at = [&](const HeadsDev& x) { return static_cast<const float*>(x.p) + b * x.sb + t * x.st + h * x.sh; };
+    q[r] = load4<VEC>(at(c.q), dd, c.D, c.q.sd);
+    go[r] = load4<VEC>(at(c.dout), dd, c.D, c.dout.sd);
+    float dl = dot4(go[r], load4<VEC>(at(c.out), dd, c.D, c.out.sd));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) dl += __shfl_xor_sync(mask, dl, o);
+    if (my_row == r) {
+      delta = dl;
+      const float ls = c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t];
+      lse2 = ls == -INFINITY ? INFINITY : ls * kLog2e;  // scores of -inf alone: no weight
+    }
+  }
+  const float f = c.scale * kLog2e;
+  auto key_row = [&](const HeadsDev& x, int64_t t) { return static_cast<const float*>(x.p) + b * x.sb + t * x.st + hk * x.sh; };
+  auto store = [&](const HeadsDev& x, int64_t t, const Quad& v) {
+    float* p = const_cast<float*>(key_row(x, t));
+    if (VEC) {
+      if (dd < c.D) *reinterpret_cast<ulonglong2*>(p + dd) = make_ulonglong2(v.a, v.b);
+    } else {
+      float e[4];
+      unpack2(v.a, &e[0], &e[1]);
+      unpack2(v.b, &e[2], &e[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (dd + i < c.D) p[(dd + i) * x.sd] = e[i];
+    }
+  };
+  for (int key = k0 + gid * U; key < k1; key += NG * U) {
+    Quad kk[U], vv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = key + u < k1;
+      kk[u] = on ? load4<VEC>(key_row(c.k, key + u), dd, c.D, c.k.sd) : Quad{0, 0};
+      vv[u] = on ? load4<VEC>(key_row(c.v, key + u), dd, c.D, c.v.sd) : Quad{0, 0};
+    }
+    float s[N], dp[N];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[r * U + u] = dot4(q[r], kk[u]);
+        dp[r * U + u] = dot4(go[r], vv[u]);
+      }
+    fold_lanes<L, N>(s, lane, mask);
+    fold_lanes<L, N>(dp, lane, mask);
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) {
+      s[e] = key + mine + e < k1 ? ex2(__fmaf_rn(s[e], f, -lse2)) : 0.f;
+      dp[e] = key + mine + e < k1 ? s[e] * (dp[e] - delta) * c.scale : 0.f;
+    }
+    Quad dk[U], dv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) dk[u] = dv[u] = Quad{0, 0};
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int from = (r * U + u) * DUP / OWN;
+        const float p = __shfl_sync(mask, s[(r * U + u) % OWN], from, L);
+        const float ds = __shfl_sync(mask, dp[(r * U + u) % OWN], from, L);
+        const uint64_t p2 = pack2(p, p), ds2 = pack2(ds, ds);
+        acc[r] = Quad{fma2(ds2, kk[u].a, acc[r].a), fma2(ds2, kk[u].b, acc[r].b)};
+        dk[u] = Quad{fma2(ds2, q[r].a, dk[u].a), fma2(ds2, q[r].b, dk[u].b)};
+        dv[u] = Quad{fma2(p2, go[r].a, dv[u].a), fma2(p2, go[r].b, dv[u].b)};
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (key + u >= k1) break;
+      store(c.dk, key + u, dk[u]);
+      store(c.dv, key + u, dv[u]);
+    }
+  }
+  // rows at and behind the key length
+  const int tail = c.Tk - n, z1 = n + (int)((int64_t)tail * (sp + 1) / d.splits);
+  for (int key = n + (int)((int64_t)tail * sp / d.splits) + gid; key < z1; key += NG) {
+    store(c.dk, key, Quad{0, 0});
+    store(c.dv, key, Quad{0, 0});
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+    *reinterpret_cast<ulonglong2*>(&s_acc[(gid * NR + r) * DP + dd]) = make_ulonglong2(acc[r].a, acc[r].b);
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < NR * DP; idx += kRowsThreads) {
+    const int r = idx / DP, e = idx % DP;
+    if (r >= c.M || e >= c.D) continue;
+    float sum = 0.f;
+    for (int g = 0; g < NG; ++g) sum += s_acc[(g * NR + r) * DP + e];
+    if (d.splits > 1) {
+      d.part[(((int64_t)sp * (c.B * c.Hk) + pr) * c.M + r) * d.ld + e] = sum;
+    } else {
+      const int g = (int)fdiv((uint32_t)r, c.f_Tq), t = r - g * c.Tq, h = hk * c.G + g;
+      static_cast<float*>(c.dq.p)[b * c.dq.sb + t * c.dq.st + h * c.dq.sh + e * c.dq.sd] = sum;
+    }
+  }
+}
+
+// dq from the parts, in order: a thread per element.
+__global__ void __launch_bounds__(256) cross_rows_sum_kernel(const RowsGradDev d) {
+  pdl_wait();
+  const CrossDev& c = d.c;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, np = (int64_t)c.B * c.Hk;
+  const int e = (int)(i % d.ld);
+  const int64_t w = i / d.ld;
+  if (w >= np * c.M || e >= c.D) return;
+  const int r = (int)(w % c.M), pr = (int)(w / c.M);
+  float sum = 0.f;
+  for (int s0 = 0; s0 < d.splits; s0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = s0 + k < d.splits ? d.part[((s0 + k) * np * c.M + w) * d.ld + e] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += x[k];
+  }
+  const int b = pr / c.Hk, g = (int)fdiv((uint32_t)r, c.f_Tq), t = r - g * c.Tq, h = pr % c.Hk * c.G + g;
+  static_cast<float*>(c.dq.p)[b * c.dq.sb + t * c.dq.st + h * c.dq.sh + e * c.dq.sd] = sum;
+}
+
 // The gradient of head sizes above 128 on the CUDA cores, a warp per row.
 __global__ void __launch_bounds__(256) cross_grad_rows_kernel(const CrossDev c) {
   const int64_t warps = (int64_t)gridDim.x * 8, w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
@@ -330,6 +490,24 @@ Error zero_heads(const HeadsDev& x, int64_t B, int T, int H, int D, cudaStream_t
 
 // ---- host side -------------------------------------------------------------------
 
+// The parts of the keys (256 keys each at least: a part's fixed cost is that of
+// about 100) that leave the fewest CTA places idle in the last wave, up to four
+// waves; `base` CTAs without parts.
+int64_t key_parts(const void* kernel, int smem, int64_t base, int Tk) {
+  const int64_t resident = (int64_t)current_device_info().sm_count * resident_blocks_smem(kernel, kRowsThreads, smem);
+  int64_t splits = 1;
+  double best = 0.0;
+  for (int64_t n = 1; n <= std::max(1, Tk / 256) && (n == 1 || n * base <= 4 * resident); ++n) {
+    const int64_t waves = (n * base + resident - 1) / resident;
+    const double use = (double)(n * base) / (double)(waves * resident);
+    if (use > best + 0.02) {
+      best = use;
+      splits = n;
+    }
+  }
+  return splits;
+}
+
 template <int NR, int L, int NV>
 Error launch_rows(RowsDev& d, cudaStream_t s) {
   const CrossDev& c = d.c;
@@ -338,21 +516,8 @@ Error launch_rows(RowsDev& d, cudaStream_t s) {
   allow_smem((const void*)k, smem);
   const int np = c.B * c.Hk;
   d.blocks = (c.M + NR - 1) / NR;
-  // the parts of the keys (256 keys each at least: a part's fixed cost is that
-  // of about 100) that leave the fewest CTA places idle in the last wave, up to
-  // four waves
-  const int64_t resident = (int64_t)current_device_info().sm_count * resident_blocks_smem((const void*)k, kRowsThreads, smem);
   const int64_t base = (int64_t)np * d.blocks;
-  int64_t splits = 1;
-  double best = 0.0;
-  for (int64_t n = 1; n <= std::max<int64_t>(1, c.Tk / 256) && (n == 1 || n * base <= 4 * resident); ++n) {
-    const int64_t waves = (n * base + resident - 1) / resident;
-    const double use = (double)(n * base) / (double)(waves * resident);
-    if (use > best + 0.02) {
-      best = use;
-      splits = n;
-    }
-  }
+  const int64_t splits = key_parts((const void*)k, smem, base, c.Tk);
   const int64_t items = base * splits;
   if (items >= (1ll << 31)) return make_error(TRS_ERR_SHAPE, "cross_attention: too many query rows");
   d.splits = (int)splits;
@@ -390,6 +555,36 @@ Error run_rows(const CrossDev& c, cudaStream_t s) {
            : c.M <= 4 ? launch_rows<4, 32, 1>(d, s) : launch_rows<8, 32, 1>(d, s);
   }
   return c.M == 1 ? launch_rows<1, 32, 2>(d, s) : c.M == 2 ? launch_rows<2, 32, 2>(d, s) : launch_rows<4, 32, 2>(d, s);
+}
+
+template <int NR, int L>
+Error launch_rows_grad(const CrossDev& c, cudaStream_t s) {
+  RowsGradDev d;
+  std::memset(static_cast<void*>(&d), 0, sizeof(d));
+  d.c = c;
+  constexpr int smem = kRowsThreads / L * NR * L * 4 * 4;
+  auto k = c.vec ? cross_rows_grad_kernel<NR, L, true> : cross_rows_grad_kernel<NR, L, false>;
+  allow_smem((const void*)k, smem);
+  const int64_t np = (int64_t)c.B * c.Hk, splits = key_parts((const void*)k, smem, np, c.Tk);
+  d.splits = (int)splits;
+  d.ld = (c.D + 3) / 4 * 4;
+  Scratch part;
+  if (splits > 1) {
+    Error e = part.alloc(sizeof(float) * (size_t)(splits * np * c.M) * d.ld, s);
+    if (!e.ok()) return e;
+    d.part = part.as<float>();
+  }
+  k<<<(unsigned)(np * splits), kRowsThreads, smem, s>>>(d);
+  Error e = check_launch("cross attention rows gradient kernel");
+  if (!e.ok() || splits == 1) return e;
+  return launch_after(cross_rows_sum_kernel, dim3((unsigned)((np * c.M * d.ld + 255) / 256)), 256, 0, s,
+                      "cross attention rows sum kernel", d);
+}
+
+template <int L>
+Error run_rows_grad(const CrossDev& c, cudaStream_t s) {
+  return c.M == 1 ? launch_rows_grad<1, L>(c, s) : c.M == 2 ? launch_rows_grad<2, L>(c, s)
+         : c.M <= 4 ? launch_rows_grad<4, L>(c, s) : launch_rows_grad<8, L>(c, s);
 }
 
 struct CrossCall {
@@ -518,6 +713,8 @@ Error run_cross(const CrossCall& c, bool backward, cudaStream_t stream) {
   // the tensor-core path splits them.  4 x 16 heads, 2048 keys, CUDA cores and
   // tensor cores: heads of 64, 16 rows 40 and 58 us, 24 rows 66 and 58; heads
   // of 128, 8 rows 58 and 94, 16 rows 97 and 94
+  if (backward && D <= 128 && d.M <= 8)
+    return D <= 32 ? run_rows_grad<8>(d, stream) : D <= 64 ? run_rows_grad<16>(d, stream) : run_rows_grad<32>(d, stream);
   const bool tc = D <= 128 && (backward || d.M > (D <= 64 ? 16 : 8));
   if (!tc) {
     if (!backward) return run_rows(d, stream);

@@ -1255,9 +1255,13 @@ void place(Arena& a, Packed& p, int np, int rows, int DP, bool norm, int pad = 1
   p.norm = norm ? a.take<float>(tiles) : nullptr;
 }
 
-Error maps(EncodeTiled enc, Packed& p, int DP) {
-  Error e = plane_map(enc, &p.map128, p.hi, 2ll * p.rows_all, DP, 128);
-  if (e.ok()) e = plane_map(enc, &p.mapKN, p.hi, 2ll * p.rows_all, DP, kTileElems / DP);
+// The operand's maps: boxes of a row tile (128 rows), of a streamed tile.
+Error maps(EncodeTiled enc, Packed& p, int DP, bool rows, bool stream) {
+  const int KN = kTileElems / DP;
+  Error e;
+  if (rows || KN == 128) e = plane_map(enc, &p.map128, p.hi, 2ll * p.rows_all, DP, 128);
+  if (KN == 128) p.mapKN = p.map128;
+  else if (e.ok() && stream) e = plane_map(enc, &p.mapKN, p.hi, 2ll * p.rows_all, DP, KN);
   return e;
 }
 
@@ -1396,9 +1400,9 @@ Error cross_tc_forward(const CrossDev& call, cudaStream_t stream) {
       if (!e.ok()) return e;
     }
   }
-  e = maps(enc, q, DP);
-  if (e.ok()) e = maps(enc, k, DP);
-  if (e.ok()) e = maps(enc, v, DP);
+  e = maps(enc, q, DP, true, false);
+  if (e.ok()) e = maps(enc, k, DP, false, true);
+  if (e.ok()) e = maps(enc, v, DP, false, true);
   if (!e.ok()) return e;
   PackDev p;
   std::memset(static_cast<void*>(&p), 0, sizeof(p));
@@ -1467,10 +1471,10 @@ Error cross_tc_backward(const CrossDev& call, cudaStream_t stream) {
       if (!e.ok()) return e;
     }
   }
-  e = maps(enc, q, DP);
-  if (e.ok()) e = maps(enc, g, DP);
-  if (e.ok()) e = maps(enc, k, DP);
-  if (e.ok()) e = maps(enc, v, DP);
+  for (Packed* x : {&q, &g, &k, &v}) {
+    e = maps(enc, *x, DP, true, true);
+    if (!e.ok()) return e;
+  }
   if (!e.ok()) return e;
   PackDev p;
   std::memset(static_cast<void*>(&p), 0, sizeof(p));

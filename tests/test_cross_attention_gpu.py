@@ -128,6 +128,10 @@ def test_strides():
     both(q, k, v, go, 0.2, dev=perm)
     slow = [cuda(x.transpose(3, 0, 1, 2)).permute(1, 2, 3, 0) for x in (q, k, v, go)]
     both(q, k, v, go, 0.2, dev=slow)
+    # the same with few query rows (CUDA cores)
+    q1, g1 = q[:, :3], go[:, :3]
+    both(q1, k, v, g1, 0.2, dev=(perm[0][:, :3], perm[1], perm[2], perm[3][:, :3]))
+    both(q1, k, v, g1, 0.2, dev=(slow[0][:, :3], slow[1], slow[2], slow[3][:, :3]))
     # one head broadcast to all as an input
     one = cuda(k[:, :, :1]).expand(2, 50, 2, 32)
     kk = np.broadcast_to(k[:, :, :1], k.shape)
