@@ -556,9 +556,10 @@ trs_status trs_head_norm_rotary_backward(
  * heads, TRS_ERR_SHAPE otherwise): every operand as two fp16 parts under a
  * power of two per tile of 8192 elements, three products each, accumulated in
  * f32, results within a few f32 roundings of the sums' terms (elements below
- * 2^-17 of their tile's largest are off by 2^-40 of that).  Fewer rows, and larger heads, run on the
- * CUDA cores in f32, as does a whole call whose inputs hold an infinity or a
- * NaN (found on the device; these propagate as in the formulas).  Workspaces
+ * 2^-17 of their tile's largest are off by 2^-40 of that).  Fewer rows, and
+ * larger heads, run on the CUDA cores in f32, as does a whole call whose inputs
+ * hold an infinity or a NaN (found on the device; these propagate as in the
+ * formulas, and a row whose scores are all -inf counts as empty).  Workspaces
  * come from the stream-ordered pool.  Outputs may overlap nothing
  * (TRS_ERR_ALIAS); repeated calls give the same bits. */
 trs_status trs_cross_attention(const trs_view* q, const trs_view* k,

@@ -21,7 +21,7 @@
 // used, which keeps 2 kHeads (4 kHeads) 16-byte loads of a lane in flight.
 // The sums of a row (x^2, dn n) are folded over the group with shuffles.
 // Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 62 us rotated
-// (5.4 TB/s, 0.84 of the copy rate), 68 us normed and rotated (4.9 TB/s); the
+// (5.4 TB/s, 0.84 of the copy rate), 63 us normed and rotated (5.3 TB/s); the
 // norm's gradient of 4096 tokens of 20 heads of 64 (63 MB) 22 us.
 //
 // Angles: the product p f_i is taken in f64 (positions of a long context times
@@ -179,8 +179,13 @@ __device__ __forceinline__ T group_sum(T x, unsigned mask) {
 
 // V: elements per vector access (1: any strides).  K: units per lane.  UH:
 // heads in flight.  G: lanes per token.
+// The norm's forward is held to the registers of three CTAs per SM (8192 tokens
+// of 40 heads of 128: 67.6 us at the two that it takes by itself, 63.1 at three,
+// 63.0 at four with two heads in flight); the rotation alone is fastest at the
+// three that it takes (62.2; 66.8 at four).
 template <class T, int V, bool IL, int MODE, int G, int K, int UH>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotDev d) {
+__global__ void __launch_bounds__(kRotThreads, MODE == kNormRotate && K == 1 && sizeof(T) == 4 ? 3 : 1)
+rotary_kernel(const RotDev d) {
   const int which = (int64_t)blockIdx.x >= d.blocks0;
   const int64_t blk = which ? (int64_t)blockIdx.x - d.blocks0 : (int64_t)blockIdx.x;
   const int64_t nblk = which ? (int64_t)gridDim.x - d.blocks0 : d.blocks0;
