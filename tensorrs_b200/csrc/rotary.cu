@@ -20,8 +20,8 @@
 // vectors of a head (V pairs); kHeads heads are loaded before the first is
 // used, which keeps 2 kHeads (4 kHeads) 16-byte loads of a lane in flight.
 // The sums of a row (x^2, dn n) are folded over the group with shuffles.
-// Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 62 us rotated
-// (5.4 TB/s, 0.84 of the copy rate), 63 us normed and rotated (5.3 TB/s); the
+// Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 58 us rotated
+// (5.8 TB/s, 0.91 of the copy rate), 63 us normed and rotated (5.3 TB/s); the
 // norm's gradient of 4096 tokens of 20 heads of 64 (63 MB) 22 us.
 //
 // Angles: the product p f_i is taken in f64 (positions of a long context times
@@ -181,10 +181,12 @@ __device__ __forceinline__ T group_sum(T x, unsigned mask) {
 // heads in flight.  G: lanes per token.
 // The norm's forward is held to the registers of three CTAs per SM (8192 tokens
 // of 40 heads of 128: 67.6 us at the two that it takes by itself, 63.1 at three,
-// 63.0 at four with two heads in flight); the rotation alone is fastest at the
-// three that it takes (62.2; 66.8 at four).
+// 63.0 at four with two heads in flight), its gradient to those of three, two
+// in f64 (8192 tokens of 10 heads of 256: 114 us with the forward, 147 without);
+// the rotation alone is fastest at the three that it takes (62.2 us; 66.8 at
+// four, before its loads were issued ahead of the angles).
 template <class T, int V, bool IL, int MODE, int G, int K, int UH>
-__global__ void __launch_bounds__(kRotThreads, MODE == kNormRotate && K == 1 && sizeof(T) == 4 ? 3 : 1)
+__global__ void __launch_bounds__(kRotThreads, MODE == kRotate || K > 1 ? 1 : sizeof(T) == 4 ? 3 : MODE == kNormBackward ? 2 : 1)
 rotary_kernel(const RotDev d) {
   const int which = (int64_t)blockIdx.x >= d.blocks0;
   const int64_t blk = which ? (int64_t)blockIdx.x - d.blocks0 : (int64_t)blockIdx.x;
@@ -223,6 +225,30 @@ rotary_kernel(const RotDev d) {
     const int h0 = (int)((uint32_t)it - tok * d.f_chunks[which].d) * d.hpc;
     const int h1 = h0 + d.hpc < H ? h0 + d.hpc : H;
     const int64_t b = fdiv(tok, d.f_T), t = tok - (uint32_t)b * d.f_T.d;
+    const T* xt = xp + b * X.sb + t * X.st;
+    T* yt = yp + b * Y.sb + t * Y.st;
+    const T* dt = dp + b * DY.sb + t * DY.st;
+    T a[UH][K][V], c[UH][K][V];
+    T ea[MODE == kNormBackward ? UH : 1][K][V], ec[MODE == kNormBackward ? UH : 1][K][V];
+    auto load_heads = [&](int h) {
+#pragma unroll
+      for (int u = 0; u < UH; ++u) {
+        const bool on = h + u < h1;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          load_vec<T, V>(a[u][k], xt + (h + u) * X.sh, un[k].o0, X.sd, on && un[k].v0);
+          load_vec<T, V>(c[u][k], xt + (h + u) * X.sh, un[k].o1, X.sd, on && un[k].v1);
+          if constexpr (MODE == kNormBackward) {
+            load_vec<T, V>(ea[u][k], dt + (h + u) * DY.sh, un[k].o0, DY.sd, on && un[k].v0);
+            load_vec<T, V>(ec[u][k], dt + (h + u) * DY.sh, un[k].o1, DY.sd, on && un[k].v1);
+          }
+        }
+      }
+    };
+    // on their way while the angles are evaluated (rotation 62.0 -> 57.9 us, f64
+    // norm 128 -> 124); the f32 norm lacks the registers (63.0 -> 64.7)
+    constexpr bool kEarly = MODE == kRotate || sizeof(T) == 8;
+    if (kEarly) load_heads(h0);
     const int64_t pi = b * d.ps_b + t * d.ps_t;
     const double p = d.pos64 ? (double)static_cast<const int64_t*>(d.pos)[pi]
                              : (double)static_cast<const int32_t*>(d.pos)[pi];
@@ -239,9 +265,6 @@ rotary_kernel(const RotDev d) {
         }
       }
     }
-    const T* xt = xp + b * X.sb + t * X.st;
-    T* yt = yp + b * Y.sb + t * Y.st;
-    const T* dt = dp + b * DY.sb + t * DY.st;
     T aa[MODE == kNormBackward ? K : 1][V], ab[MODE == kNormBackward ? K : 1][V];
     if constexpr (MODE == kNormBackward) {
 #pragma unroll
@@ -250,21 +273,7 @@ rotary_kernel(const RotDev d) {
         for (int i = 0; i < V; ++i) aa[k][i] = ab[k][i] = T(0);
     }
     for (int h = h0; h < h1; h += UH) {
-      T a[UH][K][V], c[UH][K][V];
-      T ea[MODE == kNormBackward ? UH : 1][K][V], ec[MODE == kNormBackward ? UH : 1][K][V];
-#pragma unroll
-      for (int u = 0; u < UH; ++u) {
-        const bool on = h + u < h1;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          load_vec<T, V>(a[u][k], xt + (h + u) * X.sh, un[k].o0, X.sd, on && un[k].v0);
-          load_vec<T, V>(c[u][k], xt + (h + u) * X.sh, un[k].o1, X.sd, on && un[k].v1);
-          if constexpr (MODE == kNormBackward) {
-            load_vec<T, V>(ea[u][k], dt + (h + u) * DY.sh, un[k].o0, DY.sd, on && un[k].v0);
-            load_vec<T, V>(ec[u][k], dt + (h + u) * DY.sh, un[k].o1, DY.sd, on && un[k].v1);
-          }
-        }
-      }
+      if (!kEarly || h > h0) load_heads(h);
 #pragma unroll
       for (int u = 0; u < UH; ++u) {
         if (h + u >= h1) break;
