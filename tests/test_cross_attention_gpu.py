@@ -178,6 +178,26 @@ def test_rows_of_uneven_magnitude():
     both(q, k, v, g, 0.125)
 
 
+@pytest.mark.parametrize("what", ["q", "k"])
+def test_the_low_part_of_small_elements_counts(what):
+    """One row 2^20 larger than its tile's others.  The others' parts are then off by 2^-40 of the largest, 2^-20 of
+    themselves, which needs the subnormal numbers of fp16 (without them 2^-28 of the largest, 2^-8).  The scale makes
+    up for the size: a score of D = 64 independent errors of 2^-40 2^20 |q k| is off by 2^-20 * 8 * 4, the weights by
+    twice that and the 2-norm of the result by less than 2^-13."""
+    q, k, v, g = draw(1, 130, 100, 1, 1, 64, seed=17)
+    x = {"q": q, "k": k}[what]
+    x *= np.float32(2.0**-20)
+    x[0, 0] *= np.float32(2.0**20)
+    scale = 0.125 * 2.0**20
+    out, lse = forward(cuda(q), cuda(k), cuda(v), scale)
+    t = Truth(q, k, v, scale)
+    got, want = to_host(out)[0, 1:], t.out[0, 1:]
+    if what == "k":  # the large key takes or loses all weight: rows where it lost
+        lost = np.abs(want - v[0, 0]).max((1, 2)) > 1e-3
+        got, want = got[lost], want[lost]
+    assert len(want) > 20 and np.linalg.norm(got - want) <= 2.0**-13 * np.linalg.norm(want)
+
+
 def test_peaked_rows():
     """Scores of hundreds: one key takes nearly all of the weight."""
     q, k, v, g = draw(1, 140, 180, 1, 1, 64, seed=13)

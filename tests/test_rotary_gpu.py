@@ -35,7 +35,7 @@ def check(got, want, tol, what):
 
 
 def cuda(a):
-    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return torch.from_numpy(np.array(a, order="C")).cuda()
 
 
 # B, T, Hq, Hk, D, R, dtype
