@@ -710,10 +710,45 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
 
 // ---- backward --------------------------------------------------------------------
 
+// The items of a persistent CTA: its first by its number, then whichever is
+// next of all (a counter in global memory), so that ragged lengths even out.  The
+// TMA thread takes them, one ahead, and passes them on through two slots; -1
+// ends the CTA.  Which CTA walks an item changes no result.  Forward and backward
+// against every grid-th item: 8 ragged heads of 128, 7 x 500 queries on up to 900
+// keys, 334 -> 301 us; 16 of 64, 4 x 1024 on up to 1500, 340 -> 327; equal lengths
+// (16 heads of 128, 2 x 2048 on 2048) 1091 -> 1073.  The forward kernel keeps every
+// grid-th: its items are short, and taking them cost 82 -> 84 us (4 x 1024 on up to
+// 1500, 16 heads of 64) to 143 -> 159 (6 x 403 on up to 1878, heads of 80).
+struct ItemRing {
+  int slot[2];
+  uint64_t full[2], empty[2];
+};
+__device__ __forceinline__ void items_init(ItemRing& r, uint32_t takers) {
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&r.full[i], 1);
+    mbar_init(&r.empty[i], takers);
+  }
+}
+// The TMA thread passes on the k-th item.
+__device__ __forceinline__ bool items_put(ItemRing& r, int k, int item, int* failed) {
+  if (k >= 2 && !wait_or_fail(&r.empty[k & 1], (uint32_t)(k / 2 - 1) & 1u, failed)) return false;
+  *(volatile int*)&r.slot[k & 1] = item;
+  mbar_arrive(&r.full[k & 1]);
+  return true;
+}
+// A warp takes the k-th item: -1 after the last, or when some role gave up.
+__device__ __forceinline__ int items_take(ItemRing& r, int k, int* failed) {
+  if (!__all_sync(0xffffffffu, wait_or_fail(&r.full[k & 1], (uint32_t)(k / 2) & 1u, failed))) return -1;
+  const int item = __shfl_sync(0xffffffffu, *(volatile int*)&r.slot[k & 1], 0);
+  warp_arrive(&r.empty[k & 1]);
+  return item;
+}
+
 struct BwdDev {
   CrossDev c;
   Planes a1, a2, b1, b2;       // dq: q, dout, k, v;  dk/dv: k, v, q, dout
   int mtiles, splits, items;
+  int* next;                   // items taken beyond the first of every CTA
   const float *bias, *delta, *rnorm, *dmax;  // per query row; per query tile
   float *part1, *part2;        // [split][problem][a1.rows_p][DP] when splits > 1: dq, or dk and dv
   float f;                     // |scale| log2 e
@@ -769,6 +804,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
   constexpr bool DS_IN_S = !KV && S::ahead;
   static_assert(3 * KN + (KV ? 2 : 1) * DP <= 512, "tensor memory");
   const CrossDev& c = d.c;
+  __shared__ ItemRing items;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sa1 = smem;
@@ -801,6 +837,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       mbar_init(&full2[s], 1);
       mbar_init(&empty2[s], 1);
     }
+    items_init(items, 9);
     mbar_init(a_full, 1);
     mbar_init(a_empty, 1);
     mbar_init(&s_full[0], 1);
@@ -842,7 +879,9 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
     if (warp == 9 && lane == 0) {  // TMA
       int t = 0, i2 = 0, ai = 0;   // column tiles of either operand and row tiles loaded so far
       bool ok = true;
-      for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+      for (int k = 0, item = blockIdx.x, next; ok; item = next, ++k) {
+        if (!(ok = items_put(items, k, item < d.items ? item : -1, failed)) || item >= d.items) break;
+        next = gridDim.x + atomicAdd(d.next, 1);
         const BwdItem w = bwd_item<KN, KV>(d, item);
         if (w.n == 0) continue;
         if (ai > 0 && !(ok = wait_or_fail(a_empty, (uint32_t)(ai - 1) & 1u, failed))) break;
@@ -891,7 +930,9 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       };
       int t0 = 0, ai = 0;
       bool ok = true;
-      for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+      for (int k = 0; ok; ++k) {
+        const int item = items_take(items, k, failed);
+        if (item < 0) break;
         const int n = bwd_item<KN, KV>(d, item).n;
         if (n == 0) continue;
         ok = wait_all(a_full, ai) && s_ready(t0) && dp_ready(t0);
@@ -956,7 +997,9 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
     const int at1 = d.a1.rows_p / KN, bt = d.b1.rows_p / KN;
     int t = 0;  // column tiles so far
     bool ok = true;
-    for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
+    for (int k = 0; ok; ++k) {
+      const int item = items_take(items, k, failed);
+      if (item < 0) break;
       int n, kt, limit;  // column tiles, the first one's index among all, columns of this half from it on
       int64_t qrow;      // per query row: of this row (dq) or of the columns (dk, dv)
       float ia1, ia2, r_norm;
@@ -1342,11 +1385,12 @@ void add_sum(SumOne& s, const float* part, const HeadsDev& out, int splits, int 
   s.n = (int64_t)np * G * T * (DP / 4);
 }
 
-// A zeroed word that the pack kernel sets when an input is not finite.
+// Zeroed words: one that the pack kernel sets when an input is not finite, and
+// the item counters of the two gradient kernels.
 Error flag_word(Scratch& flag, CrossDev& c, cudaStream_t stream, int** word) {
-  Error e = flag.alloc(sizeof(int), stream);
+  Error e = flag.alloc(3 * sizeof(int), stream);
   if (!e.ok()) return e;
-  const cudaError_t ce = cudaMemsetAsync(flag.get(), 0, sizeof(int), stream);
+  const cudaError_t ce = cudaMemsetAsync(flag.get(), 0, 3 * sizeof(int), stream);
   if (ce != cudaSuccess) return cuda_error(ce, "cudaMemsetAsync");
   *word = flag.as<int>();
   c.nonfinite = *word;
@@ -1445,8 +1489,10 @@ Error cross_tc_backward(const CrossDev& call, cudaStream_t stream) {
   std::memset(static_cast<void*>(&q_d), 0, sizeof(q_d));
   q_d.c = c;
   q_d.f = fabsf(c.scale) * kLog2e;
+  q_d.next = nonfinite + 1;
   q_d.err = async_error_word();
   k_d = q_d;
+  k_d.next = nonfinite + 2;
   q_d.mtiles = (c.M + 127) / 128;
   q_d.splits = pick_splits((int64_t)q_d.mtiles * np, (c.Tk + KN - 1) / KN);
   q_d.out_scale = c.scale;

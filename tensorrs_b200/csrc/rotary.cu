@@ -22,7 +22,7 @@
 // The sums of a row (x^2, dn n) are folded over the group with shuffles.
 // Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 58 us rotated
 // (5.8 TB/s, 0.91 of the copy rate), 63 us normed and rotated (5.3 TB/s); the
-// norm's gradient of 4096 tokens of 20 heads of 64 (63 MB) 22 us.
+// norm's gradient of 4096 tokens of 20 heads of 64 (63 MB) 20 us.
 //
 // Angles: the product p f_i is taken in f64 (positions of a long context times
 // a frequency of 1 lose the fraction of a turn in f32); for f32 tensors the

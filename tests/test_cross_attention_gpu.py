@@ -296,6 +296,25 @@ def test_streams_graphs_and_repeats_give_the_same_bits():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("size,lengths", [((6, 700, 900, 8, 8, 64), [900, 0, 3, 129, 900, 500]),
+                                          ((5, 500, 700, 8, 4, 128), [1, 700, 0, 64, 650])], ids=str)
+def test_more_items_than_sms_of_ragged_length(size, lengths):
+    q, k, v, g = draw(*size, seed=19)
+    n = np.array(lengths, np.int32)
+    first = both(q, k, v, g, 0.125, n)
+    q, k, v, g, n = (cuda(x) for x in (q, k, v, g, n))
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, lse = forward(q, k, v, 0.125, n)
+        again = (out, lse, *backward(g, q, k, v, out, lse, 0.125, n))
+    for _ in range(3):
+        for x in again:
+            x.fill_(float("nan"))
+        gr.replay()
+        for x, y in zip(first, again):
+            assert torch.equal(x, y)
+
+
 def test_kernels_never_gave_up_waiting():
     import ctypes
     from tensorrs_b200 import abi
