@@ -389,8 +389,11 @@ __global__ void __launch_bounds__(kRowsThreads, NR <= 4 ? 2 : 1) cross_rows_grad
     fold_lanes<L, N>(dp, lane, mask);
 #pragma unroll
     for (int e = 0; e < OWN; ++e) {
-      s[e] = key + mine + e < k1 ? ex2(__fmaf_rn(s[e], f, -lse2)) : 0.f;
-      dp[e] = key + mine + e < k1 ? s[e] * (dp[e] - delta) * c.scale : 0.f;
+      // no weight behind the last key, and none for a row that only fills up the
+      // block (its score with an infinite key is 0 * inf)
+      const bool on = my_row < c.M && key + mine + e < k1;
+      s[e] = on ? ex2(__fmaf_rn(s[e], f, -lse2)) : 0.f;
+      dp[e] = on ? s[e] * (dp[e] - delta) * c.scale : 0.f;
     }
     Quad dk[U], dv[U];
 #pragma unroll
