@@ -559,9 +559,10 @@ trs_status trs_head_norm_rotary_backward(
  * 2^-17 of their tile's largest are off by 2^-40 of that).  Fewer rows, and
  * larger heads, run on the CUDA cores in f32, as does a whole call whose inputs
  * hold an infinity or a NaN (found on the device; these propagate as in the
- * formulas, and a row whose scores are all -inf counts as empty).  Workspaces
- * come from the stream-ordered pool.  Outputs may overlap nothing
- * (TRS_ERR_ALIAS); repeated calls give the same bits. */
+ * formulas, and a row whose scores are all -inf counts as empty).  out is
+ * sum P' v / sum P' with P' = exp(S - max S), divided at the end: sum P' |v| has
+ * to stay within f32.  Workspaces come from the stream-ordered pool.  Outputs
+ * may overlap nothing (TRS_ERR_ALIAS); repeated calls give the same bits. */
 trs_status trs_cross_attention(const trs_view* q, const trs_view* k,
                                const trs_view* v, const trs_view* key_lengths,
                                double scale, trs_view* out, trs_view* lse,

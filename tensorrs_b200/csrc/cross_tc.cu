@@ -589,10 +589,11 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       float acc[DE];
 #pragma unroll
       for (int i = 0; i < DE; ++i) acc[i] = 0.f;
-      // adds tile j's P V, complete, to the output
+      // adds tile j's P V, complete, to the output; P's 2^15 goes here, an exact
+      // power of two, so that the output stays in range wherever sum P |v| does
       auto add_output = [&](int j) {
         const uint32_t src = obase + (OB == 2 ? (j & 1) * DP : 0);
-        const float fv = d.v.inv[kt + j];
+        const float fv = d.v.inv[kt + j] * 0x1p-15f;
         const uint64_t fv2 = pack2(fv, fv), keep2 = pack2(keep, keep);
 #pragma unroll
         for (int cc = 0; cc < DE / 32; ++cc) {
@@ -680,12 +681,12 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           float4* o = reinterpret_cast<float4*>(d.part + at * DP);
 #pragma unroll
           for (int i = 0; i < DE / 4; ++i) o[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
-          d.part_m[at] = m - 15.f;  // acc and l carry 2^15
-          d.part_l[at] = l;
+          d.part_m[at] = m;
+          d.part_l[at] = l * 0x1p-15f;  // l carries P's 2^15
         } else {
           const int g = (int)fdiv((uint32_t)row, c.f_Tq), tt = row - g * c.Tq, h = w.hk * c.G + g;
           float* op = static_cast<float*>(c.out.p) + w.b * c.out.sb + tt * c.out.st + h * c.out.sh;
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = l == 0.f ? 0.f : 0x1p15f / l;  // l carries P's 2^15
           if (c.vec) {
 #pragma unroll
             for (int i = 0; i < DE / 4; ++i)
@@ -697,7 +698,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
             for (int i = 0; i < DE; ++i)
               if (i < c.D) op[i * c.out.sd] = acc[i] * inv;
           }
-          if (c.lse) c.lse[w.b * c.ls_b + h * c.ls_h + tt * c.ls_t] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * kLn2;
+          if (c.lse) c.lse[w.b * c.ls_b + h * c.ls_h + tt * c.ls_t] = l == 0.f ? -INFINITY : (m + log2f(l * 0x1p-15f)) * kLn2;
         }
       }
     }

@@ -8,7 +8,7 @@ import pytest
 
 from _cross import Truth, check
 from _gpu import to_host
-from test_cross_attention_gpu import backward, cuda, draw, forward
+from test_cross_attention_gpu import backward, both, cuda, draw, forward
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,16 @@ def test_a_key_of_minus_infinity_takes_no_gradient(rows, D):
     check(dk[:, keep], t.dk, t.dk_tol, "dk")
     check(dv[:, keep], t.dv, t.dv_tol, "dv")
     check(dq[..., 1:], t.dq[..., 1:], t.dq_tol[..., 1:], "dq")  # its element 0 is 0 * inf
+
+
+# B, Tq, Tk, Hq, Hk, D: both sides of the row limits, two row tiles, a walk in parts
+RANGE = [(1, 3, 100, 1, 1, 64), (1, 16, 100, 1, 1, 64), (1, 17, 100, 1, 1, 64), (1, 130, 200, 2, 1, 64), (1, 20, 1000, 1, 1, 64),
+         (1, 8, 100, 1, 1, 128), (1, 9, 100, 1, 1, 128), (1, 300, 200, 1, 1, 128), (1, 40, 100, 1, 1, 80), (1, 20, 100, 1, 1, 160)]
+
+
+@pytest.mark.parametrize("size", RANGE, ids=str)
+@pytest.mark.parametrize("vs", [1e34, 5e35])
+def test_large_values(size, vs):
+    """Values up to 2e36, whose weighted sums (weights of 1 at most, less than 100 of them in all) stay in range."""
+    q, k, v, g = draw(*size, seed=21)
+    both(q, k, v * np.float32(vs), g * np.float32(1 / vs), size[-1] ** -0.5)
