@@ -572,7 +572,9 @@ trs_status trs_cross_attention(const trs_view* q, const trs_view* k,
  * its lse: with P = exp(S - lse), delta = sum_d grad_out out and dS = P
  * (grad_out v^T - delta), grad_q = scale dS k, grad_k = scale dS^T q and
  * grad_v = P^T grad_out, the last two summed over the query heads of a key
- * head.  Rows of grad_k and grad_v at and behind a key length are set to 0.
+ * head.  P is cut to 1; lse, an f32, holds a score to 2^-24 of itself, and P is
+ * off by as much as both are (a few percent at scores of 1e5, meaningless from
+ * 1e7 on).  Rows of grad_k and grad_v at and behind a key length are set to 0.
  * Up to D = 128 on the tensor cores as above; no atomics, so repeated calls
  * give the same bits. */
 trs_status trs_cross_attention_backward(

@@ -52,6 +52,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The smaller of the two, NaN where either is.
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 // Two f32 operations in one instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;

@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kRowsThreads, NR <= 4 ? 2 : 1) cross_rows_grad
       // no weight behind the last key, and none for a row that only fills up the
       // block (its score with an infinite key is 0 * inf)
       const bool on = my_row < c.M && key + mine + e < k1;
-      s[e] = on ? ex2(__fmaf_rn(s[e], f, -lse2)) : 0.f;
+      s[e] = on ? ex2(min_nan(__fmaf_rn(s[e], f, -lse2), 0.f)) : 0.f;  // at most 1: large scores are off from lse
       dp[e] = on ? s[e] * (dp[e] - delta) * c.scale : 0.f;
     }
     Quad dk[U], dv[U];

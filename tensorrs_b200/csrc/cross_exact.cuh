@@ -70,7 +70,8 @@ static __device__ __noinline__ void exact_rows(const CrossDev& c, int64_t w, int
   }
 }
 
-// P and dS of one pair
+// P and dS of one pair.  P = exp(S - lse) is a weight, at most 1: scores of 1e6
+// and more are off by that much from lse, which holds 24 bits of them.
 struct PairGrad {
   float p, ds;
 };
@@ -78,7 +79,7 @@ __device__ __forceinline__ PairGrad pair_grad(const CrossDev& c, const HeadRow& 
                                               const HeadRow& v, float lse, float delta) {
   PairGrad r;
   const float s = dot_row(q, k) * c.scale;
-  r.p = lse == -INFINITY ? 0.f : ex2((s - lse) * kLog2e);
+  r.p = lse == -INFINITY ? 0.f : ex2(min_nan((s - lse) * kLog2e, 0.f));
   r.ds = r.p * (dot_row(go, v) - delta) * c.scale;
   return r;
 }

@@ -57,6 +57,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <string>
@@ -243,6 +244,19 @@ __global__ void __launch_bounds__(256) cross_pack_kernel(const __grid_constant__
 }
 
 // ---- shared pieces of the tensor-core kernels ------------------------------------
+
+// Far scores.  A tile's scores (in units of log2) are f x with |x| < 2^30 DP, so
+// f alone says how large they can be.
+// An exponent 15 + S - m has to stay below 16, what fp16 holds: m and 15 - m are
+// off by half a unit of m each, 2^-4 at 2^20.  Above that the forward takes S - m
+// from rounded scores, which is 0 for a row's largest (inside the branch that
+// cuts off absent keys, where it costs nothing; a branch of its own 2 %, a
+// second copy of the loop 7 %).
+template <int DP> constexpr float kFarMax = 0x1p-10f / DP;
+// S - lse of the gradients, whose S is another sum than the one that lse came
+// from: both are off by less than 80 2^-24 of |q| |k|, together 0.7 at 2^16.
+// Above that the exponent is cut to that of P = 1.
+template <int DP> constexpr float kFarSum = 0x1p-14f / DP;
 
 // A packed operand as the kernels see it.
 struct Planes {
@@ -585,7 +599,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         limit = w.len - w.j0 * KN;
         fq = d.f * d.q.inv[w.pr * qtiles + ((w.mtile * MT + t) * 128 + rl) / KN];
       }
-      float m = -INFINITY, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
+      float m = -FLT_MAX, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
       float acc[DE];
 #pragma unroll
       for (int i = 0; i < DE; ++i) acc[i] = 0.f;
@@ -609,7 +623,8 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         }
       };
       for (int j = 0; j < n; ++j, limit -= KN) {
-        const float f = fmaxf(fq * d.k.inv[kt + j], 0x1p-126f);  // not 0: -inf stands for an absent key below
+        float f = fmaxf(fq * d.k.inv[kt + j], 0x1p-126f);  // not 0: -inf stands for an absent key below
+        const bool far = __any_sync(0xffffffffu, f >= kFarMax<DP>);
         ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)sc & 1u, failed)) != 0;
         if (!ok) break;
         ++sc;
@@ -621,12 +636,23 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         tmem_ld_done(x[0]);
 #pragma unroll
         for (int cc = 1; cc < KN / 32; ++cc) tmem_ld_tie(x[cc]);
-        if (limit < KN) {  // behind the last key: no weight
+        float base = 0.f;
+        if (far || limit < KN) {
 #pragma unroll
           for (int cc = 0; cc < KN / 32; ++cc)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (cc * 32 + i >= limit) x[cc][i] = 0xff800000u;
+              if (cc * 32 + i >= limit) x[cc][i] = 0xff800000u;  // behind the last key: no weight
+          if (far) {  // this tile's scores relative to the largest so far
+            float mx = __uint_as_float(x[0][0]);
+#pragma unroll
+            for (int i = 1; i < KN; ++i) mx = fmaxf(mx, __uint_as_float(x[i / 32][i % 32]));
+            base = fmaxf(m, mx * f);
+#pragma unroll
+            for (int i = 0; i < KN; ++i) x[i / 32][i % 32] = __float_as_uint(__uint_as_float(x[i / 32][i % 32]) * f - base);
+            m -= base;
+            f = 1.f;
+          }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -637,9 +663,8 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         const float mn = fmaxf(m, mx * f);
         const float alpha = ex2(m - mn);
-        const float bias = 15.f - mn;
-        m = mn;
-        const uint64_t f2 = pack2(f, f), b2 = pack2(bias, bias);
+        m = mn + base;
+        const uint64_t f2 = pack2(f, f), b2 = pack2(15.f - mn, 15.f - mn);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int cc = 0; cc < KN / 32; ++cc) {
@@ -1037,6 +1062,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       };
       for (int j = 0; j < n; ++j, ++t, limit -= KN) {
         const float f = ia1 * d.b1.inv[kt + j];
+        const bool far = __any_sync(0xffffffffu, f >= kFarSum<DP>);
         const uint32_t sb = tmem + lanes + (t & 1) * KN + wg * HC;
         float p[HC];  // the exponent's bias, then P (dk, dv: P 2^15)
         if (KV) {
@@ -1068,9 +1094,16 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
               float& p1 = p[cc * 32 + i + 1];
               const uint64_t bias = KV ? pack2(p0, p1) : pack2(r_bias, r_bias);
               unpack2(fma2(pack2(__uint_as_float(a[cc][i]), __uint_as_float(a[cc][i + 1])), f2, bias), &p0, &p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
             }
+          }
+          if (far) {
+#pragma unroll
+            for (int i = 0; i < HC; ++i) p[i] = min_nan(p[i], KV ? 15.f : 0.f);
+          }
+#pragma unroll
+          for (int cc = 0; cc < HC / 32; ++cc) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) p[cc * 32 + i] = ex2(p[cc * 32 + i]);
             if (KV) {
               uint32_t w[32];
 #pragma unroll

@@ -45,3 +45,37 @@ def test_large_values(size, vs):
     """Values up to 2e36, whose weighted sums (weights of 1 at most, less than 100 of them in all) stay in range."""
     q, k, v, g = draw(*size, seed=21)
     both(q, k, v * np.float32(vs), g * np.float32(1 / vs), size[-1] ** -0.5)
+
+
+@pytest.mark.parametrize("size", RANGE, ids=str)
+@pytest.mark.parametrize("amplitude", [1e3, 3e3, 1e4, 1e7])
+def test_large_scores(size, amplitude):
+    """Scores of 1e6 and more: where a row's two largest are further apart than their errors, all of the weight is the
+    largest's, and the output its value, held in 22 bits (2^-40 of the tile's largest) and rounded a few times.  The
+    gradient's P = exp(S - lse) is off by more than itself there, but it stays a weight: finite and at most 1 (the
+    exponential's 2 units and the roundings of the sum beside it), so that |dv| <= sum |grad|."""
+    f = np.float32
+    q, k, v, g = draw(*size, seed=22)
+    q, k = q * f(amplitude), k * f(amplitude)
+    scale = size[-1] ** -0.5
+    tq, tk, tv, tg = cuda(q), cuda(k), cuda(v), cuda(g)
+    out, lse = forward(tq, tk, tv, scale)
+    t = Truth(q, k, v, scale, None, g)
+    check(to_host(out), t.out, t.out_tol, "out")
+    check(to_host(lse), t.lse, t.lse_tol, "lse")
+    peaked = 0
+    for h in range(size[3]):
+        j = h // (size[3] // size[4])
+        S = scale * q[0, :, h].astype(np.float64) @ k[0, :, j].T.astype(np.float64)
+        first = S.argmax(-1)
+        gap = np.sort(S, -1)[:, -1] - np.sort(S, -1)[:, -2]
+        clear = gap > 4 * t.lse_tol[0, h] + 200
+        peaked += clear.sum()
+        want = v[0, first, j].astype(np.float64)
+        far = np.abs(to_host(out)[0, :, h] - want)[clear]
+        assert (far <= 2.0**-20 * np.abs(want[clear]) + 2.0**-38 * np.abs(v).max()).all()
+    assert peaked > 0.9 * size[1] * size[3]
+    dq, dk, dv = map(to_host, backward(tg, tq, tk, tv, out, lse, scale))
+    assert np.isfinite(dq).all() and np.isfinite(dk).all() and np.isfinite(dv).all()
+    most = np.abs(g).astype(np.float64).sum((0, 1)).reshape(size[4], -1, size[5]).sum(1)
+    assert (np.abs(dv[0]) <= most * (1 + 2.0**-10)).all()
