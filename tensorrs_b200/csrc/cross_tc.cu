@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(256) cross_pack_kernel(const __grid_constant__
           float ls = -INFINITY;
           if (row < n) {
             const int g = (int)fdiv((uint32_t)row, s.f_T), t = row - g * s.T;
-            ls = __fmaf_rn(d.lse[b * d.ls_b + (hk * s.G + g) * d.ls_h + t * d.ls_t], -kLog2e, 15.f);
+            ls = d.lse[b * d.ls_b + (hk * s.G + g) * d.ls_h + t * d.ls_t];
+            if (ls != -INFINITY) ls = __fmaf_rn(ls, -kLog2e, 15.f);  // scores of -inf alone: no weight either
           }
           s.bias[at_r] = ls;
           s.delta[at_r] = dlt;
@@ -623,7 +624,8 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
         }
       };
       for (int j = 0; j < n; ++j, limit -= KN) {
-        float f = fmaxf(fq * d.k.inv[kt + j], 0x1p-126f);  // not 0: -inf stands for an absent key below
+        // neither 0 nor inf: -inf stands for an absent key below, and a score of 0 stays 0
+        float f = fminf(fmaxf(fq * d.k.inv[kt + j], 0x1p-126f), FLT_MAX);
         const bool far = __any_sync(0xffffffffu, f >= kFarMax<DP>);
         ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)sc & 1u, failed)) != 0;
         if (!ok) break;
@@ -1061,7 +1063,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         return __all_sync(0xffffffffu, wait_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
       };
       for (int j = 0; j < n; ++j, ++t, limit -= KN) {
-        const float f = ia1 * d.b1.inv[kt + j];
+        const float f = fminf(ia1 * d.b1.inv[kt + j], FLT_MAX);  // a score of 0 stays 0
         const bool far = __any_sync(0xffffffffu, f >= kFarSum<DP>);
         const uint32_t sb = tmem + lanes + (t & 1) * KN + wg * HC;
         float p[HC];  // the exponent's bias, then P (dk, dv: P 2^15)

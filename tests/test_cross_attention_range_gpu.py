@@ -79,3 +79,34 @@ def test_large_scores(size, amplitude):
     assert np.isfinite(dq).all() and np.isfinite(dk).all() and np.isfinite(dv).all()
     most = np.abs(g).astype(np.float64).sum((0, 1)).reshape(size[4], -1, size[5]).sum(1)
     assert (np.abs(dv[0]) <= most * (1 + 2.0**-10)).all()
+
+
+@pytest.mark.parametrize("rows,D", [(3, 64), (130, 64), (40, 128), (20, 160)])
+def test_scores_beyond_f32(rows, D):
+    """Finite inputs, scores of +-1e50.  A row with one of +inf has no defined weights: NaN, not the 0 of a row without
+    keys.  Rows of -inf alone count as empty, and such keys beside others take nothing."""
+    _, _, v, g = draw(1, rows, 200, 1, 1, D, seed=23)
+    f = np.float32
+    q, k = np.full((1, rows, 1, D), 1e25, f), np.full((1, 200, 1, D), 1e25, f)
+    for last in (0, 199):  # one such score is enough, in the first tile or the last
+        some = -k
+        some[0, last] *= -1
+        for x in (k, some):
+            out, lse = (to_host(y) for y in forward(cuda(q), cuda(x), cuda(v), 0.125))
+            assert np.isnan(out).all() and not (lse < 0).any()
+    out, lse = forward(cuda(q), cuda(-k), cuda(v), 0.125)
+    assert (to_host(out) == 0).all() and (to_host(lse) == -np.inf).all()
+    for d in backward(cuda(g), cuda(q), cuda(-k), cuda(v), out, lse, 0.125):
+        assert (to_host(d) == 0).all()
+    for there in (slice(0, 64), slice(128, 200)):  # whole tiles of the other kind: scores of 0
+        some = -k
+        some[0, there] = 0
+        out, _ = forward(cuda(q), cuda(some), cuda(v), 0.125)
+        want = v[0, there].astype(np.float64).mean(0)
+        tol = 2.0**-18 * np.abs(v[0, there]).mean(0) + 2.0**-38 * np.abs(v).max()
+        assert (np.abs(to_host(out)[0] - want) <= tol).all()
+    # a query of zeros among them
+    q[0, 1] = 0
+    out, lse = (to_host(y) for y in forward(cuda(q), cuda(-k), cuda(v), 0.125))
+    assert (out[0, 0] == 0).all() and abs(lse[0, 0, 1] - np.log(200)) < 1e-5
+    assert (np.abs(out[0, 1] - v[0].astype(np.float64).mean(0)) <= 2.0**-18 * np.abs(v[0]).mean(0) + 2.0**-38 * np.abs(v).max()).all()
