@@ -1119,9 +1119,11 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
           tc_fence_before();
           warp_arrive(&p_ready[t & 1]);
         }
-        // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below 2^15
+        // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below
+        // 2^15.  A norm counts as 1 of its tile's units at least, so that a row of
+        // zeros beside large ones keeps a finite factor
         const float g = ia2 * d.b2.inv[kt + j];
-        const float bound = __fmaf_rn(r_norm * d.b2.norm[kt + j], g, KV ? d.dmax[kt + j] : fabsf(r_delta));
+        const float bound = __fmaf_rn(fmaxf(r_norm * d.b2.norm[kt + j], 1.f), g, KV ? d.dmax[kt + j] : fabsf(r_delta));
         uint32_t eb = __float_as_uint(bound) >> 23;
         eb = eb < 15u ? 15u : eb;
         const float up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);

@@ -110,3 +110,14 @@ def test_scores_beyond_f32(rows, D):
     out, lse = (to_host(y) for y in forward(cuda(q), cuda(-k), cuda(v), 0.125))
     assert (out[0, 0] == 0).all() and abs(lse[0, 0, 1] - np.log(200)) < 1e-5
     assert (np.abs(out[0, 1] - v[0].astype(np.float64).mean(0)) <= 2.0**-18 * np.abs(v[0]).mean(0) + 2.0**-38 * np.abs(v).max()).all()
+
+
+@pytest.mark.parametrize("size", [(1, 6, 90, 1, 1, 64), (1, 130, 200, 1, 1, 64), (1, 40, 100, 1, 1, 128)], ids=str)
+@pytest.mark.parametrize("gs,vs", [(1e8, 1e8), (1e30, 1e3)])
+def test_zero_rows_beside_large_ones(size, gs, vs):
+    """Queries that take no part in the loss, values that are 0, next to large ones."""
+    f = np.float32
+    q, k, v, g = draw(*size, seed=26)
+    g[:, ::3] = 0
+    v[:, ::4] = 0
+    both(q, k, v * f(vs), g * f(gs), 0.125)
