@@ -259,6 +259,13 @@ template <int DP> constexpr float kFarMax = 0x1p-10f / DP;
 // Above that the exponent is cut to that of P = 1.
 template <int DP> constexpr float kFarSum = 0x1p-14f / DP;
 
+// a b c, in an order in which no step leaves the range when the product does not:
+// the extremes first.  The factors of a tile are powers of two (and the scale).
+__device__ __forceinline__ float mul3(float a, float b, float c) {
+  const float lo = fminf(fminf(a, b), c), hi = fmaxf(fmaxf(a, b), c);
+  return lo * hi * fmaxf(fminf(a, b), fminf(fmaxf(a, b), c));
+}
+
 // A packed operand as the kernels see it.
 struct Planes {
   int rows_p;            // rows of a problem
@@ -592,13 +599,13 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
     bool ok = true;
     for (int item = blockIdx.x; item < d.items && ok; item += gridDim.x) {
       int n, kt, limit;  // key tiles, the first one's index among all, keys from it on
-      float fq;
+      float iq;
       {
         const FwdItem w = fwd_item<KN>(d, item);
         n = w.n;
         kt = w.pr * ktiles + w.j0;
         limit = w.len - w.j0 * KN;
-        fq = d.f * d.q.inv[w.pr * qtiles + ((w.mtile * MT + t) * 128 + rl) / KN];
+        iq = d.q.inv[w.pr * qtiles + ((w.mtile * MT + t) * 128 + rl) / KN];
       }
       float m = -FLT_MAX, l = 0.f, keep = 0.f;  // keep: what the output so far is scaled by when the next tile is added
       float acc[DE];
@@ -625,7 +632,7 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
       };
       for (int j = 0; j < n; ++j, limit -= KN) {
         // neither 0 nor inf: -inf stands for an absent key below, and a score of 0 stays 0
-        float f = fminf(fmaxf(fq * d.k.inv[kt + j], 0x1p-126f), FLT_MAX);
+        float f = fminf(fmaxf(mul3(d.f, iq, d.k.inv[kt + j]), 0x1p-126f), FLT_MAX);
         const bool far = __any_sync(0xffffffffu, f >= kFarMax<DP>);
         ok = __all_sync(0xffffffffu, wait_or_fail(&s_full[t], (uint32_t)sc & 1u, failed)) != 0;
         if (!ok) break;
@@ -780,7 +787,7 @@ struct BwdDev {
   const float *bias, *delta, *rnorm, *dmax;  // per query row; per query tile
   float *part1, *part2;        // [split][problem][a1.rows_p][DP] when splits > 1: dq, or dk and dv
   float f;                     // |scale| log2 e
-  float out_scale;             // of dq (scale) or dk (|scale|)
+  float out_scale, out_pow;    // of dq (scale) or dk (|scale|), as [1, 2) times a power of two
   int* err;
 };
 
@@ -1037,7 +1044,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         kt = w.pr * bt + w.j0;
         limit = w.cols - w.j0 * KN - wg * HC;
         const int row = w.mtile * 128 + rl;
-        ia1 = d.f * d.a1.inv[w.pr * at1 + row / KN];
+        ia1 = d.a1.inv[w.pr * at1 + row / KN];
         ia2 = d.a2.inv[w.pr * at1 + row / KN];
         qrow = (int64_t)w.pr * (KV ? d.b1.rows_p : d.a1.rows_p) + (KV ? w.j0 * KN + wg * HC : row);
         r_norm = KV ? d.a2.norm[w.pr * at1 + row / KN] : d.rnorm[qrow];
@@ -1046,24 +1053,36 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
       float acc[AC];
 #pragma unroll
       for (int i = 0; i < AC; ++i) acc[i] = 0.f;
-      float ds_down = 0.f;  // what the dS of the last tile was divided by, undone
-      // what tile j's result is multiplied by
-      auto weight = [&](int j) {
-        if (KV && wg == 0) return d.b2.inv[kt + j] * 0x1p-15f;
-        return d.b1.inv[kt + j] * d.out_scale * ds_down;
-      };
-      auto add_chunk = [&](int cc, const uint32_t (&o)[32], uint64_t w2) {
+      // what the last tile's results are multiplied by, powers of two: all at once
+      // (wt), or up before wt where the product is too small for an f32
+      float wt = 0.f, up = 1.f;
+      // adds a tile's results, complete, to those so far
+      auto add_results = [&]() {
+        const bool tiny = __any_sync(0xffffffffu, up != 1.f);
+        const uint64_t wt2 = pack2(wt, wt);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          unpack2(fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), w2,
-                       pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1])),
-                  &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
+        for (int cc = 0; cc < AC / 32; ++cc) {
+          if (!KV && wg * AC + cc * 32 >= DE) continue;
+          uint32_t o[32];
+          tmem_ld32_issue(t_res + cc * 32, o);
+          tmem_ld_done(o);
+          if (tiny) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * up);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            unpack2(fma2(pack2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), wt2,
+                         pack2(acc[cc * 32 + i], acc[cc * 32 + i + 1])),
+                    &acc[cc * 32 + i], &acc[cc * 32 + i + 1]);
+        }
       };
       auto wait_warp = [&](uint64_t* bar, int phase) {
         return __all_sync(0xffffffffu, wait_or_fail(bar, (uint32_t)phase & 1u, failed)) != 0;
       };
       for (int j = 0; j < n; ++j, ++t, limit -= KN) {
-        const float f = fminf(ia1 * d.b1.inv[kt + j], FLT_MAX);  // a score of 0 stays 0
+        const float ib1 = d.b1.inv[kt + j];
+        const float f = fminf(mul3(d.f, ia1, ib1), FLT_MAX);  // a score of 0 stays 0
         const bool far = __any_sync(0xffffffffu, f >= kFarSum<DP>);
         const uint32_t sb = tmem + lanes + (t & 1) * KN + wg * HC;
         float p[HC];  // the exponent's bias, then P (dk, dv: P 2^15)
@@ -1122,28 +1141,20 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         // |dS| <= |dout_i| |v_j| + |delta_i|, the largest of the tile; scaled below
         // 2^15.  A norm counts as 1 of its tile's units at least, so that a row of
         // zeros beside large ones keeps a finite factor
-        const float g = ia2 * d.b2.inv[kt + j];
-        const float bound = __fmaf_rn(fmaxf(r_norm * d.b2.norm[kt + j], 1.f), g, KV ? d.dmax[kt + j] : fabsf(r_delta));
+        const float ib2 = d.b2.inv[kt + j];
+        const float bound = mul3(fmaxf(r_norm * d.b2.norm[kt + j], 1.f), ia2, ib2) + (KV ? d.dmax[kt + j] : fabsf(r_delta));
         uint32_t eb = __float_as_uint(bound) >> 23;
         eb = eb < 15u ? 15u : eb;
-        const float up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);
-        const uint64_t gu = pack2(g * up, g * up), nup = pack2(-up, -up), ndu = pack2(-r_delta * up, -r_delta * up);
+        const float ds_up = __uint_as_float((268u - eb) << 23) * (KV ? 0x1p-15f : 1.f);
+        const float gu1 = mul3(ia2, ib2, ds_up);
+        const uint64_t gu = pack2(gu1, gu1), nup = pack2(-ds_up, -ds_up), ndu = pack2(-r_delta * ds_up, -r_delta * ds_up);
         if (!(ok = wait_warp(dp_full, t))) break;
         // the last tile's results: for (dk, dv) complete before this dP was
         // issued; for dq behind it, and read at the end
         if (KV && j > 0 && !(ok = wait_warp(r_full, t - 1))) break;
         tc_fence_after();
-        const float wt = j > 0 ? weight(j - 1) : 0.f;
-        const uint64_t w2 = pack2(wt, wt);
         if (KV && j > 0) {
-#pragma unroll
-          for (int cc = 0; cc < AC / 32; ++cc) {
-            if (!KV && wg * AC + cc * 32 >= DE) continue;
-            uint32_t o[32];
-            tmem_ld32_issue(t_res + cc * 32, o);
-            tmem_ld_done(o);
-            add_chunk(cc, o, w2);
-          }
+          add_results();
           tc_fence_before();
           if (wg == 0) warp_arrive(r_free);
         }
@@ -1177,35 +1188,34 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         if (!KV && j > 0) {
           if (!(ok = wait_warp(r_full, t - 1))) break;
           tc_fence_after();
-#pragma unroll
-          for (int cc = 0; cc < AC / 32; ++cc) {
-            if (!KV && wg * AC + cc * 32 >= DE) continue;
-            uint32_t o[32];
-            tmem_ld32_issue(t_res + cc * 32, o);
-            tmem_ld_done(o);
-            add_chunk(cc, o, w2);
-          }
+          add_results();
         }
-        ds_down = __uint_as_float((eb - 14u) << 23);
         tmem_st_done();
         tc_fence_before();
         warp_arrive(ds_ready);
+        {
+          const bool is_dv = KV && wg == 0;  // of P 2^15 alone
+          const float w1 = is_dv ? ib2 : ib1, w2 = is_dv ? 0x1p-15f : __uint_as_float((eb - 14u) << 23);
+          const float w3 = is_dv ? 1.f : d.out_pow;
+          wt = mul3(w1, w2, w3);
+          up = 1.f;
+          if (wt < 0x1p-126f) {
+            wt = fminf(fminf(w1, w2), w3);
+            up = fmaxf(fmaxf(w1, w2), w3) * fmaxf(fminf(w1, w2), fminf(fmaxf(w1, w2), w3));
+          }
+        }
       }
       if (!ok) break;
       if (n > 0) {
         if (!(ok = wait_warp(r_full, t - 1))) break;
         tc_fence_after();
-        const float wt = weight(n - 1);
-#pragma unroll
-        for (int cc = 0; cc < AC / 32; ++cc) {
-          if (!KV && wg * AC + cc * 32 >= DE) continue;
-          uint32_t o[32];
-          tmem_ld32_issue(t_res + cc * 32, o);
-          tmem_ld_done(o);
-          add_chunk(cc, o, pack2(wt, wt));
-        }
+        add_results();
         tc_fence_before();
         if (KV && wg == 0) warp_arrive(r_free);
+        if (!KV || wg == 1) {
+#pragma unroll
+          for (int i = 0; i < AC; ++i) acc[i] *= d.out_scale;
+        }
       }
       const BwdItem w = bwd_item<KN, KV>(d, item);
       const int row = w.mtile * 128 + rl;
@@ -1533,10 +1543,13 @@ Error cross_tc_backward(const CrossDev& call, cudaStream_t stream) {
   k_d.next = nonfinite + 2;
   q_d.mtiles = (c.M + 127) / 128;
   q_d.splits = pick_splits((int64_t)q_d.mtiles * np, (c.Tk + KN - 1) / KN);
-  q_d.out_scale = c.scale;
+  int e2 = 0;
+  q_d.out_scale = 2.f * frexpf(c.scale, &e2);
+  q_d.out_pow = ldexpf(1.f, e2 - 1);
   k_d.mtiles = (c.Tk + 127) / 128;
   k_d.splits = pick_splits((int64_t)k_d.mtiles * np, (c.M + KN - 1) / KN);
-  k_d.out_scale = fabsf(c.scale);
+  k_d.out_scale = fabsf(q_d.out_scale);
+  k_d.out_pow = q_d.out_pow;
   Packed q, k, v, g;
   float *bias = nullptr, *delta = nullptr, *rnorm = nullptr, *dmax = nullptr;
   Scratch buf;

@@ -6,7 +6,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from _cross import Truth, check
+from _cross import Truth, check, near
 from _gpu import to_host
 from test_cross_attention_gpu import backward, both, cuda, draw, forward
 
@@ -121,3 +121,31 @@ def test_zero_rows_beside_large_ones(size, gs, vs):
     g[:, ::3] = 0
     v[:, ::4] = 0
     both(q, k, v * f(vs), g * f(gs), 0.125)
+
+
+@pytest.mark.parametrize("size", [(1, 6, 100, 1, 1, 80), (1, 40, 100, 1, 1, 80), (1, 150, 100, 2, 1, 64), (1, 40, 300, 1, 1, 96),
+                                  (1, 12, 100, 1, 1, 128), (1, 20, 60, 1, 1, 160)], ids=str)
+@pytest.mark.parametrize("gs,vs,ks", [(1e-34, 1.0, 1.0), (1e-32, 1.0, 1e-3), (1e-16, 1e-18, 1.0), (1e-36, 1e20, 1e-18)])
+def test_small_gradients(size, gs, vs, ks):
+    """Gradients near the smallest normal number (2^-126) keep their bits: sums of some dozen terms of about 1e-35, each
+    off by half of 2^-149 where a product falls below 2^-126, 1e-10 of the sum."""
+    f = np.float32
+    q, k, v, g = draw(*size, seed=24)
+    both(q * f(1 / ks), k * f(ks), v * f(vs), g * f(gs), size[-1] ** -0.5)
+
+
+@pytest.mark.parametrize("size", [(1, 3, 90, 1, 1, 64), (1, 130, 200, 1, 1, 64), (1, 40, 100, 1, 1, 128)], ids=str)
+def test_operands_at_both_ends_of_the_range(size):
+    """Small queries on large keys under a small scale: the scores are of order 1, whatever the scale and one operand
+    make by themselves."""
+    f = np.float32
+    q, k, v, g = draw(*size, seed=25)
+    q, k = q * f(2.0**-116), k * f(2.0**124)
+    tq, tk, tv, tg = cuda(q), cuda(k), cuda(v), cuda(g)
+    out, lse = forward(tq, tk, tv, 1e-3)
+    dq = backward(tg, tq, tk, tv, out, lse, 1e-3)[0]
+    t = Truth(q, k, v, 1e-3, None, g)
+    for got, want, tol, name, terms in ((out, t.out, t.out_tol, "out", None), (lse, t.lse, t.lse_tol, "lse", None),
+                                        (dq, t.dq, t.dq_tol, "dq", t.dq_terms)):
+        check(to_host(got), want, tol, name)
+        near(to_host(got), want, name, t.s_max, terms)
