@@ -379,8 +379,10 @@ __device__ __forceinline__ void split2(uint64_t x, uint32_t* hi, uint32_t* lo) {
   *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// What a CTA still has in flight when it gave up: its copies (the slots'
-// latest phases) and its MMAs.
+// Before a CTA ends, its TMA thread waits for its copies and its MMA warps for
+// their products, whether or not some role gave up: a role cannot know that the
+// others will still read what it has in flight.  The copies are the latest of
+// every slot.
 __device__ __forceinline__ void drain(uint64_t* full, int slots, int issued) {
   for (int s = 0; s < slots && s < issued; ++s) {
     const int last = (issued - 1 - s) / slots;  // uses of this slot so far, less one
@@ -530,10 +532,8 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           else load_planes<DP, KN>(ring + s * kSlot, &mk, d.k, row, &full[s]);
         }
       }
-      if (!ok) {
-        if (qi > 0) mbar_wait(q_full, (uint32_t)(qi - 1) & 1u);
-        drain(full, NS, li);
-      }
+      if (qi > 0) mbar_wait(q_full, (uint32_t)(qi - 1) & 1u);
+      drain(full, NS, li);
     } else if (warp < MT * 5) {  // MMA of row tile t: the warp stays whole, one lane issues
       const int t = warp - MT * 4;
       const uint32_t lead = elect_lane(), ts = uniform(tmem + t * S::cols);
@@ -585,10 +585,8 @@ cross_forward_kernel(const __grid_constant__ CUtensorMap mq, const __grid_consta
           }
         }
       }
-      if (!ok) {
-        umma_commit(lead, &done[t]);
-        mbar_wait(&done[t], 0);
-      }
+      umma_commit(lead, &done[t]);
+      mbar_wait(&done[t], 0);
     }
   } else {  // softmax: one thread per row
     if (MT == 2) take_registers<56>();
@@ -937,11 +935,9 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
           ++i2;
         }
       }
-      if (!ok) {
-        if (ai > 0) mbar_wait(a_full, (uint32_t)(ai - 1) & 1u);
-        drain(full1, N1, t);
-        drain(full2, N2, i2);
-      }
+      if (ai > 0) mbar_wait(a_full, (uint32_t)(ai - 1) & 1u);
+      drain(full1, N1, t);
+      drain(full2, N2, i2);
     } else if (warp == 8) {  // MMA: the warp stays whole, one lane issues
       const uint32_t lead = elect_lane(), tm = uniform(tmem);
       const uint32_t d1 = uniform(rows_desc(sa1)), d2 = uniform(rows_desc(sa2));
@@ -1017,10 +1013,8 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         }
         t0 += n;
       }
-      if (!ok) {
-        umma_commit(lead, done);
-        mbar_wait(done, 0);
-      }
+      umma_commit(lead, done);
+      mbar_wait(done, 0);
     }
   } else {
     take_registers<KV ? 56 : 88>();
