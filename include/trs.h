@@ -474,8 +474,10 @@ trs_status trs_fold_2d(const trs_view* cols, int64_t kh, int64_t kw, int64_t sh,
 /* composes it from matmul and SoftMax): rotary positions, the per-head */
 /* norm, and the fused attention.  Tensors are views of the shape       */
 /* [batch, tokens, heads, head size] with any strides (q, k and v may   */
-/* be slices of one projection's output), on the current device.  The   */
-/* reference has no counterpart of the rotation and of the norm.        */
+/* be slices of one projection's output, along any of its dimensions;   */
+/* an output's dimensions, taken by their strides, have to step past    */
+/* what the smaller ones reach), on the current device.  The reference  */
+/* has no counterpart of the rotation and of the norm.                  */
 /* ------------------------------------------------------------------ */
 
 /* The rotation's frequencies f_i = base^(-2i / r), i < r / 2 (r the rotated

@@ -1154,7 +1154,7 @@ cross_backward_kernel(const __grid_constant__ CUtensorMap ma1, const __grid_cons
         }
 #pragma unroll
         for (int cc = 0; cc < HC / 32; ++cc) {
-          uint32_t a[32], o[32], w[32];
+          uint32_t a[32], w[32];
           float4 dl[8];
           if (KV) {
             const float4* de = reinterpret_cast<const float4*>(d.delta + qrow + j * KN + cc * 32);

@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "plan.h"
@@ -80,45 +81,44 @@ inline bool writes_collide(const trs_view* v) {
   return false;
 }
 
-// Whether two views can reach a common byte.  Their byte ranges decide,
-// except for two slices of one buffer that step through batch and tokens
-// alike (queries and keys inside one projection's output): those are disjoint
-// when their heads lie beside each other within a token.
+// Whether two views may reach a common byte.  They do not when their byte
+// ranges are apart, or when they are apart inside a period: of any stride P,
+// dimensions of either view that step by multiples of P only move by whole
+// periods, and what the others reach, taken modulo P, are two intervals of a
+// circle.  That covers slices of one buffer along any of its dimensions (queries,
+// keys and values inside one projection's output).
 inline bool heads_overlap(const trs_view* a, const trs_view* b) {
   if (numel_of(a->shape, a->ndim) == 0 || numel_of(b->shape, b->ndim) == 0) return false;
-  auto range = [](const trs_view* v, int first, int64_t* lo, int64_t* hi) {
+  // the bytes reached by the dimensions that do not step by multiples of `period`
+  // (0: by all of them)
+  auto range = [](const trs_view* v, int64_t period, int64_t* lo, int64_t* hi) {
     const int64_t es = dtype_size(v->dtype);
-    int64_t l = v->offset, h = v->offset;
-    for (int i = first; i < v->ndim; ++i) {
-      const int64_t span = (v->shape[i] - 1) * v->strides[i];
+    int64_t l = v->offset * es, h = l + es;
+    for (int i = 0; i < v->ndim; ++i) {
+      const int64_t step = v->strides[i] * es, span = (v->shape[i] - 1) * step;
+      if (span == 0 || (period > 0 && step % period == 0)) continue;
       if (span > 0) h += span; else l += span;
     }
-    *lo = (int64_t)(uintptr_t)v->data + l * es;
-    *hi = (int64_t)(uintptr_t)v->data + (h + 1) * es;
+    *lo = (int64_t)(uintptr_t)v->data + l;
+    *hi = (int64_t)(uintptr_t)v->data + h;
   };
   int64_t alo, ahi, blo, bhi;
   range(a, 0, &alo, &ahi);
   range(b, 0, &blo, &bhi);
   if (alo >= bhi || blo >= ahi) return false;
-  if (a->ndim != 4 || b->ndim != 4 || a->dtype != b->dtype) return true;
-  const int64_t es = dtype_size(a->dtype);
-  // the period of the outer dimensions, the same for both
-  int64_t period = 0;
-  for (int i = 0; i < 2; ++i) {
-    if (a->shape[i] != b->shape[i]) return true;
-    if (a->shape[i] == 1) continue;
-    if (a->strides[i] != b->strides[i] || a->strides[i] <= 0) return true;
-    const int64_t s = a->strides[i] * es;
-    if (period == 0) period = s;
-    else if (s < period) { if (period % s) return true; period = s; }
-    else if (s % period) return true;
+  for (const trs_view* v : {a, b}) {
+    for (int i = 0; i < v->ndim; ++i) {
+      int64_t period = v->strides[i] * dtype_size(v->dtype);
+      if (period < 0) period = -period;
+      if (v->shape[i] < 2 || period == 0) continue;
+      range(a, period, &alo, &ahi);
+      range(b, period, &blo, &bhi);
+      int64_t d = (blo - alo) % period;
+      if (d < 0) d += period;
+      if (d >= ahi - alo && d + (bhi - blo) <= period) return false;
+    }
   }
-  if (period == 0) return true;
-  range(a, 2, &alo, &ahi);
-  range(b, 2, &blo, &bhi);
-  int64_t d = (blo - alo) % period;
-  if (d < 0) d += period;
-  return !(d >= ahi - alo && d + (bhi - blo) <= period);
+  return true;
 }
 
 }  // namespace trs

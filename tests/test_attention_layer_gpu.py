@@ -154,3 +154,36 @@ def test_outputs_on_another_device_are_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 7)
     with pytest.raises(ValueError, match="another device"):
         device.rotary(*views, out, None)
+
+
+@pytest.mark.parametrize("where", ["heads", "batch", "tokens", "elements"])
+def test_slices_that_share_a_buffer_but_no_element(where):
+    """Queries, keys and values interleaved inside one buffer, in any order of its dimensions, rotated in place; the
+    gradients of attention written into such a buffer."""
+    from tensorrs_b200 import device
+    V = device.view_of
+    torch.manual_seed(4)
+    B, T, H, D = 2, 9, 3, 16
+    # the place of the (q, k, v) dimension and how the slice becomes [B, T, H, D]
+    shape, cut = {"heads": ((B, T, H, 3, D), lambda x, i: x[:, :, :, i]),
+                  "batch": ((B, 3, H, T, D), lambda x, i: x[:, i].transpose(1, 2)),
+                  "tokens": ((B, H, T, 3, D), lambda x, i: x[:, :, :, i].transpose(1, 2)),
+                  "elements": ((B, T, H, D, 3), lambda x, i: x[..., i])}[where]
+    buf = torch.randn(shape, device="cuda")
+    q, k, v = (cut(buf, i) for i in range(3))
+    w, pos = torch.randn(B, T, H, D, device="cuda"), torch.arange(T, device="cuda")
+    freqs = torch.empty(D // 2, dtype=torch.float64, device="cuda")
+    device.rotary_frequencies(freqs)
+    apart = [torch.empty(B, T, H, D, device="cuda") for _ in range(2)]
+    device.rotary(V(q), V(k), V(pos), V(freqs), *apart)
+    kept = v.clone()
+    device.rotary(V(q), V(k), V(pos), V(freqs), q, k)
+    assert torch.equal(q, apart[0]) and torch.equal(k, apart[1]) and torch.equal(v, kept)
+    out, lse = torch.empty(B, T, H, D, device="cuda"), torch.empty(B, H, T, device="cuda")
+    device.cross_attention(V(q), V(k), V(v), 0.25, out, lse=lse)
+    grads = [torch.empty(B, T, H, D, device="cuda") for _ in range(3)]
+    device.cross_attention_backward(V(w), V(q), V(k), V(v), V(out), V(lse), 0.25, *grads)
+    gbuf = torch.full(shape, float("nan"), device="cuda")
+    device.cross_attention_backward(V(w), V(q), V(k), V(v), V(out), V(lse), 0.25, *(cut(gbuf, i) for i in range(3)))
+    for i in range(3):
+        assert torch.equal(cut(gbuf, i), grads[i])
