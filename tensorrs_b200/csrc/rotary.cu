@@ -27,7 +27,7 @@
 // Angles: the product p f_i is taken in f64 (positions of a long context times
 // a frequency of 1 lose the fraction of a turn in f32); for f32 tensors the
 // turns are reduced in f64 and sin and cos taken in f32 of the remainder (off
-// by less than 2^-24 of a turn), for f64 tensors all of it is f64.
+// by less than 2^-24 of a turn at any position), for f64 tensors all of it is f64.
 // The row sums stay in the element type (f32 over at most 512 squares, 32
 // lanes' partial sums folded as a tree); dgamma, a sum over all rows, is
 // accumulated over the heads of a token (8 at most) in the element type and
@@ -86,21 +86,45 @@ __device__ __forceinline__ double inv_norm(double ss, double D, double eps) {
   return __ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__ddiv_rn(ss, D), eps)));
 }
 
-// cos and sin of p f, times the magnitude
-__device__ __forceinline__ void turn(double p, double f, double magnitude, float* c, float* s) {
-  double t = p * f * 0.15915494309189535;  // turns
-  t -= rint(t);
-  float sn, cs;
-  sincospif((float)(2.0 * t), &sn, &cs);
+// cos and sin of p f(0), .., p f(V - 1), times the magnitude
+template <int V, class F>
+__device__ __forceinline__ void turn(double p, F f, double magnitude, float (&c)[V], float (&s)[V]) {
+  double h[V], t[V];
+  int high = 0;  // the upper word of the largest |h|
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    h[i] = p * f(i) * 0x1.45f306dc9c883p-3;  // turns
+    t[i] = h[i] - rint(h[i]);
+    high = max(high, __double2hiint(h[i]) & 0x7fffffff);
+  }
+  // h is off by 2^-53 of itself twice: past 2^26 turns with what its rounding and
+  // that of 1 / (2 pi) left, so that the fraction stays exact to 2^-50
+  if (high >= 0x41900000) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const double a = p * f(i);
+      t[i] += __fma_rn(a, -0x1.6b01ec5417056p-57, __fma_rn(a, 0x1.45f306dc9c883p-3, -h[i]));
+      t[i] -= rint(t[i]);
+    }
+  }
   const float m = (float)magnitude;
-  *c = cs * m;
-  *s = sn * m;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float sn, cs;
+    sincospif((float)(2.0 * t[i]), &sn, &cs);
+    c[i] = cs * m;
+    s[i] = sn * m;
+  }
 }
-__device__ __forceinline__ void turn(double p, double f, double magnitude, double* c, double* s) {
-  double sn, cs;
-  sincos(p * f, &sn, &cs);
-  *c = cs * magnitude;
-  *s = sn * magnitude;
+template <int V, class F>
+__device__ __forceinline__ void turn(double p, F f, double magnitude, double (&c)[V], double (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    double sn, cs;
+    sincos(p * f(i), &sn, &cs);
+    c[i] = cs * magnitude;
+    s[i] = sn * magnitude;
+  }
 }
 
 // (a, b) of a unit turned by its V angles.  IL: the pairs lie inside the
@@ -259,10 +283,12 @@ rotary_kernel(const RotDev d) {
       for (int i = 0; i < V; ++i) {
         cs[k][i] = T(1);
         sn[k][i] = T(0);
-        if (un[k].rot) {
-          turn(p, d.freq[((lane + k * G) * V + i) * d.fs], d.magnitude, &cs[k][i], &sn[k][i]);
+      }
+      if (un[k].rot) {
+        turn<V>(p, [&](int i) { return d.freq[((lane + k * G) * V + i) * d.fs]; }, d.magnitude, cs[k], sn[k]);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
           if (d.inverse) sn[k][i] = -sn[k][i];
-        }
       }
     }
     T aa[MODE == kNormBackward ? K : 1][V], ab[MODE == kNormBackward ? K : 1][V];

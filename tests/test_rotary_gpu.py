@@ -288,3 +288,18 @@ def test_frequencies(case, n):
         keep = 1 - np.clip((i - first) / ((last - first) or ref.LD(0.001)), 0, 1)
         f = f * keep + f / factor * (1 - keep)
     assert np.all(np.abs(to_host(out) - f) <= 2.0**-44 * f)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_positions_of_any_size(layout):
+    """The f64 product p f is an angle like any other: its turns are taken off without losing what the f32 rotation can
+    hold (below 2^53 the positions themselves are exact)."""
+    from tensorrs_b200 import device
+    V = device.view_of
+    g = np.random.default_rng(7)
+    x, fr = g.standard_normal((1, 60, 2, 64)).astype(np.float32), ref.frequencies(32)
+    pos = np.concatenate([2**g.integers(30, 53, 30) - g.integers(0, 1000, 30), -(2**g.integers(30, 53, 30))])[None]
+    y = empty(x.shape, np.float32)
+    device.rotary(V(tx := cuda(x)), None, V(tp := cuda(pos)), V(tf := cuda(fr)), y, None, layout=layout)
+    check(to_host(y), ref.rotate(x, pos, fr, layout), 9 * 2.0**-24 * ref.reach(x, fr, layout), "far")
+    del tx, tp, tf
