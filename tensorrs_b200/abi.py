@@ -192,14 +192,14 @@ def check(status: int) -> int:
 def make_view(ptr: int, dtype: int, shape, strides=None, offset: int = 0,
               storage_len: int | None = None) -> View:
     """A trs_view; strides default to row-major, storage_len to the extent the view reaches."""
-    shape = tuple(shape)
+    shape = [int(s) for s in shape]
     n = len(shape)
     if strides is None:
         strides, step = [0] * n, 1
         for i in range(n - 1, -1, -1):
             strides[i] = step
-            step *= int(shape[i])
-    strides = tuple(strides)[:n]
+            step *= shape[i]
+    strides = [int(s) for s in strides][:n]
     strides += _ZEROS[:n - len(strides)]
     if storage_len is None:
         hi = offset
@@ -214,6 +214,8 @@ def pack_view(ptr: int, storage_len: int, dtype: int, shape, strides, offset: in
     """A trs_view from all of its fields; one pack of the whole struct takes a third of the time of setting its fields
     one by one, which small calls with several views notice."""
     n = len(shape)
+    if n > MAX_DIMS:
+        raise IndexError(f"a view has at most {MAX_DIMS} dimensions, not {n}")
     pad = _ZEROS[n:]
     return _from_bytes(_PACK_VIEW(ptr, storage_len, dtype, n, *shape, *pad, *strides, *pad, offset))
 
