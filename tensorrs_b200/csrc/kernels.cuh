@@ -11,6 +11,7 @@
 #include <utility>
 
 #include "bulk.cuh"
+#include "device_cache.h"
 #include "device_ops.cuh"
 #include "launch.h"
 #include "plan.h"
@@ -51,19 +52,15 @@ inline void allow_smem(const void* kernel, int bytes) {
 }
 
 inline int resident_blocks_smem(const void* kernel, int threads, int smem) {
-  static std::mutex mu;
-  static std::map<std::pair<const void*, int>, int> cache;  // (kernel, shared bytes)
-  std::lock_guard<std::mutex> lock(mu);
-  const auto key = std::make_pair(kernel, smem);
-  auto it = cache.find(key);
-  if (it != cache.end()) return it->second;
-  int b = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, kernel, threads, smem) != cudaSuccess || b < 1) {
+  static DeviceCache<std::pair<const void*, int>> cache;  // (kernel, shared bytes)
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) cudaGetLastError();
+  return cache.get(device, {kernel, smem}, [&] {
+    int b = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, kernel, threads, smem) == cudaSuccess) return b;
     cudaGetLastError();
-    b = 1;
-  }
-  cache[key] = b;
-  return b;
+    return 0;
+  });
 }
 
 // A launch that may be scheduled while the stream's previous kernel still runs
