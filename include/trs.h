@@ -551,7 +551,7 @@ trs_status trs_head_norm_rotary_backward(
  * how many keys of each batch there are (values are clamped to [0, Tk]); what
  * lies behind them is not read.  A query without keys gives 0 and an lse of
  * -inf.  lse is [B, Hq, Tq] or NULL; the backward needs it.  The scale is
- * finite, of either sign.
+ * below 2^127 in magnitude (TRS_ERR_ARG), of either sign.
  *
  * Up to D = 128 more than 16 query rows per key head (8 for D above 64 and for
  * gradients) run on the tensor cores (tcgen05; fewer than 2^29 rows of all

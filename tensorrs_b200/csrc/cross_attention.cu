@@ -624,8 +624,8 @@ Error run_cross(const CrossCall& c, bool backward, cudaStream_t stream) {
     return make_error(TRS_ERR_SHAPE, fn + ": the query heads must be a multiple of the key heads");
   if (D > kRowsMaxHead) return make_error(TRS_ERR_SHAPE, fn + ": a head size above 256");
   if (D < 1) return make_error(TRS_ERR_SHAPE, fn + ": an empty head");
-  if (!std::isfinite(c.scale) || !std::isfinite((float)c.scale))
-    return make_error(TRS_ERR_ARG, fn + ": the scale must be finite in f32");
+  if (!(std::fabs(c.scale) < 0x1p127))  // its product with log2 e is an f32
+    return make_error(TRS_ERR_ARG, fn + ": the scale must be below 2^127");
   if (c.lse) {
     e = validate_view(c.lse, "lse");
     if (!e.ok()) return e;

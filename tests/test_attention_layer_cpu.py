@@ -1,0 +1,24 @@
+"""What the attention layer's operators refuse beyond their shapes, before any
+GPU call."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+BASE = 1 << 24
+
+
+def view(trs, shape, dtype=None, at=0):
+    return trs.make_view(BASE + (at << 40), trs.F32 if dtype is None else dtype, shape)
+
+
+@pytest.mark.parametrize("scale", [2.0**127, -3.0e38, float("inf"), float("nan")])
+def test_scales_whose_log2_form_leaves_f32(trs, scale):
+    """S is taken in units of log2: the scale times log2 e has to be an f32."""
+    q, k, lse = [1, 5, 1, 16], [1, 7, 1, 16], [1, 1, 5]
+    v = [view(trs, s, at=i) for i, s in enumerate((q, k, k, q, lse, q, q, k, k))]
+    r = [ctypes.byref(x) for x in v]
+    lib = trs.load()
+    assert lib.trs_cross_attention(r[0], r[1], r[2], None, scale, r[3], r[4], None) == trs.ERR_ARG
+    assert lib.trs_cross_attention_backward(r[5], r[0], r[1], r[2], None, r[3], r[4], scale, r[6], r[7], r[8], None) == trs.ERR_ARG
