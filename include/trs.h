@@ -505,7 +505,8 @@ trs_status trs_rotary_frequencies(double base, int32_t scaling, double factor,
  * Hq, D], k [B, T, Hk, D] or NULL (with k_out), f32 or f64; positions i32 or
  * i64, [T], [1, T] or [B, T], any values; layout a trs_rotary_layout.  The
  * angle is taken in f64.  An output may be its own input (the identical
- * view), no other overlap (TRS_ERR_ALIAS).  D at most 512 (TRS_ERR_SHAPE). */
+ * view), no other overlap (TRS_ERR_ALIAS).  D at most 512, fewer than 2^31
+ * tokens and heads (TRS_ERR_SHAPE). */
 trs_status trs_rotary(const trs_view* q, const trs_view* k,
                       const trs_view* positions, const trs_view* freqs,
                       int32_t layout, double magnitude, trs_view* q_out,

@@ -639,6 +639,9 @@ Error run_rotary(const RotCall& c, cudaStream_t stream) {
   d.D = (int)D;
   d.R = (int)(2 * c.freqs->shape[0]);
   if (B * T >= (1ll << 31)) return make_error(TRS_ERR_SHAPE, fn + ": 2^31 or more tokens");
+  const int64_t most = (1ll << 31) - 16;  // room for rounding up to whole chunks of heads
+  if (c.q->shape[2] >= most || (c.k && (c.k->shape[2] >= most || c.q->shape[2] + c.k->shape[2] >= most)))
+    return make_error(TRS_ERR_SHAPE, fn + ": 2^31 or more heads");
   d.f_T = make_fastdiv((uint32_t)T);
   d.inverse = c.inverse || c.mode == kNormBackward;
   d.magnitude = c.magnitude;

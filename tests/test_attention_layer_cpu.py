@@ -22,3 +22,16 @@ def test_scales_whose_log2_form_leaves_f32(trs, scale):
     lib = trs.load()
     assert lib.trs_cross_attention(r[0], r[1], r[2], None, scale, r[3], r[4], None) == trs.ERR_ARG
     assert lib.trs_cross_attention_backward(r[5], r[0], r[1], r[2], None, r[3], r[4], scale, r[6], r[7], r[8], None) == trs.ERR_ARG
+
+
+@pytest.mark.parametrize("hq,hk", [(2**31, None), (2**31 - 8, None), (2**30, 2**30), (1, 2**32 + 1)])
+def test_more_heads_than_32_bits_count(trs, hq, hk):
+    views = {"q": view(trs, [1, 1, hq, 2]), "qo": view(trs, [1, 1, hq, 2], at=1), "pos": view(trs, [1], trs.I64, 2),
+             "fr": view(trs, [1], trs.F64, 3)}
+    if hk:
+        views.update(k=view(trs, [1, 1, hk, 2], at=4), ko=view(trs, [1, 1, hk, 2], at=5))
+    r = {n: ctypes.byref(v) for n, v in views.items()}
+    k, ko = r.get("k"), r.get("ko")
+    lib = trs.load()
+    assert lib.trs_rotary(r["q"], k, r["pos"], r["fr"], 0, 1.0, r["qo"], ko, None) == trs.ERR_SHAPE
+    assert lib.trs_head_norm_rotary(r["q"], k, None, None, 1e-6, r["pos"], r["fr"], 0, 1.0, r["qo"], ko, None) == trs.ERR_SHAPE
