@@ -45,6 +45,8 @@ ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
 class View(ctypes.Structure):
     """trs_view: a strided view of a device buffer (element units)."""
 
+    device = None  # of the tensor that it was made of, where that is known
+
     _fields_ = [
         ("data", c_void_p),
         ("storage_len", c_int64),
@@ -56,7 +58,8 @@ class View(ctypes.Structure):
     ]
 
 
-_PACK_VIEW = struct.Struct(f"@Pqii{MAX_DIMS}q{MAX_DIMS}qq").pack
+# by rank: the used places of shape and strides, zeros behind them
+_PACK_VIEW = [struct.Struct(f"@Pqii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}xq").pack for n in range(MAX_DIMS + 1)]
 _ZEROS = (0,) * MAX_DIMS
 _from_bytes = View.from_buffer_copy
 
@@ -212,12 +215,9 @@ def make_view(ptr: int, dtype: int, shape, strides=None, offset: int = 0,
 
 def pack_view(ptr: int, storage_len: int, dtype: int, shape, strides, offset: int) -> View:
     """A trs_view from all of its fields; one pack of the whole struct takes a third of the time of setting its fields
-    one by one, which small calls with several views notice."""
+    one by one, which small calls with several views notice.  IndexError for more dimensions than it holds."""
     n = len(shape)
-    if n > MAX_DIMS:
-        raise IndexError(f"a view has at most {MAX_DIMS} dimensions, not {n}")
-    pad = _ZEROS[n:]
-    return _from_bytes(_PACK_VIEW(ptr, storage_len, dtype, n, *shape, *pad, *strides, *pad, offset))
+    return _from_bytes(_PACK_VIEW[n](ptr, storage_len, dtype, n, *shape, *strides, offset))
 
 
 def program(n_in: int, op1: int = ADD, op2: int = ADD, epilogue: str | int = "none",

@@ -21,11 +21,11 @@ TORCH_TO_TRS = {torch.float32: abi.F32, torch.float64: abi.F64, torch.int32: abi
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def stream_handle() -> int:
-    """PyTorch's current stream of the current device (read straight from the binding where it offers that: the
-    Stream object costs 3 us, as much as a launch)."""
+def stream_handle(device: int | None = None) -> int:
+    """PyTorch's current stream of the current device (`device`, where the caller has asked for it already; read straight
+    from the binding where it offers that: the Stream object costs 3 us, as much as a launch)."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(torch.cuda.current_device() if device is None else device)
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -39,14 +39,18 @@ def view_of(t: torch.Tensor, shape=None, strides=None, offset=None) -> abi.View:
     st = t.untyped_storage()
     code, size = _DTYPES[t.dtype]
     if shape is None and strides is None and offset is None:
-        return abi.pack_view(st.data_ptr(), st.nbytes() // size, code, t.shape, t.stride(), t.storage_offset())
+        v = abi.pack_view(st.data_ptr(), st.nbytes() // size, code, t.shape, t.stride(), t.storage_offset())
+        v.device = t.get_device()
+        return v
     if shape is None or list(shape) == list(t.shape):
         shape = t.shape
         if strides is None:
             strides = t.stride()
     if offset is None:
         offset = t.storage_offset()
-    return abi.make_view(st.data_ptr(), code, shape, strides, offset, st.nbytes() // size)
+    v = abi.make_view(st.data_ptr(), code, shape, strides, offset, st.nbytes() // size)
+    v.device = t.get_device()
+    return v
 
 
 def _call(name: str, *args) -> int:
@@ -245,14 +249,21 @@ def fold_2d(cols: abi.View, kernel, stride, padding, out: torch.Tensor) -> torch
     return out
 
 
-def _ref(v: abi.View | None):
-    return ctypes.byref(v) if v is not None else None
+# Operands of the attention layer: inputs are views, outputs tensors, all on the current device.
 
 
-def _out(t: torch.Tensor | None):
+def _in(v: abi.View | None, here: int):
+    if v is None:
+        return None
+    if v.device != here and v.device is not None:
+        raise ValueError("an input lies on another device than the current one")
+    return ctypes.byref(v)
+
+
+def _out(t: torch.Tensor | None, here: int):
     if t is None:
         return None
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != here:
         raise ValueError("the output lies on another device than the current one")
     return ctypes.byref(view_of(t))
 
@@ -261,32 +272,36 @@ def rotary_frequencies(out: torch.Tensor, base: float = 10000.0, scaling: str = 
                        low_turns: float = 1.0, high_turns: float = 32.0, trained_context: float = 0.0) -> torch.Tensor:
     """The frequencies of rotary positions into out (f64, one per rotated pair);
     scaling as trs_rotary_scaling: none, linear, base, bands or ramp."""
+    h = torch.cuda.current_device()
     _call("trs_rotary_frequencies", float(base), abi.ROTARY_SCALINGS[scaling], float(factor), float(low_turns),
-          float(high_turns), float(trained_context), _out(out), stream_handle())
+          float(high_turns), float(trained_context), _out(out, h), stream_handle(h))
     return out
 
 
 def rotary(q: abi.View, k: abi.View | None, positions: abi.View, freqs: abi.View, q_out: torch.Tensor,
            k_out: torch.Tensor | None, layout: str = "half", magnitude: float = 1.0) -> None:
     """Rotary positions of q [B, T, Hq, D] and k [B, T, Hk, D]."""
-    _call("trs_rotary", _ref(q), _ref(k), _ref(positions), _ref(freqs), abi.ROTARY_LAYOUTS[layout], float(magnitude),
-          _out(q_out), _out(k_out), stream_handle())
+    h = torch.cuda.current_device()
+    _call("trs_rotary", _in(q, h), _in(k, h), _in(positions, h), _in(freqs, h), abi.ROTARY_LAYOUTS[layout],
+          float(magnitude), _out(q_out, h), _out(k_out, h), stream_handle(h))
 
 
 def rotary_backward(grad_q_out: abi.View, grad_k_out: abi.View | None, positions: abi.View, freqs: abi.View,
                     grad_q: torch.Tensor, grad_k: torch.Tensor | None, layout: str = "half",
                     magnitude: float = 1.0) -> None:
     """The gradient that rotary passes back to q and k."""
-    _call("trs_rotary_backward", _ref(grad_q_out), _ref(grad_k_out), _ref(positions), _ref(freqs),
-          abi.ROTARY_LAYOUTS[layout], float(magnitude), _out(grad_q), _out(grad_k), stream_handle())
+    h = torch.cuda.current_device()
+    _call("trs_rotary_backward", _in(grad_q_out, h), _in(grad_k_out, h), _in(positions, h), _in(freqs, h),
+          abi.ROTARY_LAYOUTS[layout], float(magnitude), _out(grad_q, h), _out(grad_k, h), stream_handle(h))
 
 
 def head_norm_rotary(q: abi.View, k: abi.View | None, q_gamma: abi.View | None, k_gamma: abi.View | None, eps: float,
                      positions: abi.View, freqs: abi.View, q_out: torch.Tensor, k_out: torch.Tensor | None,
                      layout: str = "half", magnitude: float = 1.0) -> None:
     """The norm of every head of q and k and its rotation, in one pass."""
-    _call("trs_head_norm_rotary", _ref(q), _ref(k), _ref(q_gamma), _ref(k_gamma), float(eps), _ref(positions),
-          _ref(freqs), abi.ROTARY_LAYOUTS[layout], float(magnitude), _out(q_out), _out(k_out), stream_handle())
+    h = torch.cuda.current_device()
+    _call("trs_head_norm_rotary", _in(q, h), _in(k, h), _in(q_gamma, h), _in(k_gamma, h), float(eps), _in(positions, h),
+          _in(freqs, h), abi.ROTARY_LAYOUTS[layout], float(magnitude), _out(q_out, h), _out(k_out, h), stream_handle(h))
 
 
 def head_norm_rotary_backward(grad_q_out: abi.View, grad_k_out: abi.View | None, q: abi.View, k: abi.View | None,
@@ -295,17 +310,20 @@ def head_norm_rotary_backward(grad_q_out: abi.View, grad_k_out: abi.View | None,
                               grad_q_gamma: torch.Tensor | None, grad_k_gamma: torch.Tensor | None,
                               layout: str = "half", magnitude: float = 1.0) -> None:
     """The gradients of head_norm_rotary for q, k and the gammas."""
-    _call("trs_head_norm_rotary_backward", _ref(grad_q_out), _ref(grad_k_out), _ref(q), _ref(k), _ref(q_gamma),
-          _ref(k_gamma), float(eps), _ref(positions), _ref(freqs), abi.ROTARY_LAYOUTS[layout], float(magnitude),
-          _out(grad_q), _out(grad_k), _out(grad_q_gamma), _out(grad_k_gamma), stream_handle())
+    h = torch.cuda.current_device()
+    _call("trs_head_norm_rotary_backward", _in(grad_q_out, h), _in(grad_k_out, h), _in(q, h), _in(k, h),
+          _in(q_gamma, h), _in(k_gamma, h), float(eps), _in(positions, h), _in(freqs, h), abi.ROTARY_LAYOUTS[layout],
+          float(magnitude), _out(grad_q, h), _out(grad_k, h), _out(grad_q_gamma, h), _out(grad_k_gamma, h),
+          stream_handle(h))
 
 
 def cross_attention(q: abi.View, k: abi.View, v: abi.View, scale: float, out: torch.Tensor,
                     lse: torch.Tensor | None = None, key_lengths: abi.View | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v per head: q [B, Tq, Hq, D], k and v [B, Tk, Hk, D], keys of batch b up to
     key_lengths[b]; lse [B, Hq, Tq] is what the backward needs."""
-    _call("trs_cross_attention", _ref(q), _ref(k), _ref(v), _ref(key_lengths), float(scale), _out(out), _out(lse),
-          stream_handle())
+    h = torch.cuda.current_device()
+    _call("trs_cross_attention", _in(q, h), _in(k, h), _in(v, h), _in(key_lengths, h), float(scale), _out(out, h),
+          _out(lse, h), stream_handle(h))
     return out
 
 
@@ -313,8 +331,9 @@ def cross_attention_backward(grad_out: abi.View, q: abi.View, k: abi.View, v: ab
                              scale: float, grad_q: torch.Tensor, grad_k: torch.Tensor, grad_v: torch.Tensor,
                              key_lengths: abi.View | None = None) -> None:
     """The gradients of cross_attention for q, k and v."""
-    _call("trs_cross_attention_backward", _ref(grad_out), _ref(q), _ref(k), _ref(v), _ref(key_lengths), _ref(out),
-          _ref(lse), float(scale), _out(grad_q), _out(grad_k), _out(grad_v), stream_handle())
+    h = torch.cuda.current_device()
+    _call("trs_cross_attention_backward", _in(grad_out, h), _in(q, h), _in(k, h), _in(v, h), _in(key_lengths, h),
+          _in(out, h), _in(lse, h), float(scale), _out(grad_q, h), _out(grad_k, h), _out(grad_v, h), stream_handle(h))
 
 
 def fill_uniform(out: torch.Tensor, seed: int, lo: float = -1.0, hi: float = 1.0, first: int = 0) -> torch.Tensor:

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
 BASE = 1 << 24
 
@@ -35,3 +36,26 @@ def test_more_heads_than_32_bits_count(trs, hq, hk):
     lib = trs.load()
     assert lib.trs_rotary(r["q"], k, r["pos"], r["fr"], 0, 1.0, r["qo"], ko, None) == trs.ERR_SHAPE
     assert lib.trs_head_norm_rotary(r["q"], k, None, None, 1e-6, r["pos"], r["fr"], 0, 1.0, r["qo"], ko, None) == trs.ERR_SHAPE
+
+
+def test_inputs_on_another_device_are_refused(trs, monkeypatch):
+    from tensorrs_b200 import device
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+    def on(where, *args):
+        v = view(trs, *args)
+        v.device = where
+        return v
+
+    x, pos, f, n = (1, 1, 1, 2), on(0, [1], trs.I64), on(0, [1], trs.F64), on(1, [1], trs.I64)
+    here, there, out = on(0, x), on(1, x), torch.empty(x)
+    calls = [lambda: device.rotary(there, None, pos, f, out, None), lambda: device.rotary(here, there, pos, f, out, out),
+             lambda: device.rotary_backward(here, None, n, f, out, None),
+             lambda: device.head_norm_rotary(here, None, on(1, [2]), None, 1e-6, pos, f, out, None),
+             lambda: device.head_norm_rotary_backward(here, None, there, None, None, None, 1e-6, pos, f, out, None, None, None),
+             lambda: device.cross_attention(here, there, here, 1.0, out),
+             lambda: device.cross_attention(here, here, here, 1.0, out, key_lengths=n),
+             lambda: device.cross_attention_backward(here, here, here, there, here, here, 1.0, out, out, out)]
+    for call in calls:
+        with pytest.raises(ValueError, match="another device"):
+            call()
