@@ -37,6 +37,11 @@ __device__ __forceinline__ float dot_row(const HeadRow& a, const HeadRow& b) {
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
+__device__ __forceinline__ HeadRow times(HeadRow r, float f) {
+#pragma unroll
+  for (int i = 0; i < kExactE; ++i) r.x[i] *= f;
+  return r;
+}
 __device__ __forceinline__ HeadRow zero_row() {
   HeadRow r;
 #pragma unroll
@@ -50,11 +55,11 @@ static __device__ __noinline__ void exact_rows(const CrossDev& c, int64_t w, int
   for (; w < nq; w += warps) {
     const int t = (int)(w % c.Tq), h = (int)(w / c.Tq % c.Hq), b = (int)(w / c.Tq / c.Hq), hk = h / c.G;
     const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
-    const HeadRow q = load_row(c.q, b, t, h, c.D);
+    const HeadRow q = times(load_row(c.q, b, t, h, c.D), c.scale * kLog2e);
     HeadRow acc = zero_row();
     float m = -INFINITY, l = 0.f;
     for (int j = 0; j < n; ++j) {
-      const float s = dot_row(q, load_row(c.k, b, j, hk, c.D)) * (c.scale * kLog2e);
+      const float s = dot_row(q, load_row(c.k, b, j, hk, c.D));
       const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
       const float alpha = ex2(m - base), p = ex2(s - base);
       const HeadRow v = load_row(c.v, b, j, hk, c.D);
@@ -70,17 +75,17 @@ static __device__ __noinline__ void exact_rows(const CrossDev& c, int64_t w, int
   }
 }
 
-// P and dS of one pair.  P = exp(S - lse) is a weight, at most 1: scores of 1e6
+// P and dS of one pair, of q times the scale.  P = exp(S - lse) is a weight, at most 1: scores of 1e6
 // and more are off by that much from lse, which holds 24 bits of them.
 struct PairGrad {
   float p, ds;
 };
-__device__ __forceinline__ PairGrad pair_grad(const CrossDev& c, const HeadRow& q, const HeadRow& go, const HeadRow& k,
-                                              const HeadRow& v, float lse, float delta) {
+__device__ __forceinline__ PairGrad pair_grad(const HeadRow& q, const HeadRow& go, const HeadRow& k, const HeadRow& v,
+                                              float lse, float delta) {
   PairGrad r;
-  const float s = dot_row(q, k) * c.scale;
+  const float s = dot_row(q, k);
   r.p = lse == -INFINITY ? 0.f : ex2(min_nan((s - lse) * kLog2e, 0.f));
-  r.ds = r.p * (dot_row(go, v) - delta) * c.scale;
+  r.ds = r.p * (dot_row(go, v) - delta);
   return r;
 }
 
@@ -90,15 +95,15 @@ static __device__ __noinline__ void exact_dq_rows(const CrossDev& c, int64_t w, 
   for (; w < nq; w += warps) {
     const int t = (int)(w % c.Tq), h = (int)(w / c.Tq % c.Hq), b = (int)(w / c.Tq / c.Hq), hk = h / c.G;
     const int n = key_count(c.len, c.len64, c.len_s, c.Tk, b);
-    const HeadRow q = load_row(c.q, b, t, h, c.D), go = load_row(c.dout, b, t, h, c.D);
+    const HeadRow q = times(load_row(c.q, b, t, h, c.D), c.scale), go = load_row(c.dout, b, t, h, c.D);
     const float delta = dot_row(go, load_row(c.out, b, t, h, c.D));
     const float lse = c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t];
     HeadRow acc = zero_row();
     for (int j = 0; j < n; ++j) {
       const HeadRow k = load_row(c.k, b, j, hk, c.D);
-      const PairGrad g = pair_grad(c, q, go, k, load_row(c.v, b, j, hk, c.D), lse, delta);
+      const PairGrad g = pair_grad(q, go, k, load_row(c.v, b, j, hk, c.D), lse, delta);
 #pragma unroll
-      for (int i = 0; i < kExactE; ++i) acc.x[i] = __fmaf_rn(g.ds, k.x[i], acc.x[i]);
+      for (int i = 0; i < kExactE; ++i) acc.x[i] = __fmaf_rn(g.ds, k.x[i] * c.scale, acc.x[i]);
     }
     store_row(c.dq, b, t, h, c.D, acc);
   }
@@ -114,9 +119,9 @@ static __device__ __noinline__ void exact_dkv_rows(const CrossDev& c, int64_t w,
       const HeadRow k = load_row(c.k, b, j, hk, c.D), v = load_row(c.v, b, j, hk, c.D);
       for (int h = hk * c.G; h < (hk + 1) * c.G; ++h) {
         for (int t = 0; t < c.Tq; ++t) {
-          const HeadRow q = load_row(c.q, b, t, h, c.D), go = load_row(c.dout, b, t, h, c.D);
+          const HeadRow q = times(load_row(c.q, b, t, h, c.D), c.scale), go = load_row(c.dout, b, t, h, c.D);
           const float delta = dot_row(go, load_row(c.out, b, t, h, c.D));
-          const PairGrad g = pair_grad(c, q, go, k, v, c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t], delta);
+          const PairGrad g = pair_grad(q, go, k, v, c.lse[b * c.ls_b + h * c.ls_h + t * c.ls_t], delta);
 #pragma unroll
           for (int i = 0; i < kExactE; ++i) {
             ak.x[i] = __fmaf_rn(g.ds, q.x[i], ak.x[i]);

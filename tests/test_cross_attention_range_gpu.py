@@ -6,7 +6,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from _cross import Truth, check, near
+from _cross import U, Truth, check, near
 from _gpu import to_host
 from test_cross_attention_gpu import backward, both, cuda, draw, forward
 
@@ -149,3 +149,24 @@ def test_operands_at_both_ends_of_the_range(size):
                                         (dq, t.dq, t.dq_tol, "dq", t.dq_terms)):
         check(to_host(got), want, tol, name)
         near(to_host(got), want, name, t.s_max, terms)
+
+
+@pytest.mark.parametrize("size", [(1, 3, 100, 1, 1, 64), (1, 16, 100, 1, 1, 64), (1, 17, 100, 1, 1, 64), (1, 130, 200, 2, 1, 64),
+                                  (1, 7, 300, 1, 1, 33), (1, 40, 100, 1, 1, 128), (1, 20, 60, 1, 1, 160)], ids=str)
+@pytest.mark.parametrize("qs,ks,vs,gs,scale", [(1e19, 1e19, 1.0, 1.0, 1.25e-38), (1e18, 1e8, 1e-20, 1.0, 1e-27),
+                                               (1e-10, 1e-8, 1e18, 1e3, 1e17)])
+def test_scales_far_from_1(size, qs, ks, vs, gs, scale):
+    """Large or small queries and keys under a scale that makes up for them: neither q k nor scale dS has to be an f32
+    for S and the gradients to be.  Where a gradient lies below 2^-126 (dq of 1e-39 in the second case), each of its n
+    terms is rounded to a multiple of 2^-149, off by half of that: n 2^-150 of an element besides."""
+    f = np.float32
+    q, k, v, g = draw(*size, seed=27)
+    q, k, v, g = q * f(qs), k * f(ks), v * f(vs), g * f(gs)
+    out, _, *grads = both(q, k, v, g, scale, norm=False)
+    t = Truth(q, k, v, scale, None, g)
+    near(to_host(out), t.out, "out", t.s_max)
+    for got, want, n, terms in zip(grads, (t.dq, t.dk, t.dv), (size[2], size[1] * size[3], size[1] * size[3]),
+                                   (t.dq_terms, t.dk_terms, np.zeros(()))):
+        far = np.linalg.norm(to_host(got) - want)
+        norm = np.linalg.norm(want) + np.linalg.norm(terms)
+        assert far <= (32 + 4 * t.s_max) * U * norm + np.sqrt(want.size) * n * 2.0**-150, far / norm
