@@ -534,9 +534,10 @@ trs_status trs_head_norm_rotary(const trs_view* q, const trs_view* k,
 
 /* The gradients of trs_head_norm_rotary: q and k are its inputs, grad_q and
  * grad_k the gradients of these, grad_q_gamma and grad_k_gamma (D elements
- * each, or NULL) those of the gammas, summed over batch, tokens and heads in
- * f64 in a fixed order and rounded once.  grad_q may be grad_q_out or q
- * through the identical view, likewise grad_k. */
+ * each, or NULL) those of the gammas: up to 8 heads of a token are summed in
+ * the tensors' type (fewer for few tokens), these sums in f64 in a fixed order
+ * and rounded once.  grad_q may be grad_q_out or q through the identical view,
+ * likewise grad_k. */
 trs_status trs_head_norm_rotary_backward(
     const trs_view* grad_q_out, const trs_view* grad_k_out, const trs_view* q,
     const trs_view* k, const trs_view* q_gamma, const trs_view* k_gamma,
@@ -560,9 +561,11 @@ trs_status trs_head_norm_rotary_backward(
  * power of two per tile of 8192 elements, three products each, accumulated in
  * f32, results within a few f32 roundings of the sums' terms (elements below
  * 2^-17 of their tile's largest are off by 2^-40 of that).  Fewer rows, and
- * larger heads, run on the CUDA cores in f32, as does a whole call whose inputs
- * hold an infinity or a NaN (found on the device; these propagate as in the
- * formulas, and a row whose scores are all -inf counts as empty).  out is
+ * larger heads, run on the CUDA cores in f32 (many rows of heads above 128 slower
+ * than separate matrix products and a softmax, their gradient by an order of
+ * magnitude), as does a whole call whose inputs hold an infinity or a NaN (found
+ * on the device; these propagate as in the formulas, and a row whose scores are
+ * all -inf counts as empty; finite scores beyond f32 are infinities).  out is
  * sum P' v / sum P' with P' = exp(S - max S), divided at the end: sum P' |v| has
  * to stay within f32.  Workspaces come from the stream-ordered pool.  Outputs
  * may overlap nothing (TRS_ERR_ALIAS); repeated calls give the same bits. */
@@ -576,8 +579,8 @@ trs_status trs_cross_attention(const trs_view* q, const trs_view* k,
  * (grad_out v^T - delta), grad_q = scale dS k, grad_k = scale dS^T q and
  * grad_v = P^T grad_out, the last two summed over the query heads of a key
  * head.  P is cut to 1; lse, an f32, holds a score to 2^-24 of itself, and P is
- * off by as much as both are (a few percent at scores of 1e5, meaningless from
- * 1e7 on).  Rows of grad_k and grad_v at and behind a key length are set to 0.
+ * off by as much as both are (a percent at scores of 1e5, meaningless from 1e7
+ * on).  Rows of grad_k and grad_v at and behind a key length are set to 0.
  * Up to D = 128 on the tensor cores as above; no atomics, so repeated calls
  * give the same bits. */
 trs_status trs_cross_attention_backward(

@@ -16,8 +16,10 @@
 // with shuffles, and the running maximum, sum and output stay in registers
 // until the CTA's groups are joined in shared memory.  Parts of the keys are
 // joined by cross_join_kernel in a fixed order.  One row is bound by the loads
-// in flight (8 x 16 heads of 64, 1024 to 2048 keys, 88 MB: 20 us, 4.4 TB/s),
-// eight by arithmetic (4 x 16 heads, 2048 keys, 67 MB: 29 us).
+// in flight (8 x 16 heads of 64, 1024 to 2048 keys, 88 MB: 20 us, 4.3 TB/s),
+// eight by arithmetic (4 x 16 heads, 2048 keys, 67 MB: 27 us).  Of heads of 256, 256
+// queries on 1024 keys, 4 x 8 heads: 500 us (the plain form, products in a library,
+// 360): four rows a CTA read k and v 64 times.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -471,7 +473,10 @@ __global__ void __launch_bounds__(256) cross_rows_sum_kernel(const RowsGradDev d
   static_cast<float*>(c.dq.p)[b * c.dq.sb + t * c.dq.st + h * c.dq.sh + e * c.dq.sd] = sum;
 }
 
-// The gradient of head sizes above 128 on the CUDA cores, a warp per row.
+// The gradient of head sizes above 128 on the CUDA cores, a warp per row: right,
+// and slow.  Every pair is walked twice with three dot products folded over the
+// warp, one pair at a time: 256 queries on 1024 keys, 4 x 8 heads of 256, take 11.4
+// ms, where the plain form takes 0.6.
 __global__ void __launch_bounds__(256) cross_grad_rows_kernel(const CrossDev c) {
   const int64_t warps = (int64_t)gridDim.x * 8, w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   exact_dq_rows(c, w, warps);

@@ -9,8 +9,9 @@
 // largest keep all 22 bits, and below that the error is 2^-40 of the largest:
 // an f32 result, at a third of the fp16 rate instead of the CUDA cores' rate.
 // P and dS are split the same way in registers, P by the fixed 2^15 of its
-// range, dS by a bound on its row (|dout_i| |v_j| + |delta_i|).  The small
-// products of a tile are accumulated before the large ones, and every tile's
+// range, dS by a bound on its row (|dout_i| |v_j| + |delta_i|).  The scales of the
+// tiles meet in f32 as powers of two, in an order that keeps every step in range.
+// The small products of a tile are accumulated before the large ones, and every tile's
 // result leaves the accumulator for f32 registers, so that a long sum is not
 // carried through the tensor core's own (truncating) additions.
 //
@@ -31,14 +32,15 @@
 //                         place, and adds O.  The row tiles run half a period
 //                         apart: one is in the softmax while the other has the
 //                         tensor core.  4 x 16 heads of 64, 2048 x 2048 tokens:
-//                         215 us, 320 TFLOP/s of f32 products (960 of fp16, two
-//                         thirds of the sustained cuBLAS rate).
+//                         214 us (226 with the split), 320 TFLOP/s of f32
+//                         products (960 of fp16, two thirds of the sustained
+//                         cuBLAS rate).
 //   cross_backward_kernel dq (rows: queries, walking keys) or dk and dv (rows:
 //                         keys, walking queries); both need S and dP = dout v^T
 //                         of the tile, and write each result once: no atomics,
 //                         at the price of computing S and dP twice.  Two
 //                         warpgroups share the 128 rows and halve the columns.
-//                         The same case: 280 us and 400 us (740 and 1030
+//                         The same case: 297 us and 402 us (1040 and 1025
 //                         TFLOP/s of fp16 products).
 //   cross_join_kernel (cross_attention.cu), cross_sum_kernel
 //                         join the parts of a walk that was split over CTAs, in
@@ -1441,8 +1443,8 @@ Error flag_word(Scratch& flag, CrossDev& c, cudaStream_t stream, int** word) {
 
 // Parts of a walk of `tiles` column tiles so that `ctas` items fill the SMs;
 // every part walks two tiles at least.  Whole walks and parts: 32 queries of 32
-// heads on 32768 keys of 4 heads 1520 and 120 us, 200 queries of 4 x 8 heads on
-// 2048 keys 71 and 54, the gradient of 333 on 777 of 3 x 2 heads 145 and 112
+// heads on 32768 keys of 4 heads 1344 and 120 us, 200 queries of 4 x 8 heads on
+// 2048 keys 61 and 47, the gradient of 333 on 777 of 3 x 2 heads 140 and 111
 // (with the forward).
 int pick_splits(int64_t ctas, int tiles) {
   const int sms = current_device_info().sm_count;
@@ -1466,7 +1468,7 @@ Error cross_tc_forward(const CrossDev& call, cudaStream_t stream) {
   const int DP = c.D <= 64 ? 64 : 128, KN = kTileElems / DP, np = c.B * c.Hk;
   // two row tiles a CTA as soon as there are two: K and V are read once for both,
   // and one softmax overlaps the other's products (4 x 16 heads, 2048 queries on
-  // 2048 keys: 244 us against 300 with one; 1024 on 1500: 81 and 86)
+  // 2048 keys, with the split: 225 us against 287 with one; 1024 on 1500: 80 and 85)
   const int MT = c.M > 128 ? 2 : 1;
   FwdDev f;
   std::memset(static_cast<void*>(&f), 0, sizeof(f));

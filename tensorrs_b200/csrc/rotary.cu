@@ -17,12 +17,14 @@
 // keeps its pairs' cos and sin in registers and walks heads with them, so an
 // angle is evaluated once per token and chunk of heads instead of once per
 // element, and no table of cos and sin is read.  A lane's unit is two 16-byte
-// vectors of a head (V pairs); kHeads heads are loaded before the first is
-// used, which keeps 2 kHeads (4 kHeads) 16-byte loads of a lane in flight.
+// vectors of a head (V pairs); UH heads are loaded before the first is
+// used, which keeps 2 UH (4 UH) 16-byte loads of a lane in flight.
 // The sums of a row (x^2, dn n) are folded over the group with shuffles.
-// Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 58 us rotated
-// (5.8 TB/s, 0.91 of the copy rate), 63 us normed and rotated (5.3 TB/s); the
-// norm's gradient of 4096 tokens of 20 heads of 64 (63 MB) 20 us.
+// Measured, 8192 tokens of 40 heads of 128 in f32 (336 MB): 57 us rotated
+// (5.9 TB/s, 0.92 of the copy rate), 62 us normed and rotated (5.4 TB/s), 124
+// normed and rotated in f64; the norm's gradient of 4096 tokens of 20 heads of 64
+// (63 MB) 21 us and 6 more for the gammas (33 and 6 in f64).  The f64 rotation of
+// 2000 tokens of 24 heads of 64 (49 MB) 8.2 us.
 //
 // Angles: the product p f_i is taken in f64 (positions of a long context times
 // a frequency of 1 lose the fraction of a turn in f32); for f32 tensors the
@@ -204,11 +206,11 @@ __device__ __forceinline__ T group_sum(T x, unsigned mask) {
 // V: elements per vector access (1: any strides).  K: units per lane.  UH:
 // heads in flight.  G: lanes per token.
 // The norm's forward is held to the registers of three CTAs per SM (8192 tokens
-// of 40 heads of 128: 67.6 us at the two that it takes by itself, 63.1 at three,
-// 63.0 at four with two heads in flight), its gradient to those of three, two
-// in f64 (8192 tokens of 10 heads of 256: 114 us with the forward, 147 without);
-// the rotation alone is fastest at the three that it takes (62.2 us; 66.8 at
-// four, before its loads were issued ahead of the angles).
+// of 40 heads of 128: 66.7 us at the two that it takes by itself, 62.4 at three),
+// its gradient to those of three, two in f64 (8192 tokens of 10 heads of 256: 110
+// us with the forward, 143 where each takes what it wants); the rotation alone is
+// fastest at the two that it takes (118 registers: 56.6 us; 61.1 at three, 68.3 at
+// four).
 template <class T, int V, bool IL, int MODE, int G, int K, int UH>
 __global__ void __launch_bounds__(kRotThreads, MODE == kRotate || K > 1 ? 1 : sizeof(T) == 4 ? 3 : MODE == kNormBackward ? 2 : 1)
 rotary_kernel(const RotDev d) {
@@ -269,8 +271,9 @@ rotary_kernel(const RotDev d) {
         }
       }
     };
-    // on their way while the angles are evaluated (rotation 62.0 -> 57.9 us, f64
-    // norm 128 -> 124); the f32 norm lacks the registers (63.0 -> 64.7)
+    // on their way while the angles are evaluated (8192 tokens of 40 heads of 128:
+    // rotation 60.4 -> 56.7 us, f64 norm 128.1 -> 124.0); the f32 norm lacks the
+    // registers (62.2 -> 62.9)
     constexpr bool kEarly = MODE == kRotate || sizeof(T) == 8;
     if (kEarly) load_heads(h0);
     const int64_t pi = b * d.ps_b + t * d.ps_t;
@@ -450,9 +453,9 @@ Error launch_rot(RotDev& d, const RotCall& c, cudaStream_t stream) {
   auto kern = rotary_kernel<T, V, IL, MODE, G, K, UH>;
   const int64_t resident = (int64_t)sms * resident_blocks_smem((const void*)kern, kRotThreads, 0);
   // heads per item: 8 that share an angle while the items still fill the GPU.
-  // 8192 tokens of 40 heads of 128, 8, 4, 2, 1 heads: rotated 58, 61, 79 and 128
-  // us, normed 63, 71, 101 and 156; 16 tokens of 20 heads of 64: 8 heads 8.2 us,
-  // one (what the rule takes there) 4.1
+  // 8192 tokens of 40 heads of 128, 8, 4, 2, 1 heads: rotated 57, 59, 73 and 113
+  // us, normed 62, 69, 96 and 149; 64 tokens of them normed: 8 heads 8.2 us, what
+  // the rule takes there 4.5
   const int64_t tokens = d.items[0];  // set by the caller: batch * tokens
   int hpc = 8;
   while (hpc > 1 && tokens * ((d.H[0] + d.H[1] + hpc - 1) / hpc) < resident * kGroups) hpc /= 2;
