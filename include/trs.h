@@ -522,9 +522,10 @@ trs_status trs_rotary_backward(const trs_view* grad_q_out,
                                trs_stream stream);
 
 /* The norm of every query's and key's head and its rotation in one pass:
- * n = x / sqrt(sum(x^2) / D + eps), y = rotary(n * gamma).  q_gamma and
- * k_gamma hold D elements of the tensors' type, or are NULL for ones; the rest
- * as trs_rotary. */
+ * n = x / sqrt(sum(x^2) / D + eps), y = rotary(n * gamma).  The sum is taken in
+ * the tensors' type: f32 elements stay below 8e17, so that it does not overflow
+ * (n would be 0), and where eps is 0 above 1e-18.  q_gamma and k_gamma hold D
+ * elements of the tensors' type, or are NULL for ones; the rest as trs_rotary. */
 trs_status trs_head_norm_rotary(const trs_view* q, const trs_view* k,
                                 const trs_view* q_gamma, const trs_view* k_gamma,
                                 double eps, const trs_view* positions,
