@@ -165,6 +165,8 @@ extern "C" {
     pub fn trs_head_norm_rotary_backward(grad_q_out: *const trs_view, grad_k_out: *const trs_view, q: *const trs_view, k: *const trs_view, q_gamma: *const trs_view, k_gamma: *const trs_view, eps: f64, positions: *const trs_view, freqs: *const trs_view, layout: i32, magnitude: f64, grad_q: *mut trs_view, grad_k: *mut trs_view, grad_q_gamma: *mut trs_view, grad_k_gamma: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_cross_attention(q: *const trs_view, k: *const trs_view, v: *const trs_view, key_lengths: *const trs_view, scale: f64, out_: *mut trs_view, lse: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_cross_attention_backward(grad_out: *const trs_view, q: *const trs_view, k: *const trs_view, v: *const trs_view, key_lengths: *const trs_view, out_: *const trs_view, lse: *const trs_view, scale: f64, grad_q: *mut trs_view, grad_k: *mut trs_view, grad_v: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_embedding(table: *const trs_view, ids: *const trs_view, scale: f64, out_: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_embedding_backward(grad_out: *const trs_view, ids: *const trs_view, scale: f64, accumulate: i32, grad_table: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_fill_uniform(out_: *mut trs_view, seed: u64, first: u64, lo: f64, hi: f64, stream: trs_stream) -> trs_status;
     pub fn trs_fill_normal(out_: *mut trs_view, seed: u64, first: u64, stream: trs_stream) -> trs_status;
     pub fn trs_set_device(device: i32) -> trs_status;

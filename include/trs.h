@@ -591,6 +591,33 @@ trs_status trs_cross_attention_backward(
     trs_view* grad_v, trs_stream stream);
 
 /* ------------------------------------------------------------------ */
+/* The ends of a language model (Embedding of src/nn; the reference's   */
+/* loss/crossentropy.rs:41-55 works on a written-out [tokens,           */
+/* vocabulary] tensor).  Rows of tokens are views [tokens, width] or    */
+/* [batch, tokens, width] with any strides (a sequence shifted by one   */
+/* is a slice), on the current device; what belongs to them has the     */
+/* same leading dimensions.                                             */
+/* ------------------------------------------------------------------ */
+
+/* out[t] = scale * table[ids[t]].  table is [V, D], f32 or f64, ids i32 or i64,
+ * [tokens] or [batch, tokens], out the same with D behind it, in the table's
+ * type.  An id outside [0, V) (padding, or a row of another shard of the table)
+ * gives a row of zeros.  out may overlap neither table nor ids (TRS_ERR_ALIAS).
+ * Fewer than 2^31 - 8192 tokens, rows and elements of a row (TRS_ERR_SHAPE). */
+trs_status trs_embedding(const trs_view* table, const trs_view* ids, double scale,
+                         trs_view* out, trs_stream stream);
+
+/* The table's gradient of trs_embedding: grad_table[v] = scale * the sum of
+ * grad_out[t] over the t with ids[t] = v, 0 for a row that no token looked up;
+ * with accumulate != 0 that is added to what grad_table holds (rows that no
+ * token looked up are left alone), as for a table that is also the weight of
+ * the last layer.  Sums are taken in f64 and rounded once, in an order that the
+ * ids alone decide: no atomics add values, repeated calls give the same bits.
+ * grad_table may overlap neither grad_out nor ids. */
+trs_status trs_embedding_backward(const trs_view* grad_out, const trs_view* ids, double scale,
+                                  int32_t accumulate, trs_view* grad_table, trs_stream stream);
+
+/* ------------------------------------------------------------------ */
 /* Seeded synthetic inputs                                              */
 /* ------------------------------------------------------------------ */
 

@@ -249,7 +249,7 @@ def fold_2d(cols: abi.View, kernel, stride, padding, out: torch.Tensor) -> torch
     return out
 
 
-# Operands of the attention layer: inputs are views, outputs tensors, all on the current device.
+# Operands of the attention layer and of a model's ends: inputs are views, outputs tensors, all on the current device.
 
 
 def _in(v: abi.View | None, here: int):
@@ -334,6 +334,22 @@ def cross_attention_backward(grad_out: abi.View, q: abi.View, k: abi.View, v: ab
     h = torch.cuda.current_device()
     _call("trs_cross_attention_backward", _in(grad_out, h), _in(q, h), _in(k, h), _in(v, h), _in(key_lengths, h),
           _in(out, h), _in(lse, h), float(scale), _out(grad_q, h), _out(grad_k, h), _out(grad_v, h), stream_handle(h))
+
+
+def embedding(table: abi.View, ids: abi.View, scale: float, out: torch.Tensor) -> torch.Tensor:
+    """scale times the rows of table [V, D] that ids name (zeros for ids outside it)."""
+    h = torch.cuda.current_device()
+    _call("trs_embedding", _in(table, h), _in(ids, h), float(scale), _out(out, h), stream_handle(h))
+    return out
+
+
+def embedding_backward(grad_out: abi.View, ids: abi.View, scale: float, grad_table: torch.Tensor,
+                       accumulate: bool = False) -> torch.Tensor:
+    """The gradient that embedding passes back to its table; with accumulate, added to what grad_table holds."""
+    h = torch.cuda.current_device()
+    _call("trs_embedding_backward", _in(grad_out, h), _in(ids, h), float(scale), int(bool(accumulate)),
+          _out(grad_table, h), stream_handle(h))
+    return grad_table
 
 
 def fill_uniform(out: torch.Tensor, seed: int, lo: float = -1.0, hi: float = 1.0, first: int = 0) -> torch.Tensor:
