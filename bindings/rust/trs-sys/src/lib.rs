@@ -167,6 +167,10 @@ extern "C" {
     pub fn trs_cross_attention_backward(grad_out: *const trs_view, q: *const trs_view, k: *const trs_view, v: *const trs_view, key_lengths: *const trs_view, out_: *const trs_view, lse: *const trs_view, scale: f64, grad_q: *mut trs_view, grad_k: *mut trs_view, grad_v: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_embedding(table: *const trs_view, ids: *const trs_view, scale: f64, out_: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_embedding_backward(grad_out: *const trs_view, ids: *const trs_view, scale: f64, accumulate: i32, grad_table: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_linear_cross_entropy(hidden: *const trs_view, weight: *const trs_view, targets: *const trs_view, smoothing: f64, loss: *mut trs_view, lse: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_linear_cross_entropy_backward(grad_loss: *const trs_view, hidden: *const trs_view, weight: *const trs_view, targets: *const trs_view, lse: *const trs_view, smoothing: f64, grad_hidden: *mut trs_view, grad_weight: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_linear_distillation(hidden: *const trs_view, weight: *const trs_view, teacher_ids: *const trs_view, teacher_logits: *const trs_view, temperature: f64, loss: *mut trs_view, lse: *mut trs_view, stream: trs_stream) -> trs_status;
+    pub fn trs_linear_distillation_backward(grad_loss: *const trs_view, hidden: *const trs_view, weight: *const trs_view, teacher_ids: *const trs_view, teacher_logits: *const trs_view, lse: *const trs_view, temperature: f64, grad_hidden: *mut trs_view, grad_weight: *mut trs_view, stream: trs_stream) -> trs_status;
     pub fn trs_fill_uniform(out_: *mut trs_view, seed: u64, first: u64, lo: f64, hi: f64, stream: trs_stream) -> trs_status;
     pub fn trs_fill_normal(out_: *mut trs_view, seed: u64, first: u64, stream: trs_stream) -> trs_status;
     pub fn trs_set_device(device: i32) -> trs_status;

@@ -617,6 +617,56 @@ trs_status trs_embedding(const trs_view* table, const trs_view* ids, double scal
 trs_status trs_embedding_backward(const trs_view* grad_out, const trs_view* ids, double scale,
                                   int32_t accumulate, trs_view* grad_table, trs_stream stream);
 
+/* The last linear layer with softmax cross entropy, without the logits: with
+ * x = hidden weight^T and lse = ln sum_v exp x_v, loss = lse - (1 - smoothing)
+ * x_target - smoothing / V sum_v x_v per token (a caller that wants the mean sums
+ * it and passes 1 / count in grad_loss below).  hidden is [tokens, D] or [batch,
+ * tokens, D], weight [V, D] (a Linear's [in, out] storage is the view with
+ * strides (1, out)), both f32 with any strides; targets i32 or i64; loss and lse
+ * f32, lse or NULL.  A token whose target lies outside [0, V) is masked: its
+ * hidden row is not read, its loss and lse are 0, it has no gradient.  Smoothing
+ * lies in [0, 1] (TRS_ERR_ARG).  Fewer than 2^30 tokens, rows and columns of
+ * weight (TRS_ERR_SHAPE); outputs may overlap nothing (TRS_ERR_ALIAS). */
+trs_status trs_linear_cross_entropy(const trs_view* hidden, const trs_view* weight,
+                                    const trs_view* targets, double smoothing,
+                                    trs_view* loss, trs_view* lse, trs_stream stream);
+
+/* The gradients of trs_linear_cross_entropy from grad_loss (f32, per token; a
+ * stride of 0 repeats one value), its inputs and its lse: with dx = grad_loss
+ * (exp(x - lse) - (1 - smoothing) [v = target] - smoothing / V), grad_hidden =
+ * dx weight and grad_weight = dx^T hidden.  The scores are computed again, in
+ * pieces of the vocabulary.  grad_hidden or grad_weight may be NULL, not both.  No atomics add values:
+ * repeated calls give the same bits. */
+trs_status trs_linear_cross_entropy_backward(const trs_view* grad_loss, const trs_view* hidden,
+                                             const trs_view* weight, const trs_view* targets,
+                                             const trs_view* lse, double smoothing,
+                                             trs_view* grad_hidden, trs_view* grad_weight,
+                                             trs_stream stream);
+
+/* The last linear layer held against a teacher's largest logits: with
+ * q = softmax(hidden weight^T / temperature) over the vocabulary and
+ * p = softmax(teacher_logits / temperature) over the token's K entries,
+ * loss = temperature^2 sum_j p_j (ln p_j - ln q[teacher_ids_j]); lse is that of
+ * hidden weight^T / temperature.  teacher_ids (i32 or i64) and teacher_logits
+ * (f32) are [tokens, K] or [batch, tokens, K], K from 1 to 1024, in any order; an
+ * entry whose id lies outside [0, V) or whose logit is -inf is absent, an id that
+ * comes twice counts twice, and a token without entries is masked.  The
+ * temperature lies in [2^-40, 2^40] (TRS_ERR_ARG).  The rest as
+ * trs_linear_cross_entropy. */
+trs_status trs_linear_distillation(const trs_view* hidden, const trs_view* weight,
+                                   const trs_view* teacher_ids, const trs_view* teacher_logits,
+                                   double temperature, trs_view* loss, trs_view* lse,
+                                   trs_stream stream);
+
+/* The gradients of trs_linear_distillation for hidden and weight: dx =
+ * grad_loss temperature (q - p), the rest as
+ * trs_linear_cross_entropy_backward. */
+trs_status trs_linear_distillation_backward(const trs_view* grad_loss, const trs_view* hidden,
+                                            const trs_view* weight, const trs_view* teacher_ids,
+                                            const trs_view* teacher_logits, const trs_view* lse,
+                                            double temperature, trs_view* grad_hidden,
+                                            trs_view* grad_weight, trs_stream stream);
+
 /* ------------------------------------------------------------------ */
 /* Seeded synthetic inputs                                              */
 /* ------------------------------------------------------------------ */

@@ -137,6 +137,10 @@ _SIGNATURES = {
     "trs_cross_attention_backward": (c_int32, [_V, _V, _V, _V, _V, _V, _V, c_double, _V, _V, _V, c_void_p]),
     "trs_embedding": (c_int32, [_V, _V, c_double, _V, c_void_p]),
     "trs_embedding_backward": (c_int32, [_V, _V, c_double, c_int32, _V, c_void_p]),
+    "trs_linear_cross_entropy": (c_int32, [_V, _V, _V, c_double, _V, _V, c_void_p]),
+    "trs_linear_cross_entropy_backward": (c_int32, [_V, _V, _V, _V, _V, c_double, _V, _V, c_void_p]),
+    "trs_linear_distillation": (c_int32, [_V, _V, _V, _V, c_double, _V, _V, c_void_p]),
+    "trs_linear_distillation_backward": (c_int32, [_V, _V, _V, _V, _V, _V, c_double, _V, _V, c_void_p]),
     "trs_fill_uniform": (c_int32, [_V, c_uint64, c_uint64, c_double, c_double, c_void_p]),
     "trs_fill_normal": (c_int32, [_V, c_uint64, c_uint64, c_void_p]),
     "trs_set_device": (c_int32, [c_int32]),

@@ -1,0 +1,712 @@
+// head.cu -- the last linear layer of a language model with its loss, without
+// the logits: softmax cross entropy against classes, and distillation from a
+// teacher's largest logits.
+//
+//   x = h w^T / temperature, lse = ln sum_v exp x_v
+//   cross entropy: loss = lse - (1 - s) x_target - s / V sum_v x_v
+//   distillation:  p = softmax(z / temperature) over the teacher's K entries,
+//                  loss = temperature^2 sum_j p_j (ln p_j - x_{id_j} + lse)
+//   gradient:      dx = g temperature (softmax(x) - t), dh = dx w, dw = dx^T h,
+//                  t the target distribution
+//
+// Rows without a target (masked positions) are listed out first and are not read.
+// This file: the checks, the rows' targets (head_teacher_kernel,
+// head_list_kernel), the join of the vocabulary's parts, and the kernels for few
+// rows, which HBM bounds: the weight is read once in f32 and every element of it
+// used for all rows.
+//
+//   head_rows_kernel  a warp per RV vocabulary rows: lanes along the width, the
+//                     hidden rows in shared memory, NR RV dot products folded by
+//                     handing over halves; then the running maximum and sum of the
+//                     softmax per lane, or the gradient of the scores
+//   head_grad_kernel  a thread per 4 columns walks vocabulary rows: a row's dw from
+//                     the hidden rows in registers, and its part of dh
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "../../include/trs.h"
+#include "head.h"
+
+namespace trs {
+
+namespace {
+
+// ---- targets ---------------------------------------------------------------------
+
+constexpr int kMaxEntries = 1024;
+
+__device__ __forceinline__ int head_id(const HeadDev& d, const RowsDev& ids, int row, int k) {
+  const int64_t at = k * ids.sd;
+  const int64_t v = d.ids64 ? head_row<const int64_t>(d, ids, row)[at] : head_row<const int32_t>(d, ids, row)[at];
+  return v < 0 || v >= d.V ? kNoToken : (int)v;
+}
+
+// A warp per row: the softmax of the entries that are there, sorted by token
+// (the rank of an entry is counted: K is small, and equal tokens keep their order).
+__global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
+  extern __shared__ int s_id[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int row = blockIdx.x * 8 + warp;
+  pdl_launch_dependents();
+  if (row >= d.N) return;
+  int* ids = s_id + warp * d.K;
+  const float* z = head_row<const float>(d, d.z, row);
+  float top = -INFINITY;
+  for (int k = lane; k < d.K; k += 32) {
+    const float x = z[k * d.z.sd];
+    int id = head_id(d, d.ids, row, k);
+    if (x == -INFINITY) id = kNoToken;
+    ids[k] = id;
+    if (id != kNoToken) top = fmaxf(top, x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  __syncwarp();
+  float sum = 0.f;
+  for (int k = lane; k < d.K; k += 32)
+    if (ids[k] != kNoToken) sum += expf(__fdiv_rn(z[k * d.z.sd] - top, d.temp));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float ln_sum = logf(sum);
+  double ent = 0.0;
+  for (int k = lane; k < d.K; k += 32) {
+    const int id = ids[k];
+    float p = 0.f;
+    if (id != kNoToken) {
+      const float a = __fdiv_rn(z[k * d.z.sd] - top, d.temp);
+      p = __fdiv_rn(expf(a), sum);
+      ent += (double)p * (double)(a - ln_sum);
+    }
+    int rank = 0;
+    for (int j = 0; j < d.K; ++j) rank += ids[j] < id || (ids[j] == id && j < k);
+    d.eid[(int64_t)row * d.K + rank] = id;
+    d.ew[(int64_t)row * d.K + rank] = p;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ent += __shfl_xor_sync(0xffffffffu, ent, o);
+  if (lane == 0) d.ent[row] = (float)ent;
+}
+
+// One CTA: the rows with a target, in order (and a class's one entry); the others
+// get their loss and lse of 0.
+__global__ void __launch_bounds__(1024) head_list_kernel(const HeadDev d) {
+  __shared__ int warps[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int done = 0;
+  for (int r0 = 0; r0 < d.N; r0 += 1024) {
+    const int row = r0 + threadIdx.x;
+    int id = kNoToken;
+    if (row < d.N) {
+      if (d.distill) {
+        id = d.eid[(int64_t)row * d.K];
+      } else {
+        id = head_id(d, d.ids, row, 0);
+        d.eid[row] = id;
+        d.ew[row] = d.weight;
+      }
+    }
+    const bool there = id != kNoToken;
+    if (row < d.N && !there && d.loss.p) {
+      *head_row<float>(d, d.loss, row) = 0.f;
+      if (d.lse.p) *head_row<float>(d, d.lse, row) = 0.f;
+    }
+    const uint32_t vote = __ballot_sync(0xffffffffu, there);
+    if (lane == 0) warps[warp] = __popc(vote);
+    __syncthreads();
+    int mine = 0, all = 0;
+    {
+      const int n = warps[lane];
+      int scan = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += y;
+      }
+      mine = __shfl_sync(0xffffffffu, scan - n, warp);
+      all = __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (there) d.rows[done + mine + __popc(vote & ((1u << lane) - 1))] = row;
+    done += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *d.live = done;
+}
+
+// Gradients of rows without a target.
+__global__ void __launch_bounds__(256) head_masked_kernel(const HeadDev d) {
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int row = blockIdx.x * 8 + threadIdx.x / 32; row < d.N; row += gridDim.x * 8) {
+    if (d.eid[(int64_t)row * d.K] != kNoToken) continue;
+    float* to = head_row<float>(d, d.dh, row);
+    for (int64_t c = threadIdx.x % 32; c < d.D; c += 32) to[c * d.dh.sd] = 0.f;
+  }
+}
+
+// ---- joining the parts of the vocabulary -------------------------------------------
+
+__device__ __forceinline__ HeadPart head_add(const HeadPart& a, const HeadPart& b) {
+  HeadPart r;
+  r.m = fmaxf(a.m, b.m);
+  // a part of -inf alone has no sum; and scores of -inf alone stay one
+  const float base = r.m == -INFINITY ? 0.f : r.m;
+  r.s = a.s * exp2f(a.m - base) + b.s * exp2f(b.m - base);
+  r.dot = a.dot + b.dot;
+  r.sum = a.sum + b.sum;
+  return r;
+}
+
+// LR rows per CTA times 256 / LR threads along a row's parts, folded in a fixed
+// order.
+template <int LR>
+__global__ void __launch_bounds__(256) head_join_kernel(const HeadDev d, const HeadPart* part, int parts, int64_t sp,
+                                                        int64_t sr) {
+  constexpr int LP = 256 / LR;
+  __shared__ HeadPart s[LP][LR];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x * LR + threadIdx.x % LR, w = threadIdx.x / LR;
+  const bool there = r < *d.live;
+  HeadPart a = {-INFINITY, 0.f, 0.f, 0.f};
+  if (there) {
+    // runs of consecutive parts, so that the order of the sums is that of the vocabulary
+    const int p0 = (int)((int64_t)parts * w / LP), p1 = (int)((int64_t)parts * (w + 1) / LP);
+    for (int p = p0; p < p1; p += 4) {
+      HeadPart x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[j] = p + j < p1 ? part[(p + j) * sp + r * sr] : HeadPart{-INFINITY, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a = head_add(a, x[j]);
+    }
+  }
+  s[w][threadIdx.x % LR] = a;
+  for (int n = LP / 2; n > 0; n /= 2) {
+    __syncthreads();
+    if (w < n) a = head_add(s[2 * w][threadIdx.x % LR], s[2 * w + 1][threadIdx.x % LR]);
+    __syncthreads();
+    if (w < n) s[w][threadIdx.x % LR] = a;
+  }
+  if (w != 0 || !there) return;
+  const int row = d.rows[r];
+  const double lse = kHeadLn2 * ((double)a.m + log2((double)a.s));
+  double loss = lse - kHeadLn2 * (double)a.dot;
+  if (d.share != 0.f) loss -= kHeadLn2 * (double)d.share * (double)a.sum;
+  if (d.distill) loss = (loss + (double)d.ent[row]) * (double)d.temp * (double)d.temp;
+  *head_row<float>(d, d.loss, row) = (float)loss;
+  if (d.lse.p) *head_row<float>(d, d.lse, row) = (float)lse;
+}
+
+}  // namespace
+
+Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
+                cudaStream_t stream) {
+  if (few) return launch_after(head_join_kernel<1>, dim3((unsigned)d.N), 256, 0, stream, "head join kernel", d, part, parts, sp, sr);
+  return launch_after(head_join_kernel<32>, dim3((unsigned)((d.N + 31) / 32)), 256, 0, stream, "head join kernel", d, part,
+                      parts, sp, sr);
+}
+
+namespace {
+
+// ---- few rows ----------------------------------------------------------------------
+
+constexpr int kRowsThreads = 256;
+constexpr int kRowsSmem = 200 * 1024;
+
+__device__ __forceinline__ uint64_t pk(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void upk(uint64_t x, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Four elements of row p from column c on; zeros behind the width.
+template <bool VEC>
+__device__ __forceinline__ float4 head_load4(const float* p, int c, int D, int64_t sd) {
+  if (VEC) return c < D ? __ldg(reinterpret_cast<const float4*>(p + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 r;
+  r.x = c < D ? p[c * sd] : 0.f;
+  r.y = c + 1 < D ? p[(c + 1) * sd] : 0.f;
+  r.z = c + 2 < D ? p[(c + 2) * sd] : 0.f;
+  r.w = c + 3 < D ? p[(c + 3) * sd] : 0.f;
+  return r;
+}
+
+// The sums over the warp of Q values per lane, by handing over halves: lane l
+// ends with value l / (32 / Q).
+template <int Q>
+__device__ __forceinline__ float head_fold(float (&a)[Q], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = Q; n > 1; n /= 2, o /= 2)
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float keep = lane & o ? a[i + n / 2] : a[i], give = lane & o ? a[i] : a[i + n / 2];
+      a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+#pragma unroll
+  for (; o > 0; o /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+  return a[0];
+}
+
+struct HeadRowsDev {
+  HeadDev d;
+  int r0;                // first live row of this launch
+  int Dp;                // the width rounded up to whole steps of 128
+  HeadPart* part;        // forward: [live row][CTA]
+  float* dx;             // backward: [V][NR]
+};
+
+template <int NR, int RV, bool VEC, bool GRAD>
+__global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const __grid_constant__ HeadRowsDev a) {
+  constexpr int Q = NR * RV, REP = 32 / Q, W = kRowsThreads / 32;
+  extern __shared__ float4 s_h[];
+  const HeadDev& d = a.d;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, live = *d.live;
+  pdl_launch_dependents();
+  if (a.r0 >= live) return;
+  for (int i = threadIdx.x; i < NR * a.Dp / 4; i += kRowsThreads) {
+    const int n = i / (a.Dp / 4), c = i % (a.Dp / 4) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.r0 + n < live) {
+      const float* p = head_row<const float>(d, d.hid, d.rows[a.r0 + n]);
+      x = head_load4<false>(p, c, d.D, d.hid.sd);
+    }
+    s_h[i] = x;
+  }
+  __syncthreads();
+  const int q = lane / REP, n = q % NR, rv = q / NR;
+  const bool there = a.r0 + n < live;
+  const int row = d.rows[there ? a.r0 + n : a.r0];
+  Entries ent;
+  ent.begin(d, row);
+  const float f = d.inv_temp * kHeadLog2e;
+  float lse2 = 0.f, g = 0.f;
+  if (GRAD) {
+    lse2 = *head_row<const float>(d, d.lse, row) * kHeadLog2e;
+    g = *head_row<const float>(d, d.gl, row) * d.temp;
+  }
+  HeadPart pt = {-INFINITY, 0.f, 0.f, 0.f};
+  for (int64_t v0 = ((int64_t)blockIdx.x * W + warp) * RV; v0 < d.V; v0 += (int64_t)gridDim.x * W * RV) {
+    uint64_t acc[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) acc[i] = 0;
+#pragma unroll 2
+    for (int c = lane * 4; c < a.Dp; c += 128) {
+      float4 x[RV];
+#pragma unroll
+      for (int j = 0; j < RV; ++j)
+        x[j] = v0 + j < d.V ? head_load4<VEC>(d.w + (v0 + j) * d.wv, c, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const float4 h = s_h[(i * a.Dp + c) / 4];
+        const uint64_t h0 = pk(h.x, h.y), h1 = pk(h.z, h.w);
+#pragma unroll
+        for (int j = 0; j < RV; ++j)
+          acc[j * NR + i] = fma2(pk(x[j].z, x[j].w), h1, fma2(pk(x[j].x, x[j].y), h0, acc[j * NR + i]));
+      }
+    }
+    float sums[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      float lo, hi;
+      upk(acc[i], &lo, &hi);
+      sums[i] = lo + hi;
+    }
+    const float x = head_fold<Q>(sums, lane) * f;  // in units of log2
+    const int64_t v = v0 + rv;
+    if (v >= d.V || !there) {
+      if (GRAD && v < d.V && lane % REP == 0) a.dx[v * NR + n] = 0.f;
+      continue;
+    }
+    float t = 0.f;
+    if (ent.next <= v) {
+      ent.skip_to((int)v);
+      t = ent.take((int)v);
+    }
+    if (GRAD) {
+      if (lane % REP == 0) a.dx[v * NR + n] = g * (head_ex2(x - lse2) - t - d.share);
+    } else {
+      const float m = fmaxf(pt.m, x);
+      pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(x - m);
+      if (m == -INFINITY) pt.s = 0.f;  // scores of -inf alone
+      pt.m = m;
+      if (t != 0.f) pt.dot = __fmaf_rn(t, x, pt.dot);
+      pt.sum += x;
+    }
+  }
+  if (GRAD) return;
+  // the CTA's parts of a row: RV lanes of each warp
+  HeadPart* s = reinterpret_cast<HeadPart*>(s_h);
+  __syncthreads();
+  if (lane % REP == 0) s[(warp * RV + rv) * NR + n] = pt;
+  for (int k = W * RV / 2; k > 0; k /= 2) {
+    __syncthreads();
+    const int w = threadIdx.x / NR, i = threadIdx.x % NR;
+    HeadPart y;
+    if (w < k) y = head_add(s[2 * w * NR + i], s[(2 * w + 1) * NR + i]);
+    __syncthreads();
+    if (w < k) s[w * NR + i] = y;
+  }
+  __syncthreads();
+  if (threadIdx.x < NR && a.r0 + threadIdx.x < live)
+    a.part[(int64_t)(a.r0 + threadIdx.x) * gridDim.x + blockIdx.x] = s[threadIdx.x];
+}
+
+struct HeadGradDev {
+  HeadDev d;
+  int r0;
+  const float* dx;       // [V][NR]
+  float* part;           // [CTA along V][NR][D] of dh
+};
+
+// 256 threads by 4 columns; blockIdx.y: a range of the vocabulary.
+template <int NR>
+__global__ void __launch_bounds__(256) head_grad_kernel(const __grid_constant__ HeadGradDev a) {
+  const HeadDev& d = a.d;
+  const int live = *d.live;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (c >= d.D || a.r0 >= (live > 0 ? live : 1)) return;
+  float h[NR][4], acc[NR][4];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.r0 + i < live) x = head_load4<false>(head_row<const float>(d, d.hid, d.rows[a.r0 + i]), c, d.D, d.hid.sd);
+    h[i][0] = x.x, h[i][1] = x.y, h[i][2] = x.z, h[i][3] = x.w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  }
+  const int64_t v1 = (int64_t)d.V * (blockIdx.y + 1) / gridDim.y;
+#pragma unroll 2
+  for (int64_t v = (int64_t)d.V * blockIdx.y / gridDim.y; v < v1; ++v) {
+    float x[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) x[i] = live > 0 ? __ldg(a.dx + v * NR + i) : 0.f;
+    if (d.dh.p) {
+      const float4 w = d.vec_w ? head_load4<true>(d.w + v * d.wv, c, d.D, 1) : head_load4<false>(d.w + v * d.wv, c, d.D, d.wd);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        acc[i][0] = __fmaf_rn(x[i], w.x, acc[i][0]);
+        acc[i][1] = __fmaf_rn(x[i], w.y, acc[i][1]);
+        acc[i][2] = __fmaf_rn(x[i], w.z, acc[i][2]);
+        acc[i][3] = __fmaf_rn(x[i], w.w, acc[i][3]);
+      }
+    }
+    if (d.dw) {
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = __fmaf_rn(x[i], h[i][j], o[j]);
+      float* to = d.dw + v * d.dwv;
+      if (d.vec_dw) {
+        float4 y = make_float4(o[0], o[1], o[2], o[3]);
+        if (a.r0 > 0) {  // behind earlier rows
+          const float4 b = *reinterpret_cast<const float4*>(to + c);
+          y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
+        }
+        *reinterpret_cast<float4*>(to + c) = y;
+      } else {
+        for (int j = 0; j < 4 && c + j < d.D; ++j) {
+          float* e = to + (c + j) * d.dwd;
+          *e = a.r0 > 0 ? *e + o[j] : o[j];
+        }
+      }
+    }
+  }
+  if (!d.dh.p) return;
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    for (int j = 0; j < 4 && c + j < d.D; ++j)
+      a.part[((int64_t)blockIdx.y * NR + i) * d.D + c + j] = acc[i][j];
+}
+
+// dh of up to NR rows from its parts, in order: 32 columns times 8 parts per CTA.
+template <int NR>
+__global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_constant__ HeadGradDev a, int parts) {
+  __shared__ float s[8][32];
+  const HeadDev& d = a.d;
+  pdl_wait();
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32, r = blockIdx.y;
+  if (a.r0 + r >= *d.live) return;
+  float sum = 0.f;
+  if (c < d.D)
+    for (int p = (int)((int64_t)parts * w / 8); p < (int)((int64_t)parts * (w + 1) / 8); ++p)
+      sum += a.part[((int64_t)p * NR + r) * d.D + c];
+  s[w][threadIdx.x % 32] = sum;
+  __syncthreads();
+  if (w != 0 || c >= d.D) return;
+  for (int i = 1; i < 8; ++i) sum += s[i][threadIdx.x];
+  head_row<float>(d, d.dh, d.rows[a.r0 + r])[c * d.dh.sd] = sum;
+}
+
+// ---- host side -------------------------------------------------------------------
+
+template <int NR, int RV, bool GRAD>
+Error launch_rows(HeadRowsDev& a, int ctas, cudaStream_t s) {
+  auto k = a.d.vec_w ? head_rows_kernel<NR, RV, true, GRAD> : head_rows_kernel<NR, RV, false, GRAD>;
+  const int smem = std::max<int>(NR * a.Dp * 4, kRowsThreads * (int)sizeof(HeadPart));
+  allow_smem((const void*)k, smem);
+  k<<<(unsigned)ctas, kRowsThreads, smem, s>>>(a);
+  return check_launch("head rows kernel");
+}
+template <bool GRAD>
+Error rows_of(int nr, HeadRowsDev& a, int ctas, cudaStream_t s) {
+  return nr == 1 ? launch_rows<1, 8, GRAD>(a, ctas, s) : nr == 2 ? launch_rows<2, 8, GRAD>(a, ctas, s)
+         : nr == 4 ? launch_rows<4, 4, GRAD>(a, ctas, s) : launch_rows<8, 4, GRAD>(a, ctas, s);
+}
+
+template <int NR>
+Error launch_grad(HeadGradDev& a, int splits, cudaStream_t s) {
+  Error e = launch_after(head_grad_kernel<NR>, dim3((unsigned)((a.d.D + 1023) / 1024), (unsigned)splits), 256, 0, s,
+                         "head gradient kernel", a);
+  if (!e.ok() || !a.d.dh.p) return e;
+  return launch_after(head_grad_join_kernel<NR>, dim3((unsigned)((a.d.D + 31) / 32), (unsigned)NR), 256, 0, s,
+                      "head gradient join kernel", a, splits);
+}
+
+Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
+  const int sms = current_device_info().sm_count;
+  HeadRowsDev a;
+  std::memset(static_cast<void*>(&a), 0, sizeof(a));
+  a.d = d;
+  a.Dp = (d.D + 127) / 128 * 128;
+  int nr = d.N >= 5 ? 8 : d.N >= 3 ? 4 : std::max(1, d.N);
+  while (nr > 1 && nr * a.Dp * 4 > kRowsSmem) nr /= 2;
+  const int ctas = 2 * sms;
+  Scratch mem;
+  Error e;
+  if (!backward) {
+    e = mem.alloc(sizeof(HeadPart) * (size_t)d.N * ctas, s);
+    if (!e.ok()) return e;
+    a.part = mem.as<HeadPart>();
+    for (a.r0 = 0; e.ok() && a.r0 < d.N; a.r0 += nr) e = rows_of<false>(nr, a, ctas, s);
+    if (e.ok()) e = head_join(d, a.part, ctas, 1, ctas, true, s);
+    return e;
+  }
+  const int colblocks = (d.D + 1023) / 1024;
+  const int splits = std::max(1, std::min(d.V, 4 * sms / colblocks));
+  const size_t nd = (size_t)d.V * nr;
+  e = mem.alloc(sizeof(float) * (nd + (size_t)splits * nr * d.D), s);
+  if (!e.ok()) return e;
+  a.dx = mem.as<float>();
+  HeadGradDev g;
+  std::memset(static_cast<void*>(&g), 0, sizeof(g));
+  g.d = d;
+  g.dx = a.dx;
+  g.part = a.dx + nd;
+  for (a.r0 = 0; e.ok() && (a.r0 == 0 || a.r0 < d.N); a.r0 += nr) {  // without rows: zeros into dw
+    g.r0 = a.r0;
+    e = rows_of<true>(nr, a, ctas, s);
+    if (!e.ok()) return e;
+    e = nr == 1 ? launch_grad<1>(g, splits, s) : nr == 2 ? launch_grad<2>(g, splits, s)
+        : nr == 4 ? launch_grad<4>(g, splits, s) : launch_grad<8>(g, splits, s);
+  }
+  return e;
+}
+
+struct HeadCall {
+  const char* fn;
+  bool distill, backward;
+  const trs_view *hidden, *weight, *ids, *logits;
+  double smoothing, temperature;
+  trs_view *loss, *lse;              // lse: read by the backward
+  const trs_view* grad_loss;
+  trs_view *grad_hidden, *grad_weight;
+};
+
+Error run_head(const HeadCall& c, cudaStream_t stream) {
+  const std::string fn = c.fn;
+  if (!c.hidden || !c.weight || !c.ids || (c.distill && !c.logits) || (!c.backward && !c.loss) ||
+      (c.backward && (!c.grad_loss || !c.lse || (!c.grad_hidden && !c.grad_weight))))
+    return make_error(TRS_ERR_ARG, fn + ": null view");
+  Error e = validate_view(c.hidden, "hidden");
+  if (!e.ok()) return e;
+  if (c.hidden->ndim < 2 || c.hidden->ndim > 3)
+    return make_error(TRS_ERR_SHAPE, fn + ": hidden must be [tokens, width] or [batch, tokens, width]");
+  const Tokens t = tokens_of(c.hidden, c.hidden->ndim - 1);
+  e = validate_view(c.weight, "the weight");
+  if (!e.ok()) return e;
+  if (c.weight->ndim != 2 || c.weight->shape[1] != c.hidden->shape[t.lead])
+    return make_error(TRS_ERR_SHAPE, fn + ": the weight must be [vocabulary, width]");
+  e = check_tokens(fn, c.ids, t, c.distill ? 1 : 0, c.distill ? "the teacher's ids" : "targets");
+  if (e.ok() && c.distill) e = check_tokens(fn, c.logits, t, 1, "the teacher's logits");
+  if (e.ok() && c.loss) e = check_tokens(fn, c.loss, t, 0, "the loss");
+  if (e.ok() && c.lse) e = check_tokens(fn, c.lse, t, 0, "lse");
+  if (e.ok() && c.grad_loss) e = check_tokens(fn, c.grad_loss, t, 0, "the loss gradient");
+  if (e.ok() && c.grad_hidden) e = check_tokens(fn, c.grad_hidden, t, 1, "the hidden gradient");
+  if (e.ok() && c.grad_weight) e = validate_view(c.grad_weight, "the weight gradient");
+  if (!e.ok()) return e;
+  if (c.grad_hidden && c.grad_hidden->shape[t.lead] != c.hidden->shape[t.lead])
+    return make_error(TRS_ERR_SHAPE, fn + ": the hidden gradient must have the shape of hidden");
+  if (c.grad_weight && !same_shape(c.grad_weight, c.weight))
+    return make_error(TRS_ERR_SHAPE, fn + ": the weight gradient must have the shape of the weight");
+  for (const trs_view* v : {c.hidden, c.weight, c.logits, (const trs_view*)c.loss, (const trs_view*)c.lse, c.grad_loss,
+                            (const trs_view*)c.grad_hidden, (const trs_view*)c.grad_weight})
+    if (v && v->dtype != TRS_F32) return make_error(TRS_ERR_DTYPE, fn + ": everything but the ids must be f32");
+  if (c.ids->dtype != TRS_I32 && c.ids->dtype != TRS_I64)
+    return make_error(TRS_ERR_DTYPE, fn + ": ids must be i32 or i64");
+  const int64_t V = c.weight->shape[0], D = c.weight->shape[1], N = t.n();
+  int64_t K = 1;
+  if (c.distill) {
+    K = c.ids->shape[t.lead];
+    if (c.logits->shape[t.lead] != K)
+      return make_error(TRS_ERR_SHAPE, fn + ": the teacher's ids and logits must have one shape");
+    if (K < 1 || K > kMaxEntries) return make_error(TRS_ERR_SHAPE, fn + ": a teacher gives 1 to 1024 logits");
+  }
+  if (V < 1 || D < 1) return make_error(TRS_ERR_SHAPE, fn + ": an empty weight");
+  if (!(c.smoothing >= 0.0 && c.smoothing <= 1.0))
+    return make_error(TRS_ERR_ARG, fn + ": the smoothing must lie in [0, 1]");
+  // its square, its inverse and the products with them stay f32 numbers
+  if (!(c.temperature >= 0x1p-40 && c.temperature <= 0x1p40))
+    return make_error(TRS_ERR_ARG, fn + ": the temperature must lie in [2^-40, 2^40]");
+  const int64_t lim = 1ll << 30;
+  if (t.B >= lim || t.T >= lim || N >= lim || V >= lim || D >= lim)
+    return make_error(TRS_ERR_SHAPE, fn + ": 2^30 or more tokens, or rows or columns of the weight");
+  e = c.backward ? check_outputs(fn, {c.grad_hidden, c.grad_weight},
+                                 {c.hidden, c.weight, c.ids, c.logits, c.lse, c.grad_loss})
+                 : check_outputs(fn, {c.loss, c.lse}, {c.hidden, c.weight, c.ids, c.logits});
+  if (!e.ok()) return e;
+
+  HeadDev d;
+  std::memset(static_cast<void*>(&d), 0, sizeof(d));
+  d.N = (int)N;
+  d.V = (int)V;
+  d.D = (int)D;
+  d.K = (int)K;
+  d.f_T = make_fastdiv((uint32_t)std::max<int64_t>(t.T, 1));
+  d.hid = rows_dev(c.hidden, t);
+  d.w = static_cast<const float*>(c.weight->data) + c.weight->offset;
+  d.wv = c.weight->strides[0];
+  d.wd = c.weight->strides[1];
+  d.ids = rows_dev(c.ids, t);
+  d.ids64 = c.ids->dtype == TRS_I64;
+  if (c.distill) d.z = rows_dev(c.logits, t);
+  if (c.loss) d.loss = rows_dev(c.loss, t);
+  if (c.lse) d.lse = rows_dev(c.lse, t);
+  d.distill = c.distill;
+  d.temp = (float)c.temperature;
+  d.inv_temp = (float)(1.0 / c.temperature);
+  d.share = (float)(c.smoothing / (double)V);
+  d.weight = (float)(1.0 - c.smoothing);
+  d.vec_w = rows_vectors(c.weight);
+  if (c.backward) {
+    d.gl = rows_dev(c.grad_loss, t);
+    if (c.grad_hidden) d.dh = rows_dev(c.grad_hidden, t);
+    if (c.grad_weight) {
+      d.dw = static_cast<float*>(c.grad_weight->data) + c.grad_weight->offset;
+      d.dwv = c.grad_weight->strides[0];
+      d.dwd = c.grad_weight->strides[1];
+      d.vec_dw = rows_vectors(c.grad_weight);
+    }
+  }
+  if (N > 0) {
+    d.vec_h = rows_vectors(c.hidden);
+    d.vec_dh = c.grad_hidden && rows_vectors(c.grad_hidden);
+  }
+  if (N == 0 && !d.dw) return Error{};
+  // the rows' targets
+  Scratch mem;
+  const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;
+  e = mem.alloc(4 * (n + 4 + 2 * nk + (c.distill ? n : 0)), stream);
+  if (!e.ok()) return e;
+  d.live = mem.as<int>();
+  d.rows = d.live + 4;
+  d.eid = d.rows + n;
+  d.ew = reinterpret_cast<float*>(d.eid + nk);
+  d.ent = d.ew + nk;
+  if (c.distill && N > 0) {
+    const int smem = 8 * d.K * 4;
+    head_teacher_kernel<<<(unsigned)((N + 7) / 8), 256, smem, stream>>>(d);
+    e = check_launch("head teacher kernel");
+    if (!e.ok()) return e;
+    e = launch_after(head_list_kernel, dim3(1), 1024, 0, stream, "head list kernel", d);
+  } else {
+    head_list_kernel<<<1, 1024, 0, stream>>>(d);
+    e = check_launch("head list kernel");
+  }
+  if (!e.ok()) return e;
+  if (c.grad_hidden && N > 0) {
+    e = launch_after(head_masked_kernel, dim3((unsigned)std::min<int64_t>((N + 7) / 8, 1024)), 256, 0, stream,
+                     "head masked rows kernel", d);
+    if (!e.ok()) return e;
+  }
+  return run_rows(d, c.backward, stream);
+}
+
+trs_status finish(const Error& e) {
+  if (!e.ok()) set_last_error(e.msg);
+  return e.status;
+}
+
+// Nothing thrown leaves a C entry.
+template <class F>
+trs_status guarded(F f) {
+  try {
+    return finish(f());
+  } catch (...) {
+    return TRS_ERR_OOM;
+  }
+}
+
+}  // namespace
+}  // namespace trs
+
+using namespace trs;
+
+extern "C" {
+
+trs_status trs_linear_cross_entropy(const trs_view* hidden, const trs_view* weight, const trs_view* targets,
+                                    double smoothing, trs_view* loss, trs_view* lse, trs_stream stream) {
+  return guarded([&] {
+    return run_head(HeadCall{"linear_cross_entropy", false, false, hidden, weight, targets, nullptr, smoothing, 1.0, loss,
+                             lse, nullptr, nullptr, nullptr},
+                    static_cast<cudaStream_t>(stream));
+  });
+}
+
+trs_status trs_linear_cross_entropy_backward(const trs_view* grad_loss, const trs_view* hidden, const trs_view* weight,
+                                             const trs_view* targets, const trs_view* lse, double smoothing,
+                                             trs_view* grad_hidden, trs_view* grad_weight, trs_stream stream) {
+  return guarded([&] {
+    return run_head(HeadCall{"linear_cross_entropy_backward", false, true, hidden, weight, targets, nullptr, smoothing, 1.0,
+                             nullptr, const_cast<trs_view*>(lse), grad_loss, grad_hidden, grad_weight},
+                    static_cast<cudaStream_t>(stream));
+  });
+}
+
+trs_status trs_linear_distillation(const trs_view* hidden, const trs_view* weight, const trs_view* teacher_ids,
+                                   const trs_view* teacher_logits, double temperature, trs_view* loss, trs_view* lse,
+                                   trs_stream stream) {
+  return guarded([&] {
+    return run_head(HeadCall{"linear_distillation", true, false, hidden, weight, teacher_ids, teacher_logits, 0.0,
+                             temperature, loss, lse, nullptr, nullptr, nullptr},
+                    static_cast<cudaStream_t>(stream));
+  });
+}
+
+trs_status trs_linear_distillation_backward(const trs_view* grad_loss, const trs_view* hidden, const trs_view* weight,
+                                            const trs_view* teacher_ids, const trs_view* teacher_logits,
+                                            const trs_view* lse, double temperature, trs_view* grad_hidden,
+                                            trs_view* grad_weight, trs_stream stream) {
+  return guarded([&] {
+    return run_head(HeadCall{"linear_distillation_backward", true, true, hidden, weight, teacher_ids, teacher_logits, 0.0,
+                             temperature, nullptr, const_cast<trs_view*>(lse), grad_loss, grad_hidden, grad_weight},
+                    static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,104 @@
+// head.h -- what the translation units of a model's last layer share (head.cu:
+// checks, the rows' targets, the CUDA-core kernels; head_tc.cu: the tensor-core
+// kernels).
+//
+// Both losses are  lse(x) - sum_v t_v x_v  of the scores x = h w^T / temperature
+// against a target distribution t, up to a constant of the row and the factor
+// temperature^2; t is a few entries (one for a class, K for a teacher's logits)
+// and, for smoothed classes, s / V everywhere.  The gradient of x is softmax(x) - t.
+// A row's entries are prepared once per call, sorted by their token, so that a
+// thread that walks the vocabulary in order meets them in order.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kernels.cuh"
+#include "tokens.h"
+
+namespace trs {
+
+constexpr float kHeadLog2e = 1.4426950408889634f;
+constexpr double kHeadLn2 = 0.6931471805599453;
+constexpr int kNoToken = 0x7fffffff;
+
+struct HeadDev {
+  RowsDev hid, dh;               // [.., D]
+  const float* w;                // [V, D]
+  int64_t wv, wd;
+  float* dw;                     // or null
+  int64_t dwv, dwd;
+  RowsDev ids, z;                // targets [..], or teacher ids and logits [.., K]
+  int ids64;
+  RowsDev gl, loss, lse;         // [..]
+  int N, V, D, K;
+  FastDiv f_T;
+  int distill;
+  float temp, inv_temp;
+  float share;                   // s / V
+  float weight;                  // 1 - s, a class's entry
+  // prepared by head_targets
+  int* rows;                     // the rows with a target, in order
+  int* live;                     // how many
+  int* eid;                      // [N][K] tokens of a row's entries, ascending, kNoToken behind them
+  float* ew;                     // [N][K] their weights
+  float* ent;                    // [N] sum of w ln w (distillation)
+  int vec_h, vec_w, vec_dh, vec_dw;  // 16-byte accesses along D
+};
+
+__device__ __forceinline__ float head_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <class T>
+__device__ __forceinline__ T* head_row(const HeadDev& d, const RowsDev& r, int i) {
+  const uint32_t b = fdiv((uint32_t)i, d.f_T), t = (uint32_t)i - b * d.f_T.d;
+  return static_cast<T*>(r.p) + b * r.sb + t * r.st;
+}
+
+// The walk of one row's entries along ascending tokens.
+struct Entries {
+  const int* id;
+  const float* w;
+  int left;
+  int next;
+  __device__ __forceinline__ void begin(const HeadDev& d, int row) {
+    id = d.eid + (int64_t)row * d.K;
+    w = d.ew + (int64_t)row * d.K;
+    left = d.K;
+    next = *id;
+  }
+  __device__ __forceinline__ void step() {
+    ++w;
+    ++id;
+    next = --left > 0 ? *id : kNoToken;
+  }
+  // skips entries below v (a binary search is not worth it for a step of a tile)
+  __device__ __forceinline__ void skip_to(int v) {
+    while (next < v) step();
+  }
+  // the weight of token v, which next may have reached
+  __device__ __forceinline__ float take(int v) {
+    float s = 0.f;
+    while (next == v) {
+      s += *w;
+      step();
+    }
+    return s;
+  }
+};
+
+// Partial statistics of a row over a part of the vocabulary: the largest score
+// in units of log2, the sum of 2^(score - largest), sum of weight times score and
+// sum of scores in units of log2 too.
+struct HeadPart {
+  float m, s, dot, sum;
+};
+// part p of live row r lies at p * sp + r * sr
+Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
+                cudaStream_t stream);
+
+}  // namespace trs

@@ -352,6 +352,43 @@ def embedding_backward(grad_out: abi.View, ids: abi.View, scale: float, grad_tab
     return grad_table
 
 
+def linear_cross_entropy(hidden: abi.View, weight: abi.View, targets: abi.View, loss: torch.Tensor,
+                         lse: torch.Tensor | None = None, smoothing: float = 0.0) -> torch.Tensor:
+    """Softmax cross entropy of hidden weight^T per token, without the logits; lse is what the backward needs."""
+    h = torch.cuda.current_device()
+    _call("trs_linear_cross_entropy", _in(hidden, h), _in(weight, h), _in(targets, h), float(smoothing), _out(loss, h),
+          _out(lse, h), stream_handle(h))
+    return loss
+
+
+def linear_cross_entropy_backward(grad_loss: abi.View, hidden: abi.View, weight: abi.View, targets: abi.View,
+                                  lse: abi.View, grad_hidden: torch.Tensor | None, grad_weight: torch.Tensor | None,
+                                  smoothing: float = 0.0) -> None:
+    """The gradients of linear_cross_entropy for hidden and the weight."""
+    h = torch.cuda.current_device()
+    _call("trs_linear_cross_entropy_backward", _in(grad_loss, h), _in(hidden, h), _in(weight, h), _in(targets, h),
+          _in(lse, h), float(smoothing), _out(grad_hidden, h), _out(grad_weight, h), stream_handle(h))
+
+
+def linear_distillation(hidden: abi.View, weight: abi.View, teacher_ids: abi.View, teacher_logits: abi.View,
+                        temperature: float, loss: torch.Tensor, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """The divergence of softmax(hidden weight^T / temperature) from a teacher's largest logits, per token."""
+    h = torch.cuda.current_device()
+    _call("trs_linear_distillation", _in(hidden, h), _in(weight, h), _in(teacher_ids, h), _in(teacher_logits, h),
+          float(temperature), _out(loss, h), _out(lse, h), stream_handle(h))
+    return loss
+
+
+def linear_distillation_backward(grad_loss: abi.View, hidden: abi.View, weight: abi.View, teacher_ids: abi.View,
+                                 teacher_logits: abi.View, lse: abi.View, temperature: float,
+                                 grad_hidden: torch.Tensor | None, grad_weight: torch.Tensor | None) -> None:
+    """The gradients of linear_distillation for hidden and the weight."""
+    h = torch.cuda.current_device()
+    _call("trs_linear_distillation_backward", _in(grad_loss, h), _in(hidden, h), _in(weight, h), _in(teacher_ids, h),
+          _in(teacher_logits, h), _in(lse, h), float(temperature), _out(grad_hidden, h), _out(grad_weight, h),
+          stream_handle(h))
+
+
 def fill_uniform(out: torch.Tensor, seed: int, lo: float = -1.0, hi: float = 1.0, first: int = 0) -> torch.Tensor:
     _call("trs_fill_uniform", ctypes.byref(view_of(out)), seed, first, lo, hi, stream_handle())
     return out
