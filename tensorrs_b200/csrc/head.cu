@@ -644,6 +644,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
                      "head masked rows kernel", d);
     if (!e.ok()) return e;
   }
+  if (N > 16) return head_tc(d, c.backward, stream);
   return run_rows(d, c.backward, stream);
 }
 

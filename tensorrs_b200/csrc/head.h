@@ -76,6 +76,19 @@ struct Entries {
     ++id;
     next = --left > 0 ? *id : kNoToken;
   }
+  // the first entry not below v
+  __device__ __forceinline__ void seek(const HeadDev& d, int row, int v) {
+    const int* all = d.eid + (int64_t)row * d.K;
+    int lo = 0, hi = d.K;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (all[mid] < v) lo = mid + 1; else hi = mid;
+    }
+    id = all + lo;
+    w = d.ew + (int64_t)row * d.K + lo;
+    left = d.K - lo;
+    next = left > 0 ? *id : kNoToken;
+  }
   // skips entries below v (a binary search is not worth it for a step of a tile)
   __device__ __forceinline__ void skip_to(int v) {
     while (next < v) step();
@@ -100,5 +113,8 @@ struct HeadPart {
 // part p of live row r lies at p * sp + r * sr
 Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
                 cudaStream_t stream);
+
+// The tensor-core path (head_tc.cu).
+Error head_tc(const HeadDev& d, bool backward, cudaStream_t stream);
 
 }  // namespace trs

@@ -1,0 +1,897 @@
+// head_tc.cu -- a model's last layer with its loss on the 5th-generation tensor
+// cores, for more rows than the CUDA cores serve at HBM's rate.
+//
+// Products.  f32 operands are written 2^e (hi + lo) with hi and lo in fp16, 11
+// bits each, e placing the largest magnitude in [2^14, 2^15): of a hidden row,
+// of a piece of the weight, of all rows of g h.  A product is hi hi + (hi lo + lo
+// hi), three tcgen05.mma with f32 accumulation.  The gradient of the scores
+// without the row's own factor, softmax(x) - t, lies in [-1, 1] and is split under
+// the fixed 2^15; the factor g temperature goes into g h for dw and onto the
+// rows of dh, so that rows with very different gradients keep their digits.
+// The tensor core cuts its sums instead of rounding them, so a sum leaves the
+// accumulator for f32 registers every 256 elements.
+//
+//   head_pack_*       the planes [hi, lo] of hidden rows (those with a target,
+//                     gathered), of a piece of the weight and of g h
+//   head_gemm_kernel  persistent CTA pairs, 256 x 256 tiles: a warp streams
+//                     64-element slabs of both operands by TMA, one warp issues
+//                     the MMAs of the pair (tcgen05 cta_group::2: each CTA holds
+//                     half of A and half of B, and its 128 rows of the result),
+//                     two warpgroups add what leaves the accumulator and finish
+//                     the tile:
+//       kScores       statistics of each row over the tile (HeadPart)
+//       kScoreGrad    softmax(x) - t, split, into planes
+//       kProducts     dw = dx^T h and dh = dx w from those planes, the contraction
+//                     along the rows of both (MN-major operands)
+//
+// The vocabulary is taken in pieces, so that the planes of the weight and of dx
+// stay small; dh collects the pieces in their order.  No atomics add values.
+//
+// Every wait is bounded; a CTA whose wait runs out sets the async-error word,
+// lets its copies and MMAs end, frees its tensor memory and returns.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "head.h"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace trs {
+namespace {
+
+// a b c, in an order in which no step leaves the range when the product does not
+__device__ __forceinline__ float mul3(float a, float b, float c) {
+  const float x = fabsf(a), y = fabsf(b), z = fabsf(c);
+  if (x > y) return y > z ? a * c * b : x > z ? a * b * c : b * c * a;
+  return x > z ? b * c * a : y > z ? a * b * c : a * c * b;
+}
+
+// ---- planes ---------------------------------------------------------------------
+
+struct PlanesDev {
+  HeadDev d;
+  __half* to;            // [2][rows][Dp]
+  int64_t plane;         // elements of a plane
+  int Dp;                // the width rounded up to whole slabs of 64
+  float* down;           // hidden: 2^e of every row; weight, g h: one
+  uint32_t* top;         // largest magnitude, as bits
+  int v0, n;             // weight: the piece's first row and its rows
+};
+
+// 2^k and 2^-k that bring a largest magnitude (its bits) into [2^14, 2^15),
+// within what an f32 holds.
+__device__ __forceinline__ void plane_scale(uint32_t top, float* up, float* down) {
+  int k = 14 - ((int)(top >> 23) - 127);
+  k = k > 126 ? 126 : k < -126 ? -126 : k;
+  *up = __uint_as_float((uint32_t)(k + 127) << 23);
+  *down = __uint_as_float((uint32_t)(127 - k) << 23);
+}
+__device__ __forceinline__ uint32_t block_top(uint32_t x, uint32_t* sm) {  // 256 threads
+  x = __reduce_max_sync(0xffffffffu, x);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = x;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, sm[threadIdx.x % 8]);
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __forceinline__ float4 piece4(const float* p, int c, int D, int64_t sd, bool vec) {
+  if (vec && c < D) return *reinterpret_cast<const float4*>(p + c);
+  float4 r;
+  r.x = c < D ? p[c * sd] : 0.f;
+  r.y = c + 1 < D ? p[(c + 1) * sd] : 0.f;
+  r.z = c + 2 < D ? p[(c + 2) * sd] : 0.f;
+  r.w = c + 3 < D ? p[(c + 3) * sd] : 0.f;
+  return r;
+}
+__device__ __forceinline__ void split_store(__half* to, int64_t plane, float a, float b, float c, float e) {
+  const float v[4] = {a, b, c, e};
+  __half h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = __float2half_rn(v[j]);
+    l[j] = __float2half_rn(v[j] - __half2float(h[j]));
+  }
+  *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(h);
+  *reinterpret_cast<uint2*>(to + plane) = *reinterpret_cast<uint2*>(l);
+}
+
+// Hidden rows with a target, gathered: a CTA per row; zeros behind the last one up
+// to a whole tile.  With a gradient also the largest |g temperature h|.
+__global__ void __launch_bounds__(256) head_pack_hidden_kernel(const __grid_constant__ PlanesDev a) {
+  __shared__ uint32_t sm[8];
+  const HeadDev& d = a.d;
+  const int live = *d.live, r = blockIdx.x;
+  if (r >= (live + 255) / 256 * 256) return;
+  const float* p = r < live ? head_row<const float>(d, d.hid, d.rows[r]) : nullptr;
+  uint32_t top = 0;
+  if (p)
+    for (int c = threadIdx.x * 4; c < d.D; c += 1024) {
+      const float4 x = piece4(p, c, d.D, d.hid.sd, d.vec_h);
+      top = max(max(top, max(magnitude(x.x), magnitude(x.y))), max(magnitude(x.z), magnitude(x.w)));
+    }
+  top = block_top(top, sm);
+  float up, down;
+  plane_scale(top, &up, &down);
+  if (threadIdx.x == 0) {
+    a.down[r] = down;
+    if (a.top && p) {
+      const float g = *head_row<const float>(d, d.gl, d.rows[r]) * d.temp;
+      atomicMax(a.top, magnitude(g * __uint_as_float(top)));
+    }
+  }
+  for (int c = threadIdx.x * 4; c < a.Dp; c += 1024) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p) x = piece4(p, c, d.D, d.hid.sd, d.vec_h);
+    split_store(a.to + (int64_t)r * a.Dp + c, a.plane, x.x * up, x.y * up, x.z * up, x.w * up);
+  }
+}
+
+// g temperature h of the same rows, under one power of two.
+__global__ void __launch_bounds__(256) head_pack_grad_kernel(const __grid_constant__ PlanesDev a) {
+  const HeadDev& d = a.d;
+  const int live = *d.live, r = blockIdx.x;
+  float up, down;
+  plane_scale(*a.top, &up, &down);
+  if (r == 0 && threadIdx.x == 0) *a.down = down;
+  if (r >= (live + 255) / 256 * 256) return;
+  const float* p = r < live ? head_row<const float>(d, d.hid, d.rows[r]) : nullptr;
+  const float g = p ? *head_row<const float>(d, d.gl, d.rows[r]) * d.temp : 0.f;
+  for (int c = threadIdx.x * 4; c < a.Dp; c += 1024) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p) x = piece4(p, c, d.D, d.hid.sd, d.vec_h);
+    split_store(a.to + (int64_t)r * a.Dp + c, a.plane, mul3(x.x, g, up), mul3(x.y, g, up), mul3(x.z, g, up),
+                mul3(x.w, g, up));
+  }
+}
+
+// The largest magnitude of a piece of the weight.  Threads run along whichever
+// dimension is the denser one.
+__global__ void __launch_bounds__(256) head_weight_top_kernel(const __grid_constant__ PlanesDev a, int along_v) {
+  __shared__ uint32_t sm[8];
+  const HeadDev& d = a.d;
+  const float* w = d.w + (int64_t)a.v0 * d.wv;
+  uint32_t top = 0;
+  if (along_v) {
+    for (int c = blockIdx.x; c < d.D; c += gridDim.x)
+      for (int v = threadIdx.x; v < a.n; v += 256) top = max(top, magnitude(w[v * d.wv + c * d.wd]));
+  } else {
+    for (int v = blockIdx.x; v < a.n; v += gridDim.x)
+      for (int c = threadIdx.x * 4; c < d.D; c += 1024) {
+        const float4 x = piece4(w + v * d.wv, c, d.D, d.wd, d.vec_w);
+        top = max(max(top, max(magnitude(x.x), magnitude(x.y))), max(magnitude(x.z), magnitude(x.w)));
+      }
+  }
+  top = block_top(top, sm);
+  if (threadIdx.x == 0) atomicMax(a.top, top);
+}
+
+// A piece of the weight: a CTA per row, or, where tokens are the dense dimension,
+// 32 x 32 tiles through shared memory.
+__global__ void __launch_bounds__(256) head_pack_weight_kernel(const __grid_constant__ PlanesDev a, int along_v) {
+  __shared__ float tile[32][33];
+  const HeadDev& d = a.d;
+  float up, down;
+  plane_scale(*a.top, &up, &down);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.down = down;
+  const float* w = d.w + (int64_t)a.v0 * d.wv;
+  if (!along_v) {
+    for (int v = blockIdx.x; v < a.n; v += gridDim.x)
+      for (int c = threadIdx.x * 4; c < a.Dp; c += 1024) {
+        const float4 x = piece4(w + v * d.wv, c, d.D, d.wd, d.vec_w);
+        split_store(a.to + (int64_t)v * a.Dp + c, a.plane, x.x * up, x.y * up, x.z * up, x.w * up);
+      }
+    return;
+  }
+  const int tv = (a.n + 31) / 32, tc = a.Dp / 32;
+  for (int64_t t = blockIdx.x; t < (int64_t)tv * tc; t += gridDim.x) {
+    const int v0 = (int)(t % tv) * 32, c0 = (int)(t / tv) * 32;
+    __syncthreads();
+    for (int i = threadIdx.x / 32; i < 32; i += 8) {
+      const int v = v0 + threadIdx.x % 32, c = c0 + i;
+      tile[i][threadIdx.x % 32] = v < a.n && c < d.D ? w[v * d.wv + c * d.wd] : 0.f;
+    }
+    __syncthreads();
+    const int v = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
+    if (v0 + v < a.n)
+      split_store(a.to + (int64_t)(v0 + v) * a.Dp + c0 + c, a.plane, tile[c][v] * up, tile[c + 1][v] * up,
+                  tile[c + 2][v] * up, tile[c + 3][v] * up);
+  }
+}
+
+// ---- pieces of the pair's plumbing ---------------------------------------------------
+
+constexpr int CG = 2;                        // CTAs of a pair
+constexpr int BM = 128 * CG, BN = 256;       // a tile of the pair
+constexpr int BR = BN / CG;                  // B's rows in each CTA
+constexpr int kSlab = 64;                    // elements of the contraction per stage
+constexpr int kABytes = 2 * 128 * 128, kBBytes = 2 * BR * 128;
+constexpr int kStage = kABytes + kBBytes;
+constexpr int kStages = 3;
+constexpr int kChunk = 4;                    // slabs per accumulator
+constexpr int kGemmThreads = 384;
+constexpr int kGemmSmem = kStages * kStage + 1024 + 256;
+constexpr int kLean = 56, kFull = 224;       // 128 * 56 + 256 * 224 = 384 * 168 registers
+static_assert(128 * kLean + 256 * kFull == kGemmThreads * 168, "all of the registers");
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address, in the pair's shared memory, of `p` of CTA `rank`
+__device__ __forceinline__ uint32_t pair_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void pair_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D (+)= A B of the pair, issued by the lane of the first CTA with lead != 0.
+__device__ __forceinline__ void pair_mma(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kSw128High), "r"(lead)
+      : "memory");
+}
+// Arrives on `bar` of both CTAs once the MMAs issued before have completed.
+__device__ __forceinline__ void pair_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(lead), "h"((uint16_t)3)
+      : "memory");
+}
+// Loads into this CTA's shared memory that complete on a barrier of the pair's
+// first CTA.
+__device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void pair_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+      "%5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
+// Waits for a phase, bounded, or until some role of the CTA has given up.
+__device__ __forceinline__ bool wait_or_fail(uint64_t* bar, uint32_t parity, int* failed) {
+  for (uint32_t i = 0; i < kWaitIters; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 63 && *(volatile int*)failed) return false;
+  }
+  atomicExch(failed, 1);
+  return false;
+}
+
+// ---- the matrix products --------------------------------------------------------------
+
+enum HeadMode { kScores, kScoreGrad, kProducts };
+
+struct GemmDev {
+  HeadDev d;
+  int v0, Vc, Vcp;       // the piece of the vocabulary, rounded up to whole tiles
+  const float* hdown;    // 2^e of the hidden rows, the piece, g h
+  const float* wdown;
+  const float* gdown;
+  HeadPart* part;        // kScores: [column half tile][ld]
+  __half* dx;            // kScoreGrad: [2][Np][ld]
+  int64_t ld, plane;
+  // kProducts
+  int dtiles;            // tiles along the width
+  int splits;            // parts of dh's contraction
+  int slabs;             // slabs of a part
+  int dh_first;
+  float* dh_part;        // [split][Np][dtiles * 256] where splits > 1
+  int add;               // dh collects an earlier piece
+  int* err;
+};
+
+// A tile: rows from m0, columns from n0, `n` slabs of the contraction from k0.
+struct GemmItem {
+  int m0, n0, k0, n, split;
+  bool dw;
+};
+
+template <int MODE>
+__device__ __forceinline__ int gemm_items(const GemmDev& g, int live) {
+  const int mt = (live + BM - 1) / BM, vt = g.Vcp / BN;
+  if (MODE != kProducts) return mt * vt;
+  return (g.d.dh.p ? mt * g.dtiles * g.splits : 0) + (g.d.dw ? vt * g.dtiles : 0);
+}
+
+template <int MODE>
+__device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int item) {
+  const int mt = (live + BM - 1) / BM, vt = g.Vcp / BN;
+  GemmItem w;
+  w.k0 = 0;
+  w.split = 0;
+  w.dw = false;
+  auto place = [&](int i, int rows, int cols) {  // groups of 8 row tiles, their columns in order
+    const int group = i / (8 * cols), first = group * 8, high = min(8, rows - first);
+    const int at = i - group * 8 * cols;
+    w.m0 = (first + at % high) * BM;
+    w.n0 = at / high * BN;
+  };
+  if (MODE != kProducts) {
+    place(item, mt, vt);
+    w.n = (g.d.D + kSlab - 1) / kSlab;
+    return w;
+  }
+  const int nh = g.d.dh.p ? mt * g.dtiles * g.splits : 0, nw = g.d.dw ? vt * g.dtiles : 0;
+  bool dh = g.dh_first ? item < nh : item >= nw;
+  const int i = dh ? item - (g.dh_first ? 0 : nw) : item - (g.dh_first ? nh : 0);
+  if (dh) {
+    const int tiles = mt * g.dtiles;
+    w.split = i / tiles;
+    place(i % tiles, mt, g.dtiles);
+    const int all = (g.Vc + kSlab - 1) / kSlab;
+    w.k0 = min(all, w.split * g.slabs);
+    w.n = min(all, w.k0 + g.slabs) - w.k0;
+  } else {
+    place(i, vt, g.dtiles);
+    w.dw = true;
+    w.n = (live + kSlab - 1) / kSlab;
+  }
+  return w;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pk(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void upk(uint64_t x, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(x));
+}
+__device__ __forceinline__ void store8(void* to, const uint32_t (&x)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+               "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+               : "memory");
+}
+
+// The finished tile's 128 columns of this thread's row.
+template <int MODE>
+__device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w, int live, int row, int col, int orig,
+                                            Entries& ent, float f, float lse2, float (&acc)[128]) {
+  const HeadDev& d = g.d;
+  if (MODE == kScores) {
+    const int limit = g.Vc - col;
+    if (limit < 128) {
+#pragma unroll
+      for (int i = 0; i < 128; ++i)
+        if (i >= limit) acc[i] = -INFINITY;
+    }
+    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 128; i += 2) mx4[i / 2 % 4] = fmaxf(fmaxf(mx4[i / 2 % 4], acc[i]), acc[i + 1]);
+    HeadPart p;
+    p.m = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * f;
+    const float base = p.m == -INFINITY ? 0.f : -p.m;
+    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 128; ++i) s4[i % 4] += head_ex2(__fmaf_rn(acc[i], f, base));
+    p.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    p.dot = 0.f;
+    const int end = g.v0 + col + (limit < 128 ? limit : 128);
+    while (__any_sync(0xffffffffu, ent.next < end)) {
+      if (ent.next < end) {
+        const int k = ent.next - g.v0 - col;
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) x = i == k ? acc[i] : x;
+        if (*ent.w != 0.f) p.dot = __fmaf_rn(*ent.w, x * f, p.dot);
+        ent.step();
+      }
+    }
+    p.sum = 0.f;
+    if (d.share != 0.f) {
+      float t4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 128; ++i)
+        if (i < limit) t4[i % 4] += acc[i];
+      p.sum = ((t4[0] + t4[1]) + (t4[2] + t4[3])) * f;
+    }
+    if (row < live) *reinterpret_cast<float4*>(&g.part[(int64_t)((g.v0 + col) / 128) * g.ld + row]) =
+        make_float4(p.m, p.s, p.dot, p.sum);
+  } else if (MODE == kScoreGrad) {
+    const int limit = row < live ? g.Vc - col : 0;
+#pragma unroll
+    for (int i = 0; i < 128; ++i) acc[i] = head_ex2(__fmaf_rn(acc[i], f, -lse2)) - d.share;
+    const int end = g.v0 + col + (limit < 128 ? limit : 128);
+    while (__any_sync(0xffffffffu, ent.next < end)) {
+      if (ent.next < end) {
+        const int k = ent.next - g.v0 - col;
+        const float t = *ent.w;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] -= i == k ? t : 0.f;
+        ent.step();
+      }
+    }
+    __half* to = g.dx + (int64_t)row * g.ld + col;
+#pragma unroll
+    for (int i = 0; i < 128; i += 16) {
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = i + 2 * j < limit ? acc[i + 2 * j] * 0x1p15f : 0.f;
+        const float b = i + 2 * j + 1 < limit ? acc[i + 2 * j + 1] * 0x1p15f : 0.f;
+        const __half2 h = __floats2half2_rn(a, b);
+        const float2 back = __half22float2(h);
+        const __half2 l = __floats2half2_rn(a - back.x, b - back.y);
+        hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+      }
+      store8(to + i, hi);
+      store8(to + g.plane + i, lo);
+    }
+  } else {
+    float* to;
+    int64_t sd;
+    bool vec, add = false;
+    float f1, f2 = 1.f;
+    int width = d.D - col;
+    if (w.dw) {
+      if (row >= g.Vc) return;
+      to = d.dw + (int64_t)(g.v0 + row) * d.dwv;
+      sd = d.dwd;
+      vec = d.vec_dw;
+      f1 = *g.gdown * 0x1p-15f;
+    } else {
+      if (row >= live) return;
+      f1 = *g.wdown * 0x1p-15f;
+      f2 = *head_row<const float>(d, d.gl, orig) * d.temp;
+      if (g.splits > 1) {
+        const int64_t np = (live + BM - 1) / BM * BM;
+        to = g.dh_part + (w.split * np + row) * ((int64_t)g.dtiles * BN);
+        sd = 1;
+        vec = true;
+        width = 128;
+      } else {
+        to = head_row<float>(d, d.dh, orig);
+        sd = d.dh.sd;
+        vec = d.vec_dh;
+        add = g.add;
+      }
+    }
+    if (vec) {
+      float4* p = reinterpret_cast<float4*>(to + col);
+#pragma unroll
+      for (int i = 0; i < 128; i += 4) {
+        if (i >= width) continue;
+        float4 x = make_float4(acc[i] * f1 * f2, acc[i + 1] * f1 * f2, acc[i + 2] * f1 * f2, acc[i + 3] * f1 * f2);
+        if (add) {
+          const float4 b = p[i / 4];
+          x.x += b.x, x.y += b.y, x.z += b.z, x.w += b.w;
+        }
+        p[i / 4] = x;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 128; ++i) {
+        if (i >= width) continue;
+        float* e = to + (int64_t)(col + i) * sd;
+        const float x = acc[i] * f1 * f2;
+        *e = add ? *e + x : x;
+      }
+    }
+  }
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
+head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
+                 const __grid_constant__ CUtensorMap ma2, const __grid_constant__ CUtensorMap mb2,
+                 const __grid_constant__ GemmDev g) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStage);  // of the first CTA: both CTAs' slabs are there
+  uint64_t* empty = full + kStages;   // of each CTA: the pair's MMAs have read the stage
+  uint64_t* tfull = empty + kStages;  // [2] of each CTA: an accumulator is complete
+  uint64_t* tempty = tfull + 2;       // [2] of the first CTA: both CTAs' warps have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cta_rank();
+  const int live = *g.d.live;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], CG * 8);
+    }
+    *failed = 0;
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (warp == 0) pair_tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  pair_sync();  // the other CTA's barriers are there before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int items = gemm_items<MODE>(g, live), pairs = gridDim.x / CG, pair = blockIdx.x / CG;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLean));
+    if (warp == 9 && lane == 0) {  // TMA
+      int li = 0;
+      bool ok = true;
+      for (int item = pair; item < items && ok; item += pairs) {
+        const GemmItem w = gemm_item<MODE>(g, live, item);
+        for (int i = 0; i < w.n; ++i, ++li) {
+          const int s = li % kStages;
+          if (li >= kStages && !(ok = wait_or_fail(&empty[s], (uint32_t)(li / kStages - 1) & 1u, failed))) break;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * kStage);
+          const uint32_t bar = pair_addr(&full[s], 0);
+          unsigned char* a = smem + s * kStage;
+          const int k = (w.k0 + i) * kSlab, m = w.m0 + rank * 128, n = w.n0 + rank * BR;
+          if (MODE != kProducts) {
+            pair_load_3d(a, &ma, k, m, 0, bar);
+            pair_load_3d(a + kABytes, &mb, k, n, 0, bar);
+          } else if (w.dw) {
+            pair_load_4d(a, &ma2, 0, k, m / 64, 0, bar);
+            pair_load_4d(a + kABytes, &mb2, 0, k, n / 64, 0, bar);
+          } else {
+            pair_load_3d(a, &ma, k, m, 0, bar);
+            pair_load_4d(a + kABytes, &mb, 0, k, n / 64, 0, bar);
+          }
+        }
+      }
+      // every copy has landed and been read, and the arrival that says so has come,
+      // before the CTA ends; after a failure, which tells nothing about the other
+      // CTA's copies, they are given time
+      for (int s = 0; s < kStages && s < li && ok; ++s)
+        ok = wait_or_fail(&empty[s], (uint32_t)((li - 1 - s) / kStages) & 1u, failed);
+      if (!ok)
+        for (int i = 0; i < 100; ++i) __nanosleep(100000);
+    } else if (warp == 8 && rank == 0) {  // MMA: the warp stays whole, one lane issues
+      const uint32_t lead = elect_lane(), tm = uniform(tmem);
+      auto wait_all = [&](uint64_t* bar, uint32_t phase) {
+        return __all_sync(0xffffffffu, wait_or_fail(bar, phase & 1u, failed)) != 0;
+      };
+      int li = 0, ci = 0;
+      bool ok = true;
+      for (int item = pair; item < items && ok; item += pairs) {
+        const GemmItem w = gemm_item<MODE>(g, live, item);
+        const bool amn = MODE == kProducts && w.dw, bmn = MODE == kProducts;
+        const uint32_t idesc = uniform((1u << 4) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u) |
+                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24));
+        const uint32_t astep = amn ? 128u : 2u, bstep = bmn ? 128u : 2u;
+        const uint32_t da0 = uniform(sw128_low(smem, amn ? 64 * 128 : 16));
+        const uint32_t db0 = uniform(sw128_low(smem + kABytes, bmn ? 64 * 128 : 16));
+        for (int i = 0; i < w.n && ok; ++i, ++li) {
+          const int s = li % kStages;
+          if (i % kChunk == 0 && ci >= 2 && !(ok = wait_all(&tempty[ci & 1], (uint32_t)(ci / 2 - 1)))) break;
+          if (!(ok = wait_all(&full[s], (uint32_t)(li / kStages)))) break;
+          tc_fence_after();
+          const uint32_t dst = tm + (ci & 1) * BN;
+          const uint32_t a = da0 + s * (kStage / 16), b = db0 + s * (kStage / 16);
+          constexpr uint32_t ALO = 128 * 128 / 16, BLO = BR * 128 / 16;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            pair_mma(lead, dst, a + ALO + k * astep, b + k * bstep, idesc, i % kChunk != 0 || k > 0);
+            pair_mma(lead, dst, a + k * astep, b + BLO + k * bstep, idesc, 1);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) pair_mma(lead, dst, a + k * astep, b + k * bstep, idesc, 1);
+          pair_commit(lead, &empty[s]);
+          if (i % kChunk == kChunk - 1 || i + 1 == w.n) {
+            pair_commit(lead, &tfull[ci & 1]);
+            ++ci;
+          }
+        }
+      }
+      // all MMAs are complete before the pair's shared memory and tensor memory go
+      if (ci > 0) wait_all(&tfull[(ci - 1) & 1], (uint32_t)((ci - 1) / 2));
+    }
+  } else {  // results: a row per thread, 128 columns per warpgroup
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFull));
+    const int half = warp / 4, rl = (warp % 4) * 32 + lane;
+    const uint32_t src = tmem + ((uint32_t)((warp % 4) * 32) << 16) + half * 128;
+    const uint32_t bars[2] = {pair_addr(&tempty[0], 0), pair_addr(&tempty[1], 0)};
+    int ci = 0;
+    bool ok = true;
+    for (int item = pair; item < items && ok; item += pairs) {
+      const GemmItem w = gemm_item<MODE>(g, live, item);
+      const int row = w.m0 + (int)rank * 128 + rl, col = w.n0 + half * 128;
+      Entries ent;
+      ent.next = kNoToken;
+      float f = 0.f, lse2 = 0.f;
+      int orig = 0;
+      if (!w.dw && row < live) {
+        orig = g.d.rows[row];
+        if (MODE != kProducts) {
+          // a power of two and the factor onto units of log2: neither 0 nor inf
+          f = fminf(fmaxf(mul3(g.hdown[row], *g.wdown, g.d.inv_temp * kHeadLog2e), 0x1p-126f), FLT_MAX);
+          ent.seek(g.d, orig, g.v0 + col);
+          if (MODE == kScoreGrad) lse2 = *head_row<const float>(g.d, g.d.lse, orig) * kHeadLog2e;
+        }
+      }
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      for (int i = 0; i < w.n; i += kChunk, ++ci) {
+        ok = __all_sync(0xffffffffu, wait_or_fail(&tfull[ci & 1], (uint32_t)(ci / 2) & 1u, failed)) != 0;
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t x[32];
+          tmem_ld32_issue(src + (ci & 1) * BN + cc * 32, x);
+          tmem_ld_done(x);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const uint64_t y = add2(pk(acc[cc * 32 + j], acc[cc * 32 + j + 1]),
+                                    pk(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+            upk(y, &acc[cc * 32 + j], &acc[cc * 32 + j + 1]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) pair_arrive(bars[ci & 1]);
+      }
+      if (ok) finish_tile<MODE>(g, w, live, row, col, orig, ent, f, lse2, acc);
+    }
+  }
+  if (threadIdx.x % 32 == 0 && *(volatile int*)failed) atomicOr(g.err, kAsyncWaitTimeout);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  pair_sync();
+  tc_fence_after();
+  if (warp == 0) pair_tmem_dealloc(tmem, 512);
+}
+
+// dh from the parts of its contraction, in order.
+__global__ void __launch_bounds__(256) head_dh_join_kernel(const __grid_constant__ GemmDev g) {
+  const HeadDev& d = g.d;
+  const int live = *d.live, r = blockIdx.x;
+  if (r >= live) return;
+  const int64_t np = (live + BM - 1) / BM * BM, ld = (int64_t)g.dtiles * BN;
+  float* to = head_row<float>(d, d.dh, d.rows[r]);
+  for (int c = blockIdx.y * 256 + threadIdx.x; c < d.D; c += gridDim.y * 256) {
+    float sum = g.add ? to[c * d.dh.sd] : 0.f;
+    for (int s = 0; s < g.splits; ++s) sum += g.dh_part[(s * np + r) * ld + c];
+    to[c * d.dh.sd] = sum;
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------
+
+Error make_map(const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+               CUtensorMap* map) {
+  Error e;
+  EncodeTiled enc = encode_fn(&e);
+  if (!enc) return e;
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box,
+                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return make_error(TRS_ERR_CUDA, "head: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return Error{};
+}
+
+// Planes [2][rows][pitch] whose contraction runs along the pitch: boxes of 64
+// elements by `high` rows by both planes.
+Error map_rows(const __half* p, int64_t rows, int64_t pitch, int64_t plane, int high, CUtensorMap* map) {
+  const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)rows, 2};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)plane * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)high, 2};
+  return make_map(p, 3, dims, strides, box, map);
+}
+// The same planes with the contraction along the rows: boxes of 64 rows by 128
+// columns, as blocks of 64, by both planes.
+Error map_cols(const __half* p, int64_t rows, int64_t pitch, int64_t plane, CUtensorMap* map) {
+  const cuuint64_t dims[4] = {64, (cuuint64_t)rows, (cuuint64_t)pitch / 64, 2};
+  const cuuint64_t strides[3] = {(cuuint64_t)pitch * 2, 128, (cuuint64_t)plane * 2};
+  const cuuint32_t box[4] = {64, kSlab, 2, 2};
+  return make_map(p, 4, dims, strides, box, map);
+}
+
+int max_pairs(const void* kernel) {
+  static DeviceCache<const void*> cache;
+  const DeviceInfo& info = current_device_info();
+  return cache.get(info.device, kernel, [&] {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(info.sm_count / CG * CG));
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = kGemmSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess) return n;
+    cudaGetLastError();
+    return 0;
+  });
+}
+
+template <int MODE>
+Error launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const GemmDev& g,
+                  int64_t most, cudaStream_t s) {
+  auto k = head_gemm_kernel<MODE>;
+  allow_smem((const void*)k, kGemmSmem);
+  const int64_t pairs = std::min<int64_t>(most, max_pairs((const void*)k));
+  if (pairs < 1) return Error{};
+  k<<<(unsigned)(pairs * CG), kGemmThreads, kGemmSmem, s>>>(a, b, a2, b2, g);
+  return check_launch("head matrix product kernel");
+}
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+constexpr int64_t kPieceBytes = 512ll << 20;  // planes of a piece
+
+}  // namespace
+
+Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
+  const int sms = current_device_info().sm_count;
+  const int64_t Np = round_up(d.N, BM), Dp = round_up(d.D, kSlab), dtiles = (d.D + BN - 1) / BN;
+  // pieces of the vocabulary of one size, whole tiles each
+  const int64_t row_bytes = 4 * Dp + (backward ? 4 * Np : 0);
+  int64_t pieces = std::max<int64_t>(1, (round_up(d.V, BN) * row_bytes + kPieceBytes - 1) / kPieceBytes);
+  const int64_t Vp = round_up((d.V + pieces - 1) / pieces, BN);
+  pieces = (d.V + Vp - 1) / Vp;
+  int* err = async_error_word();
+  if (!err) return make_error(TRS_ERR_CUDA, "head: no async-error word");
+
+  GemmDev g;
+  std::memset(static_cast<void*>(&g), 0, sizeof(g));
+  g.d = d;
+  g.err = err;
+  g.dtiles = (int)dtiles;
+  const int64_t htiles = Np / BM * dtiles, wtiles = Vp / BN * dtiles;
+  g.splits = 1;
+  if (backward && d.dh.p) {
+    // dh's few tiles with a long contraction: parts of about the average work of a pair, 8 slabs at least
+    const int64_t work = htiles * Vp + (d.dw ? wtiles * Np : 0);
+    const int64_t part = std::max<int64_t>(512, work / std::max(1, sms / CG));
+    g.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Vp + part / 2) / part));
+  }
+  g.slabs = (int)((Vp / kSlab + g.splits - 1) / g.splits);
+  g.dh_first = Vp / g.splits >= d.N;
+
+  // workspaces
+  Scratch mem;
+  const int64_t hplane = Np * Dp, wplane = Vp * Dp, xplane = backward ? Np * Vp : 0;
+  const int64_t parts = Vp * pieces / 128;
+  size_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const size_t here = at;
+    at += (size_t)round_up(bytes, 256);
+    return here;
+  };
+  const size_t o_small = take(4 * (4 + pieces) * 2), o_hdown = take(4 * Np), o_h = take(4 * hplane), o_w = take(4 * wplane);
+  const size_t o_gh = take(backward && d.dw ? 4 * hplane : 0), o_x = take(4 * xplane);
+  const size_t o_part = take(backward ? 0 : (int64_t)sizeof(HeadPart) * parts * Np);
+  const size_t o_dh = take(g.splits > 1 ? 4 * g.splits * Np * dtiles * BN : 0);
+  Error e = mem.alloc(at, s);
+  if (!e.ok()) return e;
+  char* base = mem.as<char>();
+  // largest magnitudes: of g h, then of every piece; their powers of two likewise
+  uint32_t* tops = reinterpret_cast<uint32_t*>(base + o_small);
+  float* downs = reinterpret_cast<float*>(tops + 4 + pieces);
+  cudaError_t ce = cudaMemsetAsync(tops, 0, 4 * (4 + pieces), s);
+  if (ce != cudaSuccess) return cuda_error(ce, "head clear");
+  __half *hp = reinterpret_cast<__half*>(base + o_h), *wp = reinterpret_cast<__half*>(base + o_w);
+  __half *gp = reinterpret_cast<__half*>(base + o_gh), *xp = reinterpret_cast<__half*>(base + o_x);
+
+  PlanesDev p;
+  std::memset(static_cast<void*>(&p), 0, sizeof(p));
+  p.d = d;
+  p.Dp = (int)Dp;
+  p.to = hp;
+  p.plane = hplane;
+  p.down = reinterpret_cast<float*>(base + o_hdown);
+  p.top = backward && d.dw ? tops : nullptr;
+  head_pack_hidden_kernel<<<(unsigned)Np, 256, 0, s>>>(p);
+  e = check_launch("head hidden planes kernel");
+  if (e.ok() && p.top) {
+    p.to = gp;
+    p.down = downs;
+    head_pack_grad_kernel<<<(unsigned)Np, 256, 0, s>>>(p);
+    e = check_launch("head gradient planes kernel");
+  }
+  if (!e.ok()) return e;
+
+  g.hdown = reinterpret_cast<float*>(base + o_hdown);
+  g.gdown = downs;
+  g.part = reinterpret_cast<HeadPart*>(base + o_part);
+  g.ld = backward ? Vp : Np;
+  g.dx = xp;
+  g.plane = xplane;
+  g.dh_part = reinterpret_cast<float*>(base + o_dh);
+  g.Vcp = (int)Vp;
+  const int64_t av = d.wv < 0 ? -d.wv : d.wv, ad = d.wd < 0 ? -d.wd : d.wd;
+  const int along_v = d.V > 1 && d.D > 1 && av < ad;
+  for (int64_t i = 0; i < pieces; ++i) {
+    g.v0 = (int)(i * Vp);
+    g.Vc = (int)std::min<int64_t>(Vp, d.V - i * Vp);
+    g.Vcp = (int)round_up(g.Vc, BN);
+    g.wdown = downs + 4 + i;
+    g.add = i > 0;
+    p.to = wp;
+    p.plane = wplane;
+    p.top = tops + 4 + i;
+    p.down = downs + 4 + i;
+    p.v0 = g.v0;
+    p.n = g.Vc;
+    const unsigned ctas = (unsigned)(along_v ? 8 * sms : std::min<int64_t>(g.Vc, 16 * sms));
+    head_weight_top_kernel<<<ctas, 256, 0, s>>>(p, along_v);
+    e = check_launch("head weight maximum kernel");
+    if (!e.ok()) return e;
+    head_pack_weight_kernel<<<ctas, 256, 0, s>>>(p, along_v);
+    e = check_launch("head weight planes kernel");
+    CUtensorMap ha, wb, xa, wc, xc, gc;
+    if (e.ok()) e = map_rows(hp, Np, Dp, hplane, 128, &ha);
+    if (e.ok()) e = map_rows(wp, g.Vc, Dp, wplane, BR, &wb);
+    if (!e.ok()) return e;
+    const int64_t tiles = Np / BM * (g.Vcp / BN);
+    if (!backward) {
+      e = launch_gemm<kScores>(ha, wb, ha, wb, g, tiles, s);
+      if (!e.ok()) return e;
+      continue;
+    }
+    e = launch_gemm<kScoreGrad>(ha, wb, ha, wb, g, tiles, s);
+    if (e.ok()) e = map_rows(xp, Np, Vp, xplane, 128, &xa);
+    if (e.ok()) e = map_cols(xp, Np, Vp, xplane, &xc);
+    if (e.ok()) e = map_cols(wp, g.Vc, Dp, wplane, &wc);
+    gc = wc;
+    if (e.ok() && d.dw) e = map_cols(gp, Np, Dp, hplane, &gc);
+    if (e.ok()) e = launch_gemm<kProducts>(xa, wc, xc, gc, g, htiles * g.splits + wtiles, s);
+    if (e.ok() && d.dh.p && g.splits > 1) {
+      head_dh_join_kernel<<<dim3((unsigned)d.N, (unsigned)std::min<int64_t>(16, (d.D + 255) / 256)), 256, 0, s>>>(g);
+      e = check_launch("head hidden gradient join kernel");
+    }
+    if (!e.ok()) return e;
+  }
+  if (backward) return e;
+  return head_join(d, g.part, (int)((d.V + 127) / 128), Np, 1, false, s);
+}
+
+}  // namespace trs
