@@ -44,14 +44,15 @@ __device__ __forceinline__ int head_id(const HeadDev& d, const RowsDev& ids, int
 }
 
 // A warp per row: the softmax of the entries that are there, sorted by token
-// (the rank of an entry is counted: K is small, and equal tokens keep their order).
+// (the rank of an entry is counted: K is small).
 __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
   extern __shared__ int s_id[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int row = blockIdx.x * 8 + warp;
   pdl_launch_dependents();
   if (row >= d.N) return;
-  int* ids = s_id + warp * d.K;
+  int* ids = s_id + warp * 2 * d.K;
+  float* ps = reinterpret_cast<float*>(ids + d.K);
   const float* z = head_row<const float>(d, d.z, row);
   float top = -INFINITY;
   for (int k = lane; k < d.K; k += 32) {
@@ -59,30 +60,43 @@ __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
     int id = head_id(d, d.ids, row, k);
     if (x == -INFINITY) id = kNoToken;
     ids[k] = id;
+    ps[k] = x;
     if (id != kNoToken) top = fmaxf(top, x);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  __syncwarp();
   float sum = 0.f;
   for (int k = lane; k < d.K; k += 32)
-    if (ids[k] != kNoToken) sum += expf(__fdiv_rn(z[k * d.z.sd] - top, d.temp));
+    if (ids[k] != kNoToken) sum += expf(__fdiv_rn(ps[k] - top, d.temp));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const float ln_sum = logf(sum);
   double ent = 0.0;
   for (int k = lane; k < d.K; k += 32) {
-    const int id = ids[k];
     float p = 0.f;
-    if (id != kNoToken) {
-      const float a = __fdiv_rn(z[k * d.z.sd] - top, d.temp);
+    if (ids[k] != kNoToken) {
+      const float a = __fdiv_rn(ps[k] - top, d.temp);
       p = __fdiv_rn(expf(a), sum);
       ent += (double)p * (double)(a - ln_sum);
     }
+    ps[k] = p;
+  }
+  __syncwarp();
+  for (int k = lane; k < d.K; k += 32) {
+    const int id = ids[k];
     int rank = 0;
-    for (int j = 0; j < d.K; ++j) rank += ids[j] < id || (ids[j] == id && j < k);
+    bool first = true;
+    float p = 0.f;
+    for (int j = 0; j < d.K; ++j) {
+      const int other = ids[j];
+      rank += other < id || (other == id && j < k);
+      if (other == id) {
+        first = first && j >= k;
+        p += ps[j];
+      }
+    }
     d.eid[(int64_t)row * d.K + rank] = id;
-    d.ew[(int64_t)row * d.K + rank] = p;
+    d.ew[(int64_t)row * d.K + rank] = first ? p : 0.f;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ent += __shfl_xor_sync(0xffffffffu, ent, o);
@@ -206,7 +220,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadDev d, const H
 Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
                 cudaStream_t stream) {
   if (few) return launch_after(head_join_kernel<1>, dim3((unsigned)d.N), 256, 0, stream, "head join kernel", d, part, parts, sp, sr);
-  return launch_after(head_join_kernel<32>, dim3((unsigned)((d.N + 31) / 32)), 256, 0, stream, "head join kernel", d, part,
+  return launch_after(head_join_kernel<8>, dim3((unsigned)((d.N + 7) / 8)), 256, 0, stream, "head join kernel", d, part,
                       parts, sp, sr);
 }
 
@@ -613,10 +627,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
       d.vec_dw = rows_vectors(c.grad_weight);
     }
   }
-  if (N > 0) {
-    d.vec_h = rows_vectors(c.hidden);
-    d.vec_dh = c.grad_hidden && rows_vectors(c.grad_hidden);
-  }
+  d.vec_h = N > 0 && rows_vectors(c.hidden);
   if (N == 0 && !d.dw) return Error{};
   // the rows' targets
   Scratch mem;
@@ -629,7 +640,8 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   d.ew = reinterpret_cast<float*>(d.eid + nk);
   d.ent = d.ew + nk;
   if (c.distill && N > 0) {
-    const int smem = 8 * d.K * 4;
+    const int smem = 8 * 2 * d.K * 4;
+    allow_smem((const void*)head_teacher_kernel, smem);
     head_teacher_kernel<<<(unsigned)((N + 7) / 8), 256, smem, stream>>>(d);
     e = check_launch("head teacher kernel");
     if (!e.ok()) return e;

@@ -6,8 +6,8 @@
 // against a target distribution t, up to a constant of the row and the factor
 // temperature^2; t is a few entries (one for a class, K for a teacher's logits)
 // and, for smoothed classes, s / V everywhere.  The gradient of x is softmax(x) - t.
-// A row's entries are prepared once per call, sorted by their token, so that a
-// thread that walks the vocabulary in order meets them in order.
+// A row's entries are prepared once per call, sorted by their token; where a token
+// comes several times, its first entry has all of its weight and the others 0.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -44,7 +44,7 @@ struct HeadDev {
   int* eid;                      // [N][K] tokens of a row's entries, ascending, kNoToken behind them
   float* ew;                     // [N][K] their weights
   float* ent;                    // [N] sum of w ln w (distillation)
-  int vec_h, vec_w, vec_dh, vec_dw;  // 16-byte accesses along D
+  int vec_h, vec_w, vec_dw;  // 16-byte accesses along D
 };
 
 __device__ __forceinline__ float head_ex2(float x) {
@@ -76,20 +76,7 @@ struct Entries {
     ++id;
     next = --left > 0 ? *id : kNoToken;
   }
-  // the first entry not below v
-  __device__ __forceinline__ void seek(const HeadDev& d, int row, int v) {
-    const int* all = d.eid + (int64_t)row * d.K;
-    int lo = 0, hi = d.K;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (all[mid] < v) lo = mid + 1; else hi = mid;
-    }
-    id = all + lo;
-    w = d.ew + (int64_t)row * d.K + lo;
-    left = d.K - lo;
-    next = left > 0 ? *id : kNoToken;
-  }
-  // skips entries below v (a binary search is not worth it for a step of a tile)
+  // skips entries below v
   __device__ __forceinline__ void skip_to(int v) {
     while (next < v) step();
   }

@@ -107,6 +107,8 @@ __device__ __forceinline__ void split_store(__half* to, int64_t plane, float a, 
 // to a whole tile.  With a gradient also the largest |g temperature h|.
 __global__ void __launch_bounds__(256) head_pack_hidden_kernel(const __grid_constant__ PlanesDev a) {
   __shared__ uint32_t sm[8];
+  pdl_launch_dependents();
+  pdl_wait();
   const HeadDev& d = a.d;
   const int live = *d.live, r = blockIdx.x;
   if (r >= (live + 255) / 256 * 256) return;
@@ -136,6 +138,8 @@ __global__ void __launch_bounds__(256) head_pack_hidden_kernel(const __grid_cons
 
 // g temperature h of the same rows, under one power of two.
 __global__ void __launch_bounds__(256) head_pack_grad_kernel(const __grid_constant__ PlanesDev a) {
+  pdl_launch_dependents();
+  pdl_wait();
   const HeadDev& d = a.d;
   const int live = *d.live, r = blockIdx.x;
   float up, down;
@@ -156,6 +160,8 @@ __global__ void __launch_bounds__(256) head_pack_grad_kernel(const __grid_consta
 // dimension is the denser one.
 __global__ void __launch_bounds__(256) head_weight_top_kernel(const __grid_constant__ PlanesDev a, int along_v) {
   __shared__ uint32_t sm[8];
+  pdl_launch_dependents();
+  pdl_wait();
   const HeadDev& d = a.d;
   const float* w = d.w + (int64_t)a.v0 * d.wv;
   uint32_t top = 0;
@@ -163,30 +169,45 @@ __global__ void __launch_bounds__(256) head_weight_top_kernel(const __grid_const
     for (int c = blockIdx.x; c < d.D; c += gridDim.x)
       for (int v = threadIdx.x; v < a.n; v += 256) top = max(top, magnitude(w[v * d.wv + c * d.wd]));
   } else {
-    for (int v = blockIdx.x; v < a.n; v += gridDim.x)
-      for (int c = threadIdx.x * 4; c < d.D; c += 1024) {
-        const float4 x = piece4(w + v * d.wv, c, d.D, d.wd, d.vec_w);
-        top = max(max(top, max(magnitude(x.x), magnitude(x.y))), max(magnitude(x.z), magnitude(x.w)));
+    // a warp per row, four loads in flight per lane
+    const int lane4 = threadIdx.x % 32 * 4;
+    for (int v = blockIdx.x * 8 + threadIdx.x / 32; v < a.n; v += gridDim.x * 8)
+      for (int c = lane4; c < d.D; c += 512) {
+        float4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = piece4(w + v * d.wv, c + 128 * j, d.D, d.wd, d.vec_w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          top = max(max(top, max(magnitude(x[j].x), magnitude(x[j].y))), max(magnitude(x[j].z), magnitude(x[j].w)));
       }
   }
   top = block_top(top, sm);
   if (threadIdx.x == 0) atomicMax(a.top, top);
 }
 
-// A piece of the weight: a CTA per row, or, where tokens are the dense dimension,
+// A piece of the weight: row by row, or, where tokens are the dense dimension,
 // 32 x 32 tiles through shared memory.
 __global__ void __launch_bounds__(256) head_pack_weight_kernel(const __grid_constant__ PlanesDev a, int along_v) {
   __shared__ float tile[32][33];
+  pdl_launch_dependents();
+  pdl_wait();
   const HeadDev& d = a.d;
   float up, down;
   plane_scale(*a.top, &up, &down);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.down = down;
   const float* w = d.w + (int64_t)a.v0 * d.wv;
   if (!along_v) {
-    for (int v = blockIdx.x; v < a.n; v += gridDim.x)
-      for (int c = threadIdx.x * 4; c < a.Dp; c += 1024) {
-        const float4 x = piece4(w + v * d.wv, c, d.D, d.wd, d.vec_w);
-        split_store(a.to + (int64_t)v * a.Dp + c, a.plane, x.x * up, x.y * up, x.z * up, x.w * up);
+    // a warp per row, four loads in flight per lane
+    const int lane4 = threadIdx.x % 32 * 4;
+    for (int v = blockIdx.x * 8 + threadIdx.x / 32; v < a.n; v += gridDim.x * 8)
+      for (int c = lane4; c < a.Dp; c += 512) {
+        float4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = piece4(w + v * d.wv, c + 128 * j, d.D, d.wd, d.vec_w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + 128 * j < a.Dp)
+            split_store(a.to + (int64_t)v * a.Dp + c + 128 * j, a.plane, x[j].x * up, x[j].y * up, x[j].z * up, x[j].w * up);
       }
     return;
   }
@@ -217,7 +238,9 @@ constexpr int kStage = kABytes + kBBytes;
 constexpr int kStages = 3;
 constexpr int kChunk = 4;                    // slabs per accumulator
 constexpr int kGemmThreads = 384;
-constexpr int kGemmSmem = kStages * kStage + 1024 + 256;
+constexpr int kPitch = 17;                   // a warp's buffer: 32 rows of 16 columns
+constexpr int kWarpBuf = 32 * kPitch * 4;
+constexpr int kGemmSmem = kStages * kStage + 8 * kWarpBuf + 1024 + 256;
 constexpr int kLean = 56, kFull = 224;       // 128 * 56 + 256 * 224 = 384 * 168 registers
 static_assert(128 * kLean + 256 * kFull == kGemmThreads * 168, "all of the registers");
 
@@ -315,12 +338,14 @@ struct GemmDev {
   int dh_first;
   float* dh_part;        // [split][Np][dtiles * 256] where splits > 1
   int add;               // dh collects an earlier piece
+  int wide_dw, wide_dh;  // rows take 32-byte stores
   int* err;
 };
 
 // A tile: rows from m0, columns from n0, `n` slabs of the contraction from k0.
 struct GemmItem {
   int m0, n0, k0, n, split;
+  int cols;              // of the tile: 256, or 128 where no more are left
   bool dw;
 };
 
@@ -338,6 +363,7 @@ __device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int it
   w.k0 = 0;
   w.split = 0;
   w.dw = false;
+  w.cols = BN;
   auto place = [&](int i, int rows, int cols) {  // groups of 8 row tiles, their columns in order
     const int group = i / (8 * cols), first = group * 8, high = min(8, rows - first);
     const int at = i - group * 8 * cols;
@@ -364,6 +390,7 @@ __device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int it
     w.dw = true;
     w.n = (live + kSlab - 1) / kSlab;
   }
+  if (g.d.D - w.n0 <= BN / 2) w.cols = BN / 2;
   return w;
 }
 
@@ -386,11 +413,72 @@ __device__ __forceinline__ void store8(void* to, const uint32_t (&x)[8]) {
                : "memory");
 }
 
+// A row's entries inside a tile, rows of the warp one after another, a row's
+// entries 32 at a time: its scores (or, for the gradient, its target weights) meet
+// them in the warp's buffer.  `e`: this thread's row's first entry not below
+// `first`, `id` its token; entries below `end` belong to the tile.
+template <bool GRAD>
+__device__ __forceinline__ float tile_entries(const HeadDev& d, float* buf, int lane, int orig, int e, int id, int first,
+                                              int end, float (&acc)[128]) {
+  float dot = 0.f;
+  uint32_t hits = __ballot_sync(0xffffffffu, id < end);
+  while (hits) {
+    const int r = __ffs(hits) - 1;
+    hits &= hits - 1;
+    const int64_t row = (int64_t)__shfl_sync(0xffffffffu, orig, r) * d.K;
+    const int e0 = __shfl_sync(0xffffffffu, e, r);
+    float4* b4 = reinterpret_cast<float4*>(buf);
+    if (GRAD) {
+      b4[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else if (lane == r) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) b4[i] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+    }
+    __syncwarp();
+    float sum = 0.f;
+    for (int at = e0 + lane;; at += 32) {
+      const int v = at < d.K ? d.eid[row + at] : kNoToken;
+      if (v < end) {
+        const float t = d.ew[row + at];
+        // of a token that comes twice, all but the first add 0: any order gives one result
+        if (GRAD) atomicAdd(&buf[v - first], t);
+        else if (t != 0.f) sum = __fmaf_rn(t, buf[v - first], sum);
+      }
+      if (!__all_sync(0xffffffffu, v < end)) break;
+    }
+    __syncwarp();
+    if (GRAD) {
+      if (lane == r) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float4 t = b4[i];
+          acc[4 * i] -= t.x, acc[4 * i + 1] -= t.y, acc[4 * i + 2] -= t.z, acc[4 * i + 3] -= t.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == r) dot = sum;
+    }
+    __syncwarp();
+  }
+  return dot;
+}
+
+// What a thread of the results' warpgroups knows of its row of a tile.
+struct TileRow {
+  int row, col;          // the tile's row and first column of this thread
+  int orig;              // the token of the row
+  int e, id;             // its first entry not below the column, and that entry's token
+  float f, lse2;
+};
+
 // The finished tile's 128 columns of this thread's row.
 template <int MODE>
-__device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w, int live, int row, int col, int orig,
-                                            Entries& ent, float f, float lse2, float (&acc)[128]) {
+__device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w, int live, const TileRow& t, float* buf,
+                                            int lane, float (&acc)[128]) {
   const HeadDev& d = g.d;
+  const int row = t.row, col = t.col;
   if (MODE == kScores) {
     const int limit = g.Vc - col;
     if (limit < 128) {
@@ -402,48 +490,28 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
 #pragma unroll
     for (int i = 0; i < 128; i += 2) mx4[i / 2 % 4] = fmaxf(fmaxf(mx4[i / 2 % 4], acc[i]), acc[i + 1]);
     HeadPart p;
-    p.m = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * f;
+    p.m = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * t.f;
     const float base = p.m == -INFINITY ? 0.f : -p.m;
     float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 128; ++i) s4[i % 4] += head_ex2(__fmaf_rn(acc[i], f, base));
+    for (int i = 0; i < 128; ++i) s4[i % 4] += head_ex2(__fmaf_rn(acc[i], t.f, base));
     p.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-    p.dot = 0.f;
-    const int end = g.v0 + col + (limit < 128 ? limit : 128);
-    while (__any_sync(0xffffffffu, ent.next < end)) {
-      if (ent.next < end) {
-        const int k = ent.next - g.v0 - col;
-        float x = 0.f;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) x = i == k ? acc[i] : x;
-        if (*ent.w != 0.f) p.dot = __fmaf_rn(*ent.w, x * f, p.dot);
-        ent.step();
-      }
-    }
+    p.dot = tile_entries<false>(d, buf, lane, t.orig, t.e, t.id, g.v0 + col, g.v0 + col + min(limit, 128), acc) * t.f;
     p.sum = 0.f;
     if (d.share != 0.f) {
       float t4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < 128; ++i)
         if (i < limit) t4[i % 4] += acc[i];
-      p.sum = ((t4[0] + t4[1]) + (t4[2] + t4[3])) * f;
+      p.sum = ((t4[0] + t4[1]) + (t4[2] + t4[3])) * t.f;
     }
     if (row < live) *reinterpret_cast<float4*>(&g.part[(int64_t)((g.v0 + col) / 128) * g.ld + row]) =
         make_float4(p.m, p.s, p.dot, p.sum);
   } else if (MODE == kScoreGrad) {
     const int limit = row < live ? g.Vc - col : 0;
 #pragma unroll
-    for (int i = 0; i < 128; ++i) acc[i] = head_ex2(__fmaf_rn(acc[i], f, -lse2)) - d.share;
-    const int end = g.v0 + col + (limit < 128 ? limit : 128);
-    while (__any_sync(0xffffffffu, ent.next < end)) {
-      if (ent.next < end) {
-        const int k = ent.next - g.v0 - col;
-        const float t = *ent.w;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) acc[i] -= i == k ? t : 0.f;
-        ent.step();
-      }
-    }
+    for (int i = 0; i < 128; ++i) acc[i] = head_ex2(__fmaf_rn(acc[i], t.f, -t.lse2)) - d.share;
+    tile_entries<true>(d, buf, lane, t.orig, t.e, t.id, g.v0 + col, g.v0 + col + min(g.Vc - col, 128), acc);
     __half* to = g.dx + (int64_t)row * g.ld + col;
 #pragma unroll
     for (int i = 0; i < 128; i += 16) {
@@ -462,53 +530,74 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
       store8(to + g.plane + i, lo);
     }
   } else {
-    float* to;
-    int64_t sd;
-    bool vec, add = false;
+    float* to = nullptr;   // the row's column col
+    int64_t sd = 1;
+    bool wide, add = false;
     float f1, f2 = 1.f;
-    int width = d.D - col;
+    const int width = min(128, d.D - col);
     if (w.dw) {
-      if (row >= g.Vc) return;
-      to = d.dw + (int64_t)(g.v0 + row) * d.dwv;
+      if (row < g.Vc) to = d.dw + (int64_t)(g.v0 + row) * d.dwv + (int64_t)col * d.dwd;
       sd = d.dwd;
-      vec = d.vec_dw;
+      wide = g.wide_dw;
       f1 = *g.gdown * 0x1p-15f;
     } else {
-      if (row >= live) return;
       f1 = *g.wdown * 0x1p-15f;
-      f2 = *head_row<const float>(d, d.gl, orig) * d.temp;
+      sd = d.dh.sd;
+      wide = g.wide_dh;
+      add = g.add;
+      if (row < live) {
+        f2 = *head_row<const float>(d, d.gl, t.orig) * d.temp;
+        to = head_row<float>(d, d.dh, t.orig) + col * sd;
+      }
       if (g.splits > 1) {
         const int64_t np = (live + BM - 1) / BM * BM;
-        to = g.dh_part + (w.split * np + row) * ((int64_t)g.dtiles * BN);
+        if (row < live) to = g.dh_part + (w.split * np + row) * ((int64_t)g.dtiles * BN) + col;
         sd = 1;
-        vec = true;
-        width = 128;
-      } else {
-        to = head_row<float>(d, d.dh, orig);
-        sd = d.dh.sd;
-        vec = d.vec_dh;
-        add = g.add;
+        wide = true;
+        add = false;
       }
     }
-    if (vec) {
-      float4* p = reinterpret_cast<float4*>(to + col);
+    if (width <= 0) return;
+    if (wide) {  // a whole sector per thread and store
+      if (!to) return;
 #pragma unroll
-      for (int i = 0; i < 128; i += 4) {
+      for (int i = 0; i < 128; i += 8) {
         if (i >= width) continue;
-        float4 x = make_float4(acc[i] * f1 * f2, acc[i + 1] * f1 * f2, acc[i + 2] * f1 * f2, acc[i + 3] * f1 * f2);
+        uint32_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(acc[i + j] * f1 * f2);
         if (add) {
-          const float4 b = p[i / 4];
-          x.x += b.x, x.y += b.y, x.z += b.z, x.w += b.w;
+          const float4 a = *reinterpret_cast<const float4*>(to + i), b = *reinterpret_cast<const float4*>(to + i + 4);
+          const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(y[j] + __uint_as_float(x[j]));
         }
-        p[i / 4] = x;
+        store8(to + i, x);
       }
-    } else {
+    } else if (sd == 1) {  // rows off that alignment: through the warp's buffer, 16 columns of two rows at a time
+#pragma unroll
+      for (int i = 0; i < 128; i += 16) {
+        if (i >= width) continue;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) buf[lane * kPitch + j] = acc[i + j] * f1 * f2;
+        __syncwarp();
+        const int c = lane % 16;
+#pragma unroll 4
+        for (int r = lane / 16; r < 32; r += 2) {
+          float* p = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)to, r));
+          if (!p || i + c >= width) continue;
+          const float x = buf[r * kPitch + c];
+          p[i + c] = add ? p[i + c] + x : x;
+        }
+      }
+    } else {  // columns apart: the rows lie closer
+      if (!to) return;
 #pragma unroll
       for (int i = 0; i < 128; ++i) {
         if (i >= width) continue;
-        float* e = to + (int64_t)(col + i) * sd;
         const float x = acc[i] * f1 * f2;
-        *e = add ? *e + x : x;
+        to[i * sd] = add ? to[i * sd] + x : x;
       }
     }
   }
@@ -521,7 +610,8 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
                  const __grid_constant__ GemmDev g) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStage);  // of the first CTA: both CTAs' slabs are there
+  float* bufs = reinterpret_cast<float*>(smem + kStages * kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStage + 8 * kWarpBuf);  // of the first CTA: both CTAs' slabs are there
   uint64_t* empty = full + kStages;   // of each CTA: the pair's MMAs have read the stage
   uint64_t* tfull = empty + kStages;  // [2] of each CTA: an accumulator is complete
   uint64_t* tempty = tfull + 2;       // [2] of the first CTA: both CTAs' warps have read it
@@ -529,7 +619,6 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cta_rank();
-  const int live = *g.d.live;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -550,6 +639,9 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   pair_sync();  // the other CTA's barriers are there before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();  // everything from here on reads what earlier kernels wrote
+  const int live = *g.d.live;
   const int items = gemm_items<MODE>(g, live), pairs = gridDim.x / CG, pair = blockIdx.x / CG;
 
   if (warp >= 8) {
@@ -565,7 +657,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
           if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * kStage);
           const uint32_t bar = pair_addr(&full[s], 0);
           unsigned char* a = smem + s * kStage;
-          const int k = (w.k0 + i) * kSlab, m = w.m0 + rank * 128, n = w.n0 + rank * BR;
+          const int k = (w.k0 + i) * kSlab, m = w.m0 + rank * 128, n = w.n0 + rank * (w.cols / CG);
           if (MODE != kProducts) {
             pair_load_3d(a, &ma, k, m, 0, bar);
             pair_load_3d(a + kABytes, &mb, k, n, 0, bar);
@@ -596,7 +688,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
         const GemmItem w = gemm_item<MODE>(g, live, item);
         const bool amn = MODE == kProducts && w.dw, bmn = MODE == kProducts;
         const uint32_t idesc = uniform((1u << 4) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u) |
-                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24));
+                                       ((uint32_t)(w.cols >> 3) << 17) | ((uint32_t)(BM >> 4) << 24));
         const uint32_t astep = amn ? 128u : 2u, bstep = bmn ? 128u : 2u;
         const uint32_t da0 = uniform(sw128_low(smem, amn ? 64 * 128 : 16));
         const uint32_t db0 = uniform(sw128_low(smem + kABytes, bmn ? 64 * 128 : 16));
@@ -634,18 +726,25 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
     bool ok = true;
     for (int item = pair; item < items && ok; item += pairs) {
       const GemmItem w = gemm_item<MODE>(g, live, item);
-      const int row = w.m0 + (int)rank * 128 + rl, col = w.n0 + half * 128;
-      Entries ent;
-      ent.next = kNoToken;
-      float f = 0.f, lse2 = 0.f;
-      int orig = 0;
-      if (!w.dw && row < live) {
-        orig = g.d.rows[row];
+      TileRow t;
+      t.row = w.m0 + (int)rank * 128 + rl;
+      t.col = w.n0 + half * 128;
+      t.id = kNoToken;
+      t.f = t.lse2 = 0.f;
+      t.orig = t.e = 0;
+      if (!w.dw && t.row < live) {
+        t.orig = g.d.rows[t.row];
         if (MODE != kProducts) {
           // a power of two and the factor onto units of log2: neither 0 nor inf
-          f = fminf(fmaxf(mul3(g.hdown[row], *g.wdown, g.d.inv_temp * kHeadLog2e), 0x1p-126f), FLT_MAX);
-          ent.seek(g.d, orig, g.v0 + col);
-          if (MODE == kScoreGrad) lse2 = *head_row<const float>(g.d, g.d.lse, orig) * kHeadLog2e;
+          t.f = fminf(fmaxf(mul3(g.hdown[t.row], *g.wdown, g.d.inv_temp * kHeadLog2e), 0x1p-126f), FLT_MAX);
+          const int* ids = g.d.eid + (int64_t)t.orig * g.d.K;
+          int hi = g.d.K;
+          while (t.e < hi) {
+            const int mid = (t.e + hi) / 2;
+            if (ids[mid] < g.v0 + t.col) t.e = mid + 1; else hi = mid;
+          }
+          if (t.e < g.d.K) t.id = ids[t.e];
+          if (MODE == kScoreGrad) t.lse2 = *head_row<const float>(g.d, g.d.lse, t.orig) * kHeadLog2e;
         }
       }
       float acc[128];
@@ -671,7 +770,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
         __syncwarp();
         if (lane == 0) pair_arrive(bars[ci & 1]);
       }
-      if (ok) finish_tile<MODE>(g, w, live, row, col, orig, ent, f, lse2, acc);
+      if (ok) finish_tile<MODE>(g, w, live, t, bufs + warp * (kWarpBuf / 4), lane, acc);
     }
   }
   if (threadIdx.x % 32 == 0 && *(volatile int*)failed) atomicOr(g.err, kAsyncWaitTimeout);
@@ -685,6 +784,8 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
 
 // dh from the parts of its contraction, in order.
 __global__ void __launch_bounds__(256) head_dh_join_kernel(const __grid_constant__ GemmDev g) {
+  pdl_launch_dependents();
+  pdl_wait();
   const HeadDev& d = g.d;
   const int live = *d.live, r = blockIdx.x;
   if (r >= live) return;
@@ -759,8 +860,7 @@ Error launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap&
   allow_smem((const void*)k, kGemmSmem);
   const int64_t pairs = std::min<int64_t>(most, max_pairs((const void*)k));
   if (pairs < 1) return Error{};
-  k<<<(unsigned)(pairs * CG), kGemmThreads, kGemmSmem, s>>>(a, b, a2, b2, g);
-  return check_launch("head matrix product kernel");
+  return launch_after(k, dim3((unsigned)(pairs * CG)), kGemmThreads, kGemmSmem, s, "head matrix product kernel", a, b, a2, b2, g);
 }
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -829,13 +929,11 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   p.plane = hplane;
   p.down = reinterpret_cast<float*>(base + o_hdown);
   p.top = backward && d.dw ? tops : nullptr;
-  head_pack_hidden_kernel<<<(unsigned)Np, 256, 0, s>>>(p);
-  e = check_launch("head hidden planes kernel");
+  e = launch_after(head_pack_hidden_kernel, dim3((unsigned)Np), 256, 0, s, "head hidden planes kernel", p);
   if (e.ok() && p.top) {
     p.to = gp;
     p.down = downs;
-    head_pack_grad_kernel<<<(unsigned)Np, 256, 0, s>>>(p);
-    e = check_launch("head gradient planes kernel");
+    e = launch_after(head_pack_grad_kernel, dim3((unsigned)Np), 256, 0, s, "head gradient planes kernel", p);
   }
   if (!e.ok()) return e;
 
@@ -847,6 +945,13 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   g.plane = xplane;
   g.dh_part = reinterpret_cast<float*>(base + o_dh);
   g.Vcp = (int)Vp;
+  auto wide = [](const void* p, std::initializer_list<int64_t> strides, int64_t sd) {
+    bool ok = (uintptr_t)p % 32 == 0 && sd == 1;
+    for (int64_t x : strides) ok = ok && x % 8 == 0;
+    return ok;
+  };
+  g.wide_dw = d.dw && d.D % 8 == 0 && wide(d.dw, {d.dwv}, d.dwd);
+  g.wide_dh = d.dh.p && d.D % 8 == 0 && wide(d.dh.p, {d.dh.sb, d.dh.st}, d.dh.sd);
   const int64_t av = d.wv < 0 ? -d.wv : d.wv, ad = d.wd < 0 ? -d.wd : d.wd;
   const int along_v = d.V > 1 && d.D > 1 && av < ad;
   for (int64_t i = 0; i < pieces; ++i) {
@@ -861,12 +966,9 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     p.down = downs + 4 + i;
     p.v0 = g.v0;
     p.n = g.Vc;
-    const unsigned ctas = (unsigned)(along_v ? 8 * sms : std::min<int64_t>(g.Vc, 16 * sms));
-    head_weight_top_kernel<<<ctas, 256, 0, s>>>(p, along_v);
-    e = check_launch("head weight maximum kernel");
-    if (!e.ok()) return e;
-    head_pack_weight_kernel<<<ctas, 256, 0, s>>>(p, along_v);
-    e = check_launch("head weight planes kernel");
+    const unsigned ctas = (unsigned)(along_v ? 8 * sms : std::min<int64_t>((g.Vc + 7) / 8, 8 * sms));
+    e = launch_after(head_weight_top_kernel, dim3(ctas), 256, 0, s, "head weight maximum kernel", p, along_v);
+    if (e.ok()) e = launch_after(head_pack_weight_kernel, dim3(ctas), 256, 0, s, "head weight planes kernel", p, along_v);
     CUtensorMap ha, wb, xa, wc, xc, gc;
     if (e.ok()) e = map_rows(hp, Np, Dp, hplane, 128, &ha);
     if (e.ok()) e = map_rows(wp, g.Vc, Dp, wplane, BR, &wb);
@@ -885,8 +987,8 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     if (e.ok() && d.dw) e = map_cols(gp, Np, Dp, hplane, &gc);
     if (e.ok()) e = launch_gemm<kProducts>(xa, wc, xc, gc, g, htiles * g.splits + wtiles, s);
     if (e.ok() && d.dh.p && g.splits > 1) {
-      head_dh_join_kernel<<<dim3((unsigned)d.N, (unsigned)std::min<int64_t>(16, (d.D + 255) / 256)), 256, 0, s>>>(g);
-      e = check_launch("head hidden gradient join kernel");
+      e = launch_after(head_dh_join_kernel, dim3((unsigned)d.N, (unsigned)std::min<int64_t>(16, (d.D + 255) / 256)), 256, 0, s,
+                       "head hidden gradient join kernel", g);
     }
     if (!e.ok()) return e;
   }
