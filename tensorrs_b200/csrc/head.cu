@@ -43,6 +43,11 @@ __device__ __forceinline__ int head_id(const HeadDev& d, const RowsDev& ids, int
   return v < 0 || v >= d.V ? kNoToken : (int)v;
 }
 
+// The first of a row's tokens in order (kNoToken: the row has no target).
+__device__ __forceinline__ int head_first_id(const HeadDev& d, int row) {
+  return d.distill ? d.eid[(int64_t)row * d.K] : head_id(d, d.ids, row, 0);
+}
+
 // A warp per row: the softmax of the entries that are there, sorted by token
 // (the rank of an entry is counted: K is small).
 __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
@@ -175,8 +180,9 @@ __device__ __forceinline__ HeadPart head_add(const HeadPart& a, const HeadPart& 
 }
 
 // LR rows per CTA times 256 / LR threads along a row's parts, folded in a fixed
-// order.
-template <int LR>
+// order.  FEW: parts of the call's rows, not of those with a target, which are
+// not listed out; rows without one get their zeros here.
+template <int LR, bool FEW>
 __global__ void __launch_bounds__(256) head_join_kernel(const HeadDev d, const HeadPart* part, int parts, int64_t sp,
                                                         int64_t sr) {
   constexpr int LP = 256 / LR;
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadDev d, const H
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.x * LR + threadIdx.x % LR, w = threadIdx.x / LR;
-  const bool there = r < *d.live;
+  const bool there = FEW ? head_first_id(d, r) != kNoToken : r < *d.live;
   HeadPart a = {-INFINITY, 0.f, 0.f, 0.f};
   if (there) {
     // runs of consecutive parts, so that the order of the sums is that of the vocabulary
@@ -205,22 +211,23 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadDev d, const H
     __syncthreads();
     if (w < n) s[w][threadIdx.x % LR] = a;
   }
-  if (w != 0 || !there) return;
-  const int row = d.rows[r];
+  if (w != 0 || (!FEW && !there)) return;
+  const int row = FEW ? r : d.rows[r];
   const double lse = kHeadLn2 * ((double)a.m + log2((double)a.s));
   double loss = lse - kHeadLn2 * (double)a.dot;
   if (d.share != 0.f) loss -= kHeadLn2 * (double)d.share * (double)a.sum;
   if (d.distill) loss = (loss + (double)d.ent[row]) * (double)d.temp * (double)d.temp;
-  *head_row<float>(d, d.loss, row) = (float)loss;
-  if (d.lse.p) *head_row<float>(d, d.lse, row) = (float)lse;
+  *head_row<float>(d, d.loss, row) = there ? (float)loss : 0.f;
+  if (d.lse.p) *head_row<float>(d, d.lse, row) = there ? (float)lse : 0.f;
 }
 
 }  // namespace
 
 Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
                 cudaStream_t stream) {
-  if (few) return launch_after(head_join_kernel<1>, dim3((unsigned)d.N), 256, 0, stream, "head join kernel", d, part, parts, sp, sr);
-  return launch_after(head_join_kernel<8>, dim3((unsigned)((d.N + 7) / 8)), 256, 0, stream, "head join kernel", d, part,
+  if (few)
+    return launch_after(head_join_kernel<1, true>, dim3((unsigned)d.N), 256, 0, stream, "head join kernel", d, part, parts, sp, sr);
+  return launch_after(head_join_kernel<8, false>, dim3((unsigned)((d.N + 7) / 8)), 256, 0, stream, "head join kernel", d, part,
                       parts, sp, sr);
 }
 
@@ -274,197 +281,295 @@ __device__ __forceinline__ float head_fold(float (&a)[Q], int lane) {
   return a[0];
 }
 
-struct HeadRowsDev {
-  HeadDev d;
-  int r0;                // first live row of this launch
-  int Dp;                // the width rounded up to whole steps of 128
-  HeadPart* part;        // forward: [live row][CTA]
-  float* dx;             // backward: [V][NR]
+// The same for a weight that is read once: not kept in L1.
+template <bool VEC>
+__device__ __forceinline__ float4 head_stream4(const float* p, int c, int D, int64_t sd) {
+  if (!VEC) return head_load4<false>(p, c, D, sd);
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < D)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+                 : "l"(p + c));
+  return r;
+}
+
+// Up to 8 of the call's rows from r0 on.
+template <int NR>
+struct FewRows {
+  int row[NR];           // a row with a target, or -1
+  __device__ __forceinline__ void read(const HeadDev& d, int r0) {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) row[i] = r0 + i < d.N && head_first_id(d, r0 + i) != kNoToken ? r0 + i : -1;
+  }
 };
 
+struct HeadRowsDev {
+  HeadDev d;
+  int Dp;                // the width rounded up to whole steps of 128
+  HeadPart* part;        // forward: [row][CTA]
+  float* dx;             // backward: [row block][V][NR]
+};
+
+// blockIdx.y: a block of NR rows.  Blocks run side by side, so that what one
+// reads of the weight the other finds in L2.
 template <int NR, int RV, bool VEC, bool GRAD>
-__global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const __grid_constant__ HeadRowsDev a) {
+__global__ void __launch_bounds__(kRowsThreads, 2) head_rows_kernel(const __grid_constant__ HeadRowsDev a) {
   constexpr int Q = NR * RV, REP = 32 / Q, W = kRowsThreads / 32;
   extern __shared__ float4 s_h[];
+  __shared__ int s_row[NR];
   const HeadDev& d = a.d;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, live = *d.live;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r0 = blockIdx.y * NR;
   pdl_launch_dependents();
-  if (a.r0 >= live) return;
-  for (int i = threadIdx.x; i < NR * a.Dp / 4; i += kRowsThreads) {
-    const int n = i / (a.Dp / 4), c = i % (a.Dp / 4) * 4;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.r0 + n < live) {
-      const float* p = head_row<const float>(d, d.hid, d.rows[a.r0 + n]);
-      x = head_load4<false>(p, c, d.D, d.hid.sd);
+  // the weight's rows of this warp: groups of RV, `steps` steps of 128 columns each
+  const int steps = a.Dp / 128;
+  const int64_t hop = (int64_t)gridDim.x * W * RV;
+  int64_t vl = ((int64_t)blockIdx.x * W + warp) * RV;  // the loads' group and step, two steps ahead
+  int cl = 0;
+  auto fetch = [&](float4 (&x)[RV]) {
+#pragma unroll
+    for (int j = 0; j < RV; ++j)
+      x[j] = vl + j < d.V ? head_stream4<VEC>(d.w + (vl + j) * d.wv, cl * 128 + lane * 4, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (++cl == steps) {
+      cl = 0;
+      vl += hop;
     }
-    s_h[i] = x;
+  };
+  float4 x[2][RV];
+  fetch(x[0]);
+  fetch(x[1]);
+  pdl_wait();
+  if (threadIdx.x < NR) {
+    const int r = r0 + threadIdx.x;
+    s_row[threadIdx.x] = r < d.N && head_first_id(d, r) != kNoToken ? r : -1;
   }
   __syncthreads();
-  const int q = lane / REP, n = q % NR, rv = q / NR;
-  const bool there = a.r0 + n < live;
-  const int row = d.rows[there ? a.r0 + n : a.r0];
+  for (int i = threadIdx.x; i < NR * a.Dp / 4; i += kRowsThreads) {
+    const int n = i / (a.Dp / 4), c = i % (a.Dp / 4) * 4;
+    s_h[i] = s_row[n] >= 0 ? head_load4<false>(head_row<const float>(d, d.hid, s_row[n]), c, d.D, d.hid.sd)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __syncthreads();
+  const int q = lane / REP, n = q % NR, rv = q / NR, row = s_row[n];
   Entries ent;
-  ent.begin(d, row);
+  ent.left = 0;
+  ent.next = kNoToken;
+  if (row >= 0) {
+    if (d.distill) ent.begin(d, row);
+    else ent.next = head_id(d, d.ids, row, 0);
+  }
   const float f = d.inv_temp * kHeadLog2e;
   float lse2 = 0.f, g = 0.f;
-  if (GRAD) {
+  if (GRAD && row >= 0) {
     lse2 = *head_row<const float>(d, d.lse, row) * kHeadLog2e;
     g = *head_row<const float>(d, d.gl, row) * d.temp;
   }
   HeadPart pt = {-INFINITY, 0.f, 0.f, 0.f};
-  for (int64_t v0 = ((int64_t)blockIdx.x * W + warp) * RV; v0 < d.V; v0 += (int64_t)gridDim.x * W * RV) {
-    uint64_t acc[Q];
+  uint64_t acc[Q];
 #pragma unroll
-    for (int i = 0; i < Q; ++i) acc[i] = 0;
-#pragma unroll 2
-    for (int c = lane * 4; c < a.Dp; c += 128) {
-      float4 x[RV];
+  for (int i = 0; i < Q; ++i) acc[i] = 0;
+  int64_t v0 = ((int64_t)blockIdx.x * W + warp) * RV;
+  int c = 0;
+  auto step = [&](float4 (&y)[RV]) {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const float4 h = s_h[i * (a.Dp / 4) + c * 32 + lane];
+      const uint64_t h0 = pk(h.x, h.y), h1 = pk(h.z, h.w);
 #pragma unroll
       for (int j = 0; j < RV; ++j)
-        x[j] = v0 + j < d.V ? head_load4<VEC>(d.w + (v0 + j) * d.wv, c, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const float4 h = s_h[(i * a.Dp + c) / 4];
-        const uint64_t h0 = pk(h.x, h.y), h1 = pk(h.z, h.w);
-#pragma unroll
-        for (int j = 0; j < RV; ++j)
-          acc[j * NR + i] = fma2(pk(x[j].z, x[j].w), h1, fma2(pk(x[j].x, x[j].y), h0, acc[j * NR + i]));
-      }
+        acc[j * NR + i] = fma2(pk(y[j].z, y[j].w), h1, fma2(pk(y[j].x, y[j].y), h0, acc[j * NR + i]));
     }
+    fetch(y);
+    if (++c < steps) return;
+    c = 0;
     float sums[Q];
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       float lo, hi;
       upk(acc[i], &lo, &hi);
       sums[i] = lo + hi;
+      acc[i] = 0;
     }
-    const float x = head_fold<Q>(sums, lane) * f;  // in units of log2
+    const float s = head_fold<Q>(sums, lane) * f;  // in units of log2
     const int64_t v = v0 + rv;
-    if (v >= d.V || !there) {
-      if (GRAD && v < d.V && lane % REP == 0) a.dx[v * NR + n] = 0.f;
-      continue;
+    v0 += hop;
+    if (v >= d.V) return;
+    if (row < 0) {
+      if (GRAD && lane % REP == 0) a.dx[((int64_t)blockIdx.y * d.V + v) * NR + n] = 0.f;
+      return;
     }
     float t = 0.f;
     if (ent.next <= v) {
-      ent.skip_to((int)v);
-      t = ent.take((int)v);
+      if (d.distill) {
+        ent.skip_to((int)v);
+        t = ent.take((int)v);
+      } else if (ent.next == v) {
+        t = d.weight;
+      }
     }
     if (GRAD) {
-      if (lane % REP == 0) a.dx[v * NR + n] = g * (head_ex2(x - lse2) - t - d.share);
+      if (lane % REP == 0) a.dx[((int64_t)blockIdx.y * d.V + v) * NR + n] = g * (head_ex2(s - lse2) - t - d.share);
     } else {
-      const float m = fmaxf(pt.m, x);
-      pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(x - m);
+      const float m = fmaxf(pt.m, s);
+      pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(s - m);
       if (m == -INFINITY) pt.s = 0.f;  // scores of -inf alone
       pt.m = m;
-      if (t != 0.f) pt.dot = __fmaf_rn(t, x, pt.dot);
-      pt.sum += x;
+      if (t != 0.f) pt.dot = __fmaf_rn(t, s, pt.dot);
+      pt.sum += s;
     }
+  };
+  while (v0 < d.V) {
+    step(x[0]);
+    if (v0 >= d.V) break;
+    step(x[1]);
   }
   if (GRAD) return;
   // the CTA's parts of a row: RV lanes of each warp
-  HeadPart* s = reinterpret_cast<HeadPart*>(s_h);
+  HeadPart* sp = reinterpret_cast<HeadPart*>(s_h);
   __syncthreads();
-  if (lane % REP == 0) s[(warp * RV + rv) * NR + n] = pt;
+  if (lane % REP == 0) sp[(warp * RV + rv) * NR + n] = pt;
   for (int k = W * RV / 2; k > 0; k /= 2) {
     __syncthreads();
     const int w = threadIdx.x / NR, i = threadIdx.x % NR;
     HeadPart y;
-    if (w < k) y = head_add(s[2 * w * NR + i], s[(2 * w + 1) * NR + i]);
+    if (w < k) y = head_add(sp[2 * w * NR + i], sp[(2 * w + 1) * NR + i]);
     __syncthreads();
-    if (w < k) s[w * NR + i] = y;
+    if (w < k) sp[w * NR + i] = y;
   }
   __syncthreads();
-  if (threadIdx.x < NR && a.r0 + threadIdx.x < live)
-    a.part[(int64_t)(a.r0 + threadIdx.x) * gridDim.x + blockIdx.x] = s[threadIdx.x];
+  if (threadIdx.x < NR && r0 + threadIdx.x < d.N)
+    a.part[(int64_t)(r0 + threadIdx.x) * gridDim.x + blockIdx.x] = sp[threadIdx.x];
 }
 
 struct HeadGradDev {
   HeadDev d;
-  int r0;
-  const float* dx;       // [V][NR]
-  float* part;           // [CTA along V][NR][D] of dh
+  int block;             // of NR rows
+  int lg;                // 2^lg threads (whole warps) along the width, the rest along the vocabulary
+  const float* dx;       // [row block][V][NR]
+  float* part;           // [part of the vocabulary][NR][D] of dh
 };
 
-// 256 threads by 4 columns; blockIdx.y: a range of the vocabulary.
+// A thread per 4 columns; blockIdx.y and the thread's group: a range of the
+// vocabulary.
 template <int NR>
-__global__ void __launch_bounds__(256) head_grad_kernel(const __grid_constant__ HeadGradDev a) {
+__global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant__ HeadGradDev a) {
+  constexpr int U = 4;   // rows of the vocabulary in flight
   const HeadDev& d = a.d;
-  const int live = *d.live;
   pdl_launch_dependents();
+  const int c = (blockIdx.x * 256 + (threadIdx.x & ((1 << a.lg) - 1))) * 4;
+  const int groups = 256 >> a.lg, part = blockIdx.y * groups + (threadIdx.x >> a.lg), parts = gridDim.y * groups;
+  const int r0 = a.block * NR;
+  const bool add = a.block > 0;  // behind earlier rows
   pdl_wait();
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
-  if (c >= d.D || a.r0 >= (live > 0 ? live : 1)) return;
-  float h[NR][4], acc[NR][4];
+  uint64_t h[NR][2], acc[NR][2];
+  {
+    FewRows<NR> rows;
+    rows.read(d, r0);
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.r0 + i < live) x = head_load4<false>(head_row<const float>(d, d.hid, d.rows[a.r0 + i]), c, d.D, d.hid.sd);
-    h[i][0] = x.x, h[i][1] = x.y, h[i][2] = x.z, h[i][3] = x.w;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    for (int i = 0; i < NR; ++i) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (rows.row[i] >= 0) x = head_load4<false>(head_row<const float>(d, d.hid, rows.row[i]), c, d.D, d.hid.sd);
+      h[i][0] = pk(x.x, x.y), h[i][1] = pk(x.z, x.w);
+      acc[i][0] = acc[i][1] = 0;
+    }
   }
-  const int64_t v1 = (int64_t)d.V * (blockIdx.y + 1) / gridDim.y;
-#pragma unroll 2
-  for (int64_t v = (int64_t)d.V * blockIdx.y / gridDim.y; v < v1; ++v) {
-    float x[NR];
+  const float* dx = a.dx + (int64_t)a.block * d.V * NR;
+  const int lane = threadIdx.x % 32;
+  const int64_t v1 = (int64_t)d.V * (part + 1) / parts;
+  int64_t v = (int64_t)d.V * part / parts;
+  // U rows of the weight, and one of their score gradients per lane
+  auto fetch = [&](float4 (&w)[U], float& x, int64_t at) {
+    x = lane < U * NR && at + lane / NR < v1 ? dx[at * NR + lane] : 0.f;
 #pragma unroll
-    for (int i = 0; i < NR; ++i) x[i] = live > 0 ? __ldg(a.dx + v * NR + i) : 0.f;
-    if (d.dh.p) {
-      const float4 w = d.vec_w ? head_load4<true>(d.w + v * d.wv, c, d.D, 1) : head_load4<false>(d.w + v * d.wv, c, d.D, d.wd);
+    for (int j = 0; j < U; ++j) {
+      w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (d.dh.p && at + j < v1)
+        w[j] = d.vec_w ? head_stream4<true>(d.w + (at + j) * d.wv, c, d.D, 1) : head_load4<false>(d.w + (at + j) * d.wv, c, d.D, d.wd);
+    }
+  };
+  auto work = [&](float4 (&w)[U], float xs) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      uint64_t o0 = 0, o1 = 0;
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        acc[i][0] = __fmaf_rn(x[i], w.x, acc[i][0]);
-        acc[i][1] = __fmaf_rn(x[i], w.y, acc[i][1]);
-        acc[i][2] = __fmaf_rn(x[i], w.z, acc[i][2]);
-        acc[i][3] = __fmaf_rn(x[i], w.w, acc[i][3]);
+        const float x = __shfl_sync(0xffffffffu, xs, j * NR + i);
+        const uint64_t xx = pk(x, x);
+        if (d.dh.p) {
+          acc[i][0] = fma2(xx, pk(w[j].x, w[j].y), acc[i][0]);
+          acc[i][1] = fma2(xx, pk(w[j].z, w[j].w), acc[i][1]);
+        }
+        o0 = fma2(xx, h[i][0], o0);
+        o1 = fma2(xx, h[i][1], o1);
       }
-    }
-    if (d.dw) {
-      float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = __fmaf_rn(x[i], h[i][j], o[j]);
-      float* to = d.dw + v * d.dwv;
+      if (!d.dw || v + j >= v1 || c >= d.D) continue;
+      float o[4];
+      upk(o0, &o[0], &o[1]);
+      upk(o1, &o[2], &o[3]);
+      float* to = d.dw + (v + j) * d.dwv;
       if (d.vec_dw) {
         float4 y = make_float4(o[0], o[1], o[2], o[3]);
-        if (a.r0 > 0) {  // behind earlier rows
+        if (add) {
           const float4 b = *reinterpret_cast<const float4*>(to + c);
           y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
         }
-        *reinterpret_cast<float4*>(to + c) = y;
+        __stcs(reinterpret_cast<float4*>(to + c), y);
       } else {
-        for (int j = 0; j < 4 && c + j < d.D; ++j) {
-          float* e = to + (c + j) * d.dwd;
-          *e = a.r0 > 0 ? *e + o[j] : o[j];
-        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < d.D) {
+            float* e = to + (c + k) * d.dwd;
+            *e = add ? *e + o[k] : o[k];
+          }
       }
     }
+    v += U;
+  };
+  float4 wa[U], wb[U];
+  float xa, xb;
+  fetch(wa, xa, v);
+  while (v < v1) {
+    fetch(wb, xb, v + U);
+    work(wa, xa);
+    if (v >= v1) break;
+    fetch(wa, xa, v + U);
+    work(wb, xb);
   }
   if (!d.dh.p) return;
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
-    for (int j = 0; j < 4 && c + j < d.D; ++j)
-      a.part[((int64_t)blockIdx.y * NR + i) * d.D + c + j] = acc[i][j];
+  for (int i = 0; i < NR; ++i) {
+    float y[4];
+    upk(acc[i][0], &y[0], &y[1]);
+    upk(acc[i][1], &y[2], &y[3]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < d.D) a.part[((int64_t)part * NR + i) * d.D + c + k] = y[k];
+  }
 }
 
-// dh of up to NR rows from its parts, in order: 32 columns times 8 parts per CTA.
+// dh of up to NR rows from its parts, in order: 32 columns times 8 runs of parts
+// per CTA; zeros for rows without a target.
 template <int NR>
 __global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_constant__ HeadGradDev a, int parts) {
   __shared__ float s[8][32];
   const HeadDev& d = a.d;
   pdl_wait();
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32, r = blockIdx.y;
-  if (a.r0 + r >= *d.live) return;
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32, r = blockIdx.y, row = a.block * NR + r;
+  if (row >= d.N) return;
   float sum = 0.f;
+  const int p1 = (int)((int64_t)parts * (w + 1) / 8);
   if (c < d.D)
-    for (int p = (int)((int64_t)parts * w / 8); p < (int)((int64_t)parts * (w + 1) / 8); ++p)
-      sum += a.part[((int64_t)p * NR + r) * d.D + c];
+    for (int p = (int)((int64_t)parts * w / 8); p < p1; p += 8) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = p + j < p1 ? a.part[((int64_t)(p + j) * NR + r) * d.D + c] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += x[j];
+    }
   s[w][threadIdx.x % 32] = sum;
   __syncthreads();
   if (w != 0 || c >= d.D) return;
   for (int i = 1; i < 8; ++i) sum += s[i][threadIdx.x];
-  head_row<float>(d, d.dh, d.rows[a.r0 + r])[c * d.dh.sd] = sum;
+  head_row<float>(d, d.dh, row)[c * d.dh.sd] = head_first_id(d, row) != kNoToken ? sum : 0.f;
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -474,8 +579,7 @@ Error launch_rows(HeadRowsDev& a, int ctas, cudaStream_t s) {
   auto k = a.d.vec_w ? head_rows_kernel<NR, RV, true, GRAD> : head_rows_kernel<NR, RV, false, GRAD>;
   const int smem = std::max<int>(NR * a.Dp * 4, kRowsThreads * (int)sizeof(HeadPart));
   allow_smem((const void*)k, smem);
-  k<<<(unsigned)ctas, kRowsThreads, smem, s>>>(a);
-  return check_launch("head rows kernel");
+  return launch_after(k, dim3((unsigned)ctas, (unsigned)((a.d.N + NR - 1) / NR)), kRowsThreads, smem, s, "head rows kernel", a);
 }
 template <bool GRAD>
 Error rows_of(int nr, HeadRowsDev& a, int ctas, cudaStream_t s) {
@@ -489,7 +593,16 @@ Error launch_grad(HeadGradDev& a, int splits, cudaStream_t s) {
                          "head gradient kernel", a);
   if (!e.ok() || !a.d.dh.p) return e;
   return launch_after(head_grad_join_kernel<NR>, dim3((unsigned)((a.d.D + 31) / 32), (unsigned)NR), 256, 0, s,
-                      "head gradient join kernel", a, splits);
+                      "head gradient join kernel", a, splits * (256 >> a.lg));
+}
+
+// Rows per block: as many as share one read of the weight within the shared
+// memory, 8 at most.
+int few_rows(const HeadDev& d) {
+  const int Dp = (d.D + 127) / 128 * 128;
+  int nr = d.N >= 5 ? 8 : d.N >= 3 ? 4 : std::max(1, d.N);
+  while (nr > 1 && nr * Dp * 4 > kRowsSmem) nr /= 2;
+  return nr;
 }
 
 Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
@@ -498,37 +611,35 @@ Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
   std::memset(static_cast<void*>(&a), 0, sizeof(a));
   a.d = d;
   a.Dp = (d.D + 127) / 128 * 128;
-  int nr = d.N >= 5 ? 8 : d.N >= 3 ? 4 : std::max(1, d.N);
-  while (nr > 1 && nr * a.Dp * 4 > kRowsSmem) nr /= 2;
-  const int ctas = 2 * sms;
+  const int nr = few_rows(d), blocks = (d.N + nr - 1) / nr;
+  const int ctas = std::max(sms / 2, 2 * sms / std::max(1, blocks));
   Scratch mem;
   Error e;
   if (!backward) {
     e = mem.alloc(sizeof(HeadPart) * (size_t)d.N * ctas, s);
     if (!e.ok()) return e;
     a.part = mem.as<HeadPart>();
-    for (a.r0 = 0; e.ok() && a.r0 < d.N; a.r0 += nr) e = rows_of<false>(nr, a, ctas, s);
+    e = rows_of<false>(nr, a, ctas, s);
     if (e.ok()) e = head_join(d, a.part, ctas, 1, ctas, true, s);
     return e;
   }
-  const int colblocks = (d.D + 1023) / 1024;
-  const int splits = std::max(1, std::min(d.V, 4 * sms / colblocks));
-  const size_t nd = (size_t)d.V * nr;
-  e = mem.alloc(sizeof(float) * (nd + (size_t)splits * nr * d.D), s);
-  if (!e.ok()) return e;
-  a.dx = mem.as<float>();
   HeadGradDev g;
   std::memset(static_cast<void*>(&g), 0, sizeof(g));
+  const int chunks = (d.D + 3) / 4, colblocks = (d.D + 1023) / 1024;
+  g.lg = 5;
+  while (g.lg < 8 && (1 << g.lg) < chunks) ++g.lg;
+  const int splits = std::max(1, std::min((d.V + 31) / 32, 2 * sms / colblocks));
+  const size_t nd = ((size_t)d.V * nr * blocks + 3) / 4 * 4;
+  e = mem.alloc(sizeof(float) * (nd + (size_t)splits * (256 >> g.lg) * nr * d.D), s);
+  if (!e.ok()) return e;
+  a.dx = mem.as<float>();
+  e = rows_of<true>(nr, a, ctas, s);
   g.d = d;
   g.dx = a.dx;
   g.part = a.dx + nd;
-  for (a.r0 = 0; e.ok() && (a.r0 == 0 || a.r0 < d.N); a.r0 += nr) {  // without rows: zeros into dw
-    g.r0 = a.r0;
-    e = rows_of<true>(nr, a, ctas, s);
-    if (!e.ok()) return e;
+  for (g.block = 0; e.ok() && g.block < blocks; ++g.block)
     e = nr == 1 ? launch_grad<1>(g, splits, s) : nr == 2 ? launch_grad<2>(g, splits, s)
         : nr == 4 ? launch_grad<4>(g, splits, s) : launch_grad<8>(g, splits, s);
-  }
   return e;
 }
 
@@ -629,35 +740,37 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   }
   d.vec_h = N > 0 && rows_vectors(c.hidden);
   if (N == 0 && !d.dw) return Error{};
+  // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
+  // tensor-core path writes the zeros.
+  const bool few = N > 0 && N <= 16 && d.D <= kRowsSmem / 4;
   // the rows' targets
   Scratch mem;
   const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;
-  e = mem.alloc(4 * (n + 4 + 2 * nk + (c.distill ? n : 0)), stream);
-  if (!e.ok()) return e;
-  d.live = mem.as<int>();
-  d.rows = d.live + 4;
-  d.eid = d.rows + n;
-  d.ew = reinterpret_cast<float*>(d.eid + nk);
-  d.ent = d.ew + nk;
+  if (!few || c.distill) {
+    e = mem.alloc(4 * (n + 4 + 2 * nk + (c.distill ? n : 0)), stream);
+    if (!e.ok()) return e;
+    d.live = mem.as<int>();
+    d.rows = d.live + 4;
+    d.eid = d.rows + n;
+    d.ew = reinterpret_cast<float*>(d.eid + nk);
+    d.ent = d.ew + nk;
+  }
   if (c.distill && N > 0) {
     const int smem = 8 * 2 * d.K * 4;
     allow_smem((const void*)head_teacher_kernel, smem);
     head_teacher_kernel<<<(unsigned)((N + 7) / 8), 256, smem, stream>>>(d);
     e = check_launch("head teacher kernel");
     if (!e.ok()) return e;
-    e = launch_after(head_list_kernel, dim3(1), 1024, 0, stream, "head list kernel", d);
-  } else {
-    head_list_kernel<<<1, 1024, 0, stream>>>(d);
-    e = check_launch("head list kernel");
   }
+  if (few) return run_rows(d, c.backward, stream);
+  e = launch_after(head_list_kernel, dim3(1), 1024, 0, stream, "head list kernel", d);
   if (!e.ok()) return e;
   if (c.grad_hidden && N > 0) {
     e = launch_after(head_masked_kernel, dim3((unsigned)std::min<int64_t>((N + 7) / 8, 1024)), 256, 0, stream,
                      "head masked rows kernel", d);
     if (!e.ok()) return e;
   }
-  if (N > 16) return head_tc(d, c.backward, stream);
-  return run_rows(d, c.backward, stream);
+  return head_tc(d, c.backward, stream);
 }
 
 trs_status finish(const Error& e) {

@@ -871,7 +871,7 @@ constexpr int64_t kPieceBytes = 512ll << 20;  // planes of a piece
 
 Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   const int sms = current_device_info().sm_count;
-  const int64_t Np = round_up(d.N, BM), Dp = round_up(d.D, kSlab), dtiles = (d.D + BN - 1) / BN;
+  const int64_t Np = round_up(std::max(d.N, 1), BM), Dp = round_up(d.D, kSlab), dtiles = (d.D + BN - 1) / BN;
   // pieces of the vocabulary of one size, whole tiles each
   const int64_t row_bytes = 4 * Dp + (backward ? 4 * Np : 0);
   int64_t pieces = std::max<int64_t>(1, (round_up(d.V, BN) * row_bytes + kPieceBytes - 1) / kPieceBytes);
@@ -887,10 +887,10 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   g.dtiles = (int)dtiles;
   const int64_t htiles = Np / BM * dtiles, wtiles = Vp / BN * dtiles;
   g.splits = 1;
-  if (backward && d.dh.p) {
-    // dh's few tiles with a long contraction: parts of about the average work of a pair, 8 slabs at least
+  if (backward && d.dh.p && d.N > 0) {
+    // dh's few tiles with a long contraction: parts of about a third of a pair's share of the work, 8 slabs at least
     const int64_t work = htiles * Vp + (d.dw ? wtiles * Np : 0);
-    const int64_t part = std::max<int64_t>(512, work / std::max(1, sms / CG));
+    const int64_t part = std::max<int64_t>(512, work / std::max(1, sms / CG) / 3);
     g.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Vp + part / 2) / part));
   }
   g.slabs = (int)((Vp / kSlab + g.splits - 1) / g.splits);
