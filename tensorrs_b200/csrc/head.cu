@@ -15,10 +15,11 @@
 // rows, which HBM bounds: the weight is read once in f32 and every element of it
 // used for all rows.
 //
-//   head_rows_kernel  a warp per RV vocabulary rows: lanes along the width, the
-//                     hidden rows in shared memory, NR RV dot products folded by
-//                     handing over halves; then the running maximum and sum of the
-//                     softmax per lane, or the gradient of the scores
+//   head_rows_kernel  a warp per 16 vocabulary rows, 8 or 16 hidden rows in shared
+//                     memory: f32 by three TF32 products (mma.sync, which leaves
+//                     every result with one lane and needs no shuffles; HBM, not
+//                     the tensor core, sets the pace); then the running maximum and
+//                     sum of the softmax per lane, or the gradient of the scores
 //   head_grad_kernel  a thread per 4 columns walks vocabulary rows: a row's dw from
 //                     the hidden rows in registers, and its part of dh
 #include <algorithm>
@@ -235,7 +236,6 @@ namespace {
 
 // ---- few rows ----------------------------------------------------------------------
 
-constexpr int kRowsThreads = 256;
 constexpr int kRowsSmem = 200 * 1024;
 
 __device__ __forceinline__ uint64_t pk(float a, float b) {
@@ -264,23 +264,6 @@ __device__ __forceinline__ float4 head_load4(const float* p, int c, int D, int64
   return r;
 }
 
-// The sums over the warp of Q values per lane, by handing over halves: lane l
-// ends with value l / (32 / Q).
-template <int Q>
-__device__ __forceinline__ float head_fold(float (&a)[Q], int lane) {
-  int o = 16;
-#pragma unroll
-  for (int n = Q; n > 1; n /= 2, o /= 2)
-#pragma unroll
-    for (int i = 0; i < n / 2; ++i) {
-      const float keep = lane & o ? a[i + n / 2] : a[i], give = lane & o ? a[i] : a[i + n / 2];
-      a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-    }
-#pragma unroll
-  for (; o > 0; o /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
-  return a[0];
-}
-
 // The same for a weight that is read once: not kept in L1.
 template <bool VEC>
 __device__ __forceinline__ float4 head_stream4(const float* p, int c, int D, int64_t sd) {
@@ -303,148 +286,215 @@ struct FewRows {
   }
 };
 
+// D += A B for A 16 x 8 (row major), B 8 x 8, in TF32: the upper 19 bits of each
+// element are read.
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo, hi its upper 11 significant bits; the tensor core reads the upper 11 of lo.
+__device__ __forceinline__ void tf32_split(float x, uint32_t* hi, uint32_t* lo) {
+  *hi = __float_as_uint(x) & 0xFFFFE000u;
+  *lo = __float_as_uint(x - __uint_as_float(*hi));
+}
+
 struct HeadRowsDev {
   HeadDev d;
-  int Dp;                // the width rounded up to whole steps of 128
+  int blocks;            // the width in blocks of 16, rounded up
   HeadPart* part;        // forward: [row][CTA]
-  float* dx;             // backward: [row block][V][NR]
+  float* dx;             // backward: [row block][V][8 NT]
 };
 
-// blockIdx.y: a block of NR rows.  Blocks run side by side, so that what one
-// reads of the weight the other finds in L2.
-template <int NR, int RV, bool VEC, bool GRAD>
-__global__ void __launch_bounds__(kRowsThreads, 2) head_rows_kernel(const __grid_constant__ HeadRowsDev a) {
-  constexpr int Q = NR * RV, REP = 32 / Q, W = kRowsThreads / 32;
-  extern __shared__ float4 s_h[];
+constexpr int kFewThreads = 512;
+constexpr int kAhead = 6;    // blocks of 16 columns in flight per warp
+
+// Up to 8 NT rows (blockIdx.y: which) against the whole vocabulary.  A warp takes 16
+// vocabulary rows at a time; lane l reads columns 4 (l % 4) .. + 3 of each block of
+// 16 from its rows l / 4 and l / 4 + 8, which are the elements that it supplies to
+// two MMAs (the order of the columns inside a block does not matter as long as
+// the hidden rows take the same).
+template <int NT, bool VEC, bool GRAD>
+__global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_constant__ HeadRowsDev a) {
+  constexpr int W = kFewThreads / 32, NR = 8 * NT;
+  extern __shared__ float s_h[];         // [NR][pitch]
   __shared__ int s_row[NR];
+  __shared__ HeadPart s_part[W][NR];
   const HeadDev& d = a.d;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r0 = blockIdx.y * NR;
+  const int lg = lane / 4, lt = lane % 4, pitch = a.blocks * 16 + 16;
   pdl_launch_dependents();
-  // the weight's rows of this warp: groups of RV, `steps` steps of 128 columns each
-  const int steps = a.Dp / 128;
-  const int64_t hop = (int64_t)gridDim.x * W * RV;
-  int64_t vl = ((int64_t)blockIdx.x * W + warp) * RV;  // the loads' group and step, two steps ahead
-  int cl = 0;
-  auto fetch = [&](float4 (&x)[RV]) {
+  // groups of 16 rows go around the CTAs before the warps, so that the SMs' shares differ by one at most
+  const int hop = gridDim.x * W, groups = (d.V + 15) / 16;
+  int gl = warp * gridDim.x + blockIdx.x, bl = 0;    // the loads' group and block
+  auto fetch = [&](float4 (&x)[2]) {
 #pragma unroll
-    for (int j = 0; j < RV; ++j)
-      x[j] = vl + j < d.V ? head_stream4<VEC>(d.w + (vl + j) * d.wv, cl * 128 + lane * 4, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (++cl == steps) {
-      cl = 0;
-      vl += hop;
+    for (int j = 0; j < 2; ++j) {
+      const int64_t v = (int64_t)gl * 16 + lg + 8 * j;
+      x[j] = v < d.V ? head_stream4<VEC>(d.w + v * d.wv, bl * 16 + lt * 4, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (++bl == a.blocks) {
+      bl = 0;
+      gl += hop;
     }
   };
-  float4 x[2][RV];
-  fetch(x[0]);
-  fetch(x[1]);
+  float4 x[kAhead][2];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) fetch(x[i]);
   pdl_wait();
   if (threadIdx.x < NR) {
     const int r = r0 + threadIdx.x;
     s_row[threadIdx.x] = r < d.N && head_first_id(d, r) != kNoToken ? r : -1;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < NR * a.Dp / 4; i += kRowsThreads) {
-    const int n = i / (a.Dp / 4), c = i % (a.Dp / 4) * 4;
-    s_h[i] = s_row[n] >= 0 ? head_load4<false>(head_row<const float>(d, d.hid, s_row[n]), c, d.D, d.hid.sd)
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = threadIdx.x; i < NR * a.blocks * 4; i += kFewThreads) {
+    const int n = i / (a.blocks * 4), c = i % (a.blocks * 4) * 4;
+    *reinterpret_cast<float4*>(&s_h[n * pitch + c]) =
+        s_row[n] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+        : d.vec_h    ? head_load4<true>(head_row<const float>(d, d.hid, s_row[n]), c, d.D, 1)
+                     : head_load4<false>(head_row<const float>(d, d.hid, s_row[n]), c, d.D, d.hid.sd);
   }
   __syncthreads();
-  const int q = lane / REP, n = q % NR, rv = q / NR, row = s_row[n];
-  Entries ent;
-  ent.left = 0;
-  ent.next = kNoToken;
-  if (row >= 0) {
-    if (d.distill) ent.begin(d, row);
-    else ent.next = head_id(d, d.ids, row, 0);
+  // this lane's results: rows lg and lg + 8 of a group times call rows 2 lt, 2 lt + 1 of each eight
+  constexpr int M = 2 * NT;
+  int row[M], at[M], next[M];
+  float lse2[M], gr[M];
+  HeadPart pt[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    row[i] = s_row[i / 2 * 8 + 2 * lt + i % 2];
+    at[i] = 0;
+    next[i] = row[i] < 0 ? kNoToken : head_first_id(d, row[i]);
+    lse2[i] = gr[i] = 0.f;
+    if (GRAD && row[i] >= 0) {
+      lse2[i] = *head_row<const float>(d, d.lse, row[i]) * kHeadLog2e;
+      gr[i] = *head_row<const float>(d, d.gl, row[i]) * d.temp;
+    }
+    pt[i] = HeadPart{-INFINITY, 0.f, 0.f, 0.f};
   }
   const float f = d.inv_temp * kHeadLog2e;
-  float lse2 = 0.f, g = 0.f;
-  if (GRAD && row >= 0) {
-    lse2 = *head_row<const float>(d, d.lse, row) * kHeadLog2e;
-    g = *head_row<const float>(d, d.gl, row) * d.temp;
-  }
-  HeadPart pt = {-INFINITY, 0.f, 0.f, 0.f};
-  uint64_t acc[Q];
+  float sum[NT][4], part[NT][4];
 #pragma unroll
-  for (int i = 0; i < Q; ++i) acc[i] = 0;
-  int64_t v0 = ((int64_t)blockIdx.x * W + warp) * RV;
-  int c = 0;
-  auto step = [&](float4 (&y)[RV]) {
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const float4 h = s_h[i * (a.Dp / 4) + c * 32 + lane];
-      const uint64_t h0 = pk(h.x, h.y), h1 = pk(h.z, h.w);
+    for (int j = 0; j < 4; ++j) sum[i][j] = part[i][j] = 0.f;
+  int g = warp * gridDim.x + blockIdx.x, b = 0;
+  auto step = [&](float4 (&y)[2]) {
+    uint32_t hi[2][4], lo[2][4];  // [columns 0 and 1, columns 2 and 3]
 #pragma unroll
-      for (int j = 0; j < RV; ++j)
-        acc[j * NR + i] = fma2(pk(y[j].z, y[j].w), h1, fma2(pk(y[j].x, y[j].y), h0, acc[j * NR + i]));
+    for (int j = 0; j < 2; ++j) {
+      tf32_split(y[j].x, &hi[0][j], &lo[0][j]);
+      tf32_split(y[j].y, &hi[0][2 + j], &lo[0][2 + j]);
+      tf32_split(y[j].z, &hi[1][j], &lo[1][j]);
+      tf32_split(y[j].w, &hi[1][2 + j], &lo[1][2 + j]);
     }
     fetch(y);
-    if (++c < steps) return;
-    c = 0;
-    float sums[Q];
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
-      float lo, hi;
-      upk(acc[i], &lo, &hi);
-      sums[i] = lo + hi;
-      acc[i] = 0;
-    }
-    const float s = head_fold<Q>(sums, lane) * f;  // in units of log2
-    const int64_t v = v0 + rv;
-    v0 += hop;
-    if (v >= d.V) return;
-    if (row < 0) {
-      if (GRAD && lane % REP == 0) a.dx[((int64_t)blockIdx.y * d.V + v) * NR + n] = 0.f;
-      return;
-    }
-    float t = 0.f;
-    if (ent.next <= v) {
-      if (d.distill) {
-        ent.skip_to((int)v);
-        t = ent.take((int)v);
-      } else if (ent.next == v) {
-        t = d.weight;
+    for (int i = 0; i < NT; ++i) {
+      const float4 h = *reinterpret_cast<const float4*>(&s_h[(i * 8 + lg) * pitch + b * 16 + lt * 4]);
+      uint32_t hh[4], hl[4];
+      tf32_split(h.x, &hh[0], &hl[0]);
+      tf32_split(h.y, &hh[1], &hl[1]);
+      tf32_split(h.z, &hh[2], &hl[2]);
+      tf32_split(h.w, &hh[3], &hl[3]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        mma_tf32(part[i], lo[k], hh[2 * k], hh[2 * k + 1]);
+        mma_tf32(part[i], hi[k], hl[2 * k], hl[2 * k + 1]);
+        mma_tf32(part[i], hi[k], hh[2 * k], hh[2 * k + 1]);
       }
     }
-    if (GRAD) {
-      if (lane % REP == 0) a.dx[((int64_t)blockIdx.y * d.V + v) * NR + n] = g * (head_ex2(s - lse2) - t - d.share);
-    } else {
-      const float m = fmaxf(pt.m, s);
-      pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(s - m);
-      if (m == -INFINITY) pt.s = 0.f;  // scores of -inf alone
-      pt.m = m;
-      if (t != 0.f) pt.dot = __fmaf_rn(t, s, pt.dot);
-      pt.sum += s;
+    // the tensor core cuts its sums: they go on in f32 every 256 columns
+    if ((++b & 15) == 0 || b == a.blocks) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum[i][j] += part[i][j];
+          part[i][j] = 0.f;
+        }
     }
+    if (b < a.blocks) return;
+    b = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int v = g * 16 + lg + 8 * j;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        float& s = sum[i / 2][2 * j + i % 2];
+        const float z = s * f;  // in units of log2
+        s = 0.f;
+        if (v >= d.V) continue;
+        float t = 0.f;
+        if (next[i] <= v) {
+          if (d.distill) {
+            const int* id = d.eid + (int64_t)row[i] * d.K;
+            const float* w = d.ew + (int64_t)row[i] * d.K;
+            while (next[i] <= v) {
+              if (next[i] == v) t += w[at[i]];
+              next[i] = ++at[i] < d.K ? id[at[i]] : kNoToken;
+            }
+          } else if (next[i] == v) {
+            t = d.weight;
+          }
+        }
+        if (GRAD) {
+          a.dx[((int64_t)blockIdx.y * d.V + v) * NR + i / 2 * 8 + 2 * lt + i % 2] =
+              row[i] < 0 ? 0.f : gr[i] * (head_ex2(z - lse2[i]) - t - d.share);
+        } else {
+          const float m = fmaxf(pt[i].m, z);
+          pt[i].s = pt[i].s * head_ex2(pt[i].m - m) + head_ex2(z - m);
+          if (m == -INFINITY) pt[i].s = 0.f;  // scores of -inf alone
+          pt[i].m = m;
+          if (t != 0.f) pt[i].dot = __fmaf_rn(t, z, pt[i].dot);
+          pt[i].sum += z;
+        }
+      }
+    }
+    g += hop;
   };
-  while (v0 < d.V) {
-    step(x[0]);
-    if (v0 >= d.V) break;
-    step(x[1]);
+  while (g < groups) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (g < groups) step(x[i]);
   }
   if (GRAD) return;
-  // the CTA's parts of a row: RV lanes of each warp
-  HeadPart* sp = reinterpret_cast<HeadPart*>(s_h);
-  __syncthreads();
-  if (lane % REP == 0) sp[(warp * RV + rv) * NR + n] = pt;
-  for (int k = W * RV / 2; k > 0; k /= 2) {
+  // the CTA's part of a row: 8 lanes of each warp, then the warps
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    HeadPart y = pt[i];
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2) {
+      HeadPart z;
+      z.m = __shfl_xor_sync(0xffffffffu, y.m, o);
+      z.s = __shfl_xor_sync(0xffffffffu, y.s, o);
+      z.dot = __shfl_xor_sync(0xffffffffu, y.dot, o);
+      z.sum = __shfl_xor_sync(0xffffffffu, y.sum, o);
+      y = lane & o ? head_add(z, y) : head_add(y, z);
+    }
+    if (lg == 0) s_part[warp][i / 2 * 8 + 2 * lt + i % 2] = y;
+  }
+  for (int k = W / 2; k > 0; k /= 2) {
     __syncthreads();
-    const int w = threadIdx.x / NR, i = threadIdx.x % NR;
+    const int w = threadIdx.x / NR, n = threadIdx.x % NR;
     HeadPart y;
-    if (w < k) y = head_add(sp[2 * w * NR + i], sp[(2 * w + 1) * NR + i]);
+    if (w < k) y = head_add(s_part[2 * w][n], s_part[2 * w + 1][n]);
     __syncthreads();
-    if (w < k) sp[w * NR + i] = y;
+    if (w < k) s_part[w][n] = y;
   }
   __syncthreads();
   if (threadIdx.x < NR && r0 + threadIdx.x < d.N)
-    a.part[(int64_t)(r0 + threadIdx.x) * gridDim.x + blockIdx.x] = sp[threadIdx.x];
+    a.part[(int64_t)(r0 + threadIdx.x) * gridDim.x + blockIdx.x] = s_part[0][threadIdx.x];
 }
 
 struct HeadGradDev {
   HeadDev d;
   int block;             // of NR rows
+  int64_t db;            // dx of the block: first element, and the distance of its rows
+  int ds;
   int lg;                // 2^lg threads (whole warps) along the width, the rest along the vocabulary
-  const float* dx;       // [row block][V][NR]
+  const float* dx;
   float* part;           // [part of the vocabulary][NR][D] of dh
 };
 
@@ -472,13 +522,13 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
       acc[i][0] = acc[i][1] = 0;
     }
   }
-  const float* dx = a.dx + (int64_t)a.block * d.V * NR;
+  const float* dx = a.dx + a.db;
   const int lane = threadIdx.x % 32;
   const int64_t v1 = (int64_t)d.V * (part + 1) / parts;
   int64_t v = (int64_t)d.V * part / parts;
   // U rows of the weight, and one of their score gradients per lane
   auto fetch = [&](float4 (&w)[U], float& x, int64_t at) {
-    x = lane < U * NR && at + lane / NR < v1 ? dx[at * NR + lane] : 0.f;
+    x = lane < U * NR && at + lane / NR < v1 ? dx[(at + lane / NR) * a.ds + lane % NR] : 0.f;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -574,17 +624,13 @@ __global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_consta
 
 // ---- host side -------------------------------------------------------------------
 
-template <int NR, int RV, bool GRAD>
+template <int NT, bool GRAD>
 Error launch_rows(HeadRowsDev& a, int ctas, cudaStream_t s) {
-  auto k = a.d.vec_w ? head_rows_kernel<NR, RV, true, GRAD> : head_rows_kernel<NR, RV, false, GRAD>;
-  const int smem = std::max<int>(NR * a.Dp * 4, kRowsThreads * (int)sizeof(HeadPart));
+  auto k = a.d.vec_w ? head_rows_kernel<NT, true, GRAD> : head_rows_kernel<NT, false, GRAD>;
+  const int smem = 8 * NT * (a.blocks + 1) * 64;
   allow_smem((const void*)k, smem);
-  return launch_after(k, dim3((unsigned)ctas, (unsigned)((a.d.N + NR - 1) / NR)), kRowsThreads, smem, s, "head rows kernel", a);
-}
-template <bool GRAD>
-Error rows_of(int nr, HeadRowsDev& a, int ctas, cudaStream_t s) {
-  return nr == 1 ? launch_rows<1, 8, GRAD>(a, ctas, s) : nr == 2 ? launch_rows<2, 8, GRAD>(a, ctas, s)
-         : nr == 4 ? launch_rows<4, 4, GRAD>(a, ctas, s) : launch_rows<8, 4, GRAD>(a, ctas, s);
+  return launch_after(k, dim3((unsigned)ctas, (unsigned)((a.d.N + 8 * NT - 1) / (8 * NT))), kFewThreads, smem, s,
+                      "head rows kernel", a);
 }
 
 template <int NR>
@@ -596,30 +642,22 @@ Error launch_grad(HeadGradDev& a, int splits, cudaStream_t s) {
                       "head gradient join kernel", a, splits * (256 >> a.lg));
 }
 
-// Rows per block: as many as share one read of the weight within the shared
-// memory, 8 at most.
-int few_rows(const HeadDev& d) {
-  const int Dp = (d.D + 127) / 128 * 128;
-  int nr = d.N >= 5 ? 8 : d.N >= 3 ? 4 : std::max(1, d.N);
-  while (nr > 1 && nr * Dp * 4 > kRowsSmem) nr /= 2;
-  return nr;
-}
-
 Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
   const int sms = current_device_info().sm_count;
   HeadRowsDev a;
   std::memset(static_cast<void*>(&a), 0, sizeof(a));
   a.d = d;
-  a.Dp = (d.D + 127) / 128 * 128;
-  const int nr = few_rows(d), blocks = (d.N + nr - 1) / nr;
-  const int ctas = std::max(sms / 2, 2 * sms / std::max(1, blocks));
+  a.blocks = (d.D + 15) / 16;
+  // 16 rows share one read of the weight where the shared memory holds them
+  const int nt = d.N > 8 && 16 * (a.blocks + 1) * 64 <= kRowsSmem ? 2 : 1, blocks = (d.N + 8 * nt - 1) / (8 * nt);
+  const int ctas = std::max(1, std::min(sms, (d.V + 15) / 16));
   Scratch mem;
   Error e;
   if (!backward) {
     e = mem.alloc(sizeof(HeadPart) * (size_t)d.N * ctas, s);
     if (!e.ok()) return e;
     a.part = mem.as<HeadPart>();
-    e = rows_of<false>(nr, a, ctas, s);
+    e = nt == 1 ? launch_rows<1, false>(a, ctas, s) : launch_rows<2, false>(a, ctas, s);
     if (e.ok()) e = head_join(d, a.part, ctas, 1, ctas, true, s);
     return e;
   }
@@ -629,17 +667,21 @@ Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
   g.lg = 5;
   while (g.lg < 8 && (1 << g.lg) < chunks) ++g.lg;
   const int splits = std::max(1, std::min((d.V + 31) / 32, 2 * sms / colblocks));
-  const size_t nd = ((size_t)d.V * nr * blocks + 3) / 4 * 4;
-  e = mem.alloc(sizeof(float) * (nd + (size_t)splits * (256 >> g.lg) * nr * d.D), s);
+  const size_t nd = (size_t)d.V * 8 * nt * blocks;
+  e = mem.alloc(sizeof(float) * (nd + (size_t)splits * (256 >> g.lg) * 8 * d.D), s);
   if (!e.ok()) return e;
   a.dx = mem.as<float>();
-  e = rows_of<true>(nr, a, ctas, s);
+  e = nt == 1 ? launch_rows<1, true>(a, ctas, s) : launch_rows<2, true>(a, ctas, s);
   g.d = d;
   g.dx = a.dx;
+  g.ds = 8 * nt;
   g.part = a.dx + nd;
-  for (g.block = 0; e.ok() && g.block < blocks; ++g.block)
+  const int nr = d.N <= 1 ? 1 : d.N <= 2 ? 2 : d.N <= 4 ? 4 : 8;
+  for (g.block = 0; e.ok() && g.block * nr < d.N; ++g.block) {
+    g.db = nt == 2 ? 8 * g.block : (int64_t)g.block * d.V * 8;
     e = nr == 1 ? launch_grad<1>(g, splits, s) : nr == 2 ? launch_grad<2>(g, splits, s)
         : nr == 4 ? launch_grad<4>(g, splits, s) : launch_grad<8>(g, splits, s);
+  }
   return e;
 }
 
@@ -742,7 +784,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (N == 0 && !d.dw) return Error{};
   // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
   // tensor-core path writes the zeros.
-  const bool few = N > 0 && N <= 16 && d.D <= kRowsSmem / 4;
+  const bool few = N > 0 && N <= 16 && 8 * (D + 32) * 4 <= kRowsSmem;
   // the rows' targets
   Scratch mem;
   const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;
