@@ -236,7 +236,6 @@ namespace {
 
 // ---- few rows ----------------------------------------------------------------------
 
-constexpr int kRowsSmem = 200 * 1024;
 
 __device__ __forceinline__ uint64_t pk(float a, float b) {
   uint64_t r;
@@ -315,7 +314,7 @@ constexpr int kAhead = 6;    // blocks of 16 columns in flight per warp
 // 16 from its rows l / 4 and l / 4 + 8, which are the elements that it supplies to
 // two MMAs (the order of the columns inside a block does not matter as long as
 // the hidden rows take the same).
-template <int NT, bool VEC, bool GRAD>
+template <int NT, bool GRAD>
 __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_constant__ HeadRowsDev a) {
   constexpr int W = kFewThreads / 32, NR = 8 * NT;
   extern __shared__ float s_h[];         // [NR][pitch]
@@ -332,17 +331,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int64_t v = (int64_t)gl * 16 + lg + 8 * j;
-      x[j] = v < d.V ? head_stream4<VEC>(d.w + v * d.wv, bl * 16 + lt * 4, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[j] = v < d.V ? head_load4<false>(d.w + v * d.wv, bl * 16 + lt * 4, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (++bl == a.blocks) {
       bl = 0;
       gl += hop;
     }
   };
+  pdl_wait();
   float4 x[kAhead][2];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) fetch(x[i]);
-  pdl_wait();
   if (threadIdx.x < NR) {
     const int r = r0 + threadIdx.x;
     s_row[threadIdx.x] = r < d.N && head_first_id(d, r) != kNoToken ? r : -1;
@@ -488,6 +487,283 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
     a.part[(int64_t)(r0 + threadIdx.x) * gridDim.x + blockIdx.x] = s_part[0][threadIdx.x];
 }
 
+// ---- few rows, the weight through a ring of bulk copies --------------------------------
+
+constexpr int kRingCols = 512;               // columns of a stage
+constexpr int kRingPitch = kRingCols + 16;   // so that two rows' 64 bytes lie in different banks
+constexpr int kRingStage = 16 * kRingPitch * 4;
+constexpr int kRingWarps = 16;
+constexpr int kRingThreads = kRingWarps * 32 + 32;
+constexpr int kRingSmem = 224 * 1024;
+
+enum RingMode { kRingScores, kRingScoreGrad, kRingGrad };
+
+struct HeadRingDev {
+  HeadDev d;
+  int blocks;            // the width in blocks of 16, rounded up
+  int chunks;            // stages of a group of 16 vocabulary rows
+  int stages;
+  HeadPart* part;        // kRingScores: [row][CTA]
+  float* dx;             // kRingScoreGrad: [row block][V][8 NT]
+  float* dh;             // kRingGrad: [CTA][8 NT][D]
+  int* err;
+};
+
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, int* failed) {
+  for (uint32_t i = 0; i < kWaitIters; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 63 && *(volatile int*)failed) return false;
+  }
+  atomicExch(failed, 1);
+  return false;
+}
+__device__ __forceinline__ void ring_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+
+// Up to 8 NT rows (blockIdx.y: which) against the whole vocabulary, 16 rows of it
+// at a time per CTA: a warp copies row segments of 2 KB into the ring, 16 warps
+// share a segment's columns, and their sums meet in shared memory.  kRingGrad: the
+// group stays in the ring until its dw has been written and its part of dh been
+// added, so that the weight is read once (widths up to 1024).
+template <int NT, int MODE>
+__global__ void __launch_bounds__(kRingThreads, 1) head_ring_kernel(const __grid_constant__ HeadRingDev a) {
+  constexpr int NR = 8 * NT;
+  extern __shared__ unsigned char smem_raw[];
+  const HeadDev& d = a.d;
+  float* ring = reinterpret_cast<float*>(smem_raw);                     // [stages][16][kRingPitch]
+  float* s_h = ring + a.stages * (kRingStage / 4);                      // [NR][pitch]
+  const int pitch = a.blocks * 16 + 16;
+  float4* red = reinterpret_cast<float4*>(s_h + NR * pitch);            // [2][NT][warps][32]: every warp's results of a group
+  float* s_dx = reinterpret_cast<float*>(red + 2 * NT * kRingWarps * 32);  // [16][NR]
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_dx + 16 * NR);
+  uint64_t* empty = full + a.stages;
+  __shared__ int s_row[NR], failed;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r0 = blockIdx.y * NR;
+  const int groups = (d.V + 15) / 16;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kRingWarps);
+    }
+    failed = 0;
+    fence_mbar_init();
+  }
+  // what no copy writes (columns behind the width, up to 16) meets zeros of the hidden rows: any number will do
+  for (int i = threadIdx.x; i < a.stages * (kRingStage / 16); i += kRingThreads)
+    reinterpret_cast<float4*>(ring)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  fence_proxy_async();
+  __syncthreads();
+  bool ok = true;
+  pdl_wait();
+  if (warp == kRingWarps) {  // copies
+    int li = 0;
+    for (int g = blockIdx.x; g < groups && ok; g += gridDim.x) {
+      const int rows = min(16, d.V - g * 16);
+      for (int c = 0; c < a.chunks; ++c, ++li) {
+        const int s = li % a.stages;
+        if (li >= a.stages && !(ok = __all_sync(0xffffffffu, ring_wait(&empty[s], (uint32_t)(li / a.stages - 1) & 1u, &failed)) != 0)) break;
+        const uint32_t bytes = (uint32_t)min(kRingCols, d.D - c * kRingCols) * 4;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes * rows);
+        __syncwarp();
+        if (lane < rows)
+          bulk_g2s(ring + s * (kRingStage / 4) + lane * kRingPitch, d.w + ((int64_t)g * 16 + lane) * d.wv + c * kRingCols, bytes, &full[s]);
+      }
+    }
+    if (!ok)  // what is under way lands before the CTA ends
+      for (int s = 0; s < a.stages && s < li; ++s) mbar_wait(&full[s], (uint32_t)((li - 1 - s) / a.stages) & 1u);
+  } else {
+    if (threadIdx.x < NR) {
+      const int r = r0 + threadIdx.x;
+      s_row[threadIdx.x] = r < d.N && head_first_id(d, r) != kNoToken ? r : -1;
+    }
+    ring_sync();
+    for (int i = threadIdx.x; i < NR * a.blocks * 4; i += kRingWarps * 32) {
+      const int n = i / (a.blocks * 4), c = i % (a.blocks * 4) * 4;
+      *reinterpret_cast<float4*>(&s_h[n * pitch + c]) =
+          s_row[n] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+          : d.vec_h    ? head_load4<true>(head_row<const float>(d, d.hid, s_row[n]), c, d.D, 1)
+                       : head_load4<false>(head_row<const float>(d, d.hid, s_row[n]), c, d.D, d.hid.sd);
+    }
+    ring_sync();
+    const int lg = lane / 4, lt = lane % 4;
+    // the first 16 NR threads finish a group: vocabulary row fv, call row fn
+    const int fn = threadIdx.x % NR, fv = threadIdx.x / NR;
+    const bool fin = fv < 16;
+    const int row = fin ? s_row[fn] : -1;
+    Entries ent;
+    ent.left = 0;
+    ent.next = kNoToken;
+    float lse2 = 0.f, gr = 0.f;
+    if (row >= 0) {
+      if (d.distill) ent.begin(d, row);
+      else ent.next = head_id(d, d.ids, row, 0);
+      if (MODE != kRingScores) {
+        lse2 = *head_row<const float>(d, d.lse, row) * kHeadLog2e;
+        gr = *head_row<const float>(d, d.gl, row) * d.temp;
+      }
+    }
+    HeadPart pt = {-INFINITY, 0.f, 0.f, 0.f};
+    const float f = d.inv_temp * kHeadLog2e;
+    // kRingGrad: two columns per thread
+    const int col = threadIdx.x * 2;
+    const bool mine = MODE == kRingGrad && col < d.D;
+    uint64_t hc[NR], acc[NR];
+    if (MODE == kRingGrad) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        hc[n] = mine ? pk(s_h[n * pitch + col], s_h[n * pitch + col + 1]) : 0;
+        acc[n] = 0;
+      }
+    }
+    int li = 0, k = 0;
+    for (int g = blockIdx.x; g < groups; g += gridDim.x, ++k) {
+      float sum[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] = 0.f;
+      const int first = li;
+      for (int c = 0; c < a.chunks; ++c, ++li) {
+        const int s = li % a.stages;
+        if (ok) ok = __all_sync(0xffffffffu, ring_wait(&full[s], (uint32_t)(li / a.stages) & 1u, &failed)) != 0;
+        const float* w = ring + s * (kRingStage / 4);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int b = warp * 2 + q, at = c * (kRingCols / 16) + b;  // block of the stage, of the width
+          if (at >= a.blocks) break;
+          uint32_t hi[2][4], lo[2][4];  // [columns 0 and 1, columns 2 and 3]
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4 y = *reinterpret_cast<const float4*>(&w[(lg + 8 * j) * kRingPitch + b * 16 + lt * 4]);
+            tf32_split(y.x, &hi[0][j], &lo[0][j]);
+            tf32_split(y.y, &hi[0][2 + j], &lo[0][2 + j]);
+            tf32_split(y.z, &hi[1][j], &lo[1][j]);
+            tf32_split(y.w, &hi[1][2 + j], &lo[1][2 + j]);
+          }
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const float4 h = *reinterpret_cast<const float4*>(&s_h[(i * 8 + lg) * pitch + at * 16 + lt * 4]);
+            uint32_t hh[4], hl[4];
+            tf32_split(h.x, &hh[0], &hl[0]);
+            tf32_split(h.y, &hh[1], &hl[1]);
+            tf32_split(h.z, &hh[2], &hl[2]);
+            tf32_split(h.w, &hh[3], &hl[3]);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              mma_tf32(sum[i], lo[p], hh[2 * p], hh[2 * p + 1]);
+              mma_tf32(sum[i], hi[p], hl[2 * p], hl[2 * p + 1]);
+              mma_tf32(sum[i], hi[p], hh[2 * p], hh[2 * p + 1]);
+            }
+          }
+        }
+        if (MODE != kRingGrad) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[s]);
+        }
+      }
+      float4* buf = red + (k & 1) * NT * kRingWarps * 32;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        buf[(i * kRingWarps + warp) * 32 + lane] = make_float4(sum[i][0], sum[i][1], sum[i][2], sum[i][3]);
+      ring_sync();
+      if (fin) {
+        // the result of (fv, fn) lies with lane (fv % 8) * 4 + fn % 8 / 2, element fv / 8 * 2 + fn % 2
+        const float* p = reinterpret_cast<const float*>(buf + fn / 8 * kRingWarps * 32 + (fv % 8) * 4 + fn % 8 / 2) + fv / 8 * 2 + fn % 2;
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRingWarps; ++i) z += p[i * 128];
+        z *= f;  // in units of log2
+        const int v = g * 16 + fv;
+        float x = 0.f;
+        if (v < d.V && row >= 0) {
+          float t = 0.f;
+          if (ent.next <= v) {
+            if (d.distill) {
+              ent.skip_to(v);
+              t = ent.take(v);
+            } else if (ent.next == v) {
+              t = d.weight;
+            }
+          }
+          if (MODE != kRingScores) {
+            x = gr * (head_ex2(z - lse2) - t - d.share);
+          } else {
+            const float m = fmaxf(pt.m, z);
+            pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(z - m);
+            if (m == -INFINITY) pt.s = 0.f;  // scores of -inf alone
+            pt.m = m;
+            if (t != 0.f) pt.dot = __fmaf_rn(t, z, pt.dot);
+            pt.sum += z;
+          }
+        }
+        if (MODE == kRingScoreGrad && v < d.V) a.dx[((int64_t)blockIdx.y * d.V + v) * NR + fn] = x;
+        if (MODE == kRingGrad) s_dx[fv * NR + fn] = x;
+      }
+      if (MODE != kRingGrad) continue;
+      ring_sync();
+      const int rows = min(16, d.V - g * 16);
+      if (mine) {
+        const float* w = ring + (first + col / kRingCols) % a.stages * (kRingStage / 4) + col % kRingCols;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+          const float2 y = *reinterpret_cast<const float2*>(&w[r * kRingPitch]);
+          const uint64_t w2 = pk(y.x, y.y);
+          uint64_t o = 0;
+#pragma unroll
+          for (int n = 0; n < NR; n += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&s_dx[r * NR + n]);
+            const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint64_t xx = pk(xs[i], xs[i]);
+              acc[n + i] = fma2(xx, w2, acc[n + i]);
+              o = fma2(xx, hc[n + i], o);
+            }
+          }
+          if (!d.dw) continue;
+          float o0, o1;
+          upk(o, &o0, &o1);
+          float* to = d.dw + ((int64_t)g * 16 + r) * d.dwv;
+          if (d.vec_dw) {
+            __stcs(reinterpret_cast<float2*>(to + col), make_float2(o0, o1));
+          } else {
+            to[col * d.dwd] = o0;
+            if (col + 1 < d.D) to[(col + 1) * d.dwd] = o1;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0)
+        for (int c = 0; c < a.chunks; ++c) mbar_arrive(&empty[(first + c) % a.stages]);
+    }
+    if (MODE == kRingScores) {
+      // the CTA's part of a row: 16 threads, folded in the order of their vocabulary rows
+      HeadPart* sp = reinterpret_cast<HeadPart*>(red);
+      ring_sync();
+      if (fin) sp[fv * NR + fn] = pt;
+      for (int n = 8; n > 0; n /= 2) {
+        ring_sync();
+        HeadPart y;
+        if (fv < n) y = head_add(sp[2 * fv * NR + fn], sp[(2 * fv + 1) * NR + fn]);
+        ring_sync();
+        if (fv < n) sp[fv * NR + fn] = y;
+      }
+      if (fv == 0 && r0 + fn < d.N) a.part[(int64_t)(r0 + fn) * gridDim.x + blockIdx.x] = sp[fn];
+    }
+    if (mine && d.dh.p) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        float x0, x1;
+        upk(acc[n], &x0, &x1);
+        float* to = a.dh + ((int64_t)blockIdx.x * NR + n) * d.D + col;
+        to[0] = x0;
+        if (col + 1 < d.D) to[1] = x1;
+      }
+    }
+  }
+  if (lane == 0 && !ok) atomicOr(a.err, kAsyncWaitTimeout);
+}
+
 struct HeadGradDev {
   HeadDev d;
   int block;             // of NR rows
@@ -626,11 +902,33 @@ __global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_consta
 
 template <int NT, bool GRAD>
 Error launch_rows(HeadRowsDev& a, int ctas, cudaStream_t s) {
-  auto k = a.d.vec_w ? head_rows_kernel<NT, true, GRAD> : head_rows_kernel<NT, false, GRAD>;
+  auto k = head_rows_kernel<NT, GRAD>;
   const int smem = 8 * NT * (a.blocks + 1) * 64;
   allow_smem((const void*)k, smem);
   return launch_after(k, dim3((unsigned)ctas, (unsigned)((a.d.N + 8 * NT - 1) / (8 * NT))), kFewThreads, smem, s,
                       "head rows kernel", a);
+}
+
+int ring_fixed(int nt, int blocks) {  // shared memory besides the stages
+  return 8 * nt * (blocks + 1) * 64 + 2 * nt * kRingWarps * 512 + 16 * 8 * nt * 4 + 16 * 16;
+}
+template <int NT, int MODE>
+Error launch_ring(HeadRingDev& a, int ctas, cudaStream_t s) {
+  auto k = head_ring_kernel<NT, MODE>;
+  const int fixed = ring_fixed(NT, a.blocks);
+  a.chunks = (a.d.D + kRingCols - 1) / kRingCols;
+  a.stages = std::min(8, (kRingSmem - fixed) / kRingStage);
+  const int smem = fixed + a.stages * kRingStage;
+  allow_smem((const void*)k, smem);
+  a.err = async_error_word();
+  if (!a.err) return make_error(TRS_ERR_CUDA, "head: no async-error word");
+  return launch_after(k, dim3((unsigned)ctas, (unsigned)((a.d.N + 8 * NT - 1) / (8 * NT))), kRingThreads, smem, s,
+                      "head ring kernel", a);
+}
+template <int NT>
+Error launch_ring(HeadRingDev& a, int mode, int ctas, cudaStream_t s) {
+  return mode == kRingScores ? launch_ring<NT, kRingScores>(a, ctas, s)
+         : mode == kRingGrad ? launch_ring<NT, kRingGrad>(a, ctas, s) : launch_ring<NT, kRingScoreGrad>(a, ctas, s);
 }
 
 template <int NR>
@@ -644,25 +942,44 @@ Error launch_grad(HeadGradDev& a, int splits, cudaStream_t s) {
 
 Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
   const int sms = current_device_info().sm_count;
+  const int width = (d.D + 15) / 16;
+  // 16 rows share one read of the weight where the shared memory holds them
+  const int nt = d.N > 8 && ring_fixed(2, width) + 2 * kRingStage <= kRingSmem ? 2 : 1, blocks = (d.N + 8 * nt - 1) / (8 * nt);
+  const int ctas = std::max(1, std::min(sms, (d.V + 15) / 16));
   HeadRowsDev a;
   std::memset(static_cast<void*>(&a), 0, sizeof(a));
   a.d = d;
-  a.blocks = (d.D + 15) / 16;
-  // 16 rows share one read of the weight where the shared memory holds them
-  const int nt = d.N > 8 && 16 * (a.blocks + 1) * 64 <= kRowsSmem ? 2 : 1, blocks = (d.N + 8 * nt - 1) / (8 * nt);
-  const int ctas = std::max(1, std::min(sms, (d.V + 15) / 16));
+  a.blocks = width;
+  HeadRingDev r;
+  std::memset(static_cast<void*>(&r), 0, sizeof(r));
+  r.d = d;
+  r.blocks = width;
   Scratch mem;
   Error e;
   if (!backward) {
     e = mem.alloc(sizeof(HeadPart) * (size_t)d.N * ctas, s);
     if (!e.ok()) return e;
-    a.part = mem.as<HeadPart>();
-    e = nt == 1 ? launch_rows<1, false>(a, ctas, s) : launch_rows<2, false>(a, ctas, s);
-    if (e.ok()) e = head_join(d, a.part, ctas, 1, ctas, true, s);
+    a.part = r.part = mem.as<HeadPart>();
+    if (d.vec_w) e = nt == 1 ? launch_ring<1>(r, kRingScores, ctas, s) : launch_ring<2>(r, kRingScores, ctas, s);
+    else e = nt == 1 ? launch_rows<1, false>(a, ctas, s) : launch_rows<2, false>(a, ctas, s);
+    if (e.ok()) e = head_join(d, r.part, ctas, 1, ctas, true, s);
     return e;
   }
   HeadGradDev g;
   std::memset(static_cast<void*>(&g), 0, sizeof(g));
+  g.d = d;
+  // both stages of a group and the next one's first in the ring
+  if (d.vec_w && d.D <= 2 * kRingCols && blocks == 1 &&
+      ring_fixed(nt, width) + (d.D <= kRingCols ? 2 : 3) * kRingStage <= kRingSmem) {
+    e = mem.alloc(sizeof(float) * (size_t)ctas * 8 * nt * d.D, s);
+    if (!e.ok()) return e;
+    g.part = r.dh = mem.as<float>();
+    e = nt == 1 ? launch_ring<1>(r, kRingGrad, ctas, s) : launch_ring<2>(r, kRingGrad, ctas, s);
+    if (!e.ok() || !d.dh.p) return e;
+    const dim3 grid((unsigned)((d.D + 31) / 32), (unsigned)d.N);
+    return nt == 1 ? launch_after(head_grad_join_kernel<8>, grid, 256, 0, s, "head gradient join kernel", g, ctas)
+                   : launch_after(head_grad_join_kernel<16>, grid, 256, 0, s, "head gradient join kernel", g, ctas);
+  }
   const int chunks = (d.D + 3) / 4, colblocks = (d.D + 1023) / 1024;
   g.lg = 5;
   while (g.lg < 8 && (1 << g.lg) < chunks) ++g.lg;
@@ -670,9 +987,9 @@ Error run_rows(const HeadDev& d, bool backward, cudaStream_t s) {
   const size_t nd = (size_t)d.V * 8 * nt * blocks;
   e = mem.alloc(sizeof(float) * (nd + (size_t)splits * (256 >> g.lg) * 8 * d.D), s);
   if (!e.ok()) return e;
-  a.dx = mem.as<float>();
-  e = nt == 1 ? launch_rows<1, true>(a, ctas, s) : launch_rows<2, true>(a, ctas, s);
-  g.d = d;
+  a.dx = r.dx = mem.as<float>();
+  if (d.vec_w) e = nt == 1 ? launch_ring<1>(r, kRingScoreGrad, ctas, s) : launch_ring<2>(r, kRingScoreGrad, ctas, s);
+  else e = nt == 1 ? launch_rows<1, true>(a, ctas, s) : launch_rows<2, true>(a, ctas, s);
   g.dx = a.dx;
   g.ds = 8 * nt;
   g.part = a.dx + nd;
@@ -784,7 +1101,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (N == 0 && !d.dw) return Error{};
   // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
   // tensor-core path writes the zeros.
-  const bool few = N > 0 && N <= 16 && 8 * (D + 32) * 4 <= kRowsSmem;
+  const bool few = N > 0 && N <= 16 && D <= 4096;
   // the rows' targets
   Scratch mem;
   const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;
