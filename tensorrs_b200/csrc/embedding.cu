@@ -20,7 +20,7 @@
 //                       (key, token): two launches up to V = 2^18.  Every CTA
 //                       finds its places from all tiles' counts (no CTA waits on
 //                       another), and counts the next digit as it writes.
-//   emb_sum_kernel      32 sorted positions per group of lanes: rows of one key
+//   emb_sum_kernel      up to 32 sorted positions per group of lanes: rows of one key
 //                       are added in f64 in registers and written at the end of
 //                       the run; a run that crosses into other positions leaves
 //                       partial sums
@@ -71,6 +71,7 @@ struct EmbDev {
   double* part;          // [group of positions][2][D]
   uint32_t tiles, groups;
   int digits, bits;
+  int positions;         // sorted positions per group of lanes, a power of two up to 32
 };
 
 __device__ __forceinline__ uint32_t emb_key(const EmbDev& d, uint32_t r) {
@@ -137,7 +138,6 @@ constexpr int kSortTile = 4096;              // tokens per CTA
 constexpr int kBins = 512;
 constexpr int kWarps = kSortThreads / 32;
 constexpr int kRounds = kSortTile / kSortThreads;  // a warp's share: rounds of 32 consecutive tokens
-constexpr int kPositions = 32;               // sorted positions per group of lanes
 
 // The part `share` of `shares` of the zeros, by the CTAs behind the tiles'.
 template <class T, int V>
@@ -267,16 +267,27 @@ __device__ __forceinline__ T emb_result(const EmbDev& d, double sum, T before) {
 template <class T, int V>
 __global__ void __launch_bounds__(kEmbThreads) emb_sum_kernel(const EmbDev d) {
   constexpr int U = 8;  // rows in flight
+  __shared__ uint32_t s_key[kEmbThreads], s_tok[kEmbThreads];
   pdl_launch_dependents();
   pdl_wait();
-  const int L = 1 << d.l.lg, per = kEmbThreads >> d.l.lg, c0 = threadIdx.x & (L - 1);
+  const int L = 1 << d.l.lg, per = kEmbThreads >> d.l.lg, c0 = threadIdx.x & (L - 1), P = d.positions;
   const uint32_t* key = d.key[d.digits & 1];
   const uint32_t* tok = d.tok[d.digits & 1];
-  const uint32_t g = blockIdx.x * per + (threadIdx.x >> d.l.lg);
+  // the CTA's positions, at most one per thread: groups of few lanes take fewer positions
+  const uint64_t first = (uint64_t)blockIdx.x * per * P;
+  for (int i = threadIdx.x; i < per * P; i += kEmbThreads) {
+    const bool there = first + i < d.N;
+    s_key[i] = there ? key[first + i] : ~0u;
+    s_tok[i] = there ? tok[first + i] : 0;
+  }
+  __syncthreads();
+  const int lg = threadIdx.x >> d.l.lg;  // group in the CTA
+  const uint32_t g = blockIdx.x * per + lg;
   if (g >= d.groups) return;
-  const uint32_t p0 = g * kPositions, p1 = min(p0 + kPositions, d.N);
-  const uint32_t prev = p0 > 0 ? key[p0 - 1] : ~0u, next = p1 < d.N ? key[p1] : ~0u;
-  const uint32_t head = key[p0], tail = key[p1 - 1];
+  const uint32_t p0 = g * P, n = min((uint32_t)P, d.N - p0);
+  const uint32_t *keys = s_key + lg * P, *toks = s_tok + lg * P;
+  const uint32_t prev = p0 > 0 ? key[p0 - 1] : ~0u, next = p0 + n < d.N ? key[p0 + n] : ~0u;
+  const uint32_t head = keys[0], tail = keys[n - 1];
   if (head == d.V) return;
   // a run that begins here and goes on
   if (c0 == 0 && tail == next && tail != d.V && !(head == tail && prev == head))
@@ -301,14 +312,14 @@ __global__ void __launch_bounds__(kEmbThreads) emb_sum_kernel(const EmbDev d) {
         store<T, V>(row, c, d.td, x);
       }
     };
-    for (uint32_t p = p0; p < p1; p += U) {
+    for (uint32_t p = 0; p < n; p += U) {
       uint32_t k[U];
       Vec<T, V> x[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j) k[j] = p + j < p1 ? key[p + j] : d.V;
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (k[j] < d.V) x[j] = load<T, V>(row_at<T>(d, tok[p + j]), c, d.rows.sd);
+      for (int j = 0; j < U; ++j) {
+        k[j] = p + j < n ? keys[p + j] : d.V;
+        if (k[j] < d.V) x[j] = load<T, V>(row_at<T>(d, toks[p + j]), c, d.rows.sd);
+      }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         if (k[j] >= d.V) continue;  // sorted last: nothing follows
@@ -327,46 +338,59 @@ __global__ void __launch_bounds__(kEmbThreads) emb_sum_kernel(const EmbDev d) {
   }
 }
 
-// Runs that cross from one group of positions into others: 32 lanes of columns
+// Runs that cross from one group of positions into others: 32 lanes times C columns
 // times 8 parts of the run, folded in order.
 template <class T>
 __global__ void __launch_bounds__(256) emb_join_kernel(const EmbDev d) {
-  __shared__ double s[8][32];
+  constexpr int C = 2;
+  __shared__ double s[8][32 * C];
   pdl_wait();
   const uint32_t* key = d.key[d.digits & 1];
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32, blocks = (d.D + 31) / 32;
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32, blocks = (d.D + 32 * C - 1) / (32 * C), P = d.positions;
   const uint32_t n = d.crossing[0];
   for (uint64_t item = blockIdx.x; item < (uint64_t)n * blocks; item += gridDim.x) {
     const uint32_t g = d.crossing[1 + item / blocks];
-    const int c = (int)(item % blocks) * 32 + lane;
-    const uint32_t k = key[g * kPositions + kPositions - 1];
-    // the groups behind g that begin with the key: [g + 1, end)
-    uint32_t lo = g + 2, hi = d.groups;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (key[mid * kPositions] == k) lo = mid + 1; else hi = mid;
-    }
-    const uint32_t cnt = lo - g;  // parts: group g's second slot, then the first slots
-    const uint32_t a = (uint32_t)((uint64_t)cnt * w / 8), b = (uint32_t)((uint64_t)cnt * (w + 1) / 8);
-    double sum = 0.0;
-    if (c < d.D) {
-      for (uint32_t i = a; i < b; i += 4) {
-        double x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[j] = i + j < b ? d.part[((uint64_t)(g + i + j) * 2 + (i + j == 0 ? 1 : 0)) * d.D + c] : 0.0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum = __dadd_rn(sum, x[j]);
+    const int c = (int)(item % blocks) * 32 * C + lane;
+    const uint32_t k = key[(uint64_t)g * P + P - 1];
+    // the groups behind g that begin with the key, 32 at a time
+    uint32_t end = g + 1;
+    for (;; end += 32) {
+      const uint32_t at = end + lane;
+      const uint32_t same = __ballot_sync(0xffffffffu, at < d.groups && key[(uint64_t)at * P] == k);
+      if (same != ~0u) {
+        end += __ffs(~same) - 1;
+        break;
       }
     }
+    const uint32_t cnt = end - g;  // parts: group g's second slot, then the first slots
+    const uint32_t a = (uint32_t)((uint64_t)cnt * w / 8), b = (uint32_t)((uint64_t)cnt * (w + 1) / 8);
+    double sum[C];
+#pragma unroll
+    for (int e = 0; e < C; ++e) sum[e] = 0.0;
+    for (uint32_t i = a; i < b; i += 4) {
+      double x[4][C];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < C; ++e)
+          x[j][e] = i + j < b && c + 32 * e < d.D ? d.part[((uint64_t)(g + i + j) * 2 + (i + j == 0 ? 1 : 0)) * d.D + c + 32 * e] : 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < C; ++e) sum[e] = __dadd_rn(sum[e], x[j][e]);
+    }
     __syncthreads();
-    s[w][lane] = sum;
+#pragma unroll
+    for (int e = 0; e < C; ++e) s[w][32 * e + lane] = sum[e];
     __syncthreads();
-    if (w == 0 && c < d.D) {
-      sum = s[0][lane];
-      for (int i = 1; i < 8; ++i) sum = __dadd_rn(sum, s[i][lane]);
-      T* to = reinterpret_cast<T*>(d.grad) + (int64_t)k * d.tv + (int64_t)c * d.td;
-      *to = emb_result<T>(d, sum, d.accumulate ? *to : (T)0);
+    if (threadIdx.x < 32 * C) {
+      const int col = (int)(item % blocks) * 32 * C + threadIdx.x;
+      if (col < d.D) {
+        double all = s[0][threadIdx.x];
+        for (int i = 1; i < 8; ++i) all = __dadd_rn(all, s[i][threadIdx.x]);
+        T* to = reinterpret_cast<T*>(d.grad) + (int64_t)k * d.tv + (int64_t)col * d.td;
+        *to = emb_result<T>(d, all, d.accumulate ? *to : (T)0);
+      }
     }
   }
 }
@@ -404,7 +428,12 @@ Error launch_backward(EmbDev& d, cudaStream_t s) {
   d.digits = (vbits + 8) / 9;
   d.bits = (vbits + d.digits - 1) / d.digits;
   d.tiles = (uint32_t)(((uint64_t)d.N + kSortTile - 1) / kSortTile);
-  d.groups = (uint32_t)(((uint64_t)d.N + kPositions - 1) / kPositions);
+  const int sms = current_device_info().sm_count;
+  // as many positions per group as still leave two CTAs of groups per SM, and as fit a CTA's threads
+  d.positions = 32;
+  while (d.positions > 8 && (uint64_t)d.N / d.positions < ((uint64_t)2 * sms << 8 >> d.l.lg)) d.positions /= 2;
+  while ((d.positions << 8 >> d.l.lg) > kEmbThreads) d.positions /= 2;
+  d.groups = (uint32_t)(((uint64_t)d.N + d.positions - 1) / d.positions);
   const size_t n = ((size_t)d.N + 3) / 4 * 4, h = (size_t)d.tiles * kBins;
   Scratch mem, part;
   Error e = mem.alloc(sizeof(uint32_t) * (4 * n + d.digits * h + d.groups + 4), s);
@@ -416,7 +445,6 @@ Error launch_backward(EmbDev& d, cudaStream_t s) {
   for (int i = 0; i < d.digits; ++i, at += h) d.hist[i] = at;
   d.crossing = at;
   d.part = part.as<double>();
-  const int sms = current_device_info().sm_count;
   const unsigned zeros = d.accumulate || d.V == 0 ? 0u : 2u * sms;
   if (d.tiles + zeros == 0) return Error{};
   emb_keys_kernel<T, V><<<d.tiles + zeros, kSortThreads, 0, s>>>(d);
@@ -427,8 +455,8 @@ Error launch_backward(EmbDev& d, cudaStream_t s) {
   const unsigned per = kEmbThreads >> d.l.lg;
   e = launch_after(emb_sum_kernel<T, V>, dim3((d.groups + per - 1) / per), kEmbThreads, 0, s, "embedding sum kernel", d);
   if (!e.ok() || d.groups < 2) return e;
-  const uint64_t most = (uint64_t)d.groups * ((d.D + 31) / 32);
-  return launch_after(emb_join_kernel<T>, dim3((unsigned)std::min<uint64_t>(most, 4u * sms)), 256, 0, s,
+  const uint64_t most = (uint64_t)d.groups * ((d.D + 63) / 64);
+  return launch_after(emb_join_kernel<T>, dim3((unsigned)std::min<uint64_t>(most, 8u * sms)), 256, 0, s,
                       "embedding join kernel", d);
 }
 

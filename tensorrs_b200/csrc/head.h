@@ -59,6 +59,17 @@ __device__ __forceinline__ T* head_row(const HeadDev& d, const RowsDev& r, int i
   return static_cast<T*>(r.p) + b * r.sb + t * r.st;
 }
 
+__device__ __forceinline__ int head_id(const HeadDev& d, const RowsDev& ids, int row, int k) {
+  const int64_t at = k * ids.sd;
+  const int64_t v = d.ids64 ? head_row<const int64_t>(d, ids, row)[at] : head_row<const int32_t>(d, ids, row)[at];
+  return v < 0 || v >= d.V ? kNoToken : (int)v;
+}
+
+// The first of a row's tokens in order (kNoToken: the row has no target).
+__device__ __forceinline__ int head_first_id(const HeadDev& d, int row) {
+  return d.distill ? d.eid[(int64_t)row * d.K] : head_id(d, d.ids, row, 0);
+}
+
 // The walk of one row's entries along ascending tokens.
 struct Entries {
   const int* id;
@@ -76,9 +87,17 @@ struct Entries {
     ++id;
     next = --left > 0 ? *id : kNoToken;
   }
-  // skips entries below v
+  // skips entries below v, which may be all of them
   __device__ __forceinline__ void skip_to(int v) {
-    while (next < v) step();
+    int lo = 0, hi = left;  // entries before `lo` are below v, those from `hi` on are not
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (id[mid] < v) lo = mid + 1; else hi = mid;
+    }
+    id += lo;
+    w += lo;
+    left -= lo;
+    next = left > 0 ? *id : kNoToken;
   }
   // the weight of token v, which next may have reached
   __device__ __forceinline__ float take(int v) {
@@ -97,11 +116,24 @@ struct Entries {
 struct HeadPart {
   float m, s, dot, sum;
 };
-// part p of live row r lies at p * sp + r * sr
+__device__ __forceinline__ HeadPart head_add(const HeadPart& a, const HeadPart& b) {
+  HeadPart r;
+  r.m = fmaxf(a.m, b.m);
+  // a part of -inf alone has no sum; and scores of -inf alone stay one
+  const float base = r.m == -INFINITY ? 0.f : r.m;
+  r.s = a.s * exp2f(a.m - base) + b.s * exp2f(b.m - base);
+  r.dot = a.dot + b.dot;
+  r.sum = a.sum + b.sum;
+  return r;
+}
+
+// part p of live row r (few: of the call's row r) lies at p * sp + r * sr
 Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
                 cudaStream_t stream);
 
-// The tensor-core path (head_tc.cu).
+// Up to 16 rows of widths up to 4096 (head_few.cu).
+Error head_few(const HeadDev& d, bool backward, cudaStream_t stream);
+// More rows, or none (head_tc.cu).
 Error head_tc(const HeadDev& d, bool backward, cudaStream_t stream);
 
 }  // namespace trs
