@@ -20,6 +20,7 @@
 //                       (key, token): two launches up to V = 2^18.  Every CTA
 //                       finds its places from all tiles' counts (no CTA waits on
 //                       another), and counts the next digit as it writes.
+//   emb_sort_one_kernel the keys and all digits in one launch, for up to 4096 tokens
 //   emb_sum_kernel      up to 32 sorted positions per group of lanes: rows of one key
 //                       are added in f64 in registers and written at the end of
 //                       the run; a run that crosses into other positions leaves
@@ -179,11 +180,72 @@ __global__ void __launch_bounds__(kSortThreads) emb_keys_kernel(const EmbDev d) 
   d.hist[0][blockIdx.x * kBins + threadIdx.x] = count[threadIdx.x];
 }
 
+// The lanes whose bin (of `bits` bits) is this lane's, among those that are `there`
+// (a ballot per bit: several times as fast as match.any).
+__device__ __forceinline__ uint32_t emb_peers(uint32_t bin, bool there, int bits) {
+  uint32_t peers = __ballot_sync(0xffffffffu, there);
+  for (int i = 0; i < bits; ++i) {
+    const uint32_t set = __ballot_sync(0xffffffffu, (bin >> i) & 1u);
+    peers &= (bin >> i) & 1u ? set : ~set;
+  }
+  return peers;
+}
+
+// What a CTA's stable sort by one digit shares: a warp's tokens of every bin, then
+// where they go.
+struct SortShared {
+  uint32_t at[kWarps][kBins];
+  uint32_t sums[kWarps];
+};
+
+// rank[i]: the place of this thread's token of round i among its warp's tokens of the
+// bin; at: how many each warp has.
+__device__ __forceinline__ void emb_rank(SortShared& sh, const uint32_t (&bin)[kRounds], const bool (&there)[kRounds], int bits,
+                                         uint32_t (&rank)[kRounds]) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sh.at[w][threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const uint32_t peers = emb_peers(bin[i], there[i], bits);
+    uint32_t have = 0;
+    if (there[i]) have = sh.at[warp][bin[i]];
+    __syncwarp();
+    rank[i] = have + __popc(peers & ((1u << lane) - 1));
+    if (there[i] && lane == __ffs(peers) - 1) sh.at[warp][bin[i]] = have + __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+}
+
+// at: the first place of each warp's tokens of this thread's bin, given how many of
+// the bin there are in all and before this tile.
+__device__ __forceinline__ void emb_places(SortShared& sh, uint32_t total, uint32_t before) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint32_t scan = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += y;
+  }
+  if (lane == 31) sh.sums[warp] = scan;
+  __syncthreads();
+  uint32_t place = scan - total + before;
+  for (int w = 0; w < warp; ++w) place += sh.sums[w];
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const uint32_t n = sh.at[w][threadIdx.x];
+    sh.at[w][threadIdx.x] = place;
+    place += n;
+  }
+  __syncthreads();
+}
+
 // Sorts by digit p, stable; from buffer p % 2 into the other one.
 template <class T, int V>
 __global__ void __launch_bounds__(kSortThreads) emb_sort_kernel(const EmbDev d, int p) {
-  __shared__ uint32_t at[kWarps][kBins];
-  __shared__ uint32_t sums[kWarps];
+  __shared__ SortShared sh;
   pdl_launch_dependents();
   if (blockIdx.x >= d.tiles) {
     emb_zeros<T, V>(d, p + 1, d.digits + 1);
@@ -191,68 +253,89 @@ __global__ void __launch_bounds__(kSortThreads) emb_sort_kernel(const EmbDev d, 
     return;
   }
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) at[w][threadIdx.x] = 0;
   pdl_wait();
-  __syncthreads();
   const uint32_t mask = (1u << d.bits) - 1, shift = p * d.bits;
   const uint64_t first = (uint64_t)blockIdx.x * kSortTile + warp * (32 * kRounds);
-  uint32_t key[kRounds];
+  uint32_t key[kRounds], tok[kRounds], bin[kRounds], rank[kRounds];
+  bool there[kRounds];
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
     const uint64_t r = first + i * 32 + lane;
-    key[i] = r < d.N ? d.key[p & 1][r] : 0;
+    there[i] = r < d.N;
+    key[i] = there[i] ? d.key[p & 1][r] : 0;
+    tok[i] = p == 0 ? (uint32_t)r : there[i] ? d.tok[p & 1][r] : 0;
+    bin[i] = (key[i] >> shift) & mask;
   }
-  // where this tile's tokens of the bin go: all smaller bins, then the earlier tiles
+  // this thread's bin: all tiles' tokens, and those of the earlier tiles
   uint32_t total = 0, before = 0;
   for (uint32_t t = 0; t < d.tiles; ++t) {
     const uint32_t n = d.hist[p][t * kBins + threadIdx.x];
     total += n;
     before += t < blockIdx.x ? n : 0;
   }
-  uint32_t scan = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += y;
-  }
-  if (lane == 31) sums[warp] = scan;
-  // tokens of each warp and bin
-#pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const bool there = first + i * 32 + lane < d.N;
-    const uint32_t bin = there ? (key[i] >> shift) & mask : ~0u;
-    const uint32_t peers = __match_any_sync(0xffffffffu, bin);
-    if (there && lane == __ffs(peers) - 1) at[warp][bin] += __popc(peers);
-    __syncwarp();
-  }
-  __syncthreads();
-  uint32_t place = scan - total + before;
-  for (int w = 0; w < warp; ++w) place += sums[w];
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const uint32_t n = at[w][threadIdx.x];
-    at[w][threadIdx.x] = place;
-    place += n;
-  }
-  __syncthreads();
+  emb_rank(sh, bin, there, d.bits, rank);
+  emb_places(sh, total, before);
   const bool last = p + 1 == d.digits;
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
-    const uint64_t r = first + i * 32 + lane;
-    const bool there = r < d.N;
-    const uint32_t bin = there ? (key[i] >> shift) & mask : ~0u;
-    const uint32_t peers = __match_any_sync(0xffffffffu, bin);
-    uint32_t to = 0;
-    if (there) to = at[warp][bin] + __popc(peers & ((1u << lane) - 1));
-    __syncwarp();
-    if (there && lane == __ffs(peers) - 1) at[warp][bin] += __popc(peers);
-    __syncwarp();
-    if (there) {
-      d.key[(p + 1) & 1][to] = key[i];
-      d.tok[(p + 1) & 1][to] = p == 0 ? (uint32_t)r : d.tok[p & 1][r];
-      if (!last) atomicAdd(&d.hist[p + 1][to / kSortTile * kBins + ((key[i] >> (shift + d.bits)) & mask)], 1u);
+    if (!there[i]) continue;
+    const uint32_t to = sh.at[warp][bin[i]] + rank[i];
+    d.key[(p + 1) & 1][to] = key[i];
+    d.tok[(p + 1) & 1][to] = tok[i];
+    if (!last) atomicAdd(&d.hist[p + 1][to / kSortTile * kBins + ((key[i] >> (shift + d.bits)) & mask)], 1u);
+  }
+}
+
+// All of it in one launch for tokens of one tile; the zeros by the other CTAs.
+template <class T, int V>
+__global__ void __launch_bounds__(kSortThreads) emb_sort_one_kernel(const EmbDev d) {
+  extern __shared__ uint32_t s_raw[];
+  pdl_launch_dependents();
+  if (blockIdx.x >= 1) {
+    emb_zeros<T, V>(d, 0, 1);
+    return;
+  }
+  SortShared& sh = *reinterpret_cast<SortShared*>(s_raw);
+  uint32_t* s_key = s_raw + sizeof(SortShared) / 4;
+  uint32_t* s_tok = s_key + kSortTile;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t mask = (1u << d.bits) - 1, first = warp * (32 * kRounds) + lane;
+  uint32_t key[kRounds], tok[kRounds], bin[kRounds], rank[kRounds];
+  bool there[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    tok[i] = first + i * 32;
+    there[i] = tok[i] < d.N;
+    key[i] = there[i] ? emb_key(d, tok[i]) : 0;
+  }
+  if (threadIdx.x == 0) d.crossing[0] = 0;
+  for (int p = 0; p < d.digits; ++p) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) bin[i] = (key[i] >> (p * d.bits)) & mask;
+    emb_rank(sh, bin, there, d.bits, rank);
+    uint32_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += sh.at[w][threadIdx.x];
+    emb_places(sh, total, 0);
+    const bool last = p + 1 == d.digits;
+    uint32_t* keys = last ? d.key[d.digits & 1] : s_key;
+    uint32_t* toks = last ? d.tok[d.digits & 1] : s_tok;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      if (!there[i]) continue;
+      const uint32_t to = sh.at[warp][bin[i]] + rank[i];
+      keys[to] = key[i];
+      toks[to] = tok[i];
     }
+    __syncthreads();
+    if (last) break;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i)
+      if (there[i]) {
+        key[i] = s_key[first + i * 32];
+        tok[i] = s_tok[first + i * 32];
+      }
+    __syncthreads();
   }
 }
 
@@ -447,10 +530,18 @@ Error launch_backward(EmbDev& d, cudaStream_t s) {
   d.part = part.as<double>();
   const unsigned zeros = d.accumulate || d.V == 0 ? 0u : 2u * sms;
   if (d.tiles + zeros == 0) return Error{};
-  emb_keys_kernel<T, V><<<d.tiles + zeros, kSortThreads, 0, s>>>(d);
-  e = check_launch("embedding keys kernel");
-  for (int p = 0; e.ok() && p < d.digits; ++p)
-    e = launch_after(emb_sort_kernel<T, V>, dim3(d.tiles + zeros), kSortThreads, 0, s, "embedding sort kernel", d, p);
+  if (d.tiles == 1) {
+    auto k = emb_sort_one_kernel<T, V>;
+    const int smem = (int)sizeof(SortShared) + 2 * kSortTile * 4;
+    allow_smem((const void*)k, smem);
+    k<<<1 + zeros, kSortThreads, smem, s>>>(d);
+    e = check_launch("embedding sort kernel");
+  } else {
+    emb_keys_kernel<T, V><<<d.tiles + zeros, kSortThreads, 0, s>>>(d);
+    e = check_launch("embedding keys kernel");
+    for (int p = 0; e.ok() && p < d.digits; ++p)
+      e = launch_after(emb_sort_kernel<T, V>, dim3(d.tiles + zeros), kSortThreads, 0, s, "embedding sort kernel", d, p);
+  }
   if (!e.ok() || d.N == 0) return e;
   const unsigned per = kEmbThreads >> d.l.lg;
   e = launch_after(emb_sum_kernel<T, V>, dim3((d.groups + per - 1) / per), kEmbThreads, 0, s, "embedding sum kernel", d);
