@@ -136,17 +136,6 @@ __global__ void __launch_bounds__(1024) head_list_kernel(const HeadDev d) {
   if (threadIdx.x == 0) *d.live = done;
 }
 
-// Gradients of rows without a target.
-__global__ void __launch_bounds__(256) head_masked_kernel(const HeadDev d) {
-  pdl_launch_dependents();
-  pdl_wait();
-  for (int row = blockIdx.x * 8 + threadIdx.x / 32; row < d.N; row += gridDim.x * 8) {
-    if (d.eid[(int64_t)row * d.K] != kNoToken) continue;
-    float* to = head_row<float>(d, d.dh, row);
-    for (int64_t c = threadIdx.x % 32; c < d.D; c += 32) to[c * d.dh.sd] = 0.f;
-  }
-}
-
 // ---- joining the parts of the vocabulary -------------------------------------------
 
 // LR rows per CTA times 256 / LR threads along a row's parts, folded in a fixed
@@ -325,11 +314,6 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (few) return head_few(d, c.backward, stream);
   e = launch_after(head_list_kernel, dim3(1), 1024, 0, stream, "head list kernel", d);
   if (!e.ok()) return e;
-  if (c.grad_hidden && N > 0) {
-    e = launch_after(head_masked_kernel, dim3((unsigned)std::min<int64_t>((N + 7) / 8, 1024)), 256, 0, stream,
-                     "head masked rows kernel", d);
-    if (!e.ok()) return e;
-  }
   return head_tc(d, c.backward, stream);
 }
 

@@ -3,7 +3,7 @@
 //
 // Products.  f32 operands are written 2^e (hi + lo) with hi and lo in fp16, 11
 // bits each, e placing the largest magnitude in [2^14, 2^15): of a hidden row,
-// of a piece of the weight, of all rows of g h.  A product is hi hi + (hi lo + lo
+// of 256 rows of the weight, of 256 rows of g h.  A product is hi hi + (hi lo + lo
 // hi), three tcgen05.mma with f32 accumulation.  The gradient of the scores
 // without the row's own factor, softmax(x) - t, lies in [-1, 1] and is split under
 // the fixed 2^15; the factor g temperature goes into g h for dw and onto the
@@ -11,7 +11,7 @@
 // The tensor core cuts its sums instead of rounding them, so a sum leaves the
 // accumulator for f32 registers every 256 elements.
 //
-//   head_pack_*       the planes [hi, lo] of hidden rows (those with a target,
+//   head_pack_kernel  the planes [hi, lo] of hidden rows (those with a target,
 //                     gathered), of a piece of the weight and of g h
 //   head_gemm_kernel  persistent CTA pairs, 256 x 256 tiles: a warp streams
 //                     64-element slabs of both operands by TMA, one warp issues
@@ -58,11 +58,13 @@ __device__ __forceinline__ float mul3(float a, float b, float c) {
 struct PlanesDev {
   HeadDev d;
   __half* to;            // [2][rows][Dp]
+  __half* gto;           // hidden rows with a gradient: the planes of g temperature h, alike
   int64_t plane;         // elements of a plane
   int Dp;                // the width rounded up to whole slabs of 64
-  float* down;           // hidden: 2^e of every row; weight, g h: one
-  uint32_t* top;         // largest magnitude, as bits
+  float* down;           // 2^e: hidden rows: of every row; weight: of every 256 rows
+  float* gdown;          // g h: of every 256 rows
   int v0, n;             // weight: the piece's first row and its rows
+  int along_v;           // weight: tokens are the denser dimension
 };
 
 // 2^k and 2^-k that bring a largest magnitude (its bits) into [2^14, 2^15),
@@ -73,14 +75,10 @@ __device__ __forceinline__ void plane_scale(uint32_t top, float* up, float* down
   *up = __uint_as_float((uint32_t)(k + 127) << 23);
   *down = __uint_as_float((uint32_t)(127 - k) << 23);
 }
-__device__ __forceinline__ uint32_t block_top(uint32_t x, uint32_t* sm) {  // 256 threads
-  x = __reduce_max_sync(0xffffffffu, x);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = x;
-  __syncthreads();
-  return __reduce_max_sync(0xffffffffu, sm[threadIdx.x % 8]);
-}
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t magnitude(const float4& x) {
+  return max(max(magnitude(x.x), magnitude(x.y)), max(magnitude(x.z), magnitude(x.w)));
+}
 
 __device__ __forceinline__ float4 piece4(const float* p, int c, int D, int64_t sd, bool vec) {
   if (vec && c < D) return *reinterpret_cast<const float4*>(p + c);
@@ -103,127 +101,151 @@ __device__ __forceinline__ void split_store(__half* to, int64_t plane, float a, 
   *reinterpret_cast<uint2*>(to + plane) = *reinterpret_cast<uint2*>(l);
 }
 
-// Hidden rows with a target, gathered: a CTA per row; zeros behind the last one up
-// to a whole tile.  With a gradient also the largest |g temperature h|.
-__global__ void __launch_bounds__(256) head_pack_hidden_kernel(const __grid_constant__ PlanesDev a) {
-  __shared__ uint32_t sm[8];
-  pdl_launch_dependents();
-  pdl_wait();
-  const HeadDev& d = a.d;
-  const int live = *d.live, r = blockIdx.x;
-  if (r >= (live + 255) / 256 * 256) return;
-  const float* p = r < live ? head_row<const float>(d, d.hid, d.rows[r]) : nullptr;
-  uint32_t top = 0;
-  if (p)
-    for (int c = threadIdx.x * 4; c < d.D; c += 1024) {
-      const float4 x = piece4(p, c, d.D, d.hid.sd, d.vec_h);
-      top = max(max(top, max(magnitude(x.x), magnitude(x.y))), max(magnitude(x.z), magnitude(x.w)));
-    }
-  top = block_top(top, sm);
-  float up, down;
-  plane_scale(top, &up, &down);
-  if (threadIdx.x == 0) {
-    a.down[r] = down;
-    if (a.top && p) {
-      const float g = *head_row<const float>(d, d.gl, d.rows[r]) * d.temp;
-      atomicMax(a.top, magnitude(g * __uint_as_float(top)));
-    }
-  }
-  for (int c = threadIdx.x * 4; c < a.Dp; c += 1024) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p) x = piece4(p, c, d.D, d.hid.sd, d.vec_h);
-    split_store(a.to + (int64_t)r * a.Dp + c, a.plane, x.x * up, x.y * up, x.z * up, x.w * up);
-  }
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address, in the cluster's shared memory, of `p` of CTA `rank`
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
 }
 
-// g temperature h of the same rows, under one power of two.
-__global__ void __launch_bounds__(256) head_pack_grad_kernel(const __grid_constant__ PlanesDev a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const HeadDev& d = a.d;
-  const int live = *d.live, r = blockIdx.x;
-  float up, down;
-  plane_scale(*a.top, &up, &down);
-  if (r == 0 && threadIdx.x == 0) *a.down = down;
-  if (r >= (live + 255) / 256 * 256) return;
-  const float* p = r < live ? head_row<const float>(d, d.hid, d.rows[r]) : nullptr;
-  const float g = p ? *head_row<const float>(d, d.gl, d.rows[r]) * d.temp : 0.f;
-  for (int c = threadIdx.x * 4; c < a.Dp; c += 1024) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p) x = piece4(p, c, d.D, d.hid.sd, d.vec_h);
-    split_store(a.to + (int64_t)r * a.Dp + c, a.plane, mul3(x.x, g, up), mul3(x.y, g, up), mul3(x.z, g, up),
-                mul3(x.w, g, up));
-  }
-}
+// Planes of 256 rows by a cluster of 8 CTAs, 32 rows each: the largest
+// magnitudes first, which the cluster shares, then the same rows again out of L2.
+// Hidden rows (those with a target, gathered; zeros behind the last one up to a
+// whole tile) have a power of two each, g h and the weight one per 256 rows: as
+// much as the products that contract along the rows keep in the accumulator.
+// Bound by HBM: 131 MB of weight in 58 us (262 MB read and written; 98 MB in 44 us).
+enum PackKind { kPackWeight, kPackHidden, kPackHiddenGrad };
 
-// The largest magnitude of a piece of the weight.  Threads run along whichever
-// dimension is the denser one.
-__global__ void __launch_bounds__(256) head_weight_top_kernel(const __grid_constant__ PlanesDev a, int along_v) {
-  __shared__ uint32_t sm[8];
-  pdl_launch_dependents();
-  pdl_wait();
-  const HeadDev& d = a.d;
-  const float* w = d.w + (int64_t)a.v0 * d.wv;
-  uint32_t top = 0;
-  if (along_v) {
-    for (int c = blockIdx.x; c < d.D; c += gridDim.x)
-      for (int v = threadIdx.x; v < a.n; v += 256) top = max(top, magnitude(w[v * d.wv + c * d.wd]));
-  } else {
-    // a warp per row, four loads in flight per lane
-    const int lane4 = threadIdx.x % 32 * 4;
-    for (int v = blockIdx.x * 8 + threadIdx.x / 32; v < a.n; v += gridDim.x * 8)
-      for (int c = lane4; c < d.D; c += 512) {
-        float4 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = piece4(w + v * d.wv, c + 128 * j, d.D, d.wd, d.vec_w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          top = max(max(top, max(magnitude(x[j].x), magnitude(x[j].y))), max(magnitude(x[j].z), magnitude(x[j].w)));
-      }
-  }
-  top = block_top(top, sm);
-  if (threadIdx.x == 0) atomicMax(a.top, top);
-}
-
-// A piece of the weight: row by row, or, where tokens are the dense dimension,
-// 32 x 32 tiles through shared memory.
-__global__ void __launch_bounds__(256) head_pack_weight_kernel(const __grid_constant__ PlanesDev a, int along_v) {
+template <int KIND, int W>
+__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(W * 32) head_pack_kernel(const __grid_constant__ PlanesDev a) {
+  constexpr int R = 32 / W;              // rows of a warp
+  __shared__ uint32_t warp_top[W], tops[8];
   __shared__ float tile[32][33];
+  const HeadDev& d = a.d;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const uint32_t rank = cta_rank();
+  const int t256 = blockIdx.x / 8, r0 = blockIdx.x * 32 + warp * R;  // this warp's rows
   pdl_launch_dependents();
   pdl_wait();
-  const HeadDev& d = a.d;
-  float up, down;
-  plane_scale(*a.top, &up, &down);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.down = down;
-  const float* w = d.w + (int64_t)a.v0 * d.wv;
-  if (!along_v) {
-    // a warp per row, four loads in flight per lane
-    const int lane4 = threadIdx.x % 32 * 4;
-    for (int v = blockIdx.x * 8 + threadIdx.x / 32; v < a.n; v += gridDim.x * 8)
-      for (int c = lane4; c < a.Dp; c += 512) {
-        float4 x[4];
+  if (KIND == kPackHiddenGrad && d.dh.p) {  // rows without a target have no gradient
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = piece4(w + v * d.wv, c + 128 * j, d.D, d.wd, d.vec_w);
+    for (int j = 0; j < R; ++j) {
+      if (r0 + j >= d.N || d.eid[(int64_t)(r0 + j) * d.K] != kNoToken) continue;
+      float* to = head_row<float>(d, d.dh, r0 + j);
+      for (int64_t c = lane; c < d.D; c += 32) to[c * d.dh.sd] = 0.f;
+    }
+  }
+  int rows = a.n;
+  if (KIND != kPackWeight) {
+    rows = *d.live;
+    if (t256 * 256 >= rows) {  // the whole cluster
+      if (KIND == kPackHiddenGrad && t256 == 0 && threadIdx.x == 0) a.gdown[0] = 1.f;
+      return;
+    }
+  }
+  const bool along_v = KIND == kPackWeight && a.along_v;
+  const int64_t sd = KIND == kPackWeight ? d.wd : d.hid.sd;
+  const bool vec = KIND == kPackWeight ? d.vec_w : d.vec_h;
+  const float* p[R];
+  float g[R];
+  uint32_t top[R], all = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + 128 * j < a.Dp)
-            split_store(a.to + (int64_t)v * a.Dp + c + 128 * j, a.plane, x[j].x * up, x[j].y * up, x[j].z * up, x[j].w * up);
-      }
+  for (int j = 0; j < R; ++j) {
+    p[j] = nullptr;
+    g[j] = 0.f;
+    top[j] = 0;
+    if (r0 + j >= rows) continue;
+    if (KIND == kPackWeight) {
+      p[j] = d.w + (int64_t)(a.v0 + r0 + j) * d.wv;
+    } else {
+      const int row = d.rows[r0 + j];
+      p[j] = head_row<const float>(d, d.hid, row);
+      if (KIND == kPackHiddenGrad) g[j] = *head_row<const float>(d, d.gl, row) * d.temp;
+    }
+  }
+  if (along_v) {
+    const int v = blockIdx.x * 32 + lane;
+    const float* w = d.w + (int64_t)(a.v0 + v) * d.wv;
+    if (v < rows)
+#pragma unroll 4
+      for (int c = warp; c < d.D; c += W) all = max(all, magnitude(w[c * d.wd]));
+  } else {
+#pragma unroll 8
+    for (int c = lane * 4; c < d.D; c += 128) {
+      float4 x[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j) x[j] = p[j] ? piece4(p[j], c, d.D, sd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < R; ++j) top[j] = max(top[j], magnitude(x[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      top[j] = __reduce_max_sync(0xffffffffu, top[j]);
+      all = max(all, KIND == kPackHiddenGrad ? magnitude(g[j] * __uint_as_float(top[j])) : top[j]);
+    }
+  }
+  float up = 1.f, down = 1.f;  // of the 256 rows
+  if (KIND != kPackHidden) {
+    all = __reduce_max_sync(0xffffffffu, all);
+    if (lane == 0) warp_top[warp] = all;
+    __syncthreads();
+    if (threadIdx.x < 8) {
+      uint32_t x = warp_top[0];
+      for (int i = 1; i < W; ++i) x = max(x, warp_top[i]);
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&tops[rank], threadIdx.x)), "r"(x) : "memory");
+    }
+    cluster_sync();
+    all = tops[0];
+    for (int i = 1; i < 8; ++i) all = max(all, tops[i]);
+    plane_scale(all, &up, &down);
+    if (rank == 0 && threadIdx.x == 0) (KIND == kPackWeight ? a.down : a.gdown)[t256] = down;
+  }
+  if (along_v) {  // 32 x 32 tiles through shared memory
+    const int v = blockIdx.x * 32;
+    for (int c0 = 0; c0 < a.Dp; c0 += 32) {
+      __syncthreads();
+      for (int i = warp; i < 32; i += W)
+        tile[i][lane] = v + lane < rows && c0 + i < d.D ? d.w[(int64_t)(a.v0 + v + lane) * d.wv + (c0 + i) * d.wd] : 0.f;
+      __syncthreads();
+      const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
+      if (threadIdx.x < 256 && v + r < rows)
+        split_store(a.to + (int64_t)(v + r) * a.Dp + c0 + c, a.plane, tile[c][r] * up, tile[c + 1][r] * up, tile[c + 2][r] * up,
+                    tile[c + 3][r] * up);
+    }
     return;
   }
-  const int tv = (a.n + 31) / 32, tc = a.Dp / 32;
-  for (int64_t t = blockIdx.x; t < (int64_t)tv * tc; t += gridDim.x) {
-    const int v0 = (int)(t % tv) * 32, c0 = (int)(t / tv) * 32;
-    __syncthreads();
-    for (int i = threadIdx.x / 32; i < 32; i += 8) {
-      const int v = v0 + threadIdx.x % 32, c = c0 + i;
-      tile[i][threadIdx.x % 32] = v < a.n && c < d.D ? w[v * d.wv + c * d.wd] : 0.f;
+  float ups[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) ups[j] = up;
+  if (KIND != kPackWeight) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      float dn;
+      plane_scale(top[j], &ups[j], &dn);
+      if (lane == 0) a.down[r0 + j] = dn;
     }
-    __syncthreads();
-    const int v = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
-    if (v0 + v < a.n)
-      split_store(a.to + (int64_t)(v0 + v) * a.Dp + c0 + c, a.plane, tile[c][v] * up, tile[c + 1][v] * up,
-                  tile[c + 2][v] * up, tile[c + 3][v] * up);
+  }
+#pragma unroll 4
+  for (int c = lane * 4; c < a.Dp; c += 128) {
+    float4 x[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) x[j] = p[j] ? piece4(p[j], c, d.D, sd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if (KIND == kPackWeight && !p[j]) continue;
+      const int64_t at = (int64_t)(r0 + j) * a.Dp + c;
+      split_store(a.to + at, a.plane, x[j].x * ups[j], x[j].y * ups[j], x[j].z * ups[j], x[j].w * ups[j]);
+      if (KIND == kPackHiddenGrad && a.gto)
+        split_store(a.gto + at, a.plane, mul3(x[j].x, g[j], up), mul3(x[j].y, g[j], up), mul3(x[j].z, g[j], up), mul3(x[j].w, g[j], up));
+    }
   }
 }
 
@@ -236,7 +258,7 @@ constexpr int kSlab = 64;                    // elements of the contraction per 
 constexpr int kABytes = 2 * 128 * 128, kBBytes = 2 * BR * 128;
 constexpr int kStage = kABytes + kBBytes;
 constexpr int kStages = 3;
-constexpr int kChunk = 4;                    // slabs per accumulator
+constexpr int kChunk = 4;                    // slabs per accumulator: the 256 rows that share a power of two
 constexpr int kGemmThreads = 384;
 constexpr int kPitch = 17;                   // a warp's buffer: 32 rows of 16 columns
 constexpr int kWarpBuf = 32 * kPitch * 4;
@@ -244,20 +266,6 @@ constexpr int kGemmSmem = kStages * kStage + 8 * kWarpBuf + 1024 + 256;
 constexpr int kLean = 56, kFull = 224;       // 128 * 56 + 256 * 224 = 384 * 168 registers
 static_assert(128 * kLean + 256 * kFull == kGemmThreads * 168, "all of the registers");
 
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void pair_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// the address, in the pair's shared memory, of `p` of CTA `rank`
-__device__ __forceinline__ uint32_t pair_addr(const void* p, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  return a;
-}
 // (Release at the CTA's scope: what it says is read lies in tensor memory, and its
 // loads have completed; at the cluster's scope it would wait for the stores of the
 // tile before.)
@@ -328,9 +336,9 @@ enum HeadMode { kScores, kScoreGrad, kProducts };
 struct GemmDev {
   HeadDev d;
   int v0, Vc, Vcp;       // the piece of the vocabulary, rounded up to whole tiles
-  const float* hdown;    // 2^e of the hidden rows, the piece, g h
-  const float* wdown;
-  const float* gdown;
+  const float* hdown;    // 2^e: of the hidden rows
+  const float* wdown;    // of every 256 rows of the piece
+  const float* gdown;    // of every 256 rows of g h
   HeadPart* part;        // kScores: [column half tile][ld]
   __half* dx;            // kScoreGrad: [2][Np][ld]
   int64_t ld, plane;
@@ -409,6 +417,11 @@ __device__ __forceinline__ uint64_t pk(float a, float b) {
 }
 __device__ __forceinline__ void upk(uint64_t x, float* a, float* b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 __device__ __forceinline__ void store8(void* to, const uint32_t (&x)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]),
@@ -536,15 +549,13 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
     float* to = nullptr;   // the row's column col
     int64_t sd = 1;
     bool wide, add = false;
-    float f1, f2 = 1.f;
+    float f2 = 1.f;
     const int width = min(128, d.D - col);
     if (w.dw) {
       if (row < g.Vc) to = d.dw + (int64_t)(g.v0 + row) * d.dwv + (int64_t)col * d.dwd;
       sd = d.dwd;
       wide = g.wide_dw;
-      f1 = *g.gdown * 0x1p-15f;
     } else {
-      f1 = *g.wdown * 0x1p-15f;
       sd = d.dh.sd;
       wide = g.wide_dh;
       add = g.add;
@@ -568,7 +579,7 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
         if (i >= width) continue;
         uint32_t x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(acc[i + j] * f1 * f2);
+        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(acc[i + j] * f2);
         if (add) {
           const float4 a = *reinterpret_cast<const float4*>(to + i), b = *reinterpret_cast<const float4*>(to + i + 4);
           const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -583,7 +594,7 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
         if (i >= width) continue;
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) buf[lane * kPitch + j] = acc[i + j] * f1 * f2;
+        for (int j = 0; j < 16; ++j) buf[lane * kPitch + j] = acc[i + j] * f2;
         __syncwarp();
         const int c = lane % 16;
 #pragma unroll 4
@@ -599,7 +610,7 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
 #pragma unroll
       for (int i = 0; i < 128; ++i) {
         if (i >= width) continue;
-        const float x = acc[i] * f1 * f2;
+        const float x = acc[i] * f2;
         to[i * sd] = add ? to[i * sd] + x : x;
       }
     }
@@ -639,7 +650,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   if (warp == 0) pair_tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
-  pair_sync();  // the other CTA's barriers are there before anything arrives on them
+  cluster_sync();  // the other CTA's barriers are there before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();
@@ -658,7 +669,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
           const int s = li % kStages;
           if (li >= kStages && !(ok = wait_or_fail(&empty[s], (uint32_t)(li / kStages - 1) & 1u, failed))) break;
           if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * kStage);
-          const uint32_t bar = pair_addr(&full[s], 0);
+          const uint32_t bar = cluster_addr(&full[s], 0);
           unsigned char* a = smem + s * kStage;
           const int k = (w.k0 + i) * kSlab, m = w.m0 + rank * 128, n = w.n0 + rank * (w.cols / CG);
           if (MODE != kProducts) {
@@ -724,7 +735,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFull));
     const int half = warp / 4, rl = (warp % 4) * 32 + lane;
     const uint32_t src = tmem + ((uint32_t)((warp % 4) * 32) << 16) + half * 128;
-    const uint32_t bars[2] = {pair_addr(&tempty[0], 0), pair_addr(&tempty[1], 0)};
+    const uint32_t bars[2] = {cluster_addr(&tempty[0], 0), cluster_addr(&tempty[1], 0)};
     int ci = 0;
     bool ok = true;
     for (int item = pair; item < items && ok; item += pairs) {
@@ -739,7 +750,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
         t.orig = g.d.rows[t.row];
         if (MODE != kProducts) {
           // a power of two and the factor onto units of log2: neither 0 nor inf
-          t.f = fminf(fmaxf(mul3(g.hdown[t.row], *g.wdown, g.d.inv_temp * kHeadLog2e), 0x1p-126f), FLT_MAX);
+          t.f = fminf(fmaxf(mul3(g.hdown[t.row], g.wdown[w.n0 / BN], g.d.inv_temp * kHeadLog2e), 0x1p-126f), FLT_MAX);
           const int* ids = g.d.eid + (int64_t)t.orig * g.d.K;
           int hi = g.d.K;
           while (t.e < hi) {
@@ -754,6 +765,12 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
       for (int i = 0; i < w.n; i += kChunk, ++ci) {
+        // the powers of two of the 256 rows that the chunk contracted along, and of dx
+        uint64_t scale2 = 0;
+        if (MODE == kProducts) {
+          const float f = (w.dw ? g.gdown : g.wdown)[(w.k0 + i) / kChunk] * 0x1p-15f;
+          scale2 = pk(f, f);
+        }
         ok = __all_sync(0xffffffffu, wait_or_fail(&tfull[ci & 1], (uint32_t)(ci / 2) & 1u, failed)) != 0;
         if (!ok) break;
         tc_fence_after();
@@ -764,9 +781,8 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
           tmem_ld_done(x);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const uint64_t y = add2(pk(acc[cc * 32 + j], acc[cc * 32 + j + 1]),
-                                    pk(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
-            upk(y, &acc[cc * 32 + j], &acc[cc * 32 + j + 1]);
+            const uint64_t now = pk(acc[cc * 32 + j], acc[cc * 32 + j + 1]), more = pk(__uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+            upk(MODE == kProducts ? fma2(more, scale2, now) : add2(now, more), &acc[cc * 32 + j], &acc[cc * 32 + j + 1]);
           }
         }
         tc_fence_before();
@@ -780,7 +796,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  pair_sync();
+  cluster_sync();
   tc_fence_after();
   if (warp == 0) pair_tmem_dealloc(tmem, 512);
 }
@@ -896,7 +912,7 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     const int64_t part = std::max<int64_t>(512, work / std::max(1, sms / CG) / 3);
     g.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Vp + part / 2) / part));
   }
-  g.slabs = (int)((Vp / kSlab + g.splits - 1) / g.splits);
+  g.slabs = (int)round_up((Vp / kSlab + g.splits - 1) / g.splits, kChunk);
   g.dh_first = Vp / g.splits >= d.N;
 
   // workspaces
@@ -909,18 +925,15 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     at += (size_t)round_up(bytes, 256);
     return here;
   };
-  const size_t o_small = take(4 * (4 + pieces) * 2), o_hdown = take(4 * Np), o_h = take(4 * hplane), o_w = take(4 * wplane);
+  const int64_t tiles256 = Vp * pieces / BN;
+  const size_t o_wdown = take(4 * tiles256), o_gdown = take(4 * (Np / 256)), o_hdown = take(4 * Np), o_h = take(4 * hplane),
+               o_w = take(4 * wplane);
   const size_t o_gh = take(backward && d.dw ? 4 * hplane : 0), o_x = take(4 * xplane);
   const size_t o_part = take(backward ? 0 : (int64_t)sizeof(HeadPart) * parts * Np);
   const size_t o_dh = take(g.splits > 1 ? 4 * g.splits * Np * dtiles * BN : 0);
   Error e = mem.alloc(at, s);
   if (!e.ok()) return e;
   char* base = mem.as<char>();
-  // largest magnitudes: of g h, then of every piece; their powers of two likewise
-  uint32_t* tops = reinterpret_cast<uint32_t*>(base + o_small);
-  float* downs = reinterpret_cast<float*>(tops + 4 + pieces);
-  cudaError_t ce = cudaMemsetAsync(tops, 0, 4 * (4 + pieces), s);
-  if (ce != cudaSuccess) return cuda_error(ce, "head clear");
   __half *hp = reinterpret_cast<__half*>(base + o_h), *wp = reinterpret_cast<__half*>(base + o_w);
   __half *gp = reinterpret_cast<__half*>(base + o_gh), *xp = reinterpret_cast<__half*>(base + o_x);
 
@@ -929,19 +942,16 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   p.d = d;
   p.Dp = (int)Dp;
   p.to = hp;
+  p.gto = backward && d.dw ? gp : nullptr;
   p.plane = hplane;
   p.down = reinterpret_cast<float*>(base + o_hdown);
-  p.top = backward && d.dw ? tops : nullptr;
-  e = launch_after(head_pack_hidden_kernel, dim3((unsigned)Np), 256, 0, s, "head hidden planes kernel", p);
-  if (e.ok() && p.top) {
-    p.to = gp;
-    p.down = downs;
-    e = launch_after(head_pack_grad_kernel, dim3((unsigned)Np), 256, 0, s, "head gradient planes kernel", p);
-  }
+  p.gdown = reinterpret_cast<float*>(base + o_gdown);
+  e = backward ? launch_after(head_pack_kernel<kPackHiddenGrad, 32>, dim3((unsigned)(Np / 32)), 1024, 0, s, "head hidden planes kernel", p)
+               : launch_after(head_pack_kernel<kPackHidden, 32>, dim3((unsigned)(Np / 32)), 1024, 0, s, "head hidden planes kernel", p);
   if (!e.ok()) return e;
 
   g.hdown = reinterpret_cast<float*>(base + o_hdown);
-  g.gdown = downs;
+  g.gdown = p.gdown;
   g.part = reinterpret_cast<HeadPart*>(base + o_part);
   g.ld = backward ? Vp : Np;
   g.dx = xp;
@@ -956,22 +966,20 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   g.wide_dw = d.dw && d.D % 8 == 0 && wide(d.dw, {d.dwv}, d.dwd);
   g.wide_dh = d.dh.p && d.D % 8 == 0 && wide(d.dh.p, {d.dh.sb, d.dh.st}, d.dh.sd);
   const int64_t av = d.wv < 0 ? -d.wv : d.wv, ad = d.wd < 0 ? -d.wd : d.wd;
-  const int along_v = d.V > 1 && d.D > 1 && av < ad;
+  p.along_v = d.V > 1 && d.D > 1 && av < ad;
+  p.gto = nullptr;
   for (int64_t i = 0; i < pieces; ++i) {
     g.v0 = (int)(i * Vp);
     g.Vc = (int)std::min<int64_t>(Vp, d.V - i * Vp);
     g.Vcp = (int)round_up(g.Vc, BN);
-    g.wdown = downs + 4 + i;
     g.add = i > 0;
     p.to = wp;
     p.plane = wplane;
-    p.top = tops + 4 + i;
-    p.down = downs + 4 + i;
+    p.down = reinterpret_cast<float*>(base + o_wdown) + i * (Vp / BN);
+    g.wdown = p.down;
     p.v0 = g.v0;
     p.n = g.Vc;
-    const unsigned ctas = (unsigned)(along_v ? 8 * sms : std::min<int64_t>((g.Vc + 7) / 8, 8 * sms));
-    e = launch_after(head_weight_top_kernel, dim3(ctas), 256, 0, s, "head weight maximum kernel", p, along_v);
-    if (e.ok()) e = launch_after(head_pack_weight_kernel, dim3(ctas), 256, 0, s, "head weight planes kernel", p, along_v);
+    e = launch_after(head_pack_kernel<kPackWeight, 16>, dim3((unsigned)(g.Vcp / 32)), 16 * 32, 0, s, "head weight planes kernel", p);
     CUtensorMap ha, wb, xa, wc, xc, gc;
     if (e.ok()) e = map_rows(hp, Np, Dp, hplane, 128, &ha);
     if (e.ok()) e = map_rows(wp, g.Vc, Dp, wplane, BR, &wb);
