@@ -288,6 +288,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
     }
   }
   d.vec_h = N > 0 && rows_vectors(c.hidden);
+  d.vec_dh = N > 0 && c.grad_hidden && rows_vectors(c.grad_hidden);
   if (N == 0 && !d.dw) return Error{};
   // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
   // tensor-core path writes the zeros.

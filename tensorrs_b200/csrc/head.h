@@ -44,7 +44,7 @@ struct HeadDev {
   int* eid;                      // [N][K] tokens of a row's entries, ascending, kNoToken behind them
   float* ew;                     // [N][K] their weights
   float* ent;                    // [N] sum of w ln w (distillation)
-  int vec_h, vec_w, vec_dw;  // 16-byte accesses along D
+  int vec_h, vec_w, vec_dh, vec_dw;  // 16-byte accesses along D
 };
 
 __device__ __forceinline__ float head_ex2(float x) {

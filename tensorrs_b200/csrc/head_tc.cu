@@ -124,17 +124,17 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
 // Bound by HBM: 131 MB of weight in 58 us (262 MB read and written; 98 MB in 44 us).
 enum PackKind { kPackWeight, kPackHidden, kPackHiddenGrad };
 
-template <int KIND, int W>
-__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(W * 32) head_pack_kernel(const __grid_constant__ PlanesDev a) {
-  constexpr int R = 32 / W;              // rows of a warp
+constexpr int kPackWarps = 16;
+
+template <int KIND>
+__device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
+  constexpr int W = kPackWarps, R = 32 / W;  // R: rows of a warp
   __shared__ uint32_t warp_top[W], tops[8];
   __shared__ float tile[32][33];
   const HeadDev& d = a.d;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t rank = cta_rank();
-  const int t256 = blockIdx.x / 8, r0 = blockIdx.x * 32 + warp * R;  // this warp's rows
-  pdl_launch_dependents();
-  pdl_wait();
+  const int t256 = block / 8, r0 = block * 32 + warp * R;  // this warp's rows
   if (KIND == kPackHiddenGrad && d.dh.p) {  // rows without a target have no gradient
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -172,7 +172,7 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(W * 32) head_pack_ke
     }
   }
   if (along_v) {
-    const int v = blockIdx.x * 32 + lane;
+    const int v = block * 32 + lane;
     const float* w = d.w + (int64_t)(a.v0 + v) * d.wv;
     if (v < rows)
 #pragma unroll 4
@@ -209,7 +209,7 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(W * 32) head_pack_ke
     if (rank == 0 && threadIdx.x == 0) (KIND == kPackWeight ? a.down : a.gdown)[t256] = down;
   }
   if (along_v) {  // 32 x 32 tiles through shared memory
-    const int v = blockIdx.x * 32;
+    const int v = block * 32;
     for (int c0 = 0; c0 < a.Dp; c0 += 32) {
       __syncthreads();
       for (int i = warp; i < 32; i += W)
@@ -249,6 +249,17 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(W * 32) head_pack_ke
   }
 }
 
+// The hidden rows (clusters below `hidden`, HKIND; none: a later piece) next to a
+// piece of the weight.
+template <int HKIND>
+__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(kPackWarps * 32)
+head_pack_kernel(const __grid_constant__ PlanesDev h, const __grid_constant__ PlanesDev w, int hidden) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if ((int)blockIdx.x < hidden) pack_rows<HKIND>(h, blockIdx.x);
+  else pack_rows<kPackWeight>(w, blockIdx.x - hidden);
+}
+
 // ---- pieces of the pair's plumbing ---------------------------------------------------
 
 constexpr int CG = 2;                        // CTAs of a pair
@@ -260,8 +271,7 @@ constexpr int kStage = kABytes + kBBytes;
 constexpr int kStages = 3;
 constexpr int kChunk = 4;                    // slabs per accumulator: the 256 rows that share a power of two
 constexpr int kGemmThreads = 384;
-constexpr int kPitch = 17;                   // a warp's buffer: 32 rows of 16 columns
-constexpr int kWarpBuf = 32 * kPitch * 4;
+constexpr int kWarpBuf = 32 * 128;           // a warp's buffer: 128 bytes of 32 rows
 constexpr int kGemmSmem = kStages * kStage + 8 * kWarpBuf + 1024 + 256;
 constexpr int kLean = 56, kFull = 224;       // 128 * 56 + 256 * 224 = 384 * 168 registers
 static_assert(128 * kLean + 256 * kFull == kGemmThreads * 168, "all of the registers");
@@ -349,7 +359,6 @@ struct GemmDev {
   int dh_first;
   float* dh_part;        // [split][Np][dtiles * 256] where splits > 1
   int add;               // dh collects an earlier piece
-  int wide_dw, wide_dh;  // rows take 32-byte stores
   int* err;
 };
 
@@ -423,10 +432,19 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ void store8(void* to, const uint32_t (&x)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]),
-               "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
-               : "memory");
+// 128 bytes of each of 32 rows through a warp's buffer, so that a store writes whole
+// lines: a lane puts in its row, 16 bytes at a time, in an order by its row that
+// keeps both sides free of bank conflicts.  (A tile of 256 x 256 takes 4 to 8 us
+// when all pairs write at once, 12 us where rows lie off 16 bytes.)
+__device__ __forceinline__ void rows_put(float* buf, int lane, const uint32_t (&x)[32]) {
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    reinterpret_cast<uint4*>(buf)[lane * 8 + (u ^ (lane & 7))] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+  __syncwarp();
+}
+__device__ __forceinline__ uint4 rows_get(const float* buf, int r, int u) {
+  return reinterpret_cast<const uint4*>(buf)[r * 8 + (u ^ (r & 7))];
 }
 
 // A row's entries inside a tile, rows of the warp one after another, a row's
@@ -528,12 +546,12 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
 #pragma unroll
     for (int i = 0; i < 128; ++i) acc[i] = head_ex2(__fmaf_rn(acc[i], t.f, -t.lse2)) - d.share;
     tile_entries<true>(d, buf, lane, t.orig, t.e, t.id, g.v0 + col, g.v0 + col + min(g.Vc - col, 128), acc);
-    __half* to = g.dx + (int64_t)row * g.ld + col;
+    __half* to = g.dx + (int64_t)(row - lane) * g.ld + col;  // the warp's first row
 #pragma unroll
-    for (int i = 0; i < 128; i += 16) {
-      uint32_t hi[8], lo[8];
+    for (int i = 0; i < 128; i += 64) {
+      uint32_t hi[32], lo[32];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 32; ++j) {
         const float a = i + 2 * j < limit ? acc[i + 2 * j] * 0x1p15f : 0.f;
         const float b = i + 2 * j + 1 < limit ? acc[i + 2 * j + 1] * 0x1p15f : 0.f;
         const __half2 h = __floats2half2_rn(a, b);
@@ -542,71 +560,82 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
         hi[j] = *reinterpret_cast<const uint32_t*>(&h);
         lo[j] = *reinterpret_cast<const uint32_t*>(&l);
       }
-      store8(to + i, hi);
-      store8(to + g.plane + i, lo);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        rows_put(buf, lane, p ? lo : hi);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int r = q * 4 + lane / 8;
+          *reinterpret_cast<uint4*>(to + p * g.plane + r * g.ld + i + lane % 8 * 8) = rows_get(buf, r, lane % 8);
+        }
+      }
     }
   } else {
     float* to = nullptr;   // the row's column col
-    int64_t sd = 1;
-    bool wide, add = false;
+    int64_t sd = 1, step = 0;  // step: from row to row, where that is one number
+    bool vec, add = false;
     float f2 = 1.f;
-    const int width = min(128, d.D - col);
+    const int width = min(128, d.D - col), row0 = row - lane;  // row0: the warp's first row
+    int rows;
     if (w.dw) {
-      if (row < g.Vc) to = d.dw + (int64_t)(g.v0 + row) * d.dwv + (int64_t)col * d.dwd;
+      to = d.dw + (int64_t)(g.v0 + row) * d.dwv + (int64_t)col * d.dwd;
+      step = d.dwv;
       sd = d.dwd;
-      wide = g.wide_dw;
+      vec = d.vec_dw;
+      rows = g.Vc - row0;
     } else {
-      sd = d.dh.sd;
-      wide = g.wide_dh;
-      add = g.add;
-      if (row < live) {
-        f2 = *head_row<const float>(d, d.gl, t.orig) * d.temp;
-        to = head_row<float>(d, d.dh, t.orig) + col * sd;
-      }
+      rows = live - row0;
+      if (row < live) f2 = *head_row<const float>(d, d.gl, t.orig) * d.temp;
       if (g.splits > 1) {
         const int64_t np = (live + BM - 1) / BM * BM;
-        if (row < live) to = g.dh_part + (w.split * np + row) * ((int64_t)g.dtiles * BN) + col;
-        sd = 1;
-        wide = true;
-        add = false;
+        step = (int64_t)g.dtiles * BN;
+        to = g.dh_part + (w.split * np + row) * step + col;
+        vec = true;
+      } else {
+        sd = d.dh.sd;
+        vec = d.vec_dh;
+        add = g.add;
+        if (row < live) to = head_row<float>(d, d.dh, t.orig) + col * sd;
       }
     }
-    if (width <= 0) return;
-    if (wide) {  // a whole sector per thread and store
-      if (!to) return;
+    if (width <= 0 || rows <= 0) return;
+    if (sd == 1) {  // through the warp's buffer: whole lines of 128 bytes of each row
+      float* first = to - lane * step;
 #pragma unroll
-      for (int i = 0; i < 128; i += 8) {
+      for (int i = 0; i < 128; i += 32) {
         if (i >= width) continue;
-        uint32_t x[8];
+        uint32_t x[32];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(acc[i + j] * f2);
-        if (add) {
-          const float4 a = *reinterpret_cast<const float4*>(to + i), b = *reinterpret_cast<const float4*>(to + i + 4);
-          const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(acc[i + j] * f2);
+        rows_put(buf, lane, x);
+        if (vec) {
+          const int c = i + lane % 8 * 4;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(y[j] + __uint_as_float(x[j]));
-        }
-        store8(to + i, x);
-      }
-    } else if (sd == 1) {  // rows off that alignment: through the warp's buffer, 16 columns of two rows at a time
-#pragma unroll
-      for (int i = 0; i < 128; i += 16) {
-        if (i >= width) continue;
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) buf[lane * kPitch + j] = acc[i + j] * f2;
-        __syncwarp();
-        const int c = lane % 16;
-#pragma unroll 4
-        for (int r = lane / 16; r < 32; r += 2) {
-          float* p = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)to, r));
-          if (!p || i + c >= width) continue;
-          const float x = buf[r * kPitch + c];
-          p[i + c] = add ? p[i + c] + x : x;
+          for (int q = 0; q < 8; ++q) {
+            const int r = q * 4 + lane / 8;
+            float* p = step ? first + r * step : reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)to, r));
+            if (r >= rows || c >= width) continue;
+            const uint4 y = rows_get(buf, r, lane % 8);
+            float4 z = make_float4(__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w));
+            if (add) {
+              const float4 b = *reinterpret_cast<const float4*>(p + c);
+              z.x += b.x, z.y += b.y, z.z += b.z, z.w += b.w;
+            }
+            *reinterpret_cast<float4*>(p + c) = z;
+          }
+        } else {
+          const int c = i + lane;
+#pragma unroll 8
+          for (int r = 0; r < 32; ++r) {
+            float* p = step ? first + r * step : reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)to, r));
+            if (r >= rows || c >= width) continue;
+            const float z = buf[(r * 8 + (lane / 4 ^ (r & 7))) * 4 + lane % 4];
+            p[c] = add ? p[c] + z : z;
+          }
         }
       }
     } else {  // columns apart: the rows lie closer
-      if (!to) return;
+      if (lane >= rows) return;
 #pragma unroll
       for (int i = 0; i < 128; ++i) {
         if (i >= width) continue;
@@ -634,6 +663,10 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cta_rank();
 
+  if (threadIdx.x == 32) {
+    for (const CUtensorMap* m : {&ma, &mb, &ma2, &mb2})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -812,7 +845,13 @@ __global__ void __launch_bounds__(256) head_dh_join_kernel(const __grid_constant
   float* to = head_row<float>(d, d.dh, d.rows[r]);
   for (int c = blockIdx.y * 256 + threadIdx.x; c < d.D; c += gridDim.y * 256) {
     float sum = g.add ? to[c * d.dh.sd] : 0.f;
-    for (int s = 0; s < g.splits; ++s) sum += g.dh_part[(s * np + r) * ld + c];
+    for (int s0 = 0; s0 < g.splits; s0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = s0 + k < g.splits ? g.dh_part[((s0 + k) * np + r) * ld + c] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += x[k];
+    }
     to[c * d.dh.sd] = sum;
   }
 }
@@ -937,37 +976,27 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   __half *hp = reinterpret_cast<__half*>(base + o_h), *wp = reinterpret_cast<__half*>(base + o_w);
   __half *gp = reinterpret_cast<__half*>(base + o_gh), *xp = reinterpret_cast<__half*>(base + o_x);
 
-  PlanesDev p;
+  PlanesDev hid, p;
   std::memset(static_cast<void*>(&p), 0, sizeof(p));
   p.d = d;
   p.Dp = (int)Dp;
-  p.to = hp;
-  p.gto = backward && d.dw ? gp : nullptr;
-  p.plane = hplane;
-  p.down = reinterpret_cast<float*>(base + o_hdown);
-  p.gdown = reinterpret_cast<float*>(base + o_gdown);
-  e = backward ? launch_after(head_pack_kernel<kPackHiddenGrad, 32>, dim3((unsigned)(Np / 32)), 1024, 0, s, "head hidden planes kernel", p)
-               : launch_after(head_pack_kernel<kPackHidden, 32>, dim3((unsigned)(Np / 32)), 1024, 0, s, "head hidden planes kernel", p);
-  if (!e.ok()) return e;
+  hid = p;
+  hid.to = hp;
+  hid.gto = backward && d.dw ? gp : nullptr;
+  hid.plane = hplane;
+  hid.down = reinterpret_cast<float*>(base + o_hdown);
+  hid.gdown = reinterpret_cast<float*>(base + o_gdown);
 
   g.hdown = reinterpret_cast<float*>(base + o_hdown);
-  g.gdown = p.gdown;
+  g.gdown = hid.gdown;
   g.part = reinterpret_cast<HeadPart*>(base + o_part);
   g.ld = backward ? Vp : Np;
   g.dx = xp;
   g.plane = xplane;
   g.dh_part = reinterpret_cast<float*>(base + o_dh);
   g.Vcp = (int)Vp;
-  auto wide = [](const void* p, std::initializer_list<int64_t> strides, int64_t sd) {
-    bool ok = (uintptr_t)p % 32 == 0 && sd == 1;
-    for (int64_t x : strides) ok = ok && x % 8 == 0;
-    return ok;
-  };
-  g.wide_dw = d.dw && d.D % 8 == 0 && wide(d.dw, {d.dwv}, d.dwd);
-  g.wide_dh = d.dh.p && d.D % 8 == 0 && wide(d.dh.p, {d.dh.sb, d.dh.st}, d.dh.sd);
   const int64_t av = d.wv < 0 ? -d.wv : d.wv, ad = d.wd < 0 ? -d.wd : d.wd;
   p.along_v = d.V > 1 && d.D > 1 && av < ad;
-  p.gto = nullptr;
   for (int64_t i = 0; i < pieces; ++i) {
     g.v0 = (int)(i * Vp);
     g.Vc = (int)std::min<int64_t>(Vp, d.V - i * Vp);
@@ -979,7 +1008,9 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     g.wdown = p.down;
     p.v0 = g.v0;
     p.n = g.Vc;
-    e = launch_after(head_pack_kernel<kPackWeight, 16>, dim3((unsigned)(g.Vcp / 32)), 16 * 32, 0, s, "head weight planes kernel", p);
+    const int hidden = i == 0 ? (int)(Np / 32) : 0;
+    e = launch_after(backward ? head_pack_kernel<kPackHiddenGrad> : head_pack_kernel<kPackHidden>,
+                     dim3((unsigned)(hidden + g.Vcp / 32)), kPackWarps * 32, 0, s, "head planes kernel", hid, p, hidden);
     CUtensorMap ha, wb, xa, wc, xc, gc;
     if (e.ok()) e = map_rows(hp, Np, Dp, hplane, 128, &ha);
     if (e.ok()) e = map_rows(wp, g.Vc, Dp, wplane, BR, &wb);
