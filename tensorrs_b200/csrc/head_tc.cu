@@ -80,14 +80,11 @@ __device__ __forceinline__ uint32_t magnitude(const float4& x) {
   return max(max(magnitude(x.x), magnitude(x.y)), max(magnitude(x.z), magnitude(x.w)));
 }
 
-__device__ __forceinline__ float4 piece4(const float* p, int c, int D, int64_t sd, bool vec) {
-  if (vec && c < D) return *reinterpret_cast<const float4*>(p + c);
-  float4 r;
-  r.x = c < D ? p[c * sd] : 0.f;
-  r.y = c + 1 < D ? p[(c + 1) * sd] : 0.f;
-  r.z = c + 2 < D ? p[(c + 2) * sd] : 0.f;
-  r.w = c + 3 < D ? p[(c + 3) * sd] : 0.f;
-  return r;
+__device__ __forceinline__ void split_store(__half* to, int64_t plane, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 back = __half22float2(h);
+  *reinterpret_cast<__half2*>(to) = h;
+  *reinterpret_cast<__half2*>(to + plane) = __floats2half2_rn(a - back.x, b - back.y);
 }
 __device__ __forceinline__ void split_store(__half* to, int64_t plane, float a, float b, float c, float e) {
   const float v[4] = {a, b, c, e};
@@ -151,6 +148,7 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
       return;
     }
   }
+  if (KIND != kPackHidden) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const bool along_v = KIND == kPackWeight && a.along_v;
   const int64_t sd = KIND == kPackWeight ? d.wd : d.hid.sd;
   const bool vec = KIND == kPackWeight ? d.vec_w : d.vec_h;
@@ -178,11 +176,17 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
 #pragma unroll 4
       for (int c = warp; c < d.D; c += W) all = max(all, magnitude(w[c * d.wd]));
   } else {
+    if (!vec) {  // element by element, the lanes side by side
 #pragma unroll 8
-    for (int c = lane * 4; c < d.D; c += 128) {
+      for (int c = lane; c < d.D; c += 32)
+#pragma unroll
+        for (int j = 0; j < R; ++j) top[j] = max(top[j], p[j] ? magnitude(p[j][c * sd]) : 0u);
+    }
+#pragma unroll 8
+    for (int c = lane * 4; vec && c < d.D; c += 128) {
       float4 x[R];
 #pragma unroll
-      for (int j = 0; j < R; ++j) x[j] = p[j] ? piece4(p[j], c, d.D, sd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < R; ++j) x[j] = p[j] && c < d.D ? *reinterpret_cast<const float4*>(p[j] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < R; ++j) top[j] = max(top[j], magnitude(x[j]));
     }
@@ -197,6 +201,7 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
     all = __reduce_max_sync(0xffffffffu, all);
     if (lane == 0) warp_top[warp] = all;
     __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all eight CTAs run
     if (threadIdx.x < 8) {
       uint32_t x = warp_top[0];
       for (int i = 1; i < W; ++i) x = max(x, warp_top[i]);
@@ -233,11 +238,27 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
       if (lane == 0) a.down[r0 + j] = dn;
     }
   }
+  if (!vec) {  // pairs of elements
+#pragma unroll 8
+    for (int c = lane * 2; c < a.Dp; c += 64) {
+      float2 x[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j) x[j] = make_float2(p[j] && c < d.D ? p[j][c * sd] : 0.f, p[j] && c + 1 < d.D ? p[j][(c + 1) * sd] : 0.f);
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (KIND == kPackWeight && !p[j]) continue;
+        const int64_t at = (int64_t)(r0 + j) * a.Dp + c;
+        split_store(a.to + at, a.plane, x[j].x * ups[j], x[j].y * ups[j]);
+        if (KIND == kPackHiddenGrad && a.gto) split_store(a.gto + at, a.plane, mul3(x[j].x, g[j], up), mul3(x[j].y, g[j], up));
+      }
+    }
+    return;
+  }
 #pragma unroll 4
   for (int c = lane * 4; c < a.Dp; c += 128) {
     float4 x[R];
 #pragma unroll
-    for (int j = 0; j < R; ++j) x[j] = p[j] ? piece4(p[j], c, d.D, sd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < R; ++j) x[j] = p[j] && c < d.D ? *reinterpret_cast<const float4*>(p[j] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       if (KIND == kPackWeight && !p[j]) continue;
