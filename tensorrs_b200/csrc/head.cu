@@ -292,7 +292,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (N == 0 && !d.dw) return Error{};
   // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
   // tensor-core path writes the zeros.
-  const bool few = N > 0 && N <= 16 && D <= 4096;
+  const bool few = N > 0 && N <= (c.backward ? 8 : 32) && D <= 4096 && (!c.backward || d.wd == 1 || D == 1);
   // the rows' targets
   Scratch mem;
   const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;

@@ -53,28 +53,6 @@ __device__ __forceinline__ float4 head_load4(const float* p, int c, int D, int64
   return r;
 }
 
-// The same for a weight that is read once: not kept in L1.
-template <bool VEC>
-__device__ __forceinline__ float4 head_stream4(const float* p, int c, int D, int64_t sd) {
-  if (!VEC) return head_load4<false>(p, c, D, sd);
-  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c < D)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
-                 : "l"(p + c));
-  return r;
-}
-
-// Up to 8 of the call's rows from r0 on.
-template <int NR>
-struct FewRows {
-  int row[NR];           // a row with a target, or -1
-  __device__ __forceinline__ void read(const HeadDev& d, int r0) {
-#pragma unroll
-    for (int i = 0; i < NR; ++i) row[i] = r0 + i < d.N && head_first_id(d, r0 + i) != kNoToken ? r0 + i : -1;
-  }
-};
-
 // D += A B for A 16 x 8 (row major), B 8 x 8, in TF32: the upper 19 bits of each
 // element are read.
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -514,9 +492,8 @@ __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const _
 
 // A thread per 4 columns; blockIdx.y and the thread's group: a range of the
 // vocabulary.
-template <int NR>
 __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant__ HeadGradDev a) {
-  constexpr int U = 4;   // rows of the vocabulary in flight
+  constexpr int NR = 8, U = 4;  // U: rows of the vocabulary in flight
   const HeadDev& d = a.d;
   pdl_launch_dependents();
   const int c = (blockIdx.x * 256 + (threadIdx.x & ((1 << a.lg) - 1))) * 4;
@@ -525,16 +502,13 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
   const bool add = a.block > 0;  // behind earlier rows
   pdl_wait();
   uint64_t h[NR][2], acc[NR][2];
-  {
-    FewRows<NR> rows;
-    rows.read(d, r0);
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (rows.row[i] >= 0) x = head_load4<false>(head_row<const float>(d, d.hid, rows.row[i]), c, d.D, d.hid.sd);
-      h[i][0] = pk(x.x, x.y), h[i][1] = pk(x.z, x.w);
-      acc[i][0] = acc[i][1] = 0;
-    }
+  for (int i = 0; i < NR; ++i) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r0 + i < d.N && head_first_id(d, r0 + i) != kNoToken)
+      x = head_load4<false>(head_row<const float>(d, d.hid, r0 + i), c, d.D, d.hid.sd);
+    h[i][0] = pk(x.x, x.y), h[i][1] = pk(x.z, x.w);
+    acc[i][0] = acc[i][1] = 0;
   }
   const float* dx = a.dx + a.db;
   const int lane = threadIdx.x % 32;
@@ -542,12 +516,10 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
   int64_t v = (int64_t)d.V * part / parts;
   // U rows of the weight, and one of their score gradients per lane
   auto fetch = [&](float4 (&w)[U], float& x, int64_t at) {
-    x = lane < U * NR && at + lane / NR < v1 ? dx[(at + lane / NR) * a.ds + lane % NR] : 0.f;
+    x = at + lane / NR < v1 ? dx[(at + lane / NR) * a.ds + lane % NR] : 0.f;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (d.dh.p && at + j < v1)
-        w[j] = d.vec_w ? head_stream4<true>(d.w + (at + j) * d.wv, c, d.D, 1) : head_load4<false>(d.w + (at + j) * d.wv, c, d.D, d.wd);
+      w[j] = d.dh.p && at + j < v1 ? head_load4<false>(d.w + (at + j) * d.wv, c, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
   auto work = [&](float4 (&w)[U], float xs) {
@@ -610,10 +582,10 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
   }
 }
 
-// dh of up to NR rows from its parts, in order: 32 columns times 8 runs of parts
+// dh of up to 8 rows from its parts, in order: 32 columns times 8 runs of parts
 // per CTA; zeros for rows without a target.
-template <int NR>
 __global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_constant__ HeadGradDev a, int parts) {
+  constexpr int NR = 8;
   __shared__ float s[8][32];
   const HeadDev& d = a.d;
   pdl_wait();
@@ -659,12 +631,6 @@ Error launch_scores(HeadRowsDev& a, cudaStream_t s) {
   e = launch_after(k, dim3((unsigned)ctas, (unsigned)((d.N + 8 * NT - 1) / (8 * NT))), kFewThreads, smem, s, "head rows kernel", a);
   if (e.ok() && !GRAD) e = head_join(d, a.part, ctas, 1, ctas, true, s);
   return e;
-}
-
-template <int NR>
-Error launch_grad(HeadGradDev& a, int splits, cudaStream_t s) {
-  return launch_after(head_grad_kernel<NR>, dim3((unsigned)((a.d.D + 1023) / 1024), (unsigned)splits), 256, 0, s,
-                      "head gradient kernel", a);
 }
 
 }  // namespace
@@ -714,10 +680,10 @@ Error head_few(const HeadDev& d, bool backward, cudaStream_t s) {
       allow_smem((const void*)head_columns_kernel, smem);
       e = launch_after(head_columns_kernel, dim3(across, (unsigned)splits), kColWarps * 32, smem, s, "head columns kernel", g);
     } else {
-      e = launch_grad<8>(g, splits, s);
+      e = launch_after(head_grad_kernel, dim3(across, (unsigned)splits), 256, 0, s, "head gradient kernel", g);
     }
     if (e.ok() && d.dh.p)
-      e = launch_after(head_grad_join_kernel<8>, dim3((unsigned)((d.D + 31) / 32), 8u), 256, 0, s, "head gradient join kernel", g,
+      e = launch_after(head_grad_join_kernel, dim3((unsigned)((d.D + 31) / 32), 8u), 256, 0, s, "head gradient join kernel", g,
                        parts);
   }
   return e;

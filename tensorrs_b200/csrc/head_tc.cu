@@ -956,6 +956,8 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   int64_t pieces = std::max<int64_t>(1, (round_up(d.V, BN) * row_bytes + kPieceBytes - 1) / kPieceBytes);
   const int64_t Vp = round_up((d.V + pieces - 1) / pieces, BN);
   pieces = (d.V + Vp - 1) / Vp;
+  if (Np / BM * std::max(Vp / BN, dtiles * 64) + Vp / BN * dtiles >= (1ll << 31))
+    return make_error(TRS_ERR_SHAPE, "head: 2^31 or more tiles of 256 x 256");
   int* err = async_error_word();
   if (!err) return make_error(TRS_ERR_CUDA, "head: no async-error word");
 

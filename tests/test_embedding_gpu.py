@@ -71,7 +71,8 @@ SIZES = [
     (3, 65, 513, 7, "f4", "text", "i4"), (1, 4095, 1000, 12, "f8", "text", "i8"), (1, 4096, 3, 9, "f8", "one", "i8"),
     (2, 2049, 70001, 36, "f4", "text", "i8"), (3, 3333, 300_000, 8, "f4", "text", "i4"), (5, 77, 4000, 1031, "f4", "text", "i8"),
     (2, 500, 900, 2048, "f4", "text", "i8"), (1, 257, 40, 514, "f8", "text", "i8"), (4, 100, 50, 24, "f4", "none", "i8"),
-    (2, 9000, 20, 40, "f4", "text", "i8"),
+    (2, 9000, 20, 40, "f4", "text", "i8"), (0, 100, 300_000, 8, "f4", "text", "i8"), (1, 4097, 600, 33, "f4", "one", "i4"),
+    (0, 40_000, 9, 16, "f4", "one", "i8"),
 ]
 NAMES = ["x".join(str(x) for x in s) for s in SIZES]
 

@@ -107,6 +107,8 @@ SIZES = [
     (257, 513, 300, CE, 0.9), (300, 2049, 520, SMOOTH, 0.35), (513, 1025, 1024, KD7, 0.1), (700, 10_007, 521, CE, 0.3),
     (1030, 777, 2049, CE, 0.0), (2000, 5000, 40, KD64, 0.2), (40, 30_000, 72, CE, 0.0), (1, 3, 2, ("ce", 1.0), 0.0),
     (50, 64, 16, ("ce", 1.0), 0.2), (20, 100, 24, ("kd", 1024, 3.0), 0.0), (4096, 33, 17, CE, 0.5),
+    # few rows in two blocks, of widths that bulk copies take and do not
+    (12, 300, 2800, CE, 0.1), (16, 333, 2701, KD7, 0.0), (11, 1000, 36, SMOOTH, 0.2), (13, 500, 35, KD64, 0.0),
     # nothing but masked rows
     (5, 100, 32, CE, 1.0), (300, 400, 48, KD7, 1.0),
 ]
@@ -299,8 +301,8 @@ def test_infinities_stay_in_their_rows(N):
         check_all(c, t, loss, lse, *c.backward(lse))
 
 
-def test_large_pieces():
-    """A vocabulary that the gradient takes in several pieces, and views past 2^31 elements."""
+def test_large_vocabulary():
+    """140000 tokens, and the weight as a view past 2^31 elements."""
     N, V, D = 300, 140_000, 64
     c = Case(N, V, D, SMOOTH, 0.1)
     t = c.truth()
@@ -311,6 +313,36 @@ def test_large_pieces():
     big[:, 64:64 + D] = c.d["w"]
     loss2, lse2 = c.forward(w=V_(big[:, 64:64 + D]))
     assert torch.equal(loss, loss2) and torch.equal(lse, lse2)
+
+
+def test_pieces_of_the_vocabulary():
+    """A weight that either direction takes in several pieces, the last one not whole; the definition in 64 bits on the
+    GPU, in the 2-norm."""
+    N, V, D = 300, 40_100, 4000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn((V, D), generator=g, device="cuda") * (2 / D**0.5)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    h = torch.randn((N, D), generator=g, device="cuda") + w[t]
+    gl = torch.rand((N,), generator=g, device="cuda")
+    loss, lse = torch.empty((N,), device="cuda"), torch.empty((N,), device="cuda")
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    device.linear_cross_entropy(V_(h), V_(w), V_(t), loss, lse)
+    device.linear_cross_entropy_backward(V_(gl), V_(h), V_(w), V_(t), V_(lse), dh, dw)
+    x = h.double() @ w.double().T
+    want_lse = torch.logsumexp(x, -1)
+    p = torch.exp(x - want_lse[:, None])
+    s_max = float(torch.maximum(x.abs().max(), want_lse.abs().max()))
+    here = torch.arange(N, device="cuda")
+    want = want_lse - x[here, t]
+    both = p.clone()
+    both[here, t] += 1
+    both *= gl.double()[:, None]
+    p[here, t] -= 1
+    p *= gl.double()[:, None]
+    ref.near(to_host(lse), to_host(want_lse), "lse", s_max, to_host(want_lse))
+    ref.near(to_host(loss), to_host(want), "loss", s_max, to_host(want_lse))
+    ref.near(to_host(dh), to_host(p @ w.double()), "dh", s_max, to_host(((both * both) @ w.double().square()).sqrt()))
+    ref.near(to_host(dw), to_host(p.T @ h.double()), "dw", s_max, to_host(((both * both).T @ h.double().square()).sqrt()))
 
 
 def test_streams_and_graphs():
