@@ -349,7 +349,7 @@ __device__ __forceinline__ T emb_result(const EmbDev& d, double sum, T before) {
 
 template <class T, int V>
 __global__ void __launch_bounds__(kEmbThreads) emb_sum_kernel(const EmbDev d) {
-  constexpr int U = 8;  // rows in flight
+  constexpr int U = 4;  // rows in flight (8: 82 us against 77, 16 81: the registers cost CTAs)
   __shared__ uint32_t s_key[kEmbThreads], s_tok[kEmbThreads];
   pdl_launch_dependents();
   pdl_wait();
