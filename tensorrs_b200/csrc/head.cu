@@ -95,41 +95,50 @@ __global__ void __launch_bounds__(1024) head_list_kernel(const HeadDev d) {
   __shared__ int warps[32];
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int U = 4;  // consecutive rows of a thread
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int done = 0;
-  for (int r0 = 0; r0 < d.N; r0 += 1024) {
-    const int row = r0 + threadIdx.x;
-    int id = kNoToken;
-    if (row < d.N) {
-      if (d.distill) {
-        id = d.eid[(int64_t)row * d.K];
-      } else {
-        id = head_id(d, d.ids, row, 0);
-        d.eid[row] = id;
+  for (int r0 = 0; r0 < d.N; r0 += 1024 * U) {
+    int id[U], mine = 0;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int row = r0 + threadIdx.x * U + j;
+      id[j] = row < d.N ? head_first_id(d, row) : kNoToken;
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int row = r0 + threadIdx.x * U + j;
+      mine += id[j] != kNoToken;
+      if (row >= d.N) continue;
+      if (!d.distill) {
+        d.eid[row] = id[j];
         d.ew[row] = d.weight;
       }
-    }
-    const bool there = id != kNoToken;
-    if (row < d.N && !there && d.loss.p) {
-      *head_row<float>(d, d.loss, row) = 0.f;
-      if (d.lse.p) *head_row<float>(d, d.lse, row) = 0.f;
-    }
-    const uint32_t vote = __ballot_sync(0xffffffffu, there);
-    if (lane == 0) warps[warp] = __popc(vote);
-    __syncthreads();
-    int mine = 0, all = 0;
-    {
-      const int n = warps[lane];
-      int scan = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += y;
+      if (id[j] == kNoToken && d.loss.p) {
+        *head_row<float>(d, d.loss, row) = 0.f;
+        if (d.lse.p) *head_row<float>(d, d.lse, row) = 0.f;
       }
-      mine = __shfl_sync(0xffffffffu, scan - n, warp);
-      all = __shfl_sync(0xffffffffu, scan, 31);
     }
-    if (there) d.rows[done + mine + __popc(vote & ((1u << lane) - 1))] = row;
+    // where this thread's rows begin in the list: the lanes before it, then the warps
+    int scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += y;
+    }
+    if (lane == 31) warps[warp] = scan;
+    __syncthreads();
+    int at = warps[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += y;
+    }
+    const int all = __shfl_sync(0xffffffffu, at, 31), before = __shfl_sync(0xffffffffu, at, warp > 0 ? warp - 1 : 0);
+    int to = done + (warp > 0 ? before : 0) + scan - mine;
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (id[j] != kNoToken) d.rows[to++] = r0 + threadIdx.x * U + j;
     done += all;
     __syncthreads();
   }
@@ -292,7 +301,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (N == 0 && !d.dw) return Error{};
   // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
   // tensor-core path writes the zeros.
-  const bool few = N > 0 && N <= (c.backward ? 8 : 32) && D <= 4096 && (!c.backward || d.wd == 1 || D == 1);
+  const bool few = head_few_takes(d, c.backward);
   // the rows' targets
   Scratch mem;
   const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;

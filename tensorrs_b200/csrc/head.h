@@ -131,7 +131,18 @@ __device__ __forceinline__ HeadPart head_add(const HeadPart& a, const HeadPart& 
 Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
                 cudaStream_t stream);
 
-// Up to 16 rows of widths up to 4096 (head_few.cu).
+// Few rows (head_few.cu).  8 or 16 of them share a read of the weight, which the
+// tensor-core path reads, splits, writes and reads again: on 32000 x 1024, 17 rows 78
+// us here and 113 there, 33 there alone; gradients of 8 rows 87 and 216, of 16
+// FEW16 and 217, of two blocks of rows 257 and 217.  Widths up to 4096 (4 x 4096:
+// 58 us and 243); gradients of weights whose columns lie apart are walked badly here
+// (8 rows 490 us, 300 there).
+inline bool head_few_takes(const HeadDev& d, bool backward) {
+  if (d.N < 1 || d.D > 4096) return false;
+  if (!backward) return d.N <= 32;
+  if (d.wd != 1 && d.D > 1) return false;
+  return d.N <= 8 || (d.N <= 16 && d.vec_w && d.D <= 2560);
+}
 Error head_few(const HeadDev& d, bool backward, cudaStream_t stream);
 // More rows, or none (head_tc.cu).
 Error head_tc(const HeadDev& d, bool backward, cudaStream_t stream);

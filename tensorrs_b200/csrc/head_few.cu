@@ -1,4 +1,4 @@
-// head_few.cu -- a model's last layer with its loss for up to 16 rows: the weight
+// head_few.cu -- a model's last layer with its loss for few rows: the weight
 // is read in f32, once for 8 or 16 rows, and HBM bounds it all.
 //
 //   head_rows_kernel     scores: teams of warps take 16 vocabulary rows at a time.  f32
@@ -119,7 +119,7 @@ struct HeadRowsDev {
   HeadDev d;
   int blocks;            // the width in blocks of 16, rounded up
   HeadPart* part;        // forward: [row][CTA]
-  float* dx;             // backward: [row block][V][8 NT]
+  float* dx;             // backward, of up to 8 NT rows: [V][8 NT]
   int lg;                // 2^lg warps share a row's columns
 };
 
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
     }
   }
   HeadPart pt = {-INFINITY, 0.f, 0.f, 0.f};
-  float* dx = GRAD ? a.dx + (int64_t)blockIdx.y * d.V * NR : nullptr;
+  float* dx = a.dx;
   float part[NT][4];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -286,51 +286,52 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
 
 struct HeadGradDev {
   HeadDev d;
-  int block;             // of NR rows
-  int64_t db;            // dx of the block: first element, and the distance of its rows
-  int ds;
   int lg;                // 2^lg threads (whole warps) along the width, the rest along the vocabulary
   const float* dx;
   float* part;           // [part of the vocabulary][NR][D] of dh
   int* err;
 };
 
-constexpr int kStepCols = 128;               // columns of a step
-constexpr int kColPitch = kStepCols + 8;     // four rows' 32 bytes lie in different banks
-constexpr int kColStep = 16 * kColPitch;     // floats
-constexpr int kColSteps = 3;                 // in flight
+constexpr int kColSteps = 3;                 // steps of 16 vocabulary rows in flight
 constexpr int kColWarps = 8;
+// A warp's columns, and its rows in shared memory: four rows' 32 bytes lie in different
+// banks.
+template <int NT> constexpr int kColumns = 128 / NT;
+template <int NT> constexpr int kColPitch = kColumns<NT> + 8;
+template <int NT> constexpr int kColStep = 16 * kColPitch<NT>;  // floats
 
 __device__ __forceinline__ bool step_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
 }
 
 // Rows [v, v + rows) of the weight, `bytes` of each from column c on, by one copy per
-// lane.
+// lane, into rows of PITCH floats.
+template <int PITCH>
 __device__ __forceinline__ void step_copy(const HeadDev& d, float* to, int64_t v, int rows, int c, uint32_t bytes, uint64_t* bar,
                                           int lane) {
   fence_proxy_async();  // what was read here has been read
   if (lane == 0) mbar_arrive_expect_tx(bar, bytes * rows);
   __syncwarp();
-  if (lane < rows) bulk_g2s(to + lane * kColPitch, d.w + (v + lane) * d.wv + c, bytes, bar);
+  if (lane < rows) bulk_g2s(to + lane * PITCH, d.w + (v + lane) * d.wv + c, bytes, bar);
 }
 
-// dw and a part of dh of 8 call rows for 128 columns per warp: 2^lg warps along the
-// width, the others (and blockIdx.y) along the vocabulary, 16 rows of it a step.
+// dw and a part of dh of 8 NT call rows for 128 / NT columns per warp: 2^lg warps along
+// the width, the others (and blockIdx.y) along the vocabulary, 16 rows of it a step.
 //   dw: rows of dx as the left operand, h as the right one, in registers for good:
 //       column 4 (m / 2) + m % 2 of a block of 16 is column m of one MMA, the one 2
 //       to its right of the other, so that a lane ends with four neighbours
 //   dh^T += w^T dx: 4 neighbouring columns of a lane are the rows of four MMAs
+template <int NT>
 __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const __grid_constant__ HeadGradDev a) {
+  constexpr int CW = kColumns<NT>, NB = CW / 16, HF = CW / 64, PITCH = kColPitch<NT>, STEP = kColStep<NT>;
   extern __shared__ float4 s_raw[];
   __shared__ uint64_t full[kColWarps][kColSteps];
   const HeadDev& d = a.d;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, lg = lane / 4, lt = lane % 4;
   const int across = 1 << a.lg, down = kColWarps >> a.lg;
-  const int c0 = (blockIdx.x * across + (warp & (across - 1))) * kStepCols;
+  const int c0 = (blockIdx.x * across + (warp & (across - 1))) * CW;
   const int part = blockIdx.y * down + (warp >> a.lg), parts = gridDim.y * down;
-  const bool add = a.block > 0;  // behind earlier rows
-  float* ring = reinterpret_cast<float*>(s_raw) + warp * (kColSteps * kColStep);
+  float* ring = reinterpret_cast<float*>(s_raw) + warp * (kColSteps * STEP);
   pdl_launch_dependents();
   pdl_wait();
   if (c0 >= d.D) return;
@@ -338,121 +339,123 @@ __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const _
     for (int s = 0; s < kColSteps; ++s) mbar_init(&full[warp][s], 1);
     fence_mbar_init();
   }
-  for (int i = lane; i < kColSteps * kColStep / 4; i += 32) reinterpret_cast<float4*>(ring)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  // what no copy writes only has to be finite: it meets zeros of dx, or columns that nothing takes
+  for (int i = lane; i < kColSteps * STEP / 4; i += 32) reinterpret_cast<float4*>(ring)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncwarp();
   const int groups = (d.V + 15) / 16, g1 = (int)((int64_t)groups * (part + 1) / parts);
   int g = (int)((int64_t)groups * part / parts), gl = g;
-  const uint32_t bytes = (uint32_t)min(kStepCols, d.D - c0) * 4;
+  const uint32_t bytes = (uint32_t)min(CW, d.D - c0) * 4;
   const bool want_h = d.dh.p != nullptr;
   auto copy = [&](int s) {
     if (!want_h || gl >= g1) return;
-    step_copy(d, ring + s * kColStep, (int64_t)gl * 16, min(16, d.V - gl * 16), c0, bytes, &full[warp][s], lane);
+    step_copy<PITCH>(d, ring + s * STEP, (int64_t)gl * 16, min(16, d.V - gl * 16), c0, bytes, &full[warp][s], lane);
     ++gl;
   };
 #pragma unroll
   for (int s = 0; s < kColSteps; ++s) copy(s);
-  // h of the warp's columns: [block of 16][its two MMAs][hidden rows lt, lt + 4]
-  uint32_t hh[8][2][2], hl[8][2][2];
-  {
-    const int r0 = a.block * 8;
+  // h of the warp's columns: [block of 16][its two MMAs][eight rows][hidden rows lt, lt + 4 of them]
+  uint32_t hh[NB][2][NT][2], hl[NB][2][NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
     const float* row[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = r0 + lt + 4 * e;
+      const int r = n * 8 + lt + 4 * e;
       row[e] = r < d.N && head_first_id(d, r) != kNoToken ? head_row<const float>(d, d.hid, r) : nullptr;
     }
 #pragma unroll
-    for (int b = 0; b < 8; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int c = c0 + b * 16 + 4 * (lg / 2) + lg % 2 + 2 * q;
-          tf32_split(row[e] && c < d.D ? row[e][c * d.hid.sd] : 0.f, &hh[b][q][e], &hl[b][q][e]);
+          tf32_split(row[e] && c < d.D ? row[e][c * d.hid.sd] : 0.f, &hh[b][q][n][e], &hl[b][q][n][e]);
         }
   }
-  float acc[8][4];  // dh^T: [half of 64 columns, column 4 lg + i][..]
+  float acc[4 * HF][NT][4];  // dh^T: [half of 64 columns, column 4 lg + i][..]
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4 * HF; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  const float* dx = a.dx + a.db;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.f;
   // dx of a group: this lane's elements of both operands
-  float xa[4], xb[4];
+  float xa[NT][4], xb[NT][4];
   auto fetch = [&](int at) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t va = (int64_t)at * 16 + lg + e % 2 * 8, vb = (int64_t)at * 16 + lt + 4 * e;
-      xa[e] = at < g1 && va < d.V ? dx[va * a.ds + lt + e / 2 * 4] : 0.f;
-      xb[e] = at < g1 && vb < d.V ? dx[vb * a.ds + lg] : 0.f;
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t va = (int64_t)at * 16 + lg + e % 2 * 8, vb = (int64_t)at * 16 + lt + 4 * e;
+        xa[n][e] = at < g1 && va < d.V ? a.dx[va * (8 * NT) + n * 8 + lt + e / 2 * 4] : 0.f;
+        xb[n][e] = at < g1 && vb < d.V ? a.dx[vb * (8 * NT) + n * 8 + lg] : 0.f;
+      }
   };
   fetch(g);
-  const float* w0 = ring + lt * kColPitch + 4 * lg;
+  const float* w0 = ring + lt * PITCH + 4 * lg;
   int slot = 0, phase = 0;
   bool ok = true;
   for (; g < g1; ++g) {
-    uint32_t ah[4], al[4], bh[4], bl[4];
+    uint32_t ah[NT][4], al[NT][4], bh[NT][4], bl[NT][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      tf32_split(xa[e], &ah[e], &al[e]);
-      tf32_split(xb[e], &bh[e], &bl[e]);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        tf32_split(xa[n][e], &ah[n][e], &al[n][e]);
+        tf32_split(xb[n][e], &bh[n][e], &bl[n][e]);
+      }
     fetch(g + 1);
     if (d.dw) {
       const int64_t v = (int64_t)g * 16 + lg;
       float* to[2] = {d.dw + v * d.dwv + (c0 + 4 * lt) * d.dwd, d.dw + (v + 8) * d.dwv + (c0 + 4 * lt) * d.dwd};
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
+      for (int b = 0; b < NB; ++b) {
         float o[2][4];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[q][e] = 0.f;
-          mma_tf32(o[q], al, hh[b][q][0], hh[b][q][1]);
-          mma_tf32(o[q], ah, hl[b][q][0], hl[b][q][1]);
-          mma_tf32(o[q], ah, hh[b][q][0], hh[b][q][1]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_tf32(o[q], al[n], hh[b][q][n][0], hh[b][q][n][1]);
+            mma_tf32(o[q], ah[n], hl[b][q][n][0], hl[b][q][n][1]);
+            mma_tf32(o[q], ah[n], hh[b][q][n][0], hh[b][q][n][1]);
+          }
         }
         const int c = c0 + b * 16 + 4 * lt;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (v + 8 * e >= d.V || c >= d.D) continue;
-          float4 y = make_float4(o[0][2 * e], o[0][2 * e + 1], o[1][2 * e], o[1][2 * e + 1]);
+          const float ys[4] = {o[0][2 * e], o[0][2 * e + 1], o[1][2 * e], o[1][2 * e + 1]};
           if (d.vec_dw) {
-            float4* p = reinterpret_cast<float4*>(to[e] + b * 16);
-            if (add) {
-              const float4 z = *p;
-              y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-            }
-            *p = y;
+            *reinterpret_cast<float4*>(to[e] + b * 16) = make_float4(ys[0], ys[1], ys[2], ys[3]);
           } else {
-            const float ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (c + k < d.D) {
-                float* p = to[e] + (b * 16 + k) * d.dwd;
-                *p = add ? *p + ys[k] : ys[k];
-              }
+              if (c + k < d.D) to[e][(b * 16 + k) * d.dwd] = ys[k];
           }
         }
       }
     }
     if (!want_h) continue;
     if (ok) ok = step_wait(&full[warp][slot], (uint32_t)phase);
-    const float* w = w0 + slot * kColStep;
+    const float* w = w0 + slot * STEP;
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      float sum[4][4];
+    for (int hf = 0; hf < HF; ++hf) {
+      float sum[4][NT][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[i][n][j] = 0.f;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         float y[4][4];  // [operand element][column]
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float4 z = *reinterpret_cast<const float4*>(w + (p * 8 + e / 2 * 4) * kColPitch + hf * 64 + e % 2 * 32);
+          const float4 z = *reinterpret_cast<const float4*>(w + (p * 8 + e / 2 * 4) * PITCH + hf * 64 + e % 2 * 32);
           y[e][0] = z.x, y[e][1] = z.y, y[e][2] = z.z, y[e][3] = z.w;
         }
 #pragma unroll
@@ -460,15 +463,20 @@ __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const _
           uint32_t wh[4], wl[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) tf32_split(y[e][i], &wh[e], &wl[e]);
-          mma_tf32(sum[i], wl, bh[2 * p], bh[2 * p + 1]);
-          mma_tf32(sum[i], wh, bl[2 * p], bl[2 * p + 1]);
-          mma_tf32(sum[i], wh, bh[2 * p], bh[2 * p + 1]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_tf32(sum[i][n], wl, bh[n][2 * p], bh[n][2 * p + 1]);
+            mma_tf32(sum[i][n], wh, bl[n][2 * p], bl[n][2 * p + 1]);
+            mma_tf32(sum[i][n], wh, bh[n][2 * p], bh[n][2 * p + 1]);
+          }
         }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[hf * 4 + i][j] += sum[i][j];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[hf * 4 + i][n][j] += sum[i][n][j];
     }
     copy(slot);
     if (++slot == kColSteps) {
@@ -482,12 +490,14 @@ __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const _
   }
   if (!want_h) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4 * HF; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + i / 4 * 64 + j / 2 * 32 + 4 * lg + i % 4, n = 2 * lt + j % 2;
-      if (c < d.D) a.part[((int64_t)part * 8 + n) * d.D + c] = acc[i][j];
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = c0 + i / 4 * 64 + j / 2 * 32 + 4 * lg + i % 4, r = n * 8 + 2 * lt + j % 2;
+        if (c < d.D) a.part[((int64_t)part * (8 * NT) + r) * d.D + c] = acc[i][n][j];
+      }
 }
 
 // A thread per 4 columns; blockIdx.y and the thread's group: a range of the
@@ -498,25 +508,22 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
   pdl_launch_dependents();
   const int c = (blockIdx.x * 256 + (threadIdx.x & ((1 << a.lg) - 1))) * 4;
   const int groups = 256 >> a.lg, part = blockIdx.y * groups + (threadIdx.x >> a.lg), parts = gridDim.y * groups;
-  const int r0 = a.block * NR;
-  const bool add = a.block > 0;  // behind earlier rows
   pdl_wait();
   uint64_t h[NR][2], acc[NR][2];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r0 + i < d.N && head_first_id(d, r0 + i) != kNoToken)
-      x = head_load4<false>(head_row<const float>(d, d.hid, r0 + i), c, d.D, d.hid.sd);
+    if (i < d.N && head_first_id(d, i) != kNoToken) x = head_load4<false>(head_row<const float>(d, d.hid, i), c, d.D, d.hid.sd);
     h[i][0] = pk(x.x, x.y), h[i][1] = pk(x.z, x.w);
     acc[i][0] = acc[i][1] = 0;
   }
-  const float* dx = a.dx + a.db;
+  const float* dx = a.dx;
   const int lane = threadIdx.x % 32;
   const int64_t v1 = (int64_t)d.V * (part + 1) / parts;
   int64_t v = (int64_t)d.V * part / parts;
   // U rows of the weight, and one of their score gradients per lane
   auto fetch = [&](float4 (&w)[U], float& x, int64_t at) {
-    x = at + lane / NR < v1 ? dx[(at + lane / NR) * a.ds + lane % NR] : 0.f;
+    x = at + lane / NR < v1 ? dx[at * NR + lane] : 0.f;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       w[j] = d.dh.p && at + j < v1 ? head_load4<false>(d.w + (at + j) * d.wv, c, d.D, d.wd) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -543,19 +550,11 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
       upk(o1, &o[2], &o[3]);
       float* to = d.dw + (v + j) * d.dwv;
       if (d.vec_dw) {
-        float4 y = make_float4(o[0], o[1], o[2], o[3]);
-        if (add) {
-          const float4 b = *reinterpret_cast<const float4*>(to + c);
-          y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
-        }
-        __stcs(reinterpret_cast<float4*>(to + c), y);
+        __stcs(reinterpret_cast<float4*>(to + c), make_float4(o[0], o[1], o[2], o[3]));
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (c + k < d.D) {
-            float* e = to + (c + k) * d.dwd;
-            *e = add ? *e + o[k] : o[k];
-          }
+          if (c + k < d.D) to[(c + k) * d.dwd] = o[k];
       }
     }
     v += U;
@@ -582,15 +581,13 @@ __global__ void __launch_bounds__(256, 2) head_grad_kernel(const __grid_constant
   }
 }
 
-// dh of up to 8 rows from its parts, in order: 32 columns times 8 runs of parts
+// dh from its parts, in order: 32 columns times 8 runs of parts
 // per CTA; zeros for rows without a target.
-__global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_constant__ HeadGradDev a, int parts) {
-  constexpr int NR = 8;
+__global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_constant__ HeadGradDev a, int parts, int NR) {
   __shared__ float s[8][32];
   const HeadDev& d = a.d;
   pdl_wait();
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32, r = blockIdx.y, row = a.block * NR + r;
-  if (row >= d.N) return;
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32, r = blockIdx.y;
   float sum = 0.f;
   const int p1 = (int)((int64_t)parts * (w + 1) / 8);
   if (c < d.D)
@@ -605,7 +602,7 @@ __global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_consta
   __syncthreads();
   if (w != 0 || c >= d.D) return;
   for (int i = 1; i < 8; ++i) sum += s[i][threadIdx.x];
-  head_row<float>(d, d.dh, row)[c * d.dh.sd] = head_first_id(d, row) != kNoToken ? sum : 0.f;
+  head_row<float>(d, d.dh, r)[c * d.dh.sd] = head_first_id(d, r) != kNoToken ? sum : 0.f;
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -642,7 +639,7 @@ Error head_few(const HeadDev& d, bool backward, cudaStream_t s) {
   a.d = d;
   a.blocks = (d.D + 15) / 16;
   // 16 rows share one read of the weight where the shared memory holds them
-  const int nt = d.N > 8 && d.D <= 2560 ? 2 : 1, blocks = (d.N + 8 * nt - 1) / (8 * nt);
+  const int nt = d.N > 8 && d.D <= 2560 ? 2 : 1;
   if (!backward) return nt == 1 ? launch_scores<1, false>(a, s) : launch_scores<2, false>(a, s);
   Scratch mem;
   Error e;
@@ -654,8 +651,9 @@ Error head_few(const HeadDev& d, bool backward, cudaStream_t s) {
   int splits, parts;  // of the vocabulary: CTAs, and those times a CTA's own
   unsigned across;    // CTAs along the width
   if (d.vec_w) {
-    while (g.lg < 3 && (kStepCols << g.lg) < d.D) ++g.lg;
-    across = (unsigned)((d.D + (kStepCols << g.lg) - 1) / (kStepCols << g.lg));
+    const int columns = 128 / nt;
+    while (g.lg < 3 && (columns << g.lg) < d.D) ++g.lg;
+    across = (unsigned)((d.D + (columns << g.lg) - 1) / (columns << g.lg));
     splits = std::max(1, std::min((d.V + 15) / 16, sms / (int)across));
     parts = splits * (kColWarps >> g.lg);
   } else {
@@ -665,28 +663,26 @@ Error head_few(const HeadDev& d, bool backward, cudaStream_t s) {
     splits = std::max(1, std::min((d.V + 31) / 32, 2 * sms / (int)across));
     parts = splits * (256 >> g.lg);
   }
-  const size_t nd = (size_t)d.V * 8 * nt * blocks;
-  e = mem.alloc(sizeof(float) * (nd + (size_t)parts * 8 * d.D), s);
+  const size_t nd = (size_t)d.V * 8 * nt;
+  e = mem.alloc(sizeof(float) * (nd + (size_t)parts * 8 * nt * d.D), s);
   if (!e.ok()) return e;
   a.dx = mem.as<float>();
   e = nt == 1 ? launch_scores<1, true>(a, s) : launch_scores<2, true>(a, s);
+  if (!e.ok()) return e;
   g.dx = a.dx;
-  g.ds = 8 * nt;
   g.part = a.dx + nd;
-  for (g.block = 0; e.ok() && g.block * 8 < d.N; ++g.block) {
-    g.db = nt == 2 ? 8 * g.block : (int64_t)g.block * d.V * 8;
-    if (d.vec_w) {
-      constexpr int smem = kColWarps * kColSteps * kColStep * 4;
-      allow_smem((const void*)head_columns_kernel, smem);
-      e = launch_after(head_columns_kernel, dim3(across, (unsigned)splits), kColWarps * 32, smem, s, "head columns kernel", g);
-    } else {
-      e = launch_after(head_grad_kernel, dim3(across, (unsigned)splits), 256, 0, s, "head gradient kernel", g);
-    }
-    if (e.ok() && d.dh.p)
-      e = launch_after(head_grad_join_kernel, dim3((unsigned)((d.D + 31) / 32), 8u), 256, 0, s, "head gradient join kernel", g,
-                       parts);
+  const dim3 grid(across, (unsigned)splits);
+  if (!d.vec_w) {
+    e = launch_after(head_grad_kernel, grid, 256, 0, s, "head gradient kernel", g);
+  } else {
+    auto k = nt == 1 ? head_columns_kernel<1> : head_columns_kernel<2>;
+    const int smem = kColWarps * kColSteps * 4 * (nt == 1 ? kColStep<1> : kColStep<2>);
+    allow_smem((const void*)k, smem);
+    e = launch_after(k, grid, kColWarps * 32, smem, s, "head columns kernel", g);
   }
-  return e;
+  if (!e.ok() || !d.dh.p) return e;
+  return launch_after(head_grad_join_kernel, dim3((unsigned)((d.D + 31) / 32), (unsigned)d.N), 256, 0, s,
+                      "head gradient join kernel", g, parts, 8 * nt);
 }
 
 }  // namespace trs

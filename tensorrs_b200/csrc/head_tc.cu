@@ -375,10 +375,10 @@ struct GemmDev {
   int64_t ld, plane;
   // kProducts
   int dtiles;            // tiles along the width
-  int splits;            // parts of dh's contraction
-  int slabs;             // slabs of a part
+  int splits, slabs;     // parts of dh's contraction and their slabs
+  int wsplits, wslabs;   // of dw's
   int dh_first;
-  float* dh_part;        // [split][Np][dtiles * 256] where splits > 1
+  float *dh_part, *dw_part;  // [split][rows of whole tiles][dtiles * 256] where there are several
   int add;               // dh collects an earlier piece
   int* err;
 };
@@ -394,7 +394,7 @@ template <int MODE>
 __device__ __forceinline__ int gemm_items(const GemmDev& g, int live) {
   const int mt = (live + BM - 1) / BM, vt = g.Vcp / BN;
   if (MODE != kProducts) return mt * vt;
-  return (g.d.dh.p ? mt * g.dtiles * g.splits : 0) + (g.d.dw ? vt * g.dtiles : 0);
+  return (g.d.dh.p ? mt * g.dtiles * g.splits : 0) + (g.d.dw ? vt * g.dtiles * g.wsplits : 0);
 }
 
 template <int MODE>
@@ -416,7 +416,7 @@ __device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int it
     w.n = (g.d.D + kSlab - 1) / kSlab;
     return w;
   }
-  const int nh = g.d.dh.p ? mt * g.dtiles * g.splits : 0, nw = g.d.dw ? vt * g.dtiles : 0;
+  const int nh = g.d.dh.p ? mt * g.dtiles * g.splits : 0, nw = g.d.dw ? vt * g.dtiles * g.wsplits : 0;
   bool dh = g.dh_first ? item < nh : item >= nw;
   const int i = dh ? item - (g.dh_first ? 0 : nw) : item - (g.dh_first ? nh : 0);
   if (dh) {
@@ -427,9 +427,13 @@ __device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int it
     w.k0 = min(all, w.split * g.slabs);
     w.n = min(all, w.k0 + g.slabs) - w.k0;
   } else {
-    place(i, vt, g.dtiles);
+    const int tiles = vt * g.dtiles;
+    w.split = i / tiles;
+    place(i % tiles, vt, g.dtiles);
     w.dw = true;
-    w.n = (live + kSlab - 1) / kSlab;
+    const int all = (live + kSlab - 1) / kSlab;
+    w.k0 = min(all, w.split * g.wslabs);
+    w.n = min(all, w.k0 + g.wslabs) - w.k0;
   }
   if (g.d.D - w.n0 <= BN / 2) w.cols = BN / 2;
   return w;
@@ -604,6 +608,12 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
       sd = d.dwd;
       vec = d.vec_dw;
       rows = g.Vc - row0;
+      if (g.wsplits > 1) {
+        step = (int64_t)g.dtiles * BN;
+        sd = 1;
+        to = g.dw_part + ((int64_t)w.split * g.Vcp + row) * step + col;
+        vec = true;
+      }
     } else {
       rows = live - row0;
       if (row < live) f2 = *head_row<const float>(d, d.gl, t.orig) * d.temp;
@@ -855,25 +865,28 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   if (warp == 0) pair_tmem_dealloc(tmem, 512);
 }
 
-// dh from the parts of its contraction, in order.
-__global__ void __launch_bounds__(256) head_dh_join_kernel(const __grid_constant__ GemmDev g) {
+// A row of dh, or of dw, from the parts of its contraction, in order.
+template <bool DW>
+__global__ void __launch_bounds__(256) head_parts_kernel(const __grid_constant__ GemmDev g) {
   pdl_launch_dependents();
   pdl_wait();
   const HeadDev& d = g.d;
-  const int live = *d.live, r = blockIdx.x;
-  if (r >= live) return;
-  const int64_t np = (live + BM - 1) / BM * BM, ld = (int64_t)g.dtiles * BN;
-  float* to = head_row<float>(d, d.dh, d.rows[r]);
+  const int live = *d.live, r = blockIdx.x, splits = DW ? g.wsplits : g.splits;
+  if (r >= (DW ? g.Vc : live)) return;
+  const int64_t rows = DW ? g.Vcp : (live + BM - 1) / BM * BM, ld = (int64_t)g.dtiles * BN;
+  const float* part = (DW ? g.dw_part : g.dh_part) + r * ld;
+  float* to = DW ? d.dw + (int64_t)(g.v0 + r) * d.dwv : head_row<float>(d, d.dh, d.rows[r]);
+  const int64_t sd = DW ? d.dwd : d.dh.sd;
   for (int c = blockIdx.y * 256 + threadIdx.x; c < d.D; c += gridDim.y * 256) {
-    float sum = g.add ? to[c * d.dh.sd] : 0.f;
-    for (int s0 = 0; s0 < g.splits; s0 += 8) {
+    float sum = !DW && g.add ? to[c * sd] : 0.f;
+    for (int s0 = 0; s0 < splits; s0 += 8) {
       float x[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = s0 + k < g.splits ? g.dh_part[((s0 + k) * np + r) * ld + c] : 0.f;
+      for (int k = 0; k < 8; ++k) x[k] = s0 + k < splits ? part[(s0 + k) * rows * ld + c] : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum += x[k];
     }
-    to[c * d.dh.sd] = sum;
+    to[c * sd] = sum;
   }
 }
 
@@ -967,14 +980,16 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   g.err = err;
   g.dtiles = (int)dtiles;
   const int64_t htiles = Np / BM * dtiles, wtiles = Vp / BN * dtiles;
-  g.splits = 1;
-  if (backward && d.dh.p && d.N > 0) {
-    // dh's few tiles with a long contraction: parts of about a third of a pair's share of the work, 8 slabs at least
-    const int64_t work = htiles * Vp + (d.dw ? wtiles * Np : 0);
+  g.splits = g.wsplits = 1;
+  if (backward && d.N > 0) {
+    // few tiles with a long contraction: parts of about a third of a pair's share of the work, 8 slabs at least
+    const int64_t work = (d.dh.p ? htiles * Vp : 0) + (d.dw ? wtiles * Np : 0);
     const int64_t part = std::max<int64_t>(512, work / std::max(1, sms / CG) / 3);
-    g.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Vp + part / 2) / part));
+    if (d.dh.p) g.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Vp + part / 2) / part));
+    if (d.dw) g.wsplits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Np + part / 2) / part));
   }
   g.slabs = (int)round_up((Vp / kSlab + g.splits - 1) / g.splits, kChunk);
+  g.wslabs = (int)round_up((Np / kSlab + g.wsplits - 1) / g.wsplits, kChunk);
   g.dh_first = Vp / g.splits >= d.N;
 
   // workspaces
@@ -993,6 +1008,7 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   const size_t o_gh = take(backward && d.dw ? 4 * hplane : 0), o_x = take(4 * xplane);
   const size_t o_part = take(backward ? 0 : (int64_t)sizeof(HeadPart) * parts * Np);
   const size_t o_dh = take(g.splits > 1 ? 4 * g.splits * Np * dtiles * BN : 0);
+  const size_t o_dw = take(g.wsplits > 1 ? 4 * g.wsplits * Vp * dtiles * BN : 0);
   Error e = mem.alloc(at, s);
   if (!e.ok()) return e;
   char* base = mem.as<char>();
@@ -1017,6 +1033,7 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   g.dx = xp;
   g.plane = xplane;
   g.dh_part = reinterpret_cast<float*>(base + o_dh);
+  g.dw_part = reinterpret_cast<float*>(base + o_dw);
   g.Vcp = (int)Vp;
   const int64_t av = d.wv < 0 ? -d.wv : d.wv, ad = d.wd < 0 ? -d.wd : d.wd;
   p.along_v = d.V > 1 && d.D > 1 && av < ad;
@@ -1050,11 +1067,12 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     if (e.ok()) e = map_cols(wp, g.Vc, Dp, wplane, &wc);
     gc = wc;
     if (e.ok() && d.dw) e = map_cols(gp, Np, Dp, hplane, &gc);
-    if (e.ok()) e = launch_gemm<kProducts>(xa, wc, xc, gc, g, htiles * g.splits + wtiles, s);
-    if (e.ok() && d.dh.p && g.splits > 1) {
-      e = launch_after(head_dh_join_kernel, dim3((unsigned)d.N, (unsigned)std::min<int64_t>(16, (d.D + 255) / 256)), 256, 0, s,
-                       "head hidden gradient join kernel", g);
-    }
+    if (e.ok()) e = launch_gemm<kProducts>(xa, wc, xc, gc, g, htiles * g.splits + wtiles * g.wsplits, s);
+    const unsigned across = (unsigned)std::min<int64_t>(16, (d.D + 255) / 256);
+    if (e.ok() && g.splits > 1)
+      e = launch_after(head_parts_kernel<false>, dim3((unsigned)d.N, across), 256, 0, s, "head hidden gradient join kernel", g);
+    if (e.ok() && g.wsplits > 1)
+      e = launch_after(head_parts_kernel<true>, dim3((unsigned)g.Vc, across), 256, 0, s, "head weight gradient join kernel", g);
     if (!e.ok()) return e;
   }
   if (backward) return e;
