@@ -124,7 +124,7 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
 // Hidden rows (those with a target, gathered; zeros behind the last one up to a
 // whole tile) have a power of two each, g h and the weight one per 256 rows: as
 // much as the products that contract along the rows keep in the accumulator.
-// Bound by HBM: 131 MB of weight in 58 us (262 MB read and written; 98 MB in 44 us).
+// Bound by HBM: 131 MB of weight in 50 us (262 MB read and written; 98 MB in 42 us).
 enum PackKind { kPackWeight, kPackHidden, kPackHiddenGrad };
 
 constexpr int kPackWarps = 16;
@@ -175,6 +175,13 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
       if (KIND == kPackHiddenGrad) g[j] = *head_row<const float>(d, d.gl, row) * d.temp;
     }
   }
+  constexpr int B = 4;  // 16-byte loads of each row in flight
+  auto load = [&](int j, int c) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p[j] && c < d.D)
+      asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p[j] + c));
+    return x;
+  };
   if (along_v) {
     const int v = block * 32 + lane;
     const float* w = d.w + (int64_t)(a.v0 + v) * d.wv;
@@ -188,13 +195,16 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
 #pragma unroll
         for (int j = 0; j < R; ++j) top[j] = max(top[j], p[j] ? magnitude(p[j][c * sd]) : 0u);
     }
-#pragma unroll 8
-    for (int c = lane * 4; vec && c < d.D; c += 128) {
-      float4 x[R];
+    for (int c = lane * 4; vec && c < d.D; c += 128 * B) {
+      float4 x[B][R];
 #pragma unroll
-      for (int j = 0; j < R; ++j) x[j] = p[j] && c < d.D ? *reinterpret_cast<const float4*>(p[j] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int b = 0; b < B; ++b)
 #pragma unroll
-      for (int j = 0; j < R; ++j) top[j] = max(top[j], magnitude(x[j]));
+        for (int j = 0; j < R; ++j) x[b][j] = load(j, c + 128 * b);
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int j = 0; j < R; ++j) top[j] = max(top[j], magnitude(x[b][j]));
     }
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -260,19 +270,24 @@ __device__ __forceinline__ void pack_rows(const PlanesDev& a, int block) {
     }
     return;
   }
-#pragma unroll 4
-  for (int c = lane * 4; c < a.Dp; c += 128) {
-    float4 x[R];
+  for (int c0 = lane * 4; c0 < a.Dp; c0 += 128 * B) {
+    float4 x[B][R];
 #pragma unroll
-    for (int j = 0; j < R; ++j) x[j] = p[j] && c < d.D ? *reinterpret_cast<const float4*>(p[j] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int b = 0; b < B; ++b)
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      if (KIND == kPackWeight && !p[j]) continue;
-      const int64_t at = (int64_t)(r0 + j) * a.Dp + c;
-      split_store(a.to + at, a.plane, x[j].x * ups[j], x[j].y * ups[j], x[j].z * ups[j], x[j].w * ups[j]);
-      if (KIND == kPackHiddenGrad && a.gto)
-        split_store(a.gto + at, a.plane, mul3(x[j].x, g[j], up), mul3(x[j].y, g[j], up), mul3(x[j].z, g[j], up), mul3(x[j].w, g[j], up));
-    }
+      for (int j = 0; j < R; ++j) x[b][j] = load(j, c0 + 128 * b);
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int c = c0 + 128 * b;
+        if (c >= a.Dp || (KIND == kPackWeight && !p[j])) continue;
+        const int64_t at = (int64_t)(r0 + j) * a.Dp + c;
+        const float4 y = x[b][j];
+        split_store(a.to + at, a.plane, y.x * ups[j], y.y * ups[j], y.z * ups[j], y.w * ups[j]);
+        if (KIND == kPackHiddenGrad && a.gto)
+          split_store(a.gto + at, a.plane, mul3(y.x, g[j], up), mul3(y.y, g[j], up), mul3(y.z, g[j], up), mul3(y.w, g[j], up));
+      }
   }
 }
 
