@@ -292,7 +292,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
 
 struct HeadGradDev {
   HeadDev d;
-  int lg;                // 2^lg threads (whole warps) along the width, the rest along the vocabulary
+  int lg;                // head_grad_kernel: 2^lg threads along the width, the rest along the vocabulary
+  int slices, parts;     // head_columns_kernel: warps along the width, along the vocabulary
   const float* dx;
   float* part;           // [part of the vocabulary][NR][D] of dh
   int* err;
@@ -321,8 +322,9 @@ __device__ __forceinline__ void step_copy(const HeadDev& d, float* to, int64_t v
   if (lane < rows) bulk_g2s(to + lane * PITCH, d.w + (v + lane) * d.wv + c, bytes, bar);
 }
 
-// dw and a part of dh of 8 NT call rows for 128 / NT columns per warp: 2^lg warps along
-// the width, the others (and blockIdx.y) along the vocabulary, 16 rows of it a step.
+// dw and a part of dh of 8 NT call rows for 128 / NT columns per warp: as many warps as
+// the width takes, one after another, then the next part of the vocabulary, 16 rows of
+// it a step.
 //   dw: rows of dx as the left operand, h as the right one, in registers for good:
 //       column 4 (m / 2) + m % 2 of a block of 16 is column m of one MMA, the one 2
 //       to its right of the other, so that a lane ends with four neighbours
@@ -334,13 +336,11 @@ __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const _
   __shared__ uint64_t full[kColWarps][kColSteps];
   const HeadDev& d = a.d;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, lg = lane / 4, lt = lane % 4;
-  const int across = 1 << a.lg, down = kColWarps >> a.lg;
-  const int c0 = (blockIdx.x * across + (warp & (across - 1))) * CW;
-  const int part = blockIdx.y * down + (warp >> a.lg), parts = gridDim.y * down;
+  const int at_w = blockIdx.x * kColWarps + warp, parts = a.parts, part = at_w / a.slices, c0 = at_w % a.slices * CW;
   float* ring = reinterpret_cast<float*>(s_raw) + warp * (kColSteps * STEP);
   pdl_launch_dependents();
   pdl_wait();
-  if (c0 >= d.D) return;
+  if (part >= parts) return;
   if (lane == 0) {
     for (int s = 0; s < kColSteps; ++s) mbar_init(&full[warp][s], 1);
     fence_mbar_init();
@@ -616,9 +616,12 @@ __global__ void __launch_bounds__(256) head_grad_join_kernel(const __grid_consta
 template <int NT, bool GRAD>
 Error launch_scores(HeadRowsDev& a, cudaStream_t s) {
   const HeadDev& d = a.d;
-  // 8 blocks per warp at least
+  // 8 blocks per warp, or half as many warps where that leaves fewer of them idle (width
+  // 1360: 85 blocks are 16 shares of 6, of which 11 too many, or 8 of 11)
   a.lg = 0;
   while (a.lg < 4 && (8 << a.lg) < a.blocks) ++a.lg;
+  auto taken = [&](int lg) { return ((a.blocks + (1 << lg) - 1) >> lg) << lg; };
+  if (a.lg > 0 && taken(a.lg - 1) < taken(a.lg)) --a.lg;
   const int teams = (kFewThreads / 32) >> a.lg;
   const int ctas = std::max(1, std::min(current_device_info().sm_count, (d.V + 16 * teams - 1) / (16 * teams)));
   const int smem = 4 * (kFewThreads / 32) * 512 + 8 * NT * (a.blocks + 1) * 64;
@@ -654,20 +657,19 @@ Error head_few(const HeadDev& d, bool backward, cudaStream_t s) {
   g.d = d;
   g.err = async_error_word();
   if (!g.err) return make_error(TRS_ERR_CUDA, "head: no async-error word");
-  int splits, parts;  // of the vocabulary: CTAs, and those times a CTA's own
-  unsigned across;    // CTAs along the width
+  int parts;  // of the vocabulary
+  dim3 grid;
   if (d.vec_w) {
     const int columns = 128 / nt;
-    while (g.lg < 3 && (columns << g.lg) < d.D) ++g.lg;
-    across = (unsigned)((d.D + (columns << g.lg) - 1) / (columns << g.lg));
-    splits = std::max(1, std::min((d.V + 15) / 16, sms / (int)across));
-    parts = splits * (kColWarps >> g.lg);
+    g.slices = (d.D + columns - 1) / columns;
+    parts = g.parts = std::max(1, std::min((d.V + 15) / 16, sms * kColWarps / g.slices));
+    grid = dim3((unsigned)((g.slices * parts + kColWarps - 1) / kColWarps));
   } else {
     g.lg = 5;
     while (g.lg < 8 && (1 << g.lg) < (d.D + 3) / 4) ++g.lg;
-    across = (unsigned)((d.D + 1023) / 1024);
-    splits = std::max(1, std::min((d.V + 31) / 32, 2 * sms / (int)across));
+    const int across = (d.D + 1023) / 1024, splits = std::max(1, std::min((d.V + 31) / 32, 2 * sms / across));
     parts = splits * (256 >> g.lg);
+    grid = dim3((unsigned)across, (unsigned)splits);
   }
   const size_t nd = (size_t)d.V * 8 * nt;
   e = mem.alloc(sizeof(float) * (nd + (size_t)parts * 8 * nt * d.D), s);
@@ -677,7 +679,6 @@ Error head_few(const HeadDev& d, bool backward, cudaStream_t s) {
   if (!e.ok()) return e;
   g.dx = a.dx;
   g.part = a.dx + nd;
-  const dim3 grid(across, (unsigned)splits);
   if (!d.vec_w) {
     e = launch_after(head_grad_kernel, grid, 256, 0, s, "head gradient kernel", g);
   } else {

@@ -407,19 +407,27 @@ struct GemmDev {
 // A tile: rows from m0, columns from n0, `n` slabs of the contraction from k0.
 struct GemmItem {
   int m0, n0, k0, n, split;
-  int cols;              // of the tile: 256, or 128 where no more are left
+  int cols;              // of the tile: 256, or 128
   bool dw;
 };
 
+// Scores: tiles that are left over by whole rounds of all pairs are taken in halves
+// of 128 columns where those fit one round (250 tiles over 74 pairs: 58 us, so 55; a
+// step of 6 tiles of 2688 elements 205 us, so 162).
+__device__ __forceinline__ int gemm_halved(int tiles, int pairs) {
+  const int rest = tiles % pairs;
+  return 2 * rest <= pairs ? rest : 0;
+}
+
 template <int MODE>
-__device__ __forceinline__ int gemm_items(const GemmDev& g, int live) {
+__device__ __forceinline__ int gemm_items(const GemmDev& g, int live, int pairs) {
   const int mt = (live + BM - 1) / BM, vt = g.Vcp / BN;
-  if (MODE != kProducts) return mt * vt;
+  if (MODE != kProducts) return mt * vt + gemm_halved(mt * vt, pairs);
   return (g.d.dh.p ? mt * g.dtiles * g.splits : 0) + (g.d.dw ? vt * g.dtiles * g.wsplits : 0);
 }
 
 template <int MODE>
-__device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int item) {
+__device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int item, int pairs) {
   const int mt = (live + BM - 1) / BM, vt = g.Vcp / BN;
   GemmItem w;
   w.k0 = 0;
@@ -433,7 +441,12 @@ __device__ __forceinline__ GemmItem gemm_item(const GemmDev& g, int live, int it
     w.n0 = at / high * BN;
   };
   if (MODE != kProducts) {
-    place(item, mt, vt);
+    const int whole = mt * vt - gemm_halved(mt * vt, pairs), over = item - whole;
+    place(over < 0 ? item : whole + over / 2, mt, vt);
+    if (over >= 0) {
+      w.n0 += over % 2 * (BN / 2);
+      w.cols = BN / 2;
+    }
     w.n = (g.d.D + kSlab - 1) / kSlab;
     return w;
   }
@@ -741,7 +754,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
   pdl_launch_dependents();
   pdl_wait();  // everything from here on reads what earlier kernels wrote
   const int live = *g.d.live;
-  const int items = gemm_items<MODE>(g, live), pairs = gridDim.x / CG, pair = blockIdx.x / CG;
+  const int pairs = gridDim.x / CG, pair = blockIdx.x / CG, items = gemm_items<MODE>(g, live, pairs);
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLean));
@@ -749,7 +762,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
       int li = 0;
       bool ok = true;
       for (int item = pair; item < items && ok; item += pairs) {
-        const GemmItem w = gemm_item<MODE>(g, live, item);
+        const GemmItem w = gemm_item<MODE>(g, live, item, pairs);
         for (int i = 0; i < w.n; ++i, ++li) {
           const int s = li % kStages;
           if (li >= kStages && !(ok = wait_or_fail(&empty[s], (uint32_t)(li / kStages - 1) & 1u, failed))) break;
@@ -784,7 +797,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
       int li = 0, ci = 0;
       bool ok = true;
       for (int item = pair; item < items && ok; item += pairs) {
-        const GemmItem w = gemm_item<MODE>(g, live, item);
+        const GemmItem w = gemm_item<MODE>(g, live, item, pairs);
         const bool amn = MODE == kProducts && w.dw, bmn = MODE == kProducts;
         const uint32_t idesc = uniform((1u << 4) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u) |
                                        ((uint32_t)(w.cols >> 3) << 17) | ((uint32_t)(BM >> 4) << 24));
@@ -824,7 +837,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
     int ci = 0;
     bool ok = true;
     for (int item = pair; item < items && ok; item += pairs) {
-      const GemmItem w = gemm_item<MODE>(g, live, item);
+      const GemmItem w = gemm_item<MODE>(g, live, item, pairs);
       TileRow t;
       t.row = w.m0 + (int)rank * 128 + rl;
       t.col = w.n0 + half * 128;
@@ -874,7 +887,7 @@ head_gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__
         __syncwarp();
         if (lane == 0) pair_arrive(bars[ci & 1]);
       }
-      if (ok) finish_tile<MODE>(g, w, live, t, bufs + warp * (kWarpBuf / 4), lane, acc);
+      if (ok && half * 128 < w.cols) finish_tile<MODE>(g, w, live, t, bufs + warp * (kWarpBuf / 4), lane, acc);
     }
   }
   if (threadIdx.x % 32 == 0 && *(volatile int*)failed) atomicOr(g.err, kAsyncWaitTimeout);
@@ -1078,11 +1091,11 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     if (!e.ok()) return e;
     const int64_t tiles = Np / BM * (g.Vcp / BN);
     if (!backward) {
-      e = launch_gemm<kScores>(ha, wb, ha, wb, g, tiles, s);
+      e = launch_gemm<kScores>(ha, wb, ha, wb, g, 2 * tiles, s);
       if (!e.ok()) return e;
       continue;
     }
-    e = launch_gemm<kScoreGrad>(ha, wb, ha, wb, g, tiles, s);
+    e = launch_gemm<kScoreGrad>(ha, wb, ha, wb, g, 2 * tiles, s);
     if (e.ok()) e = map_rows(xp, Np, Vp, xplane, 128, &xa);
     if (e.ok()) e = map_cols(xp, Np, Vp, xplane, &xc);
     if (e.ok()) e = map_cols(wp, g.Vc, Dp, wplane, &wc);
