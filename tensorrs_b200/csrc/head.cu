@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
   extern __shared__ int s_id[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int row = blockIdx.x * 8 + warp;
+  pdl_wait();  // before the line below: see head_list_kernel
   pdl_launch_dependents();
   if (row >= d.N) return;
   int* ids = s_id + warp * 2 * d.K;
@@ -93,8 +94,13 @@ __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
 // get their loss and lse of 0.
 __global__ void __launch_bounds__(1024) head_list_kernel(const HeadDev d) {
   __shared__ int warps[32];
-  pdl_launch_dependents();
+  // What runs next may read the call's inputs and write its workspaces without waiting
+  // for this kernel: it must not begin before the call's first kernel has waited for
+  // all that came before the call.  With a teacher's rows that kernel is theirs.
+  const bool first = !d.distill || d.N == 0;
+  if (!first) pdl_launch_dependents();
   pdl_wait();
+  if (first) pdl_launch_dependents();
   constexpr int U = 4;  // consecutive rows of a thread
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int done = 0;
@@ -317,8 +323,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (c.distill && N > 0) {
     const int smem = 8 * 2 * d.K * 4;
     allow_smem((const void*)head_teacher_kernel, smem);
-    head_teacher_kernel<<<(unsigned)((N + 7) / 8), 256, smem, stream>>>(d);
-    e = check_launch("head teacher kernel");
+    e = launch_after(head_teacher_kernel, dim3((unsigned)((N + 7) / 8)), 256, smem, stream, "head teacher kernel", d);
     if (!e.ok()) return e;
   }
   if (few) return head_few(d, c.backward, stream);

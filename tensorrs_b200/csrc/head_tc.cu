@@ -297,7 +297,9 @@ template <int HKIND>
 __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(kPackWarps * 32)
 head_pack_kernel(const __grid_constant__ PlanesDev h, const __grid_constant__ PlanesDev w, int hidden) {
   pdl_launch_dependents();
-  pdl_wait();
+  // next to the hidden rows the kernel before is the list's, which the weight does not need, and which lets this one
+  // begin only when all before it has ended
+  if ((int)blockIdx.x < hidden || hidden == 0) pdl_wait();
   if ((int)blockIdx.x < hidden) pack_rows<HKIND>(h, blockIdx.x);
   else pack_rows<kPackWeight>(w, blockIdx.x - hidden);
 }
