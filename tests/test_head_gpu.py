@@ -387,6 +387,29 @@ def test_streams_and_graphs():
     assert all(torch.equal(x, y) for x, y in zip(outs[0], want[1]))
 
 
+@pytest.mark.parametrize("N", [4, 30, 150, 700])
+@pytest.mark.parametrize("kind", [SMOOTH, KD7], ids=["ce", "kd"])
+def test_a_weight_from_the_call_before(kind, N):
+    """Each call's weight is what the call before it has just written: bit for bit the results of calls one at a time."""
+    c = Case(N, 5000, 192, kind, masked=0.2)
+    runs = []
+    for wait in (True, False):
+        w = V_(c.d["w"])
+        shapes = [(N,), (N,), (N, c.D), (c.V, c.D)] * 6  # all there before the first call: nothing runs between the calls
+        out = [torch.full(s, np.nan, device="cuda") for s in shapes]
+        for i in range(0, len(out), 4):
+            c.forward(*out[i : i + 2], w=w)
+            if wait:
+                torch.cuda.synchronize()
+            c.backward(out[i + 1], *out[i + 2 : i + 4], w=w)
+            if wait:
+                torch.cuda.synchronize()
+            w = V_(out[i + 3])
+        runs.append([to_host(x) for x in out])
+    for i, (a, b) in enumerate(zip(*runs)):
+        np.testing.assert_array_equal(a, b, err_msg=f"result {i}")
+
+
 def test_a_step_of_a_tied_model():
     """Embedding, the last layer on the same table, both gradients added up, one Adam step: a model of one table, against
     the same steps in 64 bits."""
