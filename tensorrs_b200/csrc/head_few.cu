@@ -13,11 +13,12 @@
 //                        16 bytes, or columns apart), by plain loads
 //   head_grad_join_kernel  dh from the parts of the vocabulary, in order
 //
-// TF32 products: x = hi + lo, 11 significant bits each; hi hi + hi lo + lo hi, with
-// the sums taken over to f32 additions every 256 elements, since the tensor core cuts
-// instead of rounding.
+// TF32 products: x = hi + lo, 11 significant bits each; lo hi + hi lo + hi hi, with
+// the sums taken over to f32 additions every 16 elements, since the tensor core cuts
+// instead of rounding (the small products first; all of a warp's columns in one sum:
+// 1.1e-6 of the lse of rows of 2944 and more).
 //
-// Measured, 32000 x 1024 (131 MB): scores of 4 rows 30 us (of 131072 x 1024 97: 5.5
+// Measured, 32000 x 1024 (131 MB): scores of 4 rows 31 us (of 131072 x 1024 97: 5.5
 // TB/s), dw and dh of 8 rows 51 us (262 MB read and written: 5.1 TB/s).  On the way:
 // dot products on the CUDA cores, two steps of 512 bytes per warp in flight, 31 us
 // for 4 rows and 44 for 8; a ring of bulk copies per CTA 36 and 40, per warp 39 and
@@ -67,10 +68,20 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo, hi its upper 11 significant bits; the tensor core reads the upper 11 of lo.
-__device__ __forceinline__ void tf32_split(float x, uint32_t* hi, uint32_t* lo) {
+// x = hi + lo; the tensor core reads the upper 11 bits of lo.  hi: x's upper 11
+// significant bits for the weight, and for the other operand x rounded to 11 (to the
+// largest such number where that would overflow), so that lo has either sign and the
+// products lo lo, which are left out, add up to nothing (both cut: 3e-7 of every sum,
+// and ten times that of the gradients of scores of 10; both rounded: 2 us of 32).
+__device__ __forceinline__ void tf32_cut(float x, uint32_t* hi, uint32_t* lo) {
   *hi = __float_as_uint(x) & 0xFFFFE000u;
   *lo = __float_as_uint(x - __uint_as_float(*hi));
+}
+__device__ __forceinline__ void tf32_split(float x, uint32_t* hi, uint32_t* lo) {
+  const float top = __uint_as_float(0x7F7FE000u);
+  const float h = fminf(fmaxf(__uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u), -top), top);
+  *hi = __float_as_uint(h);
+  *lo = __float_as_uint(x - h);
 }
 
 // The call rows of this block and, from shared memory [NR][pitch], their elements
@@ -100,10 +111,10 @@ __device__ __forceinline__ void few_block(const float4 (&y)[2], const float* h, 
   uint32_t hi[2][4], lo[2][4];  // [columns 0 and 1, columns 2 and 3]
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    tf32_split(y[j].x, &hi[0][j], &lo[0][j]);
-    tf32_split(y[j].y, &hi[0][2 + j], &lo[0][2 + j]);
-    tf32_split(y[j].z, &hi[1][j], &lo[1][j]);
-    tf32_split(y[j].w, &hi[1][2 + j], &lo[1][2 + j]);
+    tf32_cut(y[j].x, &hi[0][j], &lo[0][j]);
+    tf32_cut(y[j].y, &hi[0][2 + j], &lo[0][2 + j]);
+    tf32_cut(y[j].z, &hi[1][j], &lo[1][j]);
+    tf32_cut(y[j].w, &hi[1][2 + j], &lo[1][2 + j]);
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
@@ -113,12 +124,16 @@ __device__ __forceinline__ void few_block(const float4 (&y)[2], const float* h, 
     tf32_split(x.y, &hh[1], &hl[1]);
     tf32_split(x.z, &hh[2], &hl[2]);
     tf32_split(x.w, &hh[3], &hl[3]);
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      mma_tf32(part[i], lo[k], hh[2 * k], hh[2 * k + 1]);
-      mma_tf32(part[i], hi[k], hl[2 * k], hl[2 * k + 1]);
-      mma_tf32(part[i], hi[k], hh[2 * k], hh[2 * k + 1]);
+      mma_tf32(sum, lo[k], hh[2 * k], hh[2 * k + 1]);
+      mma_tf32(sum, hi[k], hl[2 * k], hl[2 * k + 1]);
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) mma_tf32(sum, hi[k], hh[2 * k], hh[2 * k + 1]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[i][j] += sum[j];
   }
 }
 struct HeadRowsDev {
@@ -468,7 +483,7 @@ __global__ void __launch_bounds__(kColWarps * 32, 1) head_columns_kernel(const _
         for (int i = 0; i < 4; ++i) {
           uint32_t wh[4], wl[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) tf32_split(y[e][i], &wh[e], &wl[e]);
+          for (int e = 0; e < 4; ++e) tf32_cut(y[e][i], &wh[e], &wl[e]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma_tf32(sum[i][n], wl, bh[n][2 * p], bh[n][2 * p + 1]);
