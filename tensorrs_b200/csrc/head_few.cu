@@ -261,10 +261,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
       if (GRAD) {
         dx[(int64_t)v * NR + fn] = row < 0 ? 0.f : gr * (head_ex2(z - lse2) - t - d.share);
       } else {
-        const float m = fmaxf(pt.m, z);
-        pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(z - m);
-        if (m == -INFINITY) pt.s = 0.f;  // scores of -inf alone
-        pt.m = m;
+        // a score of -inf adds nothing, and must not meet the maximum of -inf that a thread
+        // begins with; a NaN, which the maximum passes over, makes the sum NaN for good
+        if (z != -INFINITY) {
+          const float m = fmaxf(pt.m, z);
+          pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(z - m);
+          pt.m = m;
+        }
         if (t != 0.f) pt.dot = __fmaf_rn(t, z, pt.dot);
         pt.sum += z;
       }

@@ -301,6 +301,26 @@ def test_infinities_stay_in_their_rows(N):
         check_all(c, t, loss, lse, *c.backward(lse))
 
 
+@pytest.mark.parametrize("N", [4, 17, 130])
+@pytest.mark.parametrize("kind", [CE, KD7], ids=["ce", "kd"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_bad_weight_rows(bad, kind, N):
+    """A row of the vocabulary that is no longer a number, wherever it lies and whoever's target it is, shows in the loss
+    and lse of every token (f32: 0 inf and inf - inf are NaN), and in no masked one."""
+    for V in (300, 10_007):
+        c = Case(N, V, 48, kind, 0.2)
+        live = np.array([e is not None for e in c.entries], bool)
+        for rows in ([0], [V // 2], [V - 1], [0, 1, 2], [0, V // 3, V - 1]):
+            w = c.d["w"].clone()
+            w[rows, 7] = bad
+            loss, lse = (to_host(x) for x in c.forward(w=V_(w)))
+            assert not np.isfinite(loss[live]).any() and not np.isfinite(lse[live]).any(), (V, rows)
+            assert not loss[~live].any() and not lse[~live].any()
+        w = torch.full_like(c.d["w"], bad)  # nothing else
+        loss, lse = (to_host(x) for x in c.forward(w=V_(w)))
+        assert not np.isfinite(loss[live]).any() and not np.isfinite(lse[live]).any()
+
+
 def test_large_vocabulary():
     """140000 tokens, and the weight as a view past 2^31 elements."""
     N, V, D = 300, 140_000, 64
