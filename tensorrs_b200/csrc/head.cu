@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
     if (ids[k] != kNoToken) {
       const float a = __fdiv_rn(ps[k] - top, d.temp);
       p = __fdiv_rn(expf(a), sum);
-      ent += (double)p * (double)(a - ln_sum);
+      if (p != 0.f) ent += (double)p * (double)(a - ln_sum);  // 0 ln 0 = 0; a may have left f32's range
     }
     ps[k] = p;
   }

@@ -321,6 +321,24 @@ def test_bad_weight_rows(bad, kind, N):
         assert not np.isfinite(loss[live]).any() and not np.isfinite(lse[live]).any()
 
 
+@pytest.mark.parametrize("N", [4, 130])
+@pytest.mark.parametrize("temperature", [0.5, 2.0**-10, 3.0])
+@pytest.mark.parametrize("low", [-np.finfo(np.float32).max, -1e30])
+def test_lowest_teacher_logits(low, temperature, N):
+    """Entries masked by a logit far below the others have no share, also where its quotient by the temperature is no f32;
+    where a row has no others they share alike."""
+    c = Case(N, 300, 48, ("kd", 9, temperature))
+    c.z[:, 2::3] = low
+    c.z[1, :] = low
+    c.z[3, 1:] = low
+    c.entries = ref.teacher(c.ids, c.z, 300, temperature)
+    c.d["z"] = cuda(c.z)
+    t = c.truth()
+    loss, lse = c.forward()
+    assert np.isfinite(to_host(loss)).all()
+    check_all(c, t, loss, lse, *c.backward(lse))
+
+
 def test_large_vocabulary():
     """140000 tokens, and the weight as a view past 2^31 elements."""
     N, V, D = 300, 140_000, 64
