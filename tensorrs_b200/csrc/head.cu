@@ -96,7 +96,8 @@ __global__ void __launch_bounds__(1024) head_list_kernel(const HeadDev d) {
   __shared__ int warps[32];
   // What runs next may read the call's inputs and write its workspaces without waiting
   // for this kernel: it must not begin before the call's first kernel has waited for
-  // all that came before the call.  With a teacher's rows that kernel is theirs.
+  // all that came before the call (so the workspaces were taken before that launch).
+  // With a teacher's rows that kernel is theirs.
   const bool first = !d.distill || d.N == 0;
   if (!first) pdl_launch_dependents();
   pdl_wait();
@@ -311,10 +312,16 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   // the rows' targets
   Scratch mem;
   const size_t n = ((size_t)N + 3) / 4 * 4, nk = ((size_t)N * K + 3) / 4 * 4;
-  if (!few || c.distill) {
-    e = mem.alloc(4 * (n + 4 + 2 * nk + (c.distill ? n : 0)), stream);
+  HeadTcPlan plan;
+  if (!few) {
+    e = head_tc_plan(d, c.backward, &plan);
     if (!e.ok()) return e;
-    d.live = mem.as<int>();
+  }
+  const size_t tc = few ? 0 : plan.bytes;
+  if (!few || c.distill) {
+    e = mem.alloc(tc + 4 * (n + 4 + 2 * nk + (c.distill ? n : 0)), stream);
+    if (!e.ok()) return e;
+    d.live = reinterpret_cast<int*>(mem.as<char>() + tc);
     d.rows = d.live + 4;
     d.eid = d.rows + n;
     d.ew = reinterpret_cast<float*>(d.eid + nk);
@@ -329,7 +336,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   if (few) return head_few(d, c.backward, stream);
   e = launch_after(head_list_kernel, dim3(1), 1024, 0, stream, "head list kernel", d);
   if (!e.ok()) return e;
-  return head_tc(d, c.backward, stream);
+  return head_tc(d, c.backward, plan, mem.as<char>(), stream);
 }
 
 trs_status finish(const Error& e) {

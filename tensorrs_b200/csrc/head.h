@@ -144,7 +144,20 @@ inline bool head_few_takes(const HeadDev& d, bool backward) {
   return d.N <= 8 || (d.N <= 16 && d.vec_w && d.D <= 2560);
 }
 Error head_few(const HeadDev& d, bool backward, cudaStream_t stream);
-// More rows, or none (head_tc.cu).
-Error head_tc(const HeadDev& d, bool backward, cudaStream_t stream);
+// More rows, or none (head_tc.cu).  How the work is cut, and where its workspaces lie
+// in `bytes` of memory, which the call takes before its first launch: its first planes
+// are written without waiting for the kernel before them, so the memory must not come
+// from anything that was issued, on the same stream by another host thread, after that
+// launch.
+struct HeadTcPlan {
+  int64_t Np, Dp, dtiles;        // rows and width of the planes, tiles along the width
+  int64_t Vp, pieces;            // rows of a piece of the vocabulary
+  int64_t htiles, wtiles;
+  int splits, wsplits;           // parts of dh's and dw's contraction
+  size_t wdown, gdown, hdown, h, w, gh, x, part, dh, dw;  // offsets
+  size_t bytes;
+};
+Error head_tc_plan(const HeadDev& d, bool backward, HeadTcPlan* plan);
+Error head_tc(const HeadDev& d, bool backward, const HeadTcPlan& plan, char* base, cudaStream_t stream);
 
 }  // namespace trs

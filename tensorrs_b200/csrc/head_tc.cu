@@ -297,8 +297,9 @@ template <int HKIND>
 __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(kPackWarps * 32)
 head_pack_kernel(const __grid_constant__ PlanesDev h, const __grid_constant__ PlanesDev w, int hidden) {
   pdl_launch_dependents();
-  // next to the hidden rows the kernel before is the list's, which the weight does not need, and which lets this one
-  // begin only when all before it has ended
+  // next to the hidden rows the weight does not need the call's kernels before it, the first of which lets others begin
+  // only when all that came before the call has ended (kernels of another thread's call may lie between; the memory
+  // written here was taken before either)
   if ((int)blockIdx.x < hidden || hidden == 0) pdl_wait();
   if ((int)blockIdx.x < hidden) pack_rows<HKIND>(h, blockIdx.x);
   else pack_rows<kPackWeight>(w, blockIdx.x - hidden);
@@ -997,59 +998,69 @@ constexpr int64_t kPieceBytes = 512ll << 20;  // planes of a piece
 
 }  // namespace
 
-Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
+Error head_tc_plan(const HeadDev& d, bool backward, HeadTcPlan* out) {
+  HeadTcPlan& p = *out;
+  std::memset(static_cast<void*>(&p), 0, sizeof(p));
   const int sms = current_device_info().sm_count;
-  const int64_t Np = round_up(std::max(d.N, 1), BM), Dp = round_up(d.D, kSlab), dtiles = (d.D + BN - 1) / BN;
+  p.Np = round_up(std::max(d.N, 1), BM);
+  p.Dp = round_up(d.D, kSlab);
+  p.dtiles = (d.D + BN - 1) / BN;
   // pieces of the vocabulary of one size, whole tiles each
-  const int64_t row_bytes = 4 * Dp + (backward ? 4 * Np : 0);
-  int64_t pieces = std::max<int64_t>(1, (round_up(d.V, BN) * row_bytes + kPieceBytes - 1) / kPieceBytes);
-  const int64_t Vp = round_up((d.V + pieces - 1) / pieces, BN);
-  pieces = (d.V + Vp - 1) / Vp;
-  if (Np / BM * std::max(Vp / BN, dtiles * 64) + Vp / BN * dtiles >= (1ll << 31))
+  const int64_t row_bytes = 4 * p.Dp + (backward ? 4 * p.Np : 0);
+  p.pieces = std::max<int64_t>(1, (round_up(d.V, BN) * row_bytes + kPieceBytes - 1) / kPieceBytes);
+  p.Vp = round_up((d.V + p.pieces - 1) / p.pieces, BN);
+  p.pieces = (d.V + p.Vp - 1) / p.Vp;
+  if (p.Np / BM * std::max(p.Vp / BN, p.dtiles * 64) + p.Vp / BN * p.dtiles >= (1ll << 31))
     return make_error(TRS_ERR_SHAPE, "head: 2^31 or more tiles of 256 x 256");
-  int* err = async_error_word();
-  if (!err) return make_error(TRS_ERR_CUDA, "head: no async-error word");
-
-  GemmDev g;
-  std::memset(static_cast<void*>(&g), 0, sizeof(g));
-  g.d = d;
-  g.err = err;
-  g.dtiles = (int)dtiles;
-  const int64_t htiles = Np / BM * dtiles, wtiles = Vp / BN * dtiles;
-  g.splits = g.wsplits = 1;
+  p.htiles = p.Np / BM * p.dtiles;
+  p.wtiles = p.Vp / BN * p.dtiles;
+  p.splits = p.wsplits = 1;
   if (backward && d.N > 0) {
     // few tiles with a long contraction: parts of about a third of a pair's share of the work, 8 slabs at least
-    const int64_t work = (d.dh.p ? htiles * Vp : 0) + (d.dw ? wtiles * Np : 0);
+    const int64_t work = (d.dh.p ? p.htiles * p.Vp : 0) + (d.dw ? p.wtiles * p.Np : 0);
     const int64_t part = std::max<int64_t>(512, work / std::max(1, sms / CG) / 3);
-    if (d.dh.p) g.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Vp + part / 2) / part));
-    if (d.dw) g.wsplits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (Np + part / 2) / part));
+    if (d.dh.p) p.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (p.Vp + part / 2) / part));
+    if (d.dw) p.wsplits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (p.Np + part / 2) / part));
   }
-  g.slabs = (int)round_up((Vp / kSlab + g.splits - 1) / g.splits, kChunk);
-  g.wslabs = (int)round_up((Np / kSlab + g.wsplits - 1) / g.wsplits, kChunk);
-  g.dh_first = Vp / g.splits >= d.N;
-
-  // workspaces
-  Scratch mem;
-  const int64_t hplane = Np * Dp, wplane = Vp * Dp, xplane = backward ? Np * Vp : 0;
-  const int64_t parts = Vp * pieces / 128;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t here = at;
     at += (size_t)round_up(bytes, 256);
     return here;
   };
-  const int64_t tiles256 = Vp * pieces / BN;
-  const size_t o_wdown = take(4 * tiles256), o_gdown = take(4 * (Np / 256)), o_hdown = take(4 * Np), o_h = take(4 * hplane),
-               o_w = take(4 * wplane);
-  const size_t o_gh = take(backward && d.dw ? 4 * hplane : 0), o_x = take(4 * xplane);
-  const size_t o_part = take(backward ? 0 : (int64_t)sizeof(HeadPart) * parts * Np);
-  const size_t o_dh = take(g.splits > 1 ? 4 * g.splits * Np * dtiles * BN : 0);
-  const size_t o_dw = take(g.wsplits > 1 ? 4 * g.wsplits * Vp * dtiles * BN : 0);
-  Error e = mem.alloc(at, s);
-  if (!e.ok()) return e;
-  char* base = mem.as<char>();
-  __half *hp = reinterpret_cast<__half*>(base + o_h), *wp = reinterpret_cast<__half*>(base + o_w);
-  __half *gp = reinterpret_cast<__half*>(base + o_gh), *xp = reinterpret_cast<__half*>(base + o_x);
+  p.wdown = take(4 * (p.Vp * p.pieces / BN));
+  p.gdown = take(4 * (p.Np / 256));
+  p.hdown = take(4 * p.Np);
+  p.h = take(4 * p.Np * p.Dp);
+  p.w = take(4 * p.Vp * p.Dp);
+  p.gh = take(backward && d.dw ? 4 * p.Np * p.Dp : 0);
+  p.x = take(backward ? 4 * p.Np * p.Vp : 0);
+  p.part = take(backward ? 0 : (int64_t)sizeof(HeadPart) * (p.Vp * p.pieces / 128) * p.Np);
+  p.dh = take(p.splits > 1 ? 4 * p.splits * p.Np * p.dtiles * BN : 0);
+  p.dw = take(p.wsplits > 1 ? 4 * p.wsplits * p.Vp * p.dtiles * BN : 0);
+  p.bytes = at;
+  return Error{};
+}
+
+Error head_tc(const HeadDev& d, bool backward, const HeadTcPlan& plan, char* base, cudaStream_t s) {
+  const int64_t Np = plan.Np, Dp = plan.Dp, Vp = plan.Vp, pieces = plan.pieces, htiles = plan.htiles, wtiles = plan.wtiles;
+  int* err = async_error_word();
+  if (!err) return make_error(TRS_ERR_CUDA, "head: no async-error word");
+  Error e;
+  GemmDev g;
+  std::memset(static_cast<void*>(&g), 0, sizeof(g));
+  g.d = d;
+  g.err = err;
+  g.dtiles = (int)plan.dtiles;
+  g.splits = plan.splits;
+  g.wsplits = plan.wsplits;
+  g.slabs = (int)round_up((Vp / kSlab + g.splits - 1) / g.splits, kChunk);
+  g.wslabs = (int)round_up((Np / kSlab + g.wsplits - 1) / g.wsplits, kChunk);
+  g.dh_first = Vp / g.splits >= d.N;
+
+  const int64_t hplane = Np * Dp, wplane = Vp * Dp, xplane = backward ? Np * Vp : 0;
+  __half *hp = reinterpret_cast<__half*>(base + plan.h), *wp = reinterpret_cast<__half*>(base + plan.w);
+  __half *gp = reinterpret_cast<__half*>(base + plan.gh), *xp = reinterpret_cast<__half*>(base + plan.x);
 
   PlanesDev hid, p;
   std::memset(static_cast<void*>(&p), 0, sizeof(p));
@@ -1059,17 +1070,17 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
   hid.to = hp;
   hid.gto = backward && d.dw ? gp : nullptr;
   hid.plane = hplane;
-  hid.down = reinterpret_cast<float*>(base + o_hdown);
-  hid.gdown = reinterpret_cast<float*>(base + o_gdown);
+  hid.down = reinterpret_cast<float*>(base + plan.hdown);
+  hid.gdown = reinterpret_cast<float*>(base + plan.gdown);
 
-  g.hdown = reinterpret_cast<float*>(base + o_hdown);
+  g.hdown = reinterpret_cast<float*>(base + plan.hdown);
   g.gdown = hid.gdown;
-  g.part = reinterpret_cast<HeadPart*>(base + o_part);
+  g.part = reinterpret_cast<HeadPart*>(base + plan.part);
   g.ld = backward ? Vp : Np;
   g.dx = xp;
   g.plane = xplane;
-  g.dh_part = reinterpret_cast<float*>(base + o_dh);
-  g.dw_part = reinterpret_cast<float*>(base + o_dw);
+  g.dh_part = reinterpret_cast<float*>(base + plan.dh);
+  g.dw_part = reinterpret_cast<float*>(base + plan.dw);
   g.Vcp = (int)Vp;
   const int64_t av = d.wv < 0 ? -d.wv : d.wv, ad = d.wd < 0 ? -d.wd : d.wd;
   p.along_v = d.V > 1 && d.D > 1 && av < ad;
@@ -1080,7 +1091,7 @@ Error head_tc(const HeadDev& d, bool backward, cudaStream_t s) {
     g.add = i > 0;
     p.to = wp;
     p.plane = wplane;
-    p.down = reinterpret_cast<float*>(base + o_wdown) + i * (Vp / BN);
+    p.down = reinterpret_cast<float*>(base + plan.wdown) + i * (Vp / BN);
     g.wdown = p.down;
     p.v0 = g.v0;
     p.n = g.Vc;

@@ -425,6 +425,45 @@ def test_streams_and_graphs():
     assert all(torch.equal(x, y) for x, y in zip(outs[0], want[1]))
 
 
+def test_threads_on_one_stream():
+    """Host threads that issue whole steps on one stream, in whatever order: bit for bit the results of one thread.  The
+    vocabulary leaves SMs free, so that kernels of both can run at once."""
+    import threading
+
+    cases = [Case(200, 900, 320, KD7, 0.1, seed=1), Case(150, 700, 200, SMOOTH, 0.2, seed=2), Case(6, 700, 80, KD7, 0.1, seed=3)]
+    want = []
+    for c in cases:
+        loss, lse = c.forward()
+        want.append((loss, lse, *c.backward(lse)))
+    torch.cuda.synchronize()
+    steps, stream = 60, torch.cuda.Stream()
+    got = [[[torch.full_like(x, np.nan) for x in w] for _ in range(steps)] for w in want]
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(len(cases)), []
+
+    def work(c, outs):
+        try:
+            with torch.cuda.stream(stream):
+                start.wait(60)
+                for loss, lse, dh, dw in outs:
+                    c.forward(loss, lse)
+                    c.backward(lse, dh, dw)
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, got)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for w, outs in zip(want, got):
+        for i, out in enumerate(outs):
+            for k, (a, b) in enumerate(zip(out, w)):
+                assert torch.equal(a, b), (i, k)
+
+
 @pytest.mark.parametrize("N", [4, 30, 150, 700])
 @pytest.mark.parametrize("kind", [SMOOTH, KD7], ids=["ce", "kd"])
 def test_a_weight_from_the_call_before(kind, N):
