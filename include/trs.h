@@ -642,14 +642,19 @@ trs_status trs_linear_cross_entropy(const trs_view* hidden, const trs_view* weig
  * Numerics of this and the three calls around it: f32 products on the tensor cores,
  * every operand in two 11-bit parts, three products each, sums in f32: within a few
  * f32 roundings of the sums' terms.  Beyond 32 rows (8 with gradients; 16 where the
- * weight's rows are whole 16-byte pieces and D at most 2560) and widths above 4096
- * the parts are fp16 under a power of two per hidden row, per 256 rows of weight and
- * per 256 rows of grad_loss hidden: elements below 2^-17 of the largest there are off
- * by 2^-40 of it.  Infinities and NaNs make what depends on them infinite or NaN
- * (other tokens' losses and rows of grad_hidden do not), without the formulas' exact
- * special values.  Workspaces come from the stream-ordered pool: with gradients up to
- * about 512 MiB for a piece of the vocabulary and 8 bytes per element of hidden, more
- * where 256 rows of the vocabulary take more. */
+ * weight's rows are whole 16-byte pieces and D at most 2560), widths above 4096 and
+ * gradients of a weight whose columns lie apart, the parts are fp16 under a power of
+ * two per hidden row, per 256 rows of weight and per 256 rows of grad_loss hidden:
+ * elements below 2^-17 of the largest there are off by up to 2^-40 of it.  There
+ * softmax(x) - t is split under one power of two as well, as if its largest were 1
+ * everywhere: a row of grad_weight whose token no row finds likelier than 2^-17 is off by
+ * up to 2^-40 of the sum of the magnitudes of grad_loss hidden, which is more than its f32
+ * roundings, and it is 0 where no row finds the token likelier than 2^-40.  Infinities
+ * and NaNs make what depends on them infinite or NaN (other tokens' losses and rows of
+ * grad_hidden do not), without the formulas' exact special values.  Workspaces come from
+ * the stream-ordered pool: with gradients up to about 512 MiB for a piece of the
+ * vocabulary and 8 bytes per element of hidden, more where 256 rows of the vocabulary
+ * take more. */
 trs_status trs_linear_cross_entropy_backward(const trs_view* grad_loss, const trs_view* hidden,
                                              const trs_view* weight, const trs_view* targets,
                                              const trs_view* lse, double smoothing,

@@ -6,8 +6,12 @@
 // of 256 rows of the weight, of 256 rows of g h.  A product is hi hi + (hi lo + lo
 // hi), three tcgen05.mma with f32 accumulation.  The gradient of the scores
 // without the row's own factor, softmax(x) - t, lies in [-1, 1] and is split under
-// the fixed 2^15; the factor g temperature goes into g h for dw and onto the
-// rows of dh, so that rows with very different gradients keep their digits.
+// the fixed 2^15, off by 2^-40 at most: a tile's largest is known only when the tile
+// is, and is near 1 wherever a target lies in it.  dh, whose terms sum up to softmax
+// - t near 1, does not notice; rows of dw whose tokens are all improbable do (p of
+// 2^-21: 2e-5 of the row, 2^-29: 1e-3, 2^-40: nothing left).  The factor g temperature
+// goes into g h for dw and onto the rows of dh, so that rows with very different
+// gradients keep their digits.
 // The tensor core cuts its sums instead of rounding them, so a sum leaves the
 // accumulator for f32 registers every 256 elements.
 //

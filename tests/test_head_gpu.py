@@ -301,6 +301,43 @@ def test_infinities_stay_in_their_rows(N):
         check_all(c, t, loss, lse, *c.backward(lse))
 
 
+@pytest.mark.parametrize("N", [4, 12, 130])
+@pytest.mark.parametrize("kind", [CE, KD1], ids=["ce", "kd"])
+def test_gradients_of_improbable_tokens(kind, N):
+    """Rows of grad_weight whose tokens no row finds likely.  softmax(x) - t in two fp16 parts under 2^15 is off by half of
+    the smallest fp16 number, 2^-25 / 2^15 = 2^-40, where it is below 2^-17; few rows' kernels keep 22 bits of it."""
+    V, D = 300, 32
+    c = Case(N, V, D, kind)
+    # logarithms of the tokens' probabilities from 0 to -31: 2^-45
+    c.h[:, 0], c.w[:, 0] = 8.0, -np.linspace(0, 31 / 8, V)
+    c.d["h"], c.d["w"] = cuda(c.h), cuda(c.w)
+    t = c.truth()
+    loss, lse = c.forward()
+    dh, dw = c.backward(lse)
+    check_all(c, t, loss, lse, dh, dw)
+    # dw's bound of tests/_head.py, with 2^-40 (or nothing) in place of its 2^-38 of softmax(x) - t
+    h, w, g = c.h.astype(np.float64), c.w.astype(np.float64), np.abs(c.g.astype(np.float64))[:, None]
+    g[[e is None for e in c.entries]] = 0  # masked
+    x = h @ w.T
+    P = np.exp(x - t.lse[:, None])
+    target = np.zeros((N, V))
+    for i, e in enumerate(c.entries):
+        for v, p in e or []:
+            target[i, v] += p
+    sx = (160 + D / 64) * ref.U * (np.abs(h) @ np.abs(w).T) + 2.0**-38 * D * np.abs(h).max(-1, keepdims=True) * np.abs(w).max()
+    sx += 4 * ref.U * np.abs(x)
+    E = 2 * sx.max(-1) + (8 * np.abs(x).max(-1) + 8 * np.abs(t.lse) + 300 + V / 32) * ref.U
+    err = g * (P * E[:, None] + 60 * ref.U * target + 8 * ref.U * np.abs(P - target))
+    if N > 16:
+        err = err + g * 2.0**-40
+    dx = g * np.abs(P - target)
+    tol = err.T @ np.abs(h) + (160 + N / 64) * ref.U * (dx.T @ np.abs(h))
+    tol += 2.0**-38 * (g * np.abs(h)).max() * (P + target).sum(0)[:, None]
+    ref.check(to_host(dw), t.dw, tol, ("dw", N))
+    if N <= 16:  # the least likely ones have a gradient
+        assert np.abs(to_host(dw))[-1].max() > 0
+
+
 @pytest.mark.parametrize("N", [4, 17, 130])
 @pytest.mark.parametrize("kind", [CE, KD7], ids=["ce", "kd"])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
