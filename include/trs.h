@@ -602,7 +602,9 @@ trs_status trs_cross_attention_backward(
 /* out[t] = scale * table[ids[t]].  table is [V, D], f32 or f64, ids i32 or i64,
  * [tokens] or [batch, tokens], out the same with D behind it, in the table's
  * type.  An id outside [0, V) (padding, or a row of another shard of the table)
- * gives a row of zeros.  out may overlap neither table nor ids (TRS_ERR_ALIAS).
+ * gives a row of zeros.  For an f32 table scale is rounded to f32 if it lies among the
+ * normal f32 numbers, and is applied in f64 beyond them.  out may overlap neither table
+ * nor ids (TRS_ERR_ALIAS).
  * Fewer than 2^31 - 8192 tokens, rows and elements of a row (TRS_ERR_SHAPE). */
 trs_status trs_embedding(const trs_view* table, const trs_view* ids, double scale,
                          trs_view* out, trs_stream stream);

@@ -36,6 +36,8 @@
 // Bulk copies of zeros from shared memory (94 us in all), 32-byte stores (80) and
 // zeros next to the sums for the rows that no token looked up (101) were slower.
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 #include <cstring>
 
 #include "../../include/trs.h"
@@ -70,6 +72,7 @@ struct EmbDev {
   Lanes l;
   FastDiv f_T;
   double scale;
+  int wide;              // lookup: the scale is no normal number of the table's type
   int accumulate;
   // backward
   uint32_t *key[2], *tok[2];
@@ -109,7 +112,11 @@ template <class T, int V>
 __global__ void __launch_bounds__(kEmbThreads) emb_lookup_kernel(const EmbDev d) {
   constexpr int U = 4;  // rows of a group in flight
   const int L = 1 << d.l.lg, per = kEmbThreads >> d.l.lg, c0 = threadIdx.x & (L - 1);
+  // A scale that f32 holds as a normal number is rounded to it, as the table's own values are;
+  // any other would lose its digits or all of itself, and is applied in f64 (16384 tokens of
+  // 2048 from random rows: 45.0 and 45.3 us).
   const T scale = (T)d.scale;
+  const bool wide = d.wide;
   for (uint64_t base = (uint64_t)blockIdx.x * per * U + (threadIdx.x >> d.l.lg); base < d.N;
        base += (uint64_t)gridDim.x * per * U) {
     uint32_t id[U];
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(kEmbThreads) emb_lookup_kernel(const EmbDev d)
         const uint64_t r = base + (uint64_t)j * per;
         if (r >= d.N) continue;
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[j].v[i] = id[j] < d.V ? x[j].v[i] * scale : (T)0;
+        for (int i = 0; i < V; ++i) x[j].v[i] = id[j] >= d.V ? (T)0 : wide ? (T)((double)x[j].v[i] * d.scale) : x[j].v[i] * scale;
         store<T, V>(row_at<T>(d, (uint32_t)r), c, d.rows.sd, x[j]);
       }
     }
@@ -599,6 +606,8 @@ Error run_embedding(const EmbCall& c, bool backward, cudaStream_t stream) {
   d.D = (int)D;
   d.f_T = make_fastdiv((uint32_t)std::max<int64_t>(t.T, 1));
   d.scale = c.scale;
+  const double size = std::fabs(c.scale);
+  d.wide = dt == TRS_F32 && ((size > 0.0 && size < FLT_MIN) || (size > FLT_MAX && size <= DBL_MAX));
   d.accumulate = c.accumulate != 0;
   const bool vec = (V == 0 || rows_vectors(c.table)) && (d.N == 0 || rows_vectors(c.rows));
   if (backward) {

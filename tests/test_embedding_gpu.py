@@ -90,6 +90,18 @@ def test_lookup(size):
         check(got, want, (2 * U[dt] + U[dt] ** 2) * np.abs(want) if scale != 1.0 else 0 * want, size)
 
 
+@pytest.mark.parametrize("D", [24, 7])
+@pytest.mark.parametrize("scale,size", [(1e-50, 1e30), (1e45, 1e-30), (-1e-40, 1e20), (2.0**-149, 1e25), (2.0**128, 1e-10)])
+def test_lookup_scales_beyond_f32(scale, size, D):
+    """A scale that f32 does not hold in full, with products that it does: one rounding of f64's product."""
+    g = np.random.default_rng(D)
+    table, ids = (g.standard_normal((40, D)) * size).astype("f4"), tokens(g, 70, 40, "text")
+    out = torch.full((70, D), np.nan, device="cuda")
+    got = lookup(torch.from_numpy(table).cuda(), torch.from_numpy(ids).cuda(), scale, out)
+    want = truth_lookup(table, ids, scale)
+    check(got, want, (U["f4"] + 2.0**-52) * np.abs(want), (scale, size))
+
+
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("size", SIZES, ids=NAMES)
 def test_gradient(size, accumulate):
