@@ -604,8 +604,8 @@ trs_status trs_cross_attention_backward(
  * type.  An id outside [0, V) (padding, or a row of another shard of the table)
  * gives a row of zeros.  For an f32 table scale is rounded to f32 if it lies among the
  * normal f32 numbers, and is applied in f64 beyond them.  out may overlap neither table
- * nor ids (TRS_ERR_ALIAS).
- * Fewer than 2^31 - 8192 tokens, rows and elements of a row (TRS_ERR_SHAPE). */
+ * nor ids (TRS_ERR_ALIAS).  Fewer than 2^31 - 8192 tokens, rows and elements of a row
+ * (TRS_ERR_SHAPE). */
 trs_status trs_embedding(const trs_view* table, const trs_view* ids, double scale,
                          trs_view* out, trs_stream stream);
 
@@ -615,7 +615,9 @@ trs_status trs_embedding(const trs_view* table, const trs_view* ids, double scal
  * token looked up are left alone), as for a table that is also the weight of
  * the last layer.  Sums are taken in f64 and rounded once, in an order that the
  * ids alone decide: no atomics add values, repeated calls give the same bits.
- * grad_table may overlap neither grad_out nor ids. */
+ * grad_table may overlap neither grad_out nor ids.  Workspace, from the
+ * stream-ordered pool: some 18 bytes per token and half a byte to 2 bytes per
+ * element of grad_out, more where its rows are below 128 bytes (16 at 16 bytes). */
 trs_status trs_embedding_backward(const trs_view* grad_out, const trs_view* ids, double scale,
                                   int32_t accumulate, trs_view* grad_table, trs_stream stream);
 
@@ -653,10 +655,14 @@ trs_status trs_linear_cross_entropy(const trs_view* hidden, const trs_view* weig
  * up to 2^-40 of the sum of the magnitudes of grad_loss hidden, which is more than its f32
  * roundings, and it is 0 where no row finds the token likelier than 2^-40.  Infinities
  * and NaNs make what depends on them infinite or NaN (other tokens' losses and rows of
- * grad_hidden do not), without the formulas' exact special values.  Workspaces come from
- * the stream-ordered pool: with gradients up to about 512 MiB for a piece of the
- * vocabulary and 8 bytes per element of hidden, more where 256 rows of the vocabulary
- * take more. */
+ * grad_hidden do not), without the formulas' exact special values.
+ *
+ * Workspaces of these calls come from the stream-ordered pool.  Beyond the numbers of rows
+ * above: about 512 MiB for a piece of the vocabulary (more where 256 rows of it take
+ * more); 4 bytes per element of hidden, 8 with gradients; forward, 16 bytes per token and
+ * 128 rows of the vocabulary (2 GiB for 131072 tokens on 131072 rows); with gradients up
+ * to 80 MiB for sums in parts.  Up to those numbers: with gradients 64 bytes per row of the
+ * vocabulary and 10 MiB.  A teacher's entries take 8 bytes each. */
 trs_status trs_linear_cross_entropy_backward(const trs_view* grad_loss, const trs_view* hidden,
                                              const trs_view* weight, const trs_view* targets,
                                              const trs_view* lse, double smoothing,
