@@ -17,7 +17,7 @@
 //   emb_keys_kernel     the ids as 32-bit keys (V for those outside), and the
 //                       counts of their lowest digit per tile of 4096 tokens
 //   emb_sort_kernel     one digit (up to 9 bits) of a stable radix sort of
-//                       (key, token): two launches up to V = 2^18.  Every CTA
+//                       (key, token): two launches below V = 2^18.  Every CTA
 //                       finds its places from all tiles' counts (no CTA waits on
 //                       another), and counts the next digit as it writes.
 //   emb_sort_one_kernel the keys and all digits in one launch, for up to 4096 tokens
@@ -526,6 +526,9 @@ Error launch_backward(EmbDev& d, cudaStream_t s) {
   d.tiles = (uint32_t)(((uint64_t)d.N + kSortTile - 1) / kSortTile);
   const int sms = current_device_info().sm_count;
   // as many positions per group as still leave two CTAs of groups per SM, and as fit a CTA's threads
+  // (rows below 128 bytes get fewer than 8, so that a frequent token's run comes in many parts, which one
+  // CTA finds and adds per 64 columns: 65536 tokens into 50000 rows, a few making up most of them, 64 us
+  // for rows of 16 and 127 of 4; all of them one token 420 and 1360)
   d.positions = 32;
   while (d.positions > 8 && (uint64_t)d.N / d.positions < ((uint64_t)2 * sms << 8 >> d.l.lg)) d.positions /= 2;
   while ((d.positions << 8 >> d.l.lg) > kEmbThreads) d.positions /= 2;

@@ -29,8 +29,10 @@ namespace {
 
 constexpr int kMaxEntries = 1024;
 
-// A warp per row: the softmax of the entries that are there, sorted by token
-// (the rank of an entry is counted: K is small).
+// A warp per row: the softmax of the entries that are there, sorted by token.  The
+// rank of an entry is counted, K^2 / 32 steps of the warp, which suits the tens of
+// entries that are kept in earnest: 8192 rows of 64 entries 27 us, of 128 86, but of
+// 1024 4.8 ms (and 7 rows of those 0.86 ms).
 __global__ void __launch_bounds__(256) head_teacher_kernel(const HeadDev d) {
   extern __shared__ int s_id[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -306,8 +308,7 @@ Error run_head(const HeadCall& c, cudaStream_t stream) {
   d.vec_h = N > 0 && rows_vectors(c.hidden);
   d.vec_dh = N > 0 && c.grad_hidden && rows_vectors(c.grad_hidden);
   if (N == 0 && !d.dw) return Error{};
-  // Up to 16 rows the CUDA cores keep up with HBM, or nearly; without rows the
-  // tensor-core path writes the zeros.
+  // Without rows head_tc.cu writes the zeros.
   const bool few = head_few_takes(d, c.backward);
   // the rows' targets
   Scratch mem;

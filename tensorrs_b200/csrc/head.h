@@ -1,6 +1,6 @@
 // head.h -- what the translation units of a model's last layer share (head.cu:
-// checks, the rows' targets, the CUDA-core kernels; head_tc.cu: the tensor-core
-// kernels).
+// checks, the rows' targets, the join of the vocabulary's parts; head_few.cu: few
+// rows; head_tc.cu: more).
 //
 // Both losses are  lse(x) - sum_v t_v x_v  of the scores x = h w^T / temperature
 // against a target distribution t, up to a constant of the row and the factor
@@ -131,12 +131,12 @@ __device__ __forceinline__ HeadPart head_add(const HeadPart& a, const HeadPart& 
 Error head_join(const HeadDev& d, const HeadPart* part, int parts, int64_t sp, int64_t sr, bool few,
                 cudaStream_t stream);
 
-// Few rows (head_few.cu).  8 or 16 of them share a read of the weight, which the
-// tensor-core path reads, splits, writes and reads again: on 32000 x 1024, 17 rows 78
-// us here and 113 there, 33 there alone; gradients of 8 rows 87 and 216, of 16
-// FEW16 and 217, of two blocks of rows 257 and 217.  Widths up to 4096 (4 x 4096:
-// 58 us and 243); gradients of weights whose columns lie apart are walked badly here
-// (8 rows 490 us, 300 there).
+// Few rows (head_few.cu).  8 or 16 of them share a read of the weight, which head_tc.cu
+// reads, splits, writes and reads again, for 1 to 256 rows alike: on 32000 x 1024,
+// scores of 17 rows 82 us here, of 33 98 there; gradients of 8 rows 88 here, of 16 118,
+// of two blocks of rows 257, and 201 there.  Widths up to 4096 (scores of 4 rows
+// on 32000: of 4096 103 us here, of 4104 388 there), as shared memory holds; gradients of
+// weights whose columns lie apart are walked badly here (8 rows 490 us, 298 there).
 inline bool head_few_takes(const HeadDev& d, bool backward) {
   if (d.N < 1 || d.D > 4096) return false;
   if (!backward) return d.N <= 32;
@@ -144,7 +144,7 @@ inline bool head_few_takes(const HeadDev& d, bool backward) {
   return d.N <= 8 || (d.N <= 16 && d.vec_w && d.D <= 2560);
 }
 Error head_few(const HeadDev& d, bool backward, cudaStream_t stream);
-// More rows, or none (head_tc.cu).  How the work is cut, and where its workspaces lie
+// More rows, wider ones, or none (head_tc.cu).  How the work is cut, and where its workspaces lie
 // in `bytes` of memory, which the call takes before its first launch: its first planes
 // are written without waiting for the kernel before them, so the memory must not come
 // from anything that was issued, on the same stream by another host thread, after that

@@ -1,5 +1,5 @@
 // head_tc.cu -- a model's last layer with its loss on the 5th-generation tensor
-// cores, for more rows than the CUDA cores serve at HBM's rate.
+// cores, for more or wider rows than head_few.cu takes.
 //
 // Products.  f32 operands are written 2^e (hi + lo) with hi and lo in fp16, 11
 // bits each, e placing the largest magnitude in [2^14, 2^15): of a hidden row,
