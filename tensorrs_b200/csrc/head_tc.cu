@@ -590,11 +590,16 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
 #pragma unroll
     for (int i = 0; i < 128; i += 2) mx4[i / 2 % 4] = fmaxf(fmaxf(mx4[i / 2 % 4], acc[i]), acc[i + 1]);
     HeadPart p;
-    p.m = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * t.f;
+    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+    p.m = mx * t.f;
     const float base = p.m == -INFINITY ? 0.f : -p.m;
+    // Exponents are products less the rounded largest one.  What that was rounded by stays
+    // in the sum while it is small, and is taken out where the exponential would not bear
+    // it (scores near 2^43: up to 2^19).
+    const float off = fabsf(p.m) >= 0x1p20f && fabsf(p.m) < INFINITY ? __fmaf_rn(mx, t.f, base) : 0.f;
     float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 128; ++i) s4[i % 4] += head_ex2(__fmaf_rn(acc[i], t.f, base));
+    for (int i = 0; i < 128; ++i) s4[i % 4] += head_ex2(__fmaf_rn(acc[i], t.f, base) - off);
     p.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
     p.dot = tile_entries<false>(d, buf, lane, t.orig, t.e, t.id, g.v0 + col, g.v0 + col + min(limit, 128), acc) * t.f;
     p.sum = 0.f;

@@ -279,6 +279,24 @@ def test_range(N):
         check_all(c, t, loss, lse, *c.backward(lse))
 
 
+LARGE = [(("kd", 7, 2.0**-40), 1), (("kd", 7, 2.0**-20), 1), (("kd", 3, 2.0**-10), 1e-5), (CE, 1e6), (CE, 1e9), (SMOOTH, 1e12),
+         (("ce", 1.0), 1e30)]
+
+
+@pytest.mark.parametrize("N", [4, 20, 130])
+@pytest.mark.parametrize("kind,size", LARGE)
+def test_scores_of_any_size(kind, size, N):
+    """Scores whose last bit is worth more than the exponential's whole range."""
+    for seed in range(3):
+        c = Case(N, 700, 48, kind, 0.2, seed=seed)
+        c.h *= np.float32(size)
+        c.d["h"] = cuda(c.h)
+        t = c.truth()
+        loss, lse = c.forward()
+        ref.check(to_host(loss), t.loss, t.loss_tol, ("loss", size))
+        ref.check(to_host(lse), t.lse, t.lse_tol, ("lse", size))
+
+
 @pytest.mark.parametrize("N", [4, 130])
 def test_infinities_stay_in_their_rows(N):
     for bad in (np.inf, np.nan):
