@@ -53,6 +53,14 @@ __device__ __forceinline__ float head_ex2(float x) {
   return y;
 }
 
+// softmax(x) from the row's lse, the exponent `z` in units of log2: at most 1.  lse is
+// rounded to f32, which at scores of 1e7 and more is worth more than the exponential's
+// range; a NaN stays one.
+__device__ __forceinline__ float head_softmax(float z) {
+  asm("min.NaN.f32 %0, %0, 0f00000000;" : "+f"(z));
+  return head_ex2(z);
+}
+
 template <class T>
 __device__ __forceinline__ T* head_row(const HeadDev& d, const RowsDev& r, int i) {
   const uint32_t b = fdiv((uint32_t)i, d.f_T), t = (uint32_t)i - b * d.f_T.d;

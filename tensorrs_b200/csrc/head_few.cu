@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
         }
       }
       if (GRAD) {
-        dx[(int64_t)v * NR + fn] = row < 0 ? 0.f : gr * (head_ex2(z - lse2) - t - d.share);
+        dx[(int64_t)v * NR + fn] = row < 0 ? 0.f : gr * (head_softmax(z - lse2) - t - d.share);
       } else {
         // a score of -inf adds nothing, and must not meet the maximum of -inf that a thread
         // begins with; a NaN, which the maximum passes over, makes the sum NaN for good

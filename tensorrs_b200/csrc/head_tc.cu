@@ -615,7 +615,7 @@ __device__ __forceinline__ void finish_tile(const GemmDev& g, const GemmItem& w,
   } else if (MODE == kScoreGrad) {
     const int limit = row < live ? g.Vc - col : 0;
 #pragma unroll
-    for (int i = 0; i < 128; ++i) acc[i] = head_ex2(__fmaf_rn(acc[i], t.f, -t.lse2)) - d.share;
+    for (int i = 0; i < 128; ++i) acc[i] = head_softmax(__fmaf_rn(acc[i], t.f, -t.lse2)) - d.share;
     tile_entries<true>(d, buf, lane, t.orig, t.e, t.id, g.v0 + col, g.v0 + col + min(g.Vc - col, 128), acc);
     __half* to = g.dx + (int64_t)(row - lane) * g.ld + col;  // the warp's first row
 #pragma unroll

@@ -297,6 +297,25 @@ def test_scores_of_any_size(kind, size, N):
         ref.check(to_host(lse), t.lse, t.lse_tol, ("lse", size))
 
 
+@pytest.mark.parametrize("N", [4, 12, 20, 130])
+@pytest.mark.parametrize("kind,size", LARGE)
+def test_gradients_of_scores_of_any_size(kind, size, N):
+    """A softmax taken from an lse that is rounded to f32 lies between 0 and 1, also where the rounding leaves nothing
+    of it to compare."""
+    for seed in range(3):
+        c = Case(N, 700, 48, kind, 0.2, seed=seed)
+        c.h *= np.float32(size)
+        c.d["h"] = cuda(c.h)
+        _, lse = c.forward()
+        dh, dw = (to_host(x).astype(np.float64) for x in c.backward(lse))
+        live = np.array([e is not None for e in c.entries], bool)
+        g = np.where(live, np.abs(c.g.astype(np.float64)), 0)[:, None] * (1.0 if c.T is None else c.T)
+        h, w = np.where(live[:, None], np.abs(c.h.astype(np.float64)), 0), np.abs(c.w.astype(np.float64))
+        # every element of softmax - t lies in [-1, 1]; 2^-10 for all roundings
+        assert (np.abs(dh) <= g * w.sum(0) * (1 + 2.0**-10) + 1e-37).all()
+        assert (np.abs(dw) <= (g * h).sum(0) * (1 + 2.0**-10) + 1e-37).all()
+
+
 @pytest.mark.parametrize("N", [4, 130])
 def test_infinities_stay_in_their_rows(N):
     for bad in (np.inf, np.nan):
