@@ -649,15 +649,18 @@ trs_status trs_linear_cross_entropy(const trs_view* hidden, const trs_view* weig
  * weight's rows are whole 16-byte pieces and D at most 2560), widths above 4096 and
  * gradients of a weight whose columns lie apart, the parts are fp16 under a power of
  * two per hidden row, per 256 rows of weight and per 256 rows of grad_loss hidden:
- * elements below 2^-17 of the largest there are off by up to 2^-40 of it.  There
- * softmax(x) - t is split under one power of two as well, as if its largest were 1
- * everywhere: a row of grad_weight whose token no row finds likelier than 2^-17 is off
- * by up to 2^-40 of the sum of the magnitudes of grad_loss hidden, which is more than
- * its f32 roundings, and it is 0 where no row finds the token likelier than 2^-40.  The
- * softmax of a gradient is the exponential of x less an lse that is rounded to f32: off
- * by about 2^-22 (|x| + |lse|) of itself, and between 0 and 1 where that leaves nothing
- * of it.  Infinities and NaNs make what depends on them infinite or NaN (other tokens'
- * losses and rows of grad_hidden do not), without the formulas' exact special values.
+ * elements below 2^-17 of the largest there are off by up to 2^-40 of it. (Up to those
+ * numbers the parts are TF32, and only elements below 2^-114 lose their second one.)
+ * There softmax(x) - t is split under one power of two as well, as if its largest were
+ * 1 everywhere: a row of grad_weight whose token no row finds likelier than 2^-17 is
+ * off by up to 2^-40 of the sum of the magnitudes of grad_loss hidden, which is more
+ * than its f32 roundings, and it is 0 where no row finds the token likelier than 2^-40.
+ * The softmax of a gradient is the exponential of x less an lse that is rounded to f32:
+ * off by about 2^-22 (|x| + |lse|) of itself, and between 0 and 1 where that leaves
+ * nothing of it. grad_loss times the temperature has to be an f32 number, as the scores
+ * have to.  Infinities and NaNs make what depends on them infinite or NaN (other
+ * tokens' losses and rows of grad_hidden do not), without the formulas' exact special
+ * values.
  *
  * Workspaces of these calls come from the stream-ordered pool.  Beyond the numbers of rows
  * above: about 512 MiB for a piece of the vocabulary (more where 256 rows of it take
