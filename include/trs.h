@@ -651,9 +651,9 @@ trs_status trs_linear_cross_entropy(const trs_view* hidden, const trs_view* weig
  * two per hidden row, per 256 rows of weight and per 256 rows of grad_loss hidden:
  * elements below 2^-17 of the largest there are off by up to 2^-40 of it. (Up to those
  * numbers the parts are TF32, and only elements below 2^-114 lose their second one.)
- * There softmax(x) - t is split under one power of two as well, as if its largest were
- * 1 everywhere: a row of grad_weight whose token no row finds likelier than 2^-17 is
- * off by up to 2^-40 of the sum of the magnitudes of grad_loss hidden, which is more
+ * Beyond them softmax(x) - t is split under one power of two as well, as if its largest
+ * were 1 everywhere: a row of grad_weight whose token no row finds likelier than 2^-17
+ * is off by up to 2^-40 of the sum of the magnitudes of grad_loss hidden, which is more
  * than its f32 roundings, and it is 0 where no row finds the token likelier than 2^-40.
  * The softmax of a gradient is the exponential of x less an lse that is rounded to f32:
  * off by about 2^-22 (|x| + |lse|) of itself, and between 0 and 1 where that leaves
