@@ -24,6 +24,7 @@
 // for 4 rows and 44 for 8; a ring of bulk copies per CTA 36 and 40, per warp 39 and
 // 45; the gradient of the columns on the CUDA cores 63.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <string>
@@ -221,7 +222,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
       gr = *head_row<const float>(d, d.gl, row) * d.temp;
     }
   }
-  HeadPart pt = {-INFINITY, 0.f, 0.f, 0.f};
+  // from the lowest finite maximum: a first score of -inf adds 0, not the NaN of inf - inf
+  HeadPart pt = {-FLT_MAX, 0.f, 0.f, 0.f};
   float* dx = a.dx;
   float part[NT][4];
 #pragma unroll
@@ -261,13 +263,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) head_rows_kernel(const __grid_
       if (GRAD) {
         dx[(int64_t)v * NR + fn] = row < 0 ? 0.f : gr * (head_softmax(z - lse2) - t - d.share);
       } else {
-        // a score of -inf adds nothing, and must not meet the maximum of -inf that a thread
-        // begins with; a NaN, which the maximum passes over, makes the sum NaN for good
-        if (z != -INFINITY) {
-          const float m = fmaxf(pt.m, z);
-          pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(z - m);
-          pt.m = m;
-        }
+        const float m = fmaxf(pt.m, z);  // passes over a NaN, which makes the sum NaN for good
+        pt.s = pt.s * head_ex2(pt.m - m) + head_ex2(z - m);
+        pt.m = m;
         if (t != 0.f) pt.dot = __fmaf_rn(t, z, pt.dot);
         pt.sum += z;
       }
